@@ -9,12 +9,12 @@ Kinds of case:
   the cache then holds for them (`kv4_read`);
 * `attend`: causal attention of the last queries of each sequence over that cache (`kv4_attention`).
 
-The cache is a uint8 tensor `[pages, kv heads, page / 16, 16 (head dim + 8)]`. A block of sixteen tokens of one head holds, in this
-order: the codes of K, head dim / 2 bytes a token, dimension 2 i in the low and 2 i + 1 in the high half of byte i; the codes of V, two
-tokens after one another in pairs of 16-bit words (word i: four dimensions from 4 i on, the lowest in the lowest bits), the words of the
-even and the odd token in turn; then for K and after that for V a pair of bfloat16 a token, step and least value. A value is
-`least + step * code`; a head's vector of one token is a group of its own, `step = (max - min) / 15`, both rounded to bfloat16 before the
-codes are taken (a step below 2^-126 counts as zero; a group whose range is not finite is held as NaN).
+The cache is a uint8 tensor `[pages, kv heads, page / 16, 16 (head dim + 8)]`. A block of sixteen tokens of one head holds first the codes
+of K, head dim / 2 bytes a token, dimension 2 i in the low and 2 i + 1 in the high half of byte i; then for each two tokens a row of head
+dim + 16 bytes: the codes of V in 16-bit words (word i: four dimensions from 4 i on, the lowest in the lowest bits), the words of the
+even and the odd token in turn, and behind them for either token four bfloat16: step and least value of K, step and least value of V. A
+value is `least + step * code`; a head's vector of one token is a group of its own, `step = (max - min) / 15`, both rounded to bfloat16
+before the codes are taken (a step below 2^-126 counts as zero; a group whose range is not finite is held as NaN).
 """
 
 from __future__ import annotations
@@ -158,10 +158,12 @@ def _pages(case: dict, g: torch.Generator) -> tuple[int, torch.Tensor]:
 
 
 def _views(cache: torch.Tensor, dim: int) -> tuple[torch.Tensor, ...]:
-    """The parts of the cache as views of it: codes of K [.., 16, dim / 2], codes of V [.., 8 pairs, dim / 4, 2 tokens, 2 bytes], the
-    pairs of K and of V [.., 16, 4 bytes]."""
-    k, v, pk, pv = cache.split((8 * dim, 8 * dim, 64, 64), -1)
-    return k.unflatten(-1, (BLOCK, dim // 2)), v.unflatten(-1, (8, dim // 4, 2, 2)), pk.unflatten(-1, (BLOCK, 4)), pv.unflatten(-1, (BLOCK, 4))
+    """The parts of the cache as views of it: codes of K [.., 16, dim / 2], codes of V [.., 8, dim / 4, 2 tokens, 2 bytes], the pairs
+    (step, least value) of K and of V [.., 8, 2 tokens, 4 bytes]."""
+    k, rows = cache.split((8 * dim, 8 * dim + 128), -1)
+    v, pairs = rows.unflatten(-1, (8, dim + 16)).split((dim, 16), -1)
+    pairs = pairs.unflatten(-1, (2, 2, 4))
+    return k.unflatten(-1, (BLOCK, dim // 2)), v.unflatten(-1, (dim // 4, 2, 2)), pairs[..., 0, :], pairs[..., 1, :]
 
 
 def _quantised(x: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
@@ -189,12 +191,12 @@ def _filled(pages: int, case: dict, g: torch.Generator) -> torch.Tensor:
         n = ck.shape[0]
         codes, pair = _quantised(torch.randn(n, h, nb, BLOCK, d, generator=g, device="cuda") * large)
         ck.copy_(codes[..., 0::2] | codes[..., 1::2] << 4)
-        pk.copy_(pair.view(torch.uint8))
+        pk.copy_(pair.view(torch.uint8).unflatten(-2, (8, 2)))
         size = torch.exp(0.5 * torch.randn(n, h, nb, BLOCK, 1, generator=g, device="cuda"))
         codes, pair = _quantised(torch.randn(n, h, nb, BLOCK, d, generator=g, device="cuda") * size)
         byte = codes[..., 0::2] | codes[..., 1::2] << 4
         cv.copy_(byte.unflatten(-1, (d // 4, 2)).unflatten(-3, (8, 2)).transpose(-3, -2))
-        pv.copy_(pair.view(torch.uint8))
+        pv.copy_(pair.view(torch.uint8).unflatten(-2, (8, 2)))
     return cache
 
 
@@ -321,15 +323,15 @@ def _plain_append(s: dict) -> dict:
     ck, cv, pk, pv = _views(s["cache"], d)
     codes, pair = _quantised(kr)
     ck[page, :, block, token] = codes[..., 0::2] | codes[..., 1::2] << 4
-    pk[page, :, block, token] = pair.view(torch.uint8)
+    pk[page, :, block, token // 2, token % 2] = pair.view(torch.uint8)
     codes, pair = _quantised(v.float())
     cv[page, :, block, token // 2, :, token % 2] = (codes[..., 0::2] | codes[..., 1::2] << 4).unflatten(-1, (d // 4, 2))
-    pv[page, :, block, token] = pair.view(torch.uint8)
+    pv[page, :, block, token // 2, token % 2] = pair.view(torch.uint8)
     got = {"q": qr.to(q.dtype)}
     none = (at < 0)[:, :, None, None]
-    held = _values(_nibbles(ck[page, :, block, token]), pk[page, :, block, token])
+    held = _values(_nibbles(ck[page, :, block, token]), pk[page, :, block, token // 2, token % 2])
     got["k"] = torch.where(none, 0.0, held).to(q.dtype)
-    held = _values(_nibbles(cv[page, :, block, token // 2, :, token % 2].flatten(-2)), pv[page, :, block, token])
+    held = _values(_nibbles(cv[page, :, block, token // 2, :, token % 2].flatten(-2)), pv[page, :, block, token // 2, token % 2])
     got["v"] = torch.where(none, 0.0, held).to(q.dtype)
     return got
 
@@ -337,8 +339,8 @@ def _plain_append(s: dict) -> dict:
 def _held(cache: torch.Tensor, d: int) -> tuple[torch.Tensor, torch.Tensor]:
     """K and V of blocks `[.., blocks, heads, bytes]` as `[.., heads, 16 blocks, dim]`."""
     ck, cv, pk, pv = _views(cache, d)
-    k = _values(_nibbles(ck), pk)
-    v = _values(_nibbles(cv.transpose(-3, -2).flatten(-2)).flatten(-3, -2), pv)
+    k = _values(_nibbles(ck), pk.flatten(-3, -2))
+    v = _values(_nibbles(cv.transpose(-3, -2).flatten(-2)).flatten(-3, -2), pv.flatten(-3, -2))
     return tuple(x.transpose(-4, -3).flatten(-3, -2) for x in (k, v))
 
 
@@ -413,9 +415,10 @@ def _decoded64(blocks: torch.Tensor, d: int) -> tuple[torch.Tensor, torch.Tensor
     """K and V `[heads, tokens, dim]` of blocks `[blocks, heads, bytes]`, each code fetched by the place of its byte."""
     t, x = torch.arange(BLOCK, device="cuda")[:, None], torch.arange(d, device="cuda")
     got = []
-    for byte, pairs in ((t * (d // 2) + x // 2, 16 * d), (8 * d + t // 2 * d + x // 4 * 4 + t % 2 * 2 + x % 4 // 2, 16 * d + 64)):
+    row = 8 * d + t // 2 * (d + 16)
+    for byte, pair in ((t * (d // 2) + x // 2, 0), (row + x // 4 * 4 + t % 2 * 2 + x % 4 // 2, 4)):
         code = (blocks[..., byte] >> (4 * (x % 2))) & 15
-        word = blocks[..., pairs : pairs + 64].reshape(*blocks.shape[:-1], BLOCK, 4).to(torch.int32)
+        word = blocks[..., row + d + t % 2 * 8 + pair + torch.arange(4, device="cuda")].to(torch.int32)
         step, least = ((word[..., i] << 16 | word[..., i + 1] << 24).view(torch.float32).double()[..., None] for i in (0, 2))
         got.append((code.double() * step + least).transpose(0, 1).flatten(1, 2))
     return got[0], got[1]
