@@ -19,7 +19,9 @@ from .graphs import GraphCache
 from .gemm import ACT_GELU, ACT_GELU_TANH, ACT_NONE, ACT_RELU, gemm
 from .flash64 import FLASH_VARIANTS, Flash64, check_flash64
 from .host_io import HostAttention
+from .kv4 import kv4_append_, kv4_attention, kv4_cache, kv4_read, reserve_kv4_workspace
 from .rope import rope_qk_, rope_table
+from .rotary import qk_norm_rotary, rotary, rotary_table
 from .sam import sam_rel_terms
 from .sdpa import scaled_dot_product_attention
 
@@ -41,10 +43,18 @@ __all__ = [
     "device_status",
     "gemm",
     "kernels_unavailable_reason",
+    "kv4_append_",
+    "kv4_attention",
+    "kv4_cache",
+    "kv4_read",
+    "qk_norm_rotary",
+    "reserve_kv4_workspace",
     "reserve_workspace",
     "resolve_mode",
     "rope_qk_",
     "rope_table",
+    "rotary",
+    "rotary_table",
     "sam_rel_terms",
     "tile_layout",
     "scaled_dot_product_attention",

@@ -30,7 +30,7 @@ if TYPE_CHECKING:
 
 LIBRARY = "b200attn"
 PACKAGE_DIR = Path(__file__).resolve().parent
-SOURCES = tuple(PACKAGE_DIR / "csrc" / name for name in ("b200_attn.cu", "b200_window.cu", "b200_linear.cu", "b200_encoder.cu"))
+SOURCES = tuple(PACKAGE_DIR / "csrc" / name for name in ("b200_attn.cu", "b200_window.cu", "b200_linear.cu", "b200_encoder.cu", "b200_decoder.cu"))
 HEADERS = (
     PACKAGE_DIR / "csrc" / "host_common.h",
     PACKAGE_DIR / "csrc" / "linear_host.h",
@@ -43,8 +43,12 @@ HEADERS = (
     PACKAGE_DIR / "csrc" / "rope_sm100.cuh",
     PACKAGE_DIR / "csrc" / "gemm_sm100.cuh",
     PACKAGE_DIR / "csrc" / "encoder_kernels.cuh",
+    PACKAGE_DIR / "csrc" / "rotary_sm100.cuh",
+    PACKAGE_DIR / "csrc" / "kv4_sm100.cuh",
+    PACKAGE_DIR / "csrc" / "kv4_attn_sm100.cuh",
     PACKAGE_DIR.parent / "include" / "b200_attn.h",
     PACKAGE_DIR.parent / "include" / "b200_encoder.h",
+    PACKAGE_DIR.parent / "include" / "b200_decoder.h",
 )
 SHARED_OBJECT = PACKAGE_DIR / "libb200attn.so"
 # The host side of repeated calls, a CPython extension over torch's C++ interface (no kernels in it).
@@ -65,6 +69,11 @@ EXPORTS = (
 
 # ... and include/b200_encoder.h.
 ENCODER_EXPORTS = ("b200_encoder_workspace", "b200_encoder_forward")
+
+# ... and include/b200_decoder.h.
+DECODER_EXPORTS = (
+    "b200_rotary", "b200_rotary_workspace", "b200_kv4_append", "b200_kv4_read", "b200_kv4_attention", "b200_kv4_workspace",
+)  # fmt: skip
 
 OK, UNSUPPORTED, BAD_CONFIG, CUDA_ERROR_BASE = 0, 1, -1, 1000
 F16, BF16, F32 = 0, 1, 2
@@ -252,6 +261,119 @@ class B200EncoderArgs(ctypes.Structure):
     )
 
 
+class B200Heads(ctypes.Structure):
+    """Mirror of `struct B200Heads` (include/b200_decoder.h)."""
+
+    _fields_ = (
+        ("x", ctypes.c_void_p),
+        ("y", ctypes.c_void_p),
+        ("g", ctypes.c_void_p),
+        ("w", ctypes.c_void_p),
+        ("dw", ctypes.c_void_p),
+        ("x_stride", ctypes.c_int64 * 3),
+        ("y_stride", ctypes.c_int64 * 3),
+        ("g_stride", ctypes.c_int64 * 3),
+        ("heads", ctypes.c_int32),
+        ("reserved", ctypes.c_int32),
+    )
+
+
+class B200RotaryArgs(ctypes.Structure):
+    """Mirror of `struct B200RotaryArgs` (include/b200_decoder.h)."""
+
+    _fields_ = (
+        ("struct_size", ctypes.c_uint32),
+        ("dtype", ctypes.c_uint32),
+        ("weight_dtype", ctypes.c_uint32),
+        ("batch", ctypes.c_int32),
+        ("tokens", ctypes.c_int32),
+        ("head_dim", ctypes.c_int32),
+        ("rot", ctypes.c_int32),
+        ("interleaved", ctypes.c_int32),
+        ("norm", ctypes.c_int32),
+        ("backward", ctypes.c_int32),
+        ("tensors", ctypes.c_int32),
+        ("eps", ctypes.c_float),
+        ("cs", ctypes.c_void_p),
+        ("table_rows", ctypes.c_int32),
+        ("reserved", ctypes.c_int32),
+        ("positions", ctypes.c_void_p),
+        ("pos_stride", ctypes.c_int64 * 2),
+        ("heads", B200Heads * 2),
+        ("workspace", ctypes.c_void_p),
+        ("workspace_bytes", ctypes.c_int64),
+    )
+
+
+class B200Kv4Args(ctypes.Structure):
+    """Mirror of `struct B200Kv4Args` (include/b200_decoder.h)."""
+
+    _fields_ = (
+        ("struct_size", ctypes.c_uint32),
+        ("dtype", ctypes.c_uint32),
+        ("batch", ctypes.c_int32),
+        ("tokens", ctypes.c_int32),
+        ("q_heads", ctypes.c_int32),
+        ("kv_heads", ctypes.c_int32),
+        ("head_dim", ctypes.c_int32),
+        ("rot", ctypes.c_int32),
+        ("interleaved", ctypes.c_int32),
+        ("page", ctypes.c_int32),
+        ("pages", ctypes.c_int32),
+        ("table_pages", ctypes.c_int32),
+        ("cache", ctypes.c_void_p),
+        ("page_table", ctypes.c_void_p),
+        ("table_stride", ctypes.c_int64),
+        ("lengths", ctypes.c_void_p),
+        ("cs", ctypes.c_void_p),
+        ("table_rows", ctypes.c_int32),
+        ("reserved", ctypes.c_int32),
+        ("q", ctypes.c_void_p),
+        ("k", ctypes.c_void_p),
+        ("v", ctypes.c_void_p),
+        ("q_out", ctypes.c_void_p),
+        ("k_out", ctypes.c_void_p),
+        ("v_out", ctypes.c_void_p),
+        ("q_stride", ctypes.c_int64 * 3),
+        ("k_stride", ctypes.c_int64 * 3),
+        ("v_stride", ctypes.c_int64 * 3),
+        ("q_out_stride", ctypes.c_int64 * 3),
+        ("k_out_stride", ctypes.c_int64 * 3),
+        ("v_out_stride", ctypes.c_int64 * 3),
+    )
+
+
+class B200Kv4AttnArgs(ctypes.Structure):
+    """Mirror of `struct B200Kv4AttnArgs` (include/b200_decoder.h)."""
+
+    _fields_ = (
+        ("struct_size", ctypes.c_uint32),
+        ("dtype", ctypes.c_uint32),
+        ("batch", ctypes.c_int32),
+        ("queries", ctypes.c_int32),
+        ("q_heads", ctypes.c_int32),
+        ("kv_heads", ctypes.c_int32),
+        ("head_dim", ctypes.c_int32),
+        ("page", ctypes.c_int32),
+        ("pages", ctypes.c_int32),
+        ("table_pages", ctypes.c_int32),
+        ("scale", ctypes.c_float),
+        ("reserved", ctypes.c_int32),
+        ("cache", ctypes.c_void_p),
+        ("page_table", ctypes.c_void_p),
+        ("table_stride", ctypes.c_int64),
+        ("lengths", ctypes.c_void_p),
+        ("q", ctypes.c_void_p),
+        ("o", ctypes.c_void_p),
+        ("q_stride", ctypes.c_int64 * 3),
+        ("o_stride", ctypes.c_int64 * 3),
+        ("workspace", ctypes.c_void_p),
+        ("workspace_bytes", ctypes.c_int64),
+        ("counters", ctypes.c_void_p),
+        ("counter_words", ctypes.c_int64),
+    )
+
+
 def source_hash() -> str:
     """Digest of the sources the shared object is compiled from (16 hex digits). The build passes it to the compiler,
     which puts it into the library's version string, so a binary can be matched with the sources beside it."""
@@ -377,7 +499,7 @@ def library() -> ctypes.CDLL:
         lib = ctypes.CDLL(str(SHARED_OBJECT))
     except OSError as e:
         raise KernelUnavailableError(LIBRARY, f"cannot load {SHARED_OBJECT.name}: {e}") from e
-    missing = [name for name in (*EXPORTS, *ENCODER_EXPORTS) if not hasattr(lib, name)]
+    missing = [name for name in (*EXPORTS, *ENCODER_EXPORTS, *DECODER_EXPORTS) if not hasattr(lib, name)]
     if missing:
         raise KernelUnavailableError(LIBRARY, f"{SHARED_OBJECT.name} lacks the symbols {missing}")
     lib.b200_attn_fwd.argtypes = (ctypes.POINTER(B200AttnArgs), ctypes.c_void_p)
@@ -394,6 +516,13 @@ def library() -> ctypes.CDLL:
     lib.b200_encoder_workspace.restype = ctypes.c_int
     lib.b200_encoder_forward.argtypes = (ctypes.POINTER(B200EncoderArgs), ctypes.c_void_p)
     lib.b200_encoder_forward.restype = ctypes.c_int
+    lib.b200_rotary.argtypes = (ctypes.POINTER(B200RotaryArgs), ctypes.c_void_p)
+    lib.b200_kv4_append.argtypes = lib.b200_kv4_read.argtypes = (ctypes.POINTER(B200Kv4Args), ctypes.c_void_p)
+    lib.b200_kv4_attention.argtypes = (ctypes.POINTER(B200Kv4AttnArgs), ctypes.c_void_p)
+    lib.b200_rotary_workspace.argtypes = (ctypes.POINTER(ctypes.c_int64),)
+    lib.b200_kv4_workspace.argtypes = (ctypes.POINTER(ctypes.c_int64), ctypes.POINTER(ctypes.c_int64))
+    for name in DECODER_EXPORTS:
+        getattr(lib, name).restype = ctypes.c_int
     lib.b200_attn_query.argtypes = (ctypes.POINTER(B200AttnArgs), ctypes.POINTER(ctypes.c_int32))
     lib.b200_attn_query.restype = ctypes.c_int
     i32p = ctypes.POINTER(ctypes.c_int32)

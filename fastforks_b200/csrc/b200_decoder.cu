@@ -1,0 +1,357 @@
+// C entry points of a token decoder's layers: rotary positions, norms of q and k, the paged 4-bit cache and its attention.
+// Declarations are in include/b200_decoder.h.
+#include "../../include/b200_decoder.h"
+
+#include <algorithm>
+#include <cmath>
+
+#include "../../include/b200_attn.h"
+#include "host_common.h"
+#include "kv4_attn_sm100.cuh"
+#include "kv4_sm100.cuh"
+#include "rotary_sm100.cuh"
+
+namespace b200 {
+
+namespace {
+
+constexpr int kMaxDim = 512, kRotaryCtasPerSm = 4, kKv4CtasPerSm = 3, kKv4MaxRows = 64;
+constexpr int kCounterBytes = 256;
+
+// Whether every row of a tensor of heads starts on 16 bytes.
+bool rows_aligned(const void* p, const int64_t s[3], int batch, int tokens, int heads, int size) {
+  return aligned16(p) && (batch == 1 || s[0] * size % 16 == 0) && (tokens == 1 || s[1] * size % 16 == 0) && (heads == 1 || s[2] * size % 16 == 0);
+}
+
+int lanes_of(int dim) {
+  int lanes = 1;
+  while (16 * lanes < dim) lanes *= 2;
+  return lanes;
+}
+
+template <typename T>
+const void* rotary_kernel_of(int form, bool norm, bool backward) {
+  if (norm && backward) {
+    const void* k[3] = {reinterpret_cast<const void*>(norm_rotary_backward_kernel<T, kRowHalves>), reinterpret_cast<const void*>(norm_rotary_backward_kernel<T, kRowPairs>),
+                        reinterpret_cast<const void*>(norm_rotary_backward_kernel<T, kRowAny>)};
+    return k[form];
+  }
+  const void* k[2][3] = {
+      {reinterpret_cast<const void*>(rotary_kernel<T, kRowHalves, false>), reinterpret_cast<const void*>(rotary_kernel<T, kRowPairs, false>), reinterpret_cast<const void*>(rotary_kernel<T, kRowAny, false>)},
+      {reinterpret_cast<const void*>(rotary_kernel<T, kRowHalves, true>), reinterpret_cast<const void*>(rotary_kernel<T, kRowPairs, true>), reinterpret_cast<const void*>(rotary_kernel<T, kRowAny, true>)}};
+  return k[norm ? 1 : 0][form];
+}
+
+int check_table(const char* what, const float* cs, int rot, int dim, int table_rows) {
+  if (rot < 0 || rot > dim || rot % 2 != 0) return fail(B200_ATTN_UNSUPPORTED, "%s: rot %d must be even and 0 .. %d", what, rot, dim);
+  if (rot == 0) return B200_ATTN_OK;
+  if (cs == nullptr || table_rows < 1) return fail(B200_ATTN_BAD_CONFIG, "%s: no table of positions", what);
+  if (!aligned16(cs)) return fail(B200_ATTN_UNSUPPORTED, "%s: cs is not 16-byte aligned", what);
+  return B200_ATTN_OK;
+}
+
+// The cache, its page table and the lengths, as all three calls over it have them.
+int check_cache(const char* what, uint32_t dtype, int batch, int tokens, int kv_heads, int head_dim, int page, int pages, int table_pages, const void* cache, const int32_t* table, const int32_t* lengths) {
+  if (dtype != B200_ATTN_F16 && dtype != B200_ATTN_BF16) return fail(B200_ATTN_BAD_CONFIG, "%s: dtype %u must be fp16 (0) or bf16 (1)", what, dtype);
+  if (head_dim != 64 && head_dim != 128) return fail(B200_ATTN_UNSUPPORTED, "%s: head_dim %d, only 64 and 128 are built", what, head_dim);
+  if (batch < 1 || tokens < 1 || kv_heads < 1) return fail(B200_ATTN_BAD_CONFIG, "%s: batch %d, tokens %d, kv_heads %d", what, batch, tokens, kv_heads);
+  if (page < kKv4Block || page % kKv4Block != 0) return fail(B200_ATTN_UNSUPPORTED, "%s: a page of %d tokens, it must be a multiple of 16", what, page);
+  if (pages < 1 || table_pages < 1 || static_cast<int64_t>(table_pages) * page > INT32_MAX) return fail(B200_ATTN_BAD_CONFIG, "%s: %d pages, %d in a row of the page table", what, pages, table_pages);
+  if (cache == nullptr || table == nullptr || lengths == nullptr) return fail(B200_ATTN_BAD_CONFIG, "%s: cache, page table or lengths is NULL", what);
+  if (!aligned16(cache)) return fail(B200_ATTN_UNSUPPORTED, "%s: the cache is not 16-byte aligned", what);
+  return B200_ATTN_OK;
+}
+
+int check_heads(const char* what, const char* name, const void* p, const int64_t s[3], int batch, int tokens, int heads) {
+  if (p == nullptr) return fail(B200_ATTN_BAD_CONFIG, "%s: %s is NULL", what, name);
+  if (!rows_aligned(p, s, batch, tokens, heads, 2)) return fail(B200_ATTN_UNSUPPORTED, "%s: %s must be 16-byte aligned with strides in multiples of 8 elements", what, name);
+  return B200_ATTN_OK;
+}
+
+int check_rows(const char* what, int64_t rows) {
+  return rows <= INT32_MAX ? B200_ATTN_OK : fail(B200_ATTN_UNSUPPORTED, "%s: %lld heads of tokens, at most 2^31 - 1 a call", what, static_cast<long long>(rows));
+}
+
+void set_cache(Kv4Params* p, const B200Kv4Args* a, DeviceState* dev) {
+  p->cache = static_cast<uint8_t*>(a->cache);
+  p->page_table = a->page_table;
+  p->table_stride = a->table_stride;
+  p->lengths = a->lengths;
+  p->tokens_magic = div_magic(a->tokens);
+  p->page_magic = div_magic(a->page);
+  p->tokens = a->tokens;
+  p->q_heads = a->q_heads;
+  p->kv_heads = a->kv_heads;
+  p->page = a->page;
+  p->pages = a->pages;
+  p->table_pages = a->table_pages;
+  p->status = dev->status;
+}
+
+template <typename T, int D>
+const void* append_kernel_of(int form) {
+  const void* k[3] = {reinterpret_cast<const void*>(kv4_append_kernel<T, D, kRowHalves>), reinterpret_cast<const void*>(kv4_append_kernel<T, D, kRowPairs>), reinterpret_cast<const void*>(kv4_append_kernel<T, D, kRowAny>)};
+  return k[form];
+}
+
+struct AttnForm {
+  const void* kernel;
+  size_t smem;
+  int rows;
+};
+template <typename T, int D>
+AttnForm attn_form_of(int rw) {
+  if (rw == 0) return {reinterpret_cast<const void*>(kv4_attn_kernel<T, D, 1>), Kv4AttnSmem<D, 1>::kBytes, 16};
+  if (rw == 1) return {reinterpret_cast<const void*>(kv4_attn_kernel<T, D, 2>), Kv4AttnSmem<D, 2>::kBytes, 32};
+  return {reinterpret_cast<const void*>(kv4_attn_kernel<T, D, 4>), Kv4AttnSmem<D, 4>::kBytes, 64};
+}
+std::atomic<bool> g_attn_opted_in[kMaxDevices][2][2][3];
+
+}  // namespace
+
+}  // namespace b200
+
+using namespace b200;
+
+extern "C" {
+
+int b200_rotary_workspace(int64_t* bytes) {
+  if (bytes == nullptr) return fail(B200_ATTN_BAD_CONFIG, "bytes is NULL");
+  DeviceState* dev = nullptr;
+  if (int rc = device_state(&dev)) return rc;
+  *bytes = kCounterBytes + int64_t(2) * dev->sms * kRotaryCtasPerSm * kMaxDim * 4;
+  clear_error();
+  return B200_ATTN_OK;
+}
+
+int b200_rotary(const B200RotaryArgs* a, void* stream_ptr) {
+  if (a == nullptr) return fail(B200_ATTN_BAD_CONFIG, "args is NULL");
+  if (a->struct_size != sizeof(B200RotaryArgs)) return fail(B200_ATTN_BAD_CONFIG, "struct_size %u does not match this library's B200RotaryArgs (%zu bytes)", a->struct_size, sizeof(B200RotaryArgs));
+  if (a->dtype > B200_ATTN_F32) return fail(B200_ATTN_BAD_CONFIG, "rotary: dtype %u", a->dtype);
+  if (a->norm && a->weight_dtype != a->dtype && a->weight_dtype != B200_ATTN_F32) return fail(B200_ATTN_BAD_CONFIG, "rotary: weight_dtype %u must be fp32 or that of x", a->weight_dtype);
+  if (a->batch < 1 || a->tokens < 1 || a->tensors < 1 || a->tensors > 2) return fail(B200_ATTN_BAD_CONFIG, "rotary: batch %d, tokens %d, tensors %d", a->batch, a->tokens, a->tensors);
+  if (a->head_dim < 1 || a->head_dim > kMaxDim) return fail(B200_ATTN_UNSUPPORTED, "rotary: head_dim %d must be 1 .. %d", a->head_dim, kMaxDim);
+  if (int rc = check_table("rotary", a->cs, a->rot, a->head_dim, a->table_rows)) return rc;
+  if (a->norm && !(a->eps >= 0.f)) return fail(B200_ATTN_BAD_CONFIG, "rotary: eps must not be negative");
+  const int size = a->dtype == B200_ATTN_F32 ? 4 : 2;
+  const bool reads_x = a->norm || !a->backward;
+  RotaryParams p{};
+  bool vec = true, sums = false;
+  int64_t rows = 0;
+  for (int k = 0; k < a->tensors; ++k) {
+    const B200Heads& h = a->heads[k];
+    if (h.heads < 1) return fail(B200_ATTN_BAD_CONFIG, "rotary: tensor %d has %d heads", k, h.heads);
+    if (h.y == nullptr || (reads_x && h.x == nullptr) || (a->backward && h.g == nullptr)) return fail(B200_ATTN_BAD_CONFIG, "rotary: a pointer of tensor %d is NULL", k);
+    if ((reinterpret_cast<uintptr_t>(h.y) | (reads_x ? reinterpret_cast<uintptr_t>(h.x) : 0) | (a->backward ? reinterpret_cast<uintptr_t>(h.g) : 0)) % size != 0)
+      return fail(B200_ATTN_UNSUPPORTED, "rotary: a pointer of tensor %d is not aligned to its type", k);
+    vec = vec && rows_aligned(h.y, h.y_stride, a->batch, a->tokens, h.heads, size) && (!reads_x || rows_aligned(h.x, h.x_stride, a->batch, a->tokens, h.heads, size)) &&
+          (!a->backward || rows_aligned(h.g, h.g_stride, a->batch, a->tokens, h.heads, size));
+    RotaryTensor& t = p.t[k];
+    const bool from_g = a->backward && !a->norm;  // the gradient alone goes through
+    t.x = from_g ? h.g : h.x;
+    t.y = h.y;
+    t.g = h.g;
+    t.w = a->norm ? h.w : nullptr;
+    t.dw = a->norm && a->backward ? h.dw : nullptr;
+    sums = sums || t.dw != nullptr;
+    for (int i = 0; i < 3; ++i) t.xs[i] = from_g ? h.g_stride[i] : h.x_stride[i], t.ys[i] = h.y_stride[i], t.gs[i] = h.g_stride[i];
+    t.heads = h.heads;
+    const int64_t r = static_cast<int64_t>(a->batch) * a->tokens * h.heads;
+    rows += r;
+    if (int rc = check_rows("rotary", rows)) return rc;
+    p.t_rows[k] = static_cast<uint32_t>(r);
+    p.t_magic[k] = div_magic(h.heads);
+    p.heads += h.heads;
+  }
+  DeviceState* dev = nullptr;
+  if (int rc = device_state(&dev)) return rc;
+  p.cs = a->cs;
+  p.positions = a->positions;
+  p.ps[0] = a->pos_stride[0];
+  p.ps[1] = a->pos_stride[1];
+  p.heads_magic = div_magic(p.heads);
+  p.tokens_magic = div_magic(a->tokens);
+  p.rows = static_cast<uint32_t>(rows);
+  p.table_rows = a->table_rows;
+  p.tokens = a->tokens;
+  p.dim = a->head_dim;
+  p.rot = a->rot;
+  p.lanes = lanes_of(a->head_dim);
+  p.interleaved = a->interleaved != 0;
+  p.w_f32 = a->weight_dtype == B200_ATTN_F32;
+  p.vec = vec;
+  p.eps = a->eps;
+  p.sign = a->backward ? -1.f : 1.f;
+  p.status = dev->status;
+  // Rows whose rotation and length come in whole lanes, on 16 bytes, keep partners in one lane; the others look theirs up in shared memory.
+  const int form = vec && a->head_dim % 16 == 0 && a->rot % 16 == 0 ? (p.interleaved || a->rot == 0 ? kRowPairs : kRowHalves) : kRowAny;
+  const bool norm_back = a->norm && a->backward;
+  const void* kernel = a->dtype == B200_ATTN_F16    ? rotary_kernel_of<__half>(form, a->norm, a->backward)
+                       : a->dtype == B200_ATTN_BF16 ? rotary_kernel_of<__nv_bfloat16>(form, a->norm, a->backward)
+                                                    : rotary_kernel_of<float>(form, a->norm, a->backward);
+  const int groups = kRotaryThreads / p.lanes;
+  int64_t ctas = (rows + groups - 1) / groups;
+  size_t smem = form == kRowAny ? static_cast<size_t>(groups) * p.dim * 4 : 0;
+  if (norm_back) {
+    ctas = std::min<int64_t>(ctas, static_cast<int64_t>(dev->sms) * kRotaryCtasPerSm);
+    smem = std::max(smem, static_cast<size_t>(kRotaryThreads / 32) * p.dim * 4);
+    if (sums) {
+      if (a->workspace == nullptr || !aligned16(a->workspace) || a->workspace_bytes < kCounterBytes + 2 * ctas * p.dim * 4)
+        return fail(B200_ATTN_BAD_CONFIG, "rotary: the gradient of the weights needs a workspace (b200_rotary_workspace)");
+      p.counter = static_cast<uint32_t*>(a->workspace);
+      p.partial = reinterpret_cast<float*>(static_cast<char*>(a->workspace) + kCounterBytes);
+    }
+  }
+  void* args[] = {&p};
+  if (int rc = launch_kernel(kernel, static_cast<unsigned>(ctas), 1, kRotaryThreads, smem, 1, static_cast<cudaStream_t>(stream_ptr), args, "rotary kernel launch")) return rc;
+  clear_error();
+  return B200_ATTN_OK;
+}
+
+int b200_kv4_append(const B200Kv4Args* a, void* stream_ptr) {
+  if (a == nullptr) return fail(B200_ATTN_BAD_CONFIG, "args is NULL");
+  if (a->struct_size != sizeof(B200Kv4Args)) return fail(B200_ATTN_BAD_CONFIG, "struct_size %u does not match this library's B200Kv4Args (%zu bytes)", a->struct_size, sizeof(B200Kv4Args));
+  if (int rc = check_cache("kv4_append", a->dtype, a->batch, a->tokens, a->kv_heads, a->head_dim, a->page, a->pages, a->table_pages, a->cache, a->page_table, a->lengths)) return rc;
+  if (int rc = check_table("kv4_append", a->cs, a->rot, a->head_dim, a->table_rows)) return rc;
+  const bool with_q = a->q != nullptr;
+  if (with_q && a->q_heads < 1) return fail(B200_ATTN_BAD_CONFIG, "kv4_append: %d q heads", a->q_heads);
+  if (int rc = check_heads("kv4_append", "k", a->k, a->k_stride, a->batch, a->tokens, a->kv_heads)) return rc;
+  if (int rc = check_heads("kv4_append", "v", a->v, a->v_stride, a->batch, a->tokens, a->kv_heads)) return rc;
+  if (with_q) {
+    if (int rc = check_heads("kv4_append", "q", a->q, a->q_stride, a->batch, a->tokens, a->q_heads)) return rc;
+    if (int rc = check_heads("kv4_append", "q_out", a->q_out, a->q_out_stride, a->batch, a->tokens, a->q_heads)) return rc;
+  }
+  DeviceState* dev = nullptr;
+  if (int rc = device_state(&dev)) return rc;
+  Kv4Params p{};
+  set_cache(&p, a, dev);
+  if (!with_q) p.q_heads = 0;
+  p.heads = p.q_heads + 2 * a->kv_heads;
+  const int64_t rows = static_cast<int64_t>(a->batch) * a->tokens * p.heads;
+  if (int rc = check_rows("kv4_append", rows)) return rc;
+  p.rows = static_cast<uint32_t>(rows);
+  p.heads_magic = div_magic(p.heads);
+  p.cs = a->cs;
+  p.rot = a->rot;
+  p.table_rows = a->table_rows;
+  p.interleaved = a->interleaved != 0;
+  p.q = a->q;
+  p.k = a->k;
+  p.v = a->v;
+  p.q_out = a->q_out;
+  for (int i = 0; i < 3; ++i) p.qs[i] = a->q_stride[i], p.ks[i] = a->k_stride[i], p.vs[i] = a->v_stride[i], p.qos[i] = a->q_out_stride[i];
+  const int form = a->rot % 16 == 0 ? (p.interleaved || a->rot == 0 ? kRowPairs : kRowHalves) : kRowAny;
+  const bool f16 = a->dtype == B200_ATTN_F16;
+  const void* kernel = a->head_dim == 64 ? (f16 ? append_kernel_of<__half, 64>(form) : append_kernel_of<__nv_bfloat16, 64>(form))
+                                         : (f16 ? append_kernel_of<__half, 128>(form) : append_kernel_of<__nv_bfloat16, 128>(form));
+  const int groups = kKv4Threads / (a->head_dim / 16);
+  void* args[] = {&p};
+  if (int rc = launch_kernel(kernel, static_cast<unsigned>((rows + groups - 1) / groups), 1, kKv4Threads, 0, 1, static_cast<cudaStream_t>(stream_ptr), args, "kv4_append kernel launch")) return rc;
+  clear_error();
+  return B200_ATTN_OK;
+}
+
+int b200_kv4_read(const B200Kv4Args* a, void* stream_ptr) {
+  if (a == nullptr) return fail(B200_ATTN_BAD_CONFIG, "args is NULL");
+  if (a->struct_size != sizeof(B200Kv4Args)) return fail(B200_ATTN_BAD_CONFIG, "struct_size %u does not match this library's B200Kv4Args (%zu bytes)", a->struct_size, sizeof(B200Kv4Args));
+  if (int rc = check_cache("kv4_read", a->dtype, a->batch, a->tokens, a->kv_heads, a->head_dim, a->page, a->pages, a->table_pages, a->cache, a->page_table, a->lengths)) return rc;
+  if (int rc = check_heads("kv4_read", "k_out", a->k_out, a->k_out_stride, a->batch, a->tokens, a->kv_heads)) return rc;
+  if (int rc = check_heads("kv4_read", "v_out", a->v_out, a->v_out_stride, a->batch, a->tokens, a->kv_heads)) return rc;
+  DeviceState* dev = nullptr;
+  if (int rc = device_state(&dev)) return rc;
+  Kv4Params p{};
+  set_cache(&p, a, dev);
+  p.heads = 2 * a->kv_heads;
+  const int64_t rows = static_cast<int64_t>(a->batch) * a->tokens * p.heads;
+  if (int rc = check_rows("kv4_read", rows)) return rc;
+  p.rows = static_cast<uint32_t>(rows);
+  p.heads_magic = div_magic(p.heads);
+  p.k_out = a->k_out;
+  p.v_out = a->v_out;
+  for (int i = 0; i < 3; ++i) p.kos[i] = a->k_out_stride[i], p.vos[i] = a->v_out_stride[i];
+  const bool f16 = a->dtype == B200_ATTN_F16;
+  const void* kernel = a->head_dim == 64 ? (f16 ? reinterpret_cast<const void*>(kv4_read_kernel<__half, 64>) : reinterpret_cast<const void*>(kv4_read_kernel<__nv_bfloat16, 64>))
+                                         : (f16 ? reinterpret_cast<const void*>(kv4_read_kernel<__half, 128>) : reinterpret_cast<const void*>(kv4_read_kernel<__nv_bfloat16, 128>));
+  const int groups = kKv4Threads / (a->head_dim / 16);
+  void* args[] = {&p};
+  if (int rc = launch_kernel(kernel, static_cast<unsigned>((rows + groups - 1) / groups), 1, kKv4Threads, 0, 1, static_cast<cudaStream_t>(stream_ptr), args, "kv4_read kernel launch")) return rc;
+  clear_error();
+  return B200_ATTN_OK;
+}
+
+int b200_kv4_workspace(int64_t* bytes, int64_t* counter_words) {
+  if (bytes == nullptr || counter_words == nullptr) return fail(B200_ATTN_BAD_CONFIG, "bytes or counter_words is NULL");
+  DeviceState* dev = nullptr;
+  if (int rc = device_state(&dev)) return rc;
+  const int64_t ctas = static_cast<int64_t>(dev->sms) * kKv4CtasPerSm;
+  *bytes = ctas * 2 * kKv4MaxRows * (128 * 4 + 8);
+  *counter_words = ctas;
+  clear_error();
+  return B200_ATTN_OK;
+}
+
+int b200_kv4_attention(const B200Kv4AttnArgs* a, void* stream_ptr) {
+  if (a == nullptr) return fail(B200_ATTN_BAD_CONFIG, "args is NULL");
+  if (a->struct_size != sizeof(B200Kv4AttnArgs)) return fail(B200_ATTN_BAD_CONFIG, "struct_size %u does not match this library's B200Kv4AttnArgs (%zu bytes)", a->struct_size, sizeof(B200Kv4AttnArgs));
+  if (int rc = check_cache("kv4_attention", a->dtype, a->batch, a->queries, a->kv_heads, a->head_dim, a->page, a->pages, a->table_pages, a->cache, a->page_table, a->lengths)) return rc;
+  if (a->q_heads < 1 || a->q_heads % a->kv_heads != 0) return fail(B200_ATTN_BAD_CONFIG, "kv4_attention: %d q heads are no multiple of %d kv heads", a->q_heads, a->kv_heads);
+  if (!(a->scale > 0.f) || !std::isfinite(a->scale)) return fail(B200_ATTN_UNSUPPORTED, "kv4_attention: scale must be positive and finite");
+  if (int rc = check_heads("kv4_attention", "q", a->q, a->q_stride, a->batch, a->queries, a->q_heads)) return rc;
+  if (int rc = check_heads("kv4_attention", "o", a->o, a->o_stride, a->batch, a->queries, a->q_heads)) return rc;
+  DeviceState* dev = nullptr;
+  if (int rc = device_state(&dev)) return rc;
+  const int group = a->q_heads / a->kv_heads;
+  const int64_t rows = static_cast<int64_t>(a->queries) * group;
+  if (int rc = check_rows("kv4_attention", rows * a->kv_heads * a->batch)) return rc;
+  const int rw = rows <= 16 ? 0 : rows <= 32 ? 1 : 2;
+  const bool f16 = a->dtype == B200_ATTN_F16;
+  const AttnForm form = a->head_dim == 64 ? (f16 ? attn_form_of<__half, 64>(rw) : attn_form_of<__nv_bfloat16, 64>(rw)) : (f16 ? attn_form_of<__half, 128>(rw) : attn_form_of<__nv_bfloat16, 128>(rw));
+  Kv4AttnParams p{};
+  p.cache = static_cast<const uint8_t*>(a->cache);
+  p.page_table = a->page_table;
+  p.table_stride = a->table_stride;
+  p.lengths = a->lengths;
+  p.q = a->q;
+  p.o = a->o;
+  for (int i = 0; i < 3; ++i) p.qs[i] = a->q_stride[i], p.os[i] = a->o_stride[i];
+  p.page_blocks = a->page / kKv4Block;
+  p.group_magic = div_magic(group);
+  p.bpp_magic = div_magic(p.page_blocks);
+  p.scale_log2 = a->scale * 1.4426950408889634f;
+  p.batch = a->batch;
+  p.queries = a->queries;
+  p.q_heads = a->q_heads;
+  p.kv_heads = a->kv_heads;
+  p.group = group;
+  p.rows = static_cast<int>(rows);
+  p.row_tiles = static_cast<int>((rows + form.rows - 1) / form.rows);
+  p.pages = a->pages;
+  p.table_pages = a->table_pages;
+  p.status = dev->status;
+  // The lengths are on the device: the grid is for the longest that the page table allows, CTAs without a run leave at once.
+  p.min_run = 8;
+  const int64_t most = static_cast<int64_t>(a->batch) * p.row_tiles * a->kv_heads * a->table_pages * p.page_blocks;
+  if (most >= (int64_t(1) << 38)) return fail(B200_ATTN_UNSUPPORTED, "kv4_attention: %lld blocks of sixteen tokens, at most 2^38 a call", static_cast<long long>(most));
+  const int64_t ctas = std::min<int64_t>(static_cast<int64_t>(dev->sms) * kKv4CtasPerSm, (most + p.min_run - 1) / p.min_run);
+  const int64_t partial = ctas * 2 * form.rows * a->head_dim * 4, ml = ctas * 2 * form.rows * 8;
+  if (a->workspace == nullptr || !aligned16(a->workspace) || a->workspace_bytes < partial + ml || a->counters == nullptr || a->counter_words < ctas)
+    return fail(B200_ATTN_BAD_CONFIG, "kv4_attention: the workspace or the counters are missing or too small (b200_kv4_workspace)");
+  p.partial = static_cast<float*>(a->workspace);
+  p.partial_ml = reinterpret_cast<float2*>(static_cast<char*>(a->workspace) + partial);
+  p.counters = a->counters;
+  int device = 0;
+  cudaError_t e = cudaGetDevice(&device);
+  if (e != cudaSuccess) return cuda_fail(e, "cudaGetDevice");
+  std::atomic<bool>& opted_in = g_attn_opted_in[device][f16 ? 0 : 1][a->head_dim == 64 ? 0 : 1][rw];
+  if (!opted_in.load(std::memory_order_acquire)) {
+    e = cudaFuncSetAttribute(form.kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(form.smem));
+    if (e != cudaSuccess) return cuda_fail(e, "kv4_attention: shared memory opt-in");
+    opted_in.store(true, std::memory_order_release);
+  }
+  void* args[] = {&p};
+  if (int rc = launch_kernel(form.kernel, static_cast<unsigned>(ctas), 1, kKv4AttnThreads, form.smem, 1, static_cast<cudaStream_t>(stream_ptr), args, "kv4_attention kernel launch")) return rc;
+  clear_error();
+  return B200_ATTN_OK;
+}
+
+}  // extern "C"

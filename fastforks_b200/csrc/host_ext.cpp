@@ -11,12 +11,14 @@
 #include <c10/cuda/CUDAStream.h>
 #include <torch/csrc/autograd/python_variable.h>
 
+#include <cmath>
 #include <cstring>
 #include <memory>
 #include <mutex>
 #include <vector>
 
 #include "../../include/b200_attn.h"
+#include "../../include/b200_decoder.h"
 
 namespace {
 
@@ -316,6 +318,273 @@ PyObject* py_rope(PyObject*, PyObject* const* args, Py_ssize_t n) {
   Py_RETURN_TRUE;
 }
 
+// ---- a token decoder's layers ----
+
+bool heads_type(const at::Tensor& t) { return half_type(t) || t.scalar_type() == at::kFloat; }
+uint32_t any_dtype_code(const at::Tensor& t) { return t.scalar_type() == at::kFloat ? B200_ATTN_F32 : dtype_code(t); }
+bool fits32(const at::Tensor& t) {
+  for (int64_t n : t.sizes())
+    if (n > INT32_MAX) return false;
+  return true;
+}
+// A plain, filled tensor of heads with unit last stride.
+bool heads_of(const at::Tensor* t, c10::DeviceIndex device) {
+  return t != nullptr && plain(*t, device) && t->dim() == 4 && t->stride(3) == 1 && t->numel() > 0 && fits32(*t);
+}
+void set_heads(int64_t* s, const at::Tensor& t) {
+  for (int i = 0; i < 3; ++i) s[i] = t.stride(i);
+}
+bool table_of(const at::Tensor* t, c10::DeviceIndex device, int64_t dim) {
+  return t != nullptr && plain(*t, device) && t->scalar_type() == at::kFloat && t->dim() == 3 && t->size(1) == 2 && t->size(0) >= 1 && t->size(2) >= 1 && 2 * t->size(2) <= dim &&
+         t->is_contiguous() && fits32(*t);
+}
+
+// Table and positions of `a` for the tokens of x.
+bool set_turn(B200RotaryArgs* a, const at::Tensor& x, PyObject* table, PyObject* positions, c10::DeviceIndex device) {
+  if (table == Py_None) return positions == Py_None;
+  const at::Tensor* t = tensor_of(table);
+  if (!table_of(t, device, x.size(3))) return false;
+  a->cs = static_cast<const float*>(t->data_ptr());
+  a->rot = static_cast<int32_t>(2 * t->size(2));
+  a->table_rows = static_cast<int32_t>(t->size(0));
+  if (positions == Py_None) return t->size(0) >= x.size(1);
+  const at::Tensor* p = tensor_of(positions);
+  if (p == nullptr || !plain(*p, device) || p->scalar_type() != at::kInt) return false;
+  if (p->dim() == 1 && p->size(0) == x.size(1)) {
+    a->pos_stride[1] = p->stride(0);
+  } else if (p->dim() == 2 && p->size(0) == x.size(0) && p->size(1) == x.size(1)) {
+    a->pos_stride[0] = p->stride(0);
+    a->pos_stride[1] = p->stride(1);
+  } else {
+    return false;
+  }
+  a->positions = static_cast<const int32_t*>(p->data_ptr());
+  return true;
+}
+
+void set_rotary(B200RotaryArgs* a, const at::Tensor& x, PyObject* interleaved) {
+  a->struct_size = sizeof(*a);
+  a->dtype = a->weight_dtype = any_dtype_code(x);
+  a->batch = static_cast<int32_t>(x.size(0));
+  a->tokens = static_cast<int32_t>(x.size(1));
+  a->head_dim = static_cast<int32_t>(x.size(3));
+  a->interleaved = interleaved == Py_True;
+}
+
+// rotary(x, table, positions | None, interleaved)
+PyObject* py_rotary(PyObject*, PyObject* const* args, Py_ssize_t n) {
+  if (n != 4 || !PyBool_Check(args[3]) || args[1] == Py_None) Py_RETURN_NONE;
+  const at::Tensor* x = tensor_of(args[0]);
+  const c10::DeviceIndex device = c10::cuda::current_device();
+  if (!heads_of(x, device) || !heads_type(*x)) Py_RETURN_NONE;
+  B200RotaryArgs a;
+  std::memset(&a, 0, sizeof(a));
+  set_rotary(&a, *x, args[3]);
+  if (!set_turn(&a, *x, args[1], args[2], device)) Py_RETURN_NONE;
+  at::Tensor y = empty_like_type(x->sizes(), *x);
+  a.tensors = 1;
+  B200Heads& h = a.heads[0];
+  h.x = x->data_ptr();
+  h.y = y.data_ptr();
+  set_heads(h.x_stride, *x);
+  set_heads(h.y_stride, y);
+  h.heads = static_cast<int32_t>(x->size(2));
+  const c10::cuda::CUDAStream stream = c10::cuda::getCurrentCUDAStream(device);
+  if (launched([&] { return b200_rotary(&a, stream.stream()); }) != B200_ATTN_OK) Py_RETURN_NONE;
+  return THPVariable_Wrap(y);
+}
+
+// qk_norm_rotary(q, k, q_weight | None, k_weight | None, table | None, positions | None, eps, interleaved)
+PyObject* py_qk_norm_rotary(PyObject*, PyObject* const* args, Py_ssize_t n) {
+  if (n != 8 || !PyBool_Check(args[7])) Py_RETURN_NONE;
+  const c10::DeviceIndex device = c10::cuda::current_device();
+  const at::Tensor* x[2] = {tensor_of(args[0]), tensor_of(args[1])};
+  double eps = 0;
+  if (!heads_of(x[0], device) || !heads_of(x[1], device) || !heads_type(*x[0]) || x[1]->scalar_type() != x[0]->scalar_type() || !number(args[6], &eps) || !(eps >= 0)) Py_RETURN_NONE;
+  for (int i : {0, 1, 3})
+    if (x[1]->size(i) != x[0]->size(i)) Py_RETURN_NONE;
+  B200RotaryArgs a;
+  std::memset(&a, 0, sizeof(a));
+  set_rotary(&a, *x[0], args[7]);
+  if (!set_turn(&a, *x[0], args[4], args[5], device)) Py_RETURN_NONE;
+  const at::Tensor* first = nullptr;
+  for (int k = 0; k < 2; ++k) {
+    if (args[2 + k] == Py_None) continue;
+    const at::Tensor* w = tensor_of(args[2 + k]);
+    if (w == nullptr || !plain(*w, device) || w->dim() != 1 || w->size(0) != x[0]->size(3) || !w->is_contiguous()) Py_RETURN_NONE;
+    if (w->scalar_type() != x[0]->scalar_type() && w->scalar_type() != at::kFloat) Py_RETURN_NONE;
+    if (first != nullptr && first->scalar_type() != w->scalar_type()) Py_RETURN_NONE;
+    first = w;
+    a.heads[k].w = w->data_ptr();
+    a.weight_dtype = any_dtype_code(*w);
+  }
+  a.norm = 1;
+  a.eps = static_cast<float>(eps);
+  a.tensors = 2;
+  at::Tensor y[2];
+  for (int k = 0; k < 2; ++k) {
+    y[k] = empty_like_type(x[k]->sizes(), *x[k]);
+    B200Heads& h = a.heads[k];
+    h.x = x[k]->data_ptr();
+    h.y = y[k].data_ptr();
+    set_heads(h.x_stride, *x[k]);
+    set_heads(h.y_stride, y[k]);
+    h.heads = static_cast<int32_t>(x[k]->size(2));
+  }
+  const c10::cuda::CUDAStream stream = c10::cuda::getCurrentCUDAStream(device);
+  if (launched([&] { return b200_rotary(&a, stream.stream()); }) != B200_ATTN_OK) Py_RETURN_NONE;
+  return Py_BuildValue("(NN)", THPVariable_Wrap(y[0]), THPVariable_Wrap(y[1]));
+}
+
+// Cache, page table and lengths of a call on `batch` sequences.
+template <typename A>
+bool set_cache(A* a, PyObject* cache, PyObject* page_table, PyObject* lengths, int64_t batch, c10::DeviceIndex device) {
+  const at::Tensor *c = tensor_of(cache), *t = tensor_of(page_table), *l = tensor_of(lengths);
+  if (c == nullptr || t == nullptr || l == nullptr || !plain(*c, device) || !plain(*t, device) || !plain(*l, device)) return false;
+  if (c->scalar_type() != at::kByte || c->dim() != 4 || !c->is_contiguous() || c->numel() == 0 || !fits32(*c)) return false;
+  if (c->size(3) != 16 * (64 + 8) && c->size(3) != 16 * (128 + 8)) return false;
+  if (t->scalar_type() != at::kInt || t->dim() != 2 || t->size(0) != batch || t->size(1) < 1 || t->stride(1) != 1 || !fits32(*t)) return false;
+  if (l->scalar_type() != at::kInt || l->dim() != 1 || l->size(0) != batch || !l->is_contiguous()) return false;
+  if (c->size(2) > INT32_MAX / 16) return false;
+  a->struct_size = sizeof(*a);
+  a->batch = static_cast<int32_t>(batch);
+  a->kv_heads = static_cast<int32_t>(c->size(1));
+  a->head_dim = static_cast<int32_t>(c->size(3) / 16 - 8);
+  a->page = static_cast<int32_t>(16 * c->size(2));
+  a->pages = static_cast<int32_t>(c->size(0));
+  a->table_pages = static_cast<int32_t>(t->size(1));
+  a->cache = static_cast<uint8_t*>(c->data_ptr());
+  a->page_table = static_cast<const int32_t*>(t->data_ptr());
+  a->table_stride = t->stride(0);
+  a->lengths = static_cast<const int32_t*>(l->data_ptr());
+  return true;
+}
+
+// kv4_append_(cache, k, v, page_table, lengths, table | None, interleaved, q | None) -> the turned q, or True without q
+PyObject* py_kv4_append(PyObject*, PyObject* const* args, Py_ssize_t n) {
+  if (n != 8 || !PyBool_Check(args[6])) Py_RETURN_NONE;
+  const c10::DeviceIndex device = c10::cuda::current_device();
+  const at::Tensor *k = tensor_of(args[1]), *v = tensor_of(args[2]), *q = tensor_of(args[7]);
+  if (!heads_of(k, device) || !heads_of(v, device) || !half_type(*k) || v->scalar_type() != k->scalar_type() || v->sizes() != k->sizes()) Py_RETURN_NONE;
+  B200Kv4Args a;
+  std::memset(&a, 0, sizeof(a));
+  if (!set_cache(&a, args[0], args[3], args[4], k->size(0), device) || k->size(2) != a.kv_heads || k->size(3) != a.head_dim) Py_RETURN_NONE;
+  if (args[5] != Py_None) {
+    const at::Tensor* t = tensor_of(args[5]);
+    if (!table_of(t, device, a.head_dim)) Py_RETURN_NONE;
+    a.cs = static_cast<const float*>(t->data_ptr());
+    a.rot = static_cast<int32_t>(2 * t->size(2));
+    a.table_rows = static_cast<int32_t>(t->size(0));
+  }
+  a.dtype = dtype_code(*k);
+  a.tokens = static_cast<int32_t>(k->size(1));
+  a.interleaved = args[6] == Py_True;
+  a.k = k->data_ptr();
+  a.v = v->data_ptr();
+  set_heads(a.k_stride, *k);
+  set_heads(a.v_stride, *v);
+  at::Tensor out;
+  if (args[7] != Py_None) {
+    if (!heads_of(q, device) || q->scalar_type() != k->scalar_type() || q->size(0) != k->size(0) || q->size(1) != k->size(1) || q->size(3) != k->size(3)) Py_RETURN_NONE;
+    out = empty_like_type(q->sizes(), *q);
+    a.q_heads = static_cast<int32_t>(q->size(2));
+    a.q = q->data_ptr();
+    a.q_out = out.data_ptr();
+    set_heads(a.q_stride, *q);
+    set_heads(a.q_out_stride, out);
+  }
+  const c10::cuda::CUDAStream stream = c10::cuda::getCurrentCUDAStream(device);
+  if (launched([&] { return b200_kv4_append(&a, stream.stream()); }) != B200_ATTN_OK) Py_RETURN_NONE;
+  if (args[7] == Py_None) Py_RETURN_TRUE;
+  return THPVariable_Wrap(out);
+}
+
+// kv4_read(cache, page_table, lengths, tokens, True: fp16 | False: bf16 | None)
+PyObject* py_kv4_read(PyObject*, PyObject* const* args, Py_ssize_t n) {
+  if (n != 5 || !PyBool_Check(args[4])) Py_RETURN_NONE;
+  const c10::DeviceIndex device = c10::cuda::current_device();
+  const at::Tensor *c = tensor_of(args[0]), *l = tensor_of(args[2]);
+  int64_t tokens = 0;
+  if (c == nullptr || l == nullptr || l->dim() != 1 || l->size(0) < 1 || !integer(args[3], &tokens) || tokens < 1) Py_RETURN_NONE;
+  B200Kv4Args a;
+  std::memset(&a, 0, sizeof(a));
+  if (!set_cache(&a, args[0], args[1], args[2], l->size(0), device)) Py_RETURN_NONE;
+  const bool f16 = args[4] == Py_True;
+  a.dtype = f16 ? B200_ATTN_F16 : B200_ATTN_BF16;
+  a.tokens = static_cast<int32_t>(tokens);
+  const int64_t sizes[4] = {a.batch, tokens, a.kv_heads, a.head_dim};
+  at::Tensor k = at::detail::empty_cuda(sizes, f16 ? at::kHalf : at::kBFloat16, c->device(), std::nullopt);
+  at::Tensor v = at::detail::empty_cuda(sizes, f16 ? at::kHalf : at::kBFloat16, c->device(), std::nullopt);
+  a.k_out = k.data_ptr();
+  a.v_out = v.data_ptr();
+  set_heads(a.k_out_stride, k);
+  set_heads(a.v_out_stride, v);
+  const c10::cuda::CUDAStream stream = c10::cuda::getCurrentCUDAStream(device);
+  if (launched([&] { return b200_kv4_read(&a, stream.stream()); }) != B200_ATTN_OK) Py_RETURN_NONE;
+  return Py_BuildValue("(NN)", THPVariable_Wrap(k), THPVariable_Wrap(v));
+}
+
+// Workspace and counters of attention over the cache, registered like the attention workspaces above.
+struct Kv4Workspace {
+  int64_t v[6];  // device, stream, workspace, bytes, counters, words
+};
+std::vector<Kv4Workspace> g_kv4_workspaces;
+
+PyObject* py_register_kv4_workspace(PyObject*, PyObject* const* args, Py_ssize_t n) {
+  if (n != 6) {
+    PyErr_SetString(PyExc_TypeError, "register_kv4_workspace(device, stream, workspace, bytes, counters, words)");
+    return nullptr;
+  }
+  Kv4Workspace w;
+  for (int i = 0; i < 6; ++i) w.v[i] = static_cast<int64_t>(PyLong_AsUnsignedLongLongMask(args[i]));
+  if (PyErr_Occurred()) return nullptr;
+  std::lock_guard<std::mutex> lock(g_workspaces_mutex);
+  for (Kv4Workspace& had : g_kv4_workspaces)
+    if (had.v[0] == w.v[0] && had.v[1] == w.v[1]) {
+      had = w;
+      Py_RETURN_NONE;
+    }
+  g_kv4_workspaces.push_back(w);
+  Py_RETURN_NONE;
+}
+
+// kv4_attention(q, cache, page_table, lengths, scale | None)
+PyObject* py_kv4_attention(PyObject*, PyObject* const* args, Py_ssize_t n) {
+  if (n != 5) Py_RETURN_NONE;
+  const c10::DeviceIndex device = c10::cuda::current_device();
+  const at::Tensor* q = tensor_of(args[0]);
+  if (!heads_of(q, device) || !half_type(*q)) Py_RETURN_NONE;
+  B200Kv4AttnArgs a;
+  std::memset(&a, 0, sizeof(a));
+  if (!set_cache(&a, args[1], args[2], args[3], q->size(0), device) || q->size(3) != a.head_dim || q->size(2) % a.kv_heads != 0) Py_RETURN_NONE;
+  double scale = 0;
+  if (args[4] == Py_None) a.scale = static_cast<float>(1.0 / std::sqrt(static_cast<double>(a.head_dim)));
+  else if (number(args[4], &scale)) a.scale = static_cast<float>(scale);
+  else Py_RETURN_NONE;
+  const c10::cuda::CUDAStream stream = c10::cuda::getCurrentCUDAStream(device);
+  {
+    std::lock_guard<std::mutex> lock(g_workspaces_mutex);
+    for (const Kv4Workspace& w : g_kv4_workspaces)
+      if (w.v[0] == device && w.v[1] == reinterpret_cast<int64_t>(stream.stream())) {
+        a.workspace = reinterpret_cast<void*>(w.v[2]);
+        a.workspace_bytes = w.v[3];
+        a.counters = reinterpret_cast<uint32_t*>(w.v[4]);
+        a.counter_words = w.v[5];
+      }
+  }
+  if (a.workspace == nullptr) Py_RETURN_NONE;
+  at::Tensor out = empty_like_type(q->sizes(), *q);
+  a.dtype = dtype_code(*q);
+  a.queries = static_cast<int32_t>(q->size(1));
+  a.q_heads = static_cast<int32_t>(q->size(2));
+  a.q = q->data_ptr();
+  a.o = out.data_ptr();
+  set_heads(a.q_stride, *q);
+  set_heads(a.o_stride, out);
+  if (launched([&] { return b200_kv4_attention(&a, stream.stream()); }) != B200_ATTN_OK) Py_RETURN_NONE;
+  return THPVariable_Wrap(out);
+}
+
 // sam_rel_terms(q, rel_pos_h, rel_pos_w, side)
 PyObject* py_rel_terms(PyObject*, PyObject* const* args, Py_ssize_t n) {
   if (n != 4) Py_RETURN_NONE;
@@ -431,6 +700,12 @@ PyMethodDef methods[] = {
     {"sam_rel_terms", fast<py_rel_terms>(), METH_FASTCALL, nullptr},
     {"snapshot", fast<py_snapshot>(), METH_FASTCALL, nullptr},
     {"unchanged", fast<py_unchanged>(), METH_FASTCALL, nullptr},
+    {"rotary", fast<py_rotary>(), METH_FASTCALL, nullptr},
+    {"qk_norm_rotary", fast<py_qk_norm_rotary>(), METH_FASTCALL, nullptr},
+    {"kv4_append_", fast<py_kv4_append>(), METH_FASTCALL, nullptr},
+    {"kv4_read", fast<py_kv4_read>(), METH_FASTCALL, nullptr},
+    {"kv4_attention", fast<py_kv4_attention>(), METH_FASTCALL, nullptr},
+    {"register_kv4_workspace", fast<py_register_kv4_workspace>(), METH_FASTCALL, nullptr},
     {"register_workspace", fast<py_register_workspace>(), METH_FASTCALL, nullptr},
     {nullptr, nullptr, 0, nullptr},
 };

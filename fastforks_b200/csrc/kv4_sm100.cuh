@@ -1,0 +1,208 @@
+// A paged cache of keys and values held in 4 bits: writing new tokens (keys and queries rotated on the way) and reading them back.
+// The layout is stated in include/b200_decoder.h; it is the attention kernel's: a block of sixteen tokens of one head is contiguous, a
+// lane's codes of K are consecutive, and a 32-bit word of V holds the same four dimensions of two neighbouring tokens, which is what a
+// 16 x 8 tile of the second product takes from one lane.
+//
+// A head's vector of one token is a group: step = bf16((max - min) / 15), least = bf16(min), code = clamp(round((x - least) / step)). The
+// codes are taken against the rounded pair, so rounding it costs no accuracy that the codes do not get back; the largest value may lie
+// 15 * 2^-9 of a step above the last code. Division is by multiplication with the rounded reciprocal of 15 and of the step.
+//
+// Bound by launch latency for single tokens and by HBM for prompts. Rows (a head of q, k or v of one token) are four or eight lanes of
+// sixteen values, as in the rotary kernels.
+#pragma once
+
+#include "rotary_sm100.cuh"
+
+namespace b200 {
+
+constexpr int kKv4Block = 16;  // tokens
+template <int D>
+struct Kv4Layout {
+  static constexpr int kRowK = D / 2, kV = 8 * D, kRowV = D + 16, kBytes = 16 * (D + 8);
+};
+
+struct Kv4Params {
+  uint8_t* cache;
+  const int32_t* page_table;
+  int64_t table_stride;
+  const int32_t* lengths;
+  const float* cs;
+  const void *q, *k, *v;
+  void *q_out, *k_out, *v_out;
+  int64_t qs[3], ks[3], vs[3], qos[3], kos[3], vos[3];
+  uint64_t heads_magic, tokens_magic, page_magic;
+  uint32_t rows;
+  int tokens, q_heads, kv_heads, rot, page, pages, table_pages, table_rows, heads;
+  bool interleaved;
+  uint32_t* status;
+};
+
+constexpr int kKv4Threads = 256;
+
+// Address of the block that holds position `at` of sequence `b` for `head`, and the token's place in it; nullptr if there is none.
+template <int D>
+__device__ __forceinline__ uint8_t* kv4_block(const Kv4Params& p, uint32_t b, int at, int head, int* token) {
+  const uint32_t col = magic_div(at, p.page_magic);
+  if (col >= static_cast<uint32_t>(p.table_pages)) {
+    atomicOr(p.status, kStatusPage);
+    return nullptr;
+  }
+  const int page = p.page_table[b * p.table_stride + col];
+  if (page < 0 || page >= p.pages) {
+    atomicOr(p.status, kStatusPage);
+    return nullptr;
+  }
+  const int in_page = at - static_cast<int>(col) * p.page;
+  *token = in_page & (kKv4Block - 1);
+  const int blocks = p.page / kKv4Block;
+  return p.cache + ((static_cast<int64_t>(page) * p.kv_heads + head) * blocks + in_page / kKv4Block) * Kv4Layout<D>::kBytes;
+}
+
+__device__ __forceinline__ float min_nan(float a, float b) {
+  float r;
+  asm("min.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+  return r;
+}
+__device__ __forceinline__ float max_nan(float a, float b) {
+  float r;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+  return r;
+}
+
+// Codes of a group's values, 16 in this lane and the others in the LANES - 1 lanes beside it: eight codes in either word, the first in the
+// lowest bits. Returns the pair (step in the low, least value in the high half).
+template <int LANES>
+__device__ __forceinline__ uint32_t quantise16(const float* f, uint32_t* words) {
+  float low = f[0], high = f[0];
+#pragma unroll
+  for (int i = 1; i < 16; ++i) {
+    low = min_nan(low, f[i]);
+    high = max_nan(high, f[i]);
+  }
+#pragma unroll
+  for (int o = LANES / 2; o > 0; o >>= 1) {
+    low = min_nan(low, __shfl_xor_sync(0xffffffffu, low, o));
+    high = max_nan(high, __shfl_xor_sync(0xffffffffu, high, o));
+  }
+  const float span = __fsub_rn(high, low);
+  words[0] = words[1] = 0;
+  if (!(fabsf(span) < INFINITY)) return 0x7fc07fc0u;
+  float step = __bfloat162float(__float2bfloat16_rn(__fmul_rn(span, 1.f / 15.f)));
+  const float least = __bfloat162float(__float2bfloat16_rn(low));
+  if (!(fabsf(least) < INFINITY) || !(step < INFINITY)) return 0x7fc07fc0u;  // rounded past the largest bfloat16
+  if (step < 1.17549435e-38f) {
+    step = 0.f;
+  } else {
+    const float inverse = __frcp_rn(step);
+#pragma unroll
+    for (int i = 0; i < 16; ++i) {
+      const float t = fminf(fmaxf(rintf(__fmul_rn(__fsub_rn(f[i], least), inverse)), 0.f), 15.f);
+      words[i >> 3] |= static_cast<uint32_t>(t) << (4 * (i & 7));
+    }
+  }
+  return (__float_as_uint(step) >> 16) | (__float_as_uint(least) & 0xffff0000u);
+}
+
+template <typename T, int D, int FORM>
+__global__ void __launch_bounds__(kKv4Threads) kv4_append_kernel(const Kv4Params p) {
+  constexpr int kLanes = D / 16, kGroups = kKv4Threads / kLanes;
+  using L = Kv4Layout<D>;
+  __shared__ float rows_smem[FORM == kRowAny ? kGroups * D : 1];
+  grid_dependency_wait();
+  grid_launch_dependents();
+  const int j = threadIdx.x % kLanes, group = threadIdx.x / kLanes;
+  const uint32_t row = blockIdx.x * kGroups + group;
+  const bool there = row < p.rows;
+  const uint32_t token = magic_div(there ? row : 0, p.heads_magic);
+  int h = static_cast<int>((there ? row : 0) - token * p.heads);
+  const uint32_t b = magic_div(token, p.tokens_magic), n = token - b * p.tokens;
+  const int what = h < p.q_heads ? 0 : h < p.q_heads + p.kv_heads ? 1 : 2;
+  h -= what == 0 ? 0 : what == 1 ? p.q_heads : p.q_heads + p.kv_heads;
+  const int64_t* s = what == 0 ? p.qs : what == 1 ? p.ks : p.vs;
+  const T* x = static_cast<const T*>(what == 0 ? p.q : what == 1 ? p.k : p.v) + b * s[0] + n * s[1] + h * s[2];
+  int at0, at1;
+  lane_places<FORM>(j, p.rot, &at0, &at1);
+  if (what == 2) at0 = 16 * j, at1 = 16 * j + 8;
+  float f[16];
+  {
+    Raw8<T> u, v;
+    u.load(x + at0);
+    v.load(x + at1);
+    u.unpack(f);
+    v.unpack(f + 8);
+  }
+  const int at = p.lengths[b] - p.tokens + static_cast<int>(n);
+  const float* cs = what == 2 ? nullptr : table_row(p.cs, p.rot, p.table_rows, at, p.status);
+  rotate16<FORM>(f, cs, j, p.rot, D, 1.f, p.interleaved, rows_smem + (FORM == kRowAny ? group * D : 0));
+  uint32_t words[2];
+  const uint32_t pair = quantise16<kLanes>(f, words);
+  if (!there) return;
+  if (what == 0) {
+    T* y = static_cast<T*>(p.q_out) + b * p.qos[0] + n * p.qos[1] + h * p.qos[2];
+    store8<T>(y + at0, f);
+    store8<T>(y + at1, f + 8);
+    return;
+  }
+  if (at < 0) return;
+  int t;
+  uint8_t* block = kv4_block<D>(p, b, at, h, &t);
+  if (block == nullptr) return;
+  uint8_t* tail = block + L::kV + (t >> 1) * L::kRowV;
+  if (what == 1) {
+    uint32_t* codes = reinterpret_cast<uint32_t*>(block + t * L::kRowK);
+    codes[at0 >> 3] = words[0];
+    codes[at1 >> 3] = words[1];
+  } else {
+    uint16_t* codes = reinterpret_cast<uint16_t*>(tail) + (t & 1);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) codes[2 * (4 * j + i)] = static_cast<uint16_t>(words[i >> 1] >> (16 * (i & 1)));
+  }
+  if (j == 0) *reinterpret_cast<uint32_t*>(tail + D + (t & 1) * 8 + (what == 2 ? 4 : 0)) = pair;
+}
+
+// The values of the last tokens, in 16 bits.
+template <typename T, int D>
+__global__ void __launch_bounds__(kKv4Threads) kv4_read_kernel(const Kv4Params p) {
+  constexpr int kLanes = D / 16, kGroups = kKv4Threads / kLanes;
+  using L = Kv4Layout<D>;
+  grid_dependency_wait();
+  grid_launch_dependents();
+  const int j = threadIdx.x % kLanes;
+  const uint32_t row = blockIdx.x * kGroups + threadIdx.x / kLanes;
+  if (row >= p.rows) return;
+  const uint32_t token = magic_div(row, p.heads_magic);
+  int h = static_cast<int>(row - token * p.heads);
+  const bool is_v = h >= p.kv_heads;
+  if (is_v) h -= p.kv_heads;
+  const uint32_t b = magic_div(token, p.tokens_magic), n = token - b * p.tokens;
+  const int at = p.lengths[b] - p.tokens + static_cast<int>(n);
+  float f[16];
+#pragma unroll
+  for (int i = 0; i < 16; ++i) f[i] = 0.f;
+  int t = 0;
+  const uint8_t* block = at < 0 ? nullptr : kv4_block<D>(p, b, at, h, &t);
+  if (block != nullptr) {
+    const uint8_t* tail = block + L::kV + (t >> 1) * L::kRowV;
+    uint32_t words[2];
+    if (!is_v) {
+      const uint2 w = *reinterpret_cast<const uint2*>(block + t * L::kRowK + 8 * j);
+      words[0] = w.x;
+      words[1] = w.y;
+    } else {
+      const uint4 w = *reinterpret_cast<const uint4*>(tail + 16 * j);
+      const int low = t & 1 ? 0x7632 : 0x5410;  // this token's half of either word
+      words[0] = __byte_perm(w.x, w.y, low);
+      words[1] = __byte_perm(w.z, w.w, low);
+    }
+    const uint32_t pair = *reinterpret_cast<const uint32_t*>(tail + D + (t & 1) * 8 + (is_v ? 4 : 0));
+    const float step = __uint_as_float(pair << 16), least = __uint_as_float(pair & 0xffff0000u);
+#pragma unroll
+    for (int i = 0; i < 16; ++i) f[i] = fmaf(step, static_cast<float>((words[i >> 3] >> (4 * (i & 7))) & 15u), least);  // the product is exact
+  }
+  const int64_t* s = is_v ? p.vos : p.kos;
+  T* y = static_cast<T*>(is_v ? p.v_out : p.k_out) + b * s[0] + n * s[1] + h * s[2] + 16 * j;
+  store8<T>(y, f);
+  store8<T>(y + 8, f + 8);
+}
+
+}  // namespace b200
