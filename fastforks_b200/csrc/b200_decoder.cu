@@ -15,7 +15,7 @@ namespace b200 {
 
 namespace {
 
-constexpr int kMaxDim = 512, kRotaryCtasPerSm = 4, kKv4CtasPerSm = 3, kKv4MaxRows = 64;
+constexpr int kMaxDim = 512, kRotaryCtasPerSm = 4, kKv4CtasPerSm = 4, kKv4MaxRows = 64;
 constexpr int kCounterBytes = 256;
 
 // Whether every row of a tensor of heads starts on 16 bytes.
@@ -96,16 +96,19 @@ const void* append_kernel_of(int form) {
 
 struct AttnForm {
   const void* kernel;
-  size_t smem;
-  int rows;
+  int smem, rows, ctas_per_sm;
 };
-template <typename T, int D>
-AttnForm attn_form_of(int rw) {
-  if (rw == 0) return {reinterpret_cast<const void*>(kv4_attn_kernel<T, D, 1>), Kv4AttnSmem<D, 1>::kBytes, 16};
-  if (rw == 1) return {reinterpret_cast<const void*>(kv4_attn_kernel<T, D, 2>), Kv4AttnSmem<D, 2>::kBytes, 32};
-  return {reinterpret_cast<const void*>(kv4_attn_kernel<T, D, 4>), Kv4AttnSmem<D, 4>::kBytes, 64};
+constexpr int kAttnForms = 4;
+template <typename T, int D, int NR, int RW>
+AttnForm attn_form() {
+  using S = Kv4AttnSmem<D, NR, RW>;
+  return {reinterpret_cast<const void*>(kv4_attn_kernel<T, D, NR, RW>), S::kBytes, 8 * NR * RW, S::kCtasPerSm};
 }
-std::atomic<bool> g_attn_opted_in[kMaxDevices][2][2][3];
+template <typename T, int D>
+AttnForm attn_form_of(int form) {
+  return form == 0 ? attn_form<T, D, 1, 1>() : form == 1 ? attn_form<T, D, 2, 1>() : form == 2 ? attn_form<T, D, 2, 2>() : attn_form<T, D, 2, 4>();
+}
+std::atomic<bool> g_attn_opted_in[kMaxDevices][2][2][kAttnForms];
 
 }  // namespace
 
@@ -303,9 +306,9 @@ int b200_kv4_attention(const B200Kv4AttnArgs* a, void* stream_ptr) {
   const int group = a->q_heads / a->kv_heads;
   const int64_t rows = static_cast<int64_t>(a->queries) * group;
   if (int rc = check_rows("kv4_attention", rows * a->kv_heads * a->batch)) return rc;
-  const int rw = rows <= 16 ? 0 : rows <= 32 ? 1 : 2;
+  const int which = rows <= 8 ? 0 : rows <= 16 ? 1 : rows <= 32 ? 2 : 3;
   const bool f16 = a->dtype == B200_ATTN_F16;
-  const AttnForm form = a->head_dim == 64 ? (f16 ? attn_form_of<__half, 64>(rw) : attn_form_of<__nv_bfloat16, 64>(rw)) : (f16 ? attn_form_of<__half, 128>(rw) : attn_form_of<__nv_bfloat16, 128>(rw));
+  const AttnForm form = a->head_dim == 64 ? (f16 ? attn_form_of<__half, 64>(which) : attn_form_of<__nv_bfloat16, 64>(which)) : (f16 ? attn_form_of<__half, 128>(which) : attn_form_of<__nv_bfloat16, 128>(which));
   Kv4AttnParams p{};
   p.cache = static_cast<const uint8_t*>(a->cache);
   p.page_table = a->page_table;
@@ -329,10 +332,10 @@ int b200_kv4_attention(const B200Kv4AttnArgs* a, void* stream_ptr) {
   p.table_pages = a->table_pages;
   p.status = dev->status;
   // The lengths are on the device: the grid is for the longest that the page table allows, CTAs without a run leave at once.
-  p.min_run = 8;
-  const int64_t most = static_cast<int64_t>(a->batch) * p.row_tiles * a->kv_heads * a->table_pages * p.page_blocks;
-  if (most >= (int64_t(1) << 38)) return fail(B200_ATTN_UNSUPPORTED, "kv4_attention: %lld blocks of sixteen tokens, at most 2^38 a call", static_cast<long long>(most));
-  const int64_t ctas = std::min<int64_t>(static_cast<int64_t>(dev->sms) * kKv4CtasPerSm, (most + p.min_run - 1) / p.min_run);
+  p.min_run = 4;
+  const int64_t most = static_cast<int64_t>(a->batch) * p.row_tiles * a->kv_heads * ((static_cast<int64_t>(a->table_pages) * a->page + kKv4Step - 1) / kKv4Step);
+  if (most >= (int64_t(1) << 38)) return fail(B200_ATTN_UNSUPPORTED, "kv4_attention: %lld steps of 32 tokens, at most 2^38 a call", static_cast<long long>(most));
+  const int64_t ctas = std::min<int64_t>(static_cast<int64_t>(dev->sms) * form.ctas_per_sm, (most + p.min_run - 1) / p.min_run);
   const int64_t partial = ctas * 2 * form.rows * a->head_dim * 4, ml = ctas * 2 * form.rows * 8;
   if (a->workspace == nullptr || !aligned16(a->workspace) || a->workspace_bytes < partial + ml || a->counters == nullptr || a->counter_words < ctas)
     return fail(B200_ATTN_BAD_CONFIG, "kv4_attention: the workspace or the counters are missing or too small (b200_kv4_workspace)");
@@ -342,9 +345,9 @@ int b200_kv4_attention(const B200Kv4AttnArgs* a, void* stream_ptr) {
   int device = 0;
   cudaError_t e = cudaGetDevice(&device);
   if (e != cudaSuccess) return cuda_fail(e, "cudaGetDevice");
-  std::atomic<bool>& opted_in = g_attn_opted_in[device][f16 ? 0 : 1][a->head_dim == 64 ? 0 : 1][rw];
+  std::atomic<bool>& opted_in = g_attn_opted_in[device][f16 ? 0 : 1][a->head_dim == 64 ? 0 : 1][which];
   if (!opted_in.load(std::memory_order_acquire)) {
-    e = cudaFuncSetAttribute(form.kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(form.smem));
+    e = cudaFuncSetAttribute(form.kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, form.smem);
     if (e != cudaSuccess) return cuda_fail(e, "kv4_attention: shared memory opt-in");
     opted_in.store(true, std::memory_order_release);
   }

@@ -8,12 +8,18 @@
 // after a power of two for each row that puts its largest value near 2^10; p vs goes in as fp16 after a power of two (shared by a warp,
 // raised like a running maximum when a larger step comes along) that keeps p vs below 2^15. Logits, maxima, sums and both accumulators are fp32.
 //
-// A warp has 16 rows (queries x the q heads that share a kv head) and walks blocks of 16 tokens. CTAs of four warps: up to 16 rows all
-// four warps share the rows and take every fourth block, each with its own softmax state, joined at the end; up to 32 two and two; above
-// that four warps have 64 rows and share each block. Blocks are contiguous in the cache: one bulk copy brings codes and parameters of 16
-// tokens into a ring in shared memory.
+// Codes are the left operand: S^T = K Q^T has 16 tokens by 8 rows, O^T = V^T P^T 16 dimensions by 8 rows, so that eight rows (the q heads
+// that share a kv head, of one query) fill a product. P^T comes out of the first product with tokens along the lanes and goes
+// into the second with rows along them: one transposition of 8 x 8 in registers for each eight tokens. Codes of V multiply p vs as
+// code - 8 (one more row of the product sums 8 p vs), and vl + 8 vs takes the rest in fp32: rounding p vs then errs by a part of a value, not of a
+// code up to 15.
 //
-// Work is laid on one line: sequences, row tiles, kv heads, blocks. Each CTA takes an equal run of it, whatever the lengths are. An
+// A warp has 8 or 16 rows (queries x the q heads that share a kv head) and walks steps of 32 tokens. CTAs of four warps: up to 16 rows all
+// four warps share the rows and take every fourth step, each with its own softmax state, joined at the end; up to 32 two and two; above
+// that four warps have 64 rows and share each step. Blocks are contiguous in the cache, and so are the two of a step where pages hold a
+// multiple of 32 tokens: bulk copies bring codes and parameters into a ring in shared memory.
+//
+// Work is laid on one line: sequences, row tiles, kv heads, steps. Each CTA takes an equal run of it, whatever the lengths are. An
 // item (sequence, row tile, head) cut by the end of a run is finished by the CTA that counts last: partial outputs, maxima and sums go to
 // the workspace and are joined in their order, so the result does not depend on which CTA that is.
 #pragma once
@@ -34,26 +40,33 @@ struct Kv4AttnParams {
   float scale_log2;
   int batch, queries, q_heads, kv_heads, group, rows, row_tiles;
   int pages, table_pages, page_blocks;
-  int min_run;         // blocks a CTA takes at least
+  int min_run;         // steps a CTA takes at least
   float* partial;      // [CTA][2][row][dim], unnormalised
   float2* partial_ml;  // [CTA][2][row]: maximum (log2) and sum
   uint32_t* counters;  // [CTA]
   uint32_t* status;
 };
 
-constexpr int kKv4AttnThreads = 128, kKv4Stages = 4;
+constexpr int kKv4AttnThreads = 128, kKv4Stages = 2, kKv4Step = 2 * kKv4Block;
 constexpr uint32_t kStatusKv4Wait = 1u << 22;
 
-template <int D, int RW>
+// NR: tiles of eight rows of a warp. RW: warps with rows of their own, the other 4 / RW share theirs.
+template <int D, int NR, int RW>
 struct Kv4AttnSmem {
   static constexpr int kTW = 4 / RW;  // warps that share rows
   static constexpr int kBlock = Kv4Layout<D>::kBytes;
-  static constexpr int kRing = kTW * kKv4Stages * kBlock;
-  static constexpr int kMerge = kTW > 1 ? 4 * 32 * (D / 2) * 4 : 0;  // each warp's accumulators
-  static constexpr int kMl = kRing + kMerge;                         // [4][16] float2
-  static constexpr int kBars = kMl + 4 * 16 * 8;                     // full, empty
-  static constexpr int kFlags = kBars + 2 * kTW * kKv4Stages * 8;
+  static constexpr int kRing = kTW * kKv4Stages * 2 * kBlock;
+  static constexpr int kRegs = NR * D / 4;                           // accumulators of a lane
+  static constexpr int kMerge = kTW > 1 ? 4 * 32 * kRegs * 4 : 0;    // each warp's
+  // q's operand words are a lane's registers for one tile of rows, in shared memory for two
+  static constexpr bool kQInSmem = NR > 1;
+  static constexpr int kQ = kRing + kMerge;                                 // [RW][32 lanes][NR D / 8] words
+  static constexpr int kMl = kQ + (kQInSmem ? RW * 32 * NR * D / 8 * 4 : 0);  // [4][8 NR] float2
+  static constexpr int kBars = kMl + 4 * 8 * NR * 8;                        // full, empty
+  static constexpr int kAhead = kBars + 2 * kTW * kKv4Stages * 8;           // [kTW] Kv4Ahead
+  static constexpr int kFlags = kAhead + kTW * 48;
   static constexpr int kBytes = kFlags + 16;
+  static constexpr int kCtasPerSm = NR == 1 ? 4 : 3;
 };
 
 __device__ __forceinline__ void bulk_load(void* smem, const void* gmem, uint32_t bytes, uint64_t* bar) {
@@ -71,6 +84,13 @@ __device__ __forceinline__ void split_codes(uint32_t w, uint32_t* pairs) {
   pairs[3] = h & 0x00f000f0u;
 }
 
+// An 8 x 8 matrix of 16-bit values, lane l holding columns 2 (l % 4) and the next of row l / 4, transposed.
+__device__ __forceinline__ uint32_t transpose_8x8(uint32_t v) {
+  uint32_t r;
+  asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(v));
+  return r;
+}
+
 __device__ __forceinline__ float exp2_approx(float x) {
   float y;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
@@ -78,13 +98,20 @@ __device__ __forceinline__ float exp2_approx(float x) {
 }
 __device__ __forceinline__ float pow2(int e) { return __int_as_float((e + 127) << 23); }  // -126 <= e <= 127
 
-// A CTA's place on the line: an item and the blocks of it that are this CTA's.
+// A CTA's place on the line: an item and the steps of it that are this CTA's.
 struct Kv4Segment {
   int b, tile, head;  // head runs fastest
-  int len, blocks;    // of sequence b
+  int len, steps;     // of sequence b
   int s0, s1;
-  int left;           // blocks of the run behind this segment
+  int left;           // steps of the run behind this segment
 };
+
+// The producer's place of a token warp, in shared memory: the segment it is in, its next step there and the end of those that are seen.
+struct Kv4Ahead {
+  Kv4Segment seg;
+  int s, end, more, pad;
+};
+static_assert(sizeof(Kv4Ahead) == 48, "Kv4AttnSmem::kFlags");
 
 __device__ __forceinline__ int kv4_length(const Kv4AttnParams& p, int b) {
   const int n = p.lengths[b], most = p.table_pages * p.page_blocks * kKv4Block;
@@ -97,38 +124,38 @@ __device__ __forceinline__ bool kv4_next(const Kv4AttnParams& p, Kv4Segment& s) 
     s.head = 0;
     if (++s.tile == p.row_tiles) {
       s.tile = 0;
-      do {  // blocks are left on the line, so a sequence with some follows
+      do {  // steps are left on the line, so a sequence with some follows
         if (++s.b >= p.batch) return false;
         s.len = kv4_length(p, s.b);
       } while (s.len == 0);
-      s.blocks = (s.len + kKv4Block - 1) / kKv4Block;
+      s.steps = (s.len + kKv4Step - 1) / kKv4Step;
     }
   }
   s.s0 = 0;
-  s.s1 = min(s.blocks, s.left);
+  s.s1 = min(s.steps, s.left);
   s.left -= s.s1;
   return true;
 }
 
-// Blocks of the segment that some row of its tile sees: [s0, result).
+// Steps of the segment that some row of its tile sees: [s0, result).
 template <int ROWS>
 __device__ __forceinline__ int kv4_seen(const Kv4AttnParams& p, const Kv4Segment& s) {
   const int last = min(p.rows, (s.tile + 1) * ROWS) - 1;
   const int limit = s.len - p.queries + static_cast<int>(magic_div(last, p.group_magic)) + 1;
-  return max(s.s0, min(s.s1, (limit + kKv4Block - 1) / kKv4Block));
+  return max(s.s0, min(s.s1, (limit + kKv4Step - 1) / kKv4Step));
 }
 
-template <typename T, int D, int RW>
-__global__ void __launch_bounds__(kKv4AttnThreads, 3) kv4_attn_kernel(const Kv4AttnParams p) {
-  using S = Kv4AttnSmem<D, RW>;
+template <typename T, int D, int NR, int RW>
+__global__ void __launch_bounds__(kKv4AttnThreads, Kv4AttnSmem<D, NR, RW>::kCtasPerSm) kv4_attn_kernel(const Kv4AttnParams p) {
+  using S = Kv4AttnSmem<D, NR, RW>;
   using L = Kv4Layout<D>;
-  constexpr int kTW = S::kTW, kRows = 16 * RW;
-  constexpr int kWordsK = D / 32;            // words of codes of K in a lane, for each token
-  constexpr int kTiles = D / 8;              // column tiles of the output
+  constexpr int kTW = S::kTW, kWarpRows = 8 * NR, kRows = kWarpRows * RW;
+  constexpr int kWords = D / 32;  // words of codes in a lane, for each token of K and each two of V
+  constexpr int kTiles = D / 16;  // row tiles of the output
   extern __shared__ __align__(128) uint8_t smem[];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, r = lane >> 2, c = lane & 3;
   const int rw = warp % RW, tw = warp / RW;
-  uint8_t* ring = smem + tw * kKv4Stages * S::kBlock;
+  uint8_t* ring = smem + tw * kKv4Stages * 2 * S::kBlock;
   float* merge = reinterpret_cast<float*>(smem + S::kRing);
   float2* ml_smem = reinterpret_cast<float2*>(smem + S::kMl);
   uint64_t* full = reinterpret_cast<uint64_t*>(smem + S::kBars) + tw * kKv4Stages;
@@ -145,7 +172,7 @@ __global__ void __launch_bounds__(kKv4AttnThreads, 3) kv4_attn_kernel(const Kv4A
   grid_dependency_wait();
   grid_launch_dependents();
 
-  // The line: blocks of all items, and this CTA's run of it.
+  // The line: steps of all items, and this CTA's run of it.
   const int per = p.kv_heads * p.row_tiles;
   long long total = 0;
   {
@@ -153,14 +180,15 @@ __global__ void __launch_bounds__(kKv4AttnThreads, 3) kv4_attn_kernel(const Kv4A
     for (int b = lane; b < p.batch; b += 32) {
       const int n = p.lengths[b], len = kv4_length(p, b);
       if (n != len && n > 0 && threadIdx.x < 32 && blockIdx.x == 0) atomicOr(p.status, kStatusPage);
-      mine += (len + kKv4Block - 1) / kKv4Block;
+      mine += (len + kKv4Step - 1) / kKv4Step;
     }
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) mine += __shfl_xor_sync(0xffffffffu, mine, o);
     total = mine * per;
   }
-  const long long run = max(static_cast<long long>(p.min_run), (total + gridDim.x - 1) / gridDim.x);
-  const long long begin = run * blockIdx.x, end = min(total, begin + run);
+  const int run = static_cast<int>(max(static_cast<long long>(p.min_run), (total + gridDim.x - 1) / gridDim.x));
+  const long long begin = static_cast<long long>(run) * blockIdx.x;
+  const int count = static_cast<int>(max(0ll, min(static_cast<long long>(run), total - begin)));
 
   // Rows that see nothing at all get zeros: whole sequences without tokens are on no CTA's run, and rows in front of a sequence's start
   // are written by whoever has their item.
@@ -171,18 +199,17 @@ __global__ void __launch_bounds__(kKv4AttnThreads, 3) kv4_attn_kernel(const Kv4A
       *reinterpret_cast<uint4*>(static_cast<T*>(p.o) + b * p.os[0] + n * p.os[1] + h * p.os[2] + 8 * d) = make_uint4(0, 0, 0, 0);
     }
   }
-  if (begin >= end) return;
+  if (count == 0) return;
 
   Kv4Segment seg{};
-  long long item_begin = 0;  // of the segment's item, on the line
   {
     // The sequence the run begins in: 32 lengths at a time.
     long long before = 0;
     int b0 = 0;
     for (;; b0 += 32) {
       const int b = b0 + lane;
-      const int blocks = b < p.batch ? (kv4_length(p, b) + kKv4Block - 1) / kKv4Block : 0;
-      long long sum = static_cast<long long>(blocks) * per;
+      const int steps = b < p.batch ? (kv4_length(p, b) + kKv4Step - 1) / kKv4Step : 0;
+      long long sum = static_cast<long long>(steps) * per;
 #pragma unroll
       for (int o = 1; o < 32; o <<= 1) {
         const long long v = __shfl_up_sync(0xffffffffu, sum, o);
@@ -192,8 +219,8 @@ __global__ void __launch_bounds__(kKv4AttnThreads, 3) kv4_attn_kernel(const Kv4A
       if (hit != 0) {  // always, at the latest with the last sequence: begin < total
         const int l = __ffs(hit) - 1;
         seg.b = b0 + l;
-        seg.blocks = __shfl_sync(0xffffffffu, blocks, l);
-        before += __shfl_sync(0xffffffffu, sum, l) - static_cast<long long>(seg.blocks) * per;
+        seg.steps = __shfl_sync(0xffffffffu, steps, l);
+        before += __shfl_sync(0xffffffffu, sum, l) - static_cast<long long>(seg.steps) * per;
         break;
       }
       before += __shfl_sync(0xffffffffu, sum, 31);
@@ -201,75 +228,94 @@ __global__ void __launch_bounds__(kKv4AttnThreads, 3) kv4_attn_kernel(const Kv4A
     }
     seg.len = kv4_length(p, seg.b);
     const long long in = begin - before;
-    const int item = static_cast<int>(in / seg.blocks);
-    seg.s0 = static_cast<int>(in - static_cast<long long>(item) * seg.blocks);
+    const int item = static_cast<int>(in / seg.steps);
+    seg.s0 = static_cast<int>(in - static_cast<long long>(item) * seg.steps);
     seg.tile = item / p.kv_heads;
     seg.head = item - seg.tile * p.kv_heads;
-    item_begin = begin - seg.s0;
-    const long long count = end - begin;
-    seg.s1 = static_cast<int>(min(static_cast<long long>(seg.blocks), seg.s0 + count));
-    seg.left = static_cast<int>(count - (seg.s1 - seg.s0));
+    seg.s1 = min(seg.steps, seg.s0 + count);
+    seg.left = count - (seg.s1 - seg.s0);
   }
 
-  // The producer's own place: it runs kKv4Stages blocks ahead, over the ends of items. One lane of the first row warp of each token warp.
+  // The producer runs kKv4Stages steps ahead, over the ends of items: lane 0 of the first row warp of each token warp.
   const bool producer = rw == 0;
-  Kv4Segment ahead = seg;
-  int ahead_s = ahead.s0 + tw, ahead_end = kv4_seen<kRows>(p, ahead);
-  bool more = true;
-  uint32_t issued = 0, used = 0;  // blocks of this token warp, in order
+  Kv4Ahead& ahead = *reinterpret_cast<Kv4Ahead*>(smem + S::kAhead + tw * sizeof(Kv4Ahead));
+  uint32_t issued = 0, used = 0;  // steps of this token warp, in order
   bool ok = true;
-  auto issue = [&]() {
-    while (more && ahead_s >= ahead_end) {
-      more = kv4_next(p, ahead);
-      if (more) {
-        ahead_s = ahead.s0 + tw;
-        ahead_end = kv4_seen<kRows>(p, ahead);
+  const auto issue = [&]() {
+    int at = ahead.s, end = ahead.end;
+    if (at >= end) {
+      if (ahead.more == 0) return;
+      Kv4Segment next = ahead.seg;
+      bool more = true;
+      do {
+        more = kv4_next(p, next);
+        if (!more) break;
+        at = next.s0 + tw;
+        end = kv4_seen<kRows>(p, next);
+      } while (at >= end);
+      ahead.seg = next;
+      ahead.end = end;
+      ahead.more = more ? 1 : 0;
+      if (!more) {
+        ahead.s = end;
+        return;
       }
     }
-    if (!more) return;
     const uint32_t stage = issued % kKv4Stages, round = issued / kKv4Stages;
     if (RW > 1 && round > 0 && !mbar_wait(empty + stage, (round - 1) & 1, abort_flag)) {
+      ahead.more = 0;
+      ahead.s = end;
       ok = false;
-      more = false;
       return;
     }
-    if (lane == 0) {
-      const uint32_t col = magic_div(ahead_s, p.bpp_magic);
-      int page = p.page_table[ahead.b * p.table_stride + col];
+    const int b = ahead.seg.b, head = ahead.seg.head;
+    const auto block_at = [&](int block) {
+      const uint32_t col = magic_div(block, p.bpp_magic);
+      int page = p.page_table[b * p.table_stride + col];
       if (page < 0 || page >= p.pages) {
         atomicOr(p.status, kStatusPage);
         page = 0;
       }
-      const uint8_t* from = p.cache + ((static_cast<int64_t>(page) * p.kv_heads + ahead.head) * p.page_blocks + (ahead_s - static_cast<int>(col) * p.page_blocks)) * S::kBlock;
-      mbar_arrive_expect_tx(full + stage, S::kBlock);
-      bulk_load(ring + stage * S::kBlock, from, S::kBlock, full + stage);
-    }
-    __syncwarp();
+      return p.cache + ((static_cast<int64_t>(page) * p.kv_heads + head) * p.page_blocks + (block - static_cast<int>(col) * p.page_blocks)) * S::kBlock;
+    };
+    const bool two = at * kKv4Step + kKv4Block < ahead.seg.len;  // the second block may hold nothing: what lies there is then masked
+    const bool joined = (p.page_blocks & 1) == 0;                // the blocks of a step follow one another
+    uint8_t* to = ring + stage * 2 * S::kBlock;
+    const uint8_t* from = block_at(2 * at);
+    mbar_arrive_expect_tx(full + stage, two ? 2 * S::kBlock : S::kBlock);
+    bulk_load(to, from, two && joined ? 2 * S::kBlock : S::kBlock, full + stage);
+    if (two && !joined) bulk_load(to + S::kBlock, block_at(2 * at + 1), S::kBlock, full + stage);
     ++issued;
-    ahead_s += kTW;
+    ahead.s = at + kTW;
   };
-  if (producer) {
+  if (producer && lane == 0) {
+    ahead.seg = seg;
+    ahead.s = seg.s0 + tw;
+    ahead.end = kv4_seen<kRows>(p, seg);
+    ahead.more = 1;
     for (int i = 0; i < kKv4Stages; ++i) issue();
   }
+  __syncwarp();
 
   for (;;) {
-    // Rows r and r + 8 of this warp's 16: their queries as operand words, in the order of a lane's codes.
-    const int row0 = seg.tile * kRows + 16 * rw;
-    uint32_t qa[2][4 * kWordsK];
-    float rscale[2], qsum[2], m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f}, ms[2] = {0.f, 0.f};
-    int pos[2];
+    // Row r of each tile of eight: its queries as operand words, in the order of a lane's codes. What belongs to a row of the products
+    // is kept by the lanes that hold the products' columns, rows 2 c and 2 c + 1.
+    const int row0 = seg.tile * kRows + kWarpRows * rw;
+    uint32_t qb[S::kQInSmem ? 1 : NR][4 * kWords];
+    uint4* q_smem = reinterpret_cast<uint4*>(smem + S::kQ) + rw * 32 * NR * kWords;  // [NR][kWords][32 lanes]; the warps that share rows write the same
+    // off: the maximum that the sums are relative to (log2); limit: logits above need a larger one, -inf: nothing is seen yet.
+    float rscale[NR][2], qsum[NR][2], off[NR][2], l[NR][2], ms[NR][2], limit[NR][2];
 #pragma unroll
-    for (int i = 0; i < 2; ++i) {
-      const int row = min(row0 + r + 8 * i, p.rows - 1);
+    for (int t = 0; t < NR; ++t) {
+      const int row = min(row0 + 8 * t + r, p.rows - 1);
       const int n = static_cast<int>(magic_div(row, p.group_magic)), g = row - n * p.group;
-      pos[i] = seg.len - p.queries + n;
       const T* x = static_cast<const T*>(p.q) + seg.b * p.qs[0] + n * p.qs[1] + (seg.head * p.group + g) * p.qs[2] + c * (D / 4);
       float most = 0.f;
-      Raw8<T> raw[kWordsK];
+      Raw8<T> raw[kWords];
 #pragma unroll
-      for (int w = 0; w < kWordsK; ++w) raw[w].load(x + 8 * w);
+      for (int w = 0; w < kWords; ++w) raw[w].load(x + 8 * w);
 #pragma unroll
-      for (int w = 0; w < kWordsK; ++w) {
+      for (int w = 0; w < kWords; ++w) {
         float f[8];
         raw[w].unpack(f);
 #pragma unroll
@@ -282,7 +328,7 @@ __global__ void __launch_bounds__(kKv4AttnThreads, 3) kv4_attn_kernel(const Kv4A
       const float up = pow2(10 - e);
       float sum = 0.f;
 #pragma unroll
-      for (int w = 0; w < kWordsK; ++w) {
+      for (int w = 0; w < kWords; ++w) {
         float f[8];
         raw[w].unpack(f);
 #pragma unroll
@@ -290,26 +336,40 @@ __global__ void __launch_bounds__(kKv4AttnThreads, 3) kv4_attn_kernel(const Kv4A
           f[k] *= up;
           sum += f[k];
         }
+        uint32_t words[4];
 #pragma unroll
         for (int k = 0; k < 4; ++k) {
           const float by = k & 1 ? 0.0625f : 1.f;
-          qa[i][4 * w + k] = pack2<__half>(f[k] * by, f[k + 4] * by);
+          words[k] = pack2<__half>(f[k] * by, f[k + 4] * by);
+          if (!S::kQInSmem) qb[S::kQInSmem ? 0 : t][4 * w + k] = words[k];
         }
+        if (S::kQInSmem) q_smem[(t * kWords + w) * 32 + lane] = make_uint4(words[0], words[1], words[2], words[3]);
       }
       sum += __shfl_xor_sync(0xffffffffu, sum, 1);
       sum += __shfl_xor_sync(0xffffffffu, sum, 2);
-      qsum[i] = sum * 5.9604644775390625e-08f;                   // the logits of this row are in units of 2^(e - 10) 2^24
-      rscale[i] = p.scale_log2 * pow2(min(e + 14, 127));
-    }
-    const int seen_by_all = min(pos[0], pos[1]);  // (the lowest of the warp's rows is lane 0's, and all lanes ask it)
-    const int lowest = __shfl_sync(0xffffffffu, seen_by_all, 0);
-    float o[kTiles][4];
+      const float scale = p.scale_log2 * pow2(min(e + 14, 127));  // logits of this row are in units of 2^(e - 10) 2^24
 #pragma unroll
-    for (int i = 0; i < kTiles; ++i) o[i][0] = o[i][1] = o[i][2] = o[i][3] = 0.f;
-    int vexp = -120;      // steps of V are taken times 2^(6 - vexp)
-    float vscale = 0.f;   // 2^(6 - vexp); 0: no step seen yet
-    float vlimit = 0.f;   // steps from here on need a larger vexp
-    float limit[2] = {-INFINITY, -INFINITY};  // logits above need a larger maximum
+      for (int i = 0; i < 2; ++i) {
+        const int from = 4 * (2 * c + i);
+        qsum[t][i] = __shfl_sync(0xffffffffu, sum, from) * 5.9604644775390625e-08f;
+        rscale[t][i] = __shfl_sync(0xffffffffu, scale, from);
+        limit[t][i] = -INFINITY;
+        off[t][i] = l[t][i] = ms[t][i] = 0.f;
+      }
+    }
+    // Position of a row; a row past the last one is taken for it.
+    const auto position = [&](int row) { return seg.len - p.queries + static_cast<int>(magic_div(min(row, p.rows - 1), p.group_magic)); };
+    const int lowest = position(row0);
+    float o[NR][kTiles][4], eights[NR][4];
+#pragma unroll
+    for (int t = 0; t < NR; ++t) {
+#pragma unroll
+      for (int i = 0; i < kTiles; ++i) o[t][i][0] = o[t][i][1] = o[t][i][2] = o[t][i][3] = 0.f;
+      eights[t][0] = eights[t][1] = eights[t][2] = eights[t][3] = 0.f;
+    }
+    int vexp = -120;     // steps of V are taken times 2^(6 - vexp)
+    float vscale = 0.f;  // 2^(6 - vexp); 0: no step seen yet
+    float vlimit = 0.f;  // steps from here on need a larger vexp
 
     const int seen = kv4_seen<kRows>(p, seg);
 #pragma unroll 1
@@ -318,114 +378,148 @@ __global__ void __launch_bounds__(kKv4AttnThreads, 3) kv4_attn_kernel(const Kv4A
       ok = ok && mbar_wait(full + stage, round & 1, abort_flag);
       ok = __all_sync(0xffffffffu, ok);
       if (!ok) break;
-      const uint8_t* block = ring + stage * S::kBlock;
-      // q . u of two tiles of eight tokens
-      float x[2][4];
+      const uint8_t* step = ring + stage * 2 * S::kBlock;
+      const int base = s * kKv4Step;
+      const bool masked = base + kKv4Step - 1 > lowest;
+      float x[2][NR][4];  // blocks; tokens r and r + 8, rows 2 c and 2 c + 1
+      float vs[2][2], vl[2][2];
+      bool raise = false;
+      float big = 0.f;  // largest step of V
+      {
+        uint32_t w[2][2][kWords];
 #pragma unroll
-      for (int t = 0; t < 2; ++t) {
-        uint32_t w[kWordsK];
-        const uint8_t* at = block + (8 * t + r) * L::kRowK + c * (D / 8);
-        if constexpr (D == 128) {
-          const uint4 v = *reinterpret_cast<const uint4*>(at);
-          w[0] = v.x, w[1] = v.y, w[2] = v.z, w[3] = v.w;
-        } else {
-          const uint2 v = *reinterpret_cast<const uint2*>(at);
-          w[0] = v.x, w[1] = v.y;
-        }
-        x[t][0] = x[t][1] = x[t][2] = x[t][3] = 0.f;
-#pragma unroll
-        for (int i = 0; i < kWordsK; ++i) {
-          uint32_t u[4];
-          split_codes(w[i], u);
+        for (int h = 0; h < 2; ++h) {
 #pragma unroll
           for (int k = 0; k < 2; ++k) {
-            const uint32_t a[4] = {qa[0][4 * i + 2 * k], qa[1][4 * i + 2 * k], qa[0][4 * i + 2 * k + 1], qa[1][4 * i + 2 * k + 1]};
-            mma_16816<__half>(x[t], a, u[2 * k], u[2 * k + 1]);
+            const uint8_t* at = step + h * S::kBlock + (8 * k + r) * L::kRowK + c * (D / 8);
+            if constexpr (D == 128) {
+              const uint4 v = *reinterpret_cast<const uint4*>(at);
+              w[h][k][0] = v.x, w[h][k][1] = v.y, w[h][k][2] = v.z, w[h][k][3] = v.w;
+            } else {
+              const uint2 v = *reinterpret_cast<const uint2*>(at);
+              w[h][k][0] = v.x, w[h][k][1] = v.y;
+            }
+          }
+#pragma unroll
+          for (int t = 0; t < NR; ++t) x[h][t][0] = x[h][t][1] = x[h][t][2] = x[h][t][3] = 0.f;
+        }
+#pragma unroll
+        for (int i = 0; i < kWords; ++i) {
+          uint32_t q[NR][4];
+#pragma unroll
+          for (int t = 0; t < NR; ++t) {
+            if constexpr (S::kQInSmem) {
+              const uint4 v = q_smem[(t * kWords + i) * 32 + lane];
+              q[t][0] = v.x, q[t][1] = v.y, q[t][2] = v.z, q[t][3] = v.w;
+            } else {
+#pragma unroll
+              for (int k = 0; k < 4; ++k) q[t][k] = qb[t][4 * i + k];
+            }
+          }
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            uint32_t u0[4], u1[4];
+            split_codes(w[h][0][i], u0);
+            split_codes(w[h][1][i], u1);
+#pragma unroll
+            for (int k = 0; k < 2; ++k) {
+              const uint32_t a[4] = {u0[2 * k], u1[2 * k], u0[2 * k + 1], u1[2 * k + 1]};
+#pragma unroll
+              for (int t = 0; t < NR; ++t) mma_16816<__half>(x[h][t], a, q[t][2 * k], q[t][2 * k + 1]);
+            }
           }
         }
       }
-      // steps and least values of tokens 2 c, 2 c + 1 and 8 behind them
-      float ks[4], kl[4], vs[4], vl[4];
 #pragma unroll
-      for (int t = 0; t < 2; ++t) {
-        const uint4 v = *reinterpret_cast<const uint4*>(block + L::kV + (c + 4 * t) * L::kRowV + D);
-        ks[2 * t] = __uint_as_float(v.x << 16), kl[2 * t] = __uint_as_float(v.x & 0xffff0000u);
-        vs[2 * t] = __uint_as_float(v.y << 16), vl[2 * t] = __uint_as_float(v.y & 0xffff0000u);
-        ks[2 * t + 1] = __uint_as_float(v.z << 16), kl[2 * t + 1] = __uint_as_float(v.z & 0xffff0000u);
-        vs[2 * t + 1] = __uint_as_float(v.w << 16), vl[2 * t + 1] = __uint_as_float(v.w & 0xffff0000u);
-      }
-      const int base = s * kKv4Block;
-      const bool masked = base + kKv4Block - 1 > lowest;
-      if (masked) {  // parameters behind the sequence's end are whatever the page held
+      for (int h = 0; h < 2; ++h) {
+        const uint8_t* block = step + h * S::kBlock;
 #pragma unroll
-        for (int k = 0; k < 4; ++k)
-          if (base + 2 * c + (k & 1) + 8 * (k >> 1) >= seg.len) ks[k] = kl[k] = vs[k] = vl[k] = 0.f;
-      }
-      bool raise = false;
+        for (int k = 0; k < 2; ++k) {
+          const uint2 v = *reinterpret_cast<const uint2*>(block + L::kV + ((8 * k + r) >> 1) * L::kRowV + D + (r & 1) * 8);
+          float ks = __uint_as_float(v.x << 16), kl = __uint_as_float(v.x & 0xffff0000u);
+          vs[h][k] = __uint_as_float(v.y << 16), vl[h][k] = __uint_as_float(v.y & 0xffff0000u);
+          const int at = base + h * kKv4Block + 8 * k + r;
+          if (masked && at >= seg.len) ks = kl = vs[h][k] = vl[h][k] = 0.f;  // what lies behind the sequence's end may be anything
+          vl[h][k] = fmaf(8.f, vs[h][k], vl[h][k]);
 #pragma unroll
-      for (int i = 0; i < 2; ++i) {
+          for (int t = 0; t < NR; ++t) {
 #pragma unroll
-        for (int k = 0; k < 4; ++k) {
-          float& y = x[k >> 1][2 * i + (k & 1)];
-          y = fmaf(ks[k], y, kl[k] * qsum[i]);
-          if (masked && base + 2 * c + (k & 1) + 8 * (k >> 1) > pos[i]) y = -INFINITY;
+            for (int i = 0; i < 2; ++i) {
+              float& y = x[h][t][2 * k + i];
+              y = fmaf(ks, y, kl * qsum[t][i]);
+              if (masked && at > position(row0 + 8 * t + 2 * c + i)) y = -INFINITY;
+              raise = raise || y > limit[t][i];
+            }
+          }
+          raise = raise || vs[h][k] >= vlimit;
+          big = fmaxf(big, vs[h][k]);
         }
-        const float most = fmaxf(fmaxf(x[0][2 * i], x[0][2 * i + 1]), fmaxf(x[1][2 * i], x[1][2 * i + 1]));
-        raise = raise || most > limit[i];
       }
-      const float step = fmaxf(fmaxf(vs[0], vs[1]), fmaxf(vs[2], vs[3]));
-      raise = raise || step >= vlimit;
       if (__any_sync(0xffffffffu, raise)) {
         // New maxima for the rows and for the steps of V. Infinite and NaN steps are left out: they show in the rows that see them.
-        float big = step < INFINITY ? step : 0.f;
-        big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, 1));
-        big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, 2));
+        big = big < INFINITY ? big : 0.f;
+#pragma unroll
+        for (int d = 4; d < 32; d <<= 1) big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, d));
         const int e = max(vexp, min(static_cast<int>(__float_as_uint(big) >> 23) - 127, 126));
         const float shrink = e == vexp || vscale == 0.f ? 1.f : pow2(max(vexp - e, -126));
         vexp = e;
         vscale = pow2(6 - e);
         vlimit = e >= 126 ? INFINITY : pow2(e + 1);
-        float alpha[2];
 #pragma unroll
-        for (int i = 0; i < 2; ++i) {
-          float most = fmaxf(fmaxf(x[0][2 * i], x[0][2 * i + 1]), fmaxf(x[1][2 * i], x[1][2 * i + 1]));
-          most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, 1));
-          most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, 2));
-          most = fmaxf(most, m[i]);
-          alpha[i] = m[i] == -INFINITY ? 0.f : exp2_approx((m[i] - most) * rscale[i]);
-          m[i] = most;
-          limit[i] = most == -INFINITY ? most : most + 8.f / rscale[i];
-          l[i] *= alpha[i];
-          ms[i] *= alpha[i];
-          alpha[i] *= shrink;
-        }
+        for (int t = 0; t < NR; ++t) {
+          float alpha[2];
 #pragma unroll
-        for (int i = 0; i < kTiles; ++i) {
-          o[i][0] *= alpha[0];
-          o[i][1] *= alpha[0];
-          o[i][2] *= alpha[1];
-          o[i][3] *= alpha[1];
+          for (int i = 0; i < 2; ++i) {
+            float most = fmaxf(fmaxf(x[0][t][i], x[0][t][2 + i]), fmaxf(x[1][t][i], x[1][t][2 + i]));
+#pragma unroll
+            for (int d = 4; d < 32; d <<= 1) most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, d));
+            alpha[i] = 0.f;
+            if (most != -INFINITY) {
+              const float next = limit[t][i] == -INFINITY ? most * rscale[t][i] : fmaxf(off[t][i], most * rscale[t][i]);
+              alpha[i] = limit[t][i] == -INFINITY ? 0.f : exp2_approx(off[t][i] - next);
+              off[t][i] = next;
+              limit[t][i] = (next + 8.f) / rscale[t][i];
+            } else if (limit[t][i] != -INFINITY) {
+              alpha[i] = 1.f;
+            }
+            l[t][i] *= alpha[i];
+            ms[t][i] *= alpha[i];
+            alpha[i] *= shrink;
+          }
+#pragma unroll
+          for (int i = 0; i < kTiles; ++i) {
+            o[t][i][0] *= alpha[0];
+            o[t][i][1] *= alpha[1];
+            o[t][i][2] *= alpha[0];
+            o[t][i][3] *= alpha[1];
+          }
+          eights[t][0] *= alpha[0];
+          eights[t][1] *= alpha[1];
         }
       }
-      uint32_t a[4];
 #pragma unroll
-      for (int i = 0; i < 2; ++i) {
-        const float off = m[i] == -INFINITY ? 0.f : m[i] * rscale[i];
-        float e[4];
+      for (int h = 0; h < 2; ++h) {
+        const uint8_t* block = step + h * S::kBlock;
+        uint32_t pb[NR][2];
 #pragma unroll
-        for (int k = 0; k < 4; ++k) {
-          const float y = x[k >> 1][2 * i + (k & 1)];
-          const float pk = exp2_approx(fmaf(y, rscale[i], -off));
-          l[i] += pk;
-          const bool none = masked && y == -INFINITY;  // a masked token's parameters may be anything
-          ms[i] = none ? ms[i] : fmaf(pk, vl[k], ms[i]);
-          e[k] = none ? 0.f : pk * (vs[k] * vscale);
+        for (int k = 0; k < 2; ++k) {
+          const float by = vs[h][k] * vscale;
+#pragma unroll
+          for (int t = 0; t < NR; ++t) {
+            float e[2];
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+              const float y = x[h][t][2 * k + i];
+              const float pk = exp2_approx(fmaf(y, rscale[t][i], -off[t][i]));
+              l[t][i] += pk;
+              const bool none = masked && y == -INFINITY;  // a masked token's parameters may be anything
+              ms[t][i] = none ? ms[t][i] : fmaf(pk, vl[h][k], ms[t][i]);
+              e[i] = none ? 0.f : pk * by;
+            }
+            pb[t][k] = transpose_8x8(pack2<__half>(e[0], e[1]));
+          }
         }
-        a[i] = pack2<__half>(e[0], e[1]);
-        a[2 + i] = pack2<__half>(e[2], e[3]);
-      }
-      {
-        uint32_t w0[kWordsK], w1[kWordsK];
+        uint32_t w0[kWords], w1[kWords];
         const uint8_t* at = block + L::kV + c * L::kRowV + r * (D / 8);
         if constexpr (D == 128) {
           const uint4 v0 = *reinterpret_cast<const uint4*>(at), v1 = *reinterpret_cast<const uint4*>(at + 4 * L::kRowV);
@@ -436,117 +530,137 @@ __global__ void __launch_bounds__(kKv4AttnThreads, 3) kv4_attn_kernel(const Kv4A
           w0[0] = v0.x, w0[1] = v0.y;
           w1[0] = v1.x, w1[1] = v1.y;
         }
+        const uint32_t eight[4] = {0x00080008u, 0x00080008u, 0x00080008u, 0x00080008u};
 #pragma unroll
-        for (int i = 0; i < kWordsK; ++i) {
+        for (int t = 0; t < NR; ++t) mma_16816<__half>(eights[t], eight, pb[t][0], pb[t][1]);
+#pragma unroll
+        for (int i = 0; i < kWords; ++i) {
           uint32_t u0[4], u1[4];
           split_codes(w0[i], u0);
           split_codes(w1[i], u1);
 #pragma unroll
-          for (int k = 0; k < 4; ++k) mma_16816<__half>(o[4 * i + k], a, u0[k], u1[k]);
+          for (int k = 0; k < 2; ++k) {
+            const uint32_t a[4] = {u0[2 * k], u0[2 * k + 1], u1[2 * k], u1[2 * k + 1]};
+#pragma unroll
+            for (int t = 0; t < NR; ++t) mma_16816<__half>(o[t][2 * i + k], a, pb[t][0], pb[t][1]);
+          }
         }
       }
       __syncwarp();
       ++used;
       if (RW > 1 && lane == 0) mbar_arrive(empty + stage);
-      if (producer) issue();
+      if (producer && lane == 0) issue();
+      __syncwarp();
     }
     if (!ok && lane == 0 && atomicExch(const_cast<uint32_t*>(abort_flag), 1u) == 0) atomicOr(p.status, kStatusKv4Wait);
 
-    // This warp's sums over its lanes, and the output itself: codes' part * 2^24 (2^20 for odd nibbles) / vscale + ms. A maximum of -inf with
-    // a sum that is not zero is one of NaN logits alone: it weighs NaN.
+    // This warp's sums over its lanes, and the output itself: (codes' part * 2^24 (2^20 for odd nibbles) - eights * 2^24) / vscale + ms.
+    // A maximum of -inf with a sum that is not zero is one of NaN logits alone: it weighs NaN.
     const float unit = pow2(vexp - 6);
     constexpr float kCode = 16777216.f, kHighCode = 1048576.f;
+    float mt[NR][2], lt[NR][2], weight[kTW][NR][2];
 #pragma unroll
-    for (int i = 0; i < 2; ++i) {
+    for (int t = 0; t < NR; ++t) {
 #pragma unroll
-      for (int d = 1; d < 4; d <<= 1) {
-        l[i] += __shfl_xor_sync(0xffffffffu, l[i], d);
-        ms[i] += __shfl_xor_sync(0xffffffffu, ms[i], d);
+      for (int i = 0; i < 2; ++i) {
+#pragma unroll
+        for (int d = 4; d < 32; d <<= 1) {
+          l[t][i] += __shfl_xor_sync(0xffffffffu, l[t][i], d);
+          ms[t][i] += __shfl_xor_sync(0xffffffffu, ms[t][i], d);
+        }
+        mt[t][i] = limit[t][i] == -INFINITY ? limit[t][i] : off[t][i];
+        lt[t][i] = l[t][i];
+#pragma unroll
+        for (int q = 0; q < kTiles; ++q) {
+          o[t][q][i] = fmaf(fmaf(o[t][q][i], kCode, -kCode * eights[t][i]), unit, ms[t][i]);
+          o[t][q][2 + i] = fmaf(fmaf(o[t][q][2 + i], kHighCode, -kCode * eights[t][i]), unit, ms[t][i]);
+        }
       }
-      m[i] = m[i] == -INFINITY ? m[i] : m[i] * rscale[i];  // log2
     }
-    // Values q = 16 (or 8) of group (i, k): row r + 8 i, dimensions (2 c + k) D / 8 + q.
-    float weight[kTW][2];
-    float mt[2] = {m[0], m[1]}, lt[2] = {l[0], l[1]};
     if constexpr (kTW > 1) {
-      float* mine = merge + warp * 32 * (D / 2);
+      float* mine = merge + warp * 32 * S::kRegs;
 #pragma unroll
-      for (int g = 0; g < 4; ++g) {
+      for (int t = 0; t < NR; ++t) {
 #pragma unroll
-        for (int i = 0; i < kTiles; ++i) mine[(g * kTiles + i) * 32 + lane] = fmaf(o[i][g] * (i & 1 ? kHighCode : kCode), unit, ms[g >> 1]);
-      }
-      if (c == 0) {
-        ml_smem[warp * 16 + r] = make_float2(m[0], l[0]);
-        ml_smem[warp * 16 + r + 8] = make_float2(m[1], l[1]);
+        for (int i = 0; i < 2; ++i) {
+#pragma unroll
+          for (int q = 0; q < 2 * kTiles; ++q) mine[((2 * t + i) * 2 * kTiles + q) * 32 + lane] = o[t][q >> 1][2 * (q & 1) + i];
+          if (r == 0) ml_smem[warp * kWarpRows + 8 * t + 2 * c + i] = make_float2(mt[t][i], lt[t][i]);
+        }
       }
     }
     __syncthreads();
     const bool gone = *abort_flag != 0;
     if (kTW > 1 && !gone) {
 #pragma unroll
-      for (int i = 0; i < 2; ++i) {
-        float2 v[kTW];
-        mt[i] = -INFINITY;
-        lt[i] = 0.f;
+      for (int t = 0; t < NR; ++t) {
 #pragma unroll
-        for (int k = 0; k < kTW; ++k) {
-          v[k] = ml_smem[(k * RW + rw) * 16 + r + 8 * i];
-          mt[i] = fmaxf(mt[i], v[k].x);
-        }
+        for (int i = 0; i < 2; ++i) {
+          float2 v[kTW];
+          mt[t][i] = -INFINITY;
+          lt[t][i] = 0.f;
 #pragma unroll
-        for (int k = 0; k < kTW; ++k) {
-          weight[k][i] = v[k].x == -INFINITY ? v[k].y * 0.f : exp2_approx(v[k].x - mt[i]);
-          lt[i] = fmaf(weight[k][i], v[k].y, lt[i]);
+          for (int k = 0; k < kTW; ++k) {
+            v[k] = ml_smem[(k * RW + rw) * kWarpRows + 8 * t + 2 * c + i];
+            mt[t][i] = fmaxf(mt[t][i], v[k].x);
+          }
+#pragma unroll
+          for (int k = 0; k < kTW; ++k) {
+            weight[k][t][i] = v[k].x == -INFINITY ? v[k].y * 0.f : exp2_approx(v[k].x - mt[t][i]);
+            lt[t][i] = fmaf(weight[k][t][i], v[k].y, lt[t][i]);
+          }
         }
       }
     }
-    // Whole items go out; parts go to the workspace and are counted.
-    const bool whole = seg.s1 - seg.s0 == seg.blocks;
+    // Whole items go out; parts go to the workspace and are counted. A lane has dimensions r D / 8 + q of rows 2 c + i of each tile;
+    // four at a time, dealt to the warps that share the rows.
+    const bool whole = seg.s1 - seg.s0 == seg.steps;
     const int slot = blockIdx.x * 2 + (seg.s0 > 0 ? 0 : 1);
     if (!gone) {
 #pragma unroll
-      for (int gg = 0; gg < 4 / kTW; ++gg) {
-        const int g = kTW > 1 ? tw * (4 / kTW) + gg : gg, i = g >> 1;
-        float f[kTiles];
-        if constexpr (kTW > 1) {
+      for (int t = 0; t < NR; ++t) {
 #pragma unroll
-          for (int q = 0; q < kTiles; ++q) {
-            float v = 0.f;
+        for (int i = 0; i < 2; ++i) {
+          const int in_tile = kWarpRows * rw + 8 * t + 2 * c + i, row = seg.tile * kRows + in_tile;
+          const float inv = lt[t][i] == 0.f ? 0.f : 1.f / lt[t][i];
+          const int n = static_cast<int>(magic_div(row, p.group_magic)), head = seg.head * p.group + row - n * p.group;
 #pragma unroll
-            for (int k = 0; k < kTW; ++k) {
-              const float part = merge[((k * RW + rw) * 4 + g) * kTiles * 32 + q * 32 + lane];
-              const float by = i == 0 ? weight[k][0] : weight[k][1];
-              v = by == 0.f ? v : fmaf(by, part, v);
+          for (int q4 = 0; q4 < kTiles / 2; ++q4) {
+            if (kTW > 1 && ((2 * t + i) * (kTiles / 2) + q4) % kTW != tw) continue;
+            float f[4];
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+              const int q = 4 * q4 + k;
+              if constexpr (kTW > 1) {
+                float v = 0.f;
+#pragma unroll
+                for (int j = 0; j < kTW; ++j) {
+                  const float part = merge[(j * RW + rw) * 32 * S::kRegs + ((2 * t + i) * 2 * kTiles + q) * 32 + lane];
+                  v = weight[j][t][i] == 0.f ? v : fmaf(weight[j][t][i], part, v);
+                }
+                f[k] = v;
+              } else {
+                f[k] = o[t][q >> 1][2 * (q & 1) + i];
+              }
             }
-            f[q] = v;
-          }
-        } else {
+            if (row >= p.rows) continue;
+            const int d = r * (D / 8) + 4 * q4;
+            if (whole) {
 #pragma unroll
-          for (int q = 0; q < kTiles; ++q) f[q] = fmaf(o[q][gg] * (q & 1 ? kHighCode : kCode), unit, ms[gg >> 1]);
-        }
-        const int in_tile = 16 * rw + r + 8 * i, row = seg.tile * kRows + in_tile;
-        if (row < p.rows) {
-          if (whole) {
-            const float total_l = i == 0 ? lt[0] : lt[1];
-            const float inv = total_l == 0.f ? 0.f : 1.f / total_l;
-#pragma unroll
-            for (int q = 0; q < kTiles; ++q) f[q] = total_l == 0.f ? 0.f : f[q] * inv;
-            const int n = static_cast<int>(magic_div(row, p.group_magic)), head = seg.head * p.group + row - n * p.group;
-            T* y = static_cast<T*>(p.o) + seg.b * p.os[0] + n * p.os[1] + head * p.os[2] + (2 * c + (g & 1)) * (D / 8);
-#pragma unroll
-            for (int q = 0; q < kTiles; q += 8) store8<T>(y + q, f + q);
-          } else {
-            float* y = p.partial + (static_cast<int64_t>(slot) * kRows + in_tile) * D + (2 * c + (g & 1)) * (D / 8);
-#pragma unroll
-            for (int q = 0; q < kTiles; q += 4) __stcg(reinterpret_cast<float4*>(y + q), make_float4(f[q], f[q + 1], f[q + 2], f[q + 3]));
-            if (c == 0 && (g & 1) == 0) __stcg(p.partial_ml + static_cast<int64_t>(slot) * kRows + in_tile, i == 0 ? make_float2(mt[0], lt[0]) : make_float2(mt[1], lt[1]));
+              for (int k = 0; k < 4; ++k) f[k] = lt[t][i] == 0.f ? 0.f : f[k] * inv;
+              T* y = static_cast<T*>(p.o) + seg.b * p.os[0] + n * p.os[1] + head * p.os[2] + d;
+              *reinterpret_cast<uint2*>(y) = make_uint2(pack2<T>(f[0], f[1]), pack2<T>(f[2], f[3]));
+            } else {
+              __stcg(reinterpret_cast<float4*>(p.partial + (static_cast<int64_t>(slot) * kRows + in_tile) * D + d), make_float4(f[0], f[1], f[2], f[3]));
+              if (r == 0 && q4 == 0) __stcg(p.partial_ml + static_cast<int64_t>(slot) * kRows + in_tile, make_float2(mt[t][i], lt[t][i]));
+            }
           }
         }
       }
     }
     if (!whole && !gone) {
-      const long long item_end = item_begin + seg.blocks;
-      const int first = static_cast<int>(item_begin / run), lastc = static_cast<int>((item_end - 1) / run), parts = lastc - first + 1;
+      const long long item = static_cast<long long>(run) * blockIdx.x + count - seg.left - seg.s1;  // where it begins on the line
+      const int first = static_cast<int>(item / run), parts = static_cast<int>((item + seg.steps - 1) / run) - first + 1;
       __threadfence();
       __syncthreads();
       if (threadIdx.x == 0) *last_flag = atomicAdd(p.counters + first, 1u) == static_cast<uint32_t>(parts - 1) ? 1u : 0u;
@@ -584,11 +698,10 @@ __global__ void __launch_bounds__(kKv4AttnThreads, 3) kv4_attn_kernel(const Kv4A
     }
     __syncthreads();  // merge buffer and flags
     if (gone) break;
-    item_begin += seg.blocks;
     if (!kv4_next(p, seg)) break;
   }
   // A wait that ran out leaves copies in flight: they are waited for, again with a limit, before the shared memory goes.
-  if (*abort_flag != 0 && producer) {
+  if (*abort_flag != 0 && producer && lane == 0) {
     for (; used < issued; ++used) mbar_wait(full + used % kKv4Stages, (used / kKv4Stages) & 1, abort_flag + 2);
   }
 }
