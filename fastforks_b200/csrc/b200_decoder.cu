@@ -332,9 +332,9 @@ int b200_kv4_attention(const B200Kv4AttnArgs* a, void* stream_ptr) {
   p.table_pages = a->table_pages;
   p.status = dev->status;
   // The lengths are on the device: the grid is for the longest that the page table allows, CTAs without a run leave at once.
-  p.min_run = 4;
-  const int64_t most = static_cast<int64_t>(a->batch) * p.row_tiles * a->kv_heads * ((static_cast<int64_t>(a->table_pages) * a->page + kKv4Step - 1) / kKv4Step);
-  if (most >= (int64_t(1) << 38)) return fail(B200_ATTN_UNSUPPORTED, "kv4_attention: %lld steps of 32 tokens, at most 2^38 a call", static_cast<long long>(most));
+  p.min_run = 4 + kKv4Item;
+  const int64_t most = static_cast<int64_t>(a->batch) * p.row_tiles * a->kv_heads * ((static_cast<int64_t>(a->table_pages) * a->page + kKv4Step - 1) / kKv4Step + kKv4Item);
+  if (most >= (int64_t(1) << 38)) return fail(B200_ATTN_UNSUPPORTED, "kv4_attention: %lld steps of 32 tokens and items, at most 2^38 a call", static_cast<long long>(most));
   const int64_t ctas = std::min<int64_t>(static_cast<int64_t>(dev->sms) * form.ctas_per_sm, (most + p.min_run - 1) / p.min_run);
   const int64_t partial = ctas * 2 * form.rows * a->head_dim * 4, ml = ctas * 2 * form.rows * 8;
   if (a->workspace == nullptr || !aligned16(a->workspace) || a->workspace_bytes < partial + ml || a->counters == nullptr || a->counter_words < ctas)

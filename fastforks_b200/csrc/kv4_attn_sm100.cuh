@@ -48,6 +48,8 @@ struct Kv4AttnParams {
 };
 
 constexpr int kKv4AttnThreads = 128, kKv4Stages = 2, kKv4Step = 2 * kKv4Block;
+// What an item costs beside its steps (queries, joining the warps, output), in steps: units of the line in front of its first step.
+constexpr int kKv4Item = 4;
 constexpr uint32_t kStatusKv4Wait = 1u << 22;
 
 // NR: tiles of eight rows of a warp. RW: warps with rows of their own, the other 4 / RW share theirs.
@@ -64,7 +66,7 @@ struct Kv4AttnSmem {
   static constexpr int kMl = kQ + (kQInSmem ? RW * 32 * NR * D / 8 * 4 : 0);  // [4][8 NR] float2
   static constexpr int kBars = kMl + 4 * 8 * NR * 8;                        // full, empty
   static constexpr int kAhead = kBars + 2 * kTW * kKv4Stages * 8;           // [kTW] Kv4Ahead
-  static constexpr int kFlags = kAhead + kTW * 48;
+  static constexpr int kFlags = kAhead + kTW * 64;
   static constexpr int kBytes = kFlags + 16;
   static constexpr int kCtasPerSm = NR == 1 ? 4 : 3;
 };
@@ -103,28 +105,31 @@ struct Kv4Segment {
   int b, tile, head;  // head runs fastest
   int len, steps;     // of sequence b
   int s0, s1;
-  int left;           // steps of the run behind this segment
+  int left;           // units of the run behind this segment
 };
 
 // The producer's place of a token warp, in shared memory: the segment it is in, its next step there and the end of those that are seen.
 struct Kv4Ahead {
   Kv4Segment seg;
-  int s, end, more, pad;
+  int s, end, more;
+  int at, in;  // the step that is issued next (-1: none) and its first block's place in its page
+  int pad[3];
 };
-static_assert(sizeof(Kv4Ahead) == 48, "Kv4AttnSmem::kFlags");
+static_assert(sizeof(Kv4Ahead) == 64, "Kv4AttnSmem::kFlags");
 
 __device__ __forceinline__ int kv4_length(const Kv4AttnParams& p, int b) {
   const int n = p.lengths[b], most = p.table_pages * p.page_blocks * kKv4Block;
   return n < 0 ? 0 : n > most ? most : n;
 }
 
+// The next segment of the run, if there is one.
 __device__ __forceinline__ bool kv4_next(const Kv4AttnParams& p, Kv4Segment& s) {
-  if (s.left <= 0) return false;
+  if (s.left <= kKv4Item) return false;
   if (++s.head == p.kv_heads) {
     s.head = 0;
     if (++s.tile == p.row_tiles) {
       s.tile = 0;
-      do {  // steps are left on the line, so a sequence with some follows
+      do {  // units are left on the line, so a sequence with some follows
         if (++s.b >= p.batch) return false;
         s.len = kv4_length(p, s.b);
       } while (s.len == 0);
@@ -132,8 +137,8 @@ __device__ __forceinline__ bool kv4_next(const Kv4AttnParams& p, Kv4Segment& s) 
     }
   }
   s.s0 = 0;
-  s.s1 = min(s.steps, s.left);
-  s.left -= s.s1;
+  s.s1 = min(s.steps, s.left - kKv4Item);
+  s.left -= s.s1 + kKv4Item;
   return true;
 }
 
@@ -172,7 +177,7 @@ __global__ void __launch_bounds__(kKv4AttnThreads, Kv4AttnSmem<D, NR, RW>::kCtas
   grid_dependency_wait();
   grid_launch_dependents();
 
-  // The line: steps of all items, and this CTA's run of it.
+  // The line: units of all items, and this CTA's run of it.
   const int per = p.kv_heads * p.row_tiles;
   long long total = 0;
   {
@@ -180,7 +185,7 @@ __global__ void __launch_bounds__(kKv4AttnThreads, Kv4AttnSmem<D, NR, RW>::kCtas
     for (int b = lane; b < p.batch; b += 32) {
       const int n = p.lengths[b], len = kv4_length(p, b);
       if (n != len && n > 0 && threadIdx.x < 32 && blockIdx.x == 0) atomicOr(p.status, kStatusPage);
-      mine += (len + kKv4Step - 1) / kKv4Step;
+      mine += len == 0 ? 0 : (len + kKv4Step - 1) / kKv4Step + kKv4Item;
     }
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) mine += __shfl_xor_sync(0xffffffffu, mine, o);
@@ -208,8 +213,8 @@ __global__ void __launch_bounds__(kKv4AttnThreads, Kv4AttnSmem<D, NR, RW>::kCtas
     int b0 = 0;
     for (;; b0 += 32) {
       const int b = b0 + lane;
-      const int steps = b < p.batch ? (kv4_length(p, b) + kKv4Step - 1) / kKv4Step : 0;
-      long long sum = static_cast<long long>(steps) * per;
+      const int len = b < p.batch ? kv4_length(p, b) : 0, units = len == 0 ? 0 : (len + kKv4Step - 1) / kKv4Step + kKv4Item;
+      long long sum = static_cast<long long>(units) * per;
 #pragma unroll
       for (int o = 1; o < 32; o <<= 1) {
         const long long v = __shfl_up_sync(0xffffffffu, sum, o);
@@ -219,8 +224,8 @@ __global__ void __launch_bounds__(kKv4AttnThreads, Kv4AttnSmem<D, NR, RW>::kCtas
       if (hit != 0) {  // always, at the latest with the last sequence: begin < total
         const int l = __ffs(hit) - 1;
         seg.b = b0 + l;
-        seg.steps = __shfl_sync(0xffffffffu, steps, l);
-        before += __shfl_sync(0xffffffffu, sum, l) - static_cast<long long>(seg.steps) * per;
+        seg.steps = __shfl_sync(0xffffffffu, units, l) - kKv4Item;
+        before += __shfl_sync(0xffffffffu, sum, l) - static_cast<long long>(seg.steps + kKv4Item) * per;
         break;
       }
       before += __shfl_sync(0xffffffffu, sum, 31);
@@ -228,12 +233,13 @@ __global__ void __launch_bounds__(kKv4AttnThreads, Kv4AttnSmem<D, NR, RW>::kCtas
     }
     seg.len = kv4_length(p, seg.b);
     const long long in = begin - before;
-    const int item = static_cast<int>(in / seg.steps);
-    seg.s0 = static_cast<int>(in - static_cast<long long>(item) * seg.steps);
+    const int item = static_cast<int>(in / (seg.steps + kKv4Item)), at = static_cast<int>(in - static_cast<long long>(item) * (seg.steps + kKv4Item));
     seg.tile = item / p.kv_heads;
     seg.head = item - seg.tile * p.kv_heads;
-    seg.s1 = min(seg.steps, seg.s0 + count);
-    seg.left = count - (seg.s1 - seg.s0);
+    seg.s0 = max(0, at - kKv4Item);
+    seg.s1 = max(seg.s0, min(seg.steps, at - kKv4Item + count));
+    seg.left = count - (seg.s1 + kKv4Item - at);
+    if (seg.s1 == seg.s0) return;  // the run ends in front of the item's first step
   }
 
   // The producer runs kKv4Stages steps ahead, over the ends of items: lane 0 of the first row warp of each token warp.
@@ -241,58 +247,64 @@ __global__ void __launch_bounds__(kKv4AttnThreads, Kv4AttnSmem<D, NR, RW>::kCtas
   Kv4Ahead& ahead = *reinterpret_cast<Kv4Ahead*>(smem + S::kAhead + tw * sizeof(Kv4Ahead));
   uint32_t issued = 0, used = 0;  // steps of this token warp, in order
   bool ok = true;
-  const auto issue = [&]() {
+  const bool joined = (p.page_blocks & 1) == 0;  // the blocks of a step follow one another
+  int next_page[2] = {0, 0};
+  const auto fetch = [&]() {  // the next step and the pages of its blocks, so that their load is over when the step is issued
     int at = ahead.s, end = ahead.end;
+    ahead.at = -1;
     if (at >= end) {
       if (ahead.more == 0) return;
       Kv4Segment next = ahead.seg;
-      bool more = true;
       do {
-        more = kv4_next(p, next);
-        if (!more) break;
+        if (!kv4_next(p, next)) {
+          ahead.more = 0;
+          return;
+        }
         at = next.s0 + tw;
         end = kv4_seen<kRows>(p, next);
       } while (at >= end);
       ahead.seg = next;
       ahead.end = end;
-      ahead.more = more ? 1 : 0;
-      if (!more) {
-        ahead.s = end;
-        return;
-      }
     }
+    ahead.s = at + kTW;
+    ahead.at = at;
+    const int32_t* pages = p.page_table + ahead.seg.b * p.table_stride;
+    const uint32_t col = magic_div(2 * at, p.bpp_magic);
+    ahead.in = 2 * at - static_cast<int>(col) * p.page_blocks;
+    next_page[0] = pages[col];
+    if (!joined && at * kKv4Step + kKv4Block < ahead.seg.len) next_page[1] = pages[magic_div(2 * at + 1, p.bpp_magic)];
+  };
+  const auto issue = [&]() {
+    const int at = ahead.at, in = ahead.in;
+    if (at < 0) return;
     const uint32_t stage = issued % kKv4Stages, round = issued / kKv4Stages;
     if (RW > 1 && round > 0 && !mbar_wait(empty + stage, (round - 1) & 1, abort_flag)) {
-      ahead.more = 0;
-      ahead.s = end;
+      ahead.at = -1;
       ok = false;
       return;
     }
-    const int b = ahead.seg.b, head = ahead.seg.head;
-    const auto block_at = [&](int block) {
-      const uint32_t col = magic_div(block, p.bpp_magic);
-      int page = p.page_table[b * p.table_stride + col];
+    const int head = ahead.seg.head;
+    const auto block_at = [&](int page, int place) {
       if (page < 0 || page >= p.pages) {
         atomicOr(p.status, kStatusPage);
         page = 0;
       }
-      return p.cache + ((static_cast<int64_t>(page) * p.kv_heads + head) * p.page_blocks + (block - static_cast<int>(col) * p.page_blocks)) * S::kBlock;
+      return p.cache + ((static_cast<int64_t>(page) * p.kv_heads + head) * p.page_blocks + place) * S::kBlock;
     };
     const bool two = at * kKv4Step + kKv4Block < ahead.seg.len;  // the second block may hold nothing: what lies there is then masked
-    const bool joined = (p.page_blocks & 1) == 0;                // the blocks of a step follow one another
     uint8_t* to = ring + stage * 2 * S::kBlock;
-    const uint8_t* from = block_at(2 * at);
     mbar_arrive_expect_tx(full + stage, two ? 2 * S::kBlock : S::kBlock);
-    bulk_load(to, from, two && joined ? 2 * S::kBlock : S::kBlock, full + stage);
-    if (two && !joined) bulk_load(to + S::kBlock, block_at(2 * at + 1), S::kBlock, full + stage);
+    bulk_load(to, block_at(next_page[0], in), two && joined ? 2 * S::kBlock : S::kBlock, full + stage);
+    if (two && !joined) bulk_load(to + S::kBlock, block_at(next_page[1], in + 1 == p.page_blocks ? 0 : in + 1), S::kBlock, full + stage);
     ++issued;
-    ahead.s = at + kTW;
+    fetch();
   };
   if (producer && lane == 0) {
     ahead.seg = seg;
     ahead.s = seg.s0 + tw;
     ahead.end = kv4_seen<kRows>(p, seg);
     ahead.more = 1;
+    fetch();
     for (int i = 0; i < kKv4Stages; ++i) issue();
   }
   __syncwarp();
@@ -375,16 +387,12 @@ __global__ void __launch_bounds__(kKv4AttnThreads, Kv4AttnSmem<D, NR, RW>::kCtas
 #pragma unroll 1
     for (int s = seg.s0 + tw; s < seen; s += kTW) {
       const uint32_t stage = used % kKv4Stages, round = used / kKv4Stages;
-      ok = ok && mbar_wait(full + stage, round & 1, abort_flag);
-      ok = __all_sync(0xffffffffu, ok);
-      if (!ok) break;
+      ok = ok && mbar_wait(full + stage, round & 1, abort_flag);  // one that ran out is noticed at the vote below
       const uint8_t* step = ring + stage * 2 * S::kBlock;
       const int base = s * kKv4Step;
       const bool masked = base + kKv4Step - 1 > lowest;
       float x[2][NR][4];  // blocks; tokens r and r + 8, rows 2 c and 2 c + 1
       float vs[2][2], vl[2][2];
-      bool raise = false;
-      float big = 0.f;  // largest step of V
       {
         uint32_t w[2][2][kWords];
 #pragma unroll
@@ -436,28 +444,58 @@ __global__ void __launch_bounds__(kKv4AttnThreads, Kv4AttnSmem<D, NR, RW>::kCtas
 #pragma unroll
         for (int k = 0; k < 2; ++k) {
           const uint2 v = *reinterpret_cast<const uint2*>(block + L::kV + ((8 * k + r) >> 1) * L::kRowV + D + (r & 1) * 8);
-          float ks = __uint_as_float(v.x << 16), kl = __uint_as_float(v.x & 0xffff0000u);
-          vs[h][k] = __uint_as_float(v.y << 16), vl[h][k] = __uint_as_float(v.y & 0xffff0000u);
-          const int at = base + h * kKv4Block + 8 * k + r;
-          if (masked && at >= seg.len) ks = kl = vs[h][k] = vl[h][k] = 0.f;  // what lies behind the sequence's end may be anything
-          vl[h][k] = fmaf(8.f, vs[h][k], vl[h][k]);
+          const float ks = __uint_as_float(v.x << 16), kl = __uint_as_float(v.x & 0xffff0000u);
+          vs[h][k] = __uint_as_float(v.y << 16);
+          vl[h][k] = fmaf(8.f, vs[h][k], __uint_as_float(v.y & 0xffff0000u));
 #pragma unroll
           for (int t = 0; t < NR; ++t) {
 #pragma unroll
-            for (int i = 0; i < 2; ++i) {
-              float& y = x[h][t][2 * k + i];
-              y = fmaf(ks, y, kl * qsum[t][i]);
-              if (masked && at > position(row0 + 8 * t + 2 * c + i)) y = -INFINITY;
-              raise = raise || y > limit[t][i];
-            }
+            for (int i = 0; i < 2; ++i) x[h][t][2 * k + i] = fmaf(ks, x[h][t][2 * k + i], kl * qsum[t][i]);
           }
+        }
+      }
+      if (masked) {
+        // Tokens that a row does not see weigh nothing, whatever they hold; those behind the sequence's end hold whatever the page held.
+        // A value that is not finite is put into the logits of the rows that see it, so that it cannot reach the others through 0 * NaN.
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+#pragma unroll
+          for (int k = 0; k < 2; ++k) {
+            const int at = base + h * kKv4Block + 8 * k + r;
+            const bool spoilt = !(fabsf(vl[h][k]) < INFINITY);
+#pragma unroll
+            for (int t = 0; t < NR; ++t) {
+#pragma unroll
+              for (int i = 0; i < 2; ++i) {
+                float& y = x[h][t][2 * k + i];
+                if (spoilt) y = NAN;
+                if (at > position(row0 + 8 * t + 2 * c + i)) y = -INFINITY;
+              }
+            }
+            if (spoilt || at >= seg.len) vs[h][k] = vl[h][k] = 0.f;
+          }
+        }
+      }
+      bool raise = !ok;
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+#pragma unroll
+        for (int k = 0; k < 2; ++k) {
           raise = raise || vs[h][k] >= vlimit;
-          big = fmaxf(big, vs[h][k]);
+#pragma unroll
+          for (int t = 0; t < NR; ++t) raise = raise || x[h][t][2 * k] > limit[t][0] || x[h][t][2 * k + 1] > limit[t][1];
         }
       }
       if (__any_sync(0xffffffffu, raise)) {
+        ok = __all_sync(0xffffffffu, ok);
+        if (!ok) break;
         // New maxima for the rows and for the steps of V. Infinite and NaN steps are left out: they show in the rows that see them.
-        big = big < INFINITY ? big : 0.f;
+        float big = 0.f;
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+#pragma unroll
+          for (int k = 0; k < 2; ++k) big = fmaxf(big, vs[h][k] < INFINITY ? vs[h][k] : 0.f);
+        }
 #pragma unroll
         for (int d = 4; d < 32; d <<= 1) big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, d));
         const int e = max(vexp, min(static_cast<int>(__float_as_uint(big) >> 23) - 127, 126));
@@ -512,9 +550,8 @@ __global__ void __launch_bounds__(kKv4AttnThreads, Kv4AttnSmem<D, NR, RW>::kCtas
               const float y = x[h][t][2 * k + i];
               const float pk = exp2_approx(fmaf(y, rscale[t][i], -off[t][i]));
               l[t][i] += pk;
-              const bool none = masked && y == -INFINITY;  // a masked token's parameters may be anything
-              ms[t][i] = none ? ms[t][i] : fmaf(pk, vl[h][k], ms[t][i]);
-              e[i] = none ? 0.f : pk * by;
+              ms[t][i] = fmaf(pk, vl[h][k], ms[t][i]);
+              e[i] = pk * by;
             }
             pb[t][k] = transpose_8x8(pack2<__half>(e[0], e[1]));
           }
@@ -659,7 +696,7 @@ __global__ void __launch_bounds__(kKv4AttnThreads, Kv4AttnSmem<D, NR, RW>::kCtas
       }
     }
     if (!whole && !gone) {
-      const long long item = static_cast<long long>(run) * blockIdx.x + count - seg.left - seg.s1;  // where it begins on the line
+      const long long item = static_cast<long long>(run) * blockIdx.x + count - seg.left - seg.s1;  // where its steps begin on the line
       const int first = static_cast<int>(item / run), parts = static_cast<int>((item + seg.steps - 1) / run) - first + 1;
       __threadfence();
       __syncthreads();
