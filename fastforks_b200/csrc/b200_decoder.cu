@@ -15,7 +15,7 @@ namespace b200 {
 
 namespace {
 
-constexpr int kMaxDim = 512, kRotaryCtasPerSm = 4, kKv4CtasPerSm = 4, kKv4MaxRows = 64;
+constexpr int kMaxDim = 512, kRotaryCtasPerSm = 2, kKv4CtasPerSm = 4, kKv4MaxRows = 64;
 constexpr int kCounterBytes = 256;
 
 // Whether every row of a tensor of heads starts on 16 bytes.
@@ -23,23 +23,40 @@ bool rows_aligned(const void* p, const int64_t s[3], int batch, int tokens, int 
   return aligned16(p) && (batch == 1 || s[0] * size % 16 == 0) && (tokens == 1 || s[1] * size % 16 == 0) && (heads == 1 || s[2] * size % 16 == 0);
 }
 
-int lanes_of(int dim) {
-  int lanes = 1;
-  while (16 * lanes < dim) lanes *= 2;
-  return lanes;
+int lanes_log2_of(int dim) {
+  int n = 0;
+  while (16 << n < dim) ++n;
+  return n;
 }
 
+struct RotaryForm {
+  const void* kernel;
+  int smem, ctas_per_sm;
+};
+template <typename T, int MODE>
+RotaryForm rotary_form(int form) {
+  using S = RotaryStream<T, MODE>;
+  if (form == kRowHalves) return {reinterpret_cast<const void*>(rotary_stream_kernel<T, kRowHalves, MODE>), S::kBytes, S::kCtasPerSm};
+  if (form == kRowPairs) return {reinterpret_cast<const void*>(rotary_stream_kernel<T, kRowPairs, MODE>), S::kBytes, S::kCtasPerSm};
+  return {reinterpret_cast<const void*>(rotary_any_kernel<T, MODE>), 0, 2};
+}
 template <typename T>
-const void* rotary_kernel_of(int form, bool norm, bool backward) {
-  if (norm && backward) {
-    const void* k[3] = {reinterpret_cast<const void*>(norm_rotary_backward_kernel<T, kRowHalves>), reinterpret_cast<const void*>(norm_rotary_backward_kernel<T, kRowPairs>),
-                        reinterpret_cast<const void*>(norm_rotary_backward_kernel<T, kRowAny>)};
-    return k[form];
-  }
-  const void* k[2][3] = {
-      {reinterpret_cast<const void*>(rotary_kernel<T, kRowHalves, false>), reinterpret_cast<const void*>(rotary_kernel<T, kRowPairs, false>), reinterpret_cast<const void*>(rotary_kernel<T, kRowAny, false>)},
-      {reinterpret_cast<const void*>(rotary_kernel<T, kRowHalves, true>), reinterpret_cast<const void*>(rotary_kernel<T, kRowPairs, true>), reinterpret_cast<const void*>(rotary_kernel<T, kRowAny, true>)}};
-  return k[norm ? 1 : 0][form];
+RotaryForm rotary_form_of(int form, int mode) {
+  return mode == kTurn ? rotary_form<T, kTurn>(form) : mode == kNormTurn ? rotary_form<T, kNormTurn>(form) : rotary_form<T, kNormBack>(form);
+}
+std::atomic<bool> g_rotary_opted_in[kMaxDevices][3][3][3];
+
+// The shared-memory opt-in of a kernel on this device, once.
+int opt_in(std::atomic<bool>& done, const void* kernel, int smem, const char* what) {
+  if (done.load(std::memory_order_acquire)) return B200_ATTN_OK;
+  const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+  if (e != cudaSuccess) return cuda_fail(e, what);
+  done.store(true, std::memory_order_release);
+  return B200_ATTN_OK;
+}
+int current_device(int* device) {
+  const cudaError_t e = cudaGetDevice(device);
+  return e == cudaSuccess ? B200_ATTN_OK : cuda_fail(e, "cudaGetDevice");
 }
 
 int check_table(const char* what, const float* cs, int rot, int dim, int table_rows) {
@@ -141,6 +158,7 @@ int b200_rotary(const B200RotaryArgs* a, void* stream_ptr) {
   RotaryParams p{};
   bool vec = true, sums = false;
   int64_t rows = 0;
+  int heads = 0;
   for (int k = 0; k < a->tensors; ++k) {
     const B200Heads& h = a->heads[k];
     if (h.heads < 1) return fail(B200_ATTN_BAD_CONFIG, "rotary: tensor %d has %d heads", k, h.heads);
@@ -162,9 +180,7 @@ int b200_rotary(const B200RotaryArgs* a, void* stream_ptr) {
     const int64_t r = static_cast<int64_t>(a->batch) * a->tokens * h.heads;
     rows += r;
     if (int rc = check_rows("rotary", rows)) return rc;
-    p.t_rows[k] = static_cast<uint32_t>(r);
-    p.t_magic[k] = div_magic(h.heads);
-    p.heads += h.heads;
+    heads += h.heads;
   }
   DeviceState* dev = nullptr;
   if (int rc = device_state(&dev)) return rc;
@@ -172,14 +188,15 @@ int b200_rotary(const B200RotaryArgs* a, void* stream_ptr) {
   p.positions = a->positions;
   p.ps[0] = a->pos_stride[0];
   p.ps[1] = a->pos_stride[1];
-  p.heads_magic = div_magic(p.heads);
   p.tokens_magic = div_magic(a->tokens);
-  p.rows = static_cast<uint32_t>(rows);
+  p.all_tokens = static_cast<uint32_t>(a->batch) * static_cast<uint32_t>(a->tokens);
+  p.tensors = a->tensors;
   p.table_rows = a->table_rows;
   p.tokens = a->tokens;
   p.dim = a->head_dim;
   p.rot = a->rot;
-  p.lanes = lanes_of(a->head_dim);
+  p.lanes_log2 = lanes_log2_of(a->head_dim);
+  p.inv_dim = 1.f / static_cast<float>(a->head_dim);
   p.interleaved = a->interleaved != 0;
   p.w_f32 = a->weight_dtype == B200_ATTN_F32;
   p.vec = vec;
@@ -187,17 +204,30 @@ int b200_rotary(const B200RotaryArgs* a, void* stream_ptr) {
   p.sign = a->backward ? -1.f : 1.f;
   p.status = dev->status;
   // Rows whose rotation and length come in whole lanes, on 16 bytes, keep partners in one lane; the others look theirs up in shared memory.
-  const int form = vec && a->head_dim % 16 == 0 && a->rot % 16 == 0 ? (p.interleaved || a->rot == 0 ? kRowPairs : kRowHalves) : kRowAny;
-  const bool norm_back = a->norm && a->backward;
-  const void* kernel = a->dtype == B200_ATTN_F16    ? rotary_kernel_of<__half>(form, a->norm, a->backward)
-                       : a->dtype == B200_ATTN_BF16 ? rotary_kernel_of<__nv_bfloat16>(form, a->norm, a->backward)
-                                                    : rotary_kernel_of<float>(form, a->norm, a->backward);
-  const int groups = kRotaryThreads / p.lanes;
-  int64_t ctas = (rows + groups - 1) / groups;
-  size_t smem = form == kRowAny ? static_cast<size_t>(groups) * p.dim * 4 : 0;
-  if (norm_back) {
-    ctas = std::min<int64_t>(ctas, static_cast<int64_t>(dev->sms) * kRotaryCtasPerSm);
-    smem = std::max(smem, static_cast<size_t>(kRotaryThreads / 32) * p.dim * 4);
+  const bool pairs = p.interleaved || a->rot == 0;
+  const int form = vec && a->head_dim % 16 == 0 && a->rot % (pairs ? 8 : 16) == 0 ? (pairs ? kRowPairs : kRowHalves) : kRowAny;
+  const int mode = !a->norm ? kTurn : a->backward ? kNormBack : kNormTurn;
+  const RotaryForm kernel = a->dtype == B200_ATTN_F16 ? rotary_form_of<__half>(form, mode) : a->dtype == B200_ATTN_BF16 ? rotary_form_of<__nv_bfloat16>(form, mode) : rotary_form_of<float>(form, mode);
+  // A token's rows go to as many groups of lanes as leave each of them four rows or more; calls of few tokens use more groups than that.
+  const int groups = kRotaryThreads >> p.lanes_log2;
+  int64_t chunks = 0;
+  for (int k = 0; k < a->tensors; ++k) {
+    const int heads = a->heads[k].heads;
+    int g = 0;
+    while (2 << g <= std::min(groups, heads / 4)) ++g;
+    const auto count = [&] { return (static_cast<int64_t>(p.all_tokens) * (1 << g) + groups - 1) / groups; };
+    while (2 << g <= groups && 1 << g < heads && count() < dev->sms) ++g;
+    p.steps_log2[k] = g;
+    p.chunks[k] = static_cast<int>(count());
+    chunks = std::max(chunks, count());
+  }
+  // Every CTA gets the same number of chunks, give or take one.
+  const int64_t waves = (chunks + static_cast<int64_t>(dev->sms) * kernel.ctas_per_sm - 1) / (static_cast<int64_t>(dev->sms) * kernel.ctas_per_sm);
+  const int64_t ctas = (chunks + waves - 1) / waves;
+  int smem = kernel.smem;
+  if (form == kRowAny) smem = groups * p.dim * 4;
+  if (mode == kNormBack) {
+    smem = std::max(smem, kRotaryThreads / 32 * p.dim * 4);
     if (sums) {
       if (a->workspace == nullptr || !aligned16(a->workspace) || a->workspace_bytes < kCounterBytes + 2 * ctas * p.dim * 4)
         return fail(B200_ATTN_BAD_CONFIG, "rotary: the gradient of the weights needs a workspace (b200_rotary_workspace)");
@@ -205,8 +235,13 @@ int b200_rotary(const B200RotaryArgs* a, void* stream_ptr) {
       p.partial = reinterpret_cast<float*>(static_cast<char*>(a->workspace) + kCounterBytes);
     }
   }
+  if (form != kRowAny) {
+    int device = 0;
+    if (int rc = current_device(&device)) return rc;
+    if (int rc = opt_in(g_rotary_opted_in[device][a->dtype][form][mode], kernel.kernel, kernel.smem, "rotary: shared memory opt-in")) return rc;
+  }
   void* args[] = {&p};
-  if (int rc = launch_kernel(kernel, static_cast<unsigned>(ctas), 1, kRotaryThreads, smem, 1, static_cast<cudaStream_t>(stream_ptr), args, "rotary kernel launch")) return rc;
+  if (int rc = launch_kernel(kernel.kernel, static_cast<unsigned>(ctas), 1, kRotaryThreads, smem, 1, static_cast<cudaStream_t>(stream_ptr), args, "rotary kernel launch")) return rc;
   clear_error();
   return B200_ATTN_OK;
 }
@@ -243,7 +278,8 @@ int b200_kv4_append(const B200Kv4Args* a, void* stream_ptr) {
   p.v = a->v;
   p.q_out = a->q_out;
   for (int i = 0; i < 3; ++i) p.qs[i] = a->q_stride[i], p.ks[i] = a->k_stride[i], p.vs[i] = a->v_stride[i], p.qos[i] = a->q_out_stride[i];
-  const int form = a->rot % 16 == 0 ? (p.interleaved || a->rot == 0 ? kRowPairs : kRowHalves) : kRowAny;
+  const bool pairs = p.interleaved || a->rot == 0;
+  const int form = a->rot % (pairs ? 8 : 16) == 0 ? (pairs ? kRowPairs : kRowHalves) : kRowAny;
   const bool f16 = a->dtype == B200_ATTN_F16;
   const void* kernel = a->head_dim == 64 ? (f16 ? append_kernel_of<__half, 64>(form) : append_kernel_of<__nv_bfloat16, 64>(form))
                                          : (f16 ? append_kernel_of<__half, 128>(form) : append_kernel_of<__nv_bfloat16, 128>(form));
@@ -343,14 +379,8 @@ int b200_kv4_attention(const B200Kv4AttnArgs* a, void* stream_ptr) {
   p.partial_ml = reinterpret_cast<float2*>(static_cast<char*>(a->workspace) + partial);
   p.counters = a->counters;
   int device = 0;
-  cudaError_t e = cudaGetDevice(&device);
-  if (e != cudaSuccess) return cuda_fail(e, "cudaGetDevice");
-  std::atomic<bool>& opted_in = g_attn_opted_in[device][f16 ? 0 : 1][a->head_dim == 64 ? 0 : 1][which];
-  if (!opted_in.load(std::memory_order_acquire)) {
-    e = cudaFuncSetAttribute(form.kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, form.smem);
-    if (e != cudaSuccess) return cuda_fail(e, "kv4_attention: shared memory opt-in");
-    opted_in.store(true, std::memory_order_release);
-  }
+  if (int rc = current_device(&device)) return rc;
+  if (int rc = opt_in(g_attn_opted_in[device][f16 ? 0 : 1][a->head_dim == 64 ? 0 : 1][which], form.kernel, form.smem, "kv4_attention: shared memory opt-in")) return rc;
   void* args[] = {&p};
   if (int rc = launch_kernel(form.kernel, static_cast<unsigned>(ctas), 1, kKv4AttnThreads, form.smem, 1, static_cast<cudaStream_t>(stream_ptr), args, "kv4_attention kernel launch")) return rc;
   clear_error();

@@ -8,7 +8,10 @@
 #include <ATen/core/grad_mode.h>
 #include <ATen/cuda/EmptyTensor.h>
 #include <c10/cuda/CUDAFunctions.h>
+#include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
+#include <torch/csrc/autograd/custom_function.h>
+#include <torch/csrc/autograd/functions/basic_ops.h>
 #include <torch/csrc/autograd/python_variable.h>
 
 #include <cmath>
@@ -327,10 +330,16 @@ bool fits32(const at::Tensor& t) {
     if (n > INT32_MAX) return false;
   return true;
 }
-// A plain, filled tensor of heads with unit last stride.
-bool heads_of(const at::Tensor* t, c10::DeviceIndex device) {
-  return t != nullptr && plain(*t, device) && t->dim() == 4 && t->stride(3) == 1 && t->numel() > 0 && fits32(*t);
+// A plain CUDA tensor on `device` as above, which may need a gradient.
+bool on_device(const at::Tensor& t, c10::DeviceIndex device) {
+  return t.is_cuda() && t.layout() == at::kStrided && t.device().index() == device && !t.is_conj() && !t.is_neg() && t.has_storage();
 }
+bool wants_grad(const at::Tensor& t) { return t.requires_grad() && at::GradMode::is_enabled(); }
+// A plain, filled tensor of heads with unit last stride.
+bool heads_on(const at::Tensor* t, c10::DeviceIndex device) {
+  return t != nullptr && on_device(*t, device) && t->dim() == 4 && t->stride(3) == 1 && t->numel() > 0 && fits32(*t);
+}
+bool heads_of(const at::Tensor* t, c10::DeviceIndex device) { return heads_on(t, device) && plain(*t, device); }
 void set_heads(int64_t* s, const at::Tensor& t) {
   for (int i = 0; i < 3; ++i) s[i] = t.stride(i);
 }
@@ -339,60 +348,193 @@ bool table_of(const at::Tensor* t, c10::DeviceIndex device, int64_t dim) {
          t->is_contiguous() && fits32(*t);
 }
 
-// Table and positions of `a` for the tokens of x.
-bool set_turn(B200RotaryArgs* a, const at::Tensor& x, PyObject* table, PyObject* positions, c10::DeviceIndex device) {
+// Table and positions (undefined: none) as they go with the tokens of x.
+bool turn_of(const at::Tensor& x, PyObject* table, PyObject* positions, c10::DeviceIndex device, at::Tensor* t, at::Tensor* p) {
   if (table == Py_None) return positions == Py_None;
-  const at::Tensor* t = tensor_of(table);
-  if (!table_of(t, device, x.size(3))) return false;
-  a->cs = static_cast<const float*>(t->data_ptr());
-  a->rot = static_cast<int32_t>(2 * t->size(2));
-  a->table_rows = static_cast<int32_t>(t->size(0));
+  const at::Tensor* given = tensor_of(table);
+  if (!table_of(given, device, x.size(3))) return false;
+  *t = *given;
   if (positions == Py_None) return t->size(0) >= x.size(1);
-  const at::Tensor* p = tensor_of(positions);
-  if (p == nullptr || !plain(*p, device) || p->scalar_type() != at::kInt) return false;
-  if (p->dim() == 1 && p->size(0) == x.size(1)) {
-    a->pos_stride[1] = p->stride(0);
-  } else if (p->dim() == 2 && p->size(0) == x.size(0) && p->size(1) == x.size(1)) {
-    a->pos_stride[0] = p->stride(0);
-    a->pos_stride[1] = p->stride(1);
-  } else {
-    return false;
-  }
-  a->positions = static_cast<const int32_t*>(p->data_ptr());
-  return true;
+  given = tensor_of(positions);
+  if (given == nullptr || !plain(*given, device) || given->scalar_type() != at::kInt) return false;
+  *p = *given;
+  return (p->dim() == 1 && p->size(0) == x.size(1)) || (p->dim() == 2 && p->size(0) == x.size(0) && p->size(1) == x.size(1));
 }
 
-void set_rotary(B200RotaryArgs* a, const at::Tensor& x, PyObject* interleaved) {
+void set_rotary(B200RotaryArgs* a, const at::Tensor& x, const at::Tensor& table, const at::Tensor& positions, bool interleaved) {
+  std::memset(a, 0, sizeof(*a));
   a->struct_size = sizeof(*a);
   a->dtype = a->weight_dtype = any_dtype_code(x);
   a->batch = static_cast<int32_t>(x.size(0));
   a->tokens = static_cast<int32_t>(x.size(1));
   a->head_dim = static_cast<int32_t>(x.size(3));
-  a->interleaved = interleaved == Py_True;
+  a->interleaved = interleaved;
+  if (table.defined()) {
+    a->cs = static_cast<const float*>(table.data_ptr());
+    a->rot = static_cast<int32_t>(2 * table.size(2));
+    a->table_rows = static_cast<int32_t>(table.size(0));
+  }
+  if (positions.defined()) {
+    a->positions = static_cast<const int32_t*>(positions.data_ptr());
+    a->pos_stride[0] = positions.dim() == 2 ? positions.stride(0) : 0;
+    a->pos_stride[1] = positions.stride(-1);
+  }
 }
+
+// One tensor of a call: x and y, or, with g, what goes backward.
+void add_heads(B200RotaryArgs* a, const at::Tensor& x, const at::Tensor& y, const at::Tensor& g = {}) {
+  B200Heads& h = a->heads[a->tensors++];
+  h.x = x.defined() ? x.data_ptr() : nullptr;
+  h.y = y.data_ptr();
+  if (x.defined()) set_heads(h.x_stride, x);
+  set_heads(h.y_stride, y);
+  if (g.defined()) {
+    h.g = g.data_ptr();
+    set_heads(h.g_stride, g);
+  }
+  h.heads = static_cast<int32_t>(y.size(2));
+}
+
+// Scratch for the sums behind the weights' gradients by (device, stream), kept until the process ends; a capture gets its own.
+struct Scratch {
+  int64_t device, stream;
+  at::Tensor* memory;
+};
+std::vector<Scratch> g_rotary_scratch;
+constexpr int64_t kHeaderBytes = 256;  // zeroed
+
+at::Tensor rotary_scratch(const at::Tensor& like, const c10::cuda::CUDAStream& stream) {
+  const int64_t device = like.device().index(), id = reinterpret_cast<int64_t>(stream.stream());
+  std::lock_guard<std::mutex> lock(g_workspaces_mutex);
+  for (const Scratch& s : g_rotary_scratch)
+    if (s.device == device && s.stream == id) return *s.memory;
+  int64_t bytes = 0;
+  TORCH_CHECK(b200_rotary_workspace(&bytes) == B200_ATTN_OK, "rotary workspace: ", b200_attn_last_error());
+  const at::Tensor memory = at::empty({bytes}, like.options().dtype(at::kByte).requires_grad(false));
+  memory.narrow(0, 0, kHeaderBytes).zero_();
+  cudaStreamCaptureStatus capture = cudaStreamCaptureStatusNone;
+  if (cudaStreamIsCapturing(stream.stream(), &capture) == cudaSuccess && capture == cudaStreamCaptureStatusNone) g_rotary_scratch.push_back({device, id, new at::Tensor(memory)});
+  return memory;
+}
+
+using torch::autograd::AutogradContext;
+using torch::autograd::variable_list;
+
+// A gradient that comes in, as the kernels take it.
+at::Tensor incoming(const at::Tensor& g, const at::Tensor& like) {
+  if (!g.defined()) return at::zeros_like(like, at::MemoryFormat::Contiguous);
+  return g.stride(-1) == 1 || g.size(-1) == 1 ? g : g.contiguous();
+}
+// Gradients that must not be differentiated again, should somebody try (the kernels have no second derivative).
+variable_list once(variable_list grads) {
+  if (!at::GradMode::is_enabled()) return grads;
+  variable_list marked;
+  for (const at::Tensor& g : grads) marked.push_back(g.defined() ? g.detach().requires_grad_(true) : g);
+  auto error = std::make_shared<torch::autograd::DelayedError>("trying to differentiate twice a function that was marked with @once_differentiable", static_cast<int64_t>(marked.size()));
+  return (*error)(std::move(marked));
+}
+
+at::Tensor turned(const at::Tensor& x, const at::Tensor& table, const at::Tensor& positions, bool interleaved) {
+  at::Tensor y = empty_like_type(x.sizes(), x);
+  B200RotaryArgs a;
+  set_rotary(&a, x, table, positions, interleaved);
+  add_heads(&a, x, y);
+  TORCH_CHECK(b200_rotary(&a, c10::cuda::getCurrentCUDAStream(x.device().index()).stream()) == B200_ATTN_OK, "rotary: ", b200_attn_last_error());
+  return y;
+}
+
+struct RotaryFunction : torch::autograd::Function<RotaryFunction> {
+  static at::Tensor forward(AutogradContext* ctx, const at::Tensor& x, const at::Tensor& table, const at::Tensor& positions, bool interleaved) {
+    ctx->save_for_backward({table, positions});
+    ctx->saved_data["interleaved"] = interleaved;
+    return turned(x, table, positions, interleaved);
+  }
+  static variable_list backward(AutogradContext* ctx, const variable_list& grads) {
+    const variable_list saved = ctx->get_saved_variables();
+    variable_list result(4);
+    {
+      const at::NoGradGuard guard;
+      const c10::cuda::CUDAGuard on(grads[0].device());
+      const at::Tensor g = incoming(grads[0], grads[0]);
+      result[0] = empty_like_type(g.sizes(), g);
+      B200RotaryArgs a;
+      set_rotary(&a, g, saved[0], saved[1], ctx->saved_data["interleaved"].toBool());
+      a.backward = 1;
+      add_heads(&a, {}, result[0], g);
+      TORCH_CHECK(b200_rotary(&a, c10::cuda::getCurrentCUDAStream(g.device().index()).stream()) == B200_ATTN_OK, "rotary: ", b200_attn_last_error());
+    }
+    return once(std::move(result));
+  }
+};
 
 // rotary(x, table, positions | None, interleaved)
 PyObject* py_rotary(PyObject*, PyObject* const* args, Py_ssize_t n) {
   if (n != 4 || !PyBool_Check(args[3]) || args[1] == Py_None) Py_RETURN_NONE;
   const at::Tensor* x = tensor_of(args[0]);
   const c10::DeviceIndex device = c10::cuda::current_device();
-  if (!heads_of(x, device) || !heads_type(*x)) Py_RETURN_NONE;
-  B200RotaryArgs a;
-  std::memset(&a, 0, sizeof(a));
-  set_rotary(&a, *x, args[3]);
-  if (!set_turn(&a, *x, args[1], args[2], device)) Py_RETURN_NONE;
-  at::Tensor y = empty_like_type(x->sizes(), *x);
-  a.tensors = 1;
-  B200Heads& h = a.heads[0];
-  h.x = x->data_ptr();
-  h.y = y.data_ptr();
-  set_heads(h.x_stride, *x);
-  set_heads(h.y_stride, y);
-  h.heads = static_cast<int32_t>(x->size(2));
-  const c10::cuda::CUDAStream stream = c10::cuda::getCurrentCUDAStream(device);
-  if (launched([&] { return b200_rotary(&a, stream.stream()); }) != B200_ATTN_OK) Py_RETURN_NONE;
-  return THPVariable_Wrap(y);
+  at::Tensor table, positions;
+  if (!heads_on(x, device) || !heads_type(*x) || !turn_of(*x, args[1], args[2], device, &table, &positions)) Py_RETURN_NONE;
+  const bool interleaved = args[3] == Py_True;
+  return THPVariable_Wrap(wants_grad(*x) ? RotaryFunction::apply(*x, table, positions, interleaved) : turned(*x, table, positions, interleaved));
 }
+
+// x, weights (undefined: none) and results of the two tensors.
+variable_list normed(const at::Tensor* x, const at::Tensor* w, const at::Tensor& table, const at::Tensor& positions, double eps, bool interleaved) {
+  B200RotaryArgs a;
+  set_rotary(&a, x[0], table, positions, interleaved);
+  a.norm = 1;
+  a.eps = static_cast<float>(eps);
+  variable_list y;
+  for (int k = 0; k < 2; ++k) {
+    y.push_back(empty_like_type(x[k].sizes(), x[k]));
+    add_heads(&a, x[k], y[k]);
+    if (!w[k].defined()) continue;
+    a.heads[k].w = w[k].data_ptr();
+    a.weight_dtype = any_dtype_code(w[k]);
+  }
+  TORCH_CHECK(b200_rotary(&a, c10::cuda::getCurrentCUDAStream(x[0].device().index()).stream()) == B200_ATTN_OK, "qk_norm_rotary: ", b200_attn_last_error());
+  return y;
+}
+
+struct QkNormRotaryFunction : torch::autograd::Function<QkNormRotaryFunction> {
+  static variable_list forward(AutogradContext* ctx, const at::Tensor& q, const at::Tensor& k, const at::Tensor& wq, const at::Tensor& wk, const at::Tensor& table, const at::Tensor& positions, double eps, bool interleaved) {
+    ctx->save_for_backward({q, k, wq, wk, table, positions});
+    ctx->saved_data["eps"] = eps;
+    ctx->saved_data["interleaved"] = interleaved;
+    const at::Tensor x[2] = {q, k}, w[2] = {wq, wk};
+    return normed(x, w, table, positions, eps, interleaved);
+  }
+  static variable_list backward(AutogradContext* ctx, const variable_list& grads) {
+    const variable_list saved = ctx->get_saved_variables();
+    variable_list result(8);
+    {
+      const at::NoGradGuard guard;
+      const c10::cuda::CUDAGuard on(saved[0].device());
+      const c10::cuda::CUDAStream stream = c10::cuda::getCurrentCUDAStream(saved[0].device().index());
+      B200RotaryArgs a;
+      set_rotary(&a, saved[0], saved[4], saved[5], ctx->saved_data["interleaved"].toBool());
+      a.norm = a.backward = 1;
+      a.eps = static_cast<float>(ctx->saved_data["eps"].toDouble());
+      at::Tensor scratch, g[2];
+      for (int i = 0; i < 2; ++i) {
+        const at::Tensor &x = saved[i], &w = saved[2 + i];
+        g[i] = incoming(grads[i], x);
+        result[i] = empty_like_type(x.sizes(), x);
+        add_heads(&a, x, result[i], g[i]);
+        a.heads[i].w = w.data_ptr();
+        a.weight_dtype = any_dtype_code(w);
+        if (!ctx->needs_input_grad(2 + i)) continue;
+        result[2 + i] = empty_like_type(w.sizes(), w);
+        a.heads[i].dw = result[2 + i].data_ptr();
+        if (!scratch.defined()) scratch = rotary_scratch(x, stream);
+        a.workspace = scratch.data_ptr();
+        a.workspace_bytes = scratch.numel();
+      }
+      TORCH_CHECK(b200_rotary(&a, stream.stream()) == B200_ATTN_OK, "qk_norm_rotary: ", b200_attn_last_error());
+    }
+    return once(std::move(result));
+  }
+};
 
 // qk_norm_rotary(q, k, q_weight | None, k_weight | None, table | None, positions | None, eps, interleaved)
 PyObject* py_qk_norm_rotary(PyObject*, PyObject* const* args, Py_ssize_t n) {
@@ -400,39 +542,25 @@ PyObject* py_qk_norm_rotary(PyObject*, PyObject* const* args, Py_ssize_t n) {
   const c10::DeviceIndex device = c10::cuda::current_device();
   const at::Tensor* x[2] = {tensor_of(args[0]), tensor_of(args[1])};
   double eps = 0;
-  if (!heads_of(x[0], device) || !heads_of(x[1], device) || !heads_type(*x[0]) || x[1]->scalar_type() != x[0]->scalar_type() || !number(args[6], &eps) || !(eps >= 0)) Py_RETURN_NONE;
+  if (!heads_on(x[0], device) || !heads_on(x[1], device) || !heads_type(*x[0]) || x[1]->scalar_type() != x[0]->scalar_type() || !number(args[6], &eps) || !(eps >= 0)) Py_RETURN_NONE;
   for (int i : {0, 1, 3})
     if (x[1]->size(i) != x[0]->size(i)) Py_RETURN_NONE;
-  B200RotaryArgs a;
-  std::memset(&a, 0, sizeof(a));
-  set_rotary(&a, *x[0], args[7]);
-  if (!set_turn(&a, *x[0], args[4], args[5], device)) Py_RETURN_NONE;
-  const at::Tensor* first = nullptr;
+  at::Tensor table, positions, w[2];
+  if (!turn_of(*x[0], args[4], args[5], device, &table, &positions)) Py_RETURN_NONE;
+  bool grad = wants_grad(*x[0]) || wants_grad(*x[1]);
   for (int k = 0; k < 2; ++k) {
     if (args[2 + k] == Py_None) continue;
-    const at::Tensor* w = tensor_of(args[2 + k]);
-    if (w == nullptr || !plain(*w, device) || w->dim() != 1 || w->size(0) != x[0]->size(3) || !w->is_contiguous()) Py_RETURN_NONE;
-    if (w->scalar_type() != x[0]->scalar_type() && w->scalar_type() != at::kFloat) Py_RETURN_NONE;
-    if (first != nullptr && first->scalar_type() != w->scalar_type()) Py_RETURN_NONE;
-    first = w;
-    a.heads[k].w = w->data_ptr();
-    a.weight_dtype = any_dtype_code(*w);
+    const at::Tensor* given = tensor_of(args[2 + k]);
+    if (given == nullptr || !on_device(*given, device) || given->dim() != 1 || given->size(0) != x[0]->size(3) || !given->is_contiguous()) Py_RETURN_NONE;
+    if (given->scalar_type() != x[0]->scalar_type() && given->scalar_type() != at::kFloat) Py_RETURN_NONE;
+    if (k == 1 && w[0].defined() && w[0].scalar_type() != given->scalar_type()) Py_RETURN_NONE;
+    w[k] = *given;
+    grad = grad || wants_grad(w[k]);
   }
-  a.norm = 1;
-  a.eps = static_cast<float>(eps);
-  a.tensors = 2;
-  at::Tensor y[2];
-  for (int k = 0; k < 2; ++k) {
-    y[k] = empty_like_type(x[k]->sizes(), *x[k]);
-    B200Heads& h = a.heads[k];
-    h.x = x[k]->data_ptr();
-    h.y = y[k].data_ptr();
-    set_heads(h.x_stride, *x[k]);
-    set_heads(h.y_stride, y[k]);
-    h.heads = static_cast<int32_t>(x[k]->size(2));
-  }
-  const c10::cuda::CUDAStream stream = c10::cuda::getCurrentCUDAStream(device);
-  if (launched([&] { return b200_rotary(&a, stream.stream()); }) != B200_ATTN_OK) Py_RETURN_NONE;
+  if (grad && (!w[0].defined() || !w[1].defined())) Py_RETURN_NONE;  // the Python side has the gradient for any mix
+  const bool interleaved = args[7] == Py_True;
+  const at::Tensor both[2] = {*x[0], *x[1]};
+  const variable_list y = grad ? QkNormRotaryFunction::apply(both[0], both[1], w[0], w[1], table, positions, eps, interleaved) : normed(both, w, table, positions, eps, interleaved);
   return Py_BuildValue("(NN)", THPVariable_Wrap(y[0]), THPVariable_Wrap(y[1]));
 }
 

@@ -121,8 +121,8 @@ __global__ void __launch_bounds__(kKv4Threads) kv4_append_kernel(const Kv4Params
   const int64_t* s = what == 0 ? p.qs : what == 1 ? p.ks : p.vs;
   const T* x = static_cast<const T*>(what == 0 ? p.q : what == 1 ? p.k : p.v) + b * s[0] + n * s[1] + h * s[2];
   int at0, at1;
-  lane_places<FORM>(j, p.rot, &at0, &at1);
-  if (what == 2) at0 = 16 * j, at1 = 16 * j + 8;
+  lane_places<FORM>(j, p.rot, D, &at0, &at1);
+  if (what == 2) lane_places<kRowAny>(j, 0, D, &at0, &at1);
   float f[16];
   {
     Raw8<T> u, v;
@@ -133,7 +133,9 @@ __global__ void __launch_bounds__(kKv4Threads) kv4_append_kernel(const Kv4Params
   }
   const int at = p.lengths[b] - p.tokens + static_cast<int>(n);
   const float* cs = what == 2 ? nullptr : table_row(p.cs, p.rot, p.table_rows, at, p.status);
-  rotate16<FORM>(f, cs, j, p.rot, D, 1.f, p.interleaved, rows_smem + (FORM == kRowAny ? group * D : 0));
+  Turns<FORM> turns;
+  turns.load(cs, at0, at1, p.rot, 1.f);
+  rotate16<FORM>(f, turns, D, p.interleaved, rows_smem + (FORM == kRowAny ? group * D : 0));
   uint32_t words[2];
   const uint32_t pair = quantise16<kLanes>(f, words);
   if (!there) return;

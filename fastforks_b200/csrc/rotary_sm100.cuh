@@ -9,8 +9,7 @@
 //
 // Bound by HBM: each value is read once and written once (backward with a norm: two reads). A head is a row; 16 consecutive or
 // paired values of it are one lane's, so that a row is a group of 2, 4, 8, 16 or 32 lanes, its sums are shuffles within the group and
-// its accesses whole 16-byte words. Rows are numbered with the heads of one token next to one another: the token's row of the
-// table comes from L1.
+// its accesses whole 16-byte words. The rows of a token are dealt to a few groups of lanes, which load the token's cosines and sines once.
 #pragma once
 
 #include <cuda_bf16.h>
@@ -35,12 +34,13 @@ struct RotaryParams {
   const float* cs;
   const int32_t* positions;
   int64_t ps[2];
-  uint64_t heads_magic, tokens_magic, t_magic[2];
-  uint32_t rows;  // of both tensors
-  uint32_t t_rows[2];
-  int table_rows, tokens, dim, rot, lanes, heads;
-  bool interleaved, w_f32, vec;  // vec: every row of every tensor is 16-byte aligned
-  float eps, sign;               // sign: -1 turns back
+  uint64_t tokens_magic;
+  uint32_t all_tokens;  // batch * tokens
+  int table_rows, tokens, dim, rot, tensors;
+  int lanes_log2, steps_log2[2];      // lanes of a row; rows of a token that are worked on at once, for each tensor
+  int chunks[2];                      // of as many tokens as a CTA works on at once
+  bool interleaved, w_f32, vec;       // vec: every row of every tensor is 16-byte aligned
+  float eps, inv_dim, sign;           // sign: -1 turns back
   float* partial;                // norm, backward: [2][CTAs][dim]
   uint32_t* counter;
   uint32_t* status;
@@ -51,6 +51,7 @@ constexpr uint32_t kStatusPosition = 1u << 20, kStatusPage = 1u << 21;
 
 __device__ __forceinline__ uint32_t magic_div(uint32_t n, uint64_t magic) { return magic == 0 ? n : static_cast<uint32_t>(__umul64hi(n, magic)); }
 
+__device__ __forceinline__ bool aligned_16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
 __device__ __forceinline__ float to_f32(float v) { return v; }
 __device__ __forceinline__ float to_f32(__half v) { return __half2float(v); }
 __device__ __forceinline__ float to_f32(__nv_bfloat16 v) { return __bfloat162float(v); }
@@ -114,18 +115,26 @@ __device__ __forceinline__ void store8(T* p, const float* f) {
   }
 }
 
-// How a row lies in its lanes. kRowHalves: lane j < rot / 16 holds dimensions 8 j .. and rot / 2 + 8 j .. (the partners), the lanes behind
-// them 16 consecutive dimensions each. kRowPairs: 16 consecutive dimensions. Both want rot and dim in multiples of 16. kRowAny: 16
-// consecutive dimensions, partners through shared memory, any rot and dim.
+// How a row lies in its lanes, eight dimensions at a first and eight at a second place, so that neighbouring lanes' words are neighbours.
+// kRowHalves: lane j < rot / 16 holds dimensions 8 j .. and rot / 2 + 8 j .. (the partners), the lanes behind them the rest in the same way.
+// kRowPairs: dimensions 8 j .. and dim / 2 + 8 j ... Both want dim in multiples of 16, the one rot in multiples of 16, the other of 8.
+// kRowAny: 16 consecutive dimensions, partners through shared memory, any rot and dim.
 enum RowForm { kRowHalves = 0, kRowPairs = 1, kRowAny = 2 };
 
 template <int FORM>
-__device__ __forceinline__ void lane_places(int j, int rot, int* a, int* b) {
-  *a = 16 * j;
-  *b = 16 * j + 8;
-  if (FORM == kRowHalves && 16 * j < rot) {
+__device__ __forceinline__ void lane_places(int j, int rot, int dim, int* a, int* b) {
+  if (FORM == kRowAny) {
+    *a = 16 * j;
+    *b = 16 * j + 8;
+  } else if (FORM == kRowPairs) {
+    *a = 8 * j;
+    *b = (dim >> 1) + 8 * j;
+  } else if (16 * j < rot) {
     *a = 8 * j;
     *b = (rot >> 1) + 8 * j;
+  } else {
+    *a = (rot >> 1) + 8 * j;
+    *b = (dim >> 1) + 8 * j;
   }
 }
 
@@ -135,33 +144,62 @@ __device__ __forceinline__ void turn(float& a, float& b, float c, float s) {
   b = y;
 }
 
-// Rotates a lane's 16 values f (8 at its first place, 8 at its second). `cs`: the token's row of the table (nullptr: not rotated), the
-// cosines at 0 and the sines at rot / 2. `row`: the group's floats in shared memory (kRowAny).
+// The rotation with fused multiply-adds, behind a norm.
+__device__ __forceinline__ void turn_fused(float& a, float& b, float c, float s) {
+  const float x = fmaf(a, c, -(b * s)), y = fmaf(b, c, a * s);
+  a = x;
+  b = y;
+}
+
+// A lane's cosines and sines of a token's row of the table, the cosines at 0 and the sines at rot / 2 (nullptr: not rotated).
 template <int FORM>
-__device__ __forceinline__ void rotate16(float* f, const float* cs, int j, int rot, int dim, float sign, bool interleaved, float* row) {
-  if constexpr (FORM != kRowAny) {
-    if (cs == nullptr || 16 * j >= rot) return;
-    const float4* c4 = reinterpret_cast<const float4*>(cs + 8 * j);
-    const float4* s4 = reinterpret_cast<const float4*>(cs + (rot >> 1) + 8 * j);
-    const float4 c0 = __ldg(c4), c1 = __ldg(c4 + 1), s0 = __ldg(s4), s1 = __ldg(s4 + 1);
-    const float c[8] = {c0.x, c0.y, c0.z, c0.w, c1.x, c1.y, c1.z, c1.w};
-    const float s[8] = {s0.x, s0.y, s0.z, s0.w, s1.x, s1.y, s1.z, s1.w};
+struct Turns {
+  float c[8], s[8];
+  bool first, second;  // whether the lane's places are rotated
+  __device__ __forceinline__ void load(const float* cs, int a, int b, int rot, float sign) {
+    first = cs != nullptr && a < rot && (FORM == kRowPairs || b < rot);
+    second = cs != nullptr && b < rot;
+    const int at = FORM == kRowPairs ? a >> 1 : a, bt = FORM == kRowPairs ? b >> 1 : a + 4;
+    if (first) get(cs, at, rot, 0);
+    if (second) get(cs, bt, rot, 4);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) s[i] *= sign;
+  }
+  __device__ __forceinline__ void get(const float* cs, int at, int rot, int i) {
+    const float4 x = __ldg(reinterpret_cast<const float4*>(cs + at)), y = __ldg(reinterpret_cast<const float4*>(cs + (rot >> 1) + at));
+    c[i] = x.x, c[i + 1] = x.y, c[i + 2] = x.z, c[i + 3] = x.w;
+    s[i] = y.x, s[i + 1] = y.y, s[i + 2] = y.z, s[i + 3] = y.w;
+  }
+  template <bool FUSED>
+  __device__ __forceinline__ void apply(float* f) const {  // a lane's 16 values, 8 at its first place and 8 at its second
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
-      if (FORM == kRowHalves) turn(f[i], f[8 + i], c[i], sign * s[i]);
-      else turn(f[2 * i], f[2 * i + 1], c[i], sign * s[i]);
+      if (FORM == kRowPairs ? (i < 4 ? !first : !second) : !first) continue;
+      float &x = FORM == kRowHalves ? f[i] : f[2 * i], &y = FORM == kRowHalves ? f[8 + i] : f[2 * i + 1];
+      if (FUSED) turn_fused(x, y, c[i], s[i]);
+      else turn(x, y, c[i], s[i]);
     }
-  } else {
+  }
+};
+
+// The same for rows of any form: partners are looked up in `row`, the group's floats in shared memory.
+template <>
+struct Turns<kRowAny> {
+  const float* cs;
+  int a, rot;
+  float sign;
+  __device__ __forceinline__ void load(const float* table, int place, int, int n, float by) { cs = table, a = place, rot = n, sign = by; }
+  __device__ __forceinline__ void apply(float* f, float* row, int dim, bool interleaved) const {
     __syncwarp();
 #pragma unroll
     for (int i = 0; i < 16; ++i)
-      if (16 * j + i < dim) row[16 * j + i] = f[i];
+      if (a + i < dim) row[a + i] = f[i];
     __syncwarp();
     if (cs == nullptr) return;
     const int half = rot >> 1;
 #pragma unroll
     for (int i = 0; i < 16; ++i) {
-      const int e = 16 * j + i;
+      const int e = a + i;
       if (e >= rot) continue;
       const bool first = interleaved ? (e & 1) == 0 : e < half;
       const int at = interleaved ? e >> 1 : first ? e : e - half;
@@ -170,31 +208,37 @@ __device__ __forceinline__ void rotate16(float* f, const float* cs, int j, int r
       f[i] = first ? __fsub_rn(__fmul_rn(f[i], c), __fmul_rn(other, s)) : __fadd_rn(__fmul_rn(f[i], c), __fmul_rn(other, s));
     }
   }
+};
+
+template <int FORM>
+__device__ __forceinline__ void rotate16(float* f, const Turns<FORM>& turns, int dim, bool interleaved, float* row) {
+  if constexpr (FORM == kRowAny) turns.apply(f, row, dim, interleaved);
+  else turns.template apply<false>(f);
 }
 
-// A lane's 16 values of the row at `p`, zeros past `dim`.
-template <typename T, int FORM>
-__device__ __forceinline__ void load16(float* f, const T* p, int a, int b, int dim, bool vec) {
-  if (FORM != kRowAny || (vec && a + 16 <= dim)) {
+// 16 values from `at` on of a row, zeros past `dim`. vec: the row starts on 16 bytes.
+template <typename T>
+__device__ __forceinline__ void load16(float* f, const T* p, int at, int dim, bool vec) {
+  if (vec && at + 16 <= dim) {
     Raw8<T> u, v;
-    u.load(p + a);
-    v.load(p + b);
+    u.load(p + at);
+    v.load(p + at + 8);
     u.unpack(f);
     v.unpack(f + 8);
   } else {
 #pragma unroll
-    for (int i = 0; i < 16; ++i) f[i] = a + i < dim ? to_f32(p[a + i]) : 0.f;
+    for (int i = 0; i < 16; ++i) f[i] = at + i < dim ? to_f32(p[at + i]) : 0.f;
   }
 }
-template <typename T, int FORM>
-__device__ __forceinline__ void store16(T* p, const float* f, int a, int b, int dim, bool vec) {
-  if (FORM != kRowAny || (vec && a + 16 <= dim)) {
-    store8<T>(p + a, f);
-    store8<T>(p + b, f + 8);
+template <typename T>
+__device__ __forceinline__ void store16(T* p, const float* f, int at, int dim, bool vec) {
+  if (vec && at + 16 <= dim) {
+    store8<T>(p + at, f);
+    store8<T>(p + at + 8, f + 8);
   } else {
 #pragma unroll
     for (int i = 0; i < 16; ++i)
-      if (a + i < dim) p[a + i] = from_f32<T>(f[i]);
+      if (at + i < dim) p[at + i] = from_f32<T>(f[i]);
   }
 }
 
@@ -211,8 +255,8 @@ __device__ __forceinline__ const float* token_row(const RotaryParams& p, uint32_
   return p.rot == 0 ? nullptr : table_row(p.cs, p.rot, p.table_rows, p.positions == nullptr ? static_cast<int>(n) : p.positions[b * p.ps[0] + n * p.ps[1]], p.status);
 }
 
-__device__ __forceinline__ float group_sum(float v, int lanes) {
-  for (int o = lanes >> 1; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+__device__ __forceinline__ float group_sum(float v, int lanes_log2) {
+  for (int o = 1 << lanes_log2 >> 1; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
   return v;
 }
 
@@ -220,128 +264,72 @@ __device__ __forceinline__ float group_sum(float v, int lanes) {
 template <typename T, int FORM>
 __device__ __forceinline__ void load_weight(float* f, const RotaryParams& p, const void* w, int a, int b) {
 #pragma unroll
+  for (int i = 0; i < 16; ++i) f[i] = 1.f;
+  if (w == nullptr) return;
+  if (FORM != kRowAny && aligned_16(w)) {
+    if (p.w_f32) {
+      Raw8<float> u, v;
+      u.load(static_cast<const float*>(w) + a);
+      v.load(static_cast<const float*>(w) + b);
+      u.unpack(f);
+      v.unpack(f + 8);
+    } else {
+      Raw8<T> u, v;
+      u.load(static_cast<const T*>(w) + a);
+      v.load(static_cast<const T*>(w) + b);
+      u.unpack(f);
+      v.unpack(f + 8);
+    }
+    return;
+  }
+#pragma unroll
   for (int i = 0; i < 16; ++i) {
     const int e = (i < 8 ? a : b - 8) + i;
-    f[i] = w == nullptr || e >= p.dim ? 1.f : p.w_f32 ? __ldg(static_cast<const float*>(w) + e) : to_f32(static_cast<const T*>(w)[e]);
+    if (e < p.dim) f[i] = p.w_f32 ? __ldg(static_cast<const float*>(w) + e) : to_f32(static_cast<const T*>(w)[e]);
   }
 }
 
-// Forward, and backward without a norm (x = g, sign = -1).
-template <typename T, int FORM, bool NORM>
-__global__ void __launch_bounds__(kRotaryThreads) rotary_kernel(const RotaryParams p) {
-  extern __shared__ float rotary_smem[];
-  grid_dependency_wait();
-  grid_launch_dependents();
-  const int j = threadIdx.x & (p.lanes - 1), group = threadIdx.x / p.lanes, groups = kRotaryThreads / p.lanes;
-  float* row_smem = rotary_smem + group * p.dim;
-  int a, b;
-  lane_places<FORM>(j, p.rot, &a, &b);
-  const bool mine = 16 * j < p.dim;
-  const uint32_t row = blockIdx.x * groups + group;
-  const bool there = row < p.rows;
-  const uint32_t token = magic_div(there ? row : 0, p.heads_magic);
-  uint32_t h = (there ? row : 0) - token * p.heads;
-  const bool second = h >= static_cast<uint32_t>(p.t[0].heads);
-  const RotaryTensor& t = p.t[second ? 1 : 0];
-  if (second) h -= p.t[0].heads;
-  const uint32_t img = magic_div(token, p.tokens_magic), n = token - img * p.tokens;
-  const T* x = static_cast<const T*>(t.x) + img * t.xs[0] + n * t.xs[1] + h * t.xs[2];
-  float f[16];
-  if (there && mine) {
-    load16<T, FORM>(f, x, a, b, p.dim, p.vec);
-  } else {
+enum RotaryMode { kTurn = 0, kNormTurn = 1, kNormBack = 2 };
+
+// Rows that a lane has in flight, in its own places in shared memory: 128 KB an SM in 16 bits.
+template <typename T, int MODE>
+struct RotaryStream {
+  static constexpr int kCtasPerSm = MODE == kTurn ? 4 : MODE == kNormTurn ? 3 : 2;
+  static constexpr int kParts = sizeof(T) / 2 * 2;                        // 16-byte words of a row in a lane
+  static constexpr int kTensors = MODE == kNormBack ? 2 : 1;             // x, and g
+  static constexpr int kDepth = sizeof(T) == 4 ? 2 : 4;
+  static constexpr int kSlot = kTensors * kParts * kRotaryThreads * 16;  // bytes of one row of all lanes
+  static constexpr int kBytes = kDepth * kSlot;
+};
+
+// Sums for dw: the lanes' own of tensor k go to this CTA's line of `partial`. A lane's places are a .. a + 7 and b .. b + 7.
+__device__ __forceinline__ void put_sums(const RotaryParams& p, float* dw, float* smem, int k, int a, int b, bool place) {
+  // Lanes with the same place: within a warp by shuffles, then over the warps through shared memory.
+  for (int o = 1 << p.lanes_log2; o < 32; o <<= 1) {
 #pragma unroll
-    for (int i = 0; i < 16; ++i) f[i] = 0.f;
+    for (int i = 0; i < 16; ++i) dw[i] += __shfl_xor_sync(0xffffffffu, dw[i], o);
   }
-  const float* cs = token_row(p, img, n);
-  if constexpr (NORM) {
-    float sum = 0.f;
+  __syncthreads();  // what lay there before
+  if ((threadIdx.x & 31) >> p.lanes_log2 == 0 && place) {
 #pragma unroll
-    for (int i = 0; i < 16; ++i) sum = fmaf(f[i], f[i], sum);
-    const float r = rsqrtf(group_sum(sum, p.lanes) / p.dim + p.eps);
-    float w[16];
-    if (mine) load_weight<T, FORM>(w, p, t.w, a, b);
-#pragma unroll
-    for (int i = 0; i < 16; ++i) f[i] = f[i] * r * w[i];
+    for (int i = 0; i < 16; ++i) {
+      const int e = (i < 8 ? a : b - 8) + i;
+      if (e < p.dim) smem[(threadIdx.x >> 5) * p.dim + e] = dw[i];
+    }
   }
-  rotate16<FORM>(f, cs, j, p.rot, p.dim, p.sign, p.interleaved, row_smem);
-  if (there && mine) store16<T, FORM>(static_cast<T*>(t.y) + img * t.ys[0] + n * t.ys[1] + h * t.ys[2], f, a, b, p.dim, p.vec);
+  __syncthreads();
+  for (int e = threadIdx.x; e < p.dim; e += kRotaryThreads) {
+    float v = 0.f;
+#pragma unroll
+    for (int i = 0; i < kRotaryThreads / 32; ++i) v += smem[i * p.dim + e];
+    p.partial[(static_cast<int64_t>(k) * gridDim.x + blockIdx.x) * p.dim + e] = v;
+  }
+  __syncthreads();
 }
 
-// Gradients through norm and rotation. A CTA walks rows of the first tensor, then of the second, and keeps its lanes' sums for dw in
-// registers; they go through shared memory to a line of `partial`, and the CTA that counts last adds the lines in their order.
-template <typename T, int FORM>
-__global__ void __launch_bounds__(kRotaryThreads) norm_rotary_backward_kernel(const RotaryParams p) {
-  extern __shared__ float rotary_smem[];
-  grid_dependency_wait();
-  grid_launch_dependents();
-  const int j = threadIdx.x & (p.lanes - 1), group = threadIdx.x / p.lanes, groups = kRotaryThreads / p.lanes;
-  float* row_smem = rotary_smem + group * p.dim;
-  int a, b;
-  lane_places<FORM>(j, p.rot, &a, &b);
-  const bool mine = 16 * j < p.dim;
-  for (int k = 0; k < 2; ++k) {
-    if (p.t_rows[k] == 0) continue;
-    const RotaryTensor& t = p.t[k];
-    float w[16], dw[16];
-#pragma unroll
-    for (int i = 0; i < 16; ++i) w[i] = 1.f, dw[i] = 0.f;
-    if (mine) load_weight<T, FORM>(w, p, t.w, a, b);
-    for (uint32_t first = blockIdx.x * groups; first < p.t_rows[k]; first += gridDim.x * groups) {
-      const bool there = first + group < p.t_rows[k];
-      const uint32_t row = there ? first + group : 0;
-      const uint32_t token = magic_div(row, p.t_magic[k]), h = row - token * t.heads;
-      const uint32_t img = magic_div(token, p.tokens_magic), n = token - img * p.tokens;
-      float f[16], g[16];
-#pragma unroll
-      for (int i = 0; i < 16; ++i) f[i] = g[i] = 0.f;
-      if (there && mine) {
-        load16<T, FORM>(f, static_cast<const T*>(t.x) + img * t.xs[0] + n * t.xs[1] + h * t.xs[2], a, b, p.dim, p.vec);
-        load16<T, FORM>(g, static_cast<const T*>(t.g) + img * t.gs[0] + n * t.gs[1] + h * t.gs[2], a, b, p.dim, p.vec);
-      }
-      rotate16<FORM>(g, token_row(p, img, n), j, p.rot, p.dim, -1.f, p.interleaved, row_smem);
-      float sum = 0.f, along = 0.f;
-#pragma unroll
-      for (int i = 0; i < 16; ++i) {
-        sum = fmaf(f[i], f[i], sum);
-        along = fmaf(g[i] * w[i], f[i], along);
-      }
-      sum = group_sum(sum, p.lanes);
-      along = group_sum(along, p.lanes);
-      const float r = rsqrtf(sum / p.dim + p.eps);
-      const float back = along * r / p.dim;  // mean(t w x r)
-#pragma unroll
-      for (int i = 0; i < 16; ++i) {
-        const float hat = f[i] * r;
-        dw[i] = fmaf(g[i], hat, dw[i]);
-        f[i] = r * (g[i] * w[i] - hat * back);
-      }
-      if (there && mine) store16<T, FORM>(static_cast<T*>(t.y) + img * t.ys[0] + n * t.ys[1] + h * t.ys[2], f, a, b, p.dim, p.vec);
-    }
-    if (t.dw == nullptr) continue;
-    // Lanes with the same place: within a warp by shuffles, then over the warps through shared memory.
-    for (int o = p.lanes; o < 32; o <<= 1) {
-#pragma unroll
-      for (int i = 0; i < 16; ++i) dw[i] += __shfl_xor_sync(0xffffffffu, dw[i], o);
-    }
-    __syncthreads();  // rows of kRowAny, and the other tensor's sums
-    if ((threadIdx.x & 31) < p.lanes && mine) {
-#pragma unroll
-      for (int i = 0; i < 16; ++i) {
-        const int e = (i < 8 ? a : b - 8) + i;
-        if (e < p.dim) rotary_smem[(threadIdx.x >> 5) * p.dim + e] = dw[i];
-      }
-    }
-    __syncthreads();
-    for (int e = threadIdx.x; e < p.dim; e += kRotaryThreads) {
-      float v = 0.f;
-#pragma unroll
-      for (int i = 0; i < kRotaryThreads / 32; ++i) v += rotary_smem[i * p.dim + e];
-      p.partial[(static_cast<int64_t>(k) * gridDim.x + blockIdx.x) * p.dim + e] = v;
-    }
-    __syncthreads();
-  }
-  if (p.t[0].dw == nullptr && p.t[1].dw == nullptr) return;
+// The CTA that counts last adds all lines: eight warps take every eighth line each, and their sums are added in their order.
+template <typename T>
+__device__ __forceinline__ void join_sums(const RotaryParams& p, float* smem) {
   __shared__ uint32_t last;
   __threadfence();
   __syncthreads();
@@ -349,29 +337,241 @@ __global__ void __launch_bounds__(kRotaryThreads) norm_rotary_backward_kernel(co
   __syncthreads();
   if (last == 0) return;
   __threadfence();
-  // Eight warps take every eighth line each; a warp's sums of a column are added to the others' in their order.
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  for (int k = 0; k < 2; ++k) {
+  for (int k = 0; k < p.tensors; ++k) {
     const RotaryTensor& t = p.t[k];
-    if (p.t_rows[k] == 0 || t.dw == nullptr) continue;
+    if (t.dw == nullptr) continue;
     const float* lines = p.partial + static_cast<int64_t>(k) * gridDim.x * p.dim;
     for (int e = lane; e < p.dim; e += 32) {
       float v = 0.f;
-#pragma unroll 8
+#pragma unroll 16
       for (uint32_t c = warp; c < gridDim.x; c += 8) v += __ldcg(lines + static_cast<int64_t>(c) * p.dim + e);
-      rotary_smem[warp * p.dim + e] = v;
+      smem[warp * p.dim + e] = v;
     }
     __syncthreads();
     for (int e = threadIdx.x; e < p.dim; e += kRotaryThreads) {
       float v = 0.f;
 #pragma unroll
-      for (int i = 0; i < 8; ++i) v += rotary_smem[i * p.dim + e];
+      for (int i = 0; i < 8; ++i) v += smem[i * p.dim + e];
       if (p.w_f32) static_cast<float*>(t.dw)[e] = v;
       else static_cast<T*>(t.dw)[e] = from_f32<T>(v);
     }
     __syncthreads();
   }
   if (threadIdx.x == 0) *p.counter = 0;
+}
+
+// Rows of whole lanes on 16 bytes. A lane streams its rows through places of its own in shared memory, kDepth rows ahead, so that what is
+// in flight costs no registers; nobody else reads them, so nothing but its own copies has to be waited for. A CTA walks chunks of tokens
+// with the first tensor, then with the second (the weights, and backward the sums for dw, are one tensor's at a time).
+template <typename T, int FORM, int MODE>
+__global__ void __launch_bounds__(kRotaryThreads, RotaryStream<T, MODE>::kCtasPerSm) rotary_stream_kernel(const RotaryParams p) {
+  using S = RotaryStream<T, MODE>;
+  extern __shared__ __align__(16) float rotary_smem[];
+  grid_dependency_wait();
+  grid_launch_dependents();
+  const int j = threadIdx.x & ((1 << p.lanes_log2) - 1), group = threadIdx.x >> p.lanes_log2;
+  int a, b;
+  lane_places<FORM>(j, p.rot, p.dim, &a, &b);
+  const bool place = 16 * j < p.dim;
+  uint4* mine = reinterpret_cast<uint4*>(rotary_smem) + threadIdx.x;
+  const uint32_t mine_at = smem_u32(mine);
+  for (int k = 0; k < p.tensors; ++k) {
+    const RotaryTensor& t = p.t[k];
+    const int step = 1 << p.steps_log2[k], first = group & (step - 1), heads = t.heads;
+    const uint32_t in_chunk = group >> p.steps_log2[k], chunk_tokens = kRotaryThreads >> (p.lanes_log2 + p.steps_log2[k]);
+    const int chunks = p.chunks[k];
+    float w[16], dw[16];
+#pragma unroll
+    for (int i = 0; i < 16; ++i) w[i] = 1.f, dw[i] = 0.f;
+    if (MODE != kTurn && place) load_weight<T, FORM>(w, p, t.w, a, b);
+    // The place of the copies: a chunk of tokens, and the first of `step` heads in it.
+    int ahead = blockIdx.x, ahead_h = 0, slot = 0;
+    bool ahead_there = false;
+    const T *from_x = nullptr, *from_g = nullptr;
+    const auto token_of = [&](int chunk) { return chunk * chunk_tokens + in_chunk; };
+    const auto enter = [&]() {
+      const uint32_t token = token_of(ahead);
+      ahead_there = ahead < chunks && place && token < p.all_tokens;
+      if (!ahead_there) return;
+      const uint32_t img = magic_div(token, p.tokens_magic), n = token - img * p.tokens;
+      from_x = static_cast<const T*>(t.x) + img * t.xs[0] + n * t.xs[1] + first * t.xs[2];
+      if (MODE == kNormBack) from_g = static_cast<const T*>(t.g) + img * t.gs[0] + n * t.gs[1] + first * t.gs[2];
+    };
+    const auto copy = [&]() {
+      if (ahead < chunks) {
+        const bool valid = ahead_there && ahead_h + first < heads;
+        const uint32_t to = mine_at + slot * S::kSlot;
+        constexpr int kHalf = S::kParts / 2;
+#pragma unroll
+        for (int i = 0; i < S::kParts; ++i) {
+          const int at = i < kHalf ? a + i * (16 / static_cast<int>(sizeof(T))) : b + (i - kHalf) * (16 / static_cast<int>(sizeof(T)));
+          if (valid) {
+            cp_async_16(to + i * kRotaryThreads * 16, from_x + at, true);
+            if (MODE == kNormBack) cp_async_16(to + (S::kParts + i) * kRotaryThreads * 16, from_g + at, true);
+          }
+        }
+        from_x += step * t.xs[2];
+        if (MODE == kNormBack) from_g += step * t.gs[2];
+        ahead_h += step;
+        if (ahead_h >= heads) {
+          ahead_h = 0;
+          ahead += gridDim.x;
+          enter();
+        }
+      }
+      cp_async_commit();
+      slot = slot + 1 == S::kDepth ? 0 : slot + 1;
+    };
+    enter();
+#pragma unroll
+    for (int i = 0; i < S::kDepth - 1; ++i) copy();
+    int use = 0;
+    for (int chunk = blockIdx.x; chunk < chunks; chunk += gridDim.x) {
+      const uint32_t token = token_of(chunk);
+      const bool there = place && token < p.all_tokens;
+      const uint32_t img = there ? magic_div(token, p.tokens_magic) : 0, n = there ? token - img * p.tokens : 0;
+      T* y = static_cast<T*>(t.y) + img * t.ys[0] + n * t.ys[1] + first * t.ys[2];
+      Turns<FORM> turns;
+      turns.load(there ? token_row(p, img, n) : nullptr, a, b, p.rot, MODE == kNormBack ? -1.f : p.sign);
+      for (int h0 = 0; h0 < heads; h0 += step) {  // the same for all lanes of a warp
+        copy();
+        cp_async_wait<S::kDepth - 1>();
+        const uint4* at = mine + use * (S::kSlot / 16);
+        use = use + 1 == S::kDepth ? 0 : use + 1;
+        const bool valid = there && h0 + first < heads;
+        float f[16];
+        const auto read = [&](float* to, int part) {
+          Raw8<T> u;
+#pragma unroll
+          for (int i = 0; i < 2; ++i) {
+            if constexpr (sizeof(T) == 4) {
+              u.a = *reinterpret_cast<const float4*>(at + (part + 2 * i) * kRotaryThreads);
+              u.b = *reinterpret_cast<const float4*>(at + (part + 2 * i + 1) * kRotaryThreads);
+            } else {
+              u.v = at[(part + i) * kRotaryThreads];
+            }
+            u.unpack(to + 8 * i);
+          }
+        };
+        if (valid) {
+          read(f, 0);
+        } else {
+#pragma unroll
+          for (int i = 0; i < 16; ++i) f[i] = 0.f;
+        }
+        if constexpr (MODE == kTurn) {
+          turns.template apply<false>(f);
+        } else {
+          float e[16], sum = 0.f;
+#pragma unroll
+          for (int i = 0; i < 16; ++i) sum = fmaf(f[i], f[i], sum);
+          if constexpr (MODE == kNormTurn) {
+            const float r = rsqrtf(fmaf(group_sum(sum, p.lanes_log2), p.inv_dim, p.eps));
+#pragma unroll
+            for (int i = 0; i < 16; ++i) f[i] = f[i] * r * w[i];
+            turns.template apply<true>(f);
+          } else {
+            if (valid) {
+              read(e, S::kParts);
+            } else {
+#pragma unroll
+              for (int i = 0; i < 16; ++i) e[i] = 0.f;
+            }
+            turns.template apply<true>(e);
+            float along = 0.f;
+#pragma unroll
+            for (int i = 0; i < 16; ++i) along = fmaf(e[i] * w[i], f[i], along);
+            for (int o = 1 << p.lanes_log2 >> 1; o > 0; o >>= 1) {
+              sum += __shfl_xor_sync(0xffffffffu, sum, o);
+              along += __shfl_xor_sync(0xffffffffu, along, o);
+            }
+            const float r = rsqrtf(fmaf(sum, p.inv_dim, p.eps));
+            const float back = along * r * r * p.inv_dim;  // r mean(t w x r)
+#pragma unroll
+            for (int i = 0; i < 16; ++i) {
+              const float hat = f[i] * r;
+              dw[i] = fmaf(e[i], hat, dw[i]);
+              f[i] = fmaf(r, e[i] * w[i], -(hat * back));
+            }
+          }
+        }
+        if (valid) {
+          store8<T>(y + a, f);
+          store8<T>(y + b, f + 8);
+        }
+        y += step * t.ys[2];
+      }
+    }
+    cp_async_wait<0>();
+    if (MODE == kNormBack && t.dw != nullptr) put_sums(p, dw, rotary_smem, k, a, b, place);
+    __syncthreads();  // the places are laid anew, and were smem of the sums
+  }
+  if (MODE == kNormBack && (p.t[0].dw != nullptr || p.t[1].dw != nullptr)) join_sums<T>(p, rotary_smem);
+}
+
+// Rows of any kind, one at a time.
+template <typename T, int MODE>
+__global__ void __launch_bounds__(kRotaryThreads, 2) rotary_any_kernel(const RotaryParams p) {
+  extern __shared__ __align__(16) float rotary_smem[];
+  grid_dependency_wait();
+  grid_launch_dependents();
+  const int j = threadIdx.x & ((1 << p.lanes_log2) - 1), group = threadIdx.x >> p.lanes_log2;
+  float* row_smem = rotary_smem + group * p.dim;
+  int a, b;
+  lane_places<kRowAny>(j, p.rot, p.dim, &a, &b);
+  const bool place = a < p.dim;
+  for (int k = 0; k < p.tensors; ++k) {
+    const RotaryTensor& t = p.t[k];
+    const int step = 1 << p.steps_log2[k], first = group & (step - 1);
+    const uint32_t in_chunk = group >> p.steps_log2[k], chunk_tokens = kRotaryThreads >> (p.lanes_log2 + p.steps_log2[k]);
+    float w[16], dw[16];
+#pragma unroll
+    for (int i = 0; i < 16; ++i) w[i] = 1.f, dw[i] = 0.f;
+    if (MODE != kTurn && place) load_weight<T, kRowAny>(w, p, t.w, a, b);
+    for (int chunk = blockIdx.x; chunk < p.chunks[k]; chunk += gridDim.x) {
+      const uint32_t token = chunk * chunk_tokens + in_chunk;
+      const bool there = place && token < p.all_tokens;
+      const uint32_t img = there ? magic_div(token, p.tokens_magic) : 0, n = there ? token - img * p.tokens : 0;
+      Turns<kRowAny> turns;
+      turns.load(there ? token_row(p, img, n) : nullptr, a, b, p.rot, MODE == kNormBack ? -1.f : p.sign);
+      for (int h0 = 0; h0 < t.heads; h0 += step) {
+        const int h = h0 + first;
+        const bool valid = there && h < t.heads;
+        float f[16];
+        load16<T>(f, static_cast<const T*>(t.x) + img * t.xs[0] + n * t.xs[1] + h * t.xs[2], a, valid ? p.dim : 0, p.vec);
+        if constexpr (MODE == kTurn) {
+          turns.apply(f, row_smem, p.dim, p.interleaved);
+        } else {
+          float sum = 0.f;
+#pragma unroll
+          for (int i = 0; i < 16; ++i) sum = fmaf(f[i], f[i], sum);
+          const float r = rsqrtf(fmaf(group_sum(sum, p.lanes_log2), p.inv_dim, p.eps));
+          if constexpr (MODE == kNormTurn) {
+#pragma unroll
+            for (int i = 0; i < 16; ++i) f[i] = f[i] * r * w[i];
+            turns.apply(f, row_smem, p.dim, p.interleaved);
+          } else {
+            float e[16], along = 0.f;
+            load16<T>(e, static_cast<const T*>(t.g) + img * t.gs[0] + n * t.gs[1] + h * t.gs[2], a, valid ? p.dim : 0, p.vec);
+            turns.apply(e, row_smem, p.dim, p.interleaved);
+#pragma unroll
+            for (int i = 0; i < 16; ++i) along = fmaf(e[i] * w[i], f[i], along);
+            const float back = group_sum(along, p.lanes_log2) * r * r * p.inv_dim;
+#pragma unroll
+            for (int i = 0; i < 16; ++i) {
+              const float hat = f[i] * r;
+              dw[i] = fmaf(e[i], hat, dw[i]);
+              f[i] = fmaf(r, e[i] * w[i], -(hat * back));
+            }
+          }
+        }
+        if (valid) store16<T>(static_cast<T*>(t.y) + img * t.ys[0] + n * t.ys[1] + h * t.ys[2], f, a, p.dim, p.vec);
+      }
+    }
+    if (MODE == kNormBack && t.dw != nullptr) put_sums(p, dw, rotary_smem, k, a, b, place);
+  }
+  if (MODE == kNormBack && (p.t[0].dw != nullptr || p.t[1].dw != nullptr)) join_sums<T>(p, rotary_smem);
 }
 
 }  // namespace b200

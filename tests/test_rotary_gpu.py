@@ -228,6 +228,45 @@ def test_norm_rotary_on_another_stream_and_in_a_graph() -> None:
         assert all(torch.equal(a, b) for a, b in zip(want, held, strict=True))
 
 
+def test_a_second_derivative_is_refused() -> None:
+    table = ff.rotary_table(4, 64, device="cuda")
+    x = normal(1, 4, 2, 64, dtype=torch.float32).requires_grad_(True)
+    w = torch.ones(64, device="cuda", requires_grad=True)
+    for _ in range(2):  # the full way, and the way of repeated calls
+        for y in (ff.rotary(x, table), ff.qk_norm_rotary(x, x, w, w, table)[0]):
+            (dx,) = torch.autograd.grad(y.square().sum(), x, create_graph=True)
+            with pytest.raises(RuntimeError, match="once_differentiable"):
+                dx.sum().backward()
+
+
+def test_gradients_of_what_needs_them() -> None:
+    """Parts of the inputs alone, an output that is not used, an output that is used twice, and outputs changed in place."""
+    table = ff.rotary_table(6, 64, device="cuda")
+    q, k, wq, wk = normal(2, 6, 4, 64, dtype=torch.bfloat16, seed=1), normal(2, 6, 2, 64, dtype=torch.bfloat16, seed=2), *torch.ones(2, 64, device="cuda", dtype=torch.bfloat16)
+    g = normal(2, 6, 4, 64, dtype=torch.bfloat16, seed=3)
+    full = [t.detach().requires_grad_(True) for t in (q, k, wq, wk)]
+    want = torch.autograd.grad(ff.qk_norm_rotary(*full, table)[0], full, g, allow_unused=True)
+    assert not want[1].any()
+    assert not want[3].any()
+    for needs in ((0,), (2,), (0, 2), (1, 2)):
+        leaves = [t.detach().requires_grad_(i in needs) for i, t in enumerate((q, k, wq, wk))]
+        out = ff.qk_norm_rotary(*leaves, table)[0]
+        assert out.requires_grad
+        got = torch.autograd.grad(out, [leaves[i] for i in needs], g)
+        assert all(torch.equal(a, want[i]) for a, i in zip(got, needs, strict=True))
+    x = q.detach().requires_grad_(True)
+    y = ff.rotary(x, table)
+    (dx,) = torch.autograd.grad(y, x, g, retain_graph=True)
+    (twice,) = torch.autograd.grad((y, y), x, (g, g))
+    assert torch.equal(twice, 2 * dx)
+    z = ff.rotary(x, table)
+    z.mul_(2)
+    (scaled,) = torch.autograd.grad(z, x, g)
+    assert torch.equal(scaled, 2 * dx)
+    with torch.no_grad():
+        assert not ff.rotary(x, table).requires_grad
+
+
 def test_refusals_on_the_device() -> None:
     x, table = normal(1, 4, 2, 64, dtype=torch.float16), ff.rotary_table(4, 64, device="cuda")
     w = torch.ones(64, device="cuda", dtype=torch.float16)
