@@ -210,26 +210,22 @@ int b200_rotary(const B200RotaryArgs* a, void* stream_ptr) {
   const RotaryForm kernel = a->dtype == B200_ATTN_F16 ? rotary_form_of<__half>(form, mode) : a->dtype == B200_ATTN_BF16 ? rotary_form_of<__nv_bfloat16>(form, mode) : rotary_form_of<float>(form, mode);
   // A token's rows go to as many groups of lanes as leave each of them four rows or more; calls of few tokens use more groups than that.
   const int groups = kRotaryThreads >> p.lanes_log2;
-  int64_t chunks = 0;
+  const int64_t most = static_cast<int64_t>(dev->sms) * kernel.ctas_per_sm;
+  int64_t ctas = 1;
   for (int k = 0; k < a->tensors; ++k) {
     const int heads = a->heads[k].heads;
     int g = 0;
     while (2 << g <= std::min(groups, heads / 4)) ++g;
-    const auto count = [&] { return (static_cast<int64_t>(p.all_tokens) * (1 << g) + groups - 1) / groups; };
-    while (2 << g <= groups && 1 << g < heads && count() < dev->sms) ++g;
+    while (2 << g <= groups && 1 << g < heads && static_cast<int64_t>(p.all_tokens) * (1 << g) < most * groups) ++g;
     p.steps_log2[k] = g;
-    p.chunks[k] = static_cast<int>(count());
-    chunks = std::max(chunks, count());
+    ctas = std::max(ctas, std::min(most, (static_cast<int64_t>(p.all_tokens) * (1 << g) + groups - 1) / groups));
   }
-  // Every CTA gets the same number of chunks, give or take one.
-  const int64_t waves = (chunks + static_cast<int64_t>(dev->sms) * kernel.ctas_per_sm - 1) / (static_cast<int64_t>(dev->sms) * kernel.ctas_per_sm);
-  const int64_t ctas = (chunks + waves - 1) / waves;
   int smem = kernel.smem;
   if (form == kRowAny) smem = groups * p.dim * 4;
   if (mode == kNormBack) {
-    smem = std::max(smem, kRotaryThreads / 32 * p.dim * 4);
+    smem = std::max({smem, kRotaryThreads / 32 * p.dim * 4, kRotaryThreads * 16});
     if (sums) {
-      if (a->workspace == nullptr || !aligned16(a->workspace) || a->workspace_bytes < kCounterBytes + 2 * ctas * p.dim * 4)
+      if (a->workspace == nullptr || !aligned16(a->workspace) || a->workspace_bytes < kCounterBytes + 2 * ctas * line_floats(p.dim) * 4)
         return fail(B200_ATTN_BAD_CONFIG, "rotary: the gradient of the weights needs a workspace (b200_rotary_workspace)");
       p.counter = static_cast<uint32_t*>(a->workspace);
       p.partial = reinterpret_cast<float*>(static_cast<char*>(a->workspace) + kCounterBytes);

@@ -38,7 +38,6 @@ struct RotaryParams {
   uint32_t all_tokens;  // batch * tokens
   int table_rows, tokens, dim, rot, tensors;
   int lanes_log2, steps_log2[2];      // lanes of a row; rows of a token that are worked on at once, for each tensor
-  int chunks[2];                      // of as many tokens as a CTA works on at once
   bool interleaved, w_f32, vec;       // vec: every row of every tensor is 16-byte aligned
   float eps, inv_dim, sign;           // sign: -1 turns back
   float* partial;                // norm, backward: [2][CTAs][dim]
@@ -302,6 +301,8 @@ struct RotaryStream {
   static constexpr int kBytes = kDepth * kSlot;
 };
 
+__host__ __device__ constexpr int line_floats(int dim) { return (dim + 3) & ~3; }
+
 // Sums for dw: the lanes' own of tensor k go to this CTA's line of `partial`. A lane's places are a .. a + 7 and b .. b + 7.
 __device__ __forceinline__ void put_sums(const RotaryParams& p, float* dw, float* smem, int k, int a, int b, bool place) {
   // Lanes with the same place: within a warp by shuffles, then over the warps through shared memory.
@@ -322,12 +323,12 @@ __device__ __forceinline__ void put_sums(const RotaryParams& p, float* dw, float
     float v = 0.f;
 #pragma unroll
     for (int i = 0; i < kRotaryThreads / 32; ++i) v += smem[i * p.dim + e];
-    p.partial[(static_cast<int64_t>(k) * gridDim.x + blockIdx.x) * p.dim + e] = v;
+    p.partial[(static_cast<int64_t>(k) * gridDim.x + blockIdx.x) * line_floats(p.dim) + e] = v;
   }
   __syncthreads();
 }
 
-// The CTA that counts last adds all lines: eight warps take every eighth line each, and their sums are added in their order.
+// The CTA that counts last adds all lines: a thread takes four columns of every so-manieth line, and these sums are added in their order.
 template <typename T>
 __device__ __forceinline__ void join_sums(const RotaryParams& p, float* smem) {
   __shared__ uint32_t last;
@@ -337,33 +338,39 @@ __device__ __forceinline__ void join_sums(const RotaryParams& p, float* smem) {
   __syncthreads();
   if (last == 0) return;
   __threadfence();
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  for (int k = 0; k < p.tensors; ++k) {
-    const RotaryTensor& t = p.t[k];
-    if (t.dw == nullptr) continue;
-    const float* lines = p.partial + static_cast<int64_t>(k) * gridDim.x * p.dim;
-    for (int e = lane; e < p.dim; e += 32) {
-      float v = 0.f;
-#pragma unroll 16
-      for (uint32_t c = warp; c < gridDim.x; c += 8) v += __ldcg(lines + static_cast<int64_t>(c) * p.dim + e);
-      smem[warp * p.dim + e] = v;
-    }
-    __syncthreads();
-    for (int e = threadIdx.x; e < p.dim; e += kRotaryThreads) {
-      float v = 0.f;
+  const int quads = line_floats(p.dim) / 4, columns = 2 * quads, shares = kRotaryThreads / columns;  // both tensors' columns
+  const int share = threadIdx.x / columns, column = threadIdx.x - share * columns;
+  const int k = column >= quads ? 1 : 0;
+  float4* sums = reinterpret_cast<float4*>(smem);
+  if (share < shares && p.t[k].dw != nullptr) {
+    const float4* line = reinterpret_cast<const float4*>(p.partial) + static_cast<int64_t>(k) * gridDim.x * quads + (column - k * quads);
+    float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+    constexpr int kAtOnce = 16;  // loads in flight, the last ones too
+    for (uint32_t c = share; c < gridDim.x; c += kAtOnce * shares) {
+      float4 x[kAtOnce];
 #pragma unroll
-      for (int i = 0; i < 8; ++i) v += smem[i * p.dim + e];
-      if (p.w_f32) static_cast<float*>(t.dw)[e] = v;
-      else static_cast<T*>(t.dw)[e] = from_f32<T>(v);
+      for (int i = 0; i < kAtOnce; ++i) x[i] = c + i * shares < gridDim.x ? __ldcg(line + static_cast<int64_t>(c + i * shares) * quads) : make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+      for (int i = 0; i < kAtOnce; ++i) v.x += x[i].x, v.y += x[i].y, v.z += x[i].z, v.w += x[i].w;
     }
-    __syncthreads();
+    sums[threadIdx.x] = v;
+  }
+  __syncthreads();
+  for (int e = threadIdx.x; e < 2 * p.dim; e += kRotaryThreads) {
+    const int i = e >= p.dim ? 1 : 0, d = e - i * p.dim;
+    if (p.t[i].dw == nullptr) continue;
+    float v = 0.f;
+    for (int n = 0; n < shares; ++n) v += smem[(n * columns + i * quads) * 4 + d];
+    if (p.w_f32) static_cast<float*>(p.t[i].dw)[d] = v;
+    else static_cast<T*>(p.t[i].dw)[d] = from_f32<T>(v);
   }
   if (threadIdx.x == 0) *p.counter = 0;
 }
 
 // Rows of whole lanes on 16 bytes. A lane streams its rows through places of its own in shared memory, kDepth rows ahead, so that what is
-// in flight costs no registers; nobody else reads them, so nothing but its own copies has to be waited for. A CTA walks chunks of tokens
-// with the first tensor, then with the second (the weights, and backward the sums for dw, are one tensor's at a time).
+// in flight costs no registers; nobody else reads them, so nothing but its own copies has to be waited for. A CTA has an equal run of the
+// tokens, and walks it with the first tensor, then with the second (the weights, and backward the sums for dw, are one tensor's at a time);
+// its groups of lanes take a few heads each of a few tokens at once, and keep a token's cosines and sines for its heads.
 template <typename T, int FORM, int MODE>
 __global__ void __launch_bounds__(kRotaryThreads, RotaryStream<T, MODE>::kCtasPerSm) rotary_stream_kernel(const RotaryParams p) {
   using S = RotaryStream<T, MODE>;
@@ -374,25 +381,28 @@ __global__ void __launch_bounds__(kRotaryThreads, RotaryStream<T, MODE>::kCtasPe
   int a, b;
   lane_places<FORM>(j, p.rot, p.dim, &a, &b);
   const bool place = 16 * j < p.dim;
+  const uint32_t run_begin = static_cast<uint32_t>(static_cast<uint64_t>(p.all_tokens) * blockIdx.x / gridDim.x);
+  const uint32_t run_end = static_cast<uint32_t>(static_cast<uint64_t>(p.all_tokens) * (blockIdx.x + 1) / gridDim.x);
   uint4* mine = reinterpret_cast<uint4*>(rotary_smem) + threadIdx.x;
   const uint32_t mine_at = smem_u32(mine);
   for (int k = 0; k < p.tensors; ++k) {
     const RotaryTensor& t = p.t[k];
     const int step = 1 << p.steps_log2[k], first = group & (step - 1), heads = t.heads;
-    const uint32_t in_chunk = group >> p.steps_log2[k], chunk_tokens = kRotaryThreads >> (p.lanes_log2 + p.steps_log2[k]);
-    const int chunks = p.chunks[k];
+    const uint32_t at_once = kRotaryThreads >> (p.lanes_log2 + p.steps_log2[k]);  // tokens
+    const uint32_t token0 = run_begin + (group >> p.steps_log2[k]);
+    const uint32_t warp0 = run_begin + ((threadIdx.x & ~31) >> (p.lanes_log2 + p.steps_log2[k]));  // the warp's first
+    const int chunks = warp0 < run_end ? static_cast<int>((run_end - warp0 + at_once - 1) / at_once) : 0;
     float w[16], dw[16];
 #pragma unroll
     for (int i = 0; i < 16; ++i) w[i] = 1.f, dw[i] = 0.f;
     if (MODE != kTurn && place) load_weight<T, FORM>(w, p, t.w, a, b);
     // The place of the copies: a chunk of tokens, and the first of `step` heads in it.
-    int ahead = blockIdx.x, ahead_h = 0, slot = 0;
+    int ahead = 0, ahead_h = 0, slot = 0;
     bool ahead_there = false;
     const T *from_x = nullptr, *from_g = nullptr;
-    const auto token_of = [&](int chunk) { return chunk * chunk_tokens + in_chunk; };
     const auto enter = [&]() {
-      const uint32_t token = token_of(ahead);
-      ahead_there = ahead < chunks && place && token < p.all_tokens;
+      const uint32_t token = token0 + ahead * at_once;
+      ahead_there = ahead < chunks && place && token < run_end;
       if (!ahead_there) return;
       const uint32_t img = magic_div(token, p.tokens_magic), n = token - img * p.tokens;
       from_x = static_cast<const T*>(t.x) + img * t.xs[0] + n * t.xs[1] + first * t.xs[2];
@@ -416,7 +426,7 @@ __global__ void __launch_bounds__(kRotaryThreads, RotaryStream<T, MODE>::kCtasPe
         ahead_h += step;
         if (ahead_h >= heads) {
           ahead_h = 0;
-          ahead += gridDim.x;
+          ++ahead;
           enter();
         }
       }
@@ -427,14 +437,14 @@ __global__ void __launch_bounds__(kRotaryThreads, RotaryStream<T, MODE>::kCtasPe
 #pragma unroll
     for (int i = 0; i < S::kDepth - 1; ++i) copy();
     int use = 0;
-    for (int chunk = blockIdx.x; chunk < chunks; chunk += gridDim.x) {
-      const uint32_t token = token_of(chunk);
-      const bool there = place && token < p.all_tokens;
+    for (int chunk = 0; chunk < chunks; ++chunk) {  // the same for all lanes of a warp
+      const uint32_t token = token0 + chunk * at_once;
+      const bool there = place && token < run_end;
       const uint32_t img = there ? magic_div(token, p.tokens_magic) : 0, n = there ? token - img * p.tokens : 0;
       T* y = static_cast<T*>(t.y) + img * t.ys[0] + n * t.ys[1] + first * t.ys[2];
       Turns<FORM> turns;
       turns.load(there ? token_row(p, img, n) : nullptr, a, b, p.rot, MODE == kNormBack ? -1.f : p.sign);
-      for (int h0 = 0; h0 < heads; h0 += step) {  // the same for all lanes of a warp
+      for (int h0 = 0; h0 < heads; h0 += step) {
         copy();
         cp_async_wait<S::kDepth - 1>();
         const uint4* at = mine + use * (S::kSlot / 16);
@@ -529,8 +539,8 @@ __global__ void __launch_bounds__(kRotaryThreads, 2) rotary_any_kernel(const Rot
 #pragma unroll
     for (int i = 0; i < 16; ++i) w[i] = 1.f, dw[i] = 0.f;
     if (MODE != kTurn && place) load_weight<T, kRowAny>(w, p, t.w, a, b);
-    for (int chunk = blockIdx.x; chunk < p.chunks[k]; chunk += gridDim.x) {
-      const uint32_t token = chunk * chunk_tokens + in_chunk;
+    for (uint32_t token0 = blockIdx.x * chunk_tokens; token0 < p.all_tokens; token0 += gridDim.x * chunk_tokens) {
+      const uint32_t token = token0 + in_chunk;
       const bool there = place && token < p.all_tokens;
       const uint32_t img = there ? magic_div(token, p.tokens_magic) : 0, n = there ? token - img * p.tokens : 0;
       Turns<kRowAny> turns;
