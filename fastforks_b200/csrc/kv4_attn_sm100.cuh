@@ -66,7 +66,7 @@ struct Kv4AttnSmem {
   static constexpr int kMl = kQ + (kQInSmem ? RW * 32 * NR * D / 8 * 4 : 0);  // [4][8 NR] float2
   static constexpr int kBars = kMl + 4 * 8 * NR * 8;                        // full, empty
   static constexpr int kAhead = kBars + 2 * kTW * kKv4Stages * 8;           // [kTW] Kv4Ahead
-  static constexpr int kFlags = kAhead + kTW * 64;
+  static constexpr int kFlags = kAhead + kTW * 80;
   static constexpr int kBytes = kFlags + 16;
   static constexpr int kCtasPerSm = NR == 1 ? 4 : 3;
 };
@@ -109,13 +109,14 @@ struct Kv4Segment {
 };
 
 // The producer's place of a token warp, in shared memory: the segment it is in, its next step there and the end of those that are seen.
-struct Kv4Ahead {
+struct __align__(16) Kv4Ahead {
   Kv4Segment seg;
-  int s, end, more;
-  int at, in;  // the step that is issued next (-1: none) and its first block's place in its page
-  int pad[3];
+  int at, in, col, end;  // the step that is issued next (-1: none), its first block's place in its page, the page's column; the segment's end
+  const uint8_t* base;   // the head's blocks of page 0
+  const int32_t* pages;  // of the sequence
+  int two_end, pad[3];   // steps from here on have one block
 };
-static_assert(sizeof(Kv4Ahead) == 64, "Kv4AttnSmem::kFlags");
+static_assert(sizeof(Kv4Ahead) == 80, "Kv4AttnSmem::kFlags");
 
 __device__ __forceinline__ int kv4_length(const Kv4AttnParams& p, int b) {
   const int n = p.lengths[b], most = p.table_pages * p.page_blocks * kKv4Block;
@@ -248,63 +249,78 @@ __global__ void __launch_bounds__(kKv4AttnThreads, Kv4AttnSmem<D, NR, RW>::kCtas
   uint32_t issued = 0, used = 0;  // steps of this token warp, in order
   bool ok = true;
   const bool joined = (p.page_blocks & 1) == 0;  // the blocks of a step follow one another
+  const int64_t page_bytes = static_cast<int64_t>(p.kv_heads) * p.page_blocks * S::kBlock;
   int next_page[2] = {0, 0};
-  const auto fetch = [&]() {  // the next step and the pages of its blocks, so that their load is over when the step is issued
-    int at = ahead.s, end = ahead.end;
-    ahead.at = -1;
-    if (at >= end) {
-      if (ahead.more == 0) return;
-      Kv4Segment next = ahead.seg;
-      do {
-        if (!kv4_next(p, next)) {
-          ahead.more = 0;
-          return;
-        }
-        at = next.s0 + tw;
-        end = kv4_seen<kRows>(p, next);
-      } while (at >= end);
-      ahead.seg = next;
-      ahead.end = end;
-    }
-    ahead.s = at + kTW;
-    ahead.at = at;
-    const int32_t* pages = p.page_table + ahead.seg.b * p.table_stride;
-    const uint32_t col = magic_div(2 * at, p.bpp_magic);
-    ahead.in = 2 * at - static_cast<int>(col) * p.page_blocks;
+  // The pages of step `at` of the producer's segment, so that their load is over when the step is issued.
+  const auto fetch = [&](const int32_t* pages, int at, int in, int col, int two_end) {
     next_page[0] = pages[col];
-    if (!joined && at * kKv4Step + kKv4Block < ahead.seg.len) next_page[1] = pages[magic_div(2 * at + 1, p.bpp_magic)];
+    if (!joined && at < two_end) next_page[1] = pages[in + 1 == p.page_blocks ? col + 1 : col];
   };
+  const auto enter = [&](Kv4Segment next) {  // a segment of the producer's, or the first one behind it that has steps for this warp
+    int at = next.s0 + tw, end = kv4_seen<kRows>(p, next);
+    while (at >= end) {
+      if (!kv4_next(p, next)) {
+        ahead.at = -1;
+        return;
+      }
+      at = next.s0 + tw;
+      end = kv4_seen<kRows>(p, next);
+    }
+    ahead.seg = next;
+    ahead.at = at;
+    ahead.end = end;
+    ahead.col = static_cast<int>(magic_div(2 * at, p.bpp_magic));
+    ahead.in = 2 * at - ahead.col * p.page_blocks;
+    ahead.base = p.cache + static_cast<int64_t>(next.head) * p.page_blocks * S::kBlock;
+    ahead.pages = p.page_table + next.b * p.table_stride;
+    ahead.two_end = (next.len + kKv4Block - 1) / kKv4Step;
+    fetch(ahead.pages, at, ahead.in, ahead.col, ahead.two_end);
+  };
+  const int by_col = 2 * kTW / p.page_blocks, by_in = 2 * kTW - by_col * p.page_blocks;
   const auto issue = [&]() {
-    const int at = ahead.at, in = ahead.in;
+    const int at = ahead.at;
     if (at < 0) return;
+    int in = ahead.in, col = ahead.col;
+    const int end = ahead.end, two_end = ahead.two_end;
+    const uint8_t* base = ahead.base;
     const uint32_t stage = issued % kKv4Stages, round = issued / kKv4Stages;
     if (RW > 1 && round > 0 && !mbar_wait(empty + stage, (round - 1) & 1, abort_flag)) {
       ahead.at = -1;
       ok = false;
       return;
     }
-    const int head = ahead.seg.head;
     const auto block_at = [&](int page, int place) {
-      if (page < 0 || page >= p.pages) {
+      if (static_cast<uint32_t>(page) >= static_cast<uint32_t>(p.pages)) {
         atomicOr(p.status, kStatusPage);
         page = 0;
       }
-      return p.cache + ((static_cast<int64_t>(page) * p.kv_heads + head) * p.page_blocks + place) * S::kBlock;
+      return base + page * page_bytes + place * S::kBlock;
     };
-    const bool two = at * kKv4Step + kKv4Block < ahead.seg.len;  // the second block may hold nothing: what lies there is then masked
+    const bool two = at < two_end;  // the second block may hold nothing: what lies there is then masked
     uint8_t* to = ring + stage * 2 * S::kBlock;
     mbar_arrive_expect_tx(full + stage, two ? 2 * S::kBlock : S::kBlock);
     bulk_load(to, block_at(next_page[0], in), two && joined ? 2 * S::kBlock : S::kBlock, full + stage);
     if (two && !joined) bulk_load(to + S::kBlock, block_at(next_page[1], in + 1 == p.page_blocks ? 0 : in + 1), S::kBlock, full + stage);
     ++issued;
-    fetch();
+    if (at + kTW >= end) {
+      Kv4Segment next = ahead.seg;
+      if (kv4_next(p, next)) enter(next);
+      else ahead.at = -1;
+      return;
+    }
+    in += by_in;
+    col += by_col;
+    if (in >= p.page_blocks) {
+      in -= p.page_blocks;
+      ++col;
+    }
+    ahead.at = at + kTW;
+    ahead.in = in;
+    ahead.col = col;
+    fetch(ahead.pages, at + kTW, in, col, two_end);
   };
   if (producer && lane == 0) {
-    ahead.seg = seg;
-    ahead.s = seg.s0 + tw;
-    ahead.end = kv4_seen<kRows>(p, seg);
-    ahead.more = 1;
-    fetch();
+    enter(seg);
     for (int i = 0; i < kKv4Stages; ++i) issue();
   }
   __syncwarp();
@@ -707,22 +723,38 @@ __global__ void __launch_bounds__(kKv4AttnThreads, Kv4AttnSmem<D, NR, RW>::kCtas
         const int valid = min(kRows, p.rows - seg.tile * kRows);
         for (int u = threadIdx.x; u < valid * (D / 4); u += kKv4AttnThreads) {
           const int row = u / (D / 4), d = 4 * (u % (D / 4));
-          float most = -INFINITY;
-          for (int k = 0; k < parts; ++k) most = fmaxf(most, __ldcg(p.partial_ml + (static_cast<int64_t>(first + k) * 2 + (k == 0 ? 1 : 0)) * kRows + row).x);
-          float sum = 0.f;
+          // Parts eight at a time, all their loads in flight; the sums are brought to a new maximum when one comes along.
+          float most = -INFINITY, sum = 0.f;
           float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll 4
-          for (int k = 0; k < parts; ++k) {
-            const int64_t at = (static_cast<int64_t>(first + k) * 2 + (k == 0 ? 1 : 0)) * kRows + row;
-            const float2 v = __ldcg(p.partial_ml + at);
-            const float4 y = __ldcg(reinterpret_cast<const float4*>(p.partial + at * D + d));
-            const float by = v.x == -INFINITY ? v.y * 0.f : exp2_approx(v.x - most);
-            if (by != 0.f) {
-              sum = fmaf(by, v.y, sum);
-              acc.x = fmaf(by, y.x, acc.x);
-              acc.y = fmaf(by, y.y, acc.y);
-              acc.z = fmaf(by, y.z, acc.z);
-              acc.w = fmaf(by, y.w, acc.w);
+          constexpr int kAtOnce = 8;
+          for (int k0 = 0; k0 < parts; k0 += kAtOnce) {
+            float2 v[kAtOnce];
+            float4 y[kAtOnce];
+#pragma unroll
+            for (int i = 0; i < kAtOnce; ++i) {
+              const int k = min(k0 + i, parts - 1);
+              const int64_t at = (static_cast<int64_t>(first + k) * 2 + (k == 0 ? 1 : 0)) * kRows + row;
+              v[i] = __ldcg(p.partial_ml + at);
+              y[i] = __ldcg(reinterpret_cast<const float4*>(p.partial + at * D + d));
+              if (k0 + i >= parts) v[i] = make_float2(-INFINITY, 0.f);
+            }
+            float next = most;
+#pragma unroll
+            for (int i = 0; i < kAtOnce; ++i) next = fmaxf(next, v[i].x);
+            const float alpha = most == -INFINITY ? (sum == 0.f ? 0.f : 1.f) : exp2_approx(most - next);
+            most = next;
+            sum *= alpha;
+            acc.x *= alpha, acc.y *= alpha, acc.z *= alpha, acc.w *= alpha;
+#pragma unroll
+            for (int i = 0; i < kAtOnce; ++i) {
+              const float by = v[i].x == -INFINITY ? v[i].y * 0.f : exp2_approx(v[i].x - most);
+              if (by != 0.f) {
+                sum = fmaf(by, v[i].y, sum);
+                acc.x = fmaf(by, y[i].x, acc.x);
+                acc.y = fmaf(by, y[i].y, acc.y);
+                acc.z = fmaf(by, y[i].z, acc.z);
+                acc.w = fmaf(by, y[i].w, acc.w);
+              }
             }
           }
           const float inv = sum == 0.f ? 0.f : 1.f / sum;
