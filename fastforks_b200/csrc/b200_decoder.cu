@@ -296,7 +296,7 @@ int b200_kv4_read(const B200Kv4Args* a, void* stream_ptr) {
   if (int rc = device_state(&dev)) return rc;
   Kv4Params p{};
   set_cache(&p, a, dev);
-  p.heads = 2 * a->kv_heads;
+  p.heads = a->kv_heads;
   const int64_t rows = static_cast<int64_t>(a->batch) * a->tokens * p.heads;
   if (int rc = check_rows("kv4_read", rows)) return rc;
   p.rows = static_cast<uint32_t>(rows);

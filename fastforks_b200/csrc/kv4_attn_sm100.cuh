@@ -407,7 +407,8 @@ __global__ void __launch_bounds__(kKv4AttnThreads, Kv4AttnSmem<D, NR, RW>::kCtas
       const uint8_t* step = ring + stage * 2 * S::kBlock;
       const int base = s * kKv4Step;
       const bool masked = base + kKv4Step - 1 > lowest;
-      float x[2][NR][4];  // blocks; tokens r and r + 8, rows 2 c and 2 c + 1
+      constexpr int kChains = NR == 1 ? 2 : 1;  // sums of a logit, so that the products do not wait for one another (two tiles are two chains)
+      float x[2][NR][4], odd[2][NR][4];  // blocks; tokens r and r + 8, rows 2 c and 2 c + 1
       float vs[2][2], vl[2][2];
       {
         uint32_t w[2][2][kWords];
@@ -425,7 +426,10 @@ __global__ void __launch_bounds__(kKv4AttnThreads, Kv4AttnSmem<D, NR, RW>::kCtas
             }
           }
 #pragma unroll
-          for (int t = 0; t < NR; ++t) x[h][t][0] = x[h][t][1] = x[h][t][2] = x[h][t][3] = 0.f;
+          for (int t = 0; t < NR; ++t) {
+            x[h][t][0] = x[h][t][1] = x[h][t][2] = x[h][t][3] = 0.f;
+            odd[h][t][0] = odd[h][t][1] = odd[h][t][2] = odd[h][t][3] = 0.f;
+          }
         }
 #pragma unroll
         for (int i = 0; i < kWords; ++i) {
@@ -449,7 +453,7 @@ __global__ void __launch_bounds__(kKv4AttnThreads, Kv4AttnSmem<D, NR, RW>::kCtas
             for (int k = 0; k < 2; ++k) {
               const uint32_t a[4] = {u0[2 * k], u1[2 * k], u0[2 * k + 1], u1[2 * k + 1]};
 #pragma unroll
-              for (int t = 0; t < NR; ++t) mma_16816<__half>(x[h][t], a, q[t][2 * k], q[t][2 * k + 1]);
+              for (int t = 0; t < NR; ++t) mma_16816<__half>(k == 0 || kChains == 1 ? x[h][t] : odd[h][t], a, q[t][2 * k], q[t][2 * k + 1]);
             }
           }
         }
@@ -466,7 +470,7 @@ __global__ void __launch_bounds__(kKv4AttnThreads, Kv4AttnSmem<D, NR, RW>::kCtas
 #pragma unroll
           for (int t = 0; t < NR; ++t) {
 #pragma unroll
-            for (int i = 0; i < 2; ++i) x[h][t][2 * k + i] = fmaf(ks, x[h][t][2 * k + i], kl * qsum[t][i]);
+            for (int i = 0; i < 2; ++i) x[h][t][2 * k + i] = fmaf(ks, kChains == 1 ? x[h][t][2 * k + i] : x[h][t][2 * k + i] + odd[h][t][2 * k + i], kl * qsum[t][i]);
           }
         }
       }

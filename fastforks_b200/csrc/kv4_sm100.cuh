@@ -93,11 +93,18 @@ __device__ __forceinline__ uint32_t quantise16(const float* f, uint32_t* words) 
   if (step < 1.17549435e-38f) {
     step = 0.f;
   } else {
+    // A code between 0 and 15 is rounded to even by adding 1.5 * 2^23; four of them make a word of 16 bits, exact as a float.
+    constexpr float kWhole = 12582912.f, kWord = 8388608.f;
     const float inverse = __frcp_rn(step);
 #pragma unroll
-    for (int i = 0; i < 16; ++i) {
-      const float t = fminf(fmaxf(rintf(__fmul_rn(__fsub_rn(f[i], least), inverse)), 0.f), 15.f);
-      words[i >> 3] |= static_cast<uint32_t>(t) << (4 * (i & 7));
+    for (int h = 0; h < 4; ++h) {
+      float word = kWord;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const float t = fminf(fmaxf(__fmul_rn(__fsub_rn(f[4 * h + i], least), inverse), 0.f), 15.f);
+        word = fmaf(__fsub_rn(__fadd_rn(t, kWhole), kWhole), static_cast<float>(1 << (4 * i)), word);
+      }
+      words[h >> 1] |= (__float_as_uint(word) & 0xffffu) << (16 * (h & 1));
     }
   }
   return (__float_as_uint(step) >> 16) | (__float_as_uint(least) & 0xffff0000u);
@@ -136,8 +143,8 @@ __global__ void __launch_bounds__(kKv4Threads) kv4_append_kernel(const Kv4Params
   Turns<FORM> turns;
   turns.load(cs, at0, at1, p.rot, 1.f);
   rotate16<FORM>(f, turns, D, p.interleaved, rows_smem + (FORM == kRowAny ? group * D : 0));
-  uint32_t words[2];
-  const uint32_t pair = quantise16<kLanes>(f, words);
+  uint32_t words[2], pair = 0;
+  if (__any_sync(0xffffffffu, what != 0)) pair = quantise16<kLanes>(f, words);
   if (!there) return;
   if (what == 0) {
     T* y = static_cast<T*>(p.q_out) + b * p.qos[0] + n * p.qos[1] + h * p.qos[2];
@@ -162,7 +169,7 @@ __global__ void __launch_bounds__(kKv4Threads) kv4_append_kernel(const Kv4Params
   if (j == 0) *reinterpret_cast<uint32_t*>(tail + D + (t & 1) * 8 + (what == 2 ? 4 : 0)) = pair;
 }
 
-// The values of the last tokens, in 16 bits.
+// The values of the last tokens, in 16 bits: K and V of a head of one token by one group of lanes, whose places they share.
 template <typename T, int D>
 __global__ void __launch_bounds__(kKv4Threads) kv4_read_kernel(const Kv4Params p) {
   constexpr int kLanes = D / 16, kGroups = kKv4Threads / kLanes;
@@ -173,38 +180,37 @@ __global__ void __launch_bounds__(kKv4Threads) kv4_read_kernel(const Kv4Params p
   const uint32_t row = blockIdx.x * kGroups + threadIdx.x / kLanes;
   if (row >= p.rows) return;
   const uint32_t token = magic_div(row, p.heads_magic);
-  int h = static_cast<int>(row - token * p.heads);
-  const bool is_v = h >= p.kv_heads;
-  if (is_v) h -= p.kv_heads;
+  const int h = static_cast<int>(row - token * p.heads);
   const uint32_t b = magic_div(token, p.tokens_magic), n = token - b * p.tokens;
   const int at = p.lengths[b] - p.tokens + static_cast<int>(n);
-  float f[16];
-#pragma unroll
-  for (int i = 0; i < 16; ++i) f[i] = 0.f;
   int t = 0;
   const uint8_t* block = at < 0 ? nullptr : kv4_block<D>(p, b, at, h, &t);
+  uint32_t words[4] = {0, 0, 0, 0};
+  uint2 pairs = make_uint2(0, 0);
   if (block != nullptr) {
     const uint8_t* tail = block + L::kV + (t >> 1) * L::kRowV;
-    uint32_t words[2];
-    if (!is_v) {
-      const uint2 w = *reinterpret_cast<const uint2*>(block + t * L::kRowK + 8 * j);
-      words[0] = w.x;
-      words[1] = w.y;
-    } else {
-      const uint4 w = *reinterpret_cast<const uint4*>(tail + 16 * j);
-      const int low = t & 1 ? 0x7632 : 0x5410;  // this token's half of either word
-      words[0] = __byte_perm(w.x, w.y, low);
-      words[1] = __byte_perm(w.z, w.w, low);
-    }
-    const uint32_t pair = *reinterpret_cast<const uint32_t*>(tail + D + (t & 1) * 8 + (is_v ? 4 : 0));
-    const float step = __uint_as_float(pair << 16), least = __uint_as_float(pair & 0xffff0000u);
-#pragma unroll
-    for (int i = 0; i < 16; ++i) f[i] = fmaf(step, static_cast<float>((words[i >> 3] >> (4 * (i & 7))) & 15u), least);  // the product is exact
+    const uint2 k = *reinterpret_cast<const uint2*>(block + t * L::kRowK + 8 * j);
+    const uint4 v = *reinterpret_cast<const uint4*>(tail + 16 * j);
+    pairs = *reinterpret_cast<const uint2*>(tail + D + (t & 1) * 8);
+    const int half = t & 1 ? 0x7632 : 0x5410;  // this token's half of either word
+    words[0] = k.x;
+    words[1] = k.y;
+    words[2] = __byte_perm(v.x, v.y, half);
+    words[3] = __byte_perm(v.z, v.w, half);
   }
-  const int64_t* s = is_v ? p.vos : p.kos;
-  T* y = static_cast<T*>(is_v ? p.v_out : p.k_out) + b * s[0] + n * s[1] + h * s[2] + 16 * j;
-  store8<T>(y, f);
-  store8<T>(y + 8, f + 8);
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    const uint32_t pair = i == 0 ? pairs.x : pairs.y;
+    const float step = __uint_as_float(pair << 16), least = __uint_as_float(pair & 0xffff0000u);
+    T* y = static_cast<T*>(i == 0 ? p.k_out : p.v_out) + (i == 0 ? b * p.kos[0] + n * p.kos[1] + h * p.kos[2] : b * p.vos[0] + n * p.vos[1] + h * p.vos[2]) + 16 * j;
+#pragma unroll
+    for (int w = 0; w < 2; ++w) {
+      float f[8];
+#pragma unroll
+      for (int k = 0; k < 8; ++k) f[k] = fmaf(step, static_cast<float>((words[2 * i + w] >> (4 * k)) & 15u), least);  // the product is exact
+      store8<T>(y + 8 * w, f);
+    }
+  }
 }
 
 }  // namespace b200
