@@ -46,6 +46,7 @@ HEADERS = (
     PACKAGE_DIR / "csrc" / "rotary_sm100.cuh",
     PACKAGE_DIR / "csrc" / "kv4_sm100.cuh",
     PACKAGE_DIR / "csrc" / "kv4_attn_sm100.cuh",
+    PACKAGE_DIR / "csrc" / "kv4_tiles_sm100.cuh",
     PACKAGE_DIR.parent / "include" / "b200_attn.h",
     PACKAGE_DIR.parent / "include" / "b200_encoder.h",
     PACKAGE_DIR.parent / "include" / "b200_decoder.h",

@@ -9,6 +9,7 @@
 #include "host_common.h"
 #include "kv4_attn_sm100.cuh"
 #include "kv4_sm100.cuh"
+#include "kv4_tiles_sm100.cuh"
 #include "rotary_sm100.cuh"
 
 namespace b200 {
@@ -113,16 +114,18 @@ const void* append_kernel_of(int form) {
 
 struct AttnForm {
   const void* kernel;
-  int smem, rows, ctas_per_sm;
+  int smem, rows, ctas_per_sm, threads, step, item;
 };
-constexpr int kAttnForms = 4;
+constexpr int kTileRowsLeast = 96;
+constexpr int kAttnForms = 5, kTileForm = 4;
 template <typename T, int D, int NR, int RW>
 AttnForm attn_form() {
   using S = Kv4AttnSmem<D, NR, RW>;
-  return {reinterpret_cast<const void*>(kv4_attn_kernel<T, D, NR, RW>), S::kBytes, 8 * NR * RW, S::kCtasPerSm};
+  return {reinterpret_cast<const void*>(kv4_attn_kernel<T, D, NR, RW>), S::kBytes, 8 * NR * RW, S::kCtasPerSm, kKv4AttnThreads, kKv4Step, kKv4Item};
 }
 template <typename T, int D>
 AttnForm attn_form_of(int form) {
+  if (form == kTileForm) return {reinterpret_cast<const void*>(kv4_tiles_kernel<T, D>), Kv4TilesSmem<D>::kBytes, kKv4TileRows, 1, kKv4TileThreads, kKv4TileStep, kKv4TileItem};
   return form == 0 ? attn_form<T, D, 1, 1>() : form == 1 ? attn_form<T, D, 2, 1>() : form == 2 ? attn_form<T, D, 2, 2>() : attn_form<T, D, 2, 4>();
 }
 std::atomic<bool> g_attn_opted_in[kMaxDevices][2][2][kAttnForms];
@@ -318,9 +321,9 @@ int b200_kv4_workspace(int64_t* bytes, int64_t* counter_words) {
   if (bytes == nullptr || counter_words == nullptr) return fail(B200_ATTN_BAD_CONFIG, "bytes or counter_words is NULL");
   DeviceState* dev = nullptr;
   if (int rc = device_state(&dev)) return rc;
-  const int64_t ctas = static_cast<int64_t>(dev->sms) * kKv4CtasPerSm;
-  *bytes = ctas * 2 * kKv4MaxRows * (128 * 4 + 8);
-  *counter_words = ctas;
+  const int64_t most_rows = std::max(kKv4CtasPerSm * kKv4MaxRows, kKv4TileRows);  // of the CTAs of one SM
+  *bytes = dev->sms * 2 * most_rows * (128 * 4 + 8);
+  *counter_words = static_cast<int64_t>(dev->sms) * kKv4CtasPerSm;
   clear_error();
   return B200_ATTN_OK;
 }
@@ -338,7 +341,7 @@ int b200_kv4_attention(const B200Kv4AttnArgs* a, void* stream_ptr) {
   const int group = a->q_heads / a->kv_heads;
   const int64_t rows = static_cast<int64_t>(a->queries) * group;
   if (int rc = check_rows("kv4_attention", rows * a->kv_heads * a->batch)) return rc;
-  const int which = rows <= 8 ? 0 : rows <= 16 ? 1 : rows <= 32 ? 2 : 3;
+  const int which = rows <= 8 ? 0 : rows <= 16 ? 1 : rows <= 32 ? 2 : rows < kTileRowsLeast ? 3 : kTileForm;
   const bool f16 = a->dtype == B200_ATTN_F16;
   const AttnForm form = a->head_dim == 64 ? (f16 ? attn_form_of<__half, 64>(which) : attn_form_of<__nv_bfloat16, 64>(which)) : (f16 ? attn_form_of<__half, 128>(which) : attn_form_of<__nv_bfloat16, 128>(which));
   Kv4AttnParams p{};
@@ -364,9 +367,9 @@ int b200_kv4_attention(const B200Kv4AttnArgs* a, void* stream_ptr) {
   p.table_pages = a->table_pages;
   p.status = dev->status;
   // The lengths are on the device: the grid is for the longest that the page table allows, CTAs without a run leave at once.
-  p.min_run = 4 + kKv4Item;
-  const int64_t most = static_cast<int64_t>(a->batch) * p.row_tiles * a->kv_heads * ((static_cast<int64_t>(a->table_pages) * a->page + kKv4Step - 1) / kKv4Step + kKv4Item);
-  if (most >= (int64_t(1) << 38)) return fail(B200_ATTN_UNSUPPORTED, "kv4_attention: %lld steps of 32 tokens and items, at most 2^38 a call", static_cast<long long>(most));
+  p.min_run = (which == kTileForm ? 2 : 4) + form.item;
+  const int64_t most = static_cast<int64_t>(a->batch) * p.row_tiles * a->kv_heads * ((static_cast<int64_t>(a->table_pages) * a->page + form.step - 1) / form.step + form.item);
+  if (most >= (int64_t(1) << 38)) return fail(B200_ATTN_UNSUPPORTED, "kv4_attention: %lld steps and items, at most 2^38 a call", static_cast<long long>(most));
   const int64_t ctas = std::min<int64_t>(static_cast<int64_t>(dev->sms) * form.ctas_per_sm, (most + p.min_run - 1) / p.min_run);
   const int64_t partial = ctas * 2 * form.rows * a->head_dim * 4, ml = ctas * 2 * form.rows * 8;
   if (a->workspace == nullptr || !aligned16(a->workspace) || a->workspace_bytes < partial + ml || a->counters == nullptr || a->counter_words < ctas)
@@ -378,7 +381,7 @@ int b200_kv4_attention(const B200Kv4AttnArgs* a, void* stream_ptr) {
   if (int rc = current_device(&device)) return rc;
   if (int rc = opt_in(g_attn_opted_in[device][f16 ? 0 : 1][a->head_dim == 64 ? 0 : 1][which], form.kernel, form.smem, "kv4_attention: shared memory opt-in")) return rc;
   void* args[] = {&p};
-  if (int rc = launch_kernel(form.kernel, static_cast<unsigned>(ctas), 1, kKv4AttnThreads, form.smem, 1, static_cast<cudaStream_t>(stream_ptr), args, "kv4_attention kernel launch")) return rc;
+  if (int rc = launch_kernel(form.kernel, static_cast<unsigned>(ctas), 1, form.threads, form.smem, 1, static_cast<cudaStream_t>(stream_ptr), args, "kv4_attention kernel launch")) return rc;
   clear_error();
   return B200_ATTN_OK;
 }

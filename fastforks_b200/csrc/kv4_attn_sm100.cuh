@@ -123,9 +123,10 @@ __device__ __forceinline__ int kv4_length(const Kv4AttnParams& p, int b) {
   return n < 0 ? 0 : n > most ? most : n;
 }
 
-// The next segment of the run, if there is one.
+// The next segment of the run, if there is one. STEP: tokens of a step, ITEM: units of the line in front of an item's first step.
+template <int STEP, int ITEM>
 __device__ __forceinline__ bool kv4_next(const Kv4AttnParams& p, Kv4Segment& s) {
-  if (s.left <= kKv4Item) return false;
+  if (s.left <= ITEM) return false;
   if (++s.head == p.kv_heads) {
     s.head = 0;
     if (++s.tile == p.row_tiles) {
@@ -134,21 +135,130 @@ __device__ __forceinline__ bool kv4_next(const Kv4AttnParams& p, Kv4Segment& s) 
         if (++s.b >= p.batch) return false;
         s.len = kv4_length(p, s.b);
       } while (s.len == 0);
-      s.steps = (s.len + kKv4Step - 1) / kKv4Step;
+      s.steps = (s.len + STEP - 1) / STEP;
     }
   }
   s.s0 = 0;
-  s.s1 = min(s.steps, s.left - kKv4Item);
-  s.left -= s.s1 + kKv4Item;
+  s.s1 = min(s.steps, s.left - ITEM);
+  s.left -= s.s1 + ITEM;
   return true;
 }
 
 // Steps of the segment that some row of its tile sees: [s0, result).
-template <int ROWS>
+template <int ROWS, int STEP>
 __device__ __forceinline__ int kv4_seen(const Kv4AttnParams& p, const Kv4Segment& s) {
   const int last = min(p.rows, (s.tile + 1) * ROWS) - 1;
   const int limit = s.len - p.queries + static_cast<int>(magic_div(last, p.group_magic)) + 1;
-  return max(s.s0, min(s.s1, (limit + kKv4Step - 1) / kKv4Step));
+  return max(s.s0, min(s.s1, (limit + STEP - 1) / STEP));
+}
+
+// This CTA's run of the line and its first segment; false: it has none. For all lanes of each warp.
+template <int STEP, int ITEM>
+__device__ __forceinline__ bool kv4_start(const Kv4AttnParams& p, int* run, int* count, Kv4Segment* seg) {
+  const int lane = threadIdx.x & 31, per = p.kv_heads * p.row_tiles;
+  long long total = 0;
+  for (int b = lane; b < p.batch; b += 32) {
+    const int n = p.lengths[b], len = kv4_length(p, b);
+    if (n != len && n > 0 && threadIdx.x < 32 && blockIdx.x == 0) atomicOr(p.status, kStatusPage);
+    total += len == 0 ? 0 : (len + STEP - 1) / STEP + ITEM;
+  }
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) total += __shfl_xor_sync(0xffffffffu, total, o);
+  total *= per;
+  *run = static_cast<int>(max(static_cast<long long>(p.min_run), (total + gridDim.x - 1) / gridDim.x));
+  const long long begin = static_cast<long long>(*run) * blockIdx.x;
+  *count = static_cast<int>(max(0ll, min(static_cast<long long>(*run), total - begin)));
+  if (*count == 0) return false;
+  // The sequence the run begins in: 32 lengths at a time.
+  long long before = 0;
+  for (int b0 = 0;; b0 += 32) {
+    const int b = b0 + lane;
+    const int len = b < p.batch ? kv4_length(p, b) : 0, units = len == 0 ? 0 : (len + STEP - 1) / STEP + ITEM;
+    long long sum = static_cast<long long>(units) * per;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const long long v = __shfl_up_sync(0xffffffffu, sum, o);
+      if (lane >= o) sum += v;
+    }
+    const uint32_t hit = __ballot_sync(0xffffffffu, before + sum > begin);
+    if (hit != 0) {  // always, at the latest with the last sequence: begin < total
+      const int l = __ffs(hit) - 1;
+      seg->b = b0 + l;
+      seg->steps = __shfl_sync(0xffffffffu, units, l) - ITEM;
+      before += __shfl_sync(0xffffffffu, sum, l) - static_cast<long long>(seg->steps + ITEM) * per;
+      break;
+    }
+    before += __shfl_sync(0xffffffffu, sum, 31);
+    if (b0 + 32 >= p.batch) return false;
+  }
+  seg->len = kv4_length(p, seg->b);
+  const long long in = begin - before;
+  const int item = static_cast<int>(in / (seg->steps + ITEM)), at = static_cast<int>(in - static_cast<long long>(item) * (seg->steps + ITEM));
+  seg->tile = item / p.kv_heads;
+  seg->head = item - seg->tile * p.kv_heads;
+  seg->s0 = max(0, at - ITEM);
+  seg->s1 = max(seg->s0, min(seg->steps, at - ITEM + *count));
+  seg->left = *count - (seg->s1 + ITEM - at);
+  return seg->s1 > seg->s0;  // else the run ends in front of the item's first step
+}
+
+// Rows of sequences without tokens are on no CTA's run: they are zeros.
+template <typename T, int D>
+__device__ __forceinline__ void write_unseen(const Kv4AttnParams& p, int threads) {
+  for (int b = blockIdx.x; b < p.batch; b += gridDim.x) {
+    if (kv4_length(p, b) != 0) continue;
+    for (int i = threadIdx.x; i < p.queries * p.q_heads * (D / 8); i += threads) {
+      const int d = i % (D / 8), h = i / (D / 8) % p.q_heads, n = i / (D / 8) / p.q_heads;
+      *reinterpret_cast<uint4*>(static_cast<T*>(p.o) + b * p.os[0] + n * p.os[1] + h * p.os[2] + 8 * d) = make_uint4(0, 0, 0, 0);
+    }
+  }
+}
+
+// Joins the parts of an item, which begins with CTA `first`, and writes its rows.
+template <typename T, int D>
+__device__ __forceinline__ void join_parts(const Kv4AttnParams& p, const Kv4Segment& seg, int rows, int first, int parts, int thread, int threads) {
+  const int valid = min(rows, p.rows - seg.tile * rows);
+  for (int u = thread; u < valid * (D / 4); u += threads) {
+    const int row = u / (D / 4), d = 4 * (u % (D / 4));
+    // Parts eight at a time, all their loads in flight; the sums are brought to a new maximum when one comes along.
+    float most = -INFINITY, sum = 0.f;
+    float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+    constexpr int kAtOnce = 8;
+    for (int k0 = 0; k0 < parts; k0 += kAtOnce) {
+      float2 v[kAtOnce];
+      float4 y[kAtOnce];
+#pragma unroll
+      for (int i = 0; i < kAtOnce; ++i) {
+        const int k = min(k0 + i, parts - 1);
+        const int64_t at = (static_cast<int64_t>(first + k) * 2 + (k == 0 ? 1 : 0)) * rows + row;
+        v[i] = __ldcg(p.partial_ml + at);
+        y[i] = __ldcg(reinterpret_cast<const float4*>(p.partial + at * D + d));
+        if (k0 + i >= parts) v[i] = make_float2(-INFINITY, 0.f);
+      }
+      float next = most;
+#pragma unroll
+      for (int i = 0; i < kAtOnce; ++i) next = fmaxf(next, v[i].x);
+      const float alpha = most == -INFINITY ? (sum == 0.f ? 0.f : 1.f) : exp2_approx(most - next);
+      most = next;
+      sum *= alpha;
+      acc.x *= alpha, acc.y *= alpha, acc.z *= alpha, acc.w *= alpha;
+#pragma unroll
+      for (int i = 0; i < kAtOnce; ++i) {
+        const float by = v[i].x == -INFINITY ? v[i].y * 0.f : exp2_approx(v[i].x - most);
+        if (by != 0.f) {
+          sum = fmaf(by, v[i].y, sum);
+          acc.x = fmaf(by, y[i].x, acc.x);
+          acc.y = fmaf(by, y[i].y, acc.y);
+          acc.z = fmaf(by, y[i].z, acc.z);
+          acc.w = fmaf(by, y[i].w, acc.w);
+        }
+      }
+    }
+    const float inv = sum == 0.f ? 0.f : 1.f / sum;
+    const int at = seg.tile * rows + row, n = static_cast<int>(magic_div(at, p.group_magic)), head = seg.head * p.group + at - n * p.group;
+    T* y = static_cast<T*>(p.o) + seg.b * p.os[0] + n * p.os[1] + head * p.os[2] + d;
+    *reinterpret_cast<uint2*>(y) = make_uint2(pack2<T>(acc.x * inv, acc.y * inv), pack2<T>(acc.z * inv, acc.w * inv));
+  }
 }
 
 template <typename T, int D, int NR, int RW>
@@ -178,70 +288,10 @@ __global__ void __launch_bounds__(kKv4AttnThreads, Kv4AttnSmem<D, NR, RW>::kCtas
   grid_dependency_wait();
   grid_launch_dependents();
 
-  // The line: units of all items, and this CTA's run of it.
-  const int per = p.kv_heads * p.row_tiles;
-  long long total = 0;
-  {
-    long long mine = 0;
-    for (int b = lane; b < p.batch; b += 32) {
-      const int n = p.lengths[b], len = kv4_length(p, b);
-      if (n != len && n > 0 && threadIdx.x < 32 && blockIdx.x == 0) atomicOr(p.status, kStatusPage);
-      mine += len == 0 ? 0 : (len + kKv4Step - 1) / kKv4Step + kKv4Item;
-    }
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) mine += __shfl_xor_sync(0xffffffffu, mine, o);
-    total = mine * per;
-  }
-  const int run = static_cast<int>(max(static_cast<long long>(p.min_run), (total + gridDim.x - 1) / gridDim.x));
-  const long long begin = static_cast<long long>(run) * blockIdx.x;
-  const int count = static_cast<int>(max(0ll, min(static_cast<long long>(run), total - begin)));
-
-  // Rows that see nothing at all get zeros: whole sequences without tokens are on no CTA's run, and rows in front of a sequence's start
-  // are written by whoever has their item.
-  for (int b = blockIdx.x; b < p.batch; b += gridDim.x) {
-    if (kv4_length(p, b) != 0) continue;
-    for (int i = threadIdx.x; i < p.queries * p.q_heads * (D / 8); i += kKv4AttnThreads) {
-      const int d = i % (D / 8), h = i / (D / 8) % p.q_heads, n = i / (D / 8) / p.q_heads;
-      *reinterpret_cast<uint4*>(static_cast<T*>(p.o) + b * p.os[0] + n * p.os[1] + h * p.os[2] + 8 * d) = make_uint4(0, 0, 0, 0);
-    }
-  }
-  if (count == 0) return;
-
+  write_unseen<T, D>(p, kKv4AttnThreads);
+  int run, count;
   Kv4Segment seg{};
-  {
-    // The sequence the run begins in: 32 lengths at a time.
-    long long before = 0;
-    int b0 = 0;
-    for (;; b0 += 32) {
-      const int b = b0 + lane;
-      const int len = b < p.batch ? kv4_length(p, b) : 0, units = len == 0 ? 0 : (len + kKv4Step - 1) / kKv4Step + kKv4Item;
-      long long sum = static_cast<long long>(units) * per;
-#pragma unroll
-      for (int o = 1; o < 32; o <<= 1) {
-        const long long v = __shfl_up_sync(0xffffffffu, sum, o);
-        if (lane >= o) sum += v;
-      }
-      const uint32_t hit = __ballot_sync(0xffffffffu, before + sum > begin);
-      if (hit != 0) {  // always, at the latest with the last sequence: begin < total
-        const int l = __ffs(hit) - 1;
-        seg.b = b0 + l;
-        seg.steps = __shfl_sync(0xffffffffu, units, l) - kKv4Item;
-        before += __shfl_sync(0xffffffffu, sum, l) - static_cast<long long>(seg.steps + kKv4Item) * per;
-        break;
-      }
-      before += __shfl_sync(0xffffffffu, sum, 31);
-      if (b0 + 32 >= p.batch) return;
-    }
-    seg.len = kv4_length(p, seg.b);
-    const long long in = begin - before;
-    const int item = static_cast<int>(in / (seg.steps + kKv4Item)), at = static_cast<int>(in - static_cast<long long>(item) * (seg.steps + kKv4Item));
-    seg.tile = item / p.kv_heads;
-    seg.head = item - seg.tile * p.kv_heads;
-    seg.s0 = max(0, at - kKv4Item);
-    seg.s1 = max(seg.s0, min(seg.steps, at - kKv4Item + count));
-    seg.left = count - (seg.s1 + kKv4Item - at);
-    if (seg.s1 == seg.s0) return;  // the run ends in front of the item's first step
-  }
+  if (!kv4_start<kKv4Step, kKv4Item>(p, &run, &count, &seg)) return;
 
   // The producer runs kKv4Stages steps ahead, over the ends of items: lane 0 of the first row warp of each token warp.
   const bool producer = rw == 0;
@@ -257,14 +307,14 @@ __global__ void __launch_bounds__(kKv4AttnThreads, Kv4AttnSmem<D, NR, RW>::kCtas
     if (!joined && at < two_end) next_page[1] = pages[in + 1 == p.page_blocks ? col + 1 : col];
   };
   const auto enter = [&](Kv4Segment next) {  // a segment of the producer's, or the first one behind it that has steps for this warp
-    int at = next.s0 + tw, end = kv4_seen<kRows>(p, next);
+    int at = next.s0 + tw, end = kv4_seen<kRows, kKv4Step>(p, next);
     while (at >= end) {
-      if (!kv4_next(p, next)) {
+      if (!kv4_next<kKv4Step, kKv4Item>(p, next)) {
         ahead.at = -1;
         return;
       }
       at = next.s0 + tw;
-      end = kv4_seen<kRows>(p, next);
+      end = kv4_seen<kRows, kKv4Step>(p, next);
     }
     ahead.seg = next;
     ahead.at = at;
@@ -304,7 +354,7 @@ __global__ void __launch_bounds__(kKv4AttnThreads, Kv4AttnSmem<D, NR, RW>::kCtas
     ++issued;
     if (at + kTW >= end) {
       Kv4Segment next = ahead.seg;
-      if (kv4_next(p, next)) enter(next);
+      if (kv4_next<kKv4Step, kKv4Item>(p, next)) enter(next);
       else ahead.at = -1;
       return;
     }
@@ -399,7 +449,7 @@ __global__ void __launch_bounds__(kKv4AttnThreads, Kv4AttnSmem<D, NR, RW>::kCtas
     float vscale = 0.f;  // 2^(6 - vexp); 0: no step seen yet
     float vlimit = 0.f;  // steps from here on need a larger vexp
 
-    const int seen = kv4_seen<kRows>(p, seg);
+    const int seen = kv4_seen<kRows, kKv4Step>(p, seg);
 #pragma unroll 1
     for (int s = seg.s0 + tw; s < seen; s += kTW) {
       const uint32_t stage = used % kKv4Stages, round = used / kKv4Stages;
@@ -724,54 +774,13 @@ __global__ void __launch_bounds__(kKv4AttnThreads, Kv4AttnSmem<D, NR, RW>::kCtas
       __syncthreads();
       if (*last_flag != 0) {
         __threadfence();
-        const int valid = min(kRows, p.rows - seg.tile * kRows);
-        for (int u = threadIdx.x; u < valid * (D / 4); u += kKv4AttnThreads) {
-          const int row = u / (D / 4), d = 4 * (u % (D / 4));
-          // Parts eight at a time, all their loads in flight; the sums are brought to a new maximum when one comes along.
-          float most = -INFINITY, sum = 0.f;
-          float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-          constexpr int kAtOnce = 8;
-          for (int k0 = 0; k0 < parts; k0 += kAtOnce) {
-            float2 v[kAtOnce];
-            float4 y[kAtOnce];
-#pragma unroll
-            for (int i = 0; i < kAtOnce; ++i) {
-              const int k = min(k0 + i, parts - 1);
-              const int64_t at = (static_cast<int64_t>(first + k) * 2 + (k == 0 ? 1 : 0)) * kRows + row;
-              v[i] = __ldcg(p.partial_ml + at);
-              y[i] = __ldcg(reinterpret_cast<const float4*>(p.partial + at * D + d));
-              if (k0 + i >= parts) v[i] = make_float2(-INFINITY, 0.f);
-            }
-            float next = most;
-#pragma unroll
-            for (int i = 0; i < kAtOnce; ++i) next = fmaxf(next, v[i].x);
-            const float alpha = most == -INFINITY ? (sum == 0.f ? 0.f : 1.f) : exp2_approx(most - next);
-            most = next;
-            sum *= alpha;
-            acc.x *= alpha, acc.y *= alpha, acc.z *= alpha, acc.w *= alpha;
-#pragma unroll
-            for (int i = 0; i < kAtOnce; ++i) {
-              const float by = v[i].x == -INFINITY ? v[i].y * 0.f : exp2_approx(v[i].x - most);
-              if (by != 0.f) {
-                sum = fmaf(by, v[i].y, sum);
-                acc.x = fmaf(by, y[i].x, acc.x);
-                acc.y = fmaf(by, y[i].y, acc.y);
-                acc.z = fmaf(by, y[i].z, acc.z);
-                acc.w = fmaf(by, y[i].w, acc.w);
-              }
-            }
-          }
-          const float inv = sum == 0.f ? 0.f : 1.f / sum;
-          const int at = seg.tile * kRows + row, n = static_cast<int>(magic_div(at, p.group_magic)), head = seg.head * p.group + at - n * p.group;
-          T* y = static_cast<T*>(p.o) + seg.b * p.os[0] + n * p.os[1] + head * p.os[2] + d;
-          *reinterpret_cast<uint2*>(y) = make_uint2(pack2<T>(acc.x * inv, acc.y * inv), pack2<T>(acc.z * inv, acc.w * inv));
-        }
+        join_parts<T, D>(p, seg, kRows, first, parts, threadIdx.x, kKv4AttnThreads);
         if (threadIdx.x == 0) p.counters[first] = 0;
       }
     }
     __syncthreads();  // merge buffer and flags
     if (gone) break;
-    if (!kv4_next(p, seg)) break;
+    if (!kv4_next<kKv4Step, kKv4Item>(p, seg)) break;
   }
   // A wait that ran out leaves copies in flight: they are waited for, again with a limit, before the shared memory goes.
   if (*abort_flag != 0 && producer && lane == 0) {
