@@ -380,8 +380,17 @@ int b200_kv4_attention(const B200Kv4AttnArgs* a, void* stream_ptr) {
   int device = 0;
   if (int rc = current_device(&device)) return rc;
   if (int rc = opt_in(g_attn_opted_in[device][f16 ? 0 : 1][a->head_dim == 64 ? 0 : 1][which], form.kernel, form.smem, "kv4_attention: shared memory opt-in")) return rc;
+  const int64_t joins = static_cast<int64_t>(a->batch) * p.row_tiles * a->kv_heads * (kKv4TileRows / kKv4JoinRows);
+  if (which == kTileForm && joins > INT32_MAX) return fail(B200_ATTN_UNSUPPORTED, "kv4_attention: too many rows");
   void* args[] = {&p};
   if (int rc = launch_kernel(form.kernel, static_cast<unsigned>(ctas), 1, form.threads, form.smem, 1, static_cast<cudaStream_t>(stream_ptr), args, "kv4_attention kernel launch")) return rc;
+  if (which == kTileForm && ctas > 1) {
+    const void* join = a->head_dim == 64 ? (f16 ? reinterpret_cast<const void*>(kv4_join_kernel<__half, 64>) : reinterpret_cast<const void*>(kv4_join_kernel<__nv_bfloat16, 64>))
+                                         : (f16 ? reinterpret_cast<const void*>(kv4_join_kernel<__half, 128>) : reinterpret_cast<const void*>(kv4_join_kernel<__nv_bfloat16, 128>));
+    int main_ctas = static_cast<int>(ctas);
+    void* join_args[] = {&p, &main_ctas};
+    if (int rc = launch_kernel(join, static_cast<unsigned>(joins), 1, kKv4JoinThreads, 0, 1, static_cast<cudaStream_t>(stream_ptr), join_args, "kv4_attention: launch of the join")) return rc;
+  }
   clear_error();
   return B200_ATTN_OK;
 }

@@ -214,50 +214,62 @@ __device__ __forceinline__ void write_unseen(const Kv4AttnParams& p, int threads
   }
 }
 
-// Joins the parts of an item, which begins with CTA `first`, and writes its rows.
-template <typename T, int D>
-__device__ __forceinline__ void join_parts(const Kv4AttnParams& p, const Kv4Segment& seg, int rows, int first, int parts, int thread, int threads) {
-  const int valid = min(rows, p.rows - seg.tile * rows);
-  for (int u = thread; u < valid * (D / 4); u += threads) {
-    const int row = u / (D / 4), d = 4 * (u % (D / 4));
-    // Parts eight at a time, all their loads in flight; the sums are brought to a new maximum when one comes along.
-    float most = -INFINITY, sum = 0.f;
-    float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-    constexpr int kAtOnce = 8;
-    for (int k0 = 0; k0 < parts; k0 += kAtOnce) {
-      float2 v[kAtOnce];
-      float4 y[kAtOnce];
+// Joins the parts of an item, which begins with CTA `first`, and writes `count` of its rows from `row0` on: UNITS float4 of the output at a time, each with PARTS
+// parts' loads in flight. The sums are brought to a new maximum when one comes along.
+template <typename T, int D, int UNITS, int PARTS>
+__device__ __forceinline__ void join_parts(const Kv4AttnParams& p, const Kv4Segment& seg, int rows, int first, int parts, int row0, int count, int thread, int threads) {
+  const int units = max(0, min(count, p.rows - seg.tile * rows - row0)) * (D / 4);
+  for (int u0 = thread; u0 < units; u0 += UNITS * threads) {
+    float most[UNITS], sum[UNITS];
+    float4 acc[UNITS];
 #pragma unroll
-      for (int i = 0; i < kAtOnce; ++i) {
-        const int k = min(k0 + i, parts - 1);
-        const int64_t at = (static_cast<int64_t>(first + k) * 2 + (k == 0 ? 1 : 0)) * rows + row;
-        v[i] = __ldcg(p.partial_ml + at);
-        y[i] = __ldcg(reinterpret_cast<const float4*>(p.partial + at * D + d));
-        if (k0 + i >= parts) v[i] = make_float2(-INFINITY, 0.f);
+    for (int j = 0; j < UNITS; ++j) most[j] = -INFINITY, sum[j] = 0.f, acc[j] = make_float4(0.f, 0.f, 0.f, 0.f);
+    for (int k0 = 0; k0 < parts; k0 += PARTS) {
+      float2 v[UNITS][PARTS];
+      float4 y[UNITS][PARTS];
+#pragma unroll
+      for (int j = 0; j < UNITS; ++j) {
+        const int u = min(u0 + j * threads, units - 1), row = row0 + u / (D / 4), d = 4 * (u % (D / 4));
+#pragma unroll
+        for (int i = 0; i < PARTS; ++i) {
+          const int k = min(k0 + i, parts - 1);
+          const int64_t at = (static_cast<int64_t>(first + k) * 2 + (k == 0 ? 1 : 0)) * rows + row;
+          v[j][i] = __ldcg(p.partial_ml + at);
+          y[j][i] = __ldcg(reinterpret_cast<const float4*>(p.partial + at * D + d));
+          if (k0 + i >= parts) v[j][i] = make_float2(-INFINITY, 0.f);
+        }
       }
-      float next = most;
 #pragma unroll
-      for (int i = 0; i < kAtOnce; ++i) next = fmaxf(next, v[i].x);
-      const float alpha = most == -INFINITY ? (sum == 0.f ? 0.f : 1.f) : exp2_approx(most - next);
-      most = next;
-      sum *= alpha;
-      acc.x *= alpha, acc.y *= alpha, acc.z *= alpha, acc.w *= alpha;
+      for (int j = 0; j < UNITS; ++j) {
+        float next = most[j];
 #pragma unroll
-      for (int i = 0; i < kAtOnce; ++i) {
-        const float by = v[i].x == -INFINITY ? v[i].y * 0.f : exp2_approx(v[i].x - most);
-        if (by != 0.f) {
-          sum = fmaf(by, v[i].y, sum);
-          acc.x = fmaf(by, y[i].x, acc.x);
-          acc.y = fmaf(by, y[i].y, acc.y);
-          acc.z = fmaf(by, y[i].z, acc.z);
-          acc.w = fmaf(by, y[i].w, acc.w);
+        for (int i = 0; i < PARTS; ++i) next = fmaxf(next, v[j][i].x);
+        const float alpha = most[j] == -INFINITY ? (sum[j] == 0.f ? 0.f : 1.f) : exp2_approx(most[j] - next);
+        most[j] = next;
+        sum[j] *= alpha;
+        acc[j].x *= alpha, acc[j].y *= alpha, acc[j].z *= alpha, acc[j].w *= alpha;
+#pragma unroll
+        for (int i = 0; i < PARTS; ++i) {
+          const float by = v[j][i].x == -INFINITY ? v[j][i].y * 0.f : exp2_approx(v[j][i].x - most[j]);
+          if (by != 0.f) {
+            sum[j] = fmaf(by, v[j][i].y, sum[j]);
+            acc[j].x = fmaf(by, y[j][i].x, acc[j].x);
+            acc[j].y = fmaf(by, y[j][i].y, acc[j].y);
+            acc[j].z = fmaf(by, y[j][i].z, acc[j].z);
+            acc[j].w = fmaf(by, y[j][i].w, acc[j].w);
+          }
         }
       }
     }
-    const float inv = sum == 0.f ? 0.f : 1.f / sum;
-    const int at = seg.tile * rows + row, n = static_cast<int>(magic_div(at, p.group_magic)), head = seg.head * p.group + at - n * p.group;
-    T* y = static_cast<T*>(p.o) + seg.b * p.os[0] + n * p.os[1] + head * p.os[2] + d;
-    *reinterpret_cast<uint2*>(y) = make_uint2(pack2<T>(acc.x * inv, acc.y * inv), pack2<T>(acc.z * inv, acc.w * inv));
+#pragma unroll
+    for (int j = 0; j < UNITS; ++j) {
+      const int u = u0 + j * threads, row = row0 + u / (D / 4), d = 4 * (u % (D / 4));
+      if (u >= units) continue;
+      const float inv = sum[j] == 0.f ? 0.f : 1.f / sum[j];
+      const int at = seg.tile * rows + row, n = static_cast<int>(magic_div(at, p.group_magic)), head = seg.head * p.group + at - n * p.group;
+      T* y = static_cast<T*>(p.o) + seg.b * p.os[0] + n * p.os[1] + head * p.os[2] + d;
+      *reinterpret_cast<uint2*>(y) = make_uint2(pack2<T>(acc[j].x * inv, acc[j].y * inv), pack2<T>(acc[j].z * inv, acc[j].w * inv));
+    }
   }
 }
 
@@ -774,7 +786,7 @@ __global__ void __launch_bounds__(kKv4AttnThreads, Kv4AttnSmem<D, NR, RW>::kCtas
       __syncthreads();
       if (*last_flag != 0) {
         __threadfence();
-        join_parts<T, D>(p, seg, kRows, first, parts, threadIdx.x, kKv4AttnThreads);
+        join_parts<T, D, 1, 8>(p, seg, kRows, first, parts, 0, kRows, threadIdx.x, kKv4AttnThreads);
         if (threadIdx.x == 0) p.counters[first] = 0;
       }
     }
