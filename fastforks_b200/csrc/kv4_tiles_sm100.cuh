@@ -133,7 +133,7 @@ __global__ void __launch_bounds__(kKv4TileThreads, 1) kv4_tiles_kernel(const Kv4
 
   if (warp < 8) {
     // ---- softmax: thread `row` of tile t ----
-    reg_alloc<192>();
+    reg_alloc<184>();
     if (any) {
     const int t = warp >> 2, row = threadIdx.x & 127;
     const uint32_t lanes = static_cast<uint32_t>(warp & 3) << 21;  // the warp's lanes of tensor memory, 32 (warp % 4) in the upper half
@@ -203,8 +203,12 @@ __global__ void __launch_bounds__(kKv4TileThreads, 1) kv4_tiles_kernel(const Kv4
         const float* par = reinterpret_cast<const float*>(smem + S::kPar) + st * 256;
         const float2 scales = *reinterpret_cast<const float2*>(smem + S::kScales + st * 8);
         float x[128];
-        tmem_ld_1x64(s_tm, reinterpret_cast<uint32_t*>(x));
-        tmem_ld_1x64(s_tm + 64, reinterpret_cast<uint32_t*>(x) + 64);
+        uint32_t* xu = reinterpret_cast<uint32_t*>(x);
+#pragma unroll
+        for (int c = 0; c < 4; ++c) tmem_ld_x32_nowait(s_tm + 32 * c, xu + 32 * c);
+        tmem_ld_wait_pin(xu);
+#pragma unroll
+        for (int c = 1; c < 4; ++c) tmem_ld_pin(xu + 32 * c);
         if constexpr (kApart) {
           const float2 qs2 = make_float2(qsum, qsum);
 #pragma unroll
@@ -445,7 +449,7 @@ __global__ void __launch_bounds__(kKv4TileThreads, 1) kv4_tiles_kernel(const Kv4
     }
     }
   } else {
-    reg_dealloc<56>();
+    reg_dealloc<72>();
     if (any && warp == 12) {
       // ---- loads ----
       if (lane == 0) {
