@@ -4,7 +4,8 @@ One operator - non-causal multi-head `softmax(scale * q k^T + bias) v`, head dim
 interfaces the reference calls it through: `Flash64(variant)(q, k, v, scale)` on `[B, N, heads, 64]` views and
 `scaled_dot_product_attention(q, k, v, attn_mask, scale=...)` on `[B, heads, N, 64]` views. The arithmetic runs in
 `libb200attn.so` (hand-written tcgen05 / TMA kernels, C ABI in `include/b200_attn.h`); this package holds the host
-side only and raises when that library is missing.
+side only and raises when that library is missing. Beside it stand a token decoder's operators (`include/b200_decoder.h`):
+`rotary`, `qk_norm_rotary` and a paged cache held in 4 bits with its causal attention (`kv4_append_`, `kv4_attention`).
 """
 
 from __future__ import annotations
