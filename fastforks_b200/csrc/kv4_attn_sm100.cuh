@@ -11,8 +11,10 @@
 // Codes are the left operand: S^T = K Q^T has 16 tokens by 8 rows, O^T = V^T P^T 16 dimensions by 8 rows, so that eight rows (the q heads
 // that share a kv head, of one query) fill a product. P^T comes out of the first product with tokens along the lanes and goes
 // into the second with rows along them: one transposition of 8 x 8 in registers for each eight tokens. Codes of V multiply p vs as
-// code - 8 (one more row of the product sums 8 p vs), and vl + 8 vs takes the rest in fp32: rounding p vs then errs by a part of a value, not of a
-// code up to 15.
+// code - 8, and vl + 8 vs takes the rest in fp32: rounding p vs then errs by a part of a value, not of a code up to 15. For q in fp16 the 8 is
+// taken off in the operand (exact in subnormals, four more instructions a word), for bfloat16 one more row of the product sums 8 p vs and
+// is taken off at the end: over 20000 tokens the sums of codes cancel to 1 / 100 of themselves, which fp32 has room for
+// beside an output of 8 bits, but not of 11 (error of fp16 outputs 1.65 times the output's own rounding, 1.4 with codes less 8).
 //
 // A warp has 8 or 16 rows (queries x the q heads that share a kv head) and walks steps of 32 tokens. CTAs of four warps: up to 16 rows all
 // four warps share the rows and take every fourth step, each with its own softmax state, joined at the end; up to 32 two and two; above
@@ -84,6 +86,11 @@ __device__ __forceinline__ void split_codes(uint32_t w, uint32_t* pairs) {
   pairs[1] = w & 0x00f000f0u;
   pairs[2] = h & 0x000f000fu;
   pairs[3] = h & 0x00f000f0u;
+}
+
+__device__ __forceinline__ uint32_t half2_sum(uint32_t a, uint32_t b) {
+  const __half2 r = __hadd2(*reinterpret_cast<const __half2*>(&a), *reinterpret_cast<const __half2*>(&b));
+  return *reinterpret_cast<const uint32_t*>(&r);
 }
 
 // An 8 x 8 matrix of 16-bit values, lane l holding columns 2 (l % 4) and the next of row l / 4, transposed.
@@ -280,6 +287,7 @@ __global__ void __launch_bounds__(kKv4AttnThreads, Kv4AttnSmem<D, NR, RW>::kCtas
   constexpr int kTW = S::kTW, kWarpRows = 8 * NR, kRows = kWarpRows * RW;
   constexpr int kWords = D / 32;  // words of codes in a lane, for each token of K and each two of V
   constexpr int kTiles = D / 16;  // row tiles of the output
+  constexpr bool kLess8 = std::is_same<T, __half>::value;  // codes of V less 8 in the operands, or 8 p vs summed beside them
   extern __shared__ __align__(128) uint8_t smem[];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, r = lane >> 2, c = lane & 3;
   const int rw = warp % RW, tw = warp / RW;
@@ -651,12 +659,19 @@ __global__ void __launch_bounds__(kKv4AttnThreads, Kv4AttnSmem<D, NR, RW>::kCtas
         }
         const uint32_t eight[4] = {0x00080008u, 0x00080008u, 0x00080008u, 0x00080008u};
 #pragma unroll
-        for (int t = 0; t < NR; ++t) mma_16816<__half>(eights[t], eight, pb[t][0], pb[t][1]);
+        for (int t = 0; t < NR && !kLess8; ++t) mma_16816<__half>(eights[t], eight, pb[t][0], pb[t][1]);
 #pragma unroll
         for (int i = 0; i < kWords; ++i) {
           uint32_t u0[4], u1[4];
           split_codes(w0[i], u0);
           split_codes(w1[i], u1);
+          if constexpr (kLess8) {
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {  // 8 as either nibble has it
+              u0[k] = half2_sum(u0[k], k & 1 ? 0x80808080u : 0x80088008u);
+              u1[k] = half2_sum(u1[k], k & 1 ? 0x80808080u : 0x80088008u);
+            }
+          }
 #pragma unroll
           for (int k = 0; k < 2; ++k) {
             const uint32_t a[4] = {u0[2 * k], u0[2 * k + 1], u1[2 * k], u1[2 * k + 1]};
