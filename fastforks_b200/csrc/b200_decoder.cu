@@ -30,22 +30,29 @@ int lanes_log2_of(int dim) {
   return n;
 }
 
+constexpr int kSplitBytes = 16384;  // the rows that a CTA's groups of lanes turn, as floats: 16 dimensions a lane at most
 struct RotaryForm {
   const void* kernel;
   int smem, ctas_per_sm;
 };
+template <typename T, int FORM, int MODE>
+RotaryForm stream_form(int more) {
+  using S = RotaryStream<T, MODE, FORM>;
+  return {reinterpret_cast<const void*>(rotary_stream_kernel<T, FORM, MODE>), S::kBytes + more, S::kCtasPerSm};
+}
 template <typename T, int MODE>
 RotaryForm rotary_form(int form) {
-  using S = RotaryStream<T, MODE>;
-  if (form == kRowHalves) return {reinterpret_cast<const void*>(rotary_stream_kernel<T, kRowHalves, MODE>), S::kBytes, S::kCtasPerSm};
-  if (form == kRowPairs) return {reinterpret_cast<const void*>(rotary_stream_kernel<T, kRowPairs, MODE>), S::kBytes, S::kCtasPerSm};
+  if (form == kRowHalves) return stream_form<T, kRowHalves, MODE>(0);
+  if (form == kRowPairs) return stream_form<T, kRowPairs, MODE>(0);
+  if (form == kRowLoose) return stream_form<T, kRowLoose, MODE>(0);
+  if (form == kRowSplit) return stream_form<T, kRowSplit, MODE>(kSplitBytes);
   return {reinterpret_cast<const void*>(rotary_any_kernel<T, MODE>), 0, 2};
 }
 template <typename T>
 RotaryForm rotary_form_of(int form, int mode) {
   return mode == kTurn ? rotary_form<T, kTurn>(form) : mode == kNormTurn ? rotary_form<T, kNormTurn>(form) : rotary_form<T, kNormBack>(form);
 }
-std::atomic<bool> g_rotary_opted_in[kMaxDevices][3][3][3];
+std::atomic<bool> g_rotary_opted_in[kMaxDevices][3][kRowForms][3];
 
 // The shared-memory opt-in of a kernel on this device, once.
 int opt_in(std::atomic<bool>& done, const void* kernel, int smem, const char* what) {
@@ -108,7 +115,7 @@ void set_cache(Kv4Params* p, const B200Kv4Args* a, DeviceState* dev) {
 
 template <typename T, int D>
 const void* append_kernel_of(int form) {
-  const void* k[3] = {reinterpret_cast<const void*>(kv4_append_kernel<T, D, kRowHalves>), reinterpret_cast<const void*>(kv4_append_kernel<T, D, kRowPairs>), reinterpret_cast<const void*>(kv4_append_kernel<T, D, kRowAny>)};
+  const void* k[4] = {reinterpret_cast<const void*>(kv4_append_kernel<T, D, kRowHalves>), reinterpret_cast<const void*>(kv4_append_kernel<T, D, kRowPairs>), reinterpret_cast<const void*>(kv4_append_kernel<T, D, kRowSplit>), reinterpret_cast<const void*>(kv4_append_kernel<T, D, kRowLoose>)};
   return k[form];
 }
 
@@ -208,9 +215,9 @@ int b200_rotary(const B200RotaryArgs* a, void* stream_ptr) {
   p.eps = a->eps;
   p.sign = a->backward ? -1.f : 1.f;
   p.status = dev->status;
-  // Rows whose rotation and length come in whole lanes, on 16 bytes, keep partners in one lane; the others look theirs up in shared memory.
+  // Rows of whole words on 16 bytes are streamed; halves whose partners lie in one lane are turned there, others through shared memory.
   const bool pairs = p.interleaved || a->rot == 0;
-  const int form = vec && a->head_dim % 16 == 0 && a->rot % (pairs ? 8 : 16) == 0 ? (pairs ? kRowPairs : kRowHalves) : kRowAny;
+  const int form = !vec || a->head_dim % 8 != 0 ? kRowAny : pairs ? (a->rot % 8 == 0 && a->head_dim % 16 == 0 ? kRowPairs : kRowLoose) : a->head_dim % 16 == 0 && a->rot % 16 == 0 ? kRowHalves : kRowSplit;
   const int mode = !a->norm ? kTurn : a->backward ? kNormBack : kNormTurn;
   const RotaryForm kernel = a->dtype == B200_ATTN_F16 ? rotary_form_of<__half>(form, mode) : a->dtype == B200_ATTN_BF16 ? rotary_form_of<__nv_bfloat16>(form, mode) : rotary_form_of<float>(form, mode);
   // A token's rows go to as many groups of lanes as leave each of them four rows or more; calls of few tokens use more groups than that.
@@ -280,7 +287,7 @@ int b200_kv4_append(const B200Kv4Args* a, void* stream_ptr) {
   p.q_out = a->q_out;
   for (int i = 0; i < 3; ++i) p.qs[i] = a->q_stride[i], p.ks[i] = a->k_stride[i], p.vs[i] = a->v_stride[i], p.qos[i] = a->q_out_stride[i];
   const bool pairs = p.interleaved || a->rot == 0;
-  const int form = a->rot % (pairs ? 8 : 16) == 0 ? (pairs ? kRowPairs : kRowHalves) : kRowAny;
+  const int form = pairs ? (a->rot % 8 == 0 ? kRowPairs : kRowLoose) : a->rot % 16 == 0 ? kRowHalves : kRowSplit;
   const bool f16 = a->dtype == B200_ATTN_F16;
   const void* kernel = a->head_dim == 64 ? (f16 ? append_kernel_of<__half, 64>(form) : append_kernel_of<__nv_bfloat16, 64>(form))
                                          : (f16 ? append_kernel_of<__half, 128>(form) : append_kernel_of<__nv_bfloat16, 128>(form));

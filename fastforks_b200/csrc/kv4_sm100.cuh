@@ -114,7 +114,7 @@ template <typename T, int D, int FORM>
 __global__ void __launch_bounds__(kKv4Threads) kv4_append_kernel(const Kv4Params p) {
   constexpr int kLanes = D / 16, kGroups = kKv4Threads / kLanes;
   using L = Kv4Layout<D>;
-  __shared__ float rows_smem[FORM == kRowAny ? kGroups * D : 1];
+  __shared__ __align__(16) float rows_smem[FORM == kRowSplit ? kGroups * D : 4];
   grid_dependency_wait();
   grid_launch_dependents();
   const int j = threadIdx.x % kLanes, group = threadIdx.x / kLanes;
@@ -142,7 +142,7 @@ __global__ void __launch_bounds__(kKv4Threads) kv4_append_kernel(const Kv4Params
   const float* cs = what == 2 ? nullptr : table_row(p.cs, p.rot, p.table_rows, at, p.status);
   Turns<FORM> turns;
   turns.load(cs, at0, at1, p.rot, 1.f);
-  rotate16<FORM>(f, turns, D, p.interleaved, rows_smem + (FORM == kRowAny ? group * D : 0));
+  turns.template apply<false>(f, rows_smem + (FORM == kRowSplit ? group * D : 0), D, p.interleaved);
   uint32_t words[2], pair = 0;
   if (__any_sync(0xffffffffu, what != 0)) pair = quantise16<kLanes>(f, words);
   if (!there) return;

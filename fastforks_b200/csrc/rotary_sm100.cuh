@@ -115,19 +115,22 @@ __device__ __forceinline__ void store8(T* p, const float* f) {
 }
 
 // How a row lies in its lanes, eight dimensions at a first and eight at a second place, so that neighbouring lanes' words are neighbours.
-// kRowHalves: lane j < rot / 16 holds dimensions 8 j .. and rot / 2 + 8 j .. (the partners), the lanes behind them the rest in the same way.
-// kRowPairs: dimensions 8 j .. and dim / 2 + 8 j ... Both want dim in multiples of 16, the one rot in multiples of 16, the other of 8.
+// kRowHalves: lane j < rot / 16 holds dimensions 8 j .. and rot / 2 + 8 j .. (the partners), the lanes behind them the rest in the same way; dim and
+// rot in multiples of 16. kRowPairs (neighbours are partners, dim in multiples of 16 and rot of 8), kRowLoose (the same, any rot) and kRowSplit (halves, any
+// rot; partners through shared memory): the first half of the row's words of eight dimensions and the second, the last lane's second one
+// may be none; dim in multiples of 8.
 // kRowAny: 16 consecutive dimensions, partners through shared memory, any rot and dim.
-enum RowForm { kRowHalves = 0, kRowPairs = 1, kRowAny = 2 };
+enum RowForm { kRowHalves = 0, kRowPairs = 1, kRowSplit = 2, kRowLoose = 3, kRowAny = 4 };
+constexpr int kRowForms = 5;
 
 template <int FORM>
 __device__ __forceinline__ void lane_places(int j, int rot, int dim, int* a, int* b) {
   if (FORM == kRowAny) {
     *a = 16 * j;
     *b = 16 * j + 8;
-  } else if (FORM == kRowPairs) {
+  } else if (FORM != kRowHalves) {
     *a = 8 * j;
-    *b = (dim >> 1) + 8 * j;
+    *b = 8 * ((dim + 8) >> 4) + 8 * j;
   } else if (16 * j < rot) {
     *a = 8 * j;
     *b = (rot >> 1) + 8 * j;
@@ -154,13 +157,24 @@ __device__ __forceinline__ void turn_fused(float& a, float& b, float c, float s)
 template <int FORM>
 struct Turns {
   float c[8], s[8];
-  bool first, second;  // whether the lane's places are rotated
+  int first, second;  // pairs of the lane's places that are rotated; but for kRowLoose all of a place's or none
   __device__ __forceinline__ void load(const float* cs, int a, int b, int rot, float sign) {
-    first = cs != nullptr && a < rot && (FORM == kRowPairs || b < rot);
-    second = cs != nullptr && b < rot;
-    const int at = FORM == kRowPairs ? a >> 1 : a, bt = FORM == kRowPairs ? b >> 1 : a + 4;
-    if (first) get(cs, at, rot, 0);
-    if (second) get(cs, bt, rot, 4);
+    if (FORM == kRowLoose) {
+      first = cs == nullptr ? 0 : min(max((rot - a) >> 1, 0), 4);
+      second = cs == nullptr ? 0 : min(max((rot - b) >> 1, 0), 4);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        if ((i & 3) >= (i < 4 ? first : second)) continue;
+        const int at = (i < 4 ? a : b - 8) / 2 + i;
+        c[i] = __ldg(cs + at);
+        s[i] = __ldg(cs + (rot >> 1) + at);
+      }
+    } else {
+      first = cs != nullptr && (FORM == kRowPairs ? a : b) < rot ? 4 : 0;
+      second = cs != nullptr && b < rot ? 4 : 0;
+      if (first != 0) get(cs, FORM == kRowPairs ? a >> 1 : a, rot, 0);
+      if (second != 0) get(cs, FORM == kRowPairs ? b >> 1 : a + 4, rot, 4);
+    }
 #pragma unroll
     for (int i = 0; i < 8; ++i) s[i] *= sign;
   }
@@ -170,13 +184,49 @@ struct Turns {
     s[i] = y.x, s[i + 1] = y.y, s[i + 2] = y.z, s[i + 3] = y.w;
   }
   template <bool FUSED>
-  __device__ __forceinline__ void apply(float* f) const {  // a lane's 16 values, 8 at its first place and 8 at its second
+  __device__ __forceinline__ void apply(float* f, float*, int, bool) const {  // a lane's 16 values, 8 at its first place and 8 at its second
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
-      if (FORM == kRowPairs ? (i < 4 ? !first : !second) : !first) continue;
+      if (FORM == kRowLoose ? (i & 3) >= (i < 4 ? first : second) : (FORM == kRowHalves || i < 4 ? first : second) == 0) continue;
       float &x = FORM == kRowHalves ? f[i] : f[2 * i], &y = FORM == kRowHalves ? f[8 + i] : f[2 * i + 1];
       if (FUSED) turn_fused(x, y, c[i], s[i]);
       else turn(x, y, c[i], s[i]);
+    }
+  }
+};
+
+// Halves of any rot: a value's partner is looked up in `row`, the group's floats in shared memory; one that is not turned has cosine 1 and
+// sine 0, and a zero for a partner (no branches: sixteen of them do not fit the predicate registers).
+template <>
+struct Turns<kRowSplit> {
+  float c[16], s[16];
+  uint32_t partner[8];  // two of 16 bits; all ones: none
+  int a, b;
+  __device__ __forceinline__ void load(const float* cs, int first_place, int second_place, int rot, float sign) {
+    a = first_place, b = second_place;
+    const int half = rot >> 1;
+#pragma unroll
+    for (int i = 0; i < 16; ++i) {
+      const int e = i < 8 ? a + i : b + i - 8;
+      const bool turned = cs != nullptr && e < rot, late = e >= half;
+      const int at = late ? e - half : e;
+      c[i] = turned ? __ldg(cs + at) : 1.f;
+      s[i] = turned ? (late ? sign : -sign) * __ldg(cs + half + at) : 0.f;
+      const uint32_t other = turned ? late ? e - half : e + half : 0xffffu;
+      partner[i >> 1] = i & 1 ? partner[i >> 1] | other << 16 : other;
+    }
+  }
+  template <bool FUSED>
+  __device__ __forceinline__ void apply(float* f, float* row, int dim, bool) const {
+    __syncwarp();
+    store8<float>(row + a, f);
+    if (b < dim) store8<float>(row + b, f + 8);
+    __syncwarp();
+#pragma unroll
+    for (int i = 0; i < 16; ++i) {
+      const uint32_t at = i & 1 ? partner[i >> 1] >> 16 : partner[i >> 1] & 0xffffu;
+      const float held = row[at == 0xffffu ? 0 : at], other = at == 0xffffu ? 0.f : held;
+      f[i] = FUSED ? fmaf(f[i], c[i], other * s[i]) : __fadd_rn(__fmul_rn(f[i], c[i]), __fmul_rn(other, s[i]));
     }
   }
 };
@@ -188,6 +238,7 @@ struct Turns<kRowAny> {
   int a, rot;
   float sign;
   __device__ __forceinline__ void load(const float* table, int place, int, int n, float by) { cs = table, a = place, rot = n, sign = by; }
+  template <bool FUSED>
   __device__ __forceinline__ void apply(float* f, float* row, int dim, bool interleaved) const {
     __syncwarp();
 #pragma unroll
@@ -208,12 +259,6 @@ struct Turns<kRowAny> {
     }
   }
 };
-
-template <int FORM>
-__device__ __forceinline__ void rotate16(float* f, const Turns<FORM>& turns, int dim, bool interleaved, float* row) {
-  if constexpr (FORM == kRowAny) turns.apply(f, row, dim, interleaved);
-  else turns.template apply<false>(f);
-}
 
 // 16 values from `at` on of a row, zeros past `dim`. vec: the row starts on 16 bytes.
 template <typename T>
@@ -265,7 +310,7 @@ __device__ __forceinline__ void load_weight(float* f, const RotaryParams& p, con
 #pragma unroll
   for (int i = 0; i < 16; ++i) f[i] = 1.f;
   if (w == nullptr) return;
-  if (FORM != kRowAny && aligned_16(w)) {
+  if (FORM != kRowAny && b < p.dim && aligned_16(w)) {
     if (p.w_f32) {
       Raw8<float> u, v;
       u.load(static_cast<const float*>(w) + a);
@@ -291,9 +336,9 @@ __device__ __forceinline__ void load_weight(float* f, const RotaryParams& p, con
 enum RotaryMode { kTurn = 0, kNormTurn = 1, kNormBack = 2 };
 
 // Rows that a lane has in flight, in its own places in shared memory: 128 KB an SM in 16 bits.
-template <typename T, int MODE>
+template <typename T, int MODE, int FORM>
 struct RotaryStream {
-  static constexpr int kCtasPerSm = MODE == kTurn ? 4 : MODE == kNormTurn ? 3 : 2;
+  static constexpr int kCtasPerSm = MODE == kNormBack || (MODE == kNormTurn && FORM == kRowSplit) ? 2 : MODE == kNormTurn || FORM == kRowSplit ? 3 : 4;
   static constexpr int kParts = sizeof(T) / 2 * 2;                        // 16-byte words of a row in a lane
   static constexpr int kTensors = MODE == kNormBack ? 2 : 1;             // x, and g
   static constexpr int kDepth = sizeof(T) == 4 ? 2 : 4;
@@ -372,15 +417,18 @@ __device__ __forceinline__ void join_sums(const RotaryParams& p, float* smem) {
 // tokens, and walks it with the first tensor, then with the second (the weights, and backward the sums for dw, are one tensor's at a time);
 // its groups of lanes take a few heads each of a few tokens at once, and keep a token's cosines and sines for its heads.
 template <typename T, int FORM, int MODE>
-__global__ void __launch_bounds__(kRotaryThreads, RotaryStream<T, MODE>::kCtasPerSm) rotary_stream_kernel(const RotaryParams p) {
-  using S = RotaryStream<T, MODE>;
+__global__ void __launch_bounds__(kRotaryThreads, RotaryStream<T, MODE, FORM>::kCtasPerSm) rotary_stream_kernel(const RotaryParams p) {
+  using S = RotaryStream<T, MODE, FORM>;
   extern __shared__ __align__(16) float rotary_smem[];
   grid_dependency_wait();
   grid_launch_dependents();
   const int j = threadIdx.x & ((1 << p.lanes_log2) - 1), group = threadIdx.x >> p.lanes_log2;
   int a, b;
   lane_places<FORM>(j, p.rot, p.dim, &a, &b);
-  const bool place = 16 * j < p.dim;
+  const int words = (p.dim + 8) >> 4;  // a row's words of eight dimensions, less those at second places
+  const bool place = j < words, place_b = place && b < p.dim;
+  constexpr bool kWhole = FORM == kRowHalves || FORM == kRowPairs;  // every lane has both places
+  float* row_smem = rotary_smem + S::kBytes / 4 + group * p.dim;  // kRowSplit
   const uint32_t run_begin = static_cast<uint32_t>(static_cast<uint64_t>(p.all_tokens) * blockIdx.x / gridDim.x);
   const uint32_t run_end = static_cast<uint32_t>(static_cast<uint64_t>(p.all_tokens) * (blockIdx.x + 1) / gridDim.x);
   uint4* mine = reinterpret_cast<uint4*>(rotary_smem) + threadIdx.x;
@@ -416,7 +464,7 @@ __global__ void __launch_bounds__(kRotaryThreads, RotaryStream<T, MODE>::kCtasPe
 #pragma unroll
         for (int i = 0; i < S::kParts; ++i) {
           const int at = i < kHalf ? a + i * (16 / static_cast<int>(sizeof(T))) : b + (i - kHalf) * (16 / static_cast<int>(sizeof(T)));
-          if (valid) {
+          if (valid && (kWhole || i < kHalf || place_b)) {
             cp_async_16(to + i * kRotaryThreads * 16, from_x + at, true);
             if (MODE == kNormBack) cp_async_16(to + (S::kParts + i) * kRotaryThreads * 16, from_g + at, true);
           }
@@ -455,6 +503,11 @@ __global__ void __launch_bounds__(kRotaryThreads, RotaryStream<T, MODE>::kCtasPe
           Raw8<T> u;
 #pragma unroll
           for (int i = 0; i < 2; ++i) {
+            if (!kWhole && i == 1 && !place_b) {
+#pragma unroll
+              for (int n = 8; n < 16; ++n) to[n] = 0.f;
+              continue;
+            }
             if constexpr (sizeof(T) == 4) {
               u.a = *reinterpret_cast<const float4*>(at + (part + 2 * i) * kRotaryThreads);
               u.b = *reinterpret_cast<const float4*>(at + (part + 2 * i + 1) * kRotaryThreads);
@@ -471,7 +524,7 @@ __global__ void __launch_bounds__(kRotaryThreads, RotaryStream<T, MODE>::kCtasPe
           for (int i = 0; i < 16; ++i) f[i] = 0.f;
         }
         if constexpr (MODE == kTurn) {
-          turns.template apply<false>(f);
+          turns.template apply<false>(f, row_smem, p.dim, false);
         } else {
           float e[16], sum = 0.f;
 #pragma unroll
@@ -480,7 +533,7 @@ __global__ void __launch_bounds__(kRotaryThreads, RotaryStream<T, MODE>::kCtasPe
             const float r = rsqrtf(fmaf(group_sum(sum, p.lanes_log2), p.inv_dim, p.eps));
 #pragma unroll
             for (int i = 0; i < 16; ++i) f[i] = f[i] * r * w[i];
-            turns.template apply<true>(f);
+            turns.template apply<true>(f, row_smem, p.dim, false);
           } else {
             if (valid) {
               read(e, S::kParts);
@@ -488,7 +541,7 @@ __global__ void __launch_bounds__(kRotaryThreads, RotaryStream<T, MODE>::kCtasPe
 #pragma unroll
               for (int i = 0; i < 16; ++i) e[i] = 0.f;
             }
-            turns.template apply<true>(e);
+            turns.template apply<true>(e, row_smem, p.dim, false);
             float along = 0.f;
 #pragma unroll
             for (int i = 0; i < 16; ++i) along = fmaf(e[i] * w[i], f[i], along);
@@ -508,7 +561,7 @@ __global__ void __launch_bounds__(kRotaryThreads, RotaryStream<T, MODE>::kCtasPe
         }
         if (valid) {
           store8<T>(y + a, f);
-          store8<T>(y + b, f + 8);
+          if (kWhole || place_b) store8<T>(y + b, f + 8);
         }
         y += step * t.ys[2];
       }
@@ -551,7 +604,7 @@ __global__ void __launch_bounds__(kRotaryThreads, 2) rotary_any_kernel(const Rot
         float f[16];
         load16<T>(f, static_cast<const T*>(t.x) + img * t.xs[0] + n * t.xs[1] + h * t.xs[2], a, valid ? p.dim : 0, p.vec);
         if constexpr (MODE == kTurn) {
-          turns.apply(f, row_smem, p.dim, p.interleaved);
+          turns.template apply<false>(f, row_smem, p.dim, p.interleaved);
         } else {
           float sum = 0.f;
 #pragma unroll
@@ -560,11 +613,11 @@ __global__ void __launch_bounds__(kRotaryThreads, 2) rotary_any_kernel(const Rot
           if constexpr (MODE == kNormTurn) {
 #pragma unroll
             for (int i = 0; i < 16; ++i) f[i] = f[i] * r * w[i];
-            turns.apply(f, row_smem, p.dim, p.interleaved);
+            turns.template apply<false>(f, row_smem, p.dim, p.interleaved);
           } else {
             float e[16], along = 0.f;
             load16<T>(e, static_cast<const T*>(t.g) + img * t.gs[0] + n * t.gs[1] + h * t.gs[2], a, valid ? p.dim : 0, p.vec);
-            turns.apply(e, row_smem, p.dim, p.interleaved);
+            turns.template apply<false>(e, row_smem, p.dim, p.interleaved);
 #pragma unroll
             for (int i = 0; i < 16; ++i) along = fmaf(e[i] * w[i], f[i], along);
             const float back = group_sum(along, p.lanes_log2) * r * r * p.inv_dim;
