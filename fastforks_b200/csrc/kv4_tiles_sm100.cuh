@@ -13,6 +13,11 @@
 // next S of one tile while the other's softmax runs. Tensor memory: O 2 x head dim columns, S 2 x 128. The line of work, its runs and the
 // join of parts are those of the other kernel.
 //
+// Measured: 2 x 500 queries of 32 heads on 8 over 9000 tokens, head dim 128, bf16, 213 us, 673 TFLOP/s, 41 % of the measured dense rate (the
+// kernel of few rows took 647 us). A step of 256 rows takes some 4800 clocks, where its products need 1000 and its exponentials 2000:
+// a tile's softmax (2100), its products and the waits between them follow one another, and unpacking (3000 for both tiles by one warp on each
+// scheduler) is not much shorter (clocks are of one instrumented run).
+//
 #pragma once
 
 #include "kv4_attn_sm100.cuh"
@@ -34,7 +39,7 @@ struct Kv4TilesSmem {
   static constexpr int kBig = kPar + 2 * 2 * 128 * 4;    // [2][4] largest magnitudes of K and of V, by the warp whose tokens they are of
   static constexpr int kScales = kBig + 64;              // [2] the step's power of two of K, and that of V so far
   static constexpr int kBars = kScales + 32;
-  static constexpr int kFlags = kBars + 32 * 8;          // gave up, last of an item, zero, tensor memory
+  static constexpr int kFlags = kBars + 32 * 8;          // gave up, (unused), zero, tensor memory
   static constexpr int kBytes = kFlags + 16 + 1024;      // the tiles start on 1024
 };
 
@@ -135,318 +140,318 @@ __global__ void __launch_bounds__(kKv4TileThreads, 1) kv4_tiles_kernel(const Kv4
     // ---- softmax: thread `row` of tile t ----
     reg_alloc<184>();
     if (any) {
-    const int t = warp >> 2, row = threadIdx.x & 127;
-    const uint32_t lanes = static_cast<uint32_t>(warp & 3) << 21;  // the warp's lanes of tensor memory, 32 (warp % 4) in the upper half
-    const uint32_t s_tm = tmem + lanes + kColS + t * 128, o_tm = tmem + lanes + t * 128;
-    uint32_t steps = 0, mine = 0, items = 0;  // of the CTA; of this tile
-    for (;;) {
-      const int seen = kv4_seen<kKv4TileRows, kStep>(p, seg);
-      const int row0 = seg.tile * kKv4TileRows + 128 * t, last = min(row0 + row, p.rows - 1);
-      const bool active = row0 < p.rows && seen > seg.s0;
-      float l = 0.f, ms = 0.f, off = 0.f, rscale = 0.f, qsum = 0.f;  // off: log2 of what the sums are relative to, 2^-7 of the largest weight or so
-      bool seen_any = false;
-      float vunit = 0.f;  // O is in units of this
-      const int n = static_cast<int>(magic_div(last, p.group_magic)), g = last - n * p.group, pos = seg.len - p.queries + n;
-      const int lowest = seg.len - p.queries + static_cast<int>(magic_div(min(row0, p.rows - 1), p.group_magic));
-      if (active) {
-        const T* x = static_cast<const T*>(p.q) + seg.b * p.qs[0] + n * p.qs[1] + (seg.head * p.group + g) * p.qs[2];
-        float most = 0.f;
+      const int t = warp >> 2, row = threadIdx.x & 127;
+      const uint32_t lanes = static_cast<uint32_t>(warp & 3) << 21;  // the warp's lanes of tensor memory, 32 (warp % 4) in the upper half
+      const uint32_t s_tm = tmem + lanes + kColS + t * 128, o_tm = tmem + lanes + t * 128;
+      uint32_t steps = 0, mine = 0, items = 0;  // of the CTA; of this tile
+      for (;;) {
+        const int seen = kv4_seen<kKv4TileRows, kStep>(p, seg);
+        const int row0 = seg.tile * kKv4TileRows + 128 * t, last = min(row0 + row, p.rows - 1);
+        const bool active = row0 < p.rows && seen > seg.s0;
+        float l = 0.f, ms = 0.f, off = 0.f, rscale = 0.f, qsum = 0.f;  // off: log2 of what the sums are relative to, 2^-7 of the largest weight or so
+        bool seen_any = false;
+        float vunit = 0.f;  // O is in units of this
+        const int n = static_cast<int>(magic_div(last, p.group_magic)), g = last - n * p.group, pos = seg.len - p.queries + n;
+        const int lowest = seg.len - p.queries + static_cast<int>(magic_div(min(row0, p.rows - 1), p.group_magic));
+        if (active) {
+          const T* x = static_cast<const T*>(p.q) + seg.b * p.qs[0] + n * p.qs[1] + (seg.head * p.group + g) * p.qs[2];
+          float most = 0.f;
 #pragma unroll 4
-        for (int w = 0; w < D / 8; ++w) {
-          Raw8<T> raw;
-          float f[8];
-          raw.load(x + 8 * w);
-          raw.unpack(f);
+          for (int w = 0; w < D / 8; ++w) {
+            Raw8<T> raw;
+            float f[8];
+            raw.load(x + 8 * w);
+            raw.unpack(f);
 #pragma unroll
-          for (int k = 0; k < 8; ++k) most = fmaxf(most, fabsf(f[k]));
-        }
-        const int e = min(max(static_cast<int>(__float_as_uint(most) >> 23) - 127, -100), 126);
-        const float up = pow2(10 - e);
-#pragma unroll 4
-        for (int w = 0; w < D / 8; ++w) {
-          Raw8<T> raw;
-          float f[8];
-          raw.load(x + 8 * w);
-          raw.unpack(f);
-#pragma unroll
-          for (int k = 0; k < 8; ++k) {
-            f[k] *= up;
-            qsum += f[k];
+            for (int k = 0; k < 8; ++k) most = fmaxf(most, fabsf(f[k]));
           }
-          // in the order in which a word of codes is split
-          *reinterpret_cast<uint4*>(smem + S::kQ + t * S::kTile + (w >> 3) * 16384 + row * 128 + (((w & 7) ^ (row & 7)) << 4)) =
-              make_uint4(pack2<__half>(f[0], f[4]), pack2<__half>(f[1], f[5]), pack2<__half>(f[2], f[6]), pack2<__half>(f[3], f[7]));
+          const int e = min(max(static_cast<int>(__float_as_uint(most) >> 23) - 127, -100), 126);
+          const float up = pow2(10 - e);
+#pragma unroll 4
+          for (int w = 0; w < D / 8; ++w) {
+            Raw8<T> raw;
+            float f[8];
+            raw.load(x + 8 * w);
+            raw.unpack(f);
+#pragma unroll
+            for (int k = 0; k < 8; ++k) {
+              f[k] *= up;
+              qsum += f[k];
+            }
+            // in the order in which a word of codes is split
+            *reinterpret_cast<uint4*>(smem + S::kQ + t * S::kTile + (w >> 3) * 16384 + row * 128 + (((w & 7) ^ (row & 7)) << 4)) =
+                make_uint4(pack2<__half>(f[0], f[4]), pack2<__half>(f[1], f[5]), pack2<__half>(f[2], f[6]), pack2<__half>(f[3], f[7]));
+          }
+          rscale = p.scale_log2 * pow2(e - 10);
+          fence_proxy_async_smem();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(bars + kBarQFull + t);
         }
-        rscale = p.scale_log2 * pow2(e - 10);
-        fence_proxy_async_smem();
-        __syncwarp();
-        if (lane == 0) mbar_arrive(bars + kBarQFull + t);
-      }
-      for (int s = seg.s0; s < seen; ++s, ++steps) {
-        const int st = steps & 1;
-        if (!active) {  // keeps in step with the parameters
-          ok = ok && wait(kBarParFull + st, (steps >> 1) & 1);
+        for (int s = seg.s0; s < seen; ++s, ++steps) {
+          const int st = steps & 1;
+          if (!active) {  // keeps in step with the parameters
+            ok = ok && wait(kBarParFull + st, (steps >> 1) & 1);
+            if (!__all_sync(0xffffffffu, ok)) {
+              ok = false;
+              break;
+            }
+            if (lane == 0) mbar_arrive(bars + kBarParFree + st);
+            continue;
+          }
+          ok = ok && wait(kBarParFull + st, (steps >> 1) & 1) && wait(kBarSFull + t, mine & 1);
           if (!__all_sync(0xffffffffu, ok)) {
             ok = false;
             break;
           }
-          if (lane == 0) mbar_arrive(bars + kBarParFree + st);
-          continue;
+          ++mine;
+          tc_fence_after_sync();
+          const float* par = reinterpret_cast<const float*>(smem + S::kPar) + st * 256;
+          const float2 scales = *reinterpret_cast<const float2*>(smem + S::kScales + st * 8);
+          float x[128];
+          uint32_t* xu = reinterpret_cast<uint32_t*>(x);
+#pragma unroll
+          for (int c = 0; c < 4; ++c) tmem_ld_x32_nowait(s_tm + 32 * c, xu + 32 * c);
+          tmem_ld_wait_pin(xu);
+#pragma unroll
+          for (int c = 1; c < 4; ++c) tmem_ld_pin(xu + 32 * c);
+          if constexpr (kApart) {
+            const float2 qs2 = make_float2(qsum, qsum);
+#pragma unroll
+            for (int i = 0; i < 128; i += 4) {
+              const float4 kl = *reinterpret_cast<const float4*>(par + i);
+              const float2 a = ffma2(make_float2(kl.x, kl.y), qs2, make_float2(x[i], x[i + 1])), b = ffma2(make_float2(kl.z, kl.w), qs2, make_float2(x[i + 2], x[i + 3]));
+              x[i] = a.x, x[i + 1] = a.y, x[i + 2] = b.x, x[i + 3] = b.y;
+            }
+          }
+          const int base = s * kStep;
+          if (base + kStep - 1 > lowest) {
+            const int sees = pos - base;
+#pragma unroll
+            for (int i = 0; i < 128; ++i)
+              if (i > sees) x[i] = -INFINITY;
+          }
+          float most = -INFINITY;
+#pragma unroll
+          for (int i = 0; i < 128; i += 2) most = fmaxf(most, fmaxf(x[i], x[i + 1]));
+          const float by = rscale * scales.x;
+          most *= by;  // log2; by is positive
+          if (__any_sync(0xffffffffu, (most > off + 15.f || !seen_any) && most != -INFINITY) || scales.y != vunit) {
+            // New reference: weights are below 2^7 when it is set and below 2^15 as long as it stays.
+            const float to = most != -INFINITY && (!seen_any || most > off + 7.f) ? most - 7.f : off;
+            const float alpha = seen_any ? exp2_approx(off - to) : 0.f;
+            seen_any = seen_any || most != -INFINITY;
+            off = to;
+            l *= alpha;
+            ms *= alpha;
+            if (s > seg.s0) {
+              const float shrink = alpha * (vunit / scales.y);  // powers of two
+#pragma unroll 1
+              for (int c = 0; c < D; c += 16) {
+                uint32_t o[16];
+                tmem_ld_x16(o_tm + c, o);
+#pragma unroll
+                for (int i = 0; i < 16; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * shrink);
+                tmem_st_x16(o_tm + c, o);
+              }
+            }
+            vunit = scales.y;
+          }
+          const float2 r2 = make_float2(by, by), off2 = make_float2(-off, -off);
+          float2 l2 = make_float2(0.f, 0.f), ms2 = make_float2(0.f, 0.f);
+#pragma unroll
+          for (int c = 0; c < 4; ++c) {
+            uint32_t pk[16];
+#pragma unroll
+            for (int i = 0; i < 32; i += 4) {
+              float4 vl = make_float4(0.f, 0.f, 0.f, 0.f);
+              if constexpr (kApart) vl = *reinterpret_cast<const float4*>(par + 128 + 32 * c + i);
+#pragma unroll
+              for (int h = 0; h < 2; ++h) {
+                const int at = 32 * c + i + 2 * h;
+                const float2 y = ffma2(make_float2(x[at], x[at + 1]), r2, off2);
+                const float2 w = make_float2(exp2_approx(y.x), exp2_approx(y.y));
+                l2 = fadd2(l2, w);
+                if constexpr (kApart) ms2 = ffma2(w, h == 0 ? make_float2(vl.x, vl.y) : make_float2(vl.z, vl.w), ms2);
+                pk[(i + 2 * h) >> 1] = pack2<__half>(w.x, w.y);
+              }
+            }
+            tmem_st_x16(s_tm + 16 * c, pk);
+          }
+          l += l2.x + l2.y;
+          ms += ms2.x + ms2.y;
+          tmem_st_wait();
+          tc_fence_before_sync();
+          __syncwarp();
+          if (lane == 0) {
+            mbar_arrive(bars + kBarPFull + t);
+            mbar_arrive(bars + kBarParFree + st);
+          }
         }
-        ok = ok && wait(kBarParFull + st, (steps >> 1) & 1) && wait(kBarSFull + t, mine & 1);
+        if (active && ok) ok = wait(kBarOFull + t, items & 1);
+        if (active) ++items;
         if (!__all_sync(0xffffffffu, ok)) {
           ok = false;
-          break;
+          give_up();
         }
-        ++mine;
+        const bool gone = softmax_any(!ok || *abort_flag != 0);
+        if (gone) break;
+        // Whole items go out, parts to the workspace. O and the sums are in the same units, which cancel.
+        const bool whole = seg.s1 - seg.s0 == seg.steps;
+        const int slot = blockIdx.x * 2 + (seg.s0 > 0 ? 0 : 1), in_tile = 128 * t + row;
+        const bool there = row0 + row < p.rows;
+        const float inv = l == 0.f ? 0.f : 1.f / l;
         tc_fence_after_sync();
-        const float* par = reinterpret_cast<const float*>(smem + S::kPar) + st * 256;
-        const float2 scales = *reinterpret_cast<const float2*>(smem + S::kScales + st * 8);
-        float x[128];
-        uint32_t* xu = reinterpret_cast<uint32_t*>(x);
-#pragma unroll
-        for (int c = 0; c < 4; ++c) tmem_ld_x32_nowait(s_tm + 32 * c, xu + 32 * c);
-        tmem_ld_wait_pin(xu);
-#pragma unroll
-        for (int c = 1; c < 4; ++c) tmem_ld_pin(xu + 32 * c);
-        if constexpr (kApart) {
-          const float2 qs2 = make_float2(qsum, qsum);
-#pragma unroll
-          for (int i = 0; i < 128; i += 4) {
-            const float4 kl = *reinterpret_cast<const float4*>(par + i);
-            const float2 a = ffma2(make_float2(kl.x, kl.y), qs2, make_float2(x[i], x[i + 1])), b = ffma2(make_float2(kl.z, kl.w), qs2, make_float2(x[i + 2], x[i + 3]));
-            x[i] = a.x, x[i + 1] = a.y, x[i + 2] = b.x, x[i + 3] = b.y;
-          }
-        }
-        const int base = s * kStep;
-        if (base + kStep - 1 > lowest) {
-          const int sees = pos - base;
-#pragma unroll
-          for (int i = 0; i < 128; ++i)
-            if (i > sees) x[i] = -INFINITY;
-        }
-        float most = -INFINITY;
-#pragma unroll
-        for (int i = 0; i < 128; i += 2) most = fmaxf(most, fmaxf(x[i], x[i + 1]));
-        const float by = rscale * scales.x;
-        most *= by;  // log2; by is positive
-        if (__any_sync(0xffffffffu, (most > off + 15.f || !seen_any) && most != -INFINITY) || scales.y != vunit) {
-          // New reference: weights are below 2^7 when it is set and below 2^15 as long as it stays.
-          const float to = most != -INFINITY && (!seen_any || most > off + 7.f) ? most - 7.f : off;
-          const float alpha = seen_any ? exp2_approx(off - to) : 0.f;
-          seen_any = seen_any || most != -INFINITY;
-          off = to;
-          l *= alpha;
-          ms *= alpha;
-          if (s > seg.s0) {
-            const float shrink = alpha * (vunit / scales.y);  // powers of two
+        T* y = static_cast<T*>(p.o) + seg.b * p.os[0] + n * p.os[1] + (seg.head * p.group + g) * p.os[2];
+        float* part = p.partial + (static_cast<int64_t>(slot) * kKv4TileRows + in_tile) * D;
 #pragma unroll 1
-            for (int c = 0; c < D; c += 16) {
-              uint32_t o[16];
-              tmem_ld_x16(o_tm + c, o);
+        for (int c = 0; c < D; c += 16) {
+          float f[16];
+          if (active) {
+            tmem_ld_x16(o_tm + c, reinterpret_cast<uint32_t*>(f));
 #pragma unroll
-              for (int i = 0; i < 16; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * shrink);
-              tmem_st_x16(o_tm + c, o);
-            }
+            for (int i = 0; i < 16; ++i) f[i] = fmaf(f[i], vunit, ms);
+          } else {
+#pragma unroll
+            for (int i = 0; i < 16; ++i) f[i] = 0.f;
           }
-          vunit = scales.y;
-        }
-        const float2 r2 = make_float2(by, by), off2 = make_float2(-off, -off);
-        float2 l2 = make_float2(0.f, 0.f), ms2 = make_float2(0.f, 0.f);
+          if (!there) continue;
+          if (whole) {
 #pragma unroll
-        for (int c = 0; c < 4; ++c) {
-          uint32_t pk[16];
+            for (int i = 0; i < 16; ++i) f[i] = l == 0.f ? 0.f : f[i] * inv;
+            store8<T>(y + c, f);
+            store8<T>(y + c + 8, f + 8);
+          } else {
 #pragma unroll
-          for (int i = 0; i < 32; i += 4) {
-            float4 vl = make_float4(0.f, 0.f, 0.f, 0.f);
-            if constexpr (kApart) vl = *reinterpret_cast<const float4*>(par + 128 + 32 * c + i);
-#pragma unroll
-            for (int h = 0; h < 2; ++h) {
-              const int at = 32 * c + i + 2 * h;
-              const float2 y = ffma2(make_float2(x[at], x[at + 1]), r2, off2);
-              const float2 w = make_float2(exp2_approx(y.x), exp2_approx(y.y));
-              l2 = fadd2(l2, w);
-              if constexpr (kApart) ms2 = ffma2(w, h == 0 ? make_float2(vl.x, vl.y) : make_float2(vl.z, vl.w), ms2);
-              pk[(i + 2 * h) >> 1] = pack2<__half>(w.x, w.y);
-            }
+            for (int i = 0; i < 16; i += 4) __stcg(reinterpret_cast<float4*>(part + c + i), make_float4(f[i], f[i + 1], f[i + 2], f[i + 3]));
           }
-          tmem_st_x16(s_tm + 16 * c, pk);
         }
-        l += l2.x + l2.y;
-        ms += ms2.x + ms2.y;
-        tmem_st_wait();
         tc_fence_before_sync();
-        __syncwarp();
-        if (lane == 0) {
-          mbar_arrive(bars + kBarPFull + t);
-          mbar_arrive(bars + kBarParFree + st);
+        if (!whole) {
+          if (there) __stcg(p.partial_ml + static_cast<int64_t>(slot) * kKv4TileRows + in_tile, make_float2(seen_any ? off : -INFINITY, l));
         }
+        if (!kv4_next<kStep, kItem>(p, seg)) break;
       }
-      if (active && ok) ok = wait(kBarOFull + t, items & 1);
-      if (active) ++items;
-      if (!__all_sync(0xffffffffu, ok)) {
-        ok = false;
-        give_up();
-      }
-      const bool gone = softmax_any(!ok || *abort_flag != 0);
-      if (gone) break;
-      // Whole items go out, parts to the workspace. O and the sums are in the same units, which cancel.
-      const bool whole = seg.s1 - seg.s0 == seg.steps;
-      const int slot = blockIdx.x * 2 + (seg.s0 > 0 ? 0 : 1), in_tile = 128 * t + row;
-      const bool there = row0 + row < p.rows;
-      const float inv = l == 0.f ? 0.f : 1.f / l;
-      tc_fence_after_sync();
-      T* y = static_cast<T*>(p.o) + seg.b * p.os[0] + n * p.os[1] + (seg.head * p.group + g) * p.os[2];
-      float* part = p.partial + (static_cast<int64_t>(slot) * kKv4TileRows + in_tile) * D;
-#pragma unroll 1
-      for (int c = 0; c < D; c += 16) {
-        float f[16];
-        if (active) {
-          tmem_ld_x16(o_tm + c, reinterpret_cast<uint32_t*>(f));
-#pragma unroll
-          for (int i = 0; i < 16; ++i) f[i] = fmaf(f[i], vunit, ms);
-        } else {
-#pragma unroll
-          for (int i = 0; i < 16; ++i) f[i] = 0.f;
-        }
-        if (!there) continue;
-        if (whole) {
-#pragma unroll
-          for (int i = 0; i < 16; ++i) f[i] = l == 0.f ? 0.f : f[i] * inv;
-          store8<T>(y + c, f);
-          store8<T>(y + c + 8, f + 8);
-        } else {
-#pragma unroll
-          for (int i = 0; i < 16; i += 4) __stcg(reinterpret_cast<float4*>(part + c + i), make_float4(f[i], f[i + 1], f[i + 2], f[i + 3]));
-        }
-      }
-      tc_fence_before_sync();
-      if (!whole) {
-        if (there) __stcg(p.partial_ml + static_cast<int64_t>(slot) * kKv4TileRows + in_tile, make_float2(seen_any ? off : -INFINITY, l));
-      }
-      if (!kv4_next<kStep, kItem>(p, seg)) break;
-    }
     }
   } else if (warp < 12) {
     // ---- unpacking ----
     reg_dealloc<72>();
     if (any) {
-    const int thread = threadIdx.x & 127;
-    uint32_t steps = 0;
-    int v_exp = -100;
-    for (;;) {
-      const int seen = kv4_seen<kKv4TileRows, kStep>(p, seg);
-      for (int s = seg.s0; s < seen; ++s, ++steps) {
-        const int rs = steps & 1;
-        const uint32_t kb = 2 * steps % 3, vb = (2 * steps + 1) % 3, k_use = 2 * steps / 3, v_use = (2 * steps + 1) / 3;
-        const uint8_t* raw = smem + S::kRaw + rs * S::kRawBytes;
-        ok = ok && wait(kBarRawFull + rs, (steps >> 1) & 1) && (k_use == 0 || wait(kBarBufFree + kb, (k_use - 1) & 1)) && (steps < 2 || wait(kBarParFree + rs, ((steps >> 1) - 1) & 1));
-        // Parameters of this thread's token: zeros behind the sequence's end, where the page holds whatever it held. A token with a value that
-        // is not finite gets NaN as its key and zeros as its value, so that it shows in the rows that see it alone.
-        uint32_t k_pair, v_pair;  // (step, step), (step, rest) as halves
-        uint32_t k_rest;
-        {
-          const uint2 v = *reinterpret_cast<const uint2*>(raw + (thread >> 4) * L::kBytes + L::kV + ((thread & 15) >> 1) * L::kRowV + D + (thread & 1) * 8);
-          float ks = __uint_as_float(v.x << 16), kl = __uint_as_float(v.x & 0xffff0000u), vs = __uint_as_float(v.y << 16), vl = __uint_as_float(v.y & 0xffff0000u);
-          if (s * kStep + thread >= seg.len) ks = kl = vs = vl = 0.f;
-          kl = fmaf(8.f, ks, kl);
-          vl = fmaf(8.f, vs, vl);
-          float most_k = 8.f * ks + fabsf(kl), most_v = 8.f * vs + fabsf(vl);
-          const bool fine = most_k + most_v < INFINITY;
-          if (!fine) ks = kl = most_k = vs = vl = most_v = 0.f;
-          const uint32_t big_k = __reduce_max_sync(0xffffffffu, __float_as_uint(most_k)), big_v = __reduce_max_sync(0xffffffffu, __float_as_uint(most_v));
-          float* big = reinterpret_cast<float*>(smem + S::kBig) + rs * 8;
+      const int thread = threadIdx.x & 127;
+      uint32_t steps = 0;
+      int v_exp = -100;
+      for (;;) {
+        const int seen = kv4_seen<kKv4TileRows, kStep>(p, seg);
+        for (int s = seg.s0; s < seen; ++s, ++steps) {
+          const int rs = steps & 1;
+          const uint32_t kb = 2 * steps % 3, vb = (2 * steps + 1) % 3, k_use = 2 * steps / 3, v_use = (2 * steps + 1) / 3;
+          const uint8_t* raw = smem + S::kRaw + rs * S::kRawBytes;
+          ok = ok && wait(kBarRawFull + rs, (steps >> 1) & 1) && (k_use == 0 || wait(kBarBufFree + kb, (k_use - 1) & 1)) && (steps < 2 || wait(kBarParFree + rs, ((steps >> 1) - 1) & 1));
+          // Parameters of this thread's token: zeros behind the sequence's end, where the page holds whatever it held. A token with a value that
+          // is not finite gets NaN as its key and zeros as its value, so that it shows in the rows that see it alone.
+          uint32_t k_pair, v_pair;  // (step, step), (step, rest) as halves
+          uint32_t k_rest;
+          {
+            const uint2 v = *reinterpret_cast<const uint2*>(raw + (thread >> 4) * L::kBytes + L::kV + ((thread & 15) >> 1) * L::kRowV + D + (thread & 1) * 8);
+            float ks = __uint_as_float(v.x << 16), kl = __uint_as_float(v.x & 0xffff0000u), vs = __uint_as_float(v.y << 16), vl = __uint_as_float(v.y & 0xffff0000u);
+            if (s * kStep + thread >= seg.len) ks = kl = vs = vl = 0.f;
+            kl = fmaf(8.f, ks, kl);
+            vl = fmaf(8.f, vs, vl);
+            float most_k = 8.f * ks + fabsf(kl), most_v = 8.f * vs + fabsf(vl);
+            const bool fine = most_k + most_v < INFINITY;
+            if (!fine) ks = kl = most_k = vs = vl = most_v = 0.f;
+            const uint32_t big_k = __reduce_max_sync(0xffffffffu, __float_as_uint(most_k)), big_v = __reduce_max_sync(0xffffffffu, __float_as_uint(most_v));
+            float* big = reinterpret_cast<float*>(smem + S::kBig) + rs * 8;
+            if (lane == 0) {
+              big[warp & 3] = __uint_as_float(big_k);
+              big[4 + (warp & 3)] = __uint_as_float(big_v);
+            }
+            ok = !unpack_any(!ok);
+            if (!ok) break;
+            const float4 bk = *reinterpret_cast<const float4*>(big), bv = *reinterpret_cast<const float4*>(big + 4);
+            const int ek = tile_exponent(fmaxf(fmaxf(bk.x, bk.y), fmaxf(bk.z, bk.w)), -100);
+            v_exp = tile_exponent(fmaxf(fmaxf(bv.x, bv.y), fmaxf(bv.z, bv.w)), s == seg.s0 ? -100 : v_exp);
+            const float up_k = pow2(14 - ek), up_v = pow2(14 - v_exp);
+            k_pair = pack2<__half>(ks * up_k, ks * up_k);
+            k_rest = kApart ? 0u : pack2<__half>(kl * up_k, kl * up_k);
+            v_pair = pack2<__half>(vs * up_v, kApart ? 0.f : vl * up_v);
+            if (!fine) k_pair = k_rest = 0x7e007e00u;
+            float* par = reinterpret_cast<float*>(smem + S::kPar) + rs * 256 + thread;
+            if (kApart) {
+              par[0] = kl * up_k;
+              par[128] = vl;
+            }
+            if (thread == 0) *reinterpret_cast<float2*>(smem + S::kScales + rs * 8) = make_float2(pow2(ek - 14), pow2(v_exp - 14));
+          }
+          __syncwarp();
+          if (lane == 0) mbar_arrive(bars + kBarParFull + rs);
+          // K: a token's row, 16 bytes of codes (32 dimensions) at a time
+          uint8_t* to = smem + S::kBuf + kb * S::kTile;
+#pragma unroll
+          for (int i = 0; i < D / 32; ++i) {
+            const uint4 w = *reinterpret_cast<const uint4*>(raw + (thread >> 4) * L::kBytes + (thread & 15) * L::kRowK + 16 * i);
+            const uint32_t words[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+              uint32_t u[4];
+              centre_codes(words[k], u);
+#pragma unroll
+              for (int n = 0; n < 4; ++n) u[n] = half2_fma(u[n], k_pair, k_rest);
+              const int c = 4 * i + k;
+              *reinterpret_cast<uint4*>(to + (c >> 3) * 16384 + thread * 128 + (((c & 7) ^ (thread & 7)) << 4)) = make_uint4(u[0], u[1], u[2], u[3]);
+            }
+          }
+          fence_proxy_async_smem();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(bars + kBarBufFull + kb);
+          ok = v_use == 0 || wait(kBarBufFree + vb, (v_use - 1) & 1);
+          if (unpack_any(!ok)) {
+            ok = false;
+            break;
+          }
+          // V: 16 dimensions of two tokens at a time. Every other lane has its second token first, so that eight lanes' rows differ mod 8.
+          to = smem + S::kBuf + vb * S::kTile;
+          const int swap = lane & 1, first_half = swap ? 0x7632 : 0x5410, second_half = swap ? 0x5410 : 0x7632;
+#pragma unroll
+          for (int i = 0; i < D / 32; ++i) {
+            const int unit = (warp & 3) * (D / 32) + i;  // eight pairs of tokens (a block) by four groups of 16 dimensions
+            const int block = unit / (D / 64), group = unit % (D / 64) * 4 + (lane >> 3), pair = ((lane & 7) >> 1) + 4 * (lane & 1);
+            const uint4 w = *reinterpret_cast<const uint4*>(raw + block * L::kBytes + L::kV + pair * L::kRowV + 16 * group);
+            const uint32_t words[4] = {w.x, w.y, w.z, w.w};
+            // this warp's tokens are its lanes': steps and rests of the pair
+            const uint32_t first = __shfl_sync(0xffffffffu, v_pair, 16 * (block & 1) + 2 * pair), second = __shfl_sync(0xffffffffu, v_pair, 16 * (block & 1) + 2 * pair + 1);
+            const uint32_t v_step = __byte_perm(first, second, 0x5410), v_rest = __byte_perm(first, second, 0x7632);
+            uint32_t one[8], two[8];
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+              uint32_t u[4];
+              centre_codes(words[k], u);
+#pragma unroll
+              for (int n = 0; n < 4; ++n) u[n] = half2_fma(u[n], v_step, v_rest);
+              one[2 * k] = __byte_perm(u[0], u[1], first_half);
+              one[2 * k + 1] = __byte_perm(u[2], u[3], first_half);
+              two[2 * k] = __byte_perm(u[0], u[1], second_half);
+              two[2 * k + 1] = __byte_perm(u[2], u[3], second_half);
+            }
+            uint8_t* half = to + (group >> 2) * 16384;
+            const int r0 = 16 * block + 2 * pair + swap, r1 = r0 ^ 1, c = 2 * (group & 3);
+            *reinterpret_cast<uint4*>(half + r0 * 128 + ((c ^ (r0 & 7)) << 4)) = make_uint4(one[0], one[1], one[2], one[3]);
+            *reinterpret_cast<uint4*>(half + r0 * 128 + (((c + 1) ^ (r0 & 7)) << 4)) = make_uint4(one[4], one[5], one[6], one[7]);
+            *reinterpret_cast<uint4*>(half + r1 * 128 + ((c ^ (r1 & 7)) << 4)) = make_uint4(two[0], two[1], two[2], two[3]);
+            *reinterpret_cast<uint4*>(half + r1 * 128 + (((c + 1) ^ (r1 & 7)) << 4)) = make_uint4(two[4], two[5], two[6], two[7]);
+          }
+          fence_proxy_async_smem();
+          __syncwarp();
           if (lane == 0) {
-            big[warp & 3] = __uint_as_float(big_k);
-            big[4 + (warp & 3)] = __uint_as_float(big_v);
-          }
-          ok = !unpack_any(!ok);
-          if (!ok) break;
-          const float4 bk = *reinterpret_cast<const float4*>(big), bv = *reinterpret_cast<const float4*>(big + 4);
-          const int ek = tile_exponent(fmaxf(fmaxf(bk.x, bk.y), fmaxf(bk.z, bk.w)), -100);
-          v_exp = tile_exponent(fmaxf(fmaxf(bv.x, bv.y), fmaxf(bv.z, bv.w)), s == seg.s0 ? -100 : v_exp);
-          const float up_k = pow2(14 - ek), up_v = pow2(14 - v_exp);
-          k_pair = pack2<__half>(ks * up_k, ks * up_k);
-          k_rest = kApart ? 0u : pack2<__half>(kl * up_k, kl * up_k);
-          v_pair = pack2<__half>(vs * up_v, kApart ? 0.f : vl * up_v);
-          if (!fine) k_pair = k_rest = 0x7e007e00u;
-          float* par = reinterpret_cast<float*>(smem + S::kPar) + rs * 256 + thread;
-          if (kApart) {
-            par[0] = kl * up_k;
-            par[128] = vl;
-          }
-          if (thread == 0) *reinterpret_cast<float2*>(smem + S::kScales + rs * 8) = make_float2(pow2(ek - 14), pow2(v_exp - 14));
-        }
-        __syncwarp();
-        if (lane == 0) mbar_arrive(bars + kBarParFull + rs);
-        // K: a token's row, 16 bytes of codes (32 dimensions) at a time
-        uint8_t* to = smem + S::kBuf + kb * S::kTile;
-#pragma unroll
-        for (int i = 0; i < D / 32; ++i) {
-          const uint4 w = *reinterpret_cast<const uint4*>(raw + (thread >> 4) * L::kBytes + (thread & 15) * L::kRowK + 16 * i);
-          const uint32_t words[4] = {w.x, w.y, w.z, w.w};
-#pragma unroll
-          for (int k = 0; k < 4; ++k) {
-            uint32_t u[4];
-            centre_codes(words[k], u);
-#pragma unroll
-            for (int n = 0; n < 4; ++n) u[n] = half2_fma(u[n], k_pair, k_rest);
-            const int c = 4 * i + k;
-            *reinterpret_cast<uint4*>(to + (c >> 3) * 16384 + thread * 128 + (((c & 7) ^ (thread & 7)) << 4)) = make_uint4(u[0], u[1], u[2], u[3]);
+            mbar_arrive(bars + kBarBufFull + vb);
+            mbar_arrive(bars + kBarRawFree + rs);
           }
         }
-        fence_proxy_async_smem();
-        __syncwarp();
-        if (lane == 0) mbar_arrive(bars + kBarBufFull + kb);
-        ok = v_use == 0 || wait(kBarBufFree + vb, (v_use - 1) & 1);
-        if (unpack_any(!ok)) {
-          ok = false;
+        if (!ok) {
+          give_up();
           break;
         }
-        // V: 16 dimensions of two tokens at a time. Every other lane has its second token first, so that eight lanes' rows differ mod 8.
-        to = smem + S::kBuf + vb * S::kTile;
-        const int swap = lane & 1, first_half = swap ? 0x7632 : 0x5410, second_half = swap ? 0x5410 : 0x7632;
-#pragma unroll
-        for (int i = 0; i < D / 32; ++i) {
-          const int unit = (warp & 3) * (D / 32) + i;  // eight pairs of tokens (a block) by four groups of 16 dimensions
-          const int block = unit / (D / 64), group = unit % (D / 64) * 4 + (lane >> 3), pair = ((lane & 7) >> 1) + 4 * (lane & 1);
-          const uint4 w = *reinterpret_cast<const uint4*>(raw + block * L::kBytes + L::kV + pair * L::kRowV + 16 * group);
-          const uint32_t words[4] = {w.x, w.y, w.z, w.w};
-          // this warp's tokens are its lanes': steps and rests of the pair
-          const uint32_t first = __shfl_sync(0xffffffffu, v_pair, 16 * (block & 1) + 2 * pair), second = __shfl_sync(0xffffffffu, v_pair, 16 * (block & 1) + 2 * pair + 1);
-          const uint32_t v_step = __byte_perm(first, second, 0x5410), v_rest = __byte_perm(first, second, 0x7632);
-          uint32_t one[8], two[8];
-#pragma unroll
-          for (int k = 0; k < 4; ++k) {
-            uint32_t u[4];
-            centre_codes(words[k], u);
-#pragma unroll
-            for (int n = 0; n < 4; ++n) u[n] = half2_fma(u[n], v_step, v_rest);
-            one[2 * k] = __byte_perm(u[0], u[1], first_half);
-            one[2 * k + 1] = __byte_perm(u[2], u[3], first_half);
-            two[2 * k] = __byte_perm(u[0], u[1], second_half);
-            two[2 * k + 1] = __byte_perm(u[2], u[3], second_half);
-          }
-          uint8_t* half = to + (group >> 2) * 16384;
-          const int r0 = 16 * block + 2 * pair + swap, r1 = r0 ^ 1, c = 2 * (group & 3);
-          *reinterpret_cast<uint4*>(half + r0 * 128 + ((c ^ (r0 & 7)) << 4)) = make_uint4(one[0], one[1], one[2], one[3]);
-          *reinterpret_cast<uint4*>(half + r0 * 128 + (((c + 1) ^ (r0 & 7)) << 4)) = make_uint4(one[4], one[5], one[6], one[7]);
-          *reinterpret_cast<uint4*>(half + r1 * 128 + ((c ^ (r1 & 7)) << 4)) = make_uint4(two[0], two[1], two[2], two[3]);
-          *reinterpret_cast<uint4*>(half + r1 * 128 + (((c + 1) ^ (r1 & 7)) << 4)) = make_uint4(two[4], two[5], two[6], two[7]);
-        }
-        fence_proxy_async_smem();
-        __syncwarp();
-        if (lane == 0) {
-          mbar_arrive(bars + kBarBufFull + vb);
-          mbar_arrive(bars + kBarRawFree + rs);
-        }
+        if (!kv4_next<kStep, kItem>(p, seg)) break;
       }
-      if (!ok) {
-        give_up();
-        break;
-      }
-      if (!kv4_next<kStep, kItem>(p, seg)) break;
-    }
     }
   } else {
     reg_dealloc<72>();
@@ -497,6 +502,7 @@ __global__ void __launch_bounds__(kKv4TileThreads, 1) kv4_tiles_kernel(const Kv4
       // ---- products ----
       constexpr uint32_t idesc_s = umma_idesc_f16(UMMA_F16, 128, 128, 0, 0), idesc_o = umma_idesc_f16(UMMA_F16, 128, 64, 0, 1);
       uint32_t steps = 0, mine[2] = {0, 0}, items[2] = {0, 0};
+      uint64_t& drain = bars[kBarDrain];
       // S of tile t from K in buffer kb
       const auto issue_s = [&](int t, uint32_t kb) {
         if (elect_one()) {
@@ -563,10 +569,10 @@ __global__ void __launch_bounds__(kKv4TileThreads, 1) kv4_tiles_kernel(const Kv4
         if (!ok || !kv4_next<kStep, kItem>(p, seg)) break;
       }
       if (!ok) give_up();
-      if (__any_sync(0xffffffffu, *abort_flag != 0)) {  // products may still run: they end before tensor memory is freed
-        commit(kBarDrain);
-        mbar_wait(bars + kBarDrain, 0, abort_flag + 2);
-      }
+      // Products may still run: they end before tensor memory is freed. On every path, since another warp may give up behind a look at its flag.
+      if (elect_one()) umma_commit(&drain);
+      __syncwarp();
+      mbar_wait(&drain, 0, abort_flag + 2);
     }
   }
   tc_fence_before_sync();

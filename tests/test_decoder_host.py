@@ -247,3 +247,15 @@ def test_oracle_of_the_cache_round_trips() -> None:
     x = torch.randn(50, 128)
     step = (x.amax(-1) - x.amin(-1)) / 15
     assert ((do.quantise(x) - x.double()).abs().amax(-1) <= step * (0.5 + 15 * 2.0**-9) + x.amin(-1).abs() * 2.0**-8).all()
+
+
+def test_tiles_of_many_rows_hold_and_free_tensor_memory_in_order() -> None:
+    """The attention over many rows allocates before it lets the next kernel start, and frees behind a wait for all of its products that
+    hangs on no flag: another warp's wait may run out after this warp has looked at one. (Read, not run.)"""
+    source = next(p for p in _lib.HEADERS if p.name == "kv4_tiles_sm100.cuh").read_text()
+    body = next(b for b in source.split("__global__")[1:] if "kv4_tiles_kernel(" in b)
+    assert body.index("tmem_alloc(") < body.index("grid_launch_dependents();")
+    drained = re.search(r"if \(!ok\) give_up\(\);\s*(//[^\n]*\s*)*if \(elect_one\(\)\) umma_commit\(&drain\);\s*__syncwarp\(\);\s*mbar_wait\(&drain, 0, abort_flag \+ 2\);", body)
+    assert drained, "products are not waited for, or only under a condition"
+    assert drained.end() < body.index("tmem_dealloc(")
+    assert not re.search(r"abort_flag\[2\] = [^0a]|abort_flag \+ 2, 1", body)  # the word that this wait looks at stays zero
