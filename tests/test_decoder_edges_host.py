@@ -1,0 +1,92 @@
+"""Edges of a token decoder's layers that need no GPU: what device code does by its text, compiled for the host or read."""
+
+from __future__ import annotations
+
+import re
+import shutil
+import subprocess
+from pathlib import Path
+
+import pytest
+
+from fastforks_b200 import _lib
+
+
+def header(name: str) -> str:
+    return next(p for p in _lib.HEADERS if p.name == name).read_text()
+
+
+SPLIT_ROWS = r"""
+#include <cmath>
+#include <cstdint>
+#include <cstdio>
+#include <map>
+#define __device__
+#define __forceinline__ inline
+static float row_memory[1024], *row = row_memory;
+static std::map<int, int> writer;  // float of the row -> the lane that stored it
+static int lane_now, bad, stored;
+static void __syncwarp() {}
+static float __ldg(const float* p) { return *p; }
+static float __fmul_rn(float a, float b) { return a * b; }
+static float __fadd_rn(float a, float b) { return a + b; }
+template <typename T> void store8(T* to, const float*) {
+  for (int i = 0; i < 8; ++i) {
+    const int at = static_cast<int>(to - row) + i;
+    if (!writer.emplace(at, lane_now).second || at >= 1024) ++bad;
+    ++stored;
+  }
+}
+%(forms)s
+%(places)s
+template <int FORM> struct Turns;
+%(turns)s
+struct { int rot, dim; } p;
+int main() {
+  for (p.dim = 8; p.dim <= 512; p.dim += 8) {
+    p.rot = p.dim >= 6 ? p.dim - 2 : p.dim;
+    int lanes = 1;
+    while (16 * lanes < p.dim) lanes *= 2;
+    writer.clear();
+    bad = stored = 0;
+    for (int j = 0; j < lanes; ++j) {
+      constexpr int FORM = kRowSplit;
+      lane_now = j;
+%(kernel)s
+      (void)place_b;
+      float f[16] = {};
+      Turns<FORM> turns;
+      turns.load(nullptr, a, b, p.rot, 1.f);
+      turns.template apply<false>(f, row, p.dim, false);
+    }
+    printf("%%d %%d %%d\n", p.dim, bad, stored);
+  }
+}
+"""
+
+
+@pytest.mark.skipif(shutil.which("g++") is None, reason="needs g++")
+def test_each_place_of_a_split_row_is_stored_by_one_lane(tmp_path: Path) -> None:
+    """Halves whose partners are looked up in shared memory: a row's lanes store its values there without a barrier between one another, so
+    no float may have two writers. A row of 72, 80 or 96 has lanes that hold none of it. The kernel's own lines, run lane by lane."""
+    text = header("rotary_sm100.cuh")
+
+    def part(begin: str, end: str, start: int = 0) -> str:
+        at = text.index(begin, start)
+        return text[at : text.index(end, at) + len(end)]
+
+    kernel = text.index("rotary_stream_kernel(const RotaryParams p)")
+    source = SPLIT_ROWS % {
+        "forms": part("enum RowForm", ";"),
+        "places": part("template <int FORM>\n__device__ __forceinline__ void lane_places", "\n}\n"),
+        "turns": part("template <>\nstruct Turns<kRowSplit>", "\n};\n"),
+        "kernel": part("int a, b;", "constexpr bool kWhole", kernel).replace("constexpr bool kWhole", ""),
+    }
+    src, exe = tmp_path / "rows.cpp", tmp_path / "rows"
+    src.write_text(source)
+    subprocess.run(["g++", "-std=c++17", "-Wno-unused", "-o", str(exe), str(src)], check=True)
+    lines = subprocess.run([str(exe)], check=True, capture_output=True, text=True).stdout.split("\n")[:-1]
+    got = {int(dim): (int(bad), int(stored)) for dim, bad, stored in (line.split() for line in lines)}
+    assert sorted(got) == list(range(8, 513, 8))
+    assert {dim: n for dim, (n, _) in got.items() if n} == {}
+    assert all(stored == dim for dim, (_, stored) in got.items())  # and every float is stored
