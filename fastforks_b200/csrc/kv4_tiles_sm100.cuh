@@ -491,11 +491,9 @@ __global__ void __launch_bounds__(kKv4TileThreads, 1) kv4_tiles_kernel(const Kv4
           }
           if (!ok || !kv4_next<kStep, kItem>(p, seg)) break;
         }
-        if (!ok) {
-          give_up();
-          // the copies in flight are waited for, again with a limit
-          for (uint32_t i = steps < 2 ? 0 : steps - 2; i < steps; ++i) mbar_wait(bars + kBarRawFull + (i & 1), (i >> 1) & 1, abort_flag + 2);
-        }
+        if (!ok) give_up();
+        // Copies may still be in flight: they end before the shared memory goes. On every path, since another warp may give up when all is asked for.
+        for (uint32_t i = steps < 2 ? 0 : steps - 2; i < steps; ++i) mbar_wait(bars + kBarRawFull + (i & 1), (i >> 1) & 1, abort_flag + 2);
       }
       __syncwarp();
     } else if (any && warp == 13) {

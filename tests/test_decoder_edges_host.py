@@ -90,3 +90,24 @@ def test_each_place_of_a_split_row_is_stored_by_one_lane(tmp_path: Path) -> None
     assert sorted(got) == list(range(8, 513, 8))
     assert {dim: n for dim, (n, _) in got.items() if n} == {}
     assert all(stored == dim for dim, (_, stored) in got.items())  # and every float is stored
+
+
+def test_copies_in_flight_are_waited_for_on_every_path() -> None:
+    """The loader of the attention over many rows has asked for everything long before the others are through: a wait that runs out in
+    another warp then ends the CTA with copies on their way into its shared memory, unless the loader waits for the last of either
+    buffer whatever it has seen, with a limit and on a word that nobody raises. (Read, not run: no wait runs out on a healthy GPU.) The phases that
+    are waited for are counted here for any number of steps."""
+    source = header("kv4_tiles_sm100.cuh")
+    body = next(b for b in source.split("__global__")[1:] if "kv4_tiles_kernel(" in b)
+    loader = body[body.index("// ---- loads ----") : body.index("// ---- products ----")]
+    wait = "for (uint32_t i = steps < 2 ? 0 : steps - 2; i < steps; ++i) mbar_wait(bars + kBarRawFull + (i & 1), (i >> 1) & 1, abort_flag + 2);"
+    at = loader.index(wait)
+    begin = loader.index("if (lane == 0) {")
+    depth = loader[begin:at].count("{") - loader[begin:at].count("}")
+    assert depth == 1, "the wait is under a condition"
+    assert at > loader.rindex("bulk_load(")
+    assert not re.search(r"\breturn\b", loader[begin:at])
+    for steps in range(9):
+        waited = [(i & 1, (i >> 1) & 1) for i in range(max(0, steps - 2), steps)]
+        last = {i & 1: (i >> 1) & 1 for i in range(steps)}  # of each buffer, the phase of its last copy
+        assert dict(waited) == last and len(waited) == len(last)
