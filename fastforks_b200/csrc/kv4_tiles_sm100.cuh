@@ -20,6 +20,8 @@
 //
 #pragma once
 
+#include <float.h>
+
 #include "kv4_attn_sm100.cuh"
 
 namespace b200 {
@@ -233,7 +235,9 @@ __global__ void __launch_bounds__(kKv4TileThreads, 1) kv4_tiles_kernel(const Kv4
           float most = -INFINITY;
 #pragma unroll
           for (int i = 0; i < 128; i += 2) most = fmaxf(most, fmaxf(x[i], x[i + 1]));
-          const float by = rscale * scales.x;
+          // A row of zeros times a step of zeros leaves the range of fp32: 0 and infinity would make NaN of masked logits and of zeros. The
+          // products are below 2^33, so at the least factor they are as good as zero.
+          const float by = fminf(fmaxf(rscale * scales.x, FLT_MIN), FLT_MAX);
           most *= by;  // log2; by is positive
           if (__any_sync(0xffffffffu, (most > off + 15.f || !seen_any) && most != -INFINITY) || scales.y != vunit) {
             // New reference: weights are below 2^7 when it is set and below 2^15 as long as it stays.
