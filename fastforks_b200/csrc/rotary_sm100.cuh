@@ -553,7 +553,7 @@ __global__ void __launch_bounds__(kRotaryThreads, RotaryStream<T, MODE, FORM>::k
               sum += __shfl_xor_sync(0xffffffffu, sum, o);
               along += __shfl_xor_sync(0xffffffffu, along, o);
             }
-            const float r = rsqrtf(fmaf(sum, p.inv_dim, p.eps));
+            const float r = valid ? rsqrtf(fmaf(sum, p.inv_dim, p.eps)) : 0.f;  // no row: nothing for dw, whatever eps is
             const float back = along * r * r * p.inv_dim;  // r mean(t w x r)
 #pragma unroll
             for (int i = 0; i < 16; ++i) {
@@ -613,7 +613,7 @@ __global__ void __launch_bounds__(kRotaryThreads, 2) rotary_any_kernel(const Rot
           float sum = 0.f;
 #pragma unroll
           for (int i = 0; i < 16; ++i) sum = fmaf(f[i], f[i], sum);
-          const float r = rsqrtf(fmaf(group_sum(sum, p.lanes_log2), p.inv_dim, p.eps));
+          const float mean = fmaf(group_sum(sum, p.lanes_log2), p.inv_dim, p.eps), r = valid ? rsqrtf(mean) : 0.f;  // no row: nothing for dw, whatever eps is
           if constexpr (MODE == kNormTurn) {
 #pragma unroll
             for (int i = 0; i < 16; ++i) f[i] = f[i] * r * w[i];

@@ -1,0 +1,46 @@
+"""Edges of `rotary` and `qk_norm_rotary` on a B200 against their definitions in 64 bits. Tolerances are those of tests/test_rotary_gpu.py."""
+
+from __future__ import annotations
+
+import pytest
+import torch
+
+import fastforks_b200 as ff
+from oracle import decoder_oracle as do
+from test_rotary_gpu import DTYPES, normal, pair_size
+from test_rotary_gpu import close as close_where_finite
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.fixture(autouse=True)
+def _kernels_ran_to_the_end(request: pytest.FixtureRequest):  # noqa: ANN202
+    yield
+    assert ff.device_status() == (0 if "reports" not in request.node.name else 1 << 20)
+
+
+def close(got: torch.Tensor, ref: torch.Tensor, *rest: object) -> None:
+    """NaN is not close to anything, which a comparison for "too far" does not see."""
+    assert got.isfinite().all(), f"{int((~got.isfinite()).sum())} of {got.numel()} not finite"
+    close_where_finite(got, ref, *rest)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("heads", [(3, 5), (6, 6), (7, 1)])
+@pytest.mark.parametrize(("dim", "rot"), [(64, 64), (64, 22), (72, 72), (10, 4), (300, 128)])
+def test_gradients_without_eps(dim: int, rot: int, heads: tuple[int, int], dtype: str) -> None:
+    """With eps = 0 a head of zeros has no norm, but there is none here: places of a CTA that have no head or token count for nothing."""
+    b, n, t = 2, 37, DTYPES[dtype]
+    x = [normal(b, n, h, dim, dtype=t, seed=s).requires_grad_(True) for s, h in enumerate(heads)]
+    w = [(1 + 0.3 * normal(dim, dtype=torch.float32, seed=s)).to(t).requires_grad_(True) for s in (3, 4)]
+    g = [normal(b, n, h, dim, dtype=t, seed=5 + s) for s, h in enumerate(heads)]
+    table = ff.rotary_table(n, rot, device="cuda")
+    grads = torch.autograd.grad(ff.qk_norm_rotary(*x, *w, table, eps=0.0), (*x, *w), g)
+    for i in range(2):
+        xd, wd = x[i].detach(), w[i].detach()
+        dx, dw = do.norm_rotate_backward(xd, g[i], wd, table, None, eps=0.0, interleaved=False)
+        r = 1 / torch.sqrt(xd.double().square().mean(-1, keepdim=True))
+        hat, turned = xd.double() * r, pair_size(g[i], rot // 2, interleaved=False)
+        tw = turned * wd.double().abs()
+        close(grads[i], dx, r * (tw + hat.abs() * (tw * hat.abs()).mean(-1, keepdim=True)), 96, "dx")
+        close(grads[2 + i], dw, (turned * hat.abs()).sum((0, 1, 2)), 400, "dw")
