@@ -71,12 +71,15 @@ def rotary_table(  # noqa: PLR0913
         if original_length is None or original_length < 1:
             msg = "rotary_table: scaling 'yarn' needs original_length"
             raise ValueError(msg)
-        turns = original_length * inv / (2 * math.pi)
-        # the pair whose number of turns is beta lies at dim / 2 * ln(original_length / (2 pi beta)) / ln(base)
+        if not base > 1:
+            msg = f"rotary_table: scaling 'yarn' needs a base above 1, got {base}"
+            raise ValueError(msg)
+        # The pair whose number of turns is beta lies at dim / 2 * ln(original_length / (2 pi beta)) / ln(base). The ramp ends on whole pairs; its end may
+        # lie behind the last pair, at dim - 1 at most, as in the published method (Peng et al., YaRN, 2023).
         low, high = (dim / 2 * math.log(original_length / (2 * math.pi * beta)) / math.log(base) for beta in (beta_fast, beta_slow))
-        low, high = max(math.floor(low), 0), min(math.ceil(high), dim // 2 - 1)
+        low, high = max(math.floor(low), 0), min(math.ceil(high), dim - 1)
         kept = 1 - ((pair - low) / max(high - low, 1e-3)).clamp(0, 1)
-        inv = torch.where(turns > 0, inv * kept + inv / factor * (1 - kept), inv)
+        inv = inv * kept + inv / factor * (1 - kept)
         size = 0.1 * math.log(factor) + 1
     angle = torch.arange(length, dtype=torch.float64, device=device)[:, None] * inv
     return (torch.stack((angle.cos(), angle.sin()), 1) * size).float().contiguous()

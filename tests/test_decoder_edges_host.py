@@ -2,13 +2,16 @@
 
 from __future__ import annotations
 
+import math
 import re
 import shutil
 import subprocess
 from pathlib import Path
 
 import pytest
+import torch
 
+import fastforks_b200 as ff
 from fastforks_b200 import _lib
 
 
@@ -111,3 +114,30 @@ def test_copies_in_flight_are_waited_for_on_every_path() -> None:
         waited = [(i & 1, (i >> 1) & 1) for i in range(max(0, steps - 2), steps)]
         last = {i & 1: (i >> 1) & 1 for i in range(steps)}  # of each buffer, the phase of its last copy
         assert dict(waited) == last and len(waited) == len(last)
+
+
+@pytest.mark.parametrize(("dim", "base", "original", "factor"), [(128, 1e4, 131072, 4.0), (64, 1e4, 65536, 8.0), (128, 1e4, 2048, 4.0), (64, 500.0, 4096, 2.0), (2, 1e4, 1000, 2.0)])
+def test_yarn_divides_each_pair_by_its_number_of_turns(dim: int, base: float, original: int, factor: float) -> None:
+    """A pair's share of the plain frequency goes from one, at beta_fast turns within the original length, to none, at beta_slow, evenly over the
+    logarithm of the turns (the pairs in between are evenly spaced there): also where the slowest pair still turns more often than beta_slow.
+    The ends of the ramp lie on whole pairs, the nearest ones outside of it, which moves a pair's share by two pairs' worth at most."""
+    fast, slow = 32.0, 1.0
+    table = ff.rotary_table(2, dim, base=base, scaling="yarn", factor=factor, original_length=original)
+    plain = base ** (-2 * torch.arange(dim // 2).double() / dim)
+    ratio = torch.atan2(table[1, 1].double(), table[1, 0].double()) / plain
+    kept = (ratio - 1 / factor) / (1 - 1 / factor)
+    turns = original * plain / (2 * math.pi)
+    want = (turns.log() - math.log(slow)) / (math.log(fast) - math.log(slow))
+    pairs = dim / 2 * math.log(fast / slow) / math.log(base)  # of the ramp
+    assert ((kept - want.clamp(0, 1)).abs() <= 2 / pairs + 1e-4).all()
+    assert (kept[turns < slow] <= 1e-4 + 2 / pairs).all()
+    last = float(want[-1])
+    if last > 2 / pairs:
+        assert float(kept[-1]) > 0.0
+    assert (kept.diff() <= 1e-5).all()
+
+
+@pytest.mark.parametrize("base", [1.0, 0.5])
+def test_yarn_needs_pairs_that_get_slower(base: float) -> None:
+    with pytest.raises(ValueError, match="rotary_table"):
+        ff.rotary_table(8, 64, base=base, scaling="yarn", factor=2.0, original_length=4)
