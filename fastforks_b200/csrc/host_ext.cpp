@@ -330,9 +330,9 @@ bool fits32(const at::Tensor& t) {
     if (n > INT32_MAX) return false;
   return true;
 }
-// A plain CUDA tensor on `device` as above, which may need a gradient.
+// A plain CUDA tensor on `device` as above, which may need a gradient but carries no tangent of forward-mode differentiation.
 bool on_device(const at::Tensor& t, c10::DeviceIndex device) {
-  return t.is_cuda() && t.layout() == at::kStrided && t.device().index() == device && !t.is_conj() && !t.is_neg() && t.has_storage();
+  return t.is_cuda() && t.layout() == at::kStrided && t.device().index() == device && !t.is_conj() && !t.is_neg() && t.has_storage() && !t._fw_grad(0).defined();
 }
 bool wants_grad(const at::Tensor& t) { return t.requires_grad() && at::GradMode::is_enabled(); }
 // A plain, filled tensor of heads with unit last stride.

@@ -16,6 +16,7 @@ import threading
 import torch
 
 from . import _lib
+from .rotary import refuse_tangent
 
 BLOCK = 16  # tokens
 HEAD_DIMS = (64, 128)
@@ -100,6 +101,7 @@ def _check_heads(what: str, name: str, t: torch.Tensor, cache: torch.Tensor, dim
     if t.requires_grad and torch.is_grad_enabled():
         msg = f"{what}: {name} requires grad; the 4-bit cache is for inference (use torch.no_grad())"
         raise ValueError(msg)
+    refuse_tangent(what, name, t)
 
 
 def _fill_cache(a: _lib.B200Kv4Args | _lib.B200Kv4AttnArgs, cache: torch.Tensor, page_table: torch.Tensor, lengths: torch.Tensor, dim: int) -> None:

@@ -1,7 +1,8 @@
 """Rotary positions of heads, alone or behind the root-mean-square norm of each head, with their gradients.
 
 Host side of `b200_rotary` (include/b200_decoder.h). `rotary_table` makes the cosines and sines of a context, stretched ones
-too; `rotary` turns one tensor of heads, `qk_norm_rotary` norms and turns q and k in one launch. Both are differentiable.
+too; `rotary` turns one tensor of heads, `qk_norm_rotary` norms and turns q and k in one launch. Both are differentiable, once and backwards
+(table and positions are constants); tensors that carry a tangent of forward-mode differentiation are refused.
 `rope_qk_` remains the in-place call of DINOv3's blocks.
 """
 
@@ -103,6 +104,13 @@ def _workspace(index: int) -> torch.Tensor:
     return ws
 
 
+def refuse_tangent(what: str, name: str, t: torch.Tensor) -> None:
+    """The kernels have no forward derivative: a tensor that carries a tangent would come back without it."""
+    if torch.autograd.forward_ad.unpack_dual(t).tangent is not None:
+        msg = f"{what}: {name} carries a tangent; forward-mode differentiation is not supported"
+        raise ValueError(msg)
+
+
 def _check_heads(what: str, name: str, t: torch.Tensor, like: torch.Tensor | None = None) -> None:
     if t.dim() != 4 or t.dtype not in _DTYPES or not t.is_cuda:  # noqa: PLR2004
         msg = f"{what}: {name} must be a float16 / bfloat16 / float32 CUDA [batch, tokens, heads, dim] tensor, got {tuple(t.shape)} {t.dtype} on {t.device}"
@@ -116,6 +124,7 @@ def _check_heads(what: str, name: str, t: torch.Tensor, like: torch.Tensor | Non
     if like is not None and (t.dtype != like.dtype or t.device != like.device or t.shape[:2] != like.shape[:2] or t.shape[3] != like.shape[3]):
         msg = f"{what}: {name} {tuple(t.shape)} {t.dtype} on {t.device} does not go with {tuple(like.shape)} {like.dtype} on {like.device}"
         raise ValueError(msg)
+    refuse_tangent(what, name, t)
 
 
 def _check_table(what: str, table: torch.Tensor | None, positions: torch.Tensor | None, x: torch.Tensor) -> tuple[torch.Tensor | None, torch.Tensor | None]:
@@ -319,6 +328,7 @@ def qk_norm_rotary(  # noqa: PLR0913
         if w.shape != (q.shape[3],) or w.dtype not in (q.dtype, torch.float32) or w.dtype != weights[0].dtype or w.device != q.device or not w.is_contiguous():
             msg = f"{what}: weights must be contiguous [{q.shape[3]}] of {q.dtype} or float32 (both alike) on {q.device}, got {tuple(w.shape)} {w.dtype} on {w.device}"
             raise ValueError(msg)
+        refuse_tangent(what, "a weight", w)
     if not eps >= 0:
         msg = f"{what}: eps {eps} must not be negative"
         raise ValueError(msg)

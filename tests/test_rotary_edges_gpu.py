@@ -44,3 +44,40 @@ def test_gradients_without_eps(dim: int, rot: int, heads: tuple[int, int], dtype
         tw = turned * wd.double().abs()
         close(grads[i], dx, r * (tw + hat.abs() * (tw * hat.abs()).mean(-1, keepdim=True)), 96, "dx")
         close(grads[2 + i], dw, (turned * hat.abs()).sum((0, 1, 2)), 400, "dw")
+
+
+def test_forward_mode_is_refused() -> None:
+    """The kernels have no forward derivative: a tensor that carries a tangent is refused rather than answered without it, also where no
+    gradient is recorded, on the full way and on the way of repeated calls. Without a tangent the same calls go on."""
+    from torch.autograd import forward_ad
+
+    table = ff.rotary_table(4, 64, device="cuda")
+    x, w = normal(1, 4, 2, 64, dtype=torch.float32), torch.ones(64, device="cuda")
+    h = x.half()
+    cache, pages = ff.kv4_cache(1, 2, 64, page=16), torch.zeros(1, 1, dtype=torch.int32, device="cuda")
+    lengths = torch.full((1,), 4, dtype=torch.int32, device="cuda")
+
+    def calls(x: torch.Tensor, w: torch.Tensor, h: torch.Tensor) -> list:
+        out = torch.empty_like(h)
+        return [
+            (lambda: ff.rotary(x, table), x),
+            (lambda: ff.rotary(x, table, out=torch.empty_like(x)), x),
+            (lambda: ff.qk_norm_rotary(x, x.detach(), None, None, table), x),
+            (lambda: ff.qk_norm_rotary(w.new_ones(1, 4, 2, 64), w.new_ones(1, 4, 2, 64), w, w, table), w),
+            (lambda: ff.kv4_append_(cache, h, h, pages, lengths, table=table), h),
+            (lambda: ff.kv4_append_(cache, h.detach(), h.detach(), pages, lengths, table=table, q=h), h),
+            (lambda: ff.kv4_attention(h, cache, pages, lengths), h),
+            (lambda: ff.kv4_attention(h, cache, pages, lengths, out=out), h),
+        ]
+
+    for call, _ in calls(x, w, h):
+        call()
+    for grad in (False, True):
+        with torch.set_grad_enabled(grad), forward_ad.dual_level():
+            dual = [forward_ad.make_dual(t, torch.ones_like(t)) for t in (x, w, h)]
+            for i, (call, _) in enumerate(calls(*dual)):
+                with pytest.raises(ValueError, match="forward-mode"):
+                    call()
+                    pytest.fail(f"call {i} went through")
+            for call, _ in calls(x, w, h):
+                call()
