@@ -30,6 +30,8 @@
 // 450 or so of a step beside them; one sequence of 4000 tokens 14 us, of 100 6 us: launch, lengths, queries, first loads and the join follow one another.
 #pragma once
 
+#include <float.h>
+
 #include "kv4_sm100.cuh"
 
 namespace b200 {
@@ -449,7 +451,8 @@ __global__ void __launch_bounds__(kKv4AttnThreads, Kv4AttnSmem<D, NR, RW>::kCtas
       }
       sum += __shfl_xor_sync(0xffffffffu, sum, 1);
       sum += __shfl_xor_sync(0xffffffffu, sum, 2);
-      const float scale = p.scale_log2 * pow2(min(e + 14, 127));  // logits of this row are in units of 2^(e - 10) 2^24
+      // Logits of this row are in units of 2^(e - 10) 2^24; their factor may be neither 0 (masked logits) nor infinite (zeros).
+      const float scale = fminf(fmaxf(p.scale_log2 * pow2(min(e + 14, 127)) * pow2(max(e - 113, 0)), FLT_MIN), FLT_MAX);
 #pragma unroll
       for (int i = 0; i < 2; ++i) {
         const int from = 4 * (2 * c + i);

@@ -20,8 +20,6 @@
 //
 #pragma once
 
-#include <float.h>
-
 #include "kv4_attn_sm100.cuh"
 
 namespace b200 {

@@ -17,7 +17,7 @@ import torch
 
 import fastforks_b200 as ff
 from oracle import decoder_oracle as do
-from test_kv4_gpu import DTYPES, STATUS_PAGE, U, fill, held_tokens, normal, pages_of
+from test_kv4_gpu import DTYPES, STATUS_PAGE, U, check_attention, fill, held_tokens, normal, pages_of
 
 pytestmark = pytest.mark.gpu
 # queries and q heads on one kv head: rows for the kernel of few rows, for one tile of 128, for two, and for more
@@ -75,3 +75,31 @@ def test_zero_queries_and_keys(zero: str, rows: str, dtype: str, dim: int) -> No
     q = normal(3, n, 2 * group, dim, dtype=t, seed=3)
     q = q if zero == "keys" else torch.zeros_like(q)
     check(ff.kv4_attention(q, cache, pages, lengths), q, cache, pages, lengths, dim**-0.5)
+
+
+def check_finite(got: torch.Tensor, q: torch.Tensor, cache: torch.Tensor, pages: torch.Tensor, lengths: torch.Tensor, scale: float) -> None:
+    """The tolerance of tests/test_kv4_gpu.py (a weight times V's step is what is rounded), which NaN would pass."""
+    assert got.isfinite().all(), f"{int((~got.isfinite()).sum())} of {got.numel()} not finite"
+    check_attention(got, q, cache, pages, lengths, scale)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("rows", ROWS)
+@pytest.mark.parametrize("size", [1e-30, 1e-20, 1e-4, 1.0, 3e3, 1e20, 1e36, 1e37])
+def test_sizes_of_q(size: float, rows: str, dtype: str) -> None:
+    """Queries of any size their type has, with a scale that brings the logits back."""
+    if dtype == "fp16" and not 1e-4 <= size <= 3e3:  # noqa: PLR2004
+        pytest.skip("out of fp16's range")
+    n, group = ROWS[rows]
+    cache, pages, lengths = fill(2, 2, 64, 16, [n + 60, 7])
+    q = (normal(2, n, 2 * group, 64, dtype=torch.float32, seed=3) * size).to(DTYPES[dtype])
+    scale = 0.125 / size
+    check_finite(ff.kv4_attention(q, cache, pages, lengths, scale), q, cache, pages, lengths, scale)
+
+
+@pytest.mark.parametrize("rows", ROWS)
+def test_a_small_scale_on_zero_queries(rows: str) -> None:
+    n, group = ROWS[rows]
+    cache, pages, lengths = fill(2, 2, 128, 32, [n + 60, 7])
+    q = torch.zeros(2, n, 2 * group, 128, dtype=torch.bfloat16, device="cuda")
+    check_finite(ff.kv4_attention(q, cache, pages, lengths, 1e-30), q, cache, pages, lengths, 1e-30)
