@@ -103,3 +103,105 @@ def test_a_small_scale_on_zero_queries(rows: str) -> None:
     cache, pages, lengths = fill(2, 2, 128, 32, [n + 60, 7])
     q = torch.zeros(2, n, 2 * group, 128, dtype=torch.bfloat16, device="cuda")
     check_finite(ff.kv4_attention(q, cache, pages, lengths, 1e-30), q, cache, pages, lengths, 1e-30)
+
+
+@pytest.mark.parametrize("rows", ROWS)
+@pytest.mark.parametrize("flip", [False, True])
+def test_values_of_many_sizes(flip: bool, rows: str) -> None:
+    """V of tokens from 2^-12 to 2^12, small first and large first."""
+    n, group = ROWS[rows]
+    d, tokens = 128, 400
+    pages, total = pages_of(1, 7)
+    cache = ff.kv4_cache(total, 1, d, page=64)
+    size = torch.exp2(torch.linspace(-12, 12, tokens, device="cuda"))
+    size = size.flip(0) if flip else size
+    k, v = normal(1, tokens, 1, d, dtype=torch.float32, seed=1).bfloat16(), (normal(1, tokens, 1, d, dtype=torch.float32, seed=2) * size[:, None, None]).bfloat16()
+    lengths = torch.tensor([tokens], dtype=torch.int32, device="cuda")
+    ff.kv4_append_(cache, k, v, pages, lengths)
+    q = normal(1, n, group, d, dtype=torch.float32, seed=3).bfloat16()
+    check_finite(ff.kv4_attention(q, cache, pages, lengths), q, cache, pages, lengths, d**-0.5)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("rows", ROWS)
+@pytest.mark.parametrize("which", ["k", "v"])
+def test_nan_and_infinite_tokens(which: str, rows: str, dtype: str) -> None:
+    """A token that is held as NaN shows in the queries that see it, all of their output, and changes no bit of the others."""
+    d, t = 64, DTYPES[dtype]
+    n, group = ROWS[rows]
+    tokens = n + 137
+    for at in (tokens - 2, tokens - n + 1, 130):  # of the last queries, of all but one, of all
+        cache, pages, lengths = fill(1, 2, d, 16, [tokens], seed=5)
+        q = normal(1, n, 2 * group, d, dtype=t, seed=3)
+        k, v = ff.kv4_read(cache, pages, lengths, tokens, torch.float16)
+        ff.kv4_append_(cache, k, v, pages, lengths)
+        want = ff.kv4_attention(q, cache, pages, lengths)
+        (k if which == "k" else v)[0, at, 1, 9] = math.inf if at % 2 else math.nan
+        ff.kv4_append_(cache, k, v, pages, lengths)
+        got = ff.kv4_attention(q, cache, pages, lengths)
+        sees = torch.zeros(n, 2 * group, dtype=torch.bool, device="cuda")
+        sees[max(0, n - tokens + at) :, group:] = True
+        assert want.isfinite().all()
+        assert got[0][sees].isnan().all()
+        # the others' weights and values are what they were; but for powers of two of a step's range, so is their arithmetic
+        assert torch.allclose(got[0][~sees].double(), want[0][~sees].double(), rtol=4 * U[t], atol=2.0**-11)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("rows", ROWS)
+def test_strides_and_out(rows: str, dtype: str) -> None:
+    n, group = ROWS[rows]
+    t = DTYPES[dtype]
+    cache, pages, lengths = fill(3, 2, 128, 32, [n + 100, 1, 57])
+    packed = normal(3, n, 2 * group + 4, 128, dtype=t, seed=3)
+    q = packed[:, :, 2 : 2 * group + 2]
+    want = ff.kv4_attention(q.contiguous(), cache, pages, lengths)
+    check_finite(want, q, cache, pages, lengths, 128**-0.5)
+    assert torch.equal(ff.kv4_attention(q, cache, pages, lengths), want)
+    assert torch.equal(ff.kv4_attention(q.transpose(1, 2).contiguous().transpose(1, 2), cache, pages, lengths), want)
+    wide = torch.zeros(3, n, 2 * group, 160, dtype=t, device="cuda")
+    out = wide[..., 16:144]
+    assert ff.kv4_attention(q, cache, pages, lengths, out=out) is out
+    assert torch.equal(out, want)
+    assert not wide[..., :16].any()
+    assert not wide[..., 144:].any()
+    one = q[:, :, :1].expand_as(q)  # all heads read the same
+    assert torch.equal(ff.kv4_attention(one, cache, pages, lengths), ff.kv4_attention(one.contiguous(), cache, pages, lengths))
+
+
+@pytest.mark.parametrize("rows", ROWS)
+def test_a_graph_follows_the_lengths_and_streams_do_not_meet(rows: str) -> None:
+    n, group = ROWS[rows]
+    b, hk, d, most = 4, 2, 128, 700
+    cache, pages, lengths = fill(b, hk, d, 64, [most] * b)
+    q = normal(b, n, hk * group, d, dtype=torch.bfloat16, seed=3)
+    sets = [[700, 1, 77, 300], [3, 0, 500, 16], [700, 700, 700, 700]]
+    want = [ff.kv4_attention(q, cache, pages, torch.tensor(s, dtype=torch.int32, device="cuda")) for s in sets]
+    for s, ref in zip(sets, want, strict=True):
+        check_finite(ref, q, cache, pages, torch.tensor(s), d**-0.5)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = ff.kv4_attention(q, cache, pages, lengths)
+    for s, ref in zip(sets * 2, want * 2, strict=True):
+        lengths.copy_(torch.tensor(s, dtype=torch.int32))
+        graph.replay()
+        assert torch.equal(got, ref)
+    lengths.fill_(most)
+    streams = [torch.cuda.Stream() for _ in range(3)]
+    torch.cuda.synchronize()
+    outs = []
+    for _ in range(5):
+        for s in streams:
+            with torch.cuda.stream(s):
+                outs.append(ff.kv4_attention(q, cache, pages, lengths))
+    torch.cuda.synchronize()
+    assert all(torch.equal(o, want[2]) for o in outs)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize(("queries", "lens"), [(70, [3, 0, 70, 69]), (300, [300, 1, 299, 128]), (513, [513, 257, 0, 600])])
+def test_whole_prompts_and_padding(queries: int, lens: list[int], dtype: str) -> None:
+    """Prompts whose queries are the whole sequence, padded on the left to the longest: rows that see nothing are zeros, whole tiles of them too."""
+    cache, pages, lengths = fill(4, 2, 128, 16, lens)
+    q = normal(4, queries, 8, 128, dtype=DTYPES[dtype], seed=3)
+    check_finite(ff.kv4_attention(q, cache, pages, lengths), q, cache, pages, lengths, 128**-0.5)
