@@ -215,6 +215,21 @@ __device__ __forceinline__ bool kv4_start(const Kv4AttnParams& p, int* run, int*
   return seg->s1 > seg->s0;  // else the run ends in front of the item's first step
 }
 
+// Whether a page lies in the cache; the status says where one does not.
+__device__ __forceinline__ bool kv4_page_there(const Kv4AttnParams& p, int page) {
+  if (static_cast<uint32_t>(page) < static_cast<uint32_t>(p.pages)) return true;
+  atomicOr(p.status, kStatusPage);
+  return false;
+}
+// What stands in shared memory for a block of a page that does not: tokens held as NaN, which show in the rows that see them.
+template <int D>
+__device__ __forceinline__ void kv4_spoil(uint8_t* block) {
+  using L = Kv4Layout<D>;
+#pragma unroll 1
+  for (int i = 0; i < kKv4Block / 2; ++i) *reinterpret_cast<uint4*>(block + L::kV + i * L::kRowV + D) = make_uint4(0x7fc07fc0u, 0x7fc07fc0u, 0x7fc07fc0u, 0x7fc07fc0u);
+  fence_proxy_async_smem();  // copies will lie there again
+}
+
 // Rows of sequences without tokens are on no CTA's run: they are zeros.
 template <typename T, int D>
 __device__ __forceinline__ void write_unseen(const Kv4AttnParams& p, int threads) {
@@ -365,18 +380,14 @@ __global__ void __launch_bounds__(kKv4AttnThreads, Kv4AttnSmem<D, NR, RW>::kCtas
       ok = false;
       return;
     }
-    const auto block_at = [&](int page, int place) {
-      if (static_cast<uint32_t>(page) >= static_cast<uint32_t>(p.pages)) {
-        atomicOr(p.status, kStatusPage);
-        page = 0;
-      }
-      return base + page * page_bytes + place * S::kBlock;
-    };
     const bool two = at < two_end;  // the second block may hold nothing: what lies there is then masked
+    const bool there = kv4_page_there(p, next_page[0]), second_there = two && (joined ? there : kv4_page_there(p, next_page[1]));
     uint8_t* to = ring + stage * 2 * S::kBlock;
-    mbar_arrive_expect_tx(full + stage, two ? 2 * S::kBlock : S::kBlock);
-    bulk_load(to, block_at(next_page[0], in), two && joined ? 2 * S::kBlock : S::kBlock, full + stage);
-    if (two && !joined) bulk_load(to + S::kBlock, block_at(next_page[1], in + 1 == p.page_blocks ? 0 : in + 1), S::kBlock, full + stage);
+    if (!there) kv4_spoil<D>(to);
+    if (two && !second_there) kv4_spoil<D>(to + S::kBlock);
+    mbar_arrive_expect_tx(full + stage, (there ? S::kBlock : 0) + (second_there ? S::kBlock : 0));
+    if (there) bulk_load(to, base + next_page[0] * page_bytes + in * S::kBlock, two && joined ? 2 * S::kBlock : S::kBlock, full + stage);
+    if (second_there && !joined) bulk_load(to + S::kBlock, base + next_page[1] * page_bytes + (in + 1 == p.page_blocks ? 0 : in + 1) * S::kBlock, S::kBlock, full + stage);
     ++issued;
     if (at + kTW >= end) {
       Kv4Segment next = ahead.seg;

@@ -474,22 +474,22 @@ __global__ void __launch_bounds__(kKv4TileThreads, 1) kv4_tiles_kernel(const Kv4
             int block = 8 * s;
             const int end = min(block + 8, (seg.len + kKv4Block - 1) / kKv4Block);  // what lies behind is masked
             uint8_t* to = smem + S::kRaw + rs * S::kRawBytes;
-            mbar_arrive_expect_tx(bars + kBarRawFull + rs, (end - block) * L::kBytes);
             uint32_t col = magic_div(block, p.bpp_magic);
             int in = block - static_cast<int>(col) * p.page_blocks;
             while (block < end) {  // as many at a time as follow one another in a page
-              int page = pages[col];
-              if (static_cast<uint32_t>(page) >= static_cast<uint32_t>(p.pages)) {
-                atomicOr(p.status, kStatusPage);
-                page = 0;
+              const int page = pages[col], k = min(end - block, p.page_blocks - in);
+              if (kv4_page_there(p, page)) {
+                mbar_expect_tx(bars + kBarRawFull + rs, k * L::kBytes);
+                bulk_load(to, base + (static_cast<int64_t>(page) * p.kv_heads * p.page_blocks + in) * L::kBytes, k * L::kBytes, bars + kBarRawFull + rs);
+              } else {
+                for (int i = 0; i < k; ++i) kv4_spoil<D>(to + i * L::kBytes);
               }
-              const int k = min(end - block, p.page_blocks - in);
-              bulk_load(to, base + (static_cast<int64_t>(page) * p.kv_heads * p.page_blocks + in) * L::kBytes, k * L::kBytes, bars + kBarRawFull + rs);
               to += k * L::kBytes;
               block += k;
               ++col;
               in = 0;
             }
+            mbar_arrive(bars + kBarRawFull + rs);
           }
           if (!ok || !kv4_next<kStep, kItem>(p, seg)) break;
         }

@@ -240,7 +240,7 @@ def kv4_attention(  # noqa: PLR0913
     """Causal attention of the last `q.shape[1]` tokens of each sequence over the cache: `[batch, queries, q_heads, dim]`.
 
     Query i is at position `lengths[b] - queries + i` and sees the keys up to its own; a query in front of the sequence's start sees none
-    and gets zeros. The lengths are read on the device: work is dealt by them in equal parts whatever they are, and a captured graph
+    and gets zeros, one that sees a key on a page outside the cache gets NaN (and `device_status()` reports it). The lengths are read on the device: work is dealt by them in equal parts whatever they are, and a captured graph
     follows them. Accumulation and softmax are fp32.
 
     Args:

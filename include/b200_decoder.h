@@ -7,7 +7,8 @@
  * nothing synchronises, all work is launched on `stream` of the current device, the return value is a status code.
  * A tensor of heads is addressed as element (b, n, head, d) at ptr + b*stride[0] + n*stride[1] + head*stride[2] + d
  * (strides in elements). What a kernel finds wrong in index tensors (a position past the table, a page outside the cache)
- * reads and writes nothing out of range: the place is left out and a bit of the word that b200_attn_status returns says so.
+ * reads and writes nothing out of range, and a bit of the word that b200_attn_status returns says so: a token is not turned, a place is
+ * not written, reads as zeros, and makes NaN of the attention of queries that see it.
  */
 #ifndef B200_DECODER_H_
 #define B200_DECODER_H_
@@ -20,7 +21,7 @@ extern "C" {
 
 /* Bits of b200_attn_status that these entry points set. */
 #define B200_STATUS_POSITION (1u << 20) /* a position past the rows of the table: the token was not rotated */
-#define B200_STATUS_PAGE (1u << 21)     /* a page outside the cache, or a length past the page table: left out */
+#define B200_STATUS_PAGE (1u << 21)     /* a page outside the cache, or a length past the page table: nothing is read or written there */
 #define B200_STATUS_KV4_WAIT (1u << 22) /* attention over the cache gave up a bounded wait; its output is invalid */
 
 /* One tensor of heads and what belongs to it. */
@@ -126,7 +127,8 @@ int b200_kv4_read(const B200Kv4Args* args, void* stream);
 
 /*
  * Causal attention of the last `queries` tokens of each sequence over the cache, lengths and pages as above: query i is
- * at position lengths[b] - queries + i and sees the keys up to its own; o is zero where that leaves none. q_heads is a
+ * at position lengths[b] - queries + i and sees the keys up to its own; o is zero where that leaves none, and NaN where a key lies on
+ * a page outside the cache. A length past the page table counts as the table's end. q_heads is a
  * multiple of kv_heads, consecutive q heads share a kv head. Logits, sums and the output's accumulator are fp32; q and the
  * softmax weights go to the tensor cores as fp16 (q scaled by a power of two for each row, so that nothing is out of range).
  * `workspace`: b200_kv4_workspace bytes for partial results; `counters`: as many zeroed 32-bit words as that call

@@ -205,3 +205,28 @@ def test_whole_prompts_and_padding(queries: int, lens: list[int], dtype: str) ->
     cache, pages, lengths = fill(4, 2, 128, 16, lens)
     q = normal(4, queries, 8, 128, dtype=DTYPES[dtype], seed=3)
     check_finite(ff.kv4_attention(q, cache, pages, lengths), q, cache, pages, lengths, 128**-0.5)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("page", [16, 32])
+@pytest.mark.parametrize("rows", ROWS)
+@pytest.mark.parametrize("bad", [-1, "past", 2**31 - 1])
+def test_a_page_outside_the_cache_shows_in_the_queries_that_see_it(bad: int | str, rows: str, page: int, dtype: str) -> None:
+    """Nothing stands in for such a page, least of all another sequence's tokens: queries that see a place of it get NaN, the others what they
+    get without it, and the status says so."""
+    d, t = 64, DTYPES[dtype]
+    n, group = ROWS[rows]
+    tokens = n + 150
+    cache, pages, lengths = fill(2, 2, d, page, [tokens, tokens], seed=5)
+    q = normal(2, n, 2 * group, d, dtype=t, seed=3)
+    want = ff.kv4_attention(q, cache, pages, lengths)
+    assert want.isfinite().all()
+    for column in (0, 1, (tokens - n // 2) // page, (tokens - 1) // page):
+        broken = pages.clone()
+        broken[1, column] = cache.shape[0] if bad == "past" else bad
+        got = ff.kv4_attention(q, cache, broken, lengths)
+        assert ff.device_status() == STATUS_PAGE
+        assert torch.equal(got[0], want[0])
+        sees = tokens - n + torch.arange(n, device="cuda") >= column * page
+        assert got[1][sees].isnan().all()
+        assert torch.allclose(got[1][~sees].double(), want[1][~sees].double(), rtol=4 * U[t], atol=2.0**-11)
