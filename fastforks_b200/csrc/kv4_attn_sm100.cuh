@@ -386,8 +386,9 @@ __global__ void __launch_bounds__(kKv4AttnThreads, Kv4AttnSmem<D, NR, RW>::kCtas
     if (!there) kv4_spoil<D>(to);
     if (two && !second_there) kv4_spoil<D>(to + S::kBlock);
     mbar_arrive_expect_tx(full + stage, (there ? S::kBlock : 0) + (second_there ? S::kBlock : 0));
-    if (there) bulk_load(to, base + next_page[0] * page_bytes + in * S::kBlock, two && joined ? 2 * S::kBlock : S::kBlock, full + stage);
-    if (second_there && !joined) bulk_load(to + S::kBlock, base + next_page[1] * page_bytes + (in + 1 == p.page_blocks ? 0 : in + 1) * S::kBlock, S::kBlock, full + stage);
+    const auto block_at = [&](int page, int place) { return base + page * page_bytes + static_cast<int64_t>(place) * S::kBlock; };
+    if (there) bulk_load(to, block_at(next_page[0], in), two && joined ? 2 * S::kBlock : S::kBlock, full + stage);
+    if (second_there && !joined) bulk_load(to + S::kBlock, block_at(next_page[1], in + 1 == p.page_blocks ? 0 : in + 1), S::kBlock, full + stage);
     ++issued;
     if (at + kTW >= end) {
       Kv4Segment next = ahead.seg;

@@ -230,3 +230,38 @@ def test_a_page_outside_the_cache_shows_in_the_queries_that_see_it(bad: int | st
         sees = tokens - n + torch.arange(n, device="cuda") >= column * page
         assert got[1][sees].isnan().all()
         assert torch.allclose(got[1][~sees].double(), want[1][~sees].double(), rtol=4 * U[t], atol=2.0**-11)
+
+
+@pytest.mark.parametrize("rows", ["few", "tile"])
+@pytest.mark.parametrize("blocks", [1_875_000, 1_875_001])
+def test_blocks_behind_32_bits_of_a_page(blocks: int, rows: str) -> None:
+    """One page that holds a whole sequence of thirty million tokens: its last blocks lie more than 2^31 bytes behind its first. All but the
+    last tokens are zeros, which weigh exp(0) each beside logits of some 70 at most."""
+    d, new = 64, 40
+    n, group = ROWS[rows][0], ROWS[rows][1]
+    tokens = 16 * blocks
+    cache = ff.kv4_cache(1, 1, d, page=tokens)
+    pages, lengths = torch.zeros(1, 1, dtype=torch.int32, device="cuda"), torch.tensor([tokens], dtype=torch.int32, device="cuda")
+    k, v = (4 * normal(1, new, 1, d, dtype=torch.bfloat16, seed=1)), normal(1, new, 1, d, dtype=torch.bfloat16, seed=2)
+    ff.kv4_append_(cache, k, v, pages, lengths)
+    q = 4 * normal(1, n, group, d, dtype=torch.bfloat16, seed=3)
+    got = ff.kv4_attention(q, cache, pages, lengths)
+    small = ff.kv4_cache(4, 1, d, page=16)  # the last blocks alone: as many whole ones, with what they hold at the same places
+    small[:] = cache[:, :, -4:].transpose(0, 2)
+    table = torch.arange(4, dtype=torch.int32, device="cuda")[None]
+    held_k, held_v, pairs = held_tokens(small, table, 0, 64)
+    logits = torch.einsum("nhd,td->nht", q[0].double(), held_k[0]) * d**-0.5
+    at, last = tokens - 64 + torch.arange(64, device="cuda"), tokens - n + torch.arange(n, device="cuda")
+    logits = logits.masked_fill(at > last[:, None, None], -math.inf)
+    most = logits.amax(-1, keepdim=True).clamp(min=0.0)
+    weights = torch.exp(logits - most)
+    p = weights / (weights.sum(-1, keepdim=True) + (tokens - 64) * torch.exp(-most))
+    o = p @ held_v[0]
+    ks, kl, vs, _ = pairs[0].unbind(-1)
+    logit = d**-0.5 * q[0].double().abs().sum(-1)[..., None] * (15 * ks + kl.abs()) * 2.0**-18 + 2.0**-21
+    if rows == "tile":  # bfloat16 keys go to the tensor cores in fp16
+        logit = logit + d**-0.5 * torch.einsum("nhd,td->nht", q[0].double().abs(), 2.0**-11 * (held_k[0].abs() + (kl + 8 * ks).abs()[:, None]) + 2.0**-37 * held_k.abs().max())
+    assert float(torch.where(p > 0, logit, 0.0).max()) < 0.5  # noqa: PLR2004
+    size = held_v[0].abs() + 15 * vs[:, None]
+    bound = U[q.dtype] * o.abs() + torch.einsum("nht,td->nhd", p * (2 * logit + 2.0**-10), size) + (2 * p * logit).sum(-1)[..., None] * o.abs() + 2.0**-20
+    assert ((got[0].double() - o).abs() <= bound).all()
