@@ -235,9 +235,11 @@ template <typename T, int D>
 __device__ __forceinline__ void write_unseen(const Kv4AttnParams& p, int threads) {
   for (int b = blockIdx.x; b < p.batch; b += gridDim.x) {
     if (kv4_length(p, b) != 0) continue;
-    for (int i = threadIdx.x; i < p.queries * p.q_heads * (D / 8); i += threads) {
-      const int d = i % (D / 8), h = i / (D / 8) % p.q_heads, n = i / (D / 8) / p.q_heads;
-      *reinterpret_cast<uint4*>(static_cast<T*>(p.o) + b * p.os[0] + n * p.os[1] + h * p.os[2] + 8 * d) = make_uint4(0, 0, 0, 0);
+    const uint32_t rows = static_cast<uint32_t>(p.queries) * p.q_heads;  // below 2^31; their words of 16 bytes may be more
+    const int d = 8 * (threadIdx.x % (D / 8));
+    for (uint32_t i = threadIdx.x / (D / 8); i < rows; i += threads / (D / 8)) {
+      const uint32_t n = i / p.q_heads, h = i - n * p.q_heads;
+      *reinterpret_cast<uint4*>(static_cast<T*>(p.o) + b * p.os[0] + n * p.os[1] + h * p.os[2] + d) = make_uint4(0, 0, 0, 0);
     }
   }
 }

@@ -265,3 +265,17 @@ def test_blocks_behind_32_bits_of_a_page(blocks: int, rows: str) -> None:
     size = held_v[0].abs() + 15 * vs[:, None]
     bound = U[q.dtype] * o.abs() + torch.einsum("nht,td->nhd", p * (2 * logit + 2.0**-10), size) + (2 * p * logit).sum(-1)[..., None] * o.abs() + 2.0**-20
     assert ((got[0].double() - o).abs() <= bound).all()
+
+
+@pytest.mark.parametrize("dim", [64, 128])
+def test_zeros_of_more_than_32_bits_of_rows(dim: int) -> None:
+    """A sequence without tokens in a call whose output has 2^34 values of 16 bits and a few more: all of them are zeros. The queries are one row."""
+    heads, queries = 8, 2**34 // (8 * dim) + 3
+    cache = ff.kv4_cache(1, heads, dim, page=16)
+    pages, lengths = torch.zeros(1, 1, dtype=torch.int32, device="cuda"), torch.zeros(1, dtype=torch.int32, device="cuda")
+    q = normal(1, 1, 1, dim, dtype=torch.bfloat16, seed=3).expand(1, queries, heads, dim)
+    out = torch.full((1, queries, heads, dim), 1.0, dtype=torch.bfloat16, device="cuda")
+    ff.kv4_attention(q, cache, pages, lengths, out=out)
+    for part in out.flatten().split(2**30):
+        assert not part.any()
+    assert ff.device_status() == 0
