@@ -142,7 +142,7 @@ def _check_table(what: str, table: torch.Tensor | None, positions: torch.Tensor 
         msg = f"{what}: positions must be int32 (or int64) [{n}] or [{b}, {n}] on {x.device}, got {tuple(positions.shape)} {positions.dtype} on {positions.device}"
         raise ValueError(msg)
     else:
-        positions = positions.int()
+        positions = positions if positions.dtype == torch.int32 else positions.clamp(-1, 2**31 - 1).int()  # what 32 bits do not hold is out of range, too
     return table.contiguous(), positions
 
 

@@ -81,3 +81,17 @@ def test_forward_mode_is_refused() -> None:
                     pytest.fail(f"call {i} went through")
             for call, _ in calls(x, w, h):
                 call()
+
+
+@pytest.mark.parametrize("norm", [False, True])
+def test_a_call_reports_positions_of_64_bits(norm: bool) -> None:
+    """int64 positions mean what they say: one past 32 bits is past the table, one far below zero is negative, and neither is turned."""
+    x, table = normal(1, 5, 2, 64, dtype=torch.float32), ff.rotary_table(8, 64, device="cuda")
+    at = torch.tensor([3, 2**32 + 3, -(2**32) + 3, 2**31, -(2**63)], device="cuda")
+    want = torch.tensor([3, -1, -1, -1, -1], device="cuda", dtype=torch.int32)
+    if norm:
+        w = torch.ones(64, device="cuda")
+        got, ref = (ff.qk_norm_rotary(x, x, w, w, table, p)[0] for p in (at, want))
+    else:
+        got, ref = (ff.rotary(x, table, p) for p in (at, want))
+    assert torch.equal(got, ref)
