@@ -70,6 +70,13 @@ def reset_counters(index: int) -> None:
             counters.zero_()
 
 
+def _batch(what: str, name: str, t: torch.Tensor) -> int:
+    if t.dim() == 0:
+        msg = f"{what}: {name} has no batch dimension"
+        raise ValueError(msg)
+    return t.shape[0]
+
+
 def _check_cache(what: str, cache: torch.Tensor, page_table: torch.Tensor, lengths: torch.Tensor, batch: int) -> int:
     """The cache's head dim."""
     if cache.dim() != 4 or cache.dtype != torch.uint8 or not cache.is_cuda or not cache.is_contiguous():  # noqa: PLR2004
@@ -166,7 +173,7 @@ def kv4_append_(  # noqa: PLR0913
         if done is not None:
             return done if q is not None else None
     what = "kv4_append_"
-    dim = _check_cache(what, cache, page_table, lengths, k.shape[0])
+    dim = _check_cache(what, cache, page_table, lengths, _batch(what, "k", k))
     _check_heads(what, "k", k, cache, dim, heads=cache.shape[1])
     _check_heads(what, "v", v, cache, dim, like=k, heads=cache.shape[1])
     if q is not None:
@@ -212,7 +219,7 @@ def kv4_read(cache: torch.Tensor, page_table: torch.Tensor, lengths: torch.Tenso
         if done is not None:
             return done
     what = "kv4_read"
-    dim = _check_cache(what, cache, page_table, lengths, lengths.shape[0])
+    dim = _check_cache(what, cache, page_table, lengths, _batch(what, "lengths", lengths))
     if dtype not in _DTYPES or tokens < 0:
         msg = f"{what}: {tokens} tokens of {dtype}: expected float16 or bfloat16, and no negative count"
         raise ValueError(msg)
@@ -261,7 +268,7 @@ def kv4_attention(  # noqa: PLR0913
         if done is not None:
             return done
     what = "kv4_attention"
-    dim = _check_cache(what, cache, page_table, lengths, q.shape[0])
+    dim = _check_cache(what, cache, page_table, lengths, _batch(what, "q", q))
     _check_heads(what, "q", q, cache, dim)
     if q.shape[2] == 0 or q.shape[2] % cache.shape[1]:
         msg = f"{what}: {q.shape[2]} q heads are no multiple of {cache.shape[1]} kv heads"

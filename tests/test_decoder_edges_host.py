@@ -141,3 +141,20 @@ def test_yarn_divides_each_pair_by_its_number_of_turns(dim: int, base: float, or
 def test_yarn_needs_pairs_that_get_slower(base: float) -> None:
     with pytest.raises(ValueError, match="rotary_table"):
         ff.rotary_table(8, 64, base=base, scaling="yarn", factor=2.0, original_length=4)
+
+
+def test_operands_without_dimensions_are_refused_as_any_others() -> None:
+    nothing, none = torch.zeros(()), torch.zeros((), dtype=torch.int32)
+    cache = ff.kv4_cache(2, 2, 64, page=16, device="cpu")
+    pages, lengths = torch.zeros(1, 2, dtype=torch.int32), torch.ones(1, dtype=torch.int32)
+    for call in (
+        lambda: ff.rotary(nothing, ff.rotary_table(4, 64)),
+        lambda: ff.qk_norm_rotary(nothing, nothing, None, None, None),
+        lambda: ff.kv4_append_(cache, nothing.half(), nothing.half(), pages, lengths),
+        lambda: ff.kv4_read(cache, pages, none, 1),
+        lambda: ff.kv4_attention(nothing.half(), cache, pages, lengths),
+        lambda: ff.kv4_attention(torch.zeros(1, 1, 2, 64).half(), nothing, pages, lengths),
+        lambda: ff.kv4_attention(torch.zeros(1, 1, 2, 64).half(), cache, none, none),
+    ):
+        with pytest.raises(ValueError, match=r"rotary|kv4_"):
+            call()
