@@ -430,7 +430,7 @@ __global__ void __launch_bounds__(kRotaryThreads, RotaryStream<T, MODE, FORM>::k
   lane_places<FORM>(j, p.rot, p.dim, &a, &b);
   const int words = (p.dim + 8) >> 4;  // a row's words of eight dimensions, less those at second places
   const bool place = j < words, place_b = place && b < p.dim;
-  if (!place) a = b = p.dim;  // a lane that holds nothing of a row stores nothing of it (kRowSplit)
+  if (FORM == kRowSplit && !place) a = b = p.dim;  // a lane that holds nothing of a row stores nothing of it (kRowSplit)
   constexpr bool kWhole = FORM == kRowHalves || FORM == kRowPairs;  // every lane has both places
   float* row_smem = rotary_smem + S::kBytes / 4 + group * p.dim;  // kRowSplit
   const uint32_t run_begin = static_cast<uint32_t>(static_cast<uint64_t>(p.all_tokens) * blockIdx.x / gridDim.x);
