@@ -383,14 +383,22 @@ __global__ void __launch_bounds__(kKv4AttnThreads, Kv4AttnSmem<D, NR, RW>::kCtas
       return;
     }
     const bool two = at < two_end;  // the second block may hold nothing: what lies there is then masked
-    const bool there = kv4_page_there(p, next_page[0]), second_there = two && (joined ? there : kv4_page_there(p, next_page[1]));
     uint8_t* to = ring + stage * 2 * S::kBlock;
-    if (!there) kv4_spoil<D>(to);
-    if (two && !second_there) kv4_spoil<D>(to + S::kBlock);
-    mbar_arrive_expect_tx(full + stage, (there ? S::kBlock : 0) + (second_there ? S::kBlock : 0));
     const auto block_at = [&](int page, int place) { return base + page * page_bytes + static_cast<int64_t>(place) * S::kBlock; };
-    if (there) bulk_load(to, block_at(next_page[0], in), two && joined ? 2 * S::kBlock : S::kBlock, full + stage);
-    if (second_there && !joined) bulk_load(to + S::kBlock, block_at(next_page[1], in + 1 == p.page_blocks ? 0 : in + 1), S::kBlock, full + stage);
+    const uint32_t pages = p.pages, page0 = next_page[0], page1 = two && !joined ? next_page[1] : page0;
+    const auto load_second = [&]() { bulk_load(to + S::kBlock, block_at(page1, in + 1 == p.page_blocks ? 0 : in + 1), S::kBlock, full + stage); };
+    if (page0 < pages && page1 < pages) {
+      mbar_arrive_expect_tx(full + stage, two ? 2 * S::kBlock : S::kBlock);
+      bulk_load(to, block_at(page0, in), two && joined ? 2 * S::kBlock : S::kBlock, full + stage);
+      if (two && !joined) load_second();
+    } else {
+      atomicOr(p.status, kStatusPage);
+      if (page0 >= pages) kv4_spoil<D>(to);
+      if (page1 >= pages) kv4_spoil<D>(to + S::kBlock);
+      mbar_arrive_expect_tx(full + stage, page0 < pages || page1 < pages ? S::kBlock : 0);
+      if (page0 < pages) bulk_load(to, block_at(page0, in), S::kBlock, full + stage);
+      if (page1 < pages) load_second();
+    }
     ++issued;
     if (at + kTW >= end) {
       Kv4Segment next = ahead.seg;
