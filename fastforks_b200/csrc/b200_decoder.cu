@@ -124,7 +124,7 @@ struct AttnForm {
   int smem, rows, ctas_per_sm, threads, step, item;
 };
 // Rows of one kv head from which a call goes to the tcgen05 tiles. us, tiles and warps: 1 sequence of 9000 tokens, 64 rows 41 and 74; 8 of
-// 2000, 64 rows 40 and 44; 16 of 700 at head dim 64, 40 rows 36 and 29.
+// 2000, 64 rows 40 and 44; 16 of 700 at head dim 64, 40 rows 36 and 29. Between 40 and 64 rows, and over short contexts, nothing was measured.
 constexpr int kTileRowsLeast = 49;
 constexpr int kAttnForms = 5, kTileForm = 4;
 template <typename T, int D, int NR, int RW>

@@ -21,13 +21,17 @@
 // that four warps have 64 rows and share each step. Blocks are contiguous in the cache, and so are the two of a step where pages hold a
 // multiple of 32 tokens: bulk copies bring codes and parameters into a ring in shared memory.
 //
-// Work is laid on one line: sequences, row tiles, kv heads, steps. Each CTA takes an equal run of it, whatever the lengths are. An
+// Work is laid on one line: sequences, row tiles, kv heads, steps. Each CTA takes an equal run of it. All steps of a sequence count for each of
+// its row tiles, those behind the tile's causal limit too, which are left out when their turn comes: even for a few queries behind a long
+// text, uneven for whole prompts, where the busiest CTA has about twice the mean. An
 // item (sequence, row tile, head) cut by the end of a run is finished by the CTA that counts last: partial outputs, maxima and sums go to
 // the workspace and are joined in their order, so the result does not depend on which CTA that is.
 //
-// Measured, one query of 32 heads on 8, head dim 128, bf16: 64 sequences up to 8192 tokens (290 MB of cache) 77 to 82 us, 54 to 58 % of the copy
-// bandwidth, bound by the instructions that take codes apart (a shift and four ANDs for eight codes, on a pipe of half rate) and the
-// 450 or so of a step beside them; one sequence of 4000 tokens 14 us, of 100 6 us: launch, lengths, queries, first loads and the join follow one another.
+// Measured, one query of 32 heads on 8, head dim 128, bf16: 64 sequences up to 8192 tokens (290 MB of cache) 77 to 85 us by the pages' order, 52 to 58 %
+// of the copy bandwidth. No unit is at its end there (issue 54 %, the integer pipe that takes codes apart 51 %, DRAM 45 % of nominal): what warps wait for
+// most is the fixed latency of instructions that follow one another, at four warps a scheduler; a step has 160 instructions that take codes
+// apart and some 450 beside them. One sequence of 4000 tokens 14 us, of 1000 10, of 100 6: 6 are launch, lengths, queries and first loads, the rest is parts and
+// their join.
 #pragma once
 
 #include <float.h>

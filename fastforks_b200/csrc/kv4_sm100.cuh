@@ -4,12 +4,13 @@
 // 16 x 8 tile of the second product takes from one lane.
 //
 // A head's vector of one token is a group: step = bf16((max - min) / 15), least = bf16(min), code = clamp(round((x - least) / step)). The
-// codes are taken against the rounded pair, so rounding it costs no accuracy that the codes do not get back; the largest value may lie
-// 15 * 2^-9 of a step above the last code. Division is by multiplication with the rounded reciprocal of 15 and of the step.
+// codes are taken against the rounded pair, so they get back what its rounding costs but for the ends of the range: the largest value may
+// lie 15 * 2^-9 of a step, and either end 2^-9 of |min|, outside of what codes reach. That is below a step as long as |min| is below 34 ranges; a vector
+// whose values all lie near one large value comes back coarser (around 100 with deviation 0.25: up to 3.2 steps off). Division is by multiplication with the rounded reciprocal of 15 and of the step.
 //
-// Bound by launch latency for single tokens (append and read of 64 of them 9.8 us) and by instructions and HBM for prompts (4 x 2047 tokens,
-// 32 + 2 x 8 heads of 128, 37 and 10 us; a kernel that kept a token's place for several of its heads, and one that streamed q apart,
-// were no faster: 45 and 40 us against 41). Rows (a head of q, k or v of one token) are four or eight lanes of
+// Bound by launch latency for single tokens (64 of them: append 4.2 us, read 5.0) and by instructions and HBM for prompts (4 x 2047 tokens,
+// 32 + 2 x 8 heads of 128: append 36 us, read 10; a kernel that kept a token's place for several of its heads, and one that streamed q apart,
+// were no faster: 45 and 40 us where this one took 41 then). Rows (a head of q, k or v of one token) are four or eight lanes of
 // sixteen values, as in the rotary kernels.
 #pragma once
 

@@ -4,8 +4,8 @@
 // products take the same K and V, unpacked once for 256 rows to fp16. A code less 8 (three bits and a sign, or 8) times a step (eight bits) is
 // exact in fp16, after powers of two that put the largest value of K of the step, and of V so far, below 2^15 (a token whose step
 // is 2^26 times smaller than that loses bits). The rest of a value, least + 8 step, is treated by the type of q: in bfloat16 it is added in
-// fp16 (a value is then off by 2^-12 of itself, an eighth of what rounding the output costs), in fp16 the softmax threads put it in in
-// fp32: logit = q . (ks (u - 8)) + (kl + 8 ks) sum(q), o = sum p vs (w - 8) + sum p (vl + 8 vs).
+// fp16 (a value is then off by at most 2^-11 of itself and 2^-11 of the rest, a quarter each of what rounding the output costs; the rest is the
+// larger where a value cancels), in fp16 the softmax threads put it in in fp32: logit = q . (ks (u - 8)) + (kl + 8 ks) sum(q), o = sum p vs (w - 8) + sum p (vl + 8 vs).
 //
 // Roles: eight softmax warps (a thread has a row: S from tensor memory to registers, maximum, exponentials, P as fp16 over S's own
 // columns), four warps that unpack K and V tiles into three buffers in turn (128-byte swizzle; K as rows of tokens, V as rows of
@@ -13,11 +13,11 @@
 // next S of one tile while the other's softmax runs. Tensor memory: O 2 x head dim columns, S 2 x 128. The line of work, its runs and the
 // join of parts are those of the other kernel.
 //
-// Measured: 2 x 500 queries of 32 heads on 8 over 9000 tokens, head dim 128, bf16, 213 us, 673 TFLOP/s, 41 % of the measured dense rate (the
-// kernel of few rows took 647 us). A step of 256 rows takes some 4800 clocks, where its products need 1000 and its exponentials 2000:
-// a tile's softmax (2100), its products and the waits between them follow one another, and unpacking (3000 for both tiles by one warp on each
-// scheduler) is not much shorter (clocks are of one instrumented run).
-//
+// Measured: 2 x 500 queries of 32 heads on 8 over 9000 tokens, head dim 128, bf16, 212 us, 676 TFLOP/s, 41 % of the measured dense rate (the
+// kernel of few rows took 647 us); whole prompts, dealt unevenly as the other kernel's comment says: 1 x 2048 130 us, 265 TFLOP/s, 1 x 4096 367 us,
+// 374. A step of 256 rows takes some 4800 clocks, where its products need 1000 and its exponentials 2000: a tile's softmax (2100), its products and the
+// waits between them follow one another, and unpacking (3000 for both tiles by one warp on each scheduler) is not much shorter (clocks are of one
+// instrumented run).
 #pragma once
 
 #include "kv4_attn_sm100.cuh"
@@ -72,7 +72,8 @@ __device__ __forceinline__ uint32_t half2_fma(uint32_t a, uint32_t b, uint32_t c
   const __half2 r = __hfma2(*reinterpret_cast<const __half2*>(&a), *reinterpret_cast<const __half2*>(&b), *reinterpret_cast<const __half2*>(&c));
   return *reinterpret_cast<const uint32_t*>(&r);
 }
-// The eight codes of a word less 8, as pairs (nibble i, nibble i + 4): a code in the lowest bits of 1024 (or, times 16, of 1024) is that plus the code.
+// The eight codes of a word less 8, as pairs (nibble i, nibble i + 4), by the published conversion of small integers through the low bits of 1024 in
+// fp16: a code put there (or 16 times the code) makes 1024 plus it, and one multiply-add takes off 1024 + 8 (of a sixteenth: 64 + 8).
 __device__ __forceinline__ void centre_codes(uint32_t w, uint32_t* pairs) {
   constexpr uint32_t kOne = 0x3c003c00u, kSixteenth = 0x2c002c00u, kLow = 0xe408e408u, kHigh = 0xd480d480u;  // 1, 1 / 16, -1032, -72
   const uint32_t h = w >> 8;

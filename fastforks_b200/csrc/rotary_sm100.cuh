@@ -8,8 +8,8 @@
 // codes, which round these sums again, come out as elementwise arithmetic gives them.
 //
 // Bound by HBM: each value is read once and written once (backward with a norm: two reads). Measured, as parts of the measured copy
-// bandwidth of 6.5 TB/s: q of [32, 1029, 3, 16, 64] fp16 25.5 us (81 %), [4, 4096, 32, 128] bf16 forward and back 100 us (82 %), norms of 24 + 24
-// heads of 64 of 8 x 1370 tokens 28.2 us (73 %), of 32 + 8 heads of 128 of 2 x 4096 with all gradients 97.6 us (66 %); with a norm the
+// bandwidth of 6.5 TB/s: q of [32, 1029, 3, 16, 64] fp16 25.6 us (81 %), [4, 4096, 32, 128] bf16 forward and back 100 us (82 %), norms of 24 + 24
+// heads of 64 of 8 x 1370 tokens 28.2 us (73 %), of 32 + 8 heads of 128 of 2 x 4096 with all gradients 98.0 us (66 %); with a norm the
 // instructions weigh too (66 % of issue slots). A head is a row; 16 consecutive or
 // paired values of it are one lane's, so that a row is a group of 2, 4, 8, 16 or 32 lanes, its sums are shuffles within the group and
 // its accesses whole 16-byte words. The rows of a token are dealt to a few groups of lanes, which load the token's cosines and sines once.

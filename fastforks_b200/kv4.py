@@ -41,7 +41,7 @@ def kv4_cache(pages: int, kv_heads: int, head_dim: int, *, page: int = 64, devic
 
 
 def reserve_kv4_workspace(device: torch.device | int | None = None) -> tuple[torch.Tensor, torch.Tensor]:
-    """Scratch of the current stream of `device` for `kv4_attention`, allocated on first use: partial results (30 MB on a B200) and zeroed
+    """Scratch of the current stream of `device` for `kv4_attention`, allocated on first use: partial results (39.4 MB on a B200) and zeroed
     counters. `kv4_attention` calls this itself; called by hand on the stream of a capture, before it, it keeps the scratch out of the
     graph's own memory."""
     index = device if isinstance(device, int) else None if device is None else torch.device(device).index
@@ -247,8 +247,9 @@ def kv4_attention(  # noqa: PLR0913
     """Causal attention of the last `q.shape[1]` tokens of each sequence over the cache: `[batch, queries, q_heads, dim]`.
 
     Query i is at position `lengths[b] - queries + i` and sees the keys up to its own; a query in front of the sequence's start sees none
-    and gets zeros, one that sees a key on a page outside the cache gets NaN (and `device_status()` reports it). The lengths are read on the device: work is dealt by them in equal parts whatever they are, and a captured graph
-    follows them. Accumulation and softmax are fp32.
+    and gets zeros, one that sees a key on a page outside the cache gets NaN (and `device_status()` reports it). The lengths are read on the device: work is dealt by them in equal runs of steps, and a captured graph
+    follows them. (Steps that a tile of rows does not see count in a run too: a prompt whose queries are its whole sequence is dealt unevenly, the
+    busiest part of the GPU has about twice the mean.) Accumulation and softmax are fp32.
 
     Args:
         q: fp16 / bf16 `[batch, queries, q_heads, dim]`, already turned; q_heads a multiple of the cache's kv heads, consecutive ones
