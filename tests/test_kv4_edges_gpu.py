@@ -1,6 +1,7 @@
 """Edges of attention over the 4-bit cache, of few rows of a kv head and of many (49 and more go to kernels of their own), against 64 bits.
 
-Tolerance, element by element: the output's own rounding (U |o|); a weight is rounded to fp16, 2^-11 of it and never less than 2^-25 of a
+Tolerance of `check_finite`: that of tests/test_kv4_gpu.py. Tolerance of `check`, for weights that are all alike (powers of two, whose product with
+V's step is exact in fp16): the output's own rounding (U |o|); 2^-11 of a weight and never less than 2^-25 of a
 range that ends at 2^7, times values up to |v| (shared over the keys seen); a logit is off by 2^-18 of the sum of its magnitudes (fp32
 sums, an fp16 q of 11 bits that is exact but for values 2^-20 below a row's largest) and an exponential by 2^-21. Where q is bfloat16 and rows are
 many, K and V are rounded to fp16 themselves: least + 8 step once and the value once more, 2^-11 of either, and, below 2^-14 of the
