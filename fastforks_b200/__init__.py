@@ -5,7 +5,8 @@ interfaces the reference calls it through: `Flash64(variant)(q, k, v, scale)` on
 `scaled_dot_product_attention(q, k, v, attn_mask, scale=...)` on `[B, heads, N, 64]` views. The arithmetic runs in
 `libb200attn.so` (hand-written tcgen05 / TMA kernels, C ABI in `include/b200_attn.h`); this package holds the host
 side only and raises when that library is missing. Beside it stand a token decoder's operators (`include/b200_decoder.h`):
-`rotary`, `qk_norm_rotary` and a paged cache held in 4 bits with its causal attention (`kv4_append_`, `kv4_attention`).
+`rotary`, `qk_norm_rotary` and a paged cache held in 4 bits with its causal attention (`kv4_append_`, `kv4_attention`), and what stands between a model's
+last block and its gradients (`include/b200_training.h`): `layer_norm`, `linear_cross_entropy`, `linear_distillation`.
 """
 
 from __future__ import annotations
@@ -21,6 +22,8 @@ from .gemm import ACT_GELU, ACT_GELU_TANH, ACT_NONE, ACT_RELU, gemm
 from .flash64 import FLASH_VARIANTS, Flash64, check_flash64
 from .host_io import HostAttention
 from .kv4 import kv4_append_, kv4_attention, kv4_cache, kv4_read, reserve_kv4_workspace
+from .layer_norm import layer_norm
+from .losses import linear_cross_entropy, linear_distillation
 from .rope import rope_qk_, rope_table
 from .rotary import qk_norm_rotary, rotary, rotary_table
 from .sam import sam_rel_terms
@@ -48,6 +51,9 @@ __all__ = [
     "kv4_attention",
     "kv4_cache",
     "kv4_read",
+    "layer_norm",
+    "linear_cross_entropy",
+    "linear_distillation",
     "qk_norm_rotary",
     "reserve_kv4_workspace",
     "reserve_workspace",

@@ -30,7 +30,7 @@ if TYPE_CHECKING:
 
 LIBRARY = "b200attn"
 PACKAGE_DIR = Path(__file__).resolve().parent
-SOURCES = tuple(PACKAGE_DIR / "csrc" / name for name in ("b200_attn.cu", "b200_window.cu", "b200_linear.cu", "b200_encoder.cu", "b200_decoder.cu"))
+SOURCES = tuple(PACKAGE_DIR / "csrc" / name for name in ("b200_attn.cu", "b200_window.cu", "b200_linear.cu", "b200_encoder.cu", "b200_decoder.cu", "b200_training.cu"))
 HEADERS = (
     PACKAGE_DIR / "csrc" / "host_common.h",
     PACKAGE_DIR / "csrc" / "linear_host.h",
@@ -47,9 +47,12 @@ HEADERS = (
     PACKAGE_DIR / "csrc" / "kv4_sm100.cuh",
     PACKAGE_DIR / "csrc" / "kv4_attn_sm100.cuh",
     PACKAGE_DIR / "csrc" / "kv4_tiles_sm100.cuh",
+    PACKAGE_DIR / "csrc" / "layer_norm_sm100.cuh",
+    PACKAGE_DIR / "csrc" / "head_sm100.cuh",
     PACKAGE_DIR.parent / "include" / "b200_attn.h",
     PACKAGE_DIR.parent / "include" / "b200_encoder.h",
     PACKAGE_DIR.parent / "include" / "b200_decoder.h",
+    PACKAGE_DIR.parent / "include" / "b200_training.h",
 )
 SHARED_OBJECT = PACKAGE_DIR / "libb200attn.so"
 # The host side of repeated calls, a CPython extension over torch's C++ interface (no kernels in it).
@@ -74,6 +77,11 @@ ENCODER_EXPORTS = ("b200_encoder_workspace", "b200_encoder_forward")
 # ... and include/b200_decoder.h.
 DECODER_EXPORTS = (
     "b200_rotary", "b200_rotary_workspace", "b200_kv4_append", "b200_kv4_read", "b200_kv4_attention", "b200_kv4_workspace",
+)  # fmt: skip
+
+# ... and include/b200_training.h.
+TRAINING_EXPORTS = (
+    "b200_layer_norm", "b200_layer_norm_grad", "b200_layer_norm_workspace", "b200_head_loss", "b200_head_grad", "b200_head_sizes",
 )  # fmt: skip
 
 OK, UNSUPPORTED, BAD_CONFIG, CUDA_ERROR_BASE = 0, 1, -1, 1000
@@ -375,6 +383,70 @@ class B200Kv4AttnArgs(ctypes.Structure):
     )
 
 
+class B200LayerNormArgs(ctypes.Structure):
+    """Mirror of `struct B200LayerNormArgs` (include/b200_training.h)."""
+
+    _fields_ = (
+        ("struct_size", ctypes.c_uint32),
+        ("dtype", ctypes.c_uint32),
+        ("weight_dtype", ctypes.c_uint32),
+        ("dim", ctypes.c_int32),
+        ("rows", ctypes.c_int64),
+        ("eps", ctypes.c_float),
+        ("reserved", ctypes.c_int32),
+        ("x", ctypes.c_void_p),
+        ("x_stride", ctypes.c_int64),
+        ("y", ctypes.c_void_p),
+        ("y_stride", ctypes.c_int64),
+        ("weight", ctypes.c_void_p),
+        ("bias", ctypes.c_void_p),
+        ("stats", ctypes.c_void_p),
+        ("dy", ctypes.c_void_p),
+        ("dy_stride", ctypes.c_int64),
+        ("dx", ctypes.c_void_p),
+        ("dx_stride", ctypes.c_int64),
+        ("dweight", ctypes.c_void_p),
+        ("dbias", ctypes.c_void_p),
+        ("workspace", ctypes.c_void_p),
+        ("workspace_bytes", ctypes.c_int64),
+    )
+
+
+class B200HeadArgs(ctypes.Structure):
+    """Mirror of `struct B200HeadArgs` (include/b200_training.h)."""
+
+    _fields_ = (
+        ("struct_size", ctypes.c_uint32),
+        ("dtype", ctypes.c_uint32),
+        ("rows", ctypes.c_int32),
+        ("dim", ctypes.c_int32),
+        ("vocab", ctypes.c_int32),
+        ("top", ctypes.c_int32),
+        ("reduction", ctypes.c_int32),
+        ("target_bytes", ctypes.c_int32),
+        ("teacher_dtype", ctypes.c_uint32),
+        ("tau", ctypes.c_float),
+        ("x", ctypes.c_void_p),
+        ("ldx", ctypes.c_int64),
+        ("w", ctypes.c_void_p),
+        ("ldw", ctypes.c_int64),
+        ("targets", ctypes.c_void_p),
+        ("targets_stride", ctypes.c_int64),
+        ("ignore", ctypes.c_int64),
+        ("teacher", ctypes.c_void_p),
+        ("teacher_stride", ctypes.c_int64),
+        ("loss", ctypes.c_void_p),
+        ("state", ctypes.c_void_p),
+        ("state_bytes", ctypes.c_int64),
+        ("workspace", ctypes.c_void_p),
+        ("workspace_bytes", ctypes.c_int64),
+        ("grad", ctypes.c_void_p),
+        ("grad_stride", ctypes.c_int64),
+        ("dx", ctypes.c_void_p),
+        ("dw", ctypes.c_void_p),
+    )
+
+
 def source_hash() -> str:
     """Digest of the sources the shared object is compiled from (16 hex digits). The build passes it to the compiler,
     which puts it into the library's version string, so a binary can be matched with the sources beside it."""
@@ -500,7 +572,7 @@ def library() -> ctypes.CDLL:
         lib = ctypes.CDLL(str(SHARED_OBJECT))
     except OSError as e:
         raise KernelUnavailableError(LIBRARY, f"cannot load {SHARED_OBJECT.name}: {e}") from e
-    missing = [name for name in (*EXPORTS, *ENCODER_EXPORTS, *DECODER_EXPORTS) if not hasattr(lib, name)]
+    missing = [name for name in (*EXPORTS, *ENCODER_EXPORTS, *DECODER_EXPORTS, *TRAINING_EXPORTS) if not hasattr(lib, name)]
     if missing:
         raise KernelUnavailableError(LIBRARY, f"{SHARED_OBJECT.name} lacks the symbols {missing}")
     lib.b200_attn_fwd.argtypes = (ctypes.POINTER(B200AttnArgs), ctypes.c_void_p)
@@ -522,7 +594,12 @@ def library() -> ctypes.CDLL:
     lib.b200_kv4_attention.argtypes = (ctypes.POINTER(B200Kv4AttnArgs), ctypes.c_void_p)
     lib.b200_rotary_workspace.argtypes = (ctypes.POINTER(ctypes.c_int64),)
     lib.b200_kv4_workspace.argtypes = (ctypes.POINTER(ctypes.c_int64), ctypes.POINTER(ctypes.c_int64))
-    for name in DECODER_EXPORTS:
+    i64p = ctypes.POINTER(ctypes.c_int64)
+    lib.b200_layer_norm.argtypes = lib.b200_layer_norm_grad.argtypes = (ctypes.POINTER(B200LayerNormArgs), ctypes.c_void_p)
+    lib.b200_layer_norm_workspace.argtypes = (ctypes.POINTER(B200LayerNormArgs), i64p)
+    lib.b200_head_loss.argtypes = lib.b200_head_grad.argtypes = (ctypes.POINTER(B200HeadArgs), ctypes.c_void_p)
+    lib.b200_head_sizes.argtypes = (ctypes.POINTER(B200HeadArgs), i64p, i64p, i64p)
+    for name in (*DECODER_EXPORTS, *TRAINING_EXPORTS):
         getattr(lib, name).restype = ctypes.c_int
     lib.b200_attn_query.argtypes = (ctypes.POINTER(B200AttnArgs), ctypes.POINTER(ctypes.c_int32))
     lib.b200_attn_query.restype = ctypes.c_int

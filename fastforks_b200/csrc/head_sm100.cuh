@@ -1,0 +1,1038 @@
+// The output layer of a model and its loss, on sm_100a, without the logits. For rows x [T, D], a weight w [V, D] and logits l = x w^T:
+//
+//   cross entropy   loss_t = lse(l_t) - l_t,y                                    dl_t = g_t (softmax(l_t) - onehot_y)
+//   distillation    loss_t = tau^2 sum_k p_k (log p_k - z_t,id(k) + lse(z_t))    dl_t = g_t tau (softmax(z_t) - sum_k p_k onehot_id(k))
+//                   z = l / tau, p = softmax of the teacher's logits / tau over the row's entries
+//   dx = dl w,  dw = dl^T x
+//
+// Cross entropy is the second form with one entry of weight 1 and tau = 1; the kernels know that form alone. Rows that do not count (no
+// target, no entry) are left out of every product: where there are any, the others are copied together (head_rows_kernel) and the
+// row tiles are counted on the device.
+//
+//   head_entries_kernel  distillation: a row's p, its entropy, its entries in order of their tokens
+//   head_rows_kernel     which rows count, where they go, their copy
+//   head_stats_kernel    logits of 256 x bn tiles in tensor memory; leaves a maximum and a sum of exponentials per row and half
+//                        of a tile's columns, and the logits of the row's entries
+//   head_loss_kernel     joins those to lse and loss
+//   head_coef_kernel     gradients that differ from row to row: one power of two for all
+//   head_grads_kernel    a piece of the vocabulary: the logits again, their gradient in 16 bits
+//   head_sums_kernel     dx += G w and dw = G^T x of that piece in one launch
+//   head_dx_kernel       sums of dx, which are held in fp32, rounded and put where their rows came from
+//
+// Bound by the tensor cores: 2 T D V operations forward, 6 T D V more for the gradients, 2 T D V of which compute the logits again
+// instead of keeping them. The products are those of CTA pairs (cta_group::2, plain TMA loads, 256 x 256 tiles, two accumulators
+// in tensor memory); head_products() below is the one pipeline that all three run on.
+#pragma once
+
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+
+#include <cstddef>
+#include <type_traits>
+
+#include "gemm_sm100.cuh"
+#include "sm100_ptx.cuh"
+
+namespace b200 {
+
+constexpr uint32_t kStatusTarget = 1u << 23, kStatusHeadWait = 1u << 24;
+constexpr int kHeadThreads = 320;  // warp 0 loader, warp 1 MMA, warps 2..9 epilogue
+constexpr int kHeadRingBytes = 160 * 1024, kHeadMaxStages = 8;
+constexpr int kHeadChunkBytes = 4096;  // what an epilogue warp stages at a time: 32 rows of 128 bytes
+constexpr int kHeadBlock = 64 * 64 * 2;  // 64 values of the contiguous axis by 64 of k, an operand whose k is not contiguous
+constexpr int kNoEntry = 0x7fffffff;
+
+struct HeadSmem {
+  alignas(1024) uint8_t ring[kHeadRingBytes];          // per stage: A, 16 KB, then B
+  alignas(1024) uint8_t stage[8][2][kHeadChunkBytes];  // per epilogue warp, two deep
+  uint64_t full[kHeadMaxStages];   // the leader's: both CTAs' tiles of the stage have landed  (TMA of both CTAs)
+  uint64_t empty[kHeadMaxStages];  // the stage has been read by its products                  (MMA commit, both CTAs)
+  uint64_t acc_full[2];            // accumulator finished                                     (MMA commit, both CTAs)
+  uint64_t acc_empty[2];           // the leader's: read by the epilogue warps of both CTAs    (16 warps)
+  uint64_t drain;                  // abort path: the leader's products have finished          (MMA commit, both CTAs)
+  uint32_t tmem_base;
+  uint32_t abort;
+};
+constexpr int kHeadBarriers = 2 * kHeadMaxStages + 2 + 2 + 1;
+static_assert(offsetof(HeadSmem, drain) == offsetof(HeadSmem, full) + (kHeadBarriers - 1) * sizeof(uint64_t), "the set-up walks the barriers as one array");
+static_assert(sizeof(HeadSmem) + 1024 <= 227 * 1024, "shared memory of one CTA");
+
+// One tile of a product: rows row0 .. row0 + 255 of A, columns of B from col0 on, k-blocks kb0 .. kb1 - 1.
+struct HeadItem {
+  int kind, slot;
+  int row0, col0;
+  int kb0, kb1;
+};
+
+// The pipeline of gemm_pair_kernel with the operands' layouts, the list of tiles and the epilogue left to `job`:
+//   begin()                      reads what only the kernels in front know (after the wait for them)
+//   items(pair), item(pair, i)   this pair's tiles, the same for both CTAs and all warps
+//   stages(), stage_bytes()      the ring
+//   bytes(t), load(t, kb, ...)   one k-block of either CTA's A and B
+//   idesc(t), a_desc(), b_desc(), a_step(t), b_step(t)   what the products take; steps: 16 k-values on, in units of 16 bytes
+//   Epilogue e(job, ...); e.ask(t); e.take(t, acc, hand_back)   by each epilogue warp: before the wait for the accumulator, and after it.
+//                                `hand_back` is called once per tile, when the warp has read all it needs of the accumulator
+template <typename Job>
+__device__ __forceinline__ void head_products(Job& job, HeadSmem& sm, uint32_t* status) {
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int rank = static_cast<int>(cluster_cta_rank()), pair = blockIdx.x >> 1;
+
+  if (warp == 0) {
+    uint64_t* const first = &sm.full[0];
+    for (int i = lane; i < kHeadBarriers; i += 32) mbar_init(first + i, first + i == &sm.acc_empty[0] || first + i == &sm.acc_empty[1] ? 16 : 1);
+    if (lane == 0) sm.abort = 0;
+    mbar_init_fence();
+    __syncwarp();
+  }
+  cluster_arrive_relaxed();
+  if (warp == 0) {
+    named_barrier_arrive(1, kHeadThreads);
+  } else {
+    if (warp == 1) {
+      tmem_alloc_pair(&sm.tmem_base, 512);
+      tmem_relinquish_pair();
+    }
+    tc_fence_before_sync();
+    named_barrier_sync(1, kHeadThreads);
+    tc_fence_after_sync();
+  }
+  cluster_wait();  // the other CTA's barriers exist before anything of this one reaches for them
+  const uint32_t tmem = sm.tmem_base;  // (not the loader's)
+  volatile uint32_t* abort_flag = &sm.abort;
+  const int stages = job.stages();
+  const uint32_t stage_size = job.stage_bytes();
+
+  if (warp == 0) {
+    // ======================= loader (the whole warp, one lane issues) =================================
+    grid_dependency_wait();
+    job.begin();
+    const int n = job.items(pair);
+    bool ok = true;
+    int g = 0, st = 0;
+    uint32_t ph = 1;  // parity of the empty barriers: a ring that was never used is empty
+    for (int i = 0; i < n && ok; ++i) {
+      const HeadItem t = job.item(pair, i);
+      const uint32_t bytes = job.bytes(t);
+      for (int kb = t.kb0; kb < t.kb1; ++kb, ++g) {
+        ok = __all_sync(0xffffffffu, mbar_wait(&sm.empty[st], ph, abort_flag));
+        if (!ok) break;
+        if (elect_one()) {
+          if (rank == 0) mbar_arrive_expect_tx(&sm.full[st], bytes);
+          job.load(t, kb, rank, sm.ring + st * stage_size, cluster_map(smem_u32(&sm.full[st]), 0));  // both CTAs count on the leader's barrier
+        }
+        if (++st == stages) {
+          st = 0;
+          ph ^= 1;
+        }
+      }
+    }
+    if (!ok && lane == 0 && atomicExch(const_cast<uint32_t*>(abort_flag), 1u) == 0) atomicOr(status, kStatusHeadWait);
+    if (__any_sync(0xffffffffu, *abort_flag != 0) && rank == 0) {  // let every copy that was issued land
+      uint32_t no_abort = 0;
+      for (int j = (g > stages ? g - stages : 0); j < g; ++j) mbar_wait(&sm.full[j % stages], (j / stages) & 1, &no_abort);
+    }
+    __syncwarp();
+  } else if (warp == 1) {
+    // ======================= MMA issuer (leader only) =================================================
+    // The next kernel may start from here on: this warp's CTA holds its tensor memory.
+    grid_dependency_wait();
+    grid_launch_dependents();
+    if (rank == 0) {
+      job.begin();
+      const int n = job.items(pair);
+      bool ok = true;
+      int st = 0, it = 0;
+      uint32_t ph = 0;
+      bool landed = false;
+      for (; it < n && ok; ++it) {
+        const HeadItem t = job.item(pair, it);
+        if (it >= 2) ok = __all_sync(0xffffffffu, mbar_wait(&sm.acc_empty[it & 1], ((it >> 1) - 1) & 1, abort_flag));
+        if (!ok) break;
+        tc_fence_after_sync();
+        const uint32_t acc = tmem + (it & 1) * 256, idesc = job.idesc(t);
+        const uint64_t a0 = job.a_desc(t, smem_u32(sm.ring)), b0 = job.b_desc(t, smem_u32(sm.ring) + kGemmTileBytes);
+        const int a_step = job.a_step(t), b_step = job.b_step(t);
+        for (int kb = t.kb0; kb < t.kb1; ++kb) {
+          ok = __all_sync(0xffffffffu, landed || mbar_wait(&sm.full[st], ph, abort_flag));
+          if (!ok) break;
+          tc_fence_after_sync();
+          const int next = st + 1 == stages ? 0 : st + 1;
+          const uint32_t next_ph = st + 1 == stages ? ph ^ 1 : ph;
+          landed = mbar_test_wait(&sm.full[next], next_ph);
+          const uint64_t a = a0 + static_cast<uint64_t>(st) * (stage_size >> 4);
+          const uint64_t b = b0 + static_cast<uint64_t>(st) * (stage_size >> 4);
+          if (elect_one()) {
+#pragma unroll
+            for (int kk = 0; kk < kGemmBK / 16; ++kk) umma_ss_pair(acc, a + kk * a_step, b + kk * b_step, idesc, (kb != t.kb0 || kk != 0) ? 1u : 0u);
+            umma_commit_pair(&sm.empty[st]);
+            if (kb == t.kb1 - 1) umma_commit_pair(&sm.acc_full[it & 1]);
+          }
+          st = next;
+          ph = next_ph;
+        }
+      }
+      // The other CTA's epilogue warps signal `acc_empty` here: those of the last two items are waited for by nobody else.
+      if (ok) ok = __all_sync(0xffffffffu, lane >= min(it, 2) || mbar_wait(&sm.acc_empty[lane], ((it - 1 - lane) / 2) & 1, abort_flag));
+      if (!ok && lane == 0 && atomicExch(const_cast<uint32_t*>(abort_flag), 1u) == 0) atomicOr(status, kStatusHeadWait);
+      if (__any_sync(0xffffffffu, *abort_flag != 0)) {  // no product may be running when tensor memory is freed
+        uint32_t no_abort = 0;
+        if (elect_one()) umma_commit_pair(&sm.drain);
+        mbar_wait(&sm.drain, 0, &no_abort);
+      }
+    }
+    __syncwarp();
+  } else {
+    // ======================= epilogue warps ==========================================================
+    grid_dependency_wait();
+    job.begin();
+    const int n = job.items(pair);
+    const int e = warp - 2, part = e >> 2, quarter = warp & 3;
+    const uint32_t lane_addr = static_cast<uint32_t>(quarter * 32) << 16;
+    const uint32_t acc_empty_at[2] = {cluster_map(smem_u32(&sm.acc_empty[0]), 0), cluster_map(smem_u32(&sm.acc_empty[1]), 0)};
+    typename Job::Epilogue epilogue(job, smem_u32(sm.stage[e][0]), sm.stage[e][0], rank * 128 + quarter * 32, part);
+    bool ok = true;
+    for (int it = 0; it < n; ++it) {
+      const HeadItem t = job.item(pair, it);
+      epilogue.ask(t);
+      if (!__all_sync(0xffffffffu, mbar_wait(&sm.acc_full[it & 1], (it >> 1) & 1, abort_flag))) {
+        ok = false;
+        break;
+      }
+      tc_fence_after_sync();
+      epilogue.take(t, tmem + lane_addr + (it & 1) * 256, [&] {
+        tc_fence_before_sync();
+        __syncwarp();
+        if (lane == 0) mbar_arrive_cluster(acc_empty_at[it & 1]);
+      });
+    }
+    if (!ok && lane == 0 && atomicExch(const_cast<uint32_t*>(abort_flag), 1u) == 0) atomicOr(status, kStatusHeadWait);
+    if (lane == 0) tma_store_wait_read<0>();
+    __syncwarp();
+  }
+
+  tc_fence_before_sync();
+  __syncthreads();
+  // Neither CTA goes while the other may still multiply into its tensor memory or signal its barriers; see gemm_pair_kernel.
+  cluster_arrive_relaxed();
+  cluster_wait();
+  if (warp == 1) {
+    tc_fence_after_sync();
+    tmem_dealloc_pair(tmem, 512);
+  }
+}
+
+// The map of tiles to an order in which what runs at the same time shares operands: groups of `group` row tiles, rows fastest.
+__device__ __forceinline__ void head_raster(int tile, int tiles_m, int tiles_n, int group, int* tm, int* tn) {
+  const int per_group = group * tiles_n, g = tile / per_group, in = tile - g * per_group;
+  const int rows = min(group, tiles_m - g * group);
+  *tn = in / rows;
+  *tm = g * group + (in - *tn * rows);
+}
+
+// A tile of shared memory added to global memory (fp32); one launch adds to a place once, so the order is that of the launches.
+__device__ __forceinline__ void head_tma_add_2d(const CUtensorMap* map, const void* smem_src, int x, int y) {
+  asm volatile("cp.reduce.async.bulk.tensor.2d.global.shared::cta.add.tile.bulk_group [%0, {%2, %3}], [%1];"
+               :
+               : "l"(reinterpret_cast<uint64_t>(map)), "r"(smem_u32(smem_src)), "r"(x), "r"(y)
+               : "memory");
+}
+
+__device__ __forceinline__ float head_ex2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+
+// ---- logits: statistics, and gradients -------------------------------------------------------------------------------------------
+struct HeadLogitsParams {
+  const int* count;     // rows that count
+  const int* idx;       // [count]: which row of the caller's each is; what is indexed by rows below is by the caller's
+  int all_rows;         // rows of the caller
+  int dim, vocab;
+  int v0, tiles_n;      // first column and column tiles of this launch
+  int bn, stages, group;
+  int top;              // entries of a row
+  const int* ids;       // [all_rows, top], ascending, kNoEntry behind the last
+  const float* p;       // [all_rows, top] their weights, or null: 1
+  float log2_scale;     // log2(e) / tau
+  // statistics
+  float2* parts;        // [2 tiles_n][parts_stride]: maximum of z in units of ln 2, and the sum of 2^(z - maximum)
+  int64_t parts_stride;
+  float* picks;         // [all_rows, top]: logits of the entries
+  // gradients
+  const float* lse2;    // [all_rows], in units of ln 2
+  const float* coef;    // [all_rows] or null: 1
+  float g_scale;        // a power of two
+  uint32_t* status;
+};
+
+// G = 2^s coef_t (softmax(z_t) - p) is held in 16 bits, the operands' type: its rounding is that of an operand, 2^-9 (fp16 2^-12) of a value on
+// average below half a step, and as large in dx and dw as the rounding of their result. s = 15 for fp16, whose smallest normal
+// number is 2^-14: a softmax of 2^-29 keeps all its bits; bfloat16 has fp32's range, s = 0.
+template <typename T, bool GRADS>
+struct HeadLogitsJob {
+  const HeadLogitsParams& p;
+  const CUtensorMap *x, *x_copy, *w, *g;
+  int rows, tiles_m;
+
+  __device__ __forceinline__ HeadLogitsJob(const HeadLogitsParams& p_, const CUtensorMap* x_, const CUtensorMap* xc, const CUtensorMap* w_, const CUtensorMap* g_)
+      : p(p_), x(x_), x_copy(xc), w(w_), g(g_), rows(0), tiles_m(0) {}
+  __device__ __forceinline__ void begin() {
+    rows = __ldg(p.count);
+    tiles_m = (rows + 255) >> 8;
+    if (rows < p.all_rows) x = x_copy;
+  }
+  __device__ __forceinline__ int items(int pair) const {
+    const int tiles = tiles_m * p.tiles_n, pairs = gridDim.x >> 1;
+    return tiles > pair ? (tiles - pair + pairs - 1) / pairs : 0;
+  }
+  __device__ __forceinline__ HeadItem item(int pair, int i) const {
+    int tm, tn;
+    head_raster(pair + i * (gridDim.x >> 1), tiles_m, p.tiles_n, min(p.group, tiles_m), &tm, &tn);
+    return {0, tn, tm * 256, p.v0 + tn * p.bn, 0, (p.dim + kGemmBK - 1) / kGemmBK};
+  }
+  __device__ __forceinline__ int stages() const { return p.stages; }
+  __device__ __forceinline__ uint32_t stage_bytes() const { return kGemmTileBytes + static_cast<uint32_t>(p.bn) * kGemmBK; }
+  __device__ __forceinline__ uint32_t bytes(const HeadItem&) const { return 2u * stage_bytes(); }
+  __device__ __forceinline__ void load(const HeadItem& t, int kb, int rank, uint8_t* at, uint32_t bar) const {
+    tma_load_2d_pair(at, x, bar, kb * kGemmBK, t.row0 + rank * 128);
+    tma_load_2d_pair(at + kGemmTileBytes, w, bar, kb * kGemmBK, t.col0 + rank * (p.bn >> 1));
+  }
+  __device__ __forceinline__ uint32_t idesc(const HeadItem&) const {
+    return umma_idesc_f16(std::is_same<T, __half>::value ? UMMA_F16 : UMMA_BF16, 256, p.bn, 0, 0);
+  }
+  __device__ __forceinline__ uint64_t a_desc(const HeadItem&, uint32_t at) const { return umma_smem_desc_sw128(at, 1024, 16); }
+  __device__ __forceinline__ uint64_t b_desc(const HeadItem&, uint32_t at) const { return umma_smem_desc_sw128(at, 1024, 16); }
+  __device__ __forceinline__ int a_step(const HeadItem&) const { return 2; }
+  __device__ __forceinline__ int b_step(const HeadItem&) const { return 2; }
+
+  // A thread has a row, a warp every second 64 columns of it.
+  struct Epilogue {
+    const HeadLogitsJob& job;
+    const uint32_t stage;
+    uint8_t* const stage_ptr;
+    const int row_in, part, lane;
+    int row, src;     // this thread's row of the product, and of the caller
+    int next, pos;    // the row's first entry that has not been passed: its token, its place
+    float lse2, coef;
+    int buf;
+
+    __device__ __forceinline__ Epilogue(const HeadLogitsJob& j, uint32_t s, uint8_t* sp, int r, int pt)
+        : job(j), stage(s), stage_ptr(sp), row_in(r), part(pt), lane(threadIdx.x & 31), row(0), src(-1), next(kNoEntry), pos(0), lse2(0.f), coef(0.f), buf(0) {}
+
+    __device__ __forceinline__ int entry(int at) const { return at < job.p.top ? __ldg(job.p.ids + static_cast<int64_t>(src) * job.p.top + at) : kNoEntry; }
+
+    __device__ __forceinline__ void ask(const HeadItem& t) {
+      const HeadLogitsParams& p = job.p;
+      row = t.row0 + row_in + lane;
+      src = row < job.rows ? __ldg(p.idx + row) : -1;
+      next = kNoEntry;
+      pos = 0;
+      if (src < 0) return;
+      int hi = p.top;  // the first entry that is not in front of the tile
+      if (p.top > 1) {
+        while (pos < hi) {
+          const int mid = (pos + hi) >> 1;
+          if (entry(mid) < t.col0) pos = mid + 1;
+          else hi = mid;
+        }
+      }
+      next = entry(pos);
+      if (p.top == 1 && next < t.col0) next = kNoEntry;
+      if constexpr (GRADS) {
+        lse2 = __ldg(p.lse2 + src);
+        coef = p.coef != nullptr ? __ldg(p.coef + src) * p.g_scale : p.g_scale;
+      }
+    }
+
+    // f(j, entry) for the row's entries among the 32 columns from `base` on. Entries of the other warp's columns are passed over.
+    template <typename F>
+    __device__ __forceinline__ void for_entries(int base, F&& f) {
+      while (__any_sync(0xffffffffu, next < base + 32)) {
+        if (next < base + 32) {
+          if (next >= base) f(next - base, static_cast<int64_t>(src) * job.p.top + pos);
+          next = entry(++pos);
+        }
+      }
+    }
+
+    template <typename HandBack>
+    __device__ __forceinline__ void take(const HeadItem& t, uint32_t acc, HandBack&& hand_back) {
+      const HeadLogitsParams& p = job.p;
+      const int pieces = p.bn >> 6;
+      if constexpr (!GRADS) {
+        float m = -INFINITY, s = 0.f;
+#pragma unroll 1
+        for (int c = part; c < pieces; c += 2) {
+#pragma unroll
+          for (int half = 0; half < 2; ++half) {
+            const int base = t.col0 + c * 64 + half * 32;
+            if (base >= p.vocab) continue;
+            float v[32];
+            tmem_ld_x32(acc + c * 64 + half * 32, reinterpret_cast<uint32_t*>(v));
+            for_entries(base, [&](int j, int64_t at) {
+              float got = 0.f;
+#pragma unroll
+              for (int i = 0; i < 32; ++i) got = i == j ? v[i] : got;
+              p.picks[at] = got;
+            });
+            if (base + 32 > p.vocab) {
+#pragma unroll
+              for (int i = 0; i < 32; ++i) v[i] = base + i < p.vocab ? v[i] : -INFINITY;
+            }
+            float top = v[0];
+#pragma unroll
+            for (int i = 1; i < 32; ++i) top = fmaxf(top, v[i]);
+            const float m_new = fmaxf(m, top * p.log2_scale), from = m_new == -INFINITY ? 0.f : m_new;
+            const float2 scale2 = make_float2(p.log2_scale, p.log2_scale), from2 = make_float2(-from, -from);
+            float2 sum = make_float2(0.f, 0.f);
+#pragma unroll
+            for (int i = 0; i < 32; i += 2) {
+              const float2 z = ffma2(make_float2(v[i], v[i + 1]), scale2, from2);
+              sum = fadd2(sum, make_float2(head_ex2(z.x), head_ex2(z.y)));
+            }
+            s = s * head_ex2(m - from) + (sum.x + sum.y);
+            m = m_new;
+          }
+        }
+        hand_back();
+        if (row < job.rows) p.parts[(2 * t.slot + part) * p.parts_stride + row] = make_float2(m, s);
+      } else {
+        const bool partial = t.row0 + row_in + 32 > job.rows;  // rows behind the last are zeros: the products over rows read them
+#pragma unroll 1
+        for (int c = part; c < pieces; c += 2) {
+          const int col = t.col0 + c * 64;
+          const bool here = col < p.vocab;
+          if (lane == 0) tma_store_wait_read<1>();  // the store that used this buffer last has read it
+          __syncwarp();
+          if (here) {
+            const uint32_t at_row = stage + buf * kHeadChunkBytes + lane * 128;
+#pragma unroll
+            for (int half = 0; half < 2; ++half) {
+              const int base = col + half * 32;
+              float v[32];
+              tmem_ld_x32(acc + c * 64 + half * 32, reinterpret_cast<uint32_t*>(v));
+              const float2 scale2 = make_float2(p.log2_scale, p.log2_scale), from2 = make_float2(-lse2, -lse2), coef2 = make_float2(coef, coef);
+#pragma unroll
+              for (int i = 0; i < 32; i += 2) {
+                const float2 z = ffma2(make_float2(v[i], v[i + 1]), scale2, from2);
+                v[i] = head_ex2(z.x);
+                v[i + 1] = head_ex2(z.y);
+              }
+              for_entries(base, [&](int j, int64_t at) {
+                const float weight = p.p != nullptr ? __ldg(p.p + at) : 1.f;
+#pragma unroll
+                for (int i = 0; i < 32; ++i) v[i] -= i == j ? weight : 0.f;
+              });
+              if (base + 32 > p.vocab) {
+#pragma unroll
+                for (int i = 0; i < 32; ++i) v[i] = base + i < p.vocab ? v[i] : 0.f;
+              }
+              uint32_t out[16];
+#pragma unroll
+              for (int i = 0; i < 16; ++i) {
+                const float2 y = fmul2(make_float2(v[2 * i], v[2 * i + 1]), coef2);
+                out[i] = gemm_pack2<T>(y.x, y.y);
+              }
+              if (partial) {
+#pragma unroll
+                for (int i = 0; i < 16; ++i) out[i] = row < job.rows ? out[i] : 0u;
+              }
+#pragma unroll
+              for (int q = 0; q < 4; ++q)
+                st_shared_v4(at_row + (((4 * half + q) ^ (lane & 7)) << 4), make_uint4(out[4 * q], out[4 * q + 1], out[4 * q + 2], out[4 * q + 3]));
+            }
+            fence_proxy_async_smem();
+          }
+          if (c + 2 >= pieces) hand_back();
+          else __syncwarp();
+          if (lane == 0) {
+            if (here) tma_store_2d(job.g, stage_ptr + buf * kHeadChunkBytes, col - p.v0, t.row0 + row_in);
+            tma_store_commit();
+          }
+          buf ^= 1;
+        }
+        if (part >= pieces) hand_back();
+      }
+    }
+  };
+};
+
+// ---- sums: dx and dw of a piece ------------------------------------------------------------------------------------------------------
+// What the sums are multiplied by: everything that is the same for all rows.
+struct HeadScale {
+  const float* grad;  // gradient of a loss that is one number, or null
+  const float* norm;  // what head_coef_kernel divided the rows' gradients by, or null
+  const int* count;   // mean: rows that count, else null
+  float constant;     // tau / 2^s
+};
+__device__ __forceinline__ float head_scale(const HeadScale& s) {
+  float v = s.constant;
+  if (s.grad != nullptr) v *= __ldg(s.grad);
+  if (s.norm != nullptr) v *= __ldg(s.norm);
+  if (s.count != nullptr) v /= static_cast<float>(max(__ldg(s.count), 1));
+  return v;
+}
+
+struct HeadSumsParams {
+  const int* count;
+  int all_rows, dim, vocab;
+  int v0, cols;       // the piece: columns v0 .. v0 + cols - 1, cols a multiple of 256 or up to the last
+  int splits;         // parts of the piece's columns that dx is summed over, 0: no dx
+  int want_dw;
+  int bn, stages;
+  int first;          // the first piece: dx begins
+  int64_t slot_rows;  // rows of a part's sums, a multiple of 256
+  HeadScale scale;
+  uint32_t* status;
+};
+
+// kind 0: dx rows (tile of G, k along the piece's columns) x w (k not contiguous), fp32 sums that later pieces are added to;
+// kind 1: dw rows (G as the left operand, its rows as k: not contiguous) x rows of x (not contiguous), final.
+// An operand whose k is not contiguous comes as blocks of 64 k by 64 values, 128-byte rows with the swizzle: 8 KB from one block of
+// values to the next, 1 KB from eight k to the next.
+//
+// The tiles of dx are long (k is the piece) and those of dw short (k counts rows): every pair takes its share of the long ones first, and the
+// pairs with one fewer take so many short ones ahead of the others.
+template <typename T>
+struct HeadSumsJob {
+  const HeadSumsParams& p;
+  const CUtensorMap *g_k, *g_mn, *w, *x, *x_copy, *dx, *dw;
+  int rows, row_tiles, col_tiles, v_tiles, dx_items, pairs;
+
+  __device__ __forceinline__ HeadSumsJob(const HeadSumsParams& p_, const CUtensorMap* gk, const CUtensorMap* gm, const CUtensorMap* w_, const CUtensorMap* x_,
+                                         const CUtensorMap* xc, const CUtensorMap* dx_, const CUtensorMap* dw_)
+      : p(p_), g_k(gk), g_mn(gm), w(w_), x(x_), x_copy(xc), dx(dx_), dw(dw_) {}
+  __device__ __forceinline__ void begin() {
+    rows = __ldg(p.count);
+    if (rows < p.all_rows) x = x_copy;
+    pairs = gridDim.x >> 1;
+    row_tiles = (rows + 255) >> 8;
+    col_tiles = (p.dim + p.bn - 1) / p.bn;
+    v_tiles = (p.cols + 255) >> 8;
+    dx_items = row_tiles * col_tiles * p.splits;
+  }
+  // Short tiles that a pair with one long tile fewer takes first, of `behind` pairs.
+  __device__ __forceinline__ void ahead(int* behind, int* each) const {
+    const int rest = dx_items % pairs;
+    *behind = rest == 0 ? 0 : pairs - rest;
+    const int long_k = (p.cols + 63) / 64 / max(p.splits, 1), short_k = max(1, (rows + 63) / 64);
+    *each = *behind == 0 ? 0 : long_k / short_k;
+  }
+  __device__ __forceinline__ int items(int pair) const {
+    const int n_dw = p.want_dw ? v_tiles * col_tiles : 0;
+    int n = dx_items > pair ? (dx_items - pair + pairs - 1) / pairs : 0;
+    int behind, each;
+    ahead(&behind, &each);
+    const int early = min(n_dw, behind * each), mine = pair - (pairs - behind);
+    if (mine >= 0 && early > mine) n += (early - mine + behind - 1) / behind;
+    const int late = n_dw - early;
+    return n + (late > pair ? (late - pair + pairs - 1) / pairs : 0);
+  }
+  __device__ __forceinline__ HeadItem item(int pair, int i) const {
+    const int long_ones = dx_items > pair ? (dx_items - pair + pairs - 1) / pairs : 0;
+    if (i < long_ones) {
+      const int at = pair + i * pairs, tiles = row_tiles * col_tiles, slot = at / tiles;
+      int tm, tn;
+      head_raster(at - slot * tiles, row_tiles, col_tiles, min(8, row_tiles), &tm, &tn);
+      const int kbs = (p.cols + 63) / 64;
+      return {0, slot, tm * 256, tn * p.bn, static_cast<int>(static_cast<int64_t>(kbs) * slot / p.splits), static_cast<int>(static_cast<int64_t>(kbs) * (slot + 1) / p.splits)};
+    }
+    i -= long_ones;
+    const int n_dw = v_tiles * col_tiles;
+    int behind, each;
+    ahead(&behind, &each);
+    const int early = min(n_dw, behind * each), mine = pair - (pairs - behind);
+    const int my_early = mine >= 0 && early > mine ? (early - mine + behind - 1) / behind : 0;
+    const int at = i < my_early ? mine + i * behind : early + pair + (i - my_early) * pairs;
+    int tm, tn;
+    head_raster(at, v_tiles, col_tiles, min(8, v_tiles), &tm, &tn);
+    return {1, 0, tm * 256, tn * p.bn, 0, max(1, (rows + 63) / 64)};  // (no row counts: a product all the same, of whatever is there, and zeros stored)
+  }
+  __device__ __forceinline__ int stages() const { return p.stages; }
+  __device__ __forceinline__ uint32_t stage_bytes() const { return kGemmTileBytes + static_cast<uint32_t>(p.bn) * kGemmBK; }
+  __device__ __forceinline__ uint32_t bytes(const HeadItem&) const { return 2u * stage_bytes(); }
+  __device__ __forceinline__ void load(const HeadItem& t, int kb, int rank, uint8_t* at, uint32_t bar) const {
+    const int k = kb * kGemmBK, half = p.bn >> 1;
+    if (t.kind == 0) {
+      tma_load_2d_pair(at, g_k, bar, k, t.row0 + rank * 128);
+    } else {
+      tma_load_2d_pair(at, g_mn, bar, t.row0 + rank * 128, k);
+      tma_load_2d_pair(at + kHeadBlock, g_mn, bar, t.row0 + rank * 128 + 64, k);
+    }
+    const CUtensorMap* b = t.kind == 0 ? w : x;
+    const int b_k = t.kind == 0 ? p.v0 + k : k;
+    for (int i = 0; i < half; i += 64) tma_load_2d_pair(at + kGemmTileBytes + i / 64 * kHeadBlock, b, bar, t.col0 + rank * half + i, b_k);
+  }
+  __device__ __forceinline__ uint32_t idesc(const HeadItem& t) const {
+    return umma_idesc_f16(std::is_same<T, __half>::value ? UMMA_F16 : UMMA_BF16, 256, p.bn, t.kind, 1);
+  }
+  __device__ __forceinline__ uint64_t a_desc(const HeadItem& t, uint32_t at) const { return umma_smem_desc_sw128(at, 1024, t.kind == 0 ? 16 : kHeadBlock); }
+  __device__ __forceinline__ uint64_t b_desc(const HeadItem&, uint32_t at) const { return umma_smem_desc_sw128(at, 1024, kHeadBlock); }
+  __device__ __forceinline__ int a_step(const HeadItem& t) const { return t.kind == 0 ? 2 : 128; }
+  __device__ __forceinline__ int b_step(const HeadItem&) const { return 128; }
+
+  struct Epilogue {
+    const HeadSumsJob& job;
+    const uint32_t stage;
+    uint8_t* const stage_ptr;
+    const int row_in, part, lane;
+    int buf;
+    const float scale;
+
+    __device__ __forceinline__ Epilogue(const HeadSumsJob& j, uint32_t s, uint8_t* sp, int r, int pt)
+        : job(j), stage(s), stage_ptr(sp), row_in(r), part(pt), lane(threadIdx.x & 31), buf(0), scale(head_scale(j.p.scale)) {}
+    __device__ __forceinline__ void ask(const HeadItem&) {}
+
+    template <typename HandBack>
+    __device__ __forceinline__ void take(const HeadItem& t, uint32_t acc, HandBack&& hand_back) {
+      const HeadSumsParams& p = job.p;
+      const int width = t.kind == 0 ? 32 : 64, pieces = p.bn / width;  // 128 bytes of a row: fp32 sums of dx, 16 bits of dw
+#pragma unroll 1
+      for (int c = part; c < pieces; c += 2) {
+        const int col = t.col0 + c * width;
+        const bool here = col < p.dim;
+        if (lane == 0) tma_store_wait_read<1>();
+        __syncwarp();
+        if (here) {
+          const uint32_t at_row = stage + buf * kHeadChunkBytes + lane * 128;
+          if (t.kind == 0) {
+            uint32_t v[32];
+            tmem_ld_x32(acc + c * 32, v);
+#pragma unroll
+            for (int q = 0; q < 8; ++q) st_shared_v4(at_row + ((q ^ (lane & 7)) << 4), make_uint4(v[4 * q], v[4 * q + 1], v[4 * q + 2], v[4 * q + 3]));
+          } else {
+            const float2 scale2 = make_float2(scale, scale);
+#pragma unroll
+            for (int half = 0; half < 2; ++half) {
+              float v[32];
+              tmem_ld_x32(acc + c * 64 + half * 32, reinterpret_cast<uint32_t*>(v));
+              uint32_t out[16];
+#pragma unroll
+              for (int i = 0; i < 16; ++i) {
+                const float2 y = fmul2(make_float2(v[2 * i], v[2 * i + 1]), scale2);
+                out[i] = gemm_pack2<T>(y.x, y.y);
+              }
+              if (job.rows == 0) {
+#pragma unroll
+                for (int i = 0; i < 16; ++i) out[i] = 0;
+              }
+#pragma unroll
+              for (int q = 0; q < 4; ++q)
+                st_shared_v4(at_row + (((4 * half + q) ^ (lane & 7)) << 4), make_uint4(out[4 * q], out[4 * q + 1], out[4 * q + 2], out[4 * q + 3]));
+            }
+          }
+          fence_proxy_async_smem();
+        }
+        if (c + 2 >= pieces) hand_back();
+        else __syncwarp();
+        if (lane == 0) {
+          if (here) {
+            uint8_t* const from = stage_ptr + buf * kHeadChunkBytes;
+            const int row = t.row0 + row_in;
+            if (t.kind == 1) tma_store_2d(job.dw, from, col, p.v0 + row);
+            else if (p.first) tma_store_2d(job.dx, from, col, static_cast<int>(t.slot * p.slot_rows) + row);
+            else head_tma_add_2d(job.dx, from, col, static_cast<int>(t.slot * p.slot_rows) + row);
+          }
+          tma_store_commit();
+        }
+        buf ^= 1;
+      }
+    }
+  };
+};
+
+// ---- kernels -----------------------------------------------------------------------------------------------------------------------
+template <typename T>
+__global__ void __launch_bounds__(kHeadThreads, 1)
+head_stats_kernel(const __grid_constant__ CUtensorMap x, const __grid_constant__ CUtensorMap x_copy, const __grid_constant__ CUtensorMap w,
+                  const __grid_constant__ HeadLogitsParams p) {
+  extern __shared__ uint8_t smem_raw[];
+  HeadLogitsJob<T, false> job(p, &x, &x_copy, &w, nullptr);
+  head_products(job, *reinterpret_cast<HeadSmem*>(smem_align_1024(smem_raw)), p.status);
+}
+
+template <typename T>
+__global__ void __launch_bounds__(kHeadThreads, 1)
+head_grads_kernel(const __grid_constant__ CUtensorMap x, const __grid_constant__ CUtensorMap x_copy, const __grid_constant__ CUtensorMap w,
+                  const __grid_constant__ CUtensorMap g, const __grid_constant__ HeadLogitsParams p) {
+  extern __shared__ uint8_t smem_raw[];
+  HeadLogitsJob<T, true> job(p, &x, &x_copy, &w, &g);
+  head_products(job, *reinterpret_cast<HeadSmem*>(smem_align_1024(smem_raw)), p.status);
+}
+
+template <typename T>
+__global__ void __launch_bounds__(kHeadThreads, 1)
+head_sums_kernel(const __grid_constant__ CUtensorMap g_k, const __grid_constant__ CUtensorMap g_mn, const __grid_constant__ CUtensorMap w,
+                 const __grid_constant__ CUtensorMap x, const __grid_constant__ CUtensorMap x_copy, const __grid_constant__ CUtensorMap dx,
+                 const __grid_constant__ CUtensorMap dw, const __grid_constant__ HeadSumsParams p) {
+  extern __shared__ uint8_t smem_raw[];
+  HeadSumsJob<T> job(p, &g_k, &g_mn, &w, &x, &x_copy, &dx, &dw);
+  head_products(job, *reinterpret_cast<HeadSmem*>(smem_align_1024(smem_raw)), p.status);
+}
+
+// Distillation: the entries of a row, a warp each. Entries whose token is negative do not count; one whose token is past the vocabulary makes NaN
+// of its row. p = softmax(teacher / tau) over the others; entropy = sum p log p (0 where p is 0).
+struct HeadEntriesParams {
+  const void* ids;       // [rows, top] of id_bytes each, rows ids_stride apart
+  const void* teacher;   // [rows, top], rows teacher_stride apart
+  int64_t ids_stride, teacher_stride;
+  int id_bytes, teacher_type;  // B200_ATTN_F16, _BF16 or _F32
+  int rows, top, vocab;
+  float inverse_tau;
+  int* sorted;       // [rows, top]
+  float* p;          // [rows, top]
+  float* entropy;    // [rows]
+  int8_t* counts;    // [rows]: whether any entry counts
+  uint32_t* status;
+};
+constexpr int kEntriesWarps = 8, kEntriesMost = 256;
+
+__device__ __forceinline__ float head_warp_sum(float v) {
+#pragma unroll
+  for (int d = 16; d > 0; d >>= 1) v += __shfl_xor_sync(0xffffffffu, v, d);
+  return v;
+}
+
+__global__ void __launch_bounds__(kEntriesWarps * 32) head_entries_kernel(const HeadEntriesParams p) {
+  __shared__ int tokens[kEntriesWarps][kEntriesMost];
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  grid_dependency_wait();
+  grid_launch_dependents();
+  const int row = blockIdx.x * kEntriesWarps + warp;
+  if (row >= p.rows) return;
+  constexpr int kEach = kEntriesMost / 32;
+  int id[kEach];
+  float z[kEach];
+  float most = -INFINITY;
+  bool any = false, bad = false;
+#pragma unroll
+  for (int i = 0; i < kEach; ++i) {
+    const int k = lane + 32 * i;
+    id[i] = kNoEntry;
+    z[i] = -INFINITY;
+    if (k < p.top) {
+      const int64_t at = row * p.ids_stride + k;
+      const int64_t token = p.id_bytes == 8 ? static_cast<const int64_t*>(p.ids)[at] : static_cast<const int32_t*>(p.ids)[at];
+      if (token >= 0) {
+        any = true;
+        const int64_t from = row * p.teacher_stride + k;
+        z[i] = p.teacher_type == 0   ? __half2float(static_cast<const __half*>(p.teacher)[from])
+               : p.teacher_type == 1 ? __bfloat162float(static_cast<const __nv_bfloat16*>(p.teacher)[from])
+                                     : static_cast<const float*>(p.teacher)[from];
+        z[i] *= p.inverse_tau;
+        if (token >= p.vocab) bad = true;
+        else id[i] = static_cast<int>(token);
+      }
+      tokens[warp][k] = id[i];
+      most = fmaxf(most, z[i]);
+    }
+  }
+#pragma unroll
+  for (int d = 16; d > 0; d >>= 1) most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, d));
+  any = __any_sync(0xffffffffu, any);
+  bad = __any_sync(0xffffffffu, bad);
+  __syncwarp();
+  float sum = 0.f;
+#pragma unroll
+  for (int i = 0; i < kEach; ++i) sum += z[i] == -INFINITY ? 0.f : expf(z[i] - most);  // a logit of -inf weighs nothing; NaN and +inf give NaN
+  sum = head_warp_sum(sum);
+  const float log_sum = logf(sum);
+  float entropy = 0.f;
+#pragma unroll
+  for (int i = 0; i < kEach; ++i) {
+    const int k = lane + 32 * i;
+    if (k >= p.top) continue;
+    int rank = 0;  // entries in front of this one: of lower tokens, and of the same token further left
+    for (int j = 0; j < p.top; ++j) {
+      const int other = tokens[warp][j];
+      rank += other < id[i] || (other == id[i] && j < k) ? 1 : 0;
+    }
+    const float log_p = z[i] - most - log_sum;
+    float weight = z[i] == -INFINITY ? 0.f : expf(log_p);
+    if (any && most == -INFINITY) weight = NAN;  // entries count, but all at -inf: no distribution
+    if (weight > 0.f) entropy += weight * log_p;
+    if (isnan(weight) || bad) entropy = NAN;
+    p.sorted[static_cast<int64_t>(row) * p.top + rank] = id[i];
+    p.p[static_cast<int64_t>(row) * p.top + rank] = weight;
+  }
+  entropy = head_warp_sum(entropy);
+  if (lane == 0) {
+    p.entropy[row] = entropy;
+    p.counts[row] = any ? 1 : 0;
+    if (bad) atomicOr(p.status, kStatusTarget);
+  }
+}
+
+// Which rows count, in the caller's order, and, where not all do, those rows of x together, with zeros behind the last up to the next
+// multiple of 64 (k of the products over rows). Every CTA counts the rows in front of its own: a few kilobytes out of L2.
+struct HeadRowsParams {
+  const void* targets;   // [rows] of target_bytes each, or null: `counts`
+  const int8_t* counts;  // distillation: whether a row has an entry
+  int target_bytes;
+  int64_t ignore;
+  int rows, per_cta, vocab, dim;
+  int top;
+  const void* x;         // [rows, dim], rows ldx apart
+  int64_t ldx;
+  uint4* x_copy;         // [rows up to a multiple of 64, dim]
+  int* count;
+  unsigned* finished;    // zeroed: head_loss_kernel's CTAs count on it
+  int* idx;              // [rows]
+  int* place;            // [rows]: where a row went, -1: it does not count
+  int* ids;              // [rows] targets as 32-bit entries (not for distillation)
+  float* picks;          // [rows, top]: NaN for a target outside the vocabulary, which no tile writes
+  float* loss;           // [rows] or null: 0 for rows that do not count
+  uint32_t* status;
+};
+constexpr int kRowsThreads = 256, kRowsMost = 1024;
+
+__global__ void __launch_bounds__(kRowsThreads) head_rows_kernel(const HeadRowsParams p) {
+  __shared__ int from[kRowsMost], before_all, count_all, warp_sums[kRowsThreads / 32];
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  if (tid == 0) before_all = count_all = 0;
+  grid_dependency_wait();
+  grid_launch_dependents();
+  __syncthreads();
+  const auto target = [&](int r) { return p.target_bytes == 8 ? static_cast<const int64_t*>(p.targets)[r] : static_cast<int64_t>(static_cast<const int32_t*>(p.targets)[r]); };
+  const auto counted = [&](int r) { return p.targets == nullptr ? p.counts[r] != 0 : target(r) != p.ignore; };
+  const int r0 = blockIdx.x * p.per_cta, r1 = min(p.rows, r0 + p.per_cta);
+  int before = 0, all = 0;
+  for (int r = tid; r < p.rows; r += kRowsThreads) {
+    const int c = counted(r) ? 1 : 0;
+    all += c;
+    before += r < r0 ? c : 0;
+  }
+#pragma unroll
+  for (int d = 16; d > 0; d >>= 1) {
+    all += __shfl_xor_sync(0xffffffffu, all, d);
+    before += __shfl_xor_sync(0xffffffffu, before, d);
+  }
+  if (lane == 0) {
+    atomicAdd(&before_all, before);
+    atomicAdd(&count_all, all);
+  }
+  __syncthreads();
+  int at = before_all;
+  const int count = count_all;
+  for (int base = r0; base < r1; base += kRowsThreads) {
+    const int r = base + tid;
+    const bool c = r < r1 && counted(r);
+    const unsigned mask = __ballot_sync(0xffffffffu, c);
+    if (lane == 0) warp_sums[warp] = __popc(mask);
+    __syncthreads();
+    int off = at;
+    for (int i = 0; i < kRowsThreads / 32; ++i) {
+      if (i < warp) off += warp_sums[i];
+      at += warp_sums[i];
+    }
+    const int to = off + __popc(mask & ((1u << lane) - 1));
+    if (r < r1) {
+      from[r - r0] = c ? to : -1;
+      p.place[r] = c ? to : -1;
+      if (c) p.idx[to] = r;
+      if (!c && p.loss != nullptr) p.loss[r] = 0.f;
+      if (p.targets != nullptr) {
+        const int64_t y = target(r);
+        const bool inside = y >= 0 && y < p.vocab;
+        p.ids[r] = c && inside ? static_cast<int>(y) : kNoEntry;
+        if (c && !inside) {
+          p.picks[r] = NAN;
+          atomicOr(p.status, kStatusTarget);
+        }
+      }
+    }
+    __syncthreads();
+  }
+  if (blockIdx.x == 0 && tid == 0) {
+    *p.count = count;
+    *p.finished = 0;
+  }
+  if (count == p.rows) return;
+  const int words = p.dim >> 3;
+  for (int r = r0 + warp; r < r1; r += kRowsThreads / 32) {
+    const int to = from[r - r0];
+    if (to < 0) continue;
+    const uint4* const in = reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(p.x) + r * p.ldx);
+    for (int i = lane; i < words; i += 32) p.x_copy[static_cast<int64_t>(to) * words + i] = in[i];
+  }
+  if (blockIdx.x == gridDim.x - 1)
+    for (int64_t i = static_cast<int64_t>(count) * words + tid; i < static_cast<int64_t>((count + 63) & ~63) * words; i += kRowsThreads) p.x_copy[i] = make_uint4(0, 0, 0, 0);
+}
+
+// lse and loss of 32 rows a CTA: a lane has a row and a warp every 32nd part; then a warp has a row and a lane every 32nd entry. The
+// last CTA adds up the CTAs' sums in their order.
+struct HeadLossParams {
+  const int* count;
+  const int* idx;
+  const float2* parts;
+  int64_t parts_stride;
+  int n_parts, top;
+  const float* picks;
+  const float* p;        // [rows, top] or null: 1
+  const float* entropy;  // [rows] or null: 0
+  float log2_scale, tau;
+  float* lse2;           // [rows]
+  float* loss;           // [rows] or null
+  float* total;          // the sum or the mean, or null
+  int mean;
+  float* sums;           // [CTAs]
+  unsigned* finished;
+};
+constexpr int kLossThreads = 1024;
+
+__global__ void __launch_bounds__(kLossThreads) head_loss_kernel(const HeadLossParams p) {
+  __shared__ float2 part[32][33];
+  __shared__ float row_loss[32];
+  __shared__ double cta_sums[32];
+  __shared__ bool last;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  grid_dependency_wait();
+  grid_launch_dependents();
+  const int count = *p.count, row0 = blockIdx.x * 32;
+  float m = -INFINITY, s = 0.f;
+  if (row0 + lane < count) {
+#pragma unroll 4
+    for (int i = warp; i < p.n_parts; i += 32) {
+      const float2 v = __ldg(p.parts + i * p.parts_stride + row0 + lane);
+      const float m_new = fmaxf(m, v.x), from = m_new == -INFINITY ? 0.f : m_new;
+      s = s * head_ex2(m - from) + v.y * head_ex2(v.x - from);
+      m = m_new;
+    }
+  }
+  part[warp][lane] = make_float2(m, s);
+  __syncthreads();
+  const int row = row0 + warp;
+  float loss = 0.f;
+  if (row < count) {
+    const float2 v = part[lane][warp];
+    m = v.x;
+#pragma unroll
+    for (int d = 16; d > 0; d >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, d));
+    s = head_warp_sum(v.y * head_ex2(v.x - (m == -INFINITY ? 0.f : m)));
+    const float log2_s = log2f(s), lse2 = m + log2_s;
+    const int src = __ldg(p.idx + row);
+    for (int k = lane; k < p.top; k += 32) {
+      const int64_t at = static_cast<int64_t>(src) * p.top + k;
+      const float weight = p.p != nullptr ? __ldg(p.p + at) : 1.f;
+      // An entry that does not count has no weight, and its logit was never written. The maximum first: nothing is left of it where the entry is
+      // the maximum, and a small loss keeps its digits.
+      if (weight != 0.f) loss += weight * (((m - __ldg(p.picks + at) * p.log2_scale) + log2_s) * 0.693147180559945f);
+    }
+    loss = head_warp_sum(loss);
+    if (p.entropy != nullptr) loss += __ldg(p.entropy + src);
+    loss *= p.tau * p.tau;
+    if (lane == 0) {
+      p.lse2[src] = isnan(loss) ? NAN : lse2;  // a row without a loss has no gradient either
+      if (p.loss != nullptr) p.loss[src] = loss;
+    }
+  }
+  if (p.total == nullptr) return;
+  if (lane == 0) row_loss[warp] = loss;
+  __syncthreads();
+  if (warp == 0) {
+    const float sum = head_warp_sum(row_loss[lane]);
+    if (lane == 0) {
+      p.sums[blockIdx.x] = sum;
+      __threadfence();
+      last = atomicAdd(p.finished, 1u) == gridDim.x - 1;
+    }
+  }
+  __syncthreads();
+  if (!last) return;
+  __threadfence();
+  double all = 0.;
+  for (unsigned i = threadIdx.x; i < gridDim.x; i += kLossThreads) all += static_cast<double>(__ldcg(p.sums + i));
+#pragma unroll
+  for (int d = 16; d > 0; d >>= 1) all += __shfl_xor_sync(0xffffffffu, all, d);
+  if (lane == 0) cta_sums[warp] = all;
+  __syncthreads();
+  if (warp == 0) {
+    all = cta_sums[lane];
+#pragma unroll
+    for (int d = 16; d > 0; d >>= 1) all += __shfl_xor_sync(0xffffffffu, all, d);
+    if (lane == 0) *p.total = static_cast<float>(p.mean ? all / max(count, 1) : all);
+  }
+}
+
+// Gradients that differ from row to row, divided by the power of two above the largest: what goes into 16 bits is then at most 1.
+struct HeadCoefParams {
+  const int* count;
+  const int* idx;
+  const float* g;
+  int64_t stride;
+  float* coef;  // [rows], by the caller's rows
+  float* norm;
+};
+constexpr int kCoefThreads = 1024;
+
+__global__ void __launch_bounds__(kCoefThreads) head_coef_kernel(const HeadCoefParams p) {
+  __shared__ float warp_most[32];
+  __shared__ float norm_all;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  grid_dependency_wait();
+  grid_launch_dependents();
+  const int count = *p.count;
+  float most = 0.f;
+  for (int i = threadIdx.x; i < count; i += kCoefThreads) {
+    const float g = fabsf(__ldg(p.g + __ldg(p.idx + i) * p.stride));
+    if (g < INFINITY) most = fmaxf(most, g);
+  }
+#pragma unroll
+  for (int d = 16; d > 0; d >>= 1) most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, d));
+  if (lane == 0) warp_most[warp] = most;
+  __syncthreads();
+  if (threadIdx.x == 0) {
+    for (int i = 0; i < 32; ++i) most = fmaxf(most, warp_most[i]);
+    // 2^-126 .. 2^126: both it and its inverse are normal numbers
+    norm_all = most > 0.f ? exp2f(fminf(fmaxf(static_cast<float>(ilogbf(most)) + 1.f, -126.f), 126.f)) : 1.f;
+    *p.norm = norm_all;
+  }
+  __syncthreads();
+  const float inverse = 1.f / norm_all;
+  for (int i = threadIdx.x; i < count; i += kCoefThreads) {
+    const int src = __ldg(p.idx + i);
+    p.coef[src] = __ldg(p.g + src * p.stride) * inverse;
+  }
+}
+
+// dx: the parts' sums added in their order, scaled, rounded; zeros for rows that do not count. Eight values a thread.
+struct HeadDxParams {
+  const float* sums;  // [splits][slot_rows, dim]
+  int splits;
+  int64_t slot_rows;
+  int rows, dim;
+  const int* place;
+  void* dx;           // [rows, dim]
+  HeadScale scale;
+};
+constexpr int kDxThreads = 256;
+
+template <typename T>
+__global__ void __launch_bounds__(kDxThreads) head_dx_kernel(const HeadDxParams p) {
+  grid_dependency_wait();
+  grid_launch_dependents();
+  const int words = p.dim >> 3;
+  const int64_t all = static_cast<int64_t>(p.rows) * words;
+  const float scale = head_scale(p.scale);
+  for (int64_t i = static_cast<int64_t>(blockIdx.x) * kDxThreads + threadIdx.x; i < all; i += static_cast<int64_t>(gridDim.x) * kDxThreads) {
+    const int row = static_cast<int>(i / words), word = static_cast<int>(i - static_cast<int64_t>(row) * words);
+    const int at = __ldg(p.place + row);
+    float4 a = make_float4(0.f, 0.f, 0.f, 0.f), b = a;
+    if (at >= 0) {
+      for (int s = 0; s < p.splits; ++s) {
+        const float4* const from = reinterpret_cast<const float4*>(p.sums + (s * p.slot_rows + at) * p.dim) + 2 * word;
+        const float4 u = __ldg(from), v = __ldg(from + 1);
+        a.x += u.x; a.y += u.y; a.z += u.z; a.w += u.w;
+        b.x += v.x; b.y += v.y; b.z += v.z; b.w += v.w;
+      }
+    }
+    uint4 out = make_uint4(0, 0, 0, 0);
+    if (at >= 0)
+      out = make_uint4(gemm_pack2<T>(a.x * scale, a.y * scale), gemm_pack2<T>(a.z * scale, a.w * scale), gemm_pack2<T>(b.x * scale, b.y * scale),
+                       gemm_pack2<T>(b.z * scale, b.w * scale));
+    static_cast<uint4*>(p.dx)[i] = out;
+  }
+}
+
+}  // namespace b200
