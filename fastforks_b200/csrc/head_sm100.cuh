@@ -64,6 +64,12 @@ struct HeadItem {
   int kb0, kb1;
 };
 
+// k-blocks of an accumulator of logits. The tensor cores cut off what of a product lies below the last place of the running sum: over 4096
+// products the loss of 64 rows came out 2.1e-6 off (products and sums in fp32 arithmetic: 3.7e-7). Longer sums are taken 1024 products at a
+// time and added in fp32, which rounds: 4.7e-7. The accumulators alternate as they do between tiles, so the epilogue's additions run under
+// the next products (4096 x 128000 x 4096: 2570 us; one accumulator, as in head_grads_kernel, 2546).
+constexpr int kHeadSumBlocks = 16;
+
 // The pipeline of gemm_pair_kernel with the operands' layouts, the list of tiles and the epilogue left to `job`:
 //   begin()                      reads what only the kernels in front know (after the wait for them)
 //   items(pair), item(pair, i)   this pair's tiles, the same for both CTAs and all warps
@@ -273,10 +279,10 @@ template <typename T, bool GRADS>
 struct HeadLogitsJob {
   const HeadLogitsParams& p;
   const CUtensorMap *x, *x_copy, *w, *g;
-  int rows, tiles_m;
+  int rows, tiles_m, k_blocks, sums;  // sums: accumulators of a tile, one after the other
 
   __device__ __forceinline__ HeadLogitsJob(const HeadLogitsParams& p_, const CUtensorMap* x_, const CUtensorMap* xc, const CUtensorMap* w_, const CUtensorMap* g_)
-      : p(p_), x(x_), x_copy(xc), w(w_), g(g_), rows(0), tiles_m(0) {}
+      : p(p_), x(x_), x_copy(xc), w(w_), g(g_), rows(0), tiles_m(0), k_blocks((p_.dim + kGemmBK - 1) / kGemmBK), sums(GRADS ? 1 : (k_blocks + kHeadSumBlocks - 1) / kHeadSumBlocks) {}
   __device__ __forceinline__ void begin() {
     rows = __ldg(p.count);
     tiles_m = (rows + 255) >> 8;
@@ -284,12 +290,16 @@ struct HeadLogitsJob {
   }
   __device__ __forceinline__ int items(int pair) const {
     const int tiles = tiles_m * p.tiles_n, pairs = gridDim.x >> 1;
-    return tiles > pair ? (tiles - pair + pairs - 1) / pairs : 0;
+    return tiles > pair ? (tiles - pair + pairs - 1) / pairs * sums : 0;
   }
   __device__ __forceinline__ HeadItem item(int pair, int i) const {
-    int tm, tn;
+    int tm, tn, part = 0;
+    if (!GRADS && sums > 1) {
+      part = i % sums;
+      i /= sums;
+    }
     head_raster(pair + i * (gridDim.x >> 1), tiles_m, p.tiles_n, min(p.group, tiles_m), &tm, &tn);
-    return {0, tn, tm * 256, p.v0 + tn * p.bn, 0, (p.dim + kGemmBK - 1) / kGemmBK};
+    return {0, tn, tm * 256, p.v0 + tn * p.bn, k_blocks * part / sums, k_blocks * (part + 1) / sums};
   }
   __device__ __forceinline__ int stages() const { return p.stages; }
   __device__ __forceinline__ uint32_t stage_bytes() const { return kGemmTileBytes + static_cast<uint32_t>(p.bn) * kGemmBK; }
@@ -316,6 +326,7 @@ struct HeadLogitsJob {
     int next, pos;    // the row's first entry that has not been passed: its token, its place
     float lse2, coef;
     int buf;
+    float sum[GRADS ? 1 : 64];  // the accumulators of a tile so far, where there are several: of the first 64 columns; the others' are staged
 
     __device__ __forceinline__ Epilogue(const HeadLogitsJob& j, uint32_t s, uint8_t* sp, int r, int pt)
         : job(j), stage(s), stage_ptr(sp), row_in(r), part(pt), lane(threadIdx.x & 31), row(0), src(-1), next(kNoEntry), pos(0), lse2(0.f), coef(0.f), buf(0) {}
@@ -324,6 +335,7 @@ struct HeadLogitsJob {
 
     __device__ __forceinline__ void ask(const HeadItem& t) {
       const HeadLogitsParams& p = job.p;
+      if (t.kb1 < job.k_blocks) return;  // the last accumulator of a tile is asked for
       row = t.row0 + row_in + lane;
       src = row < job.rows ? __ldg(p.idx + row) : -1;
       next = kNoEntry;
@@ -345,6 +357,19 @@ struct HeadLogitsJob {
       }
     }
 
+    // This thread's sums of 32 columns in the warp's staging area: sixteen bytes of every lane side by side, 512 to the next sixteen.
+    __device__ __forceinline__ uint32_t staged(int which) const { return stage + which * kHeadChunkBytes + lane * 16; }
+    __device__ __forceinline__ void add_staged(float (&v)[32], int which) const {
+#pragma unroll
+      for (int q = 0; q < 8; ++q) {
+        const uint4 had = ld_shared_v4(staged(which) + q * 512);
+        v[4 * q] += __uint_as_float(had.x);
+        v[4 * q + 1] += __uint_as_float(had.y);
+        v[4 * q + 2] += __uint_as_float(had.z);
+        v[4 * q + 3] += __uint_as_float(had.w);
+      }
+    }
+
     // f(j, entry) for the row's entries among the 32 columns from `base` on. Entries of the other warp's columns are passed over.
     template <typename F>
     __device__ __forceinline__ void for_entries(int base, F&& f) {
@@ -361,6 +386,28 @@ struct HeadLogitsJob {
       const HeadLogitsParams& p = job.p;
       const int pieces = p.bn >> 6;
       if constexpr (!GRADS) {
+        if (t.kb1 < job.k_blocks) {
+#pragma unroll 1
+          for (int c = part; c < pieces; c += 2) {
+#pragma unroll
+            for (int half = 0; half < 2; ++half) {
+              float v[32];
+              tmem_ld_x32(acc + c * 64 + half * 32, reinterpret_cast<uint32_t*>(v));
+              if (c == part) {
+#pragma unroll
+                for (int j = 0; j < 32; ++j) sum[half * 32 + j] = t.kb0 == 0 ? v[j] : sum[half * 32 + j] + v[j];
+              } else {
+                if (t.kb0 > 0) add_staged(v, half);
+                const uint32_t at = staged(half);
+#pragma unroll
+                for (int q = 0; q < 8; ++q)
+                  st_shared_v4(at + q * 512, make_uint4(__float_as_uint(v[4 * q]), __float_as_uint(v[4 * q + 1]), __float_as_uint(v[4 * q + 2]), __float_as_uint(v[4 * q + 3])));
+              }
+            }
+          }
+          hand_back();
+          return;
+        }
         float m = -INFINITY, s = 0.f;
 #pragma unroll 1
         for (int c = part; c < pieces; c += 2) {
@@ -370,6 +417,14 @@ struct HeadLogitsJob {
             if (base >= p.vocab) continue;
             float v[32];
             tmem_ld_x32(acc + c * 64 + half * 32, reinterpret_cast<uint32_t*>(v));
+            if (t.kb0 > 0) {
+              if (c == part) {
+#pragma unroll
+                for (int j = 0; j < 32; ++j) v[j] += sum[half * 32 + j];
+              } else {
+                add_staged(v, half);
+              }
+            }
             for_entries(base, [&](int j, int64_t at) {
               float got = 0.f;
 #pragma unroll

@@ -22,6 +22,7 @@
 
 #include "../../include/b200_attn.h"
 #include "../../include/b200_decoder.h"
+#include "../../include/b200_training.h"
 
 namespace {
 
@@ -564,6 +565,228 @@ PyObject* py_qk_norm_rotary(PyObject*, PyObject* const* args, Py_ssize_t n) {
   return Py_BuildValue("(NN)", THPVariable_Wrap(y[0]), THPVariable_Wrap(y[1]));
 }
 
+// ---- layer norm, and the losses of an output layer ---------------------------------------------------------------------------------
+int64_t rows_of(const at::Tensor& x) { return x.numel() / x.size(-1); }
+
+void set_norm(B200LayerNormArgs* a, const at::Tensor& x, const at::Tensor& w, const at::Tensor& b, double eps) {
+  std::memset(a, 0, sizeof(*a));
+  a->struct_size = sizeof(*a);
+  a->dtype = a->weight_dtype = any_dtype_code(x);
+  a->dim = static_cast<int32_t>(x.size(-1));
+  a->rows = rows_of(x);
+  a->eps = static_cast<float>(eps);
+  a->x = x.data_ptr();
+  a->x_stride = a->y_stride = a->dy_stride = a->dx_stride = a->dim;
+  for (const at::Tensor* t : {&w, &b})
+    if (t->defined()) a->weight_dtype = any_dtype_code(*t);
+  a->weight = w.defined() ? w.data_ptr() : nullptr;
+  a->bias = b.defined() ? b.data_ptr() : nullptr;
+}
+
+// `stats`: gets what the gradients need, where they are wanted.
+at::Tensor layer_normed(const at::Tensor& x, const at::Tensor& w, const at::Tensor& b, double eps, at::Tensor* stats) {
+  at::Tensor y = empty_like_type(x.sizes(), x);
+  B200LayerNormArgs a;
+  set_norm(&a, x, w, b, eps);
+  a.y = y.data_ptr();
+  if (stats != nullptr) {
+    *stats = at::detail::empty_cuda({a.rows, 2}, at::kFloat, x.device(), std::nullopt);
+    a.stats = static_cast<float*>(stats->data_ptr());
+  }
+  TORCH_CHECK(b200_layer_norm(&a, c10::cuda::getCurrentCUDAStream(x.device().index()).stream()) == B200_ATTN_OK, "layer_norm: ", b200_attn_last_error());
+  return y;
+}
+
+struct LayerNormFunction : torch::autograd::Function<LayerNormFunction> {
+  // `has`: which of weight (1) and bias (2) there are; x stands in for the others, as apply() takes no undefined tensor.
+  static at::Tensor forward(AutogradContext* ctx, const at::Tensor& x, const at::Tensor& weight, const at::Tensor& bias, int64_t has, double eps) {
+    const at::Tensor w = has & 1 ? weight : at::Tensor(), b = has & 2 ? bias : at::Tensor();
+    at::Tensor stats;
+    at::Tensor y = layer_normed(x, w, b, eps, &stats);
+    ctx->save_for_backward({x, w, b, stats});
+    ctx->saved_data["eps"] = eps;
+    return y;
+  }
+  static variable_list backward(AutogradContext* ctx, const variable_list& grads) {
+    const variable_list saved = ctx->get_saved_variables();
+    variable_list result(5);
+    {
+      const at::NoGradGuard guard;
+      const at::Tensor &x = saved[0], &w = saved[1], &b = saved[2];
+      const c10::cuda::CUDAGuard on(x.device());
+      const at::Tensor g = grads[0].defined() ? grads[0].contiguous() : at::zeros_like(x, at::MemoryFormat::Contiguous);
+      B200LayerNormArgs a;
+      set_norm(&a, x, w, b, ctx->saved_data["eps"].toDouble());
+      a.stats = static_cast<float*>(saved[3].data_ptr());
+      a.dy = g.data_ptr();
+      if (ctx->needs_input_grad(0)) {
+        result[0] = empty_like_type(x.sizes(), x);
+        a.dx = result[0].data_ptr();
+      }
+      if (w.defined() && ctx->needs_input_grad(1)) {
+        result[1] = empty_like_type(w.sizes(), w);
+        a.dweight = result[1].data_ptr();
+      }
+      if (b.defined() && ctx->needs_input_grad(2)) {
+        result[2] = empty_like_type(b.sizes(), b);
+        a.dbias = result[2].data_ptr();
+      }
+      at::Tensor scratch;
+      if (a.dweight != nullptr || a.dbias != nullptr) {
+        TORCH_CHECK(b200_layer_norm_workspace(&a, &a.workspace_bytes) == B200_ATTN_OK, "layer_norm workspace: ", b200_attn_last_error());
+        scratch = at::detail::empty_cuda({a.workspace_bytes}, at::kByte, x.device(), std::nullopt);
+        a.workspace = scratch.data_ptr();
+      }
+      TORCH_CHECK(b200_layer_norm_grad(&a, c10::cuda::getCurrentCUDAStream(x.device().index()).stream()) == B200_ATTN_OK, "layer_norm gradient: ", b200_attn_last_error());
+    }
+    return once(std::move(result));
+  }
+};
+
+// layer_norm(x, weight | None, bias | None, eps)
+PyObject* py_layer_norm(PyObject*, PyObject* const* args, Py_ssize_t n) {
+  if (n != 4) Py_RETURN_NONE;
+  const c10::DeviceIndex device = c10::cuda::current_device();
+  const at::Tensor* x = tensor_of(args[0]);
+  double eps = 0;
+  if (x == nullptr || !on_device(*x, device) || !heads_type(*x) || x->dim() < 1 || x->numel() == 0 || !x->is_contiguous() || x->size(-1) > 32768 || !number(args[3], &eps) || !(eps >= 0) || std::isinf(eps)) Py_RETURN_NONE;
+  if (rows_of(*x) > INT32_MAX) Py_RETURN_NONE;
+  at::Tensor affine[2];
+  bool grad = wants_grad(*x);
+  for (int k = 0; k < 2; ++k) {
+    if (args[1 + k] == Py_None) continue;
+    const at::Tensor* t = tensor_of(args[1 + k]);
+    if (t == nullptr || !on_device(*t, device) || t->dim() != 1 || t->size(0) != x->size(-1) || !t->is_contiguous()) Py_RETURN_NONE;
+    if (t->scalar_type() != x->scalar_type() && t->scalar_type() != at::kFloat) Py_RETURN_NONE;
+    if (k == 1 && affine[0].defined() && affine[0].scalar_type() != t->scalar_type()) Py_RETURN_NONE;
+    affine[k] = *t;
+    grad = grad || wants_grad(*t);
+  }
+  if (!grad) return THPVariable_Wrap(layer_normed(*x, affine[0], affine[1], eps, nullptr));
+  const int64_t has = (affine[0].defined() ? 1 : 0) | (affine[1].defined() ? 2 : 0);
+  return THPVariable_Wrap(LayerNormFunction::apply(*x, has & 1 ? affine[0] : *x, has & 2 ? affine[1] : *x, has, eps));
+}
+
+void set_head(B200HeadArgs* a, const at::Tensor& x, const at::Tensor& w, int64_t top, double tau, int64_t reduction) {
+  std::memset(a, 0, sizeof(*a));
+  a->struct_size = sizeof(*a);
+  a->dtype = dtype_code(x);
+  a->rows = static_cast<int32_t>(rows_of(x));
+  a->dim = static_cast<int32_t>(x.size(-1));
+  a->vocab = static_cast<int32_t>(w.size(0));
+  a->top = static_cast<int32_t>(top);
+  a->tau = static_cast<float>(tau);
+  a->reduction = static_cast<int32_t>(reduction);
+  a->x = x.data_ptr();
+  a->w = w.data_ptr();
+  a->ldx = a->ldw = a->dim;
+}
+
+at::Tensor bytes_for(int64_t n, const at::Tensor& like) { return at::detail::empty_cuda({n}, at::kByte, like.device(), std::nullopt); }
+
+// The loss, and in `state` what its gradients need. targets [rows] or [rows, top]; teacher undefined: cross entropy.
+at::Tensor head_loss(const at::Tensor& x, const at::Tensor& w, const at::Tensor& targets, const at::Tensor& teacher, int64_t ignore, double tau, int64_t reduction, at::Tensor* state) {
+  B200HeadArgs a;
+  const int64_t top = teacher.defined() ? targets.size(-1) : 0;
+  set_head(&a, x, w, top, tau, reduction);
+  a.targets = targets.data_ptr();
+  a.target_bytes = static_cast<int32_t>(targets.element_size());
+  a.targets_stride = a.teacher_stride = top;
+  a.ignore = ignore;
+  if (teacher.defined()) {
+    a.teacher = teacher.data_ptr();
+    a.teacher_dtype = any_dtype_code(teacher);
+  }
+  int64_t grad_bytes = 0;
+  TORCH_CHECK(b200_head_sizes(&a, &a.state_bytes, &a.workspace_bytes, &grad_bytes) == B200_ATTN_OK, b200_attn_last_error());
+  at::Tensor loss = at::detail::empty_cuda(reduction == 0 ? x.sizes().slice(0, x.dim() - 1) : at::IntArrayRef(), at::kFloat, x.device(), std::nullopt);
+  *state = bytes_for(a.state_bytes, x);
+  const at::Tensor scratch = bytes_for(a.workspace_bytes, x);
+  a.loss = static_cast<float*>(loss.data_ptr());
+  a.state = state->data_ptr();
+  a.workspace = scratch.data_ptr();
+  TORCH_CHECK(b200_head_loss(&a, c10::cuda::getCurrentCUDAStream(x.device().index()).stream()) == B200_ATTN_OK, b200_attn_last_error());
+  return loss;
+}
+
+struct HeadLossFunction : torch::autograd::Function<HeadLossFunction> {
+  static at::Tensor forward(AutogradContext* ctx, const at::Tensor& x, const at::Tensor& w, const at::Tensor& targets, const at::Tensor& logits, bool distill, int64_t ignore, double tau, int64_t reduction) {
+    const at::Tensor teacher = distill ? logits : at::Tensor();  // (`targets` stand in for no teacher)
+    at::Tensor state;
+    at::Tensor loss = head_loss(x, w, targets, teacher, ignore, tau, reduction, &state);
+    ctx->save_for_backward({x, w, state});
+    ctx->saved_data["top"] = teacher.defined() ? targets.size(-1) : int64_t(0);
+    ctx->saved_data["tau"] = tau;
+    ctx->saved_data["reduction"] = reduction;
+    return loss;
+  }
+  static variable_list backward(AutogradContext* ctx, const variable_list& grads) {
+    const variable_list saved = ctx->get_saved_variables();
+    variable_list result(8);
+    {
+      const at::NoGradGuard guard;
+      const at::Tensor &x = saved[0], &w = saved[1], &state = saved[2];
+      const c10::cuda::CUDAGuard on(x.device());
+      const int64_t reduction = ctx->saved_data["reduction"].toInt();
+      B200HeadArgs a;
+      set_head(&a, x, w, ctx->saved_data["top"].toInt(), ctx->saved_data["tau"].toDouble(), reduction);
+      at::Tensor g = grads[0];
+      if (!g.defined()) g = at::zeros({reduction == 0 ? a.rows : 1}, x.options().dtype(at::kFloat).requires_grad(false));
+      if (g.dim() > 1) g = g.reshape({-1});
+      a.grad = static_cast<const float*>(g.data_ptr());
+      a.grad_stride = g.dim() == 1 ? g.stride(0) : 0;
+      if (ctx->needs_input_grad(0)) {
+        result[0] = empty_like_type(x.sizes(), x);
+        a.dx = result[0].data_ptr();
+      }
+      if (ctx->needs_input_grad(1)) {
+        result[1] = empty_like_type(w.sizes(), w);
+        a.dw = result[1].data_ptr();
+      }
+      int64_t loss_bytes = 0;
+      TORCH_CHECK(b200_head_sizes(&a, &a.state_bytes, &loss_bytes, &a.workspace_bytes) == B200_ATTN_OK, "loss gradient: ", b200_attn_last_error());
+      const at::Tensor scratch = bytes_for(a.workspace_bytes, x);
+      a.state = state.data_ptr();
+      a.workspace = scratch.data_ptr();
+      TORCH_CHECK(b200_head_grad(&a, c10::cuda::getCurrentCUDAStream(x.device().index()).stream()) == B200_ATTN_OK, "loss gradient: ", b200_attn_last_error());
+    }
+    return once(std::move(result));
+  }
+};
+
+// A matrix (or rows of any shape) as the products take it without a copy.
+bool operand_of(const at::Tensor* t, c10::DeviceIndex device) {
+  return t != nullptr && on_device(*t, device) && half_type(*t) && t->dim() >= 1 && t->numel() > 0 && t->is_contiguous() && t->size(-1) % 8 == 0 && fits32(*t) && rows_of(*t) <= INT32_MAX &&
+         reinterpret_cast<uintptr_t>(t->data_ptr()) % 16 == 0;
+}
+
+// head_loss(x, weight, targets, teacher | None, ignore, tau, reduction: 0 none, 1 sum, 2 mean)
+PyObject* py_head_loss(PyObject*, PyObject* const* args, Py_ssize_t n) {
+  if (n != 7 || !PyLong_Check(args[4])) Py_RETURN_NONE;
+  const c10::DeviceIndex device = c10::cuda::current_device();
+  const at::Tensor *x = tensor_of(args[0]), *w = tensor_of(args[1]), *y = tensor_of(args[2]);
+  if (!operand_of(x, device) || !operand_of(w, device) || w->dim() != 2 || w->scalar_type() != x->scalar_type() || w->size(1) != x->size(-1)) Py_RETURN_NONE;
+  if (y == nullptr || !plain(*y, device) || !y->is_contiguous() || (y->scalar_type() != at::kLong && y->scalar_type() != at::kInt)) Py_RETURN_NONE;
+  int overflow = 0;
+  const int64_t ignore = PyLong_AsLongLongAndOverflow(args[4], &overflow);
+  double tau = 1;
+  int64_t reduction = 0;
+  if (overflow != 0 || !number(args[5], &tau) || !(tau > 0) || std::isinf(tau) || !integer(args[6], &reduction) || reduction < 0 || reduction > 2) Py_RETURN_NONE;
+  at::Tensor teacher;
+  const at::IntArrayRef rows = x->sizes().slice(0, x->dim() - 1);
+  if (args[3] == Py_None) {
+    if (y->sizes() != rows) Py_RETURN_NONE;
+  } else {
+    const at::Tensor* t = tensor_of(args[3]);
+    if (t == nullptr || !on_device(*t, device) || wants_grad(*t) || !heads_type(*t) || !t->is_contiguous() || t->sizes() != y->sizes()) Py_RETURN_NONE;
+    if (y->dim() != x->dim() || y->sizes().slice(0, y->dim() - 1) != rows || y->size(-1) < 1 || y->size(-1) > 256) Py_RETURN_NONE;
+    teacher = *t;
+  }
+  if (wants_grad(*x) || wants_grad(*w)) return THPVariable_Wrap(HeadLossFunction::apply(*x, *w, *y, teacher.defined() ? teacher : *y, teacher.defined(), ignore, tau, reduction));
+  at::Tensor state;
+  return THPVariable_Wrap(head_loss(*x, *w, *y, teacher, ignore, tau, reduction, &state));
+}
+
 // Cache, page table and lengths of a call on `batch` sequences.
 template <typename A>
 bool set_cache(A* a, PyObject* cache, PyObject* page_table, PyObject* lengths, int64_t batch, c10::DeviceIndex device) {
@@ -830,6 +1053,8 @@ PyMethodDef methods[] = {
     {"unchanged", fast<py_unchanged>(), METH_FASTCALL, nullptr},
     {"rotary", fast<py_rotary>(), METH_FASTCALL, nullptr},
     {"qk_norm_rotary", fast<py_qk_norm_rotary>(), METH_FASTCALL, nullptr},
+    {"layer_norm", fast<py_layer_norm>(), METH_FASTCALL, nullptr},
+    {"head_loss", fast<py_head_loss>(), METH_FASTCALL, nullptr},
     {"kv4_append_", fast<py_kv4_append>(), METH_FASTCALL, nullptr},
     {"kv4_read", fast<py_kv4_read>(), METH_FASTCALL, nullptr},
     {"kv4_attention", fast<py_kv4_attention>(), METH_FASTCALL, nullptr},

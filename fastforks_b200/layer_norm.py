@@ -51,6 +51,7 @@ def _forward(x: torch.Tensor, weight: torch.Tensor | None, bias: torch.Tensor | 
     with torch.cuda.device(x.device):
         code = _lib.library().b200_layer_norm(ctypes.byref(a), torch._C._cuda_getCurrentRawStream(x.device.index))  # noqa: SLF001
     _lib.raise_for_code(code, "layer_norm")
+    _lib.use_fast()
     return kept
 
 
@@ -117,6 +118,10 @@ def layer_norm(
         ValueError: Operands outside the contract (checked before the launch).
         KernelUnavailableError: The CUDA library is not built or does not load.
     """
+    if out is None and _lib.fast is not None:
+        done = _lib.fast.layer_norm(x, weight, bias, eps)
+        if done is not None:
+            return done
     what = "layer_norm"
     if x.dtype not in _DTYPES or not x.is_cuda or x.dim() < 1 or not 1 <= x.shape[-1] <= MAX_DIM:
         msg = f"{what}: x must be a float16 / bfloat16 / float32 CUDA tensor [..., 1 .. {MAX_DIM}], got {tuple(x.shape)} {x.dtype} on {x.device}"

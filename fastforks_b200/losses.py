@@ -80,6 +80,7 @@ def _loss(what: str, x: torch.Tensor, w: torch.Tensor, targets: torch.Tensor, te
         a.loss, a.state, a.state_bytes, a.workspace, a.workspace_bytes = loss.data_ptr(), state.data_ptr(), state_bytes, ws.data_ptr(), loss_bytes
         code = _lib.library().b200_head_loss(ctypes.byref(a), torch._C._cuda_getCurrentRawStream(x.device.index))  # noqa: SLF001
     _lib.raise_for_code(code, what)
+    _lib.use_fast()
     return loss, state
 
 
@@ -150,6 +151,10 @@ def linear_cross_entropy(  # noqa: PLR0913
         ValueError: Operands outside the contract (checked before the launch).
         KernelUnavailableError: The CUDA library is not built or does not load.
     """
+    if _lib.fast is not None:
+        done = _lib.fast.head_loss(x, weight, targets, None, ignore_index, 1.0, _REDUCTIONS.get(reduction))
+        if done is not None:
+            return done
     what = "linear_cross_entropy"
     _check(what, x, weight, reduction)
     if targets.dtype not in (torch.int64, torch.int32) or targets.shape != x.shape[:-1] or targets.device != x.device:
@@ -190,6 +195,10 @@ def linear_distillation(  # noqa: PLR0913
         ValueError: Operands outside the contract (checked before the launch).
         KernelUnavailableError: The CUDA library is not built or does not load.
     """
+    if _lib.fast is not None and teacher_logits is not None:
+        done = _lib.fast.head_loss(x, weight, teacher_ids, teacher_logits, 0, temperature, _REDUCTIONS.get(reduction))
+        if done is not None:
+            return done
     what = "linear_distillation"
     _check(what, x, weight, reduction)
     if teacher_ids.dtype not in (torch.int64, torch.int32) or teacher_ids.dim() != x.dim() or teacher_ids.shape[:-1] != x.shape[:-1] or not 1 <= teacher_ids.shape[-1] <= MAX_TOP or teacher_ids.device != x.device:
