@@ -35,17 +35,16 @@ const NormForm* forward_forms(bool wide_rows, int* count) {
   *count = wide_rows ? (sizeof(T) == 2 ? 11 : 12) : 8;
   return wide_rows ? vectors : values;
 }
-// Sixteen values a thread: their part of dw and db, two values of the row and two of the next one's are registers too.
+// The gradients of rows that do not go through shared memory: too wide for it, or not on 16 bytes.
 template <typename T, int VEC, int N, int THREADS>
 NormForm grad_form() { return {reinterpret_cast<const void*>(norm_rows_grad_kernel<T, VEC, N, THREADS>), THREADS, N, VEC}; }
 template <typename T>
 const NormForm* grad_forms(bool wide_rows, int* count) {
   constexpr int V = 16 / sizeof(T), M = 16 / V;
-  static const NormForm vectors[] = {grad_form<T, V, 1, 32>(), grad_form<T, V, M / 2 + (M == 4 ? 1 : 0), 32>(), grad_form<T, V, M, 32>(), grad_form<T, V, M, 64>(), grad_form<T, V, M, 128>(),
-                                     grad_form<T, V, M, 256>(), grad_form<T, V, M, 512>(), grad_form<T, V, M, 1024>(), grad_form<T, V, 2 * M, 1024>()};
+  static const NormForm vectors[] = {grad_form<T, V, M, 512>(), grad_form<T, V, M, 1024>(), grad_form<T, V, 2 * M, 1024>()};
   static const NormForm values[] = {grad_form<T, 1, 1, 32>(), grad_form<T, 1, 4, 32>(), grad_form<T, 1, 8, 32>(), grad_form<T, 1, 8, 128>(), grad_form<T, 1, 16, 128>(),
                                     grad_form<T, 1, 16, 256>(), grad_form<T, 1, 16, 512>(), grad_form<T, 1, 16, 1024>(), grad_form<T, 1, 32, 1024>()};
-  *count = 9;
+  *count = wide_rows ? 3 : 9;
   return wide_rows ? vectors : values;
 }
 NormForm norm_form(const B200LayerNormArgs& a, bool grad, bool wide_rows) {
@@ -59,7 +58,66 @@ NormForm norm_form(const B200LayerNormArgs& a, bool grad, bool wide_rows) {
   return f[i];
 }
 
+// Gradients of rows that go through shared memory: G warps a row, N vectors a thread, in order of what they hold.
+struct RingForm {
+  const void* kernel;
+  int warps, vectors;
+};
+template <typename T, int N, int G>
+RingForm ring_form() { return {reinterpret_cast<const void*>(norm_ring_grad_kernel<T, 16 / sizeof(T), N, G>), G, N}; }
+constexpr int kMostRingForms = 10;
+template <typename T>
+const RingForm* ring_forms(int* count) {
+  if constexpr (sizeof(T) == 2) {
+    static const RingForm forms[] = {ring_form<T, 1, 1>(), ring_form<T, 2, 1>(), ring_form<T, 2, 2>(), ring_form<T, 2, 4>(), ring_form<T, 2, 8>(), ring_form<T, 3, 8>(), ring_form<T, 4, 8>()};
+    *count = 7;
+    return forms;
+  } else {
+    static const RingForm forms[] = {ring_form<T, 1, 1>(), ring_form<T, 2, 1>(), ring_form<T, 3, 1>(), ring_form<T, 4, 1>(), ring_form<T, 3, 2>(), ring_form<T, 4, 2>(), ring_form<T, 3, 4>(), ring_form<T, 4, 4>(), ring_form<T, 3, 8>(), ring_form<T, 4, 8>()};
+    *count = 10;
+    return forms;
+  }
+}
+
+// The form of a call, or no kernel: rows that are no whole 16-byte words, or too wide.
+struct RingPlan {
+  RingForm form{nullptr, 0, 0};
+  int index = 0, slots = 0, ctas = 0, smem = 0;
+};
+RingPlan ring_plan(const B200LayerNormArgs& a, bool wide_rows, int sms) {
+  RingPlan r;
+  if (!wide_rows) return r;
+  int n = 0;
+  const RingForm* f = a.dtype == B200_ATTN_F16 ? ring_forms<__half>(&n) : a.dtype == B200_ATTN_BF16 ? ring_forms<__nv_bfloat16>(&n) : ring_forms<float>(&n);
+  const int values = a.dtype == B200_ATTN_F32 ? 4 : 8;  // of a vector
+  int i = 0;
+  while (i < n && f[i].warps * f[i].vectors * 32 * values < a.dim) ++i;
+  if (i == n) return r;
+  const int groups = kLnWarps / f[i].warps, slot = 2 * f[i].warps * f[i].vectors * 512;  // (a vector of 32 lanes: 512 bytes)
+  const int per_sm = ln_ring_ctas(f[i].vectors * values);
+  r.form = f[i];
+  r.index = (a.dtype == B200_ATTN_F16 ? 0 : a.dtype == B200_ATTN_BF16 ? 1 : 2) * kMostRingForms + i;
+  r.slots = std::min(kLnMostSlots, ln_ring_bytes(per_sm) / (groups * slot));
+  r.ctas = static_cast<int>(std::min<int64_t>((a.rows + groups - 1) / groups, static_cast<int64_t>(per_sm) * sms));
+  r.smem = r.slots * groups * slot;
+  return r;
+}
+
 size_t element(uint32_t dtype) { return dtype == B200_ATTN_F32 ? 4 : 2; }
+
+// Shared memory above 48 KB is allowed per kernel and device.
+constexpr int kHeadForms = 6, kOptIns = kHeadForms + 3 * kMostRingForms;
+int opt_in(const void* kernel, int form, int smem) {
+  static std::atomic<bool> done[kMaxDevices][kOptIns];
+  int device = 0;
+  if (const cudaError_t e = cudaGetDevice(&device); e != cudaSuccess) return cuda_fail(e, "cudaGetDevice");
+  if (device >= kMaxDevices) return fail(B200_ATTN_UNSUPPORTED, "device %d: at most %d devices", device, kMaxDevices);
+  if (done[device][form].load(std::memory_order_acquire)) return B200_ATTN_OK;
+  if (const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem); e != cudaSuccess) return cuda_fail(e, "cudaFuncSetAttribute(shared memory)");
+  done[device][form].store(true, std::memory_order_release);
+  return B200_ATTN_OK;
+}
+bool whole_words(const B200LayerNormArgs& a) { return static_cast<size_t>(a.dim) * element(a.dtype) % 16 == 0; }
 
 int check_norm(const B200LayerNormArgs* a) {
   if (a == nullptr) return fail(B200_ATTN_BAD_CONFIG, "args is NULL");
@@ -251,17 +309,6 @@ int head_map(CUtensorMap* map, const void* base, uint32_t dtype, int64_t rows, i
   return B200_ATTN_OK;
 }
 
-// Shared memory above 48 KB is allowed per kernel and device.
-int opt_in(const void* kernel, int form, int smem) {
-  static std::atomic<bool> done[kMaxDevices][6];
-  int device = 0;
-  if (const cudaError_t e = cudaGetDevice(&device); e != cudaSuccess) return cuda_fail(e, "cudaGetDevice");
-  if (device >= kMaxDevices) return fail(B200_ATTN_UNSUPPORTED, "device %d: at most %d devices", device, kMaxDevices);
-  if (done[device][form].load(std::memory_order_acquire)) return B200_ATTN_OK;
-  if (const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem); e != cudaSuccess) return cuda_fail(e, "cudaFuncSetAttribute(shared memory)");
-  done[device][form].store(true, std::memory_order_release);
-  return B200_ATTN_OK;
-}
 constexpr int kHeadSmemBytes = static_cast<int>(sizeof(HeadSmem)) + 1024;
 
 template <typename P>
@@ -497,7 +544,7 @@ extern "C" {
 
 int b200_layer_norm(const B200LayerNormArgs* a, void* stream_ptr) {
   if (int rc = check_norm(a)) return rc;
-  bool wide = static_cast<size_t>(a->dim) * element(a->dtype) % 16 == 0;
+  bool wide = whole_words(*a);
   if (int rc = check_rows("x", a->x, a->x_stride, a, a->dtype, &wide)) return rc;
   if (int rc = check_rows("y", a->y, a->y_stride, a, a->dtype, &wide)) return rc;
   if (a->rows > 1 && a->y_stride < a->dim) return fail(B200_ATTN_UNSUPPORTED, "rows of y overlap");
@@ -521,14 +568,17 @@ int b200_layer_norm_workspace(const B200LayerNormArgs* a, int64_t* bytes) {
   DeviceState* dev = nullptr;
   if (int rc = device_state(&dev)) return rc;
   *bytes = 0;  // of whichever form the addresses lead to
-  for (const bool wide : {false, true}) *bytes = std::max<int64_t>(*bytes, 8LL * a->dim * grad_ctas(*a, norm_form(*a, true, wide), dev->sms));
+  for (const bool wide : {false, true}) {
+    *bytes = std::max<int64_t>(*bytes, 8LL * a->dim * grad_ctas(*a, norm_form(*a, true, wide), dev->sms));
+    *bytes = std::max<int64_t>(*bytes, 8LL * a->dim * ring_plan(*a, wide && whole_words(*a), dev->sms).ctas);
+  }
   clear_error();
   return B200_ATTN_OK;
 }
 
 int b200_layer_norm_grad(const B200LayerNormArgs* a, void* stream_ptr) {
   if (int rc = check_norm(a)) return rc;
-  bool wide = static_cast<size_t>(a->dim) * element(a->dtype) % 16 == 0;
+  bool wide = whole_words(*a);
   if (int rc = check_rows("x", a->x, a->x_stride, a, a->dtype, &wide)) return rc;
   if (int rc = check_rows("dy", a->dy, a->dy_stride, a, a->dtype, &wide)) return rc;
   if (a->dx != nullptr) {
@@ -541,8 +591,10 @@ int b200_layer_norm_grad(const B200LayerNormArgs* a, void* stream_ptr) {
     if (reinterpret_cast<uintptr_t>(p) % element(a->weight_dtype) != 0) return fail(B200_ATTN_UNSUPPORTED, "dweight or dbias is not aligned to its values");
   DeviceState* dev = nullptr;
   if (int rc = device_state(&dev)) return rc;
+  const RingPlan ring = ring_plan(*a, wide, dev->sms);
+  const bool through = ring.form.kernel != nullptr;
   const NormForm f = norm_form(*a, true, wide);
-  const int ctas = grad_ctas(*a, f, dev->sms);
+  const int ctas = through ? ring.ctas : grad_ctas(*a, f, dev->sms);
   const bool want_dw = a->dweight != nullptr || a->dbias != nullptr;
   if (want_dw && (a->workspace == nullptr || !aligned16(a->workspace) || a->workspace_bytes < 8LL * a->dim * ctas))
     return fail(B200_ATTN_BAD_CONFIG, "workspace: %lld bytes on a 16-byte boundary are needed", 8LL * a->dim * ctas);
@@ -555,8 +607,18 @@ int b200_layer_norm_grad(const B200LayerNormArgs* a, void* stream_ptr) {
   p.want_dw = want_dw;
   const cudaStream_t stream = static_cast<cudaStream_t>(stream_ptr);
   void* args[] = {&p};
-  if (a->dx != nullptr || want_dw)
-    if (int rc = launch_kernel(f.kernel, static_cast<unsigned>(ctas), 1, f.threads == 32 ? 32 * kLnGradWarps : f.threads, f.threads == 32 ? 8 * static_cast<size_t>(a->dim) : 0, 1, stream, args, "layer_norm_grad kernel launch")) return rc;
+  if (a->dx == nullptr && !want_dw) {  // nothing is asked for
+    clear_error();
+    return B200_ATTN_OK;
+  }
+  if (through) {
+    p.slots = ring.slots;
+    p.status = dev->status;
+    if (int rc = opt_in(ring.form.kernel, kHeadForms + ring.index, ln_ring_bytes(1))) return rc;
+    if (int rc = launch_kernel(ring.form.kernel, static_cast<unsigned>(ctas), 1, 32 * kLnWarps, ring.smem, 1, stream, args, "layer_norm_grad kernel launch")) return rc;
+  } else if (int rc = launch_kernel(f.kernel, static_cast<unsigned>(ctas), 1, f.threads == 32 ? 32 * kLnGradWarps : f.threads, f.threads == 32 ? 8 * static_cast<size_t>(a->dim) : 0, 1, stream, args, "layer_norm_grad kernel launch")) {
+    return rc;
+  }
   if (want_dw) {
     NormJoinParams j{};
     j.partial = p.partial;

@@ -4,7 +4,8 @@
 //   t = dy w:  dx = r (t - mean(t) - h mean(t h)),  dw = sum_rows dy h,  db = sum_rows dy
 //
 // Both are bound by HBM: a row is read once, into registers, and everything that is computed of it comes from there. A row is shared by
-// as many threads as leave each some sixteen to thirty-two values; sums and the weights' gradients are fp32.
+// as many threads as leave each some sixteen to thirty-two values; sums and the weights' gradients are fp32. norm_rows_kernel is the forward pass;
+// norm_ring_grad_kernel the gradients of rows on 16-byte boundaries of up to 8192 16-bit or 4096 fp32 values, norm_rows_grad_kernel of all others.
 #pragma once
 
 #include <cuda_bf16.h>
@@ -31,6 +32,8 @@ struct LayerNormParams {
   float* partial;   // [CTAs][2][dim]: this CTA's part of dw and of db
   int want_dw;      // any of the two
   int wide;         // weights are fp32
+  int slots;        // rows of a group's ring
+  uint32_t* status;
   int64_t rows;
   int dim;
   float eps, inverse_dim;
@@ -66,6 +69,39 @@ __device__ __forceinline__ void ln_store(T* p, const LnVec<T, VEC>& r) {
   if constexpr (sizeof(r) == 16) *reinterpret_cast<uint4*>(p) = *reinterpret_cast<const uint4*>(&r);
   else *p = r.v[0];
 }
+// Two neighbouring values of sixteen bytes.
+template <typename T>
+__device__ __forceinline__ float2 ln_pair(const uint4& raw, int j) {
+  if constexpr (std::is_same<T, float>::value) {
+    return reinterpret_cast<const float2*>(&raw)[j];
+  } else {
+    const uint32_t v = reinterpret_cast<const uint32_t*>(&raw)[j];
+    if constexpr (std::is_same<T, __half>::value) return __half22float2(*reinterpret_cast<const __half2*>(&v));
+    else return make_float2(__uint_as_float(v << 16), __uint_as_float(v & 0xffff0000u));
+  }
+}
+
+// Eight (fp32: four) values rounded and packed: pairs convert in one instruction.
+template <typename T, int PAIRS>
+__device__ __forceinline__ uint4 ln_packed(const float2 (&v)[PAIRS]) {
+  if constexpr (std::is_same<T, float>::value) {
+    return make_uint4(__float_as_uint(v[0].x), __float_as_uint(v[0].y), __float_as_uint(v[1].x), __float_as_uint(v[1].y));
+  } else {
+    uint32_t out[4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      if constexpr (std::is_same<T, __half>::value) {
+        const __half2 h = __floats2half2_rn(v[j].x, v[j].y);
+        out[j] = *reinterpret_cast<const uint32_t*>(&h);
+      } else {
+        const __nv_bfloat162 h = __floats2bfloat162_rn(v[j].x, v[j].y);
+        out[j] = *reinterpret_cast<const uint32_t*>(&h);
+      }
+    }
+    return make_uint4(out[0], out[1], out[2], out[3]);
+  }
+}
+
 // VEC weights of the rows' type or, `wide`, fp32 (beside a 16-bit row two 16-byte loads).
 template <typename T, int VEC>
 __device__ __forceinline__ void ln_weights(const void* base, int c, bool wide, float (&out)[VEC]) {
@@ -95,6 +131,31 @@ __device__ __forceinline__ void ln_weights(const void* base, int c, bool wide, f
   }
 }
 
+// The same in pairs, or `missing` without weights.
+template <typename T, int VEC, int PAIRS>
+__device__ __forceinline__ void ln_weight_pairs(const void* base, int c, bool wide, float missing, float2 (&out)[PAIRS]) {
+  if (base == nullptr) {
+#pragma unroll
+    for (int j = 0; j < PAIRS; ++j) out[j] = make_float2(missing, missing);
+  } else if constexpr (VEC == 1) {
+    float v[1];
+    ln_weights<T, 1>(base, c, wide, v);
+    out[0] = make_float2(v[0], 0.f);
+  } else if (wide && !std::is_same<T, float>::value) {
+    const float4* const from = reinterpret_cast<const float4*>(static_cast<const float*>(base) + c);
+#pragma unroll
+    for (int j = 0; j < PAIRS; j += 2) {
+      const float4 f = __ldg(from + j / 2);
+      out[j] = make_float2(f.x, f.y);
+      out[j + 1] = make_float2(f.z, f.w);
+    }
+  } else {
+    const uint4 raw = __ldg(reinterpret_cast<const uint4*>(static_cast<const T*>(base) + c));
+#pragma unroll
+    for (int j = 0; j < PAIRS; ++j) out[j] = ln_pair<T>(raw, j);
+  }
+}
+
 __device__ __forceinline__ float2 ln_warp_sum2(float2 v) {
 #pragma unroll
   for (int d = 16; d > 0; d >>= 1) {
@@ -104,7 +165,30 @@ __device__ __forceinline__ float2 ln_warp_sum2(float2 v) {
   return v;
 }
 
+__device__ __forceinline__ float ln_warp_sum(float v) {
+#pragma unroll
+  for (int d = 16; d > 0; d >>= 1) v += __shfl_xor_sync(0xffffffffu, v, d);
+  return v;
+}
+// s / n as s times the rounded 1 / n and one correction: times that alone, a row of one value would come out as the product's error over sqrt(eps).
+__device__ __forceinline__ float ln_mean(float s, float n, float inverse_n) {
+  const float m = s * inverse_n;
+  return fmaf(fmaf(-m, n, s), inverse_n, m);
+}
+
 // Sums over the THREADS threads of a row (a warp, or the whole CTA; `turn` alternates between two places, so that one barrier a sum is enough).
+template <int THREADS>
+__device__ __forceinline__ float ln_row_sum(float v, float2 (*place)[32], int& turn) {
+  v = ln_warp_sum(v);
+  if constexpr (THREADS > 32) {
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    if (lane == 0) place[turn][warp].x = v;
+    __syncthreads();
+    v = ln_warp_sum(lane < THREADS / 32 ? place[turn][lane].x : 0.f);
+    turn ^= 1;
+  }
+  return v;
+}
 template <int THREADS>
 __device__ __forceinline__ float2 ln_row_sum2(float2 v, float2 (*place)[32], int& turn) {
   v = ln_warp_sum2(v);
@@ -121,7 +205,9 @@ __device__ __forceinline__ float2 ln_row_sum2(float2 v, float2 (*place)[32], int
 
 constexpr int kLnForwardRows = 4;  // rows of a CTA whose rows are a warp's each
 
-// Forward. THREADS of a row: 32 (four rows a CTA) or the CTA. A thread has N vectors, THREADS * VEC values apart.
+// Forward. THREADS of a row: 32 (four rows a CTA) or the CTA. A thread has N vectors, THREADS * VEC values apart; they go in pairs, which the packed
+// instructions take at once. us, value by value -> in pairs, and the time of the bytes: 8192 x 4096 in bf16 28.9 -> 24.3 (20.5), 21920 x 1024 17.9 -> 15.3
+// (13.7), 16384 x 2048 31.3 -> 26.4 (20.5); 8192 x 4096 in fp32 41.7 (41.0). 197 x 768: 2.8, the launch and a chain of latencies.
 template <typename T, int VEC, int N, int THREADS>
 __global__ void __launch_bounds__(THREADS == 32 ? 32 * kLnForwardRows : THREADS) norm_rows_kernel(const LayerNormParams p) {
   __shared__ float2 place[2][32];
@@ -129,52 +215,54 @@ __global__ void __launch_bounds__(THREADS == 32 ? 32 * kLnForwardRows : THREADS)
   grid_launch_dependents();
   const int64_t row = THREADS == 32 ? static_cast<int64_t>(blockIdx.x) * kLnForwardRows + (threadIdx.x >> 5) : blockIdx.x;
   if (row >= p.rows) return;  // (a whole warp, where rows are warps'; never where they are CTAs')
+  constexpr int kStep = THREADS * VEC, kPairs = VEC > 1 ? VEC / 2 : 1;
   const int at = (threadIdx.x & (THREADS - 1)) * VEC;
   const T* const x = static_cast<const T*>(p.x) + row * p.x_stride;
   LnVec<T, VEC> raw[N];
 #pragma unroll
   for (int i = 0; i < N; ++i)
-    if (at + i * THREADS * VEC < p.dim) raw[i] = ln_load<T, VEC>(x + at + i * THREADS * VEC);
+    if (at + i * kStep < p.dim) raw[i] = ln_load<T, VEC>(x + at + i * kStep);
+  // Kept as it came, and converted at each of three uses: held as fp32, it cost warps (8192 x 4096 in bf16 34.7 us; so 24.3).
+  // A single value is a pair whose second half does not count.
+  const auto pair = [&](int i, int j) {
+    if constexpr (VEC > 1) return ln_pair<T>(*reinterpret_cast<const uint4*>(&raw[i]), j);
+    else return make_float2(ln_float(raw[i].v[0]), 0.f);
+  };
   int turn = 0;
-  float s = 0.f;
+  float2 s = make_float2(0.f, 0.f);
 #pragma unroll
   for (int i = 0; i < N; ++i)
-    if (at + i * THREADS * VEC < p.dim) {
+    if (at + i * kStep < p.dim) {
 #pragma unroll
-      for (int j = 0; j < VEC; ++j) s += ln_float(raw[i].v[j]);
+      for (int j = 0; j < kPairs; ++j) s = fadd2(s, pair(i, j));
     }
-  // Divided: times the rounded 1 / dim, a row of one value would come out as that value's last bit over sqrt(eps).
-  const float mean = ln_row_sum2<THREADS>(make_float2(s, 0.f), place, turn).x / static_cast<float>(p.dim);
-  float q = 0.f;  // of the differences: no cancellation where the mean is large
+  const float mean = ln_mean(ln_row_sum<THREADS>(s.x + s.y, place, turn), static_cast<float>(p.dim), p.inverse_dim);
+  const float2 minus = make_float2(-mean, VEC > 1 ? -mean : 0.f);
+  float2 q = make_float2(0.f, 0.f);  // of the differences: no cancellation where the mean is large
 #pragma unroll
   for (int i = 0; i < N; ++i)
-    if (at + i * THREADS * VEC < p.dim) {
+    if (at + i * kStep < p.dim) {
 #pragma unroll
-      for (int j = 0; j < VEC; ++j) {
-        const float d = ln_float(raw[i].v[j]) - mean;
-        q = fmaf(d, d, q);
+      for (int j = 0; j < kPairs; ++j) {
+        const float2 d = fadd2(pair(i, j), minus);
+        q = ffma2(d, d, q);
       }
     }
-  const float var = ln_row_sum2<THREADS>(make_float2(q, 0.f), place, turn).x * p.inverse_dim;
-  const float r = 1.f / sqrtf(var + p.eps);
+  const float r = rsqrtf(ln_row_sum<THREADS>(q.x + q.y, place, turn) * p.inverse_dim + p.eps);
   if (p.stats != nullptr && at == 0) p.stats[row] = make_float2(mean, r);
   T* const y = static_cast<T*>(p.y) + row * p.y_stride;
+  const float2 r2 = make_float2(r, r);
 #pragma unroll
   for (int i = 0; i < N; ++i) {
-    const int c = at + i * THREADS * VEC;
+    const int c = at + i * kStep;
     if (c < p.dim) {
-      float w[VEC], b[VEC];
+      float2 w[kPairs], b[kPairs];
+      ln_weight_pairs<T, VEC>(p.w, c, p.wide != 0, 1.f, w);
+      ln_weight_pairs<T, VEC>(p.b, c, p.wide != 0, 0.f, b);
 #pragma unroll
-      for (int j = 0; j < VEC; ++j) {
-        w[j] = 1.f;
-        b[j] = 0.f;
-      }
-      if (p.w != nullptr) ln_weights<T, VEC>(p.w, c, p.wide != 0, w);
-      if (p.b != nullptr) ln_weights<T, VEC>(p.b, c, p.wide != 0, b);
-      LnVec<T, VEC> out;
-#pragma unroll
-      for (int j = 0; j < VEC; ++j) out.v[j] = ln_round<T>(fmaf((ln_float(raw[i].v[j]) - mean) * r, w[j], b[j]));
-      ln_store<T, VEC>(y + c, out);
+      for (int j = 0; j < kPairs; ++j) w[j] = ffma2(fmul2(fadd2(pair(i, j), minus), r2), w[j], b[j]);
+      if constexpr (VEC > 1) *reinterpret_cast<uint4*>(y + c) = ln_packed<T>(w);
+      else y[c] = ln_round<T>(w[0].x);
     }
   }
 }
@@ -286,6 +374,238 @@ __global__ void __launch_bounds__(THREADS == 32 ? 32 * kLnGradWarps : THREADS) n
   }
 }
 
+// ---- gradients, rows through shared memory -----------------------------------------------------------------------------------------------
+// Sums behind dw and db want the CTAs to stay, and then what HBM needs in flight does not fit beside a row in registers. G warps share a row, and every
+// such group has a ring of rows that one of its lanes fills with bulk copies (cp.async.bulk, 16-byte addresses and sizes), up to 200 KB an
+// SM. A slot is filled again as soon as the group has it in registers. Slots are as wide as G warps of N vectors, with zeros behind the row, so that
+// no value is tested for being one; weights stay in registers as fp32 pairs (with a test and a conversion at each use a value took 29
+// instructions, and 8192 rows of 4096 54 us). us with the join, of bf16: a row a CTA with the next one in registers (norm_rows_grad_kernel) -> here, and
+// the time of the bytes: 8192 x 4096 75.0 -> 41.5 (30.8), 21920 x 1024 48.4 -> 32.8 (20.6), 30000 x 512 64.4 -> 22.6 (14.1); 5480 x 384 in fp32
+// 14.5 -> 11.0 (3.9). Bound by HBM and, at sixteen warps an SM, by the chain of copy, sums and barrier of each row. The same for the forward pass was
+// slower than rows in registers (8192 x 4096 29.2, 24.3 there): two barriers a row, and nothing that has to stay.
+constexpr int kLnWarps = 8, kLnMostSlots = 16;
+constexpr uint32_t kStatusNormWait = 1u << 24;
+// CTAs an SM holds, as their registers allow, and the ring of each.
+constexpr int ln_ring_ctas(int values) { return values <= 16 ? 2 : 1; }
+constexpr int ln_ring_bytes(int ctas) { return ctas == 2 ? 104 * 1024 : 208 * 1024; }
+
+struct LnRingSmem {
+  uint64_t full[kLnWarps][kLnMostSlots];
+  alignas(16) float2 place[kLnWarps][2][kLnWarps];  // of each group, alternately: its warps' sums
+  uint32_t abort;
+};
+
+__device__ __forceinline__ void ln_bulk_load(uint32_t smem_dst, const void* src, uint32_t bytes, uint64_t* bar) {
+  asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];"
+               :
+               : "r"(smem_dst), "l"(reinterpret_cast<uint64_t>(src)), "r"(bytes), "r"(smem_u32(bar))
+               : "memory");
+}
+
+template <int G>
+__device__ __forceinline__ void ln_group_sync(int group) {
+  if constexpr (G == 1) __syncwarp();
+  else asm volatile("barrier.cta.sync %0, %1;" ::"r"(group + 1), "n"(G * 32) : "memory");
+}
+// Both sums over a group, in the order of its warps: the halves of a warp take one each after the first exchange. Behind it every thread of the
+// group has passed the point where it was called.
+template <int G>
+__device__ __forceinline__ float2 ln_group_sum2(float2 v, LnRingSmem& sm, int group, int& turn) {
+  const int lane = threadIdx.x & 31;
+  float one = lane < 16 ? v.x : v.y;
+  one += __shfl_xor_sync(0xffffffffu, lane < 16 ? v.y : v.x, 16);
+#pragma unroll
+  for (int d = 8; d > 0; d >>= 1) one += __shfl_xor_sync(0xffffffffu, one, d);
+  if constexpr (G == 1) {
+    const float other = __shfl_xor_sync(0xffffffffu, one, 16);
+    return lane < 16 ? make_float2(one, other) : make_float2(other, one);
+  } else {
+    if ((lane & 15) == 0) reinterpret_cast<float*>(&sm.place[group][turn][(threadIdx.x >> 5) % G])[lane >> 4] = one;
+    ln_group_sync<G>(group);
+    const float4* const from = reinterpret_cast<const float4*>(sm.place[group][turn]);
+    float2 sum = make_float2(0.f, 0.f);
+#pragma unroll
+    for (int i = 0; i < G / 2; ++i) {
+      const float4 o = from[i];
+      sum = fadd2(fadd2(sum, make_float2(o.x, o.y)), make_float2(o.z, o.w));
+    }
+    turn ^= 1;
+    return sum;
+  }
+}
+// A group's ring: rows first, first + step, ... of x and dy, a slot for both.
+struct LnRing {
+  uint32_t slots;  // of this group, in shared memory
+  uint64_t* full;
+  const uint8_t *a, *b;  // the next row to be asked for
+  int64_t a_step, b_step;  // bytes
+  int64_t next, step, rows;
+  uint32_t bytes, row_bytes;  // of a row, and of its place
+  int count, slot;
+  uint32_t phase;
+  bool leader;
+
+  __device__ __forceinline__ void fill(int at, const uint32_t* abort) {
+    if (next < rows) {
+      if (leader && *static_cast<const volatile uint32_t*>(abort) == 0) {
+        mbar_arrive_expect_tx(&full[at], 2 * bytes);
+        ln_bulk_load(slots + 2 * at * row_bytes, a, bytes, &full[at]);
+        ln_bulk_load(slots + (2 * at + 1) * row_bytes, b, bytes, &full[at]);
+      }
+      next += step;
+      a += a_step;
+      b += b_step;
+    }
+  }
+  __device__ __forceinline__ uint32_t wait(uint32_t* abort, uint32_t* status) {
+    if (!mbar_wait(&full[slot], phase, abort) && atomicExch(abort, 1u) == 0) atomicOr(status, kStatusNormWait);  // the rest runs through, with what is there
+    return slots + 2 * slot * row_bytes;
+  }
+  __device__ __forceinline__ void advance() {
+    if (++slot == count) {
+      slot = 0;
+      phase ^= 1;
+    }
+  }
+  // Copies still on their way when a wait has run out must land before the CTA goes. (Each slot's last use; where one was never used, its
+  // barrier stands at phase 0, and the wait for phase 1 ends at once.)
+  __device__ __forceinline__ void drain(const uint32_t* abort) const {
+    if (*static_cast<const volatile uint32_t*>(abort) == 0 || !leader) return;
+    uint32_t no_abort = 0;
+    for (int i = 0; i < count; ++i) mbar_wait(&full[i], i < slot ? phase : phase ^ 1, &no_abort);
+  }
+};
+
+template <typename T, int VEC, int N, int G>
+__device__ __forceinline__ LnRing ln_ring(LnRingSmem& sm, uint8_t* memory, const LayerNormParams& p) {
+  constexpr int kGroups = kLnWarps / G;
+  const int group = (threadIdx.x >> 5) / G;
+  LnRing r;
+  r.bytes = static_cast<uint32_t>(p.dim * sizeof(T));
+  r.row_bytes = G * 32 * VEC * N * sizeof(T);
+  r.count = p.slots;
+  r.slots = smem_u32(memory) + 2 * group * p.slots * r.row_bytes;
+  r.full = sm.full[group];
+  r.rows = p.rows;
+  r.step = static_cast<int64_t>(gridDim.x) * kGroups;
+  r.next = static_cast<int64_t>(blockIdx.x) * kGroups + group;
+  r.a = reinterpret_cast<const uint8_t*>(static_cast<const T*>(p.x) + r.next * p.x_stride);
+  r.b = reinterpret_cast<const uint8_t*>(static_cast<const T*>(p.dy) + r.next * p.dy_stride);
+  r.a_step = r.step * p.x_stride * static_cast<int64_t>(sizeof(T));
+  r.b_step = r.step * p.dy_stride * static_cast<int64_t>(sizeof(T));
+  r.slot = 0;
+  r.phase = 0;
+  r.leader = threadIdx.x % (G * 32) == 0;
+  if (threadIdx.x == 0) {
+    for (int g = 0; g < kGroups; ++g)
+      for (int i = 0; i < p.slots; ++i) mbar_init(&sm.full[g][i], 1);
+    sm.abort = 0;
+    mbar_init_fence();
+  }
+  const uint32_t tail = r.row_bytes - r.bytes;  // a multiple of 16, as both are
+  if (tail > 0) {
+    const int words = static_cast<int>(tail >> 4), places = 2 * kGroups * p.slots;
+    for (int i = threadIdx.x; i < places * words; i += 32 * kLnWarps) {
+      const int at = i / words;
+      st_shared_v4(smem_u32(memory) + at * r.row_bytes + r.bytes + (i - at * words) * 16, make_uint4(0, 0, 0, 0));
+    }
+  }
+  __syncthreads();
+  return r;
+}
+
+// Gradients: one pass for the sums, dw and db, one barrier, dx from registers.
+template <typename T, int VEC, int N, int G>
+__global__ void __launch_bounds__(32 * kLnWarps, ln_ring_ctas(N * VEC)) norm_ring_grad_kernel(const LayerNormParams p) {
+  extern __shared__ __align__(128) uint8_t ln_memory[];
+  __shared__ LnRingSmem sm;
+  constexpr int kStep = G * 32 * VEC, kGroups = kLnWarps / G, kPairs = VEC / 2;
+  const int group = (threadIdx.x >> 5) / G, at = (threadIdx.x % (G * 32)) * VEC;
+  LnRing ring = ln_ring<T, VEC, N, G>(sm, ln_memory, p);
+  grid_dependency_wait();
+  grid_launch_dependents();
+  int64_t row = ring.next;
+  for (int i = 0; i < ring.count; ++i) ring.fill(i, &sm.abort);
+  float2 w[N][kPairs], dw[N][kPairs], db[N][kPairs];
+#pragma unroll
+  for (int i = 0; i < N; ++i) {
+    ln_weight_pairs<T, VEC>(at + i * kStep < p.dim ? p.w : nullptr, at + i * kStep, p.wide != 0, 1.f, w[i]);
+#pragma unroll
+    for (int j = 0; j < kPairs; ++j) dw[i][j] = db[i][j] = make_float2(0.f, 0.f);
+  }
+  float2 stats = row < p.rows ? __ldg(p.stats + row) : make_float2(0.f, 0.f);
+  T* dx = static_cast<T*>(p.dx) + row * p.dx_stride + at;
+  const int64_t dx_step = ring.step * p.dx_stride;
+  int turn = 0;
+  for (; row < p.rows; row += ring.step, dx += dx_step) {
+    const float2 minus = make_float2(-stats.x, -stats.x), r2 = make_float2(stats.y, stats.y);
+    const uint32_t slot = ring.wait(&sm.abort, p.status) + at * static_cast<int>(sizeof(T));
+    if (row + ring.step < p.rows) stats = __ldg(p.stats + row + ring.step);
+    float2 t[N][kPairs], h[N][kPairs], s = make_float2(0.f, 0.f), q = s;
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      const uint4 x = ld_shared_v4(slot + i * kStep * static_cast<int>(sizeof(T))), g = ld_shared_v4(slot + ring.row_bytes + i * kStep * static_cast<int>(sizeof(T)));
+#pragma unroll
+      for (int j = 0; j < kPairs; ++j) {
+        const float2 d = ln_pair<T>(g, j);
+        h[i][j] = fmul2(fadd2(ln_pair<T>(x, j), minus), r2);
+        db[i][j] = fadd2(db[i][j], d);
+        dw[i][j] = ffma2(d, h[i][j], dw[i][j]);
+        t[i][j] = fmul2(d, w[i][j]);
+        s = fadd2(s, t[i][j]);
+        q = ffma2(t[i][j], h[i][j], q);
+      }
+    }
+    s = ln_group_sum2<G>(make_float2(s.x + s.y, q.x + q.y), sm, group, turn);
+    if constexpr (G == 1) __syncwarp();
+    ring.fill(ring.slot, &sm.abort);
+    ring.advance();
+    if (p.dx == nullptr) continue;
+    const float mean_t = s.x * p.inverse_dim, mean_th = s.y * p.inverse_dim;
+    const float2 mt2 = make_float2(-mean_t, -mean_t), mh2 = make_float2(-mean_th, -mean_th);
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+#pragma unroll
+      for (int j = 0; j < kPairs; ++j) t[i][j] = fmul2(ffma2(h[i][j], mh2, fadd2(t[i][j], mt2)), r2);
+      if (at + i * kStep < p.dim) *reinterpret_cast<uint4*>(dx + i * kStep) = ln_packed<T>(t[i]);
+    }
+  }
+  ring.drain(&sm.abort);
+  if (!p.want_dw) return;
+  // The groups' parts, added in the order of the groups in what was the ring: every copy has landed, every slot has been read.
+  float* const out = p.partial + static_cast<int64_t>(blockIdx.x) * 2 * p.dim;
+  float* const joined = reinterpret_cast<float*>(ln_memory);
+  if constexpr (kGroups > 1) {
+    for (int turn_of = 0; turn_of < kGroups; ++turn_of) {
+      __syncthreads();
+      if (group != turn_of) continue;
+#pragma unroll
+      for (int i = 0; i < N; ++i) {
+        if (at + i * kStep >= p.dim) continue;
+#pragma unroll
+        for (int j = 0; j < kPairs; ++j) {
+          float2* const to_w = reinterpret_cast<float2*>(joined + at + i * kStep) + j;
+          float2* const to_b = reinterpret_cast<float2*>(joined + p.dim + at + i * kStep) + j;
+          *to_w = turn_of == 0 ? dw[i][j] : fadd2(*to_w, dw[i][j]);
+          *to_b = turn_of == 0 ? db[i][j] : fadd2(*to_b, db[i][j]);
+        }
+      }
+    }
+    __syncthreads();
+    for (int c = threadIdx.x; c < p.dim / 2; c += 32 * kLnWarps) reinterpret_cast<float4*>(out)[c] = reinterpret_cast<const float4*>(joined)[c];
+  } else {
+#pragma unroll
+    for (int i = 0; i < N; ++i)
+      if (at + i * kStep < p.dim) {
+#pragma unroll
+        for (int j = 0; j < kPairs; j += 2) {
+          *reinterpret_cast<float4*>(out + at + i * kStep + 2 * j) = make_float4(dw[i][j].x, dw[i][j].y, dw[i][j + 1].x, dw[i][j + 1].y);
+          *reinterpret_cast<float4*>(out + p.dim + at + i * kStep + 2 * j) = make_float4(db[i][j].x, db[i][j].y, db[i][j + 1].x, db[i][j + 1].y);
+        }
+      }
+  }
+}
+
 // The CTAs' parts of dw and db added up: 32 columns a CTA, a warp every 32nd part, then the warps' sums in their order.
 struct NormJoinParams {
   const float* partial;  // [parts][2][dim]
@@ -306,7 +626,7 @@ __global__ void __launch_bounds__(32 * kLnJoinWarps) norm_join_kernel(const Norm
   if (out == nullptr) return;
   float s = 0.f;
   if (c < p.dim) {
-#pragma unroll 4
+#pragma unroll 10
     for (int i = warp; i < p.parts; i += kLnJoinWarps) s += __ldg(p.partial + (static_cast<int64_t>(i) * 2 + which) * p.dim + c);
   }
   sums[warp][lane] = s;
