@@ -840,7 +840,7 @@ struct HeadRowsParams {
   float* loss;           // [rows] or null: 0 for rows that do not count
   uint32_t* status;
 };
-constexpr int kRowsThreads = 256, kRowsMost = 1024;
+constexpr int kRowsThreads = 256, kRowsMost = 1024, kRowsAtOnce = 8;
 
 __global__ void __launch_bounds__(kRowsThreads) head_rows_kernel(const HeadRowsParams p) {
   __shared__ int from[kRowsMost], before_all, count_all, warp_sums[kRowsThreads / 32];
@@ -853,6 +853,7 @@ __global__ void __launch_bounds__(kRowsThreads) head_rows_kernel(const HeadRowsP
   const auto counted = [&](int r) { return p.targets == nullptr ? p.counts[r] != 0 : target(r) != p.ignore; };
   const int r0 = blockIdx.x * p.per_cta, r1 = min(p.rows, r0 + p.per_cta);
   int before = 0, all = 0;
+#pragma unroll 8
   for (int r = tid; r < p.rows; r += kRowsThreads) {
     const int c = counted(r) ? 1 : 0;
     all += c;
@@ -909,7 +910,16 @@ __global__ void __launch_bounds__(kRowsThreads) head_rows_kernel(const HeadRowsP
     const int to = from[r - r0];
     if (to < 0) continue;
     const uint4* const in = reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(p.x) + r * p.ldx);
-    for (int i = lane; i < words; i += 32) p.x_copy[static_cast<int64_t>(to) * words + i] = in[i];
+    uint4* const out = p.x_copy + static_cast<int64_t>(to) * words;
+    for (int i = lane; i < words; i += 32 * kRowsAtOnce) {
+      uint4 v[kRowsAtOnce];
+#pragma unroll
+      for (int j = 0; j < kRowsAtOnce; ++j)
+        if (i + 32 * j < words) v[j] = in[i + 32 * j];
+#pragma unroll
+      for (int j = 0; j < kRowsAtOnce; ++j)
+        if (i + 32 * j < words) out[i + 32 * j] = v[j];
+    }
   }
   if (blockIdx.x == gridDim.x - 1)
     for (int64_t i = static_cast<int64_t>(count) * words + tid; i < static_cast<int64_t>((count + 63) & ~63) * words; i += kRowsThreads) p.x_copy[i] = make_uint4(0, 0, 0, 0);
@@ -934,7 +944,7 @@ struct HeadLossParams {
   float* sums;           // [CTAs]
   unsigned* finished;
 };
-constexpr int kLossThreads = 1024;
+constexpr int kLossThreads = 1024, kLossAtOnce = 8;
 
 __global__ void __launch_bounds__(kLossThreads) head_loss_kernel(const HeadLossParams p) {
   __shared__ float2 part[32][33];
@@ -947,11 +957,17 @@ __global__ void __launch_bounds__(kLossThreads) head_loss_kernel(const HeadLossP
   const int count = *p.count, row0 = blockIdx.x * 32;
   float m = -INFINITY, s = 0.f;
   if (row0 + lane < count) {
-#pragma unroll 4
-    for (int i = warp; i < p.n_parts; i += 32) {
-      const float2 v = __ldg(p.parts + i * p.parts_stride + row0 + lane);
-      const float m_new = fmaxf(m, v.x), from = m_new == -INFINITY ? 0.f : m_new;
-      s = s * head_ex2(m - from) + v.y * head_ex2(v.x - from);
+    for (int i = warp; i < p.n_parts; i += 32 * kLossAtOnce) {  // so many loads in flight, one maximum for them
+      float2 v[kLossAtOnce];
+#pragma unroll
+      for (int j = 0; j < kLossAtOnce; ++j) v[j] = i + 32 * j < p.n_parts ? __ldg(p.parts + (i + 32 * j) * p.parts_stride + row0 + lane) : make_float2(-INFINITY, 0.f);
+      float m_new = m;
+#pragma unroll
+      for (int j = 0; j < kLossAtOnce; ++j) m_new = fmaxf(m_new, v[j].x);
+      const float from = m_new == -INFINITY ? 0.f : m_new;
+      s *= head_ex2(m - from);
+#pragma unroll
+      for (int j = 0; j < kLossAtOnce; ++j) s = fmaf(v[j].y, head_ex2(v[j].x - from), s);
       m = m_new;
     }
   }
