@@ -106,7 +106,7 @@ RingPlan ring_plan(const B200LayerNormArgs& a, bool wide_rows, int sms) {
 size_t element(uint32_t dtype) { return dtype == B200_ATTN_F32 ? 4 : 2; }
 
 // Shared memory above 48 KB is allowed per kernel and device.
-constexpr int kHeadForms = 6, kOptIns = kHeadForms + 3 * kMostRingForms;
+constexpr int kHeadForms = 8, kOptIns = kHeadForms + 3 * kMostRingForms;
 int opt_in(const void* kernel, int form, int smem) {
   static std::atomic<bool> done[kMaxDevices][kOptIns];
   int device = 0;
@@ -211,19 +211,43 @@ int logits_bn(int64_t row_tiles, int64_t cols, int pairs) {
 }
 int ring_stages(int bn) { return std::min(kHeadMaxStages, kHeadRingBytes / (kGemmTileBytes + bn * kGemmBK)); }
 
+// How few rows are cut (head_few_kernel), n = 0: they go by pairs.
+struct FewPlan {
+  int n, cols, tiles, height, stages, sums, buffers;
+};
+FewPlan few_plan(const B200HeadArgs& a, int sms) {
+  FewPlan f{};
+  const int64_t n = up(a.rows, 16), cols = up(a.rows, 32);
+  const int k_blocks = (a.dim + kGemmBK - 1) / kGemmBK, sums = (k_blocks + kHeadSumBlocks - 1) / kHeadSumBlocks;
+  if (n > kFewRows || cols * sums > 512) return f;
+  f.n = static_cast<int>(n);
+  f.cols = static_cast<int>(cols);
+  f.sums = sums;
+  f.buffers = 2 * cols * sums <= 512 ? 2 : 1;
+  const int each = (a.vocab + 128 * sms - 1) / (128 * sms);  // tiles of an SM
+  f.height = static_cast<int>(std::max<int64_t>(32, up((a.vocab + static_cast<int64_t>(sms) * each - 1) / (static_cast<int64_t>(sms) * each), 8)));
+  f.tiles = (a.vocab + f.height - 1) / f.height;
+  f.stages = std::min(kFewMostStages, (kFewSmemBytes - 1024 - kFewRing) / static_cast<int>(few_stage_bytes(f.n)));
+  return f;
+}
+
 struct HeadLossWork {
-  int bn, tiles_n;
+  FewPlan few;
+  int bn, tiles_n, n_parts;
   int64_t parts_stride;
   int64_t parts, picks, sums, bytes;
 };
-HeadLossWork head_loss_work(const B200HeadArgs& a, int pairs) {
+HeadLossWork head_loss_work(const B200HeadArgs& a, int sms) {
+  const int pairs = std::max(1, sms / 2);
   HeadLossWork w{};
   const int64_t row_tiles = (a.rows + 255) / 256;
   w.bn = logits_bn(row_tiles, a.vocab, pairs);
   w.tiles_n = (a.vocab + w.bn - 1) / w.bn;
+  w.few = few_plan(a, sms);
+  w.n_parts = w.few.n > 0 ? 4 * w.few.tiles : 2 * w.tiles_n;
   w.parts_stride = up(a.rows, 32);
   Layout l;
-  w.parts = l.add(8 * 2LL * w.tiles_n * w.parts_stride);
+  w.parts = l.add(8LL * w.n_parts * w.parts_stride);
   w.picks = l.add(4LL * a.rows * std::max(a.top, 1));
   w.sums = l.add(4 * ((a.rows + 31) / 32));
   w.bytes = l.bytes;
@@ -346,15 +370,17 @@ int launch_loss(const B200HeadArgs& a, cudaStream_t stream) {
   if (int rc = device_state(&dev)) return rc;
   const int pairs = std::max(1, dev->sms / 2);
   const HeadState s = head_state(a);
-  const HeadLossWork w = head_loss_work(a, pairs);
+  const HeadLossWork w = head_loss_work(a, dev->sms);
   if (a.workspace_bytes < w.bytes) return fail(B200_ATTN_BAD_CONFIG, "workspace: %lld bytes are needed", static_cast<long long>(w.bytes));
   CUtensorMap mx, mc, mw;
-  if (int rc = head_map(&mx, a.x, a.dtype, a.rows, a.dim, a.ldx, 64, 128, "x")) return rc;
-  if (int rc = head_map(&mc, at<void>(a.state, s.x_copy), a.dtype, up(a.rows, 64), a.dim, a.dim, 64, 128, "x")) return rc;
-  if (int rc = head_map(&mw, a.w, a.dtype, a.vocab, a.dim, a.ldw, 64, w.bn / 2, "w")) return rc;
+  const bool few = w.few.n > 0;
+  if (int rc = head_map(&mx, a.x, a.dtype, a.rows, a.dim, a.ldx, 64, few ? w.few.n : 128, "x")) return rc;
+  if (int rc = head_map(&mc, at<void>(a.state, s.x_copy), a.dtype, up(a.rows, 64), a.dim, a.dim, 64, few ? w.few.n : 128, "x")) return rc;
+  if (int rc = head_map(&mw, a.w, a.dtype, a.vocab, a.dim, a.ldw, 64, few ? w.few.height : w.bn / 2, "w")) return rc;
   const bool f16 = a.dtype == B200_ATTN_F16;
+  const void* few_stats = f16 ? reinterpret_cast<const void*>(head_few_kernel<__half>) : reinterpret_cast<const void*>(head_few_kernel<__nv_bfloat16>);
   const void* stats = f16 ? reinterpret_cast<const void*>(head_stats_kernel<__half>) : reinterpret_cast<const void*>(head_stats_kernel<__nv_bfloat16>);
-  if (int rc = opt_in(stats, f16 ? 0 : 1, kHeadSmemBytes)) return rc;
+  if (int rc = few ? opt_in(few_stats, f16 ? 6 : 7, kFewSmemBytes) : opt_in(stats, f16 ? 0 : 1, kHeadSmemBytes)) return rc;
   if (a.top > 0) {
     HeadEntriesParams e{};
     e.ids = a.targets;
@@ -408,7 +434,11 @@ int launch_loss(const B200HeadArgs& a, cudaStream_t stream) {
   p.parts = at<float2>(a.workspace, w.parts);
   p.parts_stride = w.parts_stride;
   p.picks = at<float>(a.workspace, w.picks);
-  {
+  if (few) {
+    HeadFewParams q{p, w.few.tiles, w.few.height, w.few.n, w.few.cols, w.few.stages, w.few.sums, w.few.buffers};
+    void* args[] = {&mx, &mc, &mw, &q};
+    if (int rc = launch_kernel(few_stats, static_cast<unsigned>(std::min(w.few.tiles, dev->sms)), 1, kFewThreads, kFewSmemBytes, 1, stream, args, "head_few kernel launch")) return rc;
+  } else {
     const int64_t items = (static_cast<int64_t>(a.rows) + 255) / 256 * w.tiles_n;
     void* args[] = {&mx, &mc, &mw, &p};
     if (int rc = launch_kernel(stats, static_cast<unsigned>(2 * std::min<int64_t>(items, pairs)), 1, kHeadThreads, kHeadSmemBytes, 2, stream, args, "head_stats kernel launch")) return rc;
@@ -418,7 +448,7 @@ int launch_loss(const B200HeadArgs& a, cudaStream_t stream) {
   l.idx = p.idx;
   l.parts = p.parts;
   l.parts_stride = p.parts_stride;
-  l.n_parts = 2 * w.tiles_n;
+  l.n_parts = w.n_parts;
   l.top = p.top;
   l.picks = p.picks;
   l.p = p.p;
@@ -643,7 +673,7 @@ int b200_head_sizes(const B200HeadArgs* a, int64_t* state, int64_t* loss_workspa
   if (int rc = device_state(&dev)) return rc;
   const int pairs = std::max(1, dev->sms / 2);
   *state = head_state(*a).bytes;
-  *loss_workspace = head_loss_work(*a, pairs).bytes;
+  *loss_workspace = head_loss_work(*a, dev->sms).bytes;
   *grad_workspace = 0;
   for (int want = 1; want < 4; ++want) *grad_workspace = std::max(*grad_workspace, head_grad_work(*a, (want & 1) != 0, (want & 2) != 0, pairs).bytes);
   clear_error();

@@ -13,6 +13,7 @@
 //   head_rows_kernel     which rows count, where they go, their copy
 //   head_stats_kernel    logits of 256 x bn tiles in tensor memory; leaves a maximum and a sum of exponentials per row and half
 //                        of a tile's columns, and the logits of the row's entries
+//   head_few_kernel      the same of up to 256 rows
 //   head_loss_kernel     joins those to lse and loss
 //   head_coef_kernel     gradients that differ from row to row: one power of two for all
 //   head_grads_kernel    a piece of the vocabulary: the logits again, their gradient in 16 bits
@@ -513,6 +514,222 @@ struct HeadLogitsJob {
   };
 };
 
+// ---- logits of few rows: statistics ----------------------------------------------------------------------------------------------------
+// Up to 64 rows leave most of a 256 x 256 tile of the pairs empty and its tiles unevenly dealt, where only the weight's way from HBM counts. Here the
+// vocabulary is the M side: a CTA takes `height` rows of w, at most 128 and such that every SM gets the same number of tiles, against all rows of x (N, a
+// multiple of 16). Sums of more than 1024 products go to accumulators of their own, side by side in tensor memory. A warp of the epilogue has 32 rows
+// of w; it turns 32 x 32 logits through shared memory, after which a lane has a row of x. us of a loss, by pairs -> here: 1 x 32000 x 4096 79.6 -> 56.9 (the
+// weight alone 40.1), 16 rows 61.9 -> 55.3, 64 rows 64.7 -> 61.1, 64 x 128000 x 4096 206 -> 190 (160), 1 x 1000 x 768 13.4 -> 12.0; but of 128 rows 62.9 and
+// 64.9, of 256 x 32000 x 2048 38.5 and 52.1: every CTA reads all of x. Bound by HBM behind a ramp: 77 % of its peak over 1 GB, 63 % over 262 MB.
+struct HeadFewParams {
+  HeadLogitsParams l;    // (v0, tiles_n, bn, stages, group are not looked at)
+  int tiles, height;
+  int n, cols;           // columns of a product, and of an accumulator: a multiple of 32, which is what a load of the epilogue takes
+  int stages;
+  int sums, buffers;     // accumulators of a tile; tiles that fit tensor memory side by side, 1 or 2
+};
+constexpr int kFewThreads = 320;  // warp 0 loader, warp 1 MMA, warps 2..9 epilogue
+constexpr int kFewRows = 64, kFewMostStages = 12;
+struct FewSmem {
+  float turned[8][32][33];  // of each epilogue warp: [row of x][row of w]
+  uint64_t full[kFewMostStages], empty[kFewMostStages], acc_full[2], acc_empty[2], drain;
+  uint32_t tmem_base;
+  uint32_t abort;
+};
+constexpr int kFewRing = (static_cast<int>(sizeof(FewSmem)) + 1023) & ~1023;  // where the ring begins
+constexpr int kFewSmemBytes = 226 * 1024;  // with the 1024 bytes of alignment
+__host__ __device__ constexpr uint32_t few_stage_bytes(int n) { return kGemmTileBytes + static_cast<uint32_t>(n) * 128; }
+
+template <typename T>
+__device__ __forceinline__ void head_few(const CUtensorMap* x, const CUtensorMap* x_copy, const CUtensorMap* w, const HeadFewParams& p, uint8_t* memory) {
+  FewSmem& sm = *reinterpret_cast<FewSmem*>(memory);
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  if (warp == 0) {
+    for (int i = lane; i < kFewMostStages; i += 32) {
+      mbar_init(&sm.full[i], 1);
+      mbar_init(&sm.empty[i], 1);
+    }
+    if (lane < 2) {
+      mbar_init(&sm.acc_full[lane], 1);
+      mbar_init(&sm.acc_empty[lane], 8);
+    }
+    if (lane == 0) {
+      mbar_init(&sm.drain, 1);
+      sm.abort = 0;
+    }
+    mbar_init_fence();
+    __syncwarp();
+  }
+  if (warp == 1) {
+    tmem_alloc(&sm.tmem_base, 512);
+    tmem_relinquish();
+  }
+  tc_fence_before_sync();
+  __syncthreads();
+  tc_fence_after_sync();
+  const uint32_t tmem = sm.tmem_base;
+  volatile uint32_t* abort_flag = &sm.abort;
+  const int k_blocks = (p.l.dim + kGemmBK - 1) / kGemmBK;
+  uint8_t* const ring = memory + kFewRing;
+  const uint32_t stage_size = few_stage_bytes(p.n);
+  const uint32_t bytes = static_cast<uint32_t>(p.height) * 128 + static_cast<uint32_t>(p.n) * 128;
+  int early = 0;  // stages whose part of w is on its way before the wait: the kernel in front (head_rows_kernel) does not write it, and when this one
+                  // starts, whatever wrote it is done
+  if (warp == 0 && static_cast<int>(blockIdx.x) < p.tiles) {
+    for (; early < p.stages && early < k_blocks; ++early) {
+      if (elect_one()) {
+        mbar_arrive_expect_tx(&sm.full[early], bytes);
+        tma_load_2d(ring + early * stage_size, w, &sm.full[early], early * kGemmBK, blockIdx.x * p.height);
+      }
+    }
+  }
+  grid_dependency_wait();
+  grid_launch_dependents();
+  const int rows = __ldg(p.l.count);
+  const int tiles = p.tiles;
+
+  if (warp == 0) {
+    // ======================= loader ==================================================================
+    const CUtensorMap* const from = rows < p.l.all_rows ? x_copy : x;
+    bool ok = true;
+    int g = 0, st = 0;
+    uint32_t ph = 1;
+    for (int tile = blockIdx.x; tile < tiles && ok; tile += gridDim.x) {
+      for (int kb = 0; kb < k_blocks; ++kb, ++g) {
+        if (g < early) {
+          if (elect_one()) tma_load_2d(ring + st * stage_size + kGemmTileBytes, from, &sm.full[st], kb * kGemmBK, 0);
+        } else {
+          ok = __all_sync(0xffffffffu, mbar_wait(&sm.empty[st], ph, abort_flag));
+          if (!ok) break;
+          if (elect_one()) {
+            mbar_arrive_expect_tx(&sm.full[st], bytes);
+            tma_load_2d(ring + st * stage_size, w, &sm.full[st], kb * kGemmBK, tile * p.height);
+            tma_load_2d(ring + st * stage_size + kGemmTileBytes, from, &sm.full[st], kb * kGemmBK, 0);
+          }
+        }
+        if (++st == p.stages) {
+          st = 0;
+          ph ^= 1;
+        }
+      }
+    }
+    if (!ok && lane == 0 && atomicExch(const_cast<uint32_t*>(abort_flag), 1u) == 0) atomicOr(p.l.status, kStatusHeadWait);
+    if (__any_sync(0xffffffffu, *abort_flag != 0)) {  // let every copy that was issued land
+      uint32_t no_abort = 0;
+      for (int j = (g > p.stages ? g - p.stages : 0); j < g; ++j) mbar_wait(&sm.full[j % p.stages], (j / p.stages) & 1, &no_abort);
+    }
+    __syncwarp();
+  } else if (warp == 1) {
+    // ======================= MMA issuer ==============================================================
+    const uint32_t idesc = umma_idesc_f16(std::is_same<T, __half>::value ? UMMA_F16 : UMMA_BF16, 128, p.n, 0, 0);
+    const uint64_t a0 = umma_smem_desc_sw128(smem_u32(ring), 1024, 16), b0 = umma_smem_desc_sw128(smem_u32(ring) + kGemmTileBytes, 1024, 16);
+    bool ok = true, landed = false;
+    int st = 0, it = 0;
+    uint32_t ph = 0;
+    for (int tile = blockIdx.x; tile < tiles && ok; tile += gridDim.x, ++it) {
+      const int buf = p.buffers == 2 ? it & 1 : 0, turn = p.buffers == 2 ? it >> 1 : it;
+      if (turn > 0) ok = __all_sync(0xffffffffu, mbar_wait(&sm.acc_empty[buf], (turn - 1) & 1, abort_flag));
+      if (!ok) break;
+      tc_fence_after_sync();
+      for (int sum = 0; sum < p.sums && ok; ++sum) {
+        const uint32_t acc = tmem + (buf * p.sums + sum) * p.cols;
+        const int kb0 = k_blocks * sum / p.sums, kb1 = k_blocks * (sum + 1) / p.sums;
+        for (int kb = kb0; kb < kb1; ++kb) {
+          ok = __all_sync(0xffffffffu, landed || mbar_wait(&sm.full[st], ph, abort_flag));
+          if (!ok) break;
+          tc_fence_after_sync();
+          const int next = st + 1 == p.stages ? 0 : st + 1;
+          const uint32_t next_ph = st + 1 == p.stages ? ph ^ 1 : ph;
+          landed = mbar_test_wait(&sm.full[next], next_ph);
+          const uint64_t a = a0 + static_cast<uint64_t>(st) * (stage_size >> 4), b = b0 + static_cast<uint64_t>(st) * (stage_size >> 4);
+          if (elect_one()) {
+#pragma unroll
+            for (int kk = 0; kk < kGemmBK / 16; ++kk) umma_ss(acc, a + 2 * kk, b + 2 * kk, idesc, (kb != kb0 || kk != 0) ? 1u : 0u);
+            umma_commit(&sm.empty[st]);
+            if (kb == k_blocks - 1) umma_commit(&sm.acc_full[buf]);
+          }
+          st = next;
+          ph = next_ph;
+        }
+      }
+    }
+    if (!ok && lane == 0 && atomicExch(const_cast<uint32_t*>(abort_flag), 1u) == 0) atomicOr(p.l.status, kStatusHeadWait);
+    if (__any_sync(0xffffffffu, *abort_flag != 0)) {  // no product may be running when tensor memory is freed
+      uint32_t no_abort = 0;
+      if (elect_one()) umma_commit(&sm.drain);
+      mbar_wait(&sm.drain, 0, &no_abort);
+    }
+    __syncwarp();
+  } else {
+    // ======================= epilogue warps ==========================================================
+    const int quarter = warp & 3, part = (warp - 2) >> 2;  // rows of w; every second 32 rows of x
+    const uint32_t lane_addr = static_cast<uint32_t>(quarter * 32) << 16;
+    float(*const turned)[33] = sm.turned[warp - 2];
+    const int row = part * 32 + lane, src = row < rows ? __ldg(p.l.idx + row) : -1;
+    const int* const ids = p.l.ids + static_cast<int64_t>(src) * p.l.top;
+    bool ok = true;
+    int it = 0;
+    for (int tile = blockIdx.x; tile < tiles; tile += gridDim.x, ++it) {
+      const int buf = p.buffers == 2 ? it & 1 : 0, turn = p.buffers == 2 ? it >> 1 : it;
+      const int v0 = tile * p.height + quarter * 32, v1 = min(min(v0 + 32, (tile + 1) * p.height), p.l.vocab);  // this warp's rows of w
+      int pos = 0, next = kNoEntry;  // the row's first entry from v0 on, searched for before the wait
+      if (src >= 0) {
+        for (int width = p.l.top > 1 ? 1 << (31 - __clz(p.l.top)) : 0; width > 0; width >>= 1)
+          if (pos + width <= p.l.top && __ldg(ids + pos + width - 1) < v0) pos += width;
+        if (pos < p.l.top) next = __ldg(ids + pos);
+        if (next < v0) next = kNoEntry;
+      }
+      if (!__all_sync(0xffffffffu, mbar_wait(&sm.acc_full[buf], turn & 1, abort_flag))) {
+        ok = false;
+        break;
+      }
+      tc_fence_after_sync();
+      if (part * 32 < rows) {
+        const uint32_t acc = tmem + lane_addr + buf * p.sums * p.cols + part * 32;
+        float v[32];
+        tmem_ld_x32(acc, reinterpret_cast<uint32_t*>(v));
+        for (int sum = 1; sum < p.sums; ++sum) {
+          float more[32];
+          tmem_ld_x32(acc + sum * p.cols, reinterpret_cast<uint32_t*>(more));
+#pragma unroll
+          for (int j = 0; j < 32; ++j) v[j] += more[j];
+        }
+#pragma unroll
+        for (int j = 0; j < 32; ++j) turned[j][lane] = v[j];
+        __syncwarp();
+        const float* const mine = turned[lane];
+        const int n = v1 - v0;
+        float m = -INFINITY, s = 0.f;
+#pragma unroll
+        for (int j = 0; j < 32; ++j) {
+          v[j] = j < n ? mine[j] : -INFINITY;
+          m = fmaxf(m, v[j]);
+        }
+        m *= p.l.log2_scale;
+        const float from = m == -INFINITY ? 0.f : m;
+#pragma unroll
+        for (int j = 0; j < 32; ++j) s += head_ex2(fmaf(v[j], p.l.log2_scale, -from));
+        while (next < v1) {
+          p.l.picks[static_cast<int64_t>(src) * p.l.top + pos] = mine[next - v0];
+          next = ++pos < p.l.top ? __ldg(ids + pos) : kNoEntry;
+        }
+        if (src >= 0) p.l.parts[(tile * 4 + quarter) * p.l.parts_stride + row] = make_float2(m, n > 0 ? s : 0.f);
+      }
+      tc_fence_before_sync();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&sm.acc_empty[buf]);
+    }
+    if (!ok && lane == 0 && atomicExch(const_cast<uint32_t*>(abort_flag), 1u) == 0) atomicOr(p.l.status, kStatusHeadWait);
+    __syncwarp();
+  }
+  tc_fence_before_sync();
+  __syncthreads();
+  if (warp == 1) {
+    tc_fence_after_sync();
+    tmem_dealloc(tmem, 512);
+  }
+}
+
 // ---- sums: dx and dw of a piece ------------------------------------------------------------------------------------------------------
 // What the sums are multiplied by: everything that is the same for all rows.
 struct HeadScale {
@@ -705,6 +922,13 @@ head_stats_kernel(const __grid_constant__ CUtensorMap x, const __grid_constant__
   extern __shared__ uint8_t smem_raw[];
   HeadLogitsJob<T, false> job(p, &x, &x_copy, &w, nullptr);
   head_products(job, *reinterpret_cast<HeadSmem*>(smem_align_1024(smem_raw)), p.status);
+}
+
+template <typename T>
+__global__ void __launch_bounds__(kFewThreads, 1)
+head_few_kernel(const __grid_constant__ CUtensorMap x, const __grid_constant__ CUtensorMap x_copy, const __grid_constant__ CUtensorMap w, const __grid_constant__ HeadFewParams p) {
+  extern __shared__ uint8_t smem_raw[];
+  head_few<T>(&x, &x_copy, &w, p, smem_align_1024(smem_raw));
 }
 
 template <typename T>

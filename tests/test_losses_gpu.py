@@ -86,6 +86,7 @@ def check(r: oracle.Head, x: torch.Tensor, w: torch.Tensor, tau: float, loss: to
 SHAPES = [
     # rows, vocabulary, dim
     (1, 1, 8), (1, 10, 64), (2, 300, 40), (63, 129, 64), (64, 64, 128), (65, 1000, 136), (255, 257, 264), (256, 256, 256), (257, 2049, 520), (300, 5003, 768), (520, 777, 1032), (130, 20011, 72),
+    (17, 4000, 4104), (100, 700, 2056), (250, 300, 2056), (300, 600, 2056), (16, 5000, 1096),
 ]  # fmt: skip
 
 

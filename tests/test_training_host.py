@@ -237,16 +237,37 @@ def test_losses_refuse() -> None:
         ff.linear_cross_entropy(torch.autograd.forward_ad.make_dual(x, x), w, y)
 
 
-def test_the_pipeline_of_the_losses_holds_its_tensor_memory() -> None:
-    """What all three kernels of products run on: tensor memory is held before the next kernel may start, products end before it is freed, and the
-    leader waits for the other CTA's last signals. (Read, not run: nothing makes a wait run out on a healthy GPU.)"""
-    text = (ROOT / "fastforks_b200" / "csrc" / "head_sm100.cuh").read_text()
-    body = text[text.index("void head_products(") : text.index("// The map of tiles")]
-    assert text.count("tmem_alloc_pair(") == text.count("tmem_dealloc_pair(") == 1
-    assert body.index("tmem_alloc_pair(") < body.index("grid_launch_dependents();")
-    drained, freed = body.index("umma_commit_pair(&sm.drain)"), body.index("tmem_dealloc_pair(")
+HEAD = (ROOT / "fastforks_b200" / "csrc" / "head_sm100.cuh").read_text()
+
+
+@pytest.mark.parametrize(("name", "end", "pair"), [("head_products", "// The map of tiles", "_pair"), ("head_few", "// ---- sums: dx and dw", "")])
+def test_the_pipelines_of_the_losses_hold_their_tensor_memory(name: str, end: str, pair: str) -> None:
+    """What the kernels of products run on: tensor memory is held before the next kernel may start, products end before it is freed. (Read, not run:
+    nothing makes a wait run out on a healthy GPU.)"""
+    body = HEAD[HEAD.index(f"void {name}(") : HEAD.index(end)]
+    assert body.count(f"tmem_alloc{pair}(") == body.count(f"tmem_dealloc{pair}(") == 1
+    assert body.index(f"tmem_alloc{pair}(") < body.index("grid_launch_dependents();")
+    drained, freed = body.index(f"umma_commit{pair}(&sm.drain)"), body.index(f"tmem_dealloc{pair}(")
     assert drained < body.index("mbar_wait(&sm.drain", drained) < freed
-    signals = body.index("mbar_wait(&sm.acc_empty[lane]")
-    assert signals < freed
-    kernels = re.findall(r"__global__ [^{]*?(head_\w+_kernel)\(", text)
-    assert [k for k in kernels if "head_products(" in text[text.index(f"{k}(const") : text.index("\n}", text.index(f"{k}(const"))]] == ["head_stats_kernel", "head_grads_kernel", "head_sums_kernel"]
+    landed = body.index("for (int j = (g > ")  # copies in flight when a loader gives up
+    assert landed < body.index("mbar_wait(&sm.full[j %", landed) < freed
+
+
+def test_a_pair_of_ctas_waits_for_the_last_signals_of_the_other() -> None:
+    body = HEAD[HEAD.index("void head_products(") : HEAD.index("// The map of tiles")]
+    assert body.index("mbar_wait(&sm.acc_empty[lane]") < body.index("tmem_dealloc_pair(")
+
+
+def test_the_kernels_of_products_by_name() -> None:
+    kernels = re.findall(r"__global__ [^{]*?(head_\w+_kernel)\(", HEAD)
+    on = {k: re.findall(r"head_products\(|head_few<", HEAD[HEAD.index(f"{k}(const") : HEAD.index("\n}", HEAD.index(f"{k}(const"))]) for k in kernels}
+    assert {k: v[0] for k, v in on.items() if v} == {
+        "head_stats_kernel": "head_products(", "head_few_kernel": "head_few<", "head_grads_kernel": "head_products(", "head_sums_kernel": "head_products(",
+    }  # fmt: skip
+
+
+def test_rows_on_their_way_land_before_a_layer_norm_that_gives_up_ends() -> None:
+    text = (ROOT / "fastforks_b200" / "csrc" / "layer_norm_sm100.cuh").read_text()
+    body = text[text.index("norm_ring_grad_kernel(const") :]
+    assert body.index("ring.drain(&sm.abort);") < body.index("joined")
+    assert "mbar_wait(&full[i]" in text[text.index("void drain(") : text.index("__device__ __forceinline__ LnRing ln_ring(")]
