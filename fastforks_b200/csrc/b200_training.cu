@@ -26,26 +26,44 @@ template <typename T, int VEC, int N, int THREADS>
 NormForm forward_form() { return {reinterpret_cast<const void*>(norm_rows_kernel<T, VEC, N, THREADS>), THREADS, N, VEC}; }
 template <typename T>
 const NormForm* forward_forms(bool wide_rows, int* count) {
-  constexpr int V = 16 / sizeof(T);
-  static const NormForm vectors[] = {forward_form<T, V, 1, 32>(), forward_form<T, V, 2, 32>(), forward_form<T, V, 3, 32>(), forward_form<T, V, 4, 32>(),
-                                     forward_form<T, V, 2, 128>(), forward_form<T, V, 3, 128>(), forward_form<T, V, 4, 128>(), forward_form<T, V, 3, 256>(), forward_form<T, V, 4, 256>(),
-                                     forward_form<T, V, 4, 512>(), forward_form<T, V, 4, 1024>(), forward_form<T, V, 8, 1024>()};
   static const NormForm values[] = {forward_form<T, 1, 1, 32>(), forward_form<T, 1, 4, 32>(), forward_form<T, 1, 8, 32>(), forward_form<T, 1, 4, 256>(), forward_form<T, 1, 8, 256>(),
                                     forward_form<T, 1, 16, 256>(), forward_form<T, 1, 16, 1024>(), forward_form<T, 1, 32, 1024>()};
-  *count = wide_rows ? (sizeof(T) == 2 ? 11 : 12) : 8;
-  return wide_rows ? vectors : values;
+  if (!wide_rows) {
+    *count = 8;
+    return values;
+  }
+  if constexpr (sizeof(T) == 2) {
+    static const NormForm vectors[] = {forward_form<T, 8, 1, 32>(), forward_form<T, 8, 2, 32>(), forward_form<T, 8, 3, 32>(), forward_form<T, 8, 4, 32>(), forward_form<T, 8, 2, 128>(),
+                                       forward_form<T, 8, 4, 128>(), forward_form<T, 8, 3, 256>(), forward_form<T, 8, 4, 256>(), forward_form<T, 8, 4, 512>(), forward_form<T, 8, 4, 1024>()};
+    *count = 10;
+    return vectors;
+  } else {
+    static const NormForm vectors[] = {forward_form<T, 4, 1, 32>(), forward_form<T, 4, 2, 32>(), forward_form<T, 4, 3, 32>(), forward_form<T, 4, 4, 32>(), forward_form<T, 4, 2, 128>(),
+                                       forward_form<T, 4, 3, 128>(), forward_form<T, 4, 4, 128>(), forward_form<T, 4, 4, 256>(), forward_form<T, 4, 4, 512>(), forward_form<T, 4, 4, 1024>(), forward_form<T, 4, 8, 1024>()};
+    *count = 11;
+    return vectors;
+  }
 }
 // The gradients of rows that do not go through shared memory: too wide for it, or not on 16 bytes.
 template <typename T, int VEC, int N, int THREADS>
 NormForm grad_form() { return {reinterpret_cast<const void*>(norm_rows_grad_kernel<T, VEC, N, THREADS>), THREADS, N, VEC}; }
 template <typename T>
 const NormForm* grad_forms(bool wide_rows, int* count) {
-  constexpr int V = 16 / sizeof(T), M = 16 / V;
-  static const NormForm vectors[] = {grad_form<T, V, M, 512>(), grad_form<T, V, M, 1024>(), grad_form<T, V, 2 * M, 1024>()};
   static const NormForm values[] = {grad_form<T, 1, 1, 32>(), grad_form<T, 1, 4, 32>(), grad_form<T, 1, 8, 32>(), grad_form<T, 1, 8, 128>(), grad_form<T, 1, 16, 128>(),
                                     grad_form<T, 1, 16, 256>(), grad_form<T, 1, 16, 512>(), grad_form<T, 1, 16, 1024>(), grad_form<T, 1, 32, 1024>()};
-  *count = wide_rows ? 3 : 9;
-  return wide_rows ? vectors : values;
+  if (!wide_rows) {
+    *count = 9;
+    return values;
+  }
+  if constexpr (sizeof(T) == 2) {
+    static const NormForm vectors[] = {grad_form<T, 8, 2, 1024>(), grad_form<T, 8, 4, 1024>()};
+    *count = 2;
+    return vectors;
+  } else {
+    static const NormForm vectors[] = {grad_form<T, 4, 4, 512>(), grad_form<T, 4, 4, 1024>(), grad_form<T, 4, 8, 1024>()};
+    *count = 3;
+    return vectors;
+  }
 }
 NormForm norm_form(const B200LayerNormArgs& a, bool grad, bool wide_rows) {
   int n = 0;
@@ -65,7 +83,7 @@ struct RingForm {
 };
 template <typename T, int N, int G>
 RingForm ring_form() { return {reinterpret_cast<const void*>(norm_ring_grad_kernel<T, 16 / sizeof(T), N, G>), G, N}; }
-constexpr int kMostRingForms = 10;
+constexpr int kMostRingForms = 9;
 template <typename T>
 const RingForm* ring_forms(int* count) {
   if constexpr (sizeof(T) == 2) {
@@ -73,8 +91,8 @@ const RingForm* ring_forms(int* count) {
     *count = 7;
     return forms;
   } else {
-    static const RingForm forms[] = {ring_form<T, 1, 1>(), ring_form<T, 2, 1>(), ring_form<T, 3, 1>(), ring_form<T, 4, 1>(), ring_form<T, 3, 2>(), ring_form<T, 4, 2>(), ring_form<T, 3, 4>(), ring_form<T, 4, 4>(), ring_form<T, 3, 8>(), ring_form<T, 4, 8>()};
-    *count = 10;
+    static const RingForm forms[] = {ring_form<T, 1, 1>(), ring_form<T, 2, 1>(), ring_form<T, 3, 1>(), ring_form<T, 4, 1>(), ring_form<T, 3, 2>(), ring_form<T, 4, 2>(), ring_form<T, 3, 4>(), ring_form<T, 4, 4>(), ring_form<T, 4, 8>()};
+    *count = 9;
     return forms;
   }
 }
@@ -82,7 +100,7 @@ const RingForm* ring_forms(int* count) {
 // The form of a call, or no kernel: rows that are no whole 16-byte words, or too wide.
 struct RingPlan {
   RingForm form{nullptr, 0, 0};
-  int index = 0, slots = 0, ctas = 0, smem = 0;
+  int index = 0, slots = 0, ctas = 0, threads = 0, smem = 0;
 };
 RingPlan ring_plan(const B200LayerNormArgs& a, bool wide_rows, int sms) {
   RingPlan r;
@@ -93,12 +111,12 @@ RingPlan ring_plan(const B200LayerNormArgs& a, bool wide_rows, int sms) {
   int i = 0;
   while (i < n && f[i].warps * f[i].vectors * 32 * values < a.dim) ++i;
   if (i == n) return r;
-  const int groups = kLnWarps / f[i].warps, slot = 2 * f[i].warps * f[i].vectors * 512;  // (a vector of 32 lanes: 512 bytes)
-  const int per_sm = ln_ring_ctas(f[i].vectors * values);
+  r.threads = 32 * ln_ring_warps(f[i].vectors * values);
+  const int groups = r.threads / 32 / f[i].warps, slot = 2 * f[i].warps * f[i].vectors * 512;  // (a vector of 32 lanes: 512 bytes)
   r.form = f[i];
   r.index = (a.dtype == B200_ATTN_F16 ? 0 : a.dtype == B200_ATTN_BF16 ? 1 : 2) * kMostRingForms + i;
-  r.slots = std::min(kLnMostSlots, ln_ring_bytes(per_sm) / (groups * slot));
-  r.ctas = static_cast<int>(std::min<int64_t>((a.rows + groups - 1) / groups, static_cast<int64_t>(per_sm) * sms));
+  r.slots = std::min(kLnMostSlots, kLnRingBytes / (groups * slot));
+  r.ctas = static_cast<int>(std::min<int64_t>((a.rows + groups - 1) / groups, static_cast<int64_t>(sms)));
   r.smem = r.slots * groups * slot;
   return r;
 }
@@ -644,8 +662,8 @@ int b200_layer_norm_grad(const B200LayerNormArgs* a, void* stream_ptr) {
   if (through) {
     p.slots = ring.slots;
     p.status = dev->status;
-    if (int rc = opt_in(ring.form.kernel, kHeadForms + ring.index, ln_ring_bytes(1))) return rc;
-    if (int rc = launch_kernel(ring.form.kernel, static_cast<unsigned>(ctas), 1, 32 * kLnWarps, ring.smem, 1, stream, args, "layer_norm_grad kernel launch")) return rc;
+    if (int rc = opt_in(ring.form.kernel, kHeadForms + ring.index, kLnRingBytes)) return rc;
+    if (int rc = launch_kernel(ring.form.kernel, static_cast<unsigned>(ctas), 1, static_cast<unsigned>(ring.threads), ring.smem, 1, stream, args, "layer_norm_grad kernel launch")) return rc;
   } else if (int rc = launch_kernel(f.kernel, static_cast<unsigned>(ctas), 1, f.threads == 32 ? 32 * kLnGradWarps : f.threads, f.threads == 32 ? 8 * static_cast<size_t>(a->dim) : 0, 1, stream, args, "layer_norm_grad kernel launch")) {
     return rc;
   }

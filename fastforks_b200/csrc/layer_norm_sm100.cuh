@@ -376,22 +376,22 @@ __global__ void __launch_bounds__(THREADS == 32 ? 32 * kLnGradWarps : THREADS) n
 
 // ---- gradients, rows through shared memory -----------------------------------------------------------------------------------------------
 // Sums behind dw and db want the CTAs to stay, and then what HBM needs in flight does not fit beside a row in registers. G warps share a row, and every
-// such group has a ring of rows that one of its lanes fills with bulk copies (cp.async.bulk, 16-byte addresses and sizes), up to 200 KB an
+// such group has a ring of rows that one of its lanes fills with bulk copies (cp.async.bulk, 16-byte addresses and sizes), some 200 KB an
 // SM. A slot is filled again as soon as the group has it in registers. Slots are as wide as G warps of N vectors, with zeros behind the row, so that
 // no value is tested for being one; weights stay in registers as fp32 pairs (with a test and a conversion at each use a value took 29
 // instructions, and 8192 rows of 4096 54 us). us with the join, of bf16: a row a CTA with the next one in registers (norm_rows_grad_kernel) -> here, and
-// the time of the bytes: 8192 x 4096 75.0 -> 41.5 (30.8), 21920 x 1024 48.4 -> 32.8 (20.6), 30000 x 512 64.4 -> 22.6 (14.1); 5480 x 384 in fp32
-// 14.5 -> 11.0 (3.9). Bound by HBM and, at sixteen warps an SM, by the chain of copy, sums and barrier of each row. The same for the forward pass was
-// slower than rows in registers (8192 x 4096 29.2, 24.3 there): two barriers a row, and nothing that has to stay.
-constexpr int kLnWarps = 8, kLnMostSlots = 16;
+// the time of the bytes: 8192 x 4096 75.0 -> 40.9 (30.8), 21920 x 1024 48.4 -> 30.8 (20.6), 30000 x 512 64.4 -> 20.5 (14.1), 300 x 4096 18.3 -> 7.8; fp32
+// 8192 x 4096 74.3 -> 67.7 (61.6), 5480 x 384 14.5 -> 8.9 (3.9). Bound by HBM at its mix of reads and writes and, at sixteen warps an SM, by the chain of
+// copy, sums and barrier of each row. The same for the forward pass was slower than rows in registers (8192 x 4096 29.2, 24.3 there): two barriers a
+// row, and nothing that has to stay. (Groups added one after the other into one place took 5 us more at 16 groups.)
+constexpr int kLnMostWarps = 16, kLnMostSlots = 16, kLnRingBytes = 208 * 1024;
 constexpr uint32_t kStatusNormWait = 1u << 24;
-// CTAs an SM holds, as their registers allow, and the ring of each.
-constexpr int ln_ring_ctas(int values) { return values <= 16 ? 2 : 1; }
-constexpr int ln_ring_bytes(int ctas) { return ctas == 2 ? 104 * 1024 : 208 * 1024; }
+// Warps of a CTA, one on each SM, as the registers of so many values a thread allow. (Two CTAs of eight warps leave twice as many parts to join.)
+constexpr int ln_ring_warps(int values) { return values <= 16 ? 16 : 8; }
 
 struct LnRingSmem {
-  uint64_t full[kLnWarps][kLnMostSlots];
-  alignas(16) float2 place[kLnWarps][2][kLnWarps];  // of each group, alternately: its warps' sums
+  uint64_t full[kLnMostWarps][kLnMostSlots];
+  alignas(16) float2 place[kLnMostWarps][2][8];  // of each group, alternately: its warps' sums
   uint32_t abort;
 };
 
@@ -478,7 +478,7 @@ struct LnRing {
 
 template <typename T, int VEC, int N, int G>
 __device__ __forceinline__ LnRing ln_ring(LnRingSmem& sm, uint8_t* memory, const LayerNormParams& p) {
-  constexpr int kGroups = kLnWarps / G;
+  constexpr int kWarps = ln_ring_warps(N * VEC), kGroups = kWarps / G;
   const int group = (threadIdx.x >> 5) / G;
   LnRing r;
   r.bytes = static_cast<uint32_t>(p.dim * sizeof(T));
@@ -505,7 +505,7 @@ __device__ __forceinline__ LnRing ln_ring(LnRingSmem& sm, uint8_t* memory, const
   const uint32_t tail = r.row_bytes - r.bytes;  // a multiple of 16, as both are
   if (tail > 0) {
     const int words = static_cast<int>(tail >> 4), places = 2 * kGroups * p.slots;
-    for (int i = threadIdx.x; i < places * words; i += 32 * kLnWarps) {
+    for (int i = threadIdx.x; i < places * words; i += 32 * kWarps) {
       const int at = i / words;
       st_shared_v4(smem_u32(memory) + at * r.row_bytes + r.bytes + (i - at * words) * 16, make_uint4(0, 0, 0, 0));
     }
@@ -516,10 +516,10 @@ __device__ __forceinline__ LnRing ln_ring(LnRingSmem& sm, uint8_t* memory, const
 
 // Gradients: one pass for the sums, dw and db, one barrier, dx from registers.
 template <typename T, int VEC, int N, int G>
-__global__ void __launch_bounds__(32 * kLnWarps, ln_ring_ctas(N * VEC)) norm_ring_grad_kernel(const LayerNormParams p) {
+__global__ void __launch_bounds__(32 * ln_ring_warps(N * VEC), 1) norm_ring_grad_kernel(const LayerNormParams p) {
   extern __shared__ __align__(128) uint8_t ln_memory[];
   __shared__ LnRingSmem sm;
-  constexpr int kStep = G * 32 * VEC, kGroups = kLnWarps / G, kPairs = VEC / 2;
+  constexpr int kStep = G * 32 * VEC, kWarps = ln_ring_warps(N * VEC), kGroups = kWarps / G, kPairs = VEC / 2;
   const int group = (threadIdx.x >> 5) / G, at = (threadIdx.x % (G * 32)) * VEC;
   LnRing ring = ln_ring<T, VEC, N, G>(sm, ln_memory, p);
   grid_dependency_wait();
@@ -572,27 +572,33 @@ __global__ void __launch_bounds__(32 * kLnWarps, ln_ring_ctas(N * VEC)) norm_rin
   }
   ring.drain(&sm.abort);
   if (!p.want_dw) return;
-  // The groups' parts, added in the order of the groups in what was the ring: every copy has landed, every slot has been read.
+  // The groups' parts side by side in what was the ring (every copy has landed; every slot has been read), then added in the order of the groups.
   float* const out = p.partial + static_cast<int64_t>(blockIdx.x) * 2 * p.dim;
-  float* const joined = reinterpret_cast<float*>(ln_memory);
   if constexpr (kGroups > 1) {
-    for (int turn_of = 0; turn_of < kGroups; ++turn_of) {
-      __syncthreads();
-      if (group != turn_of) continue;
+    float* const joined = reinterpret_cast<float*>(ln_memory);
+    __syncthreads();
+    float* const mine = joined + static_cast<size_t>(group) * 2 * p.dim + at;
 #pragma unroll
-      for (int i = 0; i < N; ++i) {
-        if (at + i * kStep >= p.dim) continue;
+    for (int i = 0; i < N; ++i) {
+      if (at + i * kStep >= p.dim) continue;
 #pragma unroll
-        for (int j = 0; j < kPairs; ++j) {
-          float2* const to_w = reinterpret_cast<float2*>(joined + at + i * kStep) + j;
-          float2* const to_b = reinterpret_cast<float2*>(joined + p.dim + at + i * kStep) + j;
-          *to_w = turn_of == 0 ? dw[i][j] : fadd2(*to_w, dw[i][j]);
-          *to_b = turn_of == 0 ? db[i][j] : fadd2(*to_b, db[i][j]);
-        }
+      for (int j = 0; j < kPairs; j += 2) {
+        *reinterpret_cast<float4*>(mine + i * kStep + 2 * j) = make_float4(dw[i][j].x, dw[i][j].y, dw[i][j + 1].x, dw[i][j + 1].y);
+        *reinterpret_cast<float4*>(mine + p.dim + i * kStep + 2 * j) = make_float4(db[i][j].x, db[i][j].y, db[i][j + 1].x, db[i][j + 1].y);
       }
     }
     __syncthreads();
-    for (int c = threadIdx.x; c < p.dim / 2; c += 32 * kLnWarps) reinterpret_cast<float4*>(out)[c] = reinterpret_cast<const float4*>(joined)[c];
+    for (int c = threadIdx.x; c < p.dim / 2; c += 32 * kWarps) {
+      float4 sum = reinterpret_cast<const float4*>(joined)[c];
+      for (int g = 1; g < kGroups; ++g) {
+        const float4 more = reinterpret_cast<const float4*>(joined + static_cast<size_t>(g) * 2 * p.dim)[c];
+        sum.x += more.x;
+        sum.y += more.y;
+        sum.z += more.z;
+        sum.w += more.w;
+      }
+      reinterpret_cast<float4*>(out)[c] = sum;
+    }
   } else {
 #pragma unroll
     for (int i = 0; i < N; ++i)

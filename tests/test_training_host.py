@@ -269,5 +269,5 @@ def test_the_kernels_of_products_by_name() -> None:
 def test_rows_on_their_way_land_before_a_layer_norm_that_gives_up_ends() -> None:
     text = (ROOT / "fastforks_b200" / "csrc" / "layer_norm_sm100.cuh").read_text()
     body = text[text.index("norm_ring_grad_kernel(const") :]
-    assert body.index("ring.drain(&sm.abort);") < body.index("joined")
+    assert body.index("ring.drain(&sm.abort);") < body.index("joined = ")
     assert "mbar_wait(&full[i]" in text[text.index("void drain(") : text.index("__device__ __forceinline__ LnRing ln_ring(")]
