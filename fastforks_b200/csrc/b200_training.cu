@@ -236,8 +236,10 @@ struct FewPlan {
 FewPlan few_plan(const B200HeadArgs& a, int sms) {
   FewPlan f{};
   const int64_t n = up(a.rows, 16), cols = up(a.rows, 32);
-  const int k_blocks = (a.dim + kGemmBK - 1) / kGemmBK, sums = (k_blocks + kHeadSumBlocks - 1) / kHeadSumBlocks;
-  if (n > kFewRows || cols * sums > 512) return f;
+  // As many accumulators of a tile as tensor memory holds, of 256 products or more, and of no more than the pairs take at once: the fewer products, the
+  // less the tensor cores cut off, and a single row's loss has no others to average with (1 x 72 x 2048, 1024 at a time: 2.3e-6 off; 512: 7.7e-7).
+  const int k_blocks = (a.dim + kGemmBK - 1) / kGemmBK, sums = static_cast<int>(std::min<int64_t>((k_blocks + 3) / 4, 512 / cols));
+  if (n > kFewRows || (k_blocks + sums - 1) / sums > kHeadSumBlocks) return f;
   f.n = static_cast<int>(n);
   f.cols = static_cast<int>(cols);
   f.sums = sums;
@@ -275,8 +277,12 @@ HeadLossWork head_loss_work(const B200HeadArgs& a, int sms) {
 // Gradients of logits in 16 bits of as many columns at a time as kPieceBytes holds, or 2048. Each piece costs the fp32 sums of dx once more
 // through L2 and HBM, under the products, and the rounds of two launches that are not full.
 constexpr int64_t kPieceBytes = 256 << 20;
+// Where what the rounding of logits' gradients took is kept and multiplied too: few rows, whose products wait for memory, and products that are small beside
+// the host's side of a call (2^31 multiply-adds more each for dx and dw, some 5 us; a call's forward and backward pass through autograd take 75).
+constexpr int64_t kRestRows = 128, kRestProducts = int64_t(1) << 31;
 struct HeadGradWork {
   int64_t slot_rows;  // rows of G and of a part of dx
+  int64_t g_rows;     // with those of what G's rounding took
   int cols;           // columns of G
   int splits, sums_bn;
   int64_t g, sums, coef, norm, bytes;
@@ -284,7 +290,8 @@ struct HeadGradWork {
 HeadGradWork head_grad_work(const B200HeadArgs& a, bool want_dx, bool want_dw, int pairs) {
   HeadGradWork w{};
   w.slot_rows = up(a.rows, 256);
-  const int64_t most = std::max<int64_t>(2048, kPieceBytes / (2 * w.slot_rows) / 256 * 256);
+  w.g_rows = a.rows <= kRestRows || static_cast<double>(a.rows) * a.dim * a.vocab <= static_cast<double>(kRestProducts) ? 2 * w.slot_rows : w.slot_rows;
+  const int64_t most = std::max<int64_t>(2048, kPieceBytes / (2 * w.g_rows) / 256 * 256);
   const int64_t pieces = (a.vocab + most - 1) / most;
   w.cols = static_cast<int>(up((a.vocab + pieces - 1) / pieces, 256));
   w.sums_bn = a.dim > 128 ? 256 : 128;
@@ -305,7 +312,7 @@ HeadGradWork head_grad_work(const B200HeadArgs& a, bool want_dx, bool want_dw, i
     }
   }
   Layout l;
-  w.g = l.add(w.slot_rows * w.cols * 2);
+  w.g = l.add(w.g_rows * w.cols * 2);
   w.sums = l.add(w.splits * w.slot_rows * a.dim * 4);
   w.coef = l.add(4LL * a.rows);
   w.norm = l.add(4);
@@ -500,9 +507,9 @@ int launch_grad(const B200HeadArgs& a, cudaStream_t stream) {
   if (int rc = head_map(&x_k, a.x, a.dtype, a.rows, a.dim, a.ldx, 64, 128, "x")) return rc;
   if (int rc = head_map(&copy_k, x_copy, a.dtype, up(a.rows, 64), a.dim, a.dim, 64, 128, "x")) return rc;
   if (int rc = head_map(&w_k, a.w, a.dtype, a.vocab, a.dim, a.ldw, 64, bn / 2, "w")) return rc;
-  if (int rc = head_map(&g_out, g, a.dtype, w.slot_rows, w.cols, w.cols, 64, 32, "workspace")) return rc;
-  if (int rc = head_map(&g_k, g, a.dtype, w.slot_rows, w.cols, w.cols, 64, 128, "workspace")) return rc;
-  if (int rc = head_map(&g_mn, g, a.dtype, w.slot_rows, w.cols, w.cols, 64, 64, "workspace")) return rc;
+  if (int rc = head_map(&g_out, g, a.dtype, w.g_rows, w.cols, w.cols, 64, 32, "workspace")) return rc;
+  if (int rc = head_map(&g_k, g, a.dtype, w.g_rows, w.cols, w.cols, 64, 128, "workspace")) return rc;
+  if (int rc = head_map(&g_mn, g, a.dtype, w.g_rows, w.cols, w.cols, 64, 64, "workspace")) return rc;
   if (int rc = head_map(&w_mn, a.w, a.dtype, a.vocab, a.dim, a.ldw, 64, 64, "w")) return rc;
   if (int rc = head_map(&x_mn, a.x, a.dtype, a.rows, a.dim, a.ldx, 64, 64, "x")) return rc;
   if (int rc = head_map(&copy_mn, x_copy, a.dtype, up(a.rows, 64), a.dim, a.dim, 64, 64, "x")) return rc;
@@ -522,6 +529,7 @@ int launch_grad(const B200HeadArgs& a, cudaStream_t stream) {
   HeadLogitsParams p = logits_params(a, s, dev->status);
   p.lse2 = at<float>(a.state, s.lse2);
   p.g_scale = g_scale;
+  p.rest_at = w.g_rows > w.slot_rows ? static_cast<int>(w.slot_rows) : 0;
   p.bn = bn;
   p.stages = ring_stages(bn);
   if (a.reduction == B200_HEAD_NONE) {
@@ -549,6 +557,7 @@ int launch_grad(const B200HeadArgs& a, cudaStream_t stream) {
   q.bn = w.sums_bn;
   q.stages = ring_stages(w.sums_bn);
   q.slot_rows = w.slot_rows;
+  q.rest_at = p.rest_at;
   q.scale = scale;
   q.status = dev->status;
   const int64_t col_tiles = (a.dim + w.sums_bn - 1) / w.sums_bn;

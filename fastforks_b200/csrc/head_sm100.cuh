@@ -68,7 +68,8 @@ struct HeadItem {
 // k-blocks of an accumulator of logits. The tensor cores cut off what of a product lies below the last place of the running sum: over 4096
 // products the loss of 64 rows came out 2.1e-6 off (products and sums in fp32 arithmetic: 3.7e-7). Longer sums are taken 1024 products at a
 // time and added in fp32, which rounds: 4.7e-7. The accumulators alternate as they do between tiles, so the epilogue's additions run under
-// the next products (4096 x 128000 x 4096: 2570 us; one accumulator, as in head_grads_kernel, 2546).
+// the next products (4096 x 128000 x 4096: 2570 us; one accumulator, as in head_grads_kernel, 2546). 512 at a time halve the error once more and cost up to 6 %
+// of a loss with its gradients (4096 x 64000 x 2048, rows that count 3/4: 2330 -> 2469 us), 256 up to 15 %.
 constexpr int kHeadSumBlocks = 16;
 
 // The pipeline of gemm_pair_kernel with the operands' layouts, the list of tiles and the epilogue left to `job`:
@@ -270,12 +271,15 @@ struct HeadLogitsParams {
   const float* lse2;    // [all_rows], in units of ln 2
   const float* coef;    // [all_rows] or null: 1
   float g_scale;        // a power of two
+  int rest_at;          // G's row where what its rounding took is kept, or 0: it is not
   uint32_t* status;
 };
 
 // G = 2^s coef_t (softmax(z_t) - p) is held in 16 bits, the operands' type: its rounding is that of an operand, 2^-9 (fp16 2^-12) of a value on
 // average below half a step, and as large in dx and dw as the rounding of their result. s = 15 for fp16, whose smallest normal
-// number is 2^-14: a softmax of 2^-29 keeps all its bits; bfloat16 has fp32's range, s = 0.
+// number is 2^-14: a softmax of 2^-29 keeps all its bits; bfloat16 has fp32's range, s = 0. Over many rows that adds up to 1.1 to 1.45 times the error that
+// the results' own rounding has; of a few rows each hangs on one or two roundings, and 1.7 times came out. Few rows and small products (head_grad_work in
+// b200_training.cu) therefore keep what the rounding took, in as many rows more, and both go through the products: the error is that of the results' rounding.
 template <typename T, bool GRADS>
 struct HeadLogitsJob {
   const HeadLogitsParams& p;
@@ -459,10 +463,13 @@ struct HeadLogitsJob {
         for (int c = part; c < pieces; c += 2) {
           const int col = t.col0 + c * 64;
           const bool here = col < p.vocab;
-          if (lane == 0) tma_store_wait_read<1>();  // the store that used this buffer last has read it
+          if (lane == 0) {  // the store that used this buffer last has read it
+            if (p.rest_at > 0) tma_store_wait_read<0>();
+            else tma_store_wait_read<1>();
+          }
           __syncwarp();
           if (here) {
-            const uint32_t at_row = stage + buf * kHeadChunkBytes + lane * 128;
+            const uint32_t at_row = stage + buf * kHeadChunkBytes + lane * 128, at_rest = stage + (buf ^ 1) * kHeadChunkBytes + lane * 128;
 #pragma unroll
             for (int half = 0; half < 2; ++half) {
               const int base = col + half * 32;
@@ -497,6 +504,18 @@ struct HeadLogitsJob {
 #pragma unroll
               for (int q = 0; q < 4; ++q)
                 st_shared_v4(at_row + (((4 * half + q) ^ (lane & 7)) << 4), make_uint4(out[4 * q], out[4 * q + 1], out[4 * q + 2], out[4 * q + 3]));
+              if (p.rest_at > 0) {
+#pragma unroll
+                for (int i = 0; i < 16; ++i) {
+                  const float2 y = fmul2(make_float2(v[2 * i], v[2 * i + 1]), coef2), held = gemm_unpack2<T>(out[i]);
+                  // (what is not finite has no rest: it is whole already)
+                  const float2 rest = make_float2(isfinite(held.x) ? y.x - held.x : 0.f, isfinite(held.y) ? y.y - held.y : 0.f);
+                  out[i] = row < job.rows ? gemm_pack2<T>(rest.x, rest.y) : 0u;
+                }
+#pragma unroll
+                for (int q = 0; q < 4; ++q)
+                  st_shared_v4(at_rest + (((4 * half + q) ^ (lane & 7)) << 4), make_uint4(out[4 * q], out[4 * q + 1], out[4 * q + 2], out[4 * q + 3]));
+              }
             }
             fence_proxy_async_smem();
           }
@@ -504,6 +523,7 @@ struct HeadLogitsJob {
           else __syncwarp();
           if (lane == 0) {
             if (here) tma_store_2d(job.g, stage_ptr + buf * kHeadChunkBytes, col - p.v0, t.row0 + row_in);
+            if (here && p.rest_at > 0) tma_store_2d(job.g, stage_ptr + (buf ^ 1) * kHeadChunkBytes, col - p.v0, p.rest_at + t.row0 + row_in);
             tma_store_commit();
           }
           buf ^= 1;
@@ -517,9 +537,9 @@ struct HeadLogitsJob {
 // ---- logits of few rows: statistics ----------------------------------------------------------------------------------------------------
 // Up to 64 rows leave most of a 256 x 256 tile of the pairs empty and its tiles unevenly dealt, where only the weight's way from HBM counts. Here the
 // vocabulary is the M side: a CTA takes `height` rows of w, at most 128 and such that every SM gets the same number of tiles, against all rows of x (N, a
-// multiple of 16). Sums of more than 1024 products go to accumulators of their own, side by side in tensor memory. A warp of the epilogue has 32 rows
+// multiple of 16). Sums of products go to several accumulators side by side in tensor memory (few_plan in b200_training.cu). A warp of the epilogue has 32 rows
 // of w; it turns 32 x 32 logits through shared memory, after which a lane has a row of x. us of a loss, by pairs -> here: 1 x 32000 x 4096 79.6 -> 56.9 (the
-// weight alone 40.1), 16 rows 61.9 -> 55.3, 64 rows 64.7 -> 61.1, 64 x 128000 x 4096 206 -> 190 (160), 1 x 1000 x 768 13.4 -> 12.0; but of 128 rows 62.9 and
+// weight alone 40.1), 16 rows 61.9 -> 55.3, 64 rows 64.7 -> 61.1, 64 x 128000 x 4096 206 -> 190 (160), 1 x 1000 x 768 13.4 -> 12.2; but of 128 rows 62.9 and
 // 64.9, of 256 x 32000 x 2048 38.5 and 52.1: every CTA reads all of x. Bound by HBM behind a ramp: 77 % of its peak over 1 GB, 63 % over 262 MB.
 struct HeadFewParams {
   HeadLogitsParams l;    // (v0, tiles_n, bn, stages, group are not looked at)
@@ -754,6 +774,7 @@ struct HeadSumsParams {
   int want_dw;
   int bn, stages;
   int first;          // the first piece: dx begins
+  int rest_at;        // see HeadLogitsParams
   int64_t slot_rows;  // rows of a part's sums, a multiple of 256
   HeadScale scale;
   uint32_t* status;
@@ -771,10 +792,11 @@ struct HeadSumsJob {
   const HeadSumsParams& p;
   const CUtensorMap *g_k, *g_mn, *w, *x, *x_copy, *dx, *dw;
   int rows, row_tiles, col_tiles, v_tiles, dx_items, pairs;
+  int twice;  // 2: k goes over G and then over what its rounding took
 
   __device__ __forceinline__ HeadSumsJob(const HeadSumsParams& p_, const CUtensorMap* gk, const CUtensorMap* gm, const CUtensorMap* w_, const CUtensorMap* x_,
                                          const CUtensorMap* xc, const CUtensorMap* dx_, const CUtensorMap* dw_)
-      : p(p_), g_k(gk), g_mn(gm), w(w_), x(x_), x_copy(xc), dx(dx_), dw(dw_) {}
+      : p(p_), g_k(gk), g_mn(gm), w(w_), x(x_), x_copy(xc), dx(dx_), dw(dw_), twice(p_.rest_at > 0 ? 2 : 1) {}
   __device__ __forceinline__ void begin() {
     rows = __ldg(p.count);
     if (rows < p.all_rows) x = x_copy;
@@ -807,7 +829,7 @@ struct HeadSumsJob {
       const int at = pair + i * pairs, tiles = row_tiles * col_tiles, slot = at / tiles;
       int tm, tn;
       head_raster(at - slot * tiles, row_tiles, col_tiles, min(8, row_tiles), &tm, &tn);
-      const int kbs = (p.cols + 63) / 64;
+      const int kbs = (p.cols + 63) / 64 * twice;
       return {0, slot, tm * 256, tn * p.bn, static_cast<int>(static_cast<int64_t>(kbs) * slot / p.splits), static_cast<int>(static_cast<int64_t>(kbs) * (slot + 1) / p.splits)};
     }
     i -= long_ones;
@@ -819,18 +841,20 @@ struct HeadSumsJob {
     const int at = i < my_early ? mine + i * behind : early + pair + (i - my_early) * pairs;
     int tm, tn;
     head_raster(at, v_tiles, col_tiles, min(8, v_tiles), &tm, &tn);
-    return {1, 0, tm * 256, tn * p.bn, 0, max(1, (rows + 63) / 64)};  // (no row counts: a product all the same, of whatever is there, and zeros stored)
+    return {1, 0, tm * 256, tn * p.bn, 0, max(1, (rows + 63) / 64) * twice};  // (no row counts: a product all the same, of whatever is there, and zeros stored)
   }
   __device__ __forceinline__ int stages() const { return p.stages; }
   __device__ __forceinline__ uint32_t stage_bytes() const { return kGemmTileBytes + static_cast<uint32_t>(p.bn) * kGemmBK; }
   __device__ __forceinline__ uint32_t bytes(const HeadItem&) const { return 2u * stage_bytes(); }
   __device__ __forceinline__ void load(const HeadItem& t, int kb, int rank, uint8_t* at, uint32_t bar) const {
-    const int k = kb * kGemmBK, half = p.bn >> 1;
+    const int half = p.bn >> 1, once = t.kind == 0 ? (p.cols + 63) / 64 : max(1, (rows + 63) / 64);
+    const bool rest = kb >= once;
+    const int k = (rest ? kb - once : kb) * kGemmBK, g_row = rest ? p.rest_at : 0;
     if (t.kind == 0) {
-      tma_load_2d_pair(at, g_k, bar, k, t.row0 + rank * 128);
+      tma_load_2d_pair(at, g_k, bar, k, g_row + t.row0 + rank * 128);
     } else {
-      tma_load_2d_pair(at, g_mn, bar, t.row0 + rank * 128, k);
-      tma_load_2d_pair(at + kHeadBlock, g_mn, bar, t.row0 + rank * 128 + 64, k);
+      tma_load_2d_pair(at, g_mn, bar, t.row0 + rank * 128, g_row + k);
+      tma_load_2d_pair(at + kHeadBlock, g_mn, bar, t.row0 + rank * 128 + 64, g_row + k);
     }
     const CUtensorMap* b = t.kind == 0 ? w : x;
     const int b_k = t.kind == 0 ? p.v0 + k : k;
