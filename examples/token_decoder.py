@@ -1,11 +1,12 @@
-"""A small token decoder on the framework's operators: a prompt in pieces, then token by token from a captured graph, and a gradient step.
+"""A small token decoder on the framework's operators: a prompt in pieces, then token by token from a captured graph, and gradient steps.
 
     python examples/token_decoder.py [--layers 2] [--batch 4] [--prompt 100] [--steps 16]
 
 Each layer is `gemm` (qkv), positions, the 4-bit cache, attention over it and `gemm` again; its queries and keys are normed
 (`qk_norm_rotary`) in every other layer and only turned on their way into the cache (`kv4_append_`) in the rest. Weights are random: what
-is shown is how the calls go together, and that pieces, single tokens and a replayed graph agree. The last part takes a step of gradient descent on
-the norms' weights through `qk_norm_rotary` and `rotary`.
+is shown is how the calls go together, and that pieces, single tokens and a replayed graph agree. The last parts take a step of gradient descent on
+the norms' weights through `qk_norm_rotary` and `rotary`, and one on the last norm and the output layer (`layer_norm`, `linear_cross_entropy`,
+`linear_distillation`).
 """
 
 from __future__ import annotations
@@ -144,6 +145,30 @@ def learn(cfg: Config) -> tuple[float, float]:
     return float(before.detach()), float(loss().detach())
 
 
+def output_layer(cfg: Config, batch: int, tokens: int, vocabulary: int) -> dict[str, torch.Tensor]:
+    """The decoder's last states normed and scored against the next tokens and, half as much, against a teacher's eight largest logits: the loss and
+    its gradients for the norm and the output layer. The first tokens of each sequence are a prompt, which does not count."""
+    g = torch.Generator(device="cuda").manual_seed(3)
+    with torch.no_grad():
+        states = Decoder(cfg, batch).extend(torch.randn(batch, tokens, cfg.dim, generator=g, device="cuda").to(cfg.dtype))
+    weights = {
+        "norm": torch.ones(cfg.dim, device="cuda", dtype=cfg.dtype),
+        "shift": torch.zeros(cfg.dim, device="cuda", dtype=cfg.dtype),
+        "head": (torch.randn(vocabulary, cfg.dim, generator=g, device="cuda") / math.sqrt(cfg.dim)).to(cfg.dtype),
+    }
+    targets = torch.randint(0, vocabulary, (batch, tokens), generator=g, device="cuda")
+    teacher_ids = torch.randint(0, vocabulary, (batch, tokens, 8), generator=g, device="cuda")
+    teacher_ids[..., 0] = targets
+    teacher_logits = torch.randn(batch, tokens, 8, generator=g, device="cuda").sort(-1, descending=True).values
+    targets[:, : tokens // 3], teacher_ids[:, : tokens // 3] = -100, -1
+    leaves = {name: w.requires_grad_(True) for name, w in weights.items()}
+    x = ff.layer_norm(states, leaves["norm"], leaves["shift"])
+    loss = ff.linear_cross_entropy(x, leaves["head"], targets) + 0.5 * ff.linear_distillation(x, leaves["head"], teacher_ids, teacher_logits, temperature=2.0)
+    grads = torch.autograd.grad(loss, list(leaves.values()))
+    return {"loss": loss.detach(), "states": states, "targets": targets, "teacher_ids": teacher_ids, "teacher_logits": teacher_logits,
+            **weights, **{f"d{name}": d for name, d in zip(leaves, grads, strict=True)}}  # fmt: skip
+
+
 def main() -> None:
     p = argparse.ArgumentParser()
     for name, default in (("layers", 2), ("batch", 4), ("prompt", 100), ("steps", 16)):
@@ -153,6 +178,9 @@ def main() -> None:
     print(f"tokens from a replayed graph against all at once: relative difference {decode(cfg, a.batch, a.prompt, a.steps):.2e}")
     before, after = learn(cfg)
     print(f"a gradient step on the norms' weights: loss {before:.6f} -> {after:.6f}")
+    step = output_layer(cfg, a.batch, a.prompt, 1000)
+    sizes = ", ".join(f"{name} {float(step['d' + name].float().norm()):.3f}" for name in ("norm", "shift", "head"))
+    print(f"the output layer's loss {float(step['loss']):.4f}, gradients' norms: {sizes}")
     status = ff.device_status()
     if status:
         sys.exit(f"device status {status}")

@@ -368,7 +368,7 @@ def test_a_training_step_of_norm_and_both_losses() -> None:
     p, logq = torch.softmax(teacher.double() / 2, 1), torch.log_softmax(logits / 2, 1)
     kd = 4 * (p * (p.log() - logq.gather(1, ids))).sum(1).mean()
     want = torch.autograd.grad(ce + 0.5 * kd, exact)
-    assert abs(float(loss) - float(ce + 0.5 * kd)) < 1e-4  # noqa: PLR2004
+    assert abs(float(loss.detach()) - float((ce + 0.5 * kd).detach())) < 1e-4  # noqa: PLR2004
     for name, a, b in zip(("h", "norm weight", "norm bias", "weight"), got, want, strict=True):
         # a rounding to bfloat16 is off by 2^-8 / sqrt(3) of a value at most, in the mean; up to five of them follow one another, none helps another
         assert float((a.double() - b).norm() / b.norm()) < 5**0.5 * 2.0**-8 / 3**0.5, name
