@@ -275,7 +275,8 @@ HeadLossWork head_loss_work(const B200HeadArgs& a, int sms) {
 }
 
 // Gradients of logits in 16 bits of as many columns at a time as kPieceBytes holds, or 2048. Each piece costs the fp32 sums of dx once more
-// through L2 and HBM, under the products, and the rounds of two launches that are not full.
+// through L2 and HBM, under the products, and the rounds of two launches that are not full. us of a loss with its gradients at 128, 256 and 512 MB:
+// 2047 x 50001 x 1024 609, 596, 596; 4096 x 64000 x 2048 (three quarters of the rows) 2378, 2335, 2299; 4096 x 128000 x 4096 12240, 12110, 12030.
 constexpr int64_t kPieceBytes = 256 << 20;
 // Where what the rounding of logits' gradients took is kept and multiplied too: few rows, whose products wait for memory, and products that are small beside
 // the host's side of a call (2^31 multiply-adds more each for dx and dw, some 5 us; a call's forward and backward pass through autograd take 75).
