@@ -444,6 +444,8 @@ class B200HeadArgs(ctypes.Structure):
         ("grad_stride", ctypes.c_int64),
         ("dx", ctypes.c_void_p),
         ("dw", ctypes.c_void_p),
+        ("bias", ctypes.c_void_p),
+        ("dbias", ctypes.c_void_p),
     )
 
 

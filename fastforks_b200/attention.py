@@ -328,7 +328,8 @@ def device_status(device: torch.device | int | None = None) -> int:
     """Read and clear the device-side error word (synchronises the device). 0 = every kernel ran to the end.
 
     A non-zero value means a kernel gave up a bounded wait and returned early, its output is invalid; or (bits 20 and 21) that an index
-    tensor of a rotary or 4-bit cache call pointed past its table or cache, where nothing was read or written.
+    tensor of a rotary or 4-bit cache call pointed past its table or cache, where nothing was read or written, or (bit 23) that a target or an
+    entry of a loss was past its vocabulary.
     """
     word = ctypes.c_uint32(0)
     with torch.cuda.device(device):

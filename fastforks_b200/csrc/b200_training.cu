@@ -341,6 +341,7 @@ int check_head(const B200HeadArgs* a, bool sizes_only) {
     if (!aligned16(o.p)) return fail(B200_ATTN_UNSUPPORTED, "%s is not 16-byte aligned", o.name);
     if (o.ld < a->dim || o.ld % 8 != 0 || o.ld >= (int64_t(1) << 38)) return fail(B200_ATTN_UNSUPPORTED, "%s: row stride %lld must cover the row and be a multiple of 8", o.name, static_cast<long long>(o.ld));
   }
+  if (!aligned16(a->bias)) return fail(B200_ATTN_UNSUPPORTED, "bias is not 16-byte aligned");
   if (a->state == nullptr || reinterpret_cast<uintptr_t>(a->state) % 256 != 0 || a->state_bytes < head_state(*a).bytes) return fail(B200_ATTN_BAD_CONFIG, "state: %lld bytes on a 256-byte boundary are needed", static_cast<long long>(head_state(*a).bytes));
   if (a->workspace == nullptr || reinterpret_cast<uintptr_t>(a->workspace) % 256 != 0) return fail(B200_ATTN_BAD_CONFIG, "workspace must lie on a 256-byte boundary");
   return B200_ATTN_OK;
@@ -378,6 +379,7 @@ HeadLogitsParams logits_params(const B200HeadArgs& a, const HeadState& s, uint32
   p.ids = at<int>(a.state, s.ids);
   p.p = a.top > 0 ? at<float>(a.state, s.p) : nullptr;
   p.log2_scale = log2_scale(a);
+  p.bias = a.bias;
   p.status = status;
   return p;
 }
@@ -497,7 +499,7 @@ int launch_grad(const B200HeadArgs& a, cudaStream_t stream) {
   if (int rc = device_state(&dev)) return rc;
   const int pairs = std::max(1, dev->sms / 2);
   const HeadState s = head_state(a);
-  const bool want_dx = a.dx != nullptr, want_dw = a.dw != nullptr, f16 = a.dtype == B200_ATTN_F16;
+  const bool want_dx = a.dx != nullptr, want_dw = a.dw != nullptr, want_db = a.dbias != nullptr, f16 = a.dtype == B200_ATTN_F16;
   const HeadGradWork w = head_grad_work(a, want_dx, want_dw, pairs);
   if (a.workspace_bytes < w.bytes) return fail(B200_ATTN_BAD_CONFIG, "workspace: %lld bytes are needed", static_cast<long long>(w.bytes));
   const int64_t row_tiles = w.slot_rows / 256;
@@ -573,6 +575,13 @@ int launch_grad(const B200HeadArgs& a, cudaStream_t stream) {
     q.first = v0 == 0;
     q.splits = std::min(w.splits, (cols + 63) / 64);  // a part without a k-block would never finish; the first piece has one for each
     const int64_t items = row_tiles * col_tiles * q.splits + (want_dw ? static_cast<int64_t>((cols + 255) / 256) * col_tiles : 0);
+    if (want_db) {
+      HeadDbParams d{p.count, g, w.cols, p.rest_at, v0, cols, a.vocab, a.dbias, scale};
+      void* db_args[] = {&d};
+      const void* kernel = f16 ? reinterpret_cast<const void*>(head_db_kernel<__half>) : reinterpret_cast<const void*>(head_db_kernel<__nv_bfloat16>);
+      if (int rc = launch_kernel(kernel, static_cast<unsigned>((cols + 63) / 64), 1, kDbThreads, 0, 1, stream, db_args, "head_db kernel launch")) return rc;
+    }
+    if (!want_dx && !want_dw) continue;
     void* sums_args[] = {&g_k, &g_mn, &w_mn, &x_mn, &copy_mn, &dx, &dw, &q};
     if (int rc = launch_kernel(sums, static_cast<unsigned>(2 * std::min<int64_t>(items, pairs)), 1, kHeadThreads, kHeadSmemBytes, 2, stream, sums_args, "head_sums kernel launch")) return rc;
   }
@@ -703,7 +712,7 @@ int b200_head_sizes(const B200HeadArgs* a, int64_t* state, int64_t* loss_workspa
   *state = head_state(*a).bytes;
   *loss_workspace = head_loss_work(*a, dev->sms).bytes;
   *grad_workspace = 0;
-  for (int want = 1; want < 4; ++want) *grad_workspace = std::max(*grad_workspace, head_grad_work(*a, (want & 1) != 0, (want & 2) != 0, pairs).bytes);
+  for (int want = 0; want < 4; ++want) *grad_workspace = std::max(*grad_workspace, head_grad_work(*a, (want & 1) != 0, (want & 2) != 0, pairs).bytes);
   clear_error();
   return B200_ATTN_OK;
 }
@@ -727,8 +736,8 @@ int b200_head_loss(const B200HeadArgs* a, void* stream_ptr) {
 int b200_head_grad(const B200HeadArgs* a, void* stream_ptr) {
   if (int rc = check_head(a, false)) return rc;
   if (a->grad == nullptr || reinterpret_cast<uintptr_t>(a->grad) % 4 != 0 || a->grad_stride < 0) return fail(B200_ATTN_BAD_CONFIG, "grad must not be NULL, lie on 4 bytes and have no negative stride");
-  if (!aligned16(a->dx) || !aligned16(a->dw)) return fail(B200_ATTN_UNSUPPORTED, "dx or dw is not 16-byte aligned");
-  if (a->dx != nullptr || a->dw != nullptr)
+  if (!aligned16(a->dx) || !aligned16(a->dw) || !aligned16(a->dbias)) return fail(B200_ATTN_UNSUPPORTED, "dx, dw or dbias is not 16-byte aligned");
+  if (a->dx != nullptr || a->dw != nullptr || a->dbias != nullptr)
     if (int rc = launch_grad(*a, static_cast<cudaStream_t>(stream_ptr))) return rc;
   clear_error();
   return B200_ATTN_OK;

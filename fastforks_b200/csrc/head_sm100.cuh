@@ -1,9 +1,9 @@
-// The output layer of a model and its loss, on sm_100a, without the logits. For rows x [T, D], a weight w [V, D] and logits l = x w^T:
+// The output layer of a model and its loss, on sm_100a, without the logits. For rows x [T, D], a weight w [V, D] and logits l = x w^T (+ bias [V]):
 //
 //   cross entropy   loss_t = lse(l_t) - l_t,y                                    dl_t = g_t (softmax(l_t) - onehot_y)
 //   distillation    loss_t = tau^2 sum_k p_k (log p_k - z_t,id(k) + lse(z_t))    dl_t = g_t tau (softmax(z_t) - sum_k p_k onehot_id(k))
 //                   z = l / tau, p = softmax of the teacher's logits / tau over the row's entries
-//   dx = dl w,  dw = dl^T x
+//   dx = dl w,  dw = dl^T x,  dbias = sum_t dl_t
 //
 // Cross entropy is the second form with one entry of weight 1 and tau = 1; the kernels know that form alone. Rows that do not count (no
 // target, no entry) are left out of every product: where there are any, the others are copied together (head_rows_kernel) and the
@@ -18,6 +18,7 @@
 //   head_coef_kernel     gradients that differ from row to row: one power of two for all
 //   head_grads_kernel    a piece of the vocabulary: the logits again, their gradient in 16 bits
 //   head_sums_kernel     dx += G w and dw = G^T x of that piece in one launch
+//   head_db_kernel       dbias of that piece
 //   head_dx_kernel       sums of dx, which are held in fp32, rounded and put where their rows came from
 //
 // Bound by the tensor cores: 2 T D V operations forward, 6 T D V more for the gradients, 2 T D V of which compute the logits again
@@ -263,6 +264,7 @@ struct HeadLogitsParams {
   const int* ids;       // [all_rows, top], ascending, kNoEntry behind the last
   const float* p;       // [all_rows, top] their weights, or null: 1
   float log2_scale;     // log2(e) / tau
+  const void* bias;     // [vocab] or null
   // statistics
   float2* parts;        // [2 tiles_n][parts_stride]: maximum of z in units of ln 2, and the sum of 2^(z - maximum)
   int64_t parts_stride;
@@ -274,6 +276,29 @@ struct HeadLogitsParams {
   int rest_at;          // G's row where what its rounding took is kept, or 0: it is not
   uint32_t* status;
 };
+
+// Adds the bias of 32 columns from `base` on, a multiple of 32: the same for all lanes.
+template <typename T>
+__device__ __forceinline__ void head_add_bias(float (&v)[32], const void* bias, int base, int vocab) {
+  const T* const b = static_cast<const T*>(bias) + base;
+  if (base + 32 <= vocab) {
+#pragma unroll
+    for (int q = 0; q < 4; ++q) {
+      const uint4 raw = __ldg(reinterpret_cast<const uint4*>(b) + q);
+      const uint32_t words[4] = {raw.x, raw.y, raw.z, raw.w};
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const float2 f = gemm_unpack2<T>(words[i]);
+        v[8 * q + 2 * i] += f.x;
+        v[8 * q + 2 * i + 1] += f.y;
+      }
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < 32; ++i)
+      if (base + i < vocab) v[i] += static_cast<float>(b[i]);
+  }
+}
 
 // G = 2^s coef_t (softmax(z_t) - p) is held in 16 bits, the operands' type: its rounding is that of an operand, 2^-9 (fp16 2^-12) of a value on
 // average below half a step, and as large in dx and dw as the rounding of their result. s = 15 for fp16, whose smallest normal
@@ -430,6 +455,7 @@ struct HeadLogitsJob {
                 add_staged(v, half);
               }
             }
+            if (p.bias != nullptr) head_add_bias<T>(v, p.bias, base, p.vocab);
             for_entries(base, [&](int j, int64_t at) {
               float got = 0.f;
 #pragma unroll
@@ -475,6 +501,7 @@ struct HeadLogitsJob {
               const int base = col + half * 32;
               float v[32];
               tmem_ld_x32(acc + c * 64 + half * 32, reinterpret_cast<uint32_t*>(v));
+              if (p.bias != nullptr && base < p.vocab) head_add_bias<T>(v, p.bias, base, p.vocab);
               const float2 scale2 = make_float2(p.log2_scale, p.log2_scale), from2 = make_float2(-lse2, -lse2), coef2 = make_float2(coef, coef);
 #pragma unroll
               for (int i = 0; i < 32; i += 2) {
@@ -714,8 +741,9 @@ __device__ __forceinline__ void head_few(const CUtensorMap* x, const CUtensorMap
 #pragma unroll
           for (int j = 0; j < 32; ++j) v[j] += more[j];
         }
+        const float bias = p.l.bias != nullptr && v0 + lane < v1 ? static_cast<float>(static_cast<const T*>(p.l.bias)[v0 + lane]) : 0.f;
 #pragma unroll
-        for (int j = 0; j < 32; ++j) turned[j][lane] = v[j];
+        for (int j = 0; j < 32; ++j) turned[j][lane] = v[j] + bias;
         __syncwarp();
         const float* const mine = turned[lane];
         const int n = v1 - v0;
@@ -1313,6 +1341,49 @@ __global__ void __launch_bounds__(kCoefThreads) head_coef_kernel(const HeadCoefP
     const int src = __ldg(p.idx + i);
     p.coef[src] = __ldg(p.g + src * p.stride) * inverse;
   }
+}
+
+// dbias of a piece: columns of G (and of what its rounding took) summed over the rows, 64 columns a CTA, eight a thread, every 32nd row each, the
+// threads' sums in their order. One pass over G, a fiftieth of the products' time.
+struct HeadDbParams {
+  const int* count;
+  const void* g;    // [.., stride]
+  int64_t stride;
+  int rest_at, v0, cols, vocab;
+  void* db;         // [vocab]
+  HeadScale scale;
+};
+constexpr int kDbThreads = 256;
+
+template <typename T>
+__global__ void __launch_bounds__(kDbThreads) head_db_kernel(const HeadDbParams p) {
+  __shared__ float sums[kDbThreads / 8][65];
+  grid_dependency_wait();
+  grid_launch_dependents();
+  const int count = __ldg(p.count), group = threadIdx.x & 7, first = threadIdx.x >> 3;
+  float s[8] = {};
+  for (int at = 0; at <= p.rest_at; at += max(p.rest_at, 1)) {  // (once without a rest)
+    const T* const g = static_cast<const T*>(p.g) + at * p.stride + blockIdx.x * 64 + group * 8;
+#pragma unroll 4
+    for (int r = first; r < count; r += kDbThreads / 8) {
+      const uint4 raw = __ldg(reinterpret_cast<const uint4*>(g + r * p.stride));
+      const uint32_t words[4] = {raw.x, raw.y, raw.z, raw.w};
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const float2 f = gemm_unpack2<T>(words[i]);
+        s[2 * i] += f.x;
+        s[2 * i + 1] += f.y;
+      }
+    }
+  }
+#pragma unroll
+  for (int i = 0; i < 8; ++i) sums[first][group * 8 + i] = s[i];
+  __syncthreads();
+  const int col = blockIdx.x * 64 + threadIdx.x;
+  if (threadIdx.x >= 64 || col >= p.cols) return;
+  float sum = 0.f;
+  for (int i = 0; i < kDbThreads / 8; ++i) sum += sums[i][threadIdx.x];
+  static_cast<T*>(p.db)[p.v0 + col] = static_cast<T>(sum * head_scale(p.scale));
 }
 
 // dx: the parts' sums added in their order, scaled, rounded; zeros for rows that do not count. Eight values a thread.

@@ -667,7 +667,7 @@ PyObject* py_layer_norm(PyObject*, PyObject* const* args, Py_ssize_t n) {
   return THPVariable_Wrap(LayerNormFunction::apply(*x, has & 1 ? affine[0] : *x, has & 2 ? affine[1] : *x, has, eps));
 }
 
-void set_head(B200HeadArgs* a, const at::Tensor& x, const at::Tensor& w, int64_t top, double tau, int64_t reduction) {
+void set_head(B200HeadArgs* a, const at::Tensor& x, const at::Tensor& w, const at::Tensor& bias, int64_t top, double tau, int64_t reduction) {
   std::memset(a, 0, sizeof(*a));
   a->struct_size = sizeof(*a);
   a->dtype = dtype_code(x);
@@ -680,15 +680,16 @@ void set_head(B200HeadArgs* a, const at::Tensor& x, const at::Tensor& w, int64_t
   a->x = x.data_ptr();
   a->w = w.data_ptr();
   a->ldx = a->ldw = a->dim;
+  a->bias = bias.defined() ? bias.data_ptr() : nullptr;
 }
 
 at::Tensor bytes_for(int64_t n, const at::Tensor& like) { return at::detail::empty_cuda({n}, at::kByte, like.device(), std::nullopt); }
 
 // The loss, and in `state` what its gradients need. targets [rows] or [rows, top]; teacher undefined: cross entropy.
-at::Tensor head_loss(const at::Tensor& x, const at::Tensor& w, const at::Tensor& targets, const at::Tensor& teacher, int64_t ignore, double tau, int64_t reduction, at::Tensor* state) {
+at::Tensor head_loss(const at::Tensor& x, const at::Tensor& w, const at::Tensor& bias, const at::Tensor& targets, const at::Tensor& teacher, int64_t ignore, double tau, int64_t reduction, at::Tensor* state) {
   B200HeadArgs a;
   const int64_t top = teacher.defined() ? targets.size(-1) : 0;
-  set_head(&a, x, w, top, tau, reduction);
+  set_head(&a, x, w, bias, top, tau, reduction);
   a.targets = targets.data_ptr();
   a.target_bytes = static_cast<int32_t>(targets.element_size());
   a.targets_stride = a.teacher_stride = top;
@@ -710,11 +711,12 @@ at::Tensor head_loss(const at::Tensor& x, const at::Tensor& w, const at::Tensor&
 }
 
 struct HeadLossFunction : torch::autograd::Function<HeadLossFunction> {
-  static at::Tensor forward(AutogradContext* ctx, const at::Tensor& x, const at::Tensor& w, const at::Tensor& targets, const at::Tensor& logits, bool distill, int64_t ignore, double tau, int64_t reduction) {
-    const at::Tensor teacher = distill ? logits : at::Tensor();  // (`targets` stand in for no teacher)
+  // (x stands in for no bias, and `targets` for no teacher: apply() takes no undefined tensor.)
+  static at::Tensor forward(AutogradContext* ctx, const at::Tensor& x, const at::Tensor& w, const at::Tensor& vector, const at::Tensor& targets, const at::Tensor& logits, bool biased, bool distill, int64_t ignore, double tau, int64_t reduction) {
+    const at::Tensor teacher = distill ? logits : at::Tensor(), bias = biased ? vector : at::Tensor();
     at::Tensor state;
-    at::Tensor loss = head_loss(x, w, targets, teacher, ignore, tau, reduction, &state);
-    ctx->save_for_backward({x, w, state});
+    at::Tensor loss = head_loss(x, w, bias, targets, teacher, ignore, tau, reduction, &state);
+    ctx->save_for_backward({x, w, bias, state});
     ctx->saved_data["top"] = teacher.defined() ? targets.size(-1) : int64_t(0);
     ctx->saved_data["tau"] = tau;
     ctx->saved_data["reduction"] = reduction;
@@ -722,14 +724,14 @@ struct HeadLossFunction : torch::autograd::Function<HeadLossFunction> {
   }
   static variable_list backward(AutogradContext* ctx, const variable_list& grads) {
     const variable_list saved = ctx->get_saved_variables();
-    variable_list result(8);
+    variable_list result(10);
     {
       const at::NoGradGuard guard;
-      const at::Tensor &x = saved[0], &w = saved[1], &state = saved[2];
+      const at::Tensor &x = saved[0], &w = saved[1], &bias = saved[2], &state = saved[3];
       const c10::cuda::CUDAGuard on(x.device());
       const int64_t reduction = ctx->saved_data["reduction"].toInt();
       B200HeadArgs a;
-      set_head(&a, x, w, ctx->saved_data["top"].toInt(), ctx->saved_data["tau"].toDouble(), reduction);
+      set_head(&a, x, w, bias, ctx->saved_data["top"].toInt(), ctx->saved_data["tau"].toDouble(), reduction);
       at::Tensor g = grads[0];
       if (!g.defined()) g = at::zeros({reduction == 0 ? a.rows : 1}, x.options().dtype(at::kFloat).requires_grad(false));
       if (g.dim() > 1) g = g.reshape({-1});
@@ -742,6 +744,10 @@ struct HeadLossFunction : torch::autograd::Function<HeadLossFunction> {
       if (ctx->needs_input_grad(1)) {
         result[1] = empty_like_type(w.sizes(), w);
         a.dw = result[1].data_ptr();
+      }
+      if (bias.defined() && ctx->needs_input_grad(2)) {
+        result[2] = empty_like_type(bias.sizes(), bias);
+        a.dbias = result[2].data_ptr();
       }
       int64_t loss_bytes = 0;
       TORCH_CHECK(b200_head_sizes(&a, &a.state_bytes, &loss_bytes, &a.workspace_bytes) == B200_ATTN_OK, "loss gradient: ", b200_attn_last_error());
@@ -760,31 +766,38 @@ bool operand_of(const at::Tensor* t, c10::DeviceIndex device) {
          reinterpret_cast<uintptr_t>(t->data_ptr()) % 16 == 0;
 }
 
-// head_loss(x, weight, targets, teacher | None, ignore, tau, reduction: 0 none, 1 sum, 2 mean)
+// head_loss(x, weight, bias | None, targets, teacher | None, ignore, tau, reduction: 0 none, 1 sum, 2 mean)
 PyObject* py_head_loss(PyObject*, PyObject* const* args, Py_ssize_t n) {
-  if (n != 7 || !PyLong_Check(args[4])) Py_RETURN_NONE;
+  if (n != 8 || !PyLong_Check(args[5])) Py_RETURN_NONE;
   const c10::DeviceIndex device = c10::cuda::current_device();
-  const at::Tensor *x = tensor_of(args[0]), *w = tensor_of(args[1]), *y = tensor_of(args[2]);
+  const at::Tensor *x = tensor_of(args[0]), *w = tensor_of(args[1]), *y = tensor_of(args[3]);
   if (!operand_of(x, device) || !operand_of(w, device) || w->dim() != 2 || w->scalar_type() != x->scalar_type() || w->size(1) != x->size(-1)) Py_RETURN_NONE;
   if (y == nullptr || !plain(*y, device) || !y->is_contiguous() || (y->scalar_type() != at::kLong && y->scalar_type() != at::kInt)) Py_RETURN_NONE;
   int overflow = 0;
-  const int64_t ignore = PyLong_AsLongLongAndOverflow(args[4], &overflow);
+  const int64_t ignore = PyLong_AsLongLongAndOverflow(args[5], &overflow);
   double tau = 1;
   int64_t reduction = 0;
-  if (overflow != 0 || !number(args[5], &tau) || !(tau > 0) || std::isinf(tau) || !integer(args[6], &reduction) || reduction < 0 || reduction > 2) Py_RETURN_NONE;
-  at::Tensor teacher;
+  if (overflow != 0 || !number(args[6], &tau) || !(tau > 0) || std::isinf(tau) || !integer(args[7], &reduction) || reduction < 0 || reduction > 2) Py_RETURN_NONE;
+  at::Tensor teacher, bias;
+  if (args[2] != Py_None) {
+    const at::Tensor* b = tensor_of(args[2]);
+    if (b == nullptr || !on_device(*b, device) || b->scalar_type() != x->scalar_type() || b->dim() != 1 || b->size(0) != w->size(0) || !b->is_contiguous() || reinterpret_cast<uintptr_t>(b->data_ptr()) % 16 != 0) Py_RETURN_NONE;
+    bias = *b;
+  }
   const at::IntArrayRef rows = x->sizes().slice(0, x->dim() - 1);
-  if (args[3] == Py_None) {
+  if (args[4] == Py_None) {
     if (y->sizes() != rows) Py_RETURN_NONE;
   } else {
-    const at::Tensor* t = tensor_of(args[3]);
+    const at::Tensor* t = tensor_of(args[4]);
     if (t == nullptr || !on_device(*t, device) || wants_grad(*t) || !heads_type(*t) || !t->is_contiguous() || t->sizes() != y->sizes()) Py_RETURN_NONE;
     if (y->dim() != x->dim() || y->sizes().slice(0, y->dim() - 1) != rows || y->size(-1) < 1 || y->size(-1) > 256) Py_RETURN_NONE;
     teacher = *t;
   }
-  if (wants_grad(*x) || wants_grad(*w)) return THPVariable_Wrap(HeadLossFunction::apply(*x, *w, *y, teacher.defined() ? teacher : *y, teacher.defined(), ignore, tau, reduction));
+  const bool biased = bias.defined(), distill = teacher.defined();
+  if (wants_grad(*x) || wants_grad(*w) || (biased && wants_grad(bias)))
+    return THPVariable_Wrap(HeadLossFunction::apply(*x, *w, biased ? bias : *x, *y, distill ? teacher : *y, biased, distill, ignore, tau, reduction));
   at::Tensor state;
-  return THPVariable_Wrap(head_loss(*x, *w, *y, teacher, ignore, tau, reduction, &state));
+  return THPVariable_Wrap(head_loss(*x, *w, bias, *y, teacher, ignore, tau, reduction, &state));
 }
 
 // Cache, page table and lengths of a call on `batch` sequences.

@@ -28,7 +28,12 @@ def _rows(t: torch.Tensor) -> torch.Tensor:
     return t
 
 
-def _check(what: str, x: torch.Tensor, w: torch.Tensor, reduction: str) -> None:
+def _vector(t: torch.Tensor | None) -> torch.Tensor | None:
+    """A bias on 16 bytes."""
+    return t if t is None or (t.is_contiguous() and t.data_ptr() % 16 == 0) else t.clone(memory_format=torch.contiguous_format)
+
+
+def _check(what: str, x: torch.Tensor, w: torch.Tensor, bias: torch.Tensor | None, reduction: str) -> None:
     if x.dtype not in (torch.float16, torch.bfloat16) or not x.is_cuda or x.dim() < 1:
         msg = f"{what}: x must be a float16 / bfloat16 CUDA tensor [..., dim], got {tuple(x.shape)} {x.dtype} on {x.device}"
         raise ValueError(msg)
@@ -41,11 +46,16 @@ def _check(what: str, x: torch.Tensor, w: torch.Tensor, reduction: str) -> None:
     if reduction not in _REDUCTIONS:
         msg = f"{what}: reduction {reduction!r} must be one of {tuple(_REDUCTIONS)}"
         raise ValueError(msg)
+    if bias is not None and (bias.dtype != x.dtype or bias.device != x.device or bias.shape != w.shape[:1]):
+        msg = f"{what}: bias must be {x.dtype} [{w.shape[0]}] on {x.device}, got {tuple(bias.shape)} {bias.dtype} on {bias.device}"
+        raise ValueError(msg)
     refuse_tangent(what, "x", x)
     refuse_tangent(what, "weight", w)
+    if bias is not None:
+        refuse_tangent(what, "bias", bias)
 
 
-def _args(x: torch.Tensor, w: torch.Tensor, top: int, tau: float, reduction: int) -> _lib.B200HeadArgs:
+def _args(x: torch.Tensor, w: torch.Tensor, bias: torch.Tensor | None, top: int, tau: float, reduction: int) -> _lib.B200HeadArgs:  # noqa: PLR0913
     a = _lib.B200HeadArgs()
     a.struct_size = ctypes.sizeof(a)
     a.dtype, a.rows, a.dim, a.vocab, a.top, a.tau, a.reduction = _DTYPES[x.dtype], x.shape[0], x.shape[1], w.shape[0], top, tau, reduction
@@ -54,6 +64,8 @@ def _args(x: torch.Tensor, w: torch.Tensor, top: int, tau: float, reduction: int
         a.ldx = x.shape[1]
     if w.shape[0] == 1:
         a.ldw = w.shape[1]
+    if bias is not None:
+        a.bias = bias.data_ptr()
     return a
 
 
@@ -67,9 +79,9 @@ def _buffer(size: int, like: torch.Tensor) -> torch.Tensor:
     return torch.empty(size, dtype=torch.uint8, device=like.device)
 
 
-def _loss(what: str, x: torch.Tensor, w: torch.Tensor, targets: torch.Tensor, teacher: torch.Tensor | None, ignore: int, tau: float, reduction: int) -> tuple[torch.Tensor, torch.Tensor]:  # noqa: PLR0913
+def _loss(what: str, x: torch.Tensor, w: torch.Tensor, bias: torch.Tensor | None, targets: torch.Tensor, teacher: torch.Tensor | None, ignore: int, tau: float, reduction: int) -> tuple[torch.Tensor, torch.Tensor]:  # noqa: PLR0913
     """The loss (per row, or one number) and what its gradients need."""
-    a = _args(x, w, 0 if teacher is None else targets.shape[1], tau, reduction)
+    a = _args(x, w, bias, 0 if teacher is None else targets.shape[1], tau, reduction)
     a.targets, a.target_bytes, a.ignore = targets.data_ptr(), targets.element_size(), ignore
     if teacher is not None:
         a.targets_stride, a.teacher, a.teacher_stride, a.teacher_dtype = targets.stride(0), teacher.data_ptr(), teacher.stride(0), _DTYPES[teacher.dtype]
@@ -86,43 +98,44 @@ def _loss(what: str, x: torch.Tensor, w: torch.Tensor, targets: torch.Tensor, te
 
 class _HeadLoss(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, what, x, w, targets, teacher, ignore, tau, reduction):  # noqa: ANN001, ANN205, PLR0913
-        loss, state = _loss(what, _rows(x), _rows(w), targets, teacher, ignore, tau, reduction)
-        ctx.save_for_backward(x, w, state)
+    def forward(ctx, what, x, w, bias, targets, teacher, ignore, tau, reduction):  # noqa: ANN001, ANN205, PLR0913
+        loss, state = _loss(what, _rows(x), _rows(w), _vector(bias), targets, teacher, ignore, tau, reduction)
+        ctx.save_for_backward(x, w, bias, state)
         ctx.what, ctx.top, ctx.tau, ctx.reduction = what, 0 if teacher is None else targets.shape[1], tau, reduction
         return loss
 
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, g):  # noqa: ANN001, ANN205
-        x, w, state = ctx.saved_tensors
-        rows, weight = _rows(x), _rows(w)
-        a = _args(rows, weight, ctx.top, ctx.tau, ctx.reduction)
+        x, w, bias, state = ctx.saved_tensors
+        rows, weight, vector = _rows(x), _rows(w), _vector(bias)
+        a = _args(rows, weight, vector, ctx.top, ctx.tau, ctx.reduction)
         dx = torch.empty(x.shape, dtype=x.dtype, device=x.device) if ctx.needs_input_grad[1] else None
         dw = torch.empty(w.shape, dtype=w.dtype, device=w.device) if ctx.needs_input_grad[2] else None
+        db = torch.empty(bias.shape, dtype=bias.dtype, device=bias.device) if ctx.needs_input_grad[3] else None
         a.grad, a.grad_stride = g.data_ptr(), g.stride(0) if g.dim() else 0
-        a.dx, a.dw = None if dx is None else dx.data_ptr(), None if dw is None else dw.data_ptr()
+        a.dx, a.dw, a.dbias = (None if t is None else t.data_ptr() for t in (dx, dw, db))
         with torch.cuda.device(x.device):
             _, _, size = _sizes(f"{ctx.what} gradient", a)
             ws = _buffer(size, x)
             a.state, a.state_bytes, a.workspace, a.workspace_bytes = state.data_ptr(), state.numel(), ws.data_ptr(), size
             code = _lib.library().b200_head_grad(ctypes.byref(a), torch._C._cuda_getCurrentRawStream(x.device.index))  # noqa: SLF001
         _lib.raise_for_code(code, f"{ctx.what} gradient")
-        return None, dx, dw, None, None, None, None, None
+        return None, dx, dw, db, None, None, None, None, None
 
 
-def _run(what: str, x: torch.Tensor, w: torch.Tensor, targets: torch.Tensor, teacher: torch.Tensor | None, ignore: int, tau: float, reduction: str) -> torch.Tensor:  # noqa: PLR0913
+def _run(what: str, x: torch.Tensor, w: torch.Tensor, bias: torch.Tensor | None, targets: torch.Tensor, teacher: torch.Tensor | None, ignore: int, tau: float, reduction: str) -> torch.Tensor:  # noqa: PLR0913
     shape = x.shape[:-1] if reduction == "none" else ()
-    grad = torch.is_grad_enabled() and (x.requires_grad or w.requires_grad)
+    grad = torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x, w, bias))
     if x.numel() == 0:
         if grad:
             msg = f"{what}: x {tuple(x.shape)} without a row has no gradient"
             raise ValueError(msg)
         return torch.zeros(shape, dtype=torch.float32, device=x.device)
     if grad:
-        loss = _HeadLoss.apply(what, x, w, targets, teacher, ignore, tau, _REDUCTIONS[reduction])
+        loss = _HeadLoss.apply(what, x, w, bias, targets, teacher, ignore, tau, _REDUCTIONS[reduction])
     else:
-        loss, _ = _loss(what, _rows(x), _rows(w), targets, teacher, ignore, tau, _REDUCTIONS[reduction])
+        loss, _ = _loss(what, _rows(x), _rows(w), _vector(bias), targets, teacher, ignore, tau, _REDUCTIONS[reduction])
     return loss.view(shape)
 
 
@@ -131,10 +144,11 @@ def linear_cross_entropy(  # noqa: PLR0913
     weight: torch.Tensor,
     targets: torch.Tensor,
     *,
+    bias: torch.Tensor | None = None,
     ignore_index: int = -100,
     reduction: str = "mean",
 ) -> torch.Tensor:
-    """Softmax cross entropy of the logits `x @ weight^T`, which are never in memory; differentiable (once, backwards) in x and weight.
+    """Softmax cross entropy of the logits `x @ weight^T + bias`, which are never in memory; differentiable (once, backwards) in x, weight and bias.
 
     `logsumexp(logits) - logits[target]` of each row, products and sums in fp32, the loss in fp32. The gradients of the logits are rounded to
     x's type once, on their way into the two products that give those of x and weight. Rows that do not count are left out of all work.
@@ -144,6 +158,7 @@ def linear_cross_entropy(  # noqa: PLR0913
         weight: `[vocabulary, dim]` of x's type.
         targets: int64 or int32 `[...]`, the shape of x without its last dimension. One outside the vocabulary (and not `ignore_index`)
             makes NaN of its row, and `device_status()` reports it.
+        bias: `[vocabulary]` of x's type, or None.
         ignore_index: Target of rows that do not count: their loss is 0, they have no gradient, and what x holds there is not looked at.
         reduction: `"mean"` or `"sum"` over the rows that count (0 where none does), or `"none"`: the loss of each row.
 
@@ -152,18 +167,18 @@ def linear_cross_entropy(  # noqa: PLR0913
         KernelUnavailableError: The CUDA library is not built or does not load.
     """
     if _lib.fast is not None:
-        done = _lib.fast.head_loss(x, weight, targets, None, ignore_index, 1.0, _REDUCTIONS.get(reduction))
+        done = _lib.fast.head_loss(x, weight, bias, targets, None, ignore_index, 1.0, _REDUCTIONS.get(reduction))
         if done is not None:
             return done
     what = "linear_cross_entropy"
-    _check(what, x, weight, reduction)
+    _check(what, x, weight, bias, reduction)
     if targets.dtype not in (torch.int64, torch.int32) or targets.shape != x.shape[:-1] or targets.device != x.device:
         msg = f"{what}: targets must be int64 or int32 {tuple(x.shape[:-1])} on {x.device}, got {tuple(targets.shape)} {targets.dtype} on {targets.device}"
         raise ValueError(msg)
     if not -(2**63) <= ignore_index < 2**63:
         msg = f"{what}: ignore_index {ignore_index} is no 64-bit number"
         raise ValueError(msg)
-    return _run(what, x, weight, targets.contiguous(), None, ignore_index, 1.0, reduction)
+    return _run(what, x, weight, bias, targets.contiguous(), None, ignore_index, 1.0, reduction)
 
 
 def linear_distillation(  # noqa: PLR0913
@@ -172,10 +187,12 @@ def linear_distillation(  # noqa: PLR0913
     teacher_ids: torch.Tensor,
     teacher_logits: torch.Tensor,
     *,
+    bias: torch.Tensor | None = None,
     temperature: float = 1.0,
     reduction: str = "mean",
 ) -> torch.Tensor:
-    """Divergence of the distribution of the logits `x @ weight^T` from a teacher's largest logits; differentiable (once, backwards) in x and weight.
+    """Divergence of the distribution of the logits `x @ weight^T + bias` from a teacher's largest logits; differentiable (once, backwards) in x,
+    weight and bias.
 
     With p the softmax of the teacher's logits of a row over `temperature`, and q that of all of the row's own logits over `temperature`:
     `temperature ** 2 * sum(p * (log p - log q))` over the teacher's entries, in fp32. Otherwise as `linear_cross_entropy`.
@@ -188,6 +205,7 @@ def linear_distillation(  # noqa: PLR0913
             `device_status()` reports it.
         teacher_logits: fp16 / bf16 / fp32 of the same shape (log probabilities are logits too). An entry of -inf has no weight; a row whose entries
             all are is NaN.
+        bias: `[vocabulary]` of x's type, or None.
         temperature: Positive.
         reduction: `"mean"` or `"sum"` over the rows that count (0 where none does), or `"none"`: the loss of each row, 0 where it does not count.
 
@@ -196,11 +214,11 @@ def linear_distillation(  # noqa: PLR0913
         KernelUnavailableError: The CUDA library is not built or does not load.
     """
     if _lib.fast is not None and teacher_logits is not None:
-        done = _lib.fast.head_loss(x, weight, teacher_ids, teacher_logits, 0, temperature, _REDUCTIONS.get(reduction))
+        done = _lib.fast.head_loss(x, weight, bias, teacher_ids, teacher_logits, 0, temperature, _REDUCTIONS.get(reduction))
         if done is not None:
             return done
     what = "linear_distillation"
-    _check(what, x, weight, reduction)
+    _check(what, x, weight, bias, reduction)
     if teacher_ids.dtype not in (torch.int64, torch.int32) or teacher_ids.dim() != x.dim() or teacher_ids.shape[:-1] != x.shape[:-1] or not 1 <= teacher_ids.shape[-1] <= MAX_TOP or teacher_ids.device != x.device:
         msg = f"{what}: teacher_ids must be int64 or int32 {tuple(x.shape[:-1])} and 1 .. {MAX_TOP} entries on {x.device}, got {tuple(teacher_ids.shape)} {teacher_ids.dtype} on {teacher_ids.device}"
         raise ValueError(msg)
@@ -217,4 +235,4 @@ def linear_distillation(  # noqa: PLR0913
     k = teacher_ids.shape[-1]
     ids, logits = (t.reshape(-1, k) for t in (teacher_ids, teacher_logits))
     ids, logits = (t if t.stride(1) == 1 or k == 1 else t.contiguous() for t in (ids, logits))
-    return _run(what, x, weight, ids, logits, 0, float(temperature), reduction)
+    return _run(what, x, weight, bias, ids, logits, 0, float(temperature), reduction)

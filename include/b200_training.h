@@ -57,13 +57,13 @@ int b200_layer_norm_grad(const B200LayerNormArgs* args, void* stream);
 int b200_layer_norm_workspace(const B200LayerNormArgs* args, int64_t* bytes);
 
 /*
- * The loss of an output layer of weight w [vocab, dim] at rows x [rows, dim], logits l = x w^T (never in memory):
+ * The loss of an output layer of weight w [vocab, dim] at rows x [rows, dim], logits l = x w^T + bias (never in memory):
  *     top = 0   loss_t = logsumexp(l_t) - l_t[targets[t]]; a row whose target is `ignore` does not count
  *     top > 0   z = l / tau; p = softmax(teacher[t] / tau) over the row's entries whose token (targets[t, k]) is not negative;
  *               loss_t = tau^2 * sum_k p_k (log p_k - z[token k] + logsumexp(z)); a row without an entry does not count
  * A token past the vocabulary makes NaN of its row (loss and gradients) and sets B200_STATUS_TARGET. Rows that do not count have loss 0 and no
  * gradient, and what x holds there is not looked at. The sum and the mean are over the rows that count, 0 where none does.
- * b200_head_grad gives dx = dl w and dw = dl^T x, with dl = grad_t * tau * (softmax(z_t) - p at its tokens) held in `dtype` on its way into
+ * b200_head_grad gives dx = dl w, dw = dl^T x and dbias = sum over rows of dl, with dl = grad_t * tau * (softmax(z_t) - p at its tokens) held in `dtype` on its way into
  * the products. It reads the `state` of the forward call, which may be shared by several calls and stays as it is.
  * Products accumulate in fp32; sums are taken in a fixed order.
  */
@@ -99,11 +99,13 @@ typedef struct B200HeadArgs {
   int64_t grad_stride;
   void* dx;             /* [rows, dim] contiguous, or NULL: not asked for */
   void* dw;             /* [vocab, dim] contiguous, or NULL: not asked for */
+  const void* bias;     /* [vocab] of `dtype`, 16-byte aligned, or NULL */
+  void* dbias;          /* [vocab] of `dtype`, 16-byte aligned, or NULL: not asked for */
 } B200HeadArgs;
 
 int b200_head_loss(const B200HeadArgs* args, void* stream);
 int b200_head_grad(const B200HeadArgs* args, void* stream);
-/* Bytes of `state`, and of `workspace` for the loss and for the gradients (dx and dw both asked for; fewer otherwise suffice). */
+/* Bytes of `state`, and of `workspace` for the loss and for the gradients, whichever of them are asked for. */
 int b200_head_sizes(const B200HeadArgs* args, int64_t* state, int64_t* loss_workspace, int64_t* grad_workspace);
 
 #ifdef __cplusplus

@@ -45,12 +45,13 @@ class Head:
     dl: torch.Tensor | None = None  # gradient of the logits
     dx: torch.Tensor | None = None
     dw: torch.Tensor | None = None
+    db: torch.Tensor | None = None
 
 
-def head(x: torch.Tensor, w: torch.Tensor, p: torch.Tensor, entropy: torch.Tensor, counts: torch.Tensor, tau: float, reduction: str, g: torch.Tensor | None) -> Head:  # noqa: PLR0913
+def head(x: torch.Tensor, w: torch.Tensor, p: torch.Tensor, entropy: torch.Tensor, counts: torch.Tensor, tau: float, reduction: str, g: torch.Tensor | None, bias: torch.Tensor | None) -> Head:  # noqa: PLR0913
     """p `[T, V]` over the vocabulary; entropy = sum p log p; g: gradient of the result (a number, or one for each row)."""
     x = torch.where(counts[:, None], x.double(), 0.0)
-    z = x @ w.double().T / tau
+    z = (x @ w.double().T + (0.0 if bias is None else bias.double())) / tau
     logq = z - torch.logsumexp(z, 1, keepdim=True)
     rows = torch.where(counts, tau**2 * (entropy - (p * torch.where(p > 0, logq, 0.0)).sum(1)), 0.0)
     n = counts.sum().clamp(min=1)
@@ -59,18 +60,18 @@ def head(x: torch.Tensor, w: torch.Tensor, p: torch.Tensor, entropy: torch.Tenso
     if g is not None:
         each = g.double().expand(rows.shape) / (n if reduction == "mean" else 1)
         r.dl = torch.where(counts[:, None], (each * tau)[:, None] * (r.q - p), 0.0)
-        r.dx, r.dw = r.dl @ w.double(), r.dl.T @ x
+        r.dx, r.dw, r.db = r.dl @ w.double(), r.dl.T @ x, r.dl.sum(0)
     return r
 
 
-def cross_entropy(x: torch.Tensor, w: torch.Tensor, targets: torch.Tensor, ignore: int, reduction: str, g: torch.Tensor | None = None) -> Head:  # noqa: PLR0913
+def cross_entropy(x: torch.Tensor, w: torch.Tensor, targets: torch.Tensor, ignore: int, reduction: str, g: torch.Tensor | None = None, bias: torch.Tensor | None = None) -> Head:  # noqa: PLR0913
     counts = targets != ignore
     p = torch.zeros(x.shape[0], w.shape[0], dtype=torch.float64, device=x.device)
     p[counts, targets[counts].long()] = 1.0
-    return head(x, w, p, torch.zeros_like(p[:, 0]), counts, 1.0, reduction, g)
+    return head(x, w, p, torch.zeros_like(p[:, 0]), counts, 1.0, reduction, g, bias)
 
 
-def distillation(x: torch.Tensor, w: torch.Tensor, ids: torch.Tensor, teacher: torch.Tensor, tau: float, reduction: str, g: torch.Tensor | None = None) -> Head:  # noqa: PLR0913
+def distillation(x: torch.Tensor, w: torch.Tensor, ids: torch.Tensor, teacher: torch.Tensor, tau: float, reduction: str, g: torch.Tensor | None = None, bias: torch.Tensor | None = None) -> Head:  # noqa: PLR0913
     there = ids >= 0
     counts = there.any(1)
     z = (teacher.double() / tau).masked_fill(~there, -torch.inf)
@@ -79,4 +80,4 @@ def distillation(x: torch.Tensor, w: torch.Tensor, ids: torch.Tensor, teacher: t
     entropy = torch.where(each > 0, each * logp, 0.0).sum(1)
     p = torch.zeros(x.shape[0], w.shape[0], dtype=torch.float64, device=x.device)
     p.scatter_add_(1, ids.clamp(min=0).long(), each)
-    return head(x, w, p, entropy, counts, tau, reduction, g)
+    return head(x, w, p, entropy, counts, tau, reduction, g, bias)

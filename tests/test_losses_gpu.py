@@ -47,10 +47,10 @@ def layer(rows: int, vocab: int, dim: int, dtype: torch.dtype, seed: int = 0) ->
     return (normal(rows, dim, seed=seed + 3) + lean * w[y].float()).to(dtype), w, y
 
 
-def logit_error(x: torch.Tensor, w: torch.Tensor, counts: torch.Tensor) -> torch.Tensor:
+def logit_error(x: torch.Tensor, w: torch.Tensor, counts: torch.Tensor, bias: torch.Tensor | float) -> torch.Tensor:
     """Of each row, the largest."""
     x = torch.where(counts[:, None], x.double(), 0.0)
-    return 2 * F32 * (x.shape[1] / 16 + 16) * (x.abs() @ w.double().abs().T).amax(1)
+    return 2 * F32 * (x.shape[1] / 16 + 16) * (x.abs() @ w.double().abs().T + abs(bias)).amax(1)
 
 
 def near(got: torch.Tensor, ref: torch.Tensor, bound: torch.Tensor, what: str) -> None:
@@ -59,10 +59,10 @@ def near(got: torch.Tensor, ref: torch.Tensor, bound: torch.Tensor, what: str) -
     assert bool((off <= bound).all()), f"{what}: worst {float((off / bound).max()):.2f} bounds"
 
 
-def check(r: oracle.Head, x: torch.Tensor, w: torch.Tensor, tau: float, loss: torch.Tensor, grads: dict, g: torch.Tensor | None, reduction: str) -> None:  # noqa: PLR0913
-    x, w = x.detach(), w.detach()
-    d = logit_error(x, w, r.counts) / tau
-    z = (torch.where(r.counts[:, None], x.double(), 0.0) @ w.double().T / tau).abs().amax(1)
+def check(r: oracle.Head, x: torch.Tensor, w: torch.Tensor, tau: float, loss: torch.Tensor, grads: dict, g: torch.Tensor | None, reduction: str, bias: torch.Tensor | None = None) -> None:  # noqa: PLR0913
+    x, w, b64 = x.detach(), w.detach(), 0.0 if bias is None else bias.detach().double()
+    d = logit_error(x, w, r.counts, b64) / tau
+    z = ((torch.where(r.counts[:, None], x.double(), 0.0) @ w.double().T + b64) / tau).abs().amax(1)
     e_rows = torch.where(r.counts, tau**2 * (2 * d + 40 * F32 * (z + 3)) + 40 * F32 * r.rows.abs(), 0.0)
     n = int(r.counts.sum().clamp(min=1))
     e_loss = {"none": e_rows, "sum": e_rows.sum(), "mean": e_rows.sum() / n}[reduction]
@@ -81,6 +81,9 @@ def check(r: oracle.Head, x: torch.Tensor, w: torch.Tensor, tau: float, loss: to
             size = left.abs() @ right.abs()
             e = error @ right.abs() + 2 * F32 * (left.shape[1] / 16 + 64) * size
             near(grads[name].detach(), ref, half * (ref.abs() + e) + e + TINY[x.dtype], name)
+    if "db" in grads:
+        e = e_dl.sum(0) + 2 * F32 * (x.shape[0] / 32 + 64) * r.dl.abs().sum(0)
+        near(grads["db"].detach(), r.db, half * (r.db.abs() + e) + e + TINY[x.dtype], "db")
 
 
 SHAPES = [
@@ -128,6 +131,36 @@ def test_distillation(shape: tuple[int, int, int], top: int, tau: float, dtype: 
         order = torch.rand(rows, top, device="cuda").argsort(1)  # entries in another order: the same sums but for their order
         other = ff.linear_distillation(x, w, ids.gather(1, order).int(), teacher.gather(1, order), temperature=tau, reduction=reduction)
         check(r, x, w, tau, other, {}, None, reduction)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize(("shape", "top"), [((1, 10, 64), 0), ((40, 300, 72), 5), ((64, 1000, 2056), 0), ((130, 20011, 72), 3), ((300, 1000, 768), 0), ((257, 777, 1096), 20), ((2048, 70001, 64), 0)])
+def test_a_bias(shape: tuple[int, int, int], top: int, dtype: str) -> None:
+    rows, vocab, dim = shape
+    x, w, y = layer(rows, vocab, dim, DTYPES[dtype])
+    bias = normal(vocab, dtype=DTYPES[dtype], seed=11)
+    y[::5] = -100
+    leaves = [t.detach().requires_grad_(True) for t in (x, w, bias)]
+    if top:
+        ids, teacher = integers(0, vocab, (rows, top), 6), normal(rows, top, seed=4)
+        ids[::5] = -1
+        call = lambda a, b, c: ff.linear_distillation(a, b, ids, teacher, bias=c, temperature=2.0)  # noqa: E731
+    else:
+        call = lambda a, b, c: ff.linear_cross_entropy(a, b, y, bias=c)  # noqa: E731
+    g = torch.tensor(1.5, device="cuda")
+    tau = 2.0 if top else 1.0
+    r = oracle.distillation(x, w, ids, teacher, 2.0, "mean", g, bias) if top else oracle.cross_entropy(x, w, y, -100, "mean", g, bias)
+    loss = call(*leaves)
+    grads = dict(zip(("dx", "dw", "db"), torch.autograd.grad(loss, leaves, g), strict=True))
+    check(r, x, w, tau, loss, grads, g, "mean", bias)
+    odd = torch.cat((bias[:1], bias))[1:].requires_grad_(True)  # two bytes off: copied; and its gradient alone
+    loss = call(x, w, odd)
+    check(r, x, w, tau, loss, {"db": torch.autograd.grad(loss, odd, g)[0]}, g, "mean", bias)
+    same = call(*leaves)
+    again = torch.autograd.grad(same, leaves[2], g)[0]
+    assert torch.equal(again, grads["db"])
+    with torch.no_grad():
+        assert torch.equal(call(*leaves), loss)
 
 
 def test_one_entry_is_cross_entropy() -> None:

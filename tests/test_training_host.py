@@ -97,7 +97,7 @@ def head_args(**kw: object) -> _lib.B200HeadArgs:
     a = _lib.B200HeadArgs()
     a.struct_size = ctypes.sizeof(a)
     a.dtype, a.rows, a.dim, a.vocab, a.top, a.reduction, a.target_bytes, a.tau, a.teacher_dtype = _lib.F16, 100, 64, 500, 0, 2, 8, 1.0, _lib.F32
-    a.x = a.w = a.targets = a.teacher = a.loss = a.state = a.workspace = a.grad = a.dx = a.dw = 0x10000
+    a.x = a.w = a.targets = a.teacher = a.loss = a.state = a.workspace = a.grad = a.dx = a.dw = a.bias = a.dbias = 0x10000
     a.ldx = a.ldw = 64
     a.state_bytes = a.workspace_bytes = 1 << 40
     for name, v in kw.items():
@@ -129,6 +129,7 @@ def head_args(**kw: object) -> _lib.B200HeadArgs:
         ({"ldx": 56}, _lib.UNSUPPORTED, "x: row stride"),
         ({"ldw": 68}, _lib.UNSUPPORTED, "w: row stride"),
         ({"ldx": 2**38}, _lib.UNSUPPORTED, "x: row stride"),
+        ({"bias": 0x10008}, _lib.UNSUPPORTED, "bias"),
         ({"state": 0x10010}, _lib.BAD_CONFIG, "state"),
         ({"state_bytes": 100}, _lib.BAD_CONFIG, "state"),
         ({"workspace": 0}, _lib.BAD_CONFIG, "workspace"),
@@ -151,9 +152,9 @@ def test_the_forward_call_looks_at_its_own(lib: ctypes.CDLL, kw: dict, word: str
 
 
 def test_the_gradient_call_looks_at_its_own(lib: ctypes.CDLL) -> None:
-    for kw in ({"grad": 0}, {"grad": 0x10002}, {"grad_stride": -1}, {"dx": 0x10008}, {"dw": 0x10008}):
+    for kw in ({"grad": 0}, {"grad": 0x10002}, {"grad_stride": -1}, {"dx": 0x10008}, {"dw": 0x10008}, {"dbias": 0x10008}):
         assert lib.b200_head_grad(ctypes.byref(head_args(**kw)), None) in (_lib.BAD_CONFIG, _lib.UNSUPPORTED)
-    assert lib.b200_head_grad(ctypes.byref(head_args(dx=0, dw=0)), None) == _lib.OK  # nothing asked for
+    assert lib.b200_head_grad(ctypes.byref(head_args(dx=0, dw=0, dbias=0)), None) == _lib.OK  # nothing asked for
     for call in (lib.b200_head_loss, lib.b200_head_grad):
         assert call(None, None) == _lib.BAD_CONFIG
 
@@ -212,6 +213,10 @@ def test_losses_refuse() -> None:
         lambda: ff.linear_cross_entropy(x, w[0], y),
         lambda: ff.linear_cross_entropy(x, w.cpu(), y),
         lambda: ff.linear_cross_entropy(x[:, :4], w[:, :4], y),
+        lambda: ff.linear_cross_entropy(x, w, y, bias=w[:, 0].float()),
+        lambda: ff.linear_cross_entropy(x, w, y, bias=x[:, 0]),
+        lambda: ff.linear_cross_entropy(x, w, y, bias=w[:, 0].cpu()),
+        lambda: ff.linear_distillation(x, w, ids, teacher, bias=w[:, :1]),
         lambda: ff.linear_cross_entropy(x, w, y[:3]),
         lambda: ff.linear_cross_entropy(x, w, y.float()),
         lambda: ff.linear_cross_entropy(x, w, y.cpu()),
