@@ -1262,9 +1262,9 @@ __global__ void __launch_bounds__(kLossThreads) head_loss_kernel(const HeadLossP
     for (int k = lane; k < p.top; k += 32) {
       const int64_t at = static_cast<int64_t>(src) * p.top + k;
       const float weight = p.p != nullptr ? __ldg(p.p + at) : 1.f;
-      // An entry that does not count has no weight, and its logit was never written. The maximum first: nothing is left of it where the entry is
-      // the maximum, and a small loss keeps its digits.
-      if (weight != 0.f) loss += weight * (((m - __ldg(p.picks + at) * p.log2_scale) + log2_s) * 0.693147180559945f);
+      // An entry that does not count has no weight, and its logit was never written. The maximum first, and the product unrounded, as it is behind the
+      // exponentials: where the entry is the maximum what is left is the maximum's own rounding, which the sum holds too, and a small loss keeps its digits.
+      if (weight != 0.f) loss += weight * ((fmaf(-__ldg(p.picks + at), p.log2_scale, m) + log2_s) * 0.693147180559945f);
     }
     loss = head_warp_sum(loss);
     if (p.entropy != nullptr) loss += __ldg(p.entropy + src);

@@ -180,6 +180,25 @@ def test_teachers_of_every_type_and_stride(teacher_type: torch.dtype) -> None:
     check(r, x, w, 1.0, want, {}, None, "none")
 
 
+@pytest.mark.parametrize("rows", [3, 300])
+def test_small_losses_keep_their_digits(rows: int) -> None:
+    """Logits of a single product are exact. The target's is the largest, of about 100, the others lie 4 to 20 below: losses of 1e-3 to 0.2. What is left is
+    fp32's error of a sum of about 1 (8 u: each half tile's, their sum's, the logarithm's), 2^-21 of the other terms (exponential and sums), and log2(e)'s
+    rounding, u of the distances that the terms have."""
+    x = torch.zeros(rows, 64, dtype=torch.bfloat16, device="cuda")
+    x[:, 0] = 8.0
+    w = torch.zeros(1000, 64, dtype=torch.bfloat16, device="cuda")
+    w[:, 0] = 10.0 + 1.5 * torch.rand(1000, generator=torch.Generator(device="cuda").manual_seed(3), device="cuda")
+    y = torch.zeros(rows, dtype=torch.int64, device="cuda")
+    w[0, 0] = 12.5
+    r = oracle.cross_entropy(x, w, y, -100, "none")
+    assert 1e-3 < float(r.rows.min()) < 0.2  # noqa: PLR2004
+    z = x.double() @ w.double().T
+    others = r.q[:, 1:].sum(1)
+    bound = 8 * F32 + 2.0**-21 * others + F32 * (r.q * (z - z[:, :1]).abs()).sum(1) + F32 * r.rows
+    near(ff.linear_cross_entropy(x, w, y, reduction="none"), r.rows, bound, "loss")
+
+
 def test_large_weights_of_the_vocabulary_in_several_pieces() -> None:
     """More columns than a piece holds, and a last piece that is nearly empty: dx is the sum of all pieces."""
     rows, vocab, dim = 4096, 32768 + 8 + 32768, 64
