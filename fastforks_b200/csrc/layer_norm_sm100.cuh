@@ -207,7 +207,8 @@ constexpr int kLnForwardRows = 4;  // rows of a CTA whose rows are a warp's each
 
 // Forward. THREADS of a row: 32 (four rows a CTA) or the CTA. A thread has N vectors, THREADS * VEC values apart; they go in pairs, which the packed
 // instructions take at once. us, value by value -> in pairs, and the time of the bytes: 8192 x 4096 in bf16 28.9 -> 24.3 (20.5), 21920 x 1024 17.9 -> 15.3
-// (13.7), 16384 x 2048 31.3 -> 26.4 (20.5); 8192 x 4096 in fp32 41.7 (41.0). 197 x 768: 2.8, the launch and a chain of latencies.
+// (13.7), 16384 x 2048 31.3 -> 26.4 (20.5); 8192 x 4096 in fp32 41.7 (41.0). Those are of one input again and again, part of which L2 holds; with several in turn
+// 27.9, 19.5, 27.9 and 43.2. 197 x 768: 2.8, the launch and a chain of latencies.
 template <typename T, int VEC, int N, int THREADS>
 __global__ void __launch_bounds__(THREADS == 32 ? 32 * kLnForwardRows : THREADS) norm_rows_kernel(const LayerNormParams p) {
   __shared__ float2 place[2][32];
@@ -382,8 +383,8 @@ __global__ void __launch_bounds__(THREADS == 32 ? 32 * kLnGradWarps : THREADS) n
 // instructions, and 8192 rows of 4096 54 us). us with the join, of bf16: a row a CTA with the next one in registers (norm_rows_grad_kernel) -> here, and
 // the time of the bytes: 8192 x 4096 75.0 -> 40.9 (30.8), 21920 x 1024 48.4 -> 30.8 (20.6), 30000 x 512 64.4 -> 20.5 (14.1), 300 x 4096 18.3 -> 7.8; fp32
 // 8192 x 4096 74.3 -> 67.7 (61.6), 5480 x 384 14.5 -> 8.9 (3.9). Bound by HBM at its mix of reads and writes and, at sixteen warps an SM, by the chain of
-// copy, sums and barrier of each row. The same for the forward pass was slower than rows in registers (8192 x 4096 29.2, 24.3 there): two barriers a
-// row, and nothing that has to stay. (Groups added one after the other into one place took 5 us more at 16 groups.)
+// copy, sums and barrier of each row. The same for the forward pass was slower than rows in registers but for the largest calls (several
+// inputs in turn: 1200 x 4096 10.1 against 7.6, 5000 x 4096 19.7 and 19.6, 10000 x 4096 30.7 and 32.8): two barriers a row, and nothing that has to stay. (Groups added one after the other into one place took 5 us more at 16 groups.)
 constexpr int kLnMostWarps = 16, kLnMostSlots = 16, kLnRingBytes = 208 * 1024;
 constexpr uint32_t kStatusNormWait = 1u << 24;
 // Warps of a CTA, one on each SM, as the registers of so many values a thread allow. (Two CTAs of eight warps leave twice as many parts to join.)
