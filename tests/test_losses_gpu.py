@@ -9,7 +9,10 @@ sums of it over V and T, in chains like a logit's, rounded once more.
 
 from __future__ import annotations
 
+import subprocess
+import sys
 import threading
+from pathlib import Path
 
 import pytest
 import torch
@@ -363,6 +366,45 @@ def test_the_gradients_may_be_asked_for_twice_and_from_another_thread() -> None:
     with pytest.raises(RuntimeError):
         dx = torch.autograd.grad(loss, x, create_graph=True)[0]
         torch.autograd.grad(dx.float().sum(), x)
+
+
+def test_gradients_are_the_first_thing_that_autograds_thread_does() -> None:
+    """Autograd runs them in a thread of its own, which has no context until it makes a CUDA call: a process whose first gradients these are."""
+    code = """
+import torch, fastforks_b200 as ff
+x, w = (torch.randn(n, 64, device="cuda").half().requires_grad_(True) for n in (300, 500))
+loss = ff.linear_cross_entropy(x, w, torch.zeros(300, dtype=torch.int64, device="cuda"))
+assert all(g.isfinite().all() for g in torch.autograd.grad(loss, (x, w)))
+assert ff.device_status() == 0
+"""
+    done = subprocess.run([sys.executable, "-c", code], cwd=Path(__file__).resolve().parent.parent, capture_output=True, text=True, timeout=300, check=False)
+    assert done.returncode == 0, done.stderr
+
+
+def test_a_single_row_without_a_batch() -> None:
+    x, w, y = layer(1, 50, 64, torch.bfloat16)
+    for reduction in ("none", "sum", "mean"):
+        for way in range(2):
+            leaf = x[0].detach().requires_grad_(True)
+            if way:  # two bytes off: copied
+                leaf = torch.cat((x[0, :1], x[0]))[1:].detach().requires_grad_(True)
+            loss = ff.linear_cross_entropy(leaf, w, y[0], reduction=reduction)
+            assert loss.shape == ()
+            (dx,) = torch.autograd.grad(loss, leaf)
+            g = torch.ones(1, device="cuda")
+            r = oracle.cross_entropy(x, w, y, -100, "none", g)
+            check(r, x, w, 1.0, loss.reshape(1), {"dx": dx.reshape(1, 64)}, g, "none")
+
+
+def test_rows_whose_offsets_pass_32_bits() -> None:
+    if torch.cuda.mem_get_info()[0] < 6 * 2**30:
+        pytest.skip("no room")
+    x, w, y = layer(70, 300, 64, torch.float16)
+    stride = 2**25 + 8
+    far = torch.zeros(70 * stride, dtype=torch.float16, device="cuda").as_strided((70, 64), (stride, 1))
+    far.copy_(x)
+    y[::4] = -100
+    assert torch.equal(ff.linear_cross_entropy(far, w, y, reduction="none"), ff.linear_cross_entropy(x, w, y, reduction="none"))
 
 
 def test_a_stream_and_two_graphs_at_once() -> None:
