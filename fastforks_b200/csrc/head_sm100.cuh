@@ -13,7 +13,7 @@
 //   head_rows_kernel     which rows count, where they go, their copy
 //   head_stats_kernel    logits of 256 x bn tiles in tensor memory; leaves a maximum and a sum of exponentials per row and half
 //                        of a tile's columns, and the logits of the row's entries
-//   head_few_kernel      the same of up to 256 rows
+//   head_few_kernel      the same of up to 64 rows
 //   head_loss_kernel     joins those to lse and loss
 //   head_coef_kernel     gradients that differ from row to row: one power of two for all
 //   head_grads_kernel    a piece of the vocabulary: the logits again, their gradient in 16 bits
@@ -23,7 +23,7 @@
 //
 // Bound by the tensor cores: 2 T D V operations forward, 6 T D V more for the gradients, 2 T D V of which compute the logits again
 // instead of keeping them. The products are those of CTA pairs (cta_group::2, plain TMA loads, 256 x 256 tiles, two accumulators
-// in tensor memory); head_products() below is the one pipeline that all three run on.
+// in tensor memory); head_products() below is the one pipeline that statistics, gradients of logits and sums run on.
 #pragma once
 
 #include <cuda_bf16.h>
@@ -300,9 +300,8 @@ __device__ __forceinline__ void head_add_bias(float (&v)[32], const void* bias, 
   }
 }
 
-// G = 2^s coef_t (softmax(z_t) - p) is held in 16 bits, the operands' type: its rounding is that of an operand, 2^-9 (fp16 2^-12) of a value on
-// average below half a step, and as large in dx and dw as the rounding of their result. s = 15 for fp16, whose smallest normal
-// number is 2^-14: a softmax of 2^-29 keeps all its bits; bfloat16 has fp32's range, s = 0. Over many rows that adds up to 1.1 to 1.45 times the error that
+// G = 2^s coef_t (softmax(z_t) - p) is held in 16 bits, the operands' type: off by half a step at most, 2^-8 of a value (fp16 2^-11). s = 15 for
+// fp16, whose smallest normal number is 2^-14: a softmax of 2^-29 keeps all its bits; bfloat16 has fp32's range, s = 0. Over many rows that adds up to 1.1 to 1.45 times the error that
 // the results' own rounding has; of a few rows each hangs on one or two roundings, and 1.7 times came out. Few rows and small products (head_grad_work in
 // b200_training.cu) therefore keep what the rounding took, in as many rows more, and both go through the products: the error is that of the results' rounding.
 template <typename T, bool GRADS>
