@@ -3,6 +3,7 @@
 
 #include <algorithm>
 #include <cmath>
+#include <iterator>
 
 #include "../../include/b200_attn.h"
 #include "head_sm100.cuh"
@@ -18,29 +19,38 @@ struct NormForm {
   const void* kernel;
   int threads;  // of a row
   int vectors, vec;
+  int rows = 1;                   // at a time
+  int from = 0, below = 1 << 30;  // rows of the call for each SM
 };
 
-// The fewest threads a row that leave each at most so many vectors. A warp has a row up to 1024 16-bit values (four vectors a lane): no
-// barrier; then the CTA has one.
-template <typename T, int VEC, int N, int THREADS>
-NormForm forward_form() { return {reinterpret_cast<const void*>(norm_rows_kernel<T, VEC, N, THREADS>), THREADS, N, VEC}; }
+// The first that holds the row and is for so many rows. us of bf16 with several inputs in turn (threads x vectors; two: two rows at a time):
+//   2400 x 1024  32 x 4 5.9, 64 x 2 two 4.4      1200 x 1024  32 x 4 5.4, 64 x 2 3.6      19200 x 1024  32 x 4 18.1, 64 x 2 two 16.5
+//   2400 x 2048  128 x 2 7.6, two 6.1            9600 x 2048  128 x 2 18.0, two 16.9
+//    600 x 4096  128 x 4 6.7, 256 x 2 4.7        1200 x 4096  128 x 4 7.8, 256 x 2 8.0    9600 x 4096   128 x 4 32.0, two 30.6
+//   9600 x 512   32 x 2 6.9, two 5.7
+// Few rows want many threads each, many rows few of them and more bytes in flight. Up to 768 values a warp has a row, without a barrier (two at a time were 3 %
+// faster at 19200 x 768 and slower below).
+template <typename T, int VEC, int N, int THREADS, int ROWS = 1>
+NormForm forward_form(int from = 0, int below = 1 << 30) { return {reinterpret_cast<const void*>(norm_rows_kernel<T, VEC, N, THREADS, ROWS>), THREADS, N, VEC, ROWS, from, below}; }
 template <typename T>
 const NormForm* forward_forms(bool wide_rows, int* count) {
   static const NormForm values[] = {forward_form<T, 1, 1, 32>(), forward_form<T, 1, 4, 32>(), forward_form<T, 1, 8, 32>(), forward_form<T, 1, 4, 256>(), forward_form<T, 1, 8, 256>(),
                                     forward_form<T, 1, 16, 256>(), forward_form<T, 1, 16, 1024>(), forward_form<T, 1, 32, 1024>()};
   if (!wide_rows) {
-    *count = 8;
+    *count = static_cast<int>(std::size(values));
     return values;
   }
   if constexpr (sizeof(T) == 2) {
-    static const NormForm vectors[] = {forward_form<T, 8, 1, 32>(), forward_form<T, 8, 2, 32>(), forward_form<T, 8, 3, 32>(), forward_form<T, 8, 4, 32>(), forward_form<T, 8, 2, 128>(),
-                                       forward_form<T, 8, 4, 128>(), forward_form<T, 8, 3, 256>(), forward_form<T, 8, 4, 256>(), forward_form<T, 8, 4, 512>(), forward_form<T, 8, 4, 1024>()};
-    *count = 10;
+    static const NormForm vectors[] = {forward_form<T, 8, 1, 32>(), forward_form<T, 8, 2, 32>(0, 64), forward_form<T, 8, 2, 32, 2>(64), forward_form<T, 8, 3, 32>(),
+                                       forward_form<T, 8, 2, 64>(0, 16), forward_form<T, 8, 2, 64, 2>(16), forward_form<T, 8, 2, 128>(0, 16), forward_form<T, 8, 2, 128, 2>(16),
+                                       forward_form<T, 8, 2, 256>(0, 8), forward_form<T, 8, 4, 128>(8, 32), forward_form<T, 8, 4, 128, 2>(32), forward_form<T, 8, 3, 256>(),
+                                       forward_form<T, 8, 4, 256>(), forward_form<T, 8, 4, 512>(), forward_form<T, 8, 4, 1024>()};
+    *count = static_cast<int>(std::size(vectors));
     return vectors;
   } else {
     static const NormForm vectors[] = {forward_form<T, 4, 1, 32>(), forward_form<T, 4, 2, 32>(), forward_form<T, 4, 3, 32>(), forward_form<T, 4, 4, 32>(), forward_form<T, 4, 2, 128>(),
                                        forward_form<T, 4, 3, 128>(), forward_form<T, 4, 4, 128>(), forward_form<T, 4, 4, 256>(), forward_form<T, 4, 4, 512>(), forward_form<T, 4, 4, 1024>(), forward_form<T, 4, 8, 1024>()};
-    *count = 11;
+    *count = static_cast<int>(std::size(vectors));
     return vectors;
   }
 }
@@ -52,27 +62,28 @@ const NormForm* grad_forms(bool wide_rows, int* count) {
   static const NormForm values[] = {grad_form<T, 1, 1, 32>(), grad_form<T, 1, 4, 32>(), grad_form<T, 1, 8, 32>(), grad_form<T, 1, 8, 128>(), grad_form<T, 1, 16, 128>(),
                                     grad_form<T, 1, 16, 256>(), grad_form<T, 1, 16, 512>(), grad_form<T, 1, 16, 1024>(), grad_form<T, 1, 32, 1024>()};
   if (!wide_rows) {
-    *count = 9;
+    *count = static_cast<int>(std::size(values));
     return values;
   }
   if constexpr (sizeof(T) == 2) {
     static const NormForm vectors[] = {grad_form<T, 8, 2, 1024>(), grad_form<T, 8, 4, 1024>()};
-    *count = 2;
+    *count = static_cast<int>(std::size(vectors));
     return vectors;
   } else {
     static const NormForm vectors[] = {grad_form<T, 4, 4, 512>(), grad_form<T, 4, 4, 1024>(), grad_form<T, 4, 8, 1024>()};
-    *count = 3;
+    *count = static_cast<int>(std::size(vectors));
     return vectors;
   }
 }
-NormForm norm_form(const B200LayerNormArgs& a, bool grad, bool wide_rows) {
+NormForm norm_form(const B200LayerNormArgs& a, bool grad, bool wide_rows, int sms) {
   int n = 0;
   const NormForm* f = nullptr;
   if (a.dtype == B200_ATTN_F16) f = grad ? grad_forms<__half>(wide_rows, &n) : forward_forms<__half>(wide_rows, &n);
   else if (a.dtype == B200_ATTN_BF16) f = grad ? grad_forms<__nv_bfloat16>(wide_rows, &n) : forward_forms<__nv_bfloat16>(wide_rows, &n);
   else f = grad ? grad_forms<float>(wide_rows, &n) : forward_forms<float>(wide_rows, &n);
+  const int64_t each = a.rows / sms;
   int i = 0;
-  while (i < n - 1 && f[i].threads * f[i].vectors * f[i].vec < a.dim) ++i;
+  while (i < n - 1 && (f[i].threads * f[i].vectors * f[i].vec < a.dim || each < f[i].from || each >= f[i].below)) ++i;
   return f[i];
 }
 
@@ -88,11 +99,11 @@ template <typename T>
 const RingForm* ring_forms(int* count) {
   if constexpr (sizeof(T) == 2) {
     static const RingForm forms[] = {ring_form<T, 1, 1>(), ring_form<T, 2, 1>(), ring_form<T, 2, 2>(), ring_form<T, 2, 4>(), ring_form<T, 2, 8>(), ring_form<T, 3, 8>(), ring_form<T, 4, 8>()};
-    *count = 7;
+    *count = static_cast<int>(std::size(forms));
     return forms;
   } else {
     static const RingForm forms[] = {ring_form<T, 1, 1>(), ring_form<T, 2, 1>(), ring_form<T, 3, 1>(), ring_form<T, 4, 1>(), ring_form<T, 3, 2>(), ring_form<T, 4, 2>(), ring_form<T, 3, 4>(), ring_form<T, 4, 4>(), ring_form<T, 4, 8>()};
-    *count = 9;
+    *count = static_cast<int>(std::size(forms));
     return forms;
   }
 }
@@ -633,8 +644,10 @@ int b200_layer_norm(const B200LayerNormArgs* a, void* stream_ptr) {
   p.y = a->y;
   p.y_stride = a->y_stride;
   p.b = a->bias;
-  const NormForm f = norm_form(*a, false, wide);
-  const int64_t ctas = f.threads == 32 ? (a->rows + kLnForwardRows - 1) / kLnForwardRows : a->rows;
+  DeviceState* dev = nullptr;
+  if (int rc = device_state(&dev)) return rc;
+  const NormForm f = norm_form(*a, false, wide, dev->sms);
+  const int64_t each = (f.threads == 32 ? kLnForwardRows : 1) * f.rows, ctas = (a->rows + each - 1) / each;
   void* args[] = {&p};
   if (int rc = launch_kernel(f.kernel, static_cast<unsigned>(ctas), 1, f.threads == 32 ? 32 * kLnForwardRows : f.threads, 0, 1, static_cast<cudaStream_t>(stream_ptr), args, "layer_norm kernel launch")) return rc;
   clear_error();
@@ -648,7 +661,7 @@ int b200_layer_norm_workspace(const B200LayerNormArgs* a, int64_t* bytes) {
   if (int rc = device_state(&dev)) return rc;
   *bytes = 0;  // of whichever form the addresses lead to
   for (const bool wide : {false, true}) {
-    *bytes = std::max<int64_t>(*bytes, 8LL * a->dim * grad_ctas(*a, norm_form(*a, true, wide), dev->sms));
+    *bytes = std::max<int64_t>(*bytes, 8LL * a->dim * grad_ctas(*a, norm_form(*a, true, wide, dev->sms), dev->sms));
     *bytes = std::max<int64_t>(*bytes, 8LL * a->dim * ring_plan(*a, wide && whole_words(*a), dev->sms).ctas);
   }
   clear_error();
@@ -672,7 +685,7 @@ int b200_layer_norm_grad(const B200LayerNormArgs* a, void* stream_ptr) {
   if (int rc = device_state(&dev)) return rc;
   const RingPlan ring = ring_plan(*a, wide, dev->sms);
   const bool through = ring.form.kernel != nullptr;
-  const NormForm f = norm_form(*a, true, wide);
+  const NormForm f = norm_form(*a, true, wide, dev->sms);
   const int ctas = through ? ring.ctas : grad_ctas(*a, f, dev->sms);
   const bool want_dw = a->dweight != nullptr || a->dbias != nullptr;
   if (want_dw && (a->workspace == nullptr || !aligned16(a->workspace) || a->workspace_bytes < 8LL * a->dim * ctas))

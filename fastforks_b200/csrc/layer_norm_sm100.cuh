@@ -205,54 +205,74 @@ __device__ __forceinline__ float2 ln_row_sum2(float2 v, float2 (*place)[32], int
 
 constexpr int kLnForwardRows = 4;  // rows of a CTA whose rows are a warp's each
 
-// Forward. THREADS of a row: 32 (four rows a CTA) or the CTA. A thread has N vectors, THREADS * VEC values apart; they go in pairs, which the packed
-// instructions take at once. us, value by value -> in pairs, and the time of the bytes: 8192 x 4096 in bf16 28.9 -> 24.3 (20.5), 21920 x 1024 17.9 -> 15.3
-// (13.7), 16384 x 2048 31.3 -> 26.4 (20.5); 8192 x 4096 in fp32 41.7 (41.0). Those are of one input again and again, part of which L2 holds; with several in turn
-// 27.9, 19.5, 27.9 and 43.2. 197 x 768: 2.8, the launch and a chain of latencies.
-template <typename T, int VEC, int N, int THREADS>
+// Forward. THREADS of a row: 32 (four rows a CTA) or the CTA; ROWS rows at a time, which share weights and barriers (forward_forms in b200_training.cu).
+// A thread has N vectors, THREADS * VEC values apart; they go in pairs, which the packed instructions take at once. us, value by value -> in pairs, one row at a
+// time and one input again and again (part of it in L2): 8192 x 4096 in bf16 28.9 -> 24.3, 21920 x 1024 17.9 -> 15.3. Now, several inputs in turn, and the time of
+// the bytes: 8192 x 4096 27.3 (20.5), 21920 x 1024 18.2 (13.7), 16384 x 2048 25.7 (20.5), 21920 x 768 in fp16 16.0 (10.3), 8192 x 4096 in fp32 43.0 (41.0).
+// 197 x 768: 2.7, the launch and a chain of latencies.
+template <typename T, int VEC, int N, int THREADS, int ROWS>
 __global__ void __launch_bounds__(THREADS == 32 ? 32 * kLnForwardRows : THREADS) norm_rows_kernel(const LayerNormParams p) {
   __shared__ float2 place[2][32];
   grid_dependency_wait();
   grid_launch_dependents();
-  const int64_t row = THREADS == 32 ? static_cast<int64_t>(blockIdx.x) * kLnForwardRows + (threadIdx.x >> 5) : blockIdx.x;
-  if (row >= p.rows) return;  // (a whole warp, where rows are warps'; never where they are CTAs')
-  constexpr int kStep = THREADS * VEC, kPairs = VEC > 1 ? VEC / 2 : 1;
+  constexpr int kStep = THREADS * VEC, kPairs = VEC > 1 ? VEC / 2 : 1, kWarpRows = THREADS == 32 ? kLnForwardRows : 1;
+  const int64_t row0 = static_cast<int64_t>(blockIdx.x) * kWarpRows * ROWS + (THREADS == 32 ? threadIdx.x >> 5 : 0);  // and kWarpRows further on
+  if (row0 >= p.rows) return;  // (a whole warp, where rows are warps'; never where they are CTAs')
   const int at = (threadIdx.x & (THREADS - 1)) * VEC;
-  const T* const x = static_cast<const T*>(p.x) + row * p.x_stride;
-  LnVec<T, VEC> raw[N];
+  const auto there = [&](int k) { return k == 0 || row0 + kWarpRows < p.rows; };
+  LnVec<T, VEC> raw[ROWS][N];
 #pragma unroll
-  for (int i = 0; i < N; ++i)
-    if (at + i * kStep < p.dim) raw[i] = ln_load<T, VEC>(x + at + i * kStep);
-  // Kept as it came, and converted at each of three uses: held as fp32, it cost warps (8192 x 4096 in bf16 34.7 us; so 24.3).
+  for (int k = 0; k < ROWS; ++k)
+#pragma unroll
+    for (int i = 0; i < N; ++i)
+      if (at + i * kStep < p.dim && there(k)) raw[k][i] = ln_load<T, VEC>(static_cast<const T*>(p.x) + (row0 + k * kWarpRows) * p.x_stride + at + i * kStep);
+  // Kept as it came, and converted at each of three uses: held as fp32, it cost warps (8192 x 4096 in bf16, one row at a time, 34.7 us; so 24.3).
   // A single value is a pair whose second half does not count.
-  const auto pair = [&](int i, int j) {
-    if constexpr (VEC > 1) return ln_pair<T>(*reinterpret_cast<const uint4*>(&raw[i]), j);
-    else return make_float2(ln_float(raw[i].v[0]), 0.f);
+  const auto pair = [&](int k, int i, int j) {
+    if constexpr (VEC > 1) return ln_pair<T>(*reinterpret_cast<const uint4*>(&raw[k][i]), j);
+    else return make_float2(ln_float(raw[k][i].v[0]), 0.f);
   };
   int turn = 0;
-  float2 s = make_float2(0.f, 0.f);
+  const auto row_sums = [&](const float2 (&s)[ROWS]) {
+    if constexpr (ROWS == 1) return make_float2(ln_row_sum<THREADS>(s[0].x + s[0].y, place, turn), 0.f);
+    else return ln_row_sum2<THREADS>(make_float2(s[0].x + s[0].y, s[1].x + s[1].y), place, turn);
+  };
+  float2 s[ROWS];
 #pragma unroll
-  for (int i = 0; i < N; ++i)
-    if (at + i * kStep < p.dim) {
+  for (int k = 0; k < ROWS; ++k) {
+    s[k] = make_float2(0.f, 0.f);
 #pragma unroll
-      for (int j = 0; j < kPairs; ++j) s = fadd2(s, pair(i, j));
-    }
-  const float mean = ln_mean(ln_row_sum<THREADS>(s.x + s.y, place, turn), static_cast<float>(p.dim), p.inverse_dim);
-  const float2 minus = make_float2(-mean, VEC > 1 ? -mean : 0.f);
-  float2 q = make_float2(0.f, 0.f);  // of the differences: no cancellation where the mean is large
+    for (int i = 0; i < N; ++i)
+      if (at + i * kStep < p.dim) {
 #pragma unroll
-  for (int i = 0; i < N; ++i)
-    if (at + i * kStep < p.dim) {
-#pragma unroll
-      for (int j = 0; j < kPairs; ++j) {
-        const float2 d = fadd2(pair(i, j), minus);
-        q = ffma2(d, d, q);
+        for (int j = 0; j < kPairs; ++j) s[k] = fadd2(s[k], pair(k, i, j));
       }
-    }
-  const float r = rsqrtf(ln_row_sum<THREADS>(q.x + q.y, place, turn) * p.inverse_dim + p.eps);
-  if (p.stats != nullptr && at == 0) p.stats[row] = make_float2(mean, r);
-  T* const y = static_cast<T*>(p.y) + row * p.y_stride;
-  const float2 r2 = make_float2(r, r);
+  }
+  const float2 sums = row_sums(s);
+  float2 minus[ROWS];
+#pragma unroll
+  for (int k = 0; k < ROWS; ++k) {
+    const float mean = ln_mean(k == 0 ? sums.x : sums.y, static_cast<float>(p.dim), p.inverse_dim);
+    minus[k] = make_float2(-mean, VEC > 1 ? -mean : 0.f);
+    s[k] = make_float2(0.f, 0.f);  // of the differences: no cancellation where the mean is large
+#pragma unroll
+    for (int i = 0; i < N; ++i)
+      if (at + i * kStep < p.dim) {
+#pragma unroll
+        for (int j = 0; j < kPairs; ++j) {
+          const float2 d = fadd2(pair(k, i, j), minus[k]);
+          s[k] = ffma2(d, d, s[k]);
+        }
+      }
+  }
+  const float2 squares = row_sums(s);
+  float2 r2[ROWS];
+#pragma unroll
+  for (int k = 0; k < ROWS; ++k) {
+    const float r = rsqrtf((k == 0 ? squares.x : squares.y) * p.inverse_dim + p.eps);
+    r2[k] = make_float2(r, r);
+    if (p.stats != nullptr && at == 0 && there(k)) p.stats[row0 + k * kWarpRows] = make_float2(-minus[k].x, r);
+  }
 #pragma unroll
   for (int i = 0; i < N; ++i) {
     const int c = at + i * kStep;
@@ -261,9 +281,15 @@ __global__ void __launch_bounds__(THREADS == 32 ? 32 * kLnForwardRows : THREADS)
       ln_weight_pairs<T, VEC>(p.w, c, p.wide != 0, 1.f, w);
       ln_weight_pairs<T, VEC>(p.b, c, p.wide != 0, 0.f, b);
 #pragma unroll
-      for (int j = 0; j < kPairs; ++j) w[j] = ffma2(fmul2(fadd2(pair(i, j), minus), r2), w[j], b[j]);
-      if constexpr (VEC > 1) *reinterpret_cast<uint4*>(y + c) = ln_packed<T>(w);
-      else y[c] = ln_round<T>(w[0].x);
+      for (int k = 0; k < ROWS; ++k) {
+        if (!there(k)) continue;
+        T* const y = static_cast<T*>(p.y) + (row0 + k * kWarpRows) * p.y_stride + c;
+        float2 v[kPairs];
+#pragma unroll
+        for (int j = 0; j < kPairs; ++j) v[j] = ffma2(fmul2(fadd2(pair(k, i, j), minus[k]), r2[k]), w[j], b[j]);
+        if constexpr (VEC > 1) *reinterpret_cast<uint4*>(y) = ln_packed<T>(v);
+        else *y = ln_round<T>(v[0].x);
+      }
     }
   }
 }

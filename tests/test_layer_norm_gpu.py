@@ -88,6 +88,17 @@ def test_forward_and_gradients(shape: tuple[int, int], dtype: str) -> None:
         assert torch.equal(same, y)
 
 
+@pytest.mark.parametrize(("rows", "dim"), [(9601, 504), (2401, 776), (4801, 1024), (2401, 2040), (1201, 2056), (1201, 4096), (4801, 2600), (4801, 4096)])
+def test_many_rows(rows: int, dim: int) -> None:  # odd: the last has no other to go with, where rows go two at a time
+    x, w, b = normal(rows, dim, dtype=torch.bfloat16, seed=dim), normal(dim, dtype=torch.bfloat16, seed=1), normal(dim, dtype=torch.bfloat16, seed=2)
+    y = torch.full((rows + 3, dim), 7.0, dtype=torch.bfloat16, device="cuda")
+    ff.layer_norm(x, w, b, eps=EPS, out=y[:rows])
+    assert bool((y[rows:] == 7.0).all())  # noqa: PLR2004
+    check(x, w, b, y[:rows])
+    same = x.clone()
+    assert torch.equal(ff.layer_norm(same, w, b, eps=EPS, out=same), y[:rows])
+
+
 @pytest.mark.parametrize("wanted", [(1, 0, 0), (0, 1, 0), (0, 0, 1), (0, 1, 1), (1, 0, 1), (1, 1, 0)])
 @pytest.mark.parametrize("dim", [72, 768, 1500])
 def test_only_the_gradients_that_are_asked_for(dim: int, wanted: tuple[int, int, int]) -> None:
