@@ -308,8 +308,9 @@ struct HeadGradWork {
   int64_t slot_rows;  // rows of G and of a part of dx
   int64_t g_rows;     // with those of what G's rounding took
   int cols;           // columns of G
-  int splits, sums_bn;
-  int64_t g, sums, coef, norm, bytes;
+  int splits, dw_splits, sums_bn;
+  int64_t dw_slot_rows;
+  int64_t g, sums, dw_sums, coef, norm, bytes;
 };
 HeadGradWork head_grad_work(const B200HeadArgs& a, bool want_dx, bool want_dw, int pairs) {
   HeadGradWork w{};
@@ -320,24 +321,31 @@ HeadGradWork head_grad_work(const B200HeadArgs& a, bool want_dx, bool want_dw, i
   w.cols = static_cast<int>(up((a.vocab + pieces - 1) / pieces, 256));
   w.sums_bn = a.dim > 128 ? 256 : 128;
   const int64_t col_tiles = (a.dim + w.sums_bn - 1) / w.sums_bn, tiles = w.slot_rows / 256 * col_tiles;
-  // Parts of k that dx is summed over: what gives the shortest longest list, in k-blocks of 64 (0.3 us). A tile of dx costs some four more
-  // for its fp32 sums, and every part a pass over them.
-  const int64_t k_blocks = (std::min<int64_t>(a.vocab, w.cols) + 63) / 64, row_blocks = (a.rows + 63) / 64;
-  const double short_work = want_dw ? static_cast<double>(w.cols / 256) * static_cast<double>(col_tiles * row_blocks) : 0.;
+  // Parts of k that dx and dw are summed over: what gives the shortest longest list, in k-blocks of 64 (0.3 us). A tile of fp32 sums costs some four
+  // more, every part a pass over them, and dw's (only where a piece is all of the vocabulary: they are not added to) a launch where dx does not have it.
+  const int64_t twice = w.g_rows / w.slot_rows, k_blocks = (std::min<int64_t>(a.vocab, w.cols) + 63) / 64, row_blocks = (a.rows + 63) / 64;
+  const int64_t dw_tiles = want_dw ? w.cols / 256 * col_tiles : 0, most_dx = want_dx ? std::min<int64_t>(32, k_blocks) : 1, most_dw = want_dw && pieces == 1 ? std::min<int64_t>(32, row_blocks) : 1;
   double best = 1e300;
-  for (int64_t s = 1; want_dx && s <= std::min<int64_t>(32, k_blocks); ++s) {
-    const double rounds = static_cast<double>((tiles * s + pairs - 1) / pairs), each = static_cast<double>((k_blocks + s - 1) / s) + 4.;
-    const double even = (static_cast<double>(tiles * s) * each + short_work) / pairs + (want_dw ? 0.5 * static_cast<double>(row_blocks) : 0.);
-    const double pass = static_cast<double>(s * a.rows) * a.dim * 8. / 6.5e6 / 0.3;  // written and read
-    const double cost = std::max(rounds * each, even) + pass;
-    if (cost < best) {
-      best = cost;
-      w.splits = static_cast<int>(s);
+  for (int64_t sw = 1; sw <= most_dw; ++sw) {
+    const double short_each = static_cast<double>((row_blocks * twice + sw - 1) / sw) + (sw > 1 ? 4. : 0.), short_work = static_cast<double>(dw_tiles * sw) * short_each;
+    const double short_pass = sw > 1 ? static_cast<double>(sw * a.vocab) * a.dim * 8. / 6.5e6 / 0.3 + 0.3 * static_cast<double>(sw) + (want_dx ? 0. : 8.) : 0.;
+    for (int64_t s = 1; s <= most_dx; ++s) {
+      const double rounds = want_dx ? static_cast<double>((tiles * s + pairs - 1) / pairs) : 0., each = static_cast<double>((k_blocks * twice + s - 1) / s) + 4.;
+      const double even = ((want_dx ? static_cast<double>(tiles * s) * each : 0.) + short_work) / pairs + (want_dw ? 0.5 * short_each : 0.);
+      const double pass = want_dx ? static_cast<double>(s * a.rows) * a.dim * 8. / 6.5e6 / 0.3 : 0.;  // written and read
+      const double cost = std::max({rounds * each, even, want_dw ? short_each : 0.}) + pass + short_pass;
+      if (cost < best) {
+        best = cost;
+        w.splits = want_dx ? static_cast<int>(s) : 0;
+        w.dw_splits = static_cast<int>(sw);
+      }
     }
   }
+  w.dw_slot_rows = up(a.vocab, 256);
   Layout l;
   w.g = l.add(w.g_rows * w.cols * 2);
   w.sums = l.add(w.splits * w.slot_rows * a.dim * 4);
+  w.dw_sums = l.add(w.dw_splits > 1 ? w.dw_splits * w.dw_slot_rows * a.dim * 4 : 0);
   w.coef = l.add(4LL * a.rows);
   w.norm = l.add(4);
   w.bytes = l.bytes;
@@ -542,8 +550,12 @@ int launch_grad(const B200HeadArgs& a, cudaStream_t stream) {
   dx = dw = g_out;
   if (want_dx)
     if (int rc = head_map(&dx, at<void>(a.workspace, w.sums), B200_ATTN_F32, w.splits * w.slot_rows, a.dim, a.dim, 32, 32, "workspace")) return rc;
-  if (want_dw)
+  const bool dw_parts = want_dw && w.dw_splits > 1;
+  if (dw_parts) {
+    if (int rc = head_map(&dw, at<void>(a.workspace, w.dw_sums), B200_ATTN_F32, w.dw_splits * w.dw_slot_rows, a.dim, a.dim, 32, 32, "workspace")) return rc;
+  } else if (want_dw) {
     if (int rc = head_map(&dw, a.dw, a.dtype, a.vocab, a.dim, a.dim, 64, 32, "dw")) return rc;
+  }
   const void* grads = f16 ? reinterpret_cast<const void*>(head_grads_kernel<__half>) : reinterpret_cast<const void*>(head_grads_kernel<__nv_bfloat16>);
   const void* sums = f16 ? reinterpret_cast<const void*>(head_sums_kernel<__half>) : reinterpret_cast<const void*>(head_sums_kernel<__nv_bfloat16>);
   if (int rc = opt_in(grads, f16 ? 2 : 3, kHeadSmemBytes)) return rc;
@@ -580,6 +592,8 @@ int launch_grad(const B200HeadArgs& a, cudaStream_t stream) {
   q.dim = a.dim;
   q.vocab = a.vocab;
   q.want_dw = want_dw;
+  q.dw_splits = w.dw_splits;
+  q.dw_slot_rows = static_cast<int>(w.dw_slot_rows);
   q.bn = w.sums_bn;
   q.stages = ring_stages(w.sums_bn);
   q.slot_rows = w.slot_rows;
@@ -597,7 +611,7 @@ int launch_grad(const B200HeadArgs& a, cudaStream_t stream) {
     q.cols = cols;
     q.first = v0 == 0;
     q.splits = std::min(w.splits, (cols + 63) / 64);  // a part without a k-block would never finish; the first piece has one for each
-    const int64_t items = row_tiles * col_tiles * q.splits + (want_dw ? static_cast<int64_t>((cols + 255) / 256) * col_tiles : 0);
+    const int64_t items = row_tiles * col_tiles * q.splits + (want_dw ? static_cast<int64_t>((cols + 255) / 256) * col_tiles * w.dw_splits : 0);
     if (want_db) {
       HeadDbParams d{p.count, g, w.cols, p.rest_at, v0, cols, a.vocab, a.dbias, scale};
       void* db_args[] = {&d};
@@ -608,17 +622,24 @@ int launch_grad(const B200HeadArgs& a, cudaStream_t stream) {
     void* sums_args[] = {&g_k, &g_mn, &w_mn, &x_mn, &copy_mn, &dx, &dw, &q};
     if (int rc = launch_kernel(sums, static_cast<unsigned>(2 * std::min<int64_t>(items, pairs)), 1, kHeadThreads, kHeadSmemBytes, 2, stream, sums_args, "head_sums kernel launch")) return rc;
   }
-  if (!want_dx) return B200_ATTN_OK;
+  if (!want_dx && !dw_parts) return B200_ATTN_OK;
   HeadDxParams d{};
   d.sums = at<float>(a.workspace, w.sums);
   d.splits = w.splits;
   d.slot_rows = w.slot_rows;
-  d.rows = a.rows;
+  d.rows = want_dx ? a.rows : 0;
+  d.dw_sums = at<float>(a.workspace, w.dw_sums);
+  d.dw_splits = w.dw_splits;
+  d.dw_slot_rows = static_cast<int>(w.dw_slot_rows);
+  d.vocab = dw_parts ? a.vocab : 0;
+  d.twice = p.rest_at > 0 ? 2 : 1;
+  d.count = p.count;
+  d.dw = a.dw;
   d.dim = a.dim;
   d.place = at<int>(a.state, s.place);
   d.dx = a.dx;
   d.scale = scale;
-  const int64_t words = static_cast<int64_t>(a.rows) * (a.dim / 8);
+  const int64_t words = static_cast<int64_t>(d.rows + d.vocab) * (a.dim / 8);
   const void* kernel = f16 ? reinterpret_cast<const void*>(head_dx_kernel<__half>) : reinterpret_cast<const void*>(head_dx_kernel<__nv_bfloat16>);
   void* args[] = {&d};
   return launch_kernel(kernel, static_cast<unsigned>(std::min<int64_t>((words + kDxThreads - 1) / kDxThreads, 8LL * dev->sms)), 1, kDxThreads, 0, 1, stream, args, "head_dx kernel launch");

@@ -19,7 +19,7 @@
 //   head_grads_kernel    a piece of the vocabulary: the logits again, their gradient in 16 bits
 //   head_sums_kernel     dx += G w and dw = G^T x of that piece in one launch
 //   head_db_kernel       dbias of that piece
-//   head_dx_kernel       sums of dx, which are held in fp32, rounded and put where their rows came from
+//   head_dx_kernel       sums of dx (and of dw in parts), which are held in fp32, rounded; rows of dx put where they came from
 //
 // Bound by the tensor cores: 2 T D V operations forward, 6 T D V more for the gradients, 2 T D V of which compute the logits again
 // instead of keeping them. The products are those of CTA pairs (cta_group::2, plain TMA loads, 256 x 256 tiles, two accumulators
@@ -793,12 +793,17 @@ __device__ __forceinline__ float head_scale(const HeadScale& s) {
   return v;
 }
 
+// Parts that dw is summed over: none without a k-block, whose product would never finish.
+__device__ __forceinline__ int head_dw_parts(int rows, int twice, int splits) { return min(splits, max(1, (rows + 63) / 64) * twice); }
+
 struct HeadSumsParams {
   const int* count;
   int all_rows, dim, vocab;
   int v0, cols;       // the piece: columns v0 .. v0 + cols - 1, cols a multiple of 256 or up to the last
   int splits;         // parts of the piece's columns that dx is summed over, 0: no dx
   int want_dw;
+  int dw_splits;      // parts of the rows that dw is summed over; more than one, where a piece is all of the vocabulary: fp32 sums in place of dw
+  int dw_slot_rows;   // rows of a part of those
   int bn, stages;
   int first;          // the first piece: dx begins
   int rest_at;        // see HeadLogitsParams
@@ -808,17 +813,20 @@ struct HeadSumsParams {
 };
 
 // kind 0: dx rows (tile of G, k along the piece's columns) x w (k not contiguous), fp32 sums that later pieces are added to;
-// kind 1: dw rows (G as the left operand, its rows as k: not contiguous) x rows of x (not contiguous), final.
+// kind 1: dw rows (G as the left operand, its rows as k: not contiguous) x rows of x (not contiguous), final;
+// kind 2: the same over a part of the rows, fp32 sums.
 // An operand whose k is not contiguous comes as blocks of 64 k by 64 values, 128-byte rows with the swizzle: 8 KB from one block of
 // values to the next, 1 KB from eight k to the next.
 //
 // The tiles of dx are long (k is the piece) and those of dw short (k counts rows): every pair takes its share of the long ones first, and the
-// pairs with one fewer take so many short ones ahead of the others.
+// pairs with one fewer take so many short ones ahead of the others. Where a small vocabulary leaves few tiles of dw, each as long as there are rows, they
+// are cut along the rows (forward and all gradients in us, one part -> cut: 8192 x 100 x 256 111 -> 50, 8192 x 10 x 64 100 -> 40, 2048 x 1000 x 1024 69 -> 51,
+// 65536 x 256 x 512 517 -> 234).
 template <typename T>
 struct HeadSumsJob {
   const HeadSumsParams& p;
   const CUtensorMap *g_k, *g_mn, *w, *x, *x_copy, *dx, *dw;
-  int rows, row_tiles, col_tiles, v_tiles, dx_items, pairs;
+  int rows, row_tiles, col_tiles, v_tiles, dx_items, n_dw, dw_parts, pairs;
   int twice;  // 2: k goes over G and then over what its rounding took
 
   __device__ __forceinline__ HeadSumsJob(const HeadSumsParams& p_, const CUtensorMap* gk, const CUtensorMap* gm, const CUtensorMap* w_, const CUtensorMap* x_,
@@ -832,16 +840,17 @@ struct HeadSumsJob {
     col_tiles = (p.dim + p.bn - 1) / p.bn;
     v_tiles = (p.cols + 255) >> 8;
     dx_items = row_tiles * col_tiles * p.splits;
+    dw_parts = head_dw_parts(rows, twice, p.dw_splits);
+    n_dw = p.want_dw ? v_tiles * col_tiles * dw_parts : 0;
   }
   // Short tiles that a pair with one long tile fewer takes first, of `behind` pairs.
   __device__ __forceinline__ void ahead(int* behind, int* each) const {
     const int rest = dx_items % pairs;
     *behind = rest == 0 ? 0 : pairs - rest;
-    const int long_k = (p.cols + 63) / 64 / max(p.splits, 1), short_k = max(1, (rows + 63) / 64);
+    const int long_k = (p.cols + 63) / 64 / max(p.splits, 1), short_k = max(1, (rows + 63) / 64 / dw_parts);
     *each = *behind == 0 ? 0 : long_k / short_k;
   }
   __device__ __forceinline__ int items(int pair) const {
-    const int n_dw = p.want_dw ? v_tiles * col_tiles : 0;
     int n = dx_items > pair ? (dx_items - pair + pairs - 1) / pairs : 0;
     int behind, each;
     ahead(&behind, &each);
@@ -860,15 +869,16 @@ struct HeadSumsJob {
       return {0, slot, tm * 256, tn * p.bn, static_cast<int>(static_cast<int64_t>(kbs) * slot / p.splits), static_cast<int>(static_cast<int64_t>(kbs) * (slot + 1) / p.splits)};
     }
     i -= long_ones;
-    const int n_dw = v_tiles * col_tiles;
     int behind, each;
     ahead(&behind, &each);
     const int early = min(n_dw, behind * each), mine = pair - (pairs - behind);
     const int my_early = mine >= 0 && early > mine ? (early - mine + behind - 1) / behind : 0;
     const int at = i < my_early ? mine + i * behind : early + pair + (i - my_early) * pairs;
+    const int tiles = v_tiles * col_tiles, slot = at / tiles;
     int tm, tn;
-    head_raster(at, v_tiles, col_tiles, min(8, v_tiles), &tm, &tn);
-    return {1, 0, tm * 256, tn * p.bn, 0, max(1, (rows + 63) / 64) * twice};  // (no row counts: a product all the same, of whatever is there, and zeros stored)
+    head_raster(at - slot * tiles, v_tiles, col_tiles, min(8, v_tiles), &tm, &tn);
+    const int64_t kbs = max(1, (rows + 63) / 64) * twice;  // (no row counts: a product all the same, of whatever is there, and zeros stored)
+    return {p.dw_splits > 1 ? 2 : 1, slot, tm * 256, tn * p.bn, static_cast<int>(kbs * slot / dw_parts), static_cast<int>(kbs * (slot + 1) / dw_parts)};
   }
   __device__ __forceinline__ int stages() const { return p.stages; }
   __device__ __forceinline__ uint32_t stage_bytes() const { return kGemmTileBytes + static_cast<uint32_t>(p.bn) * kGemmBK; }
@@ -888,7 +898,7 @@ struct HeadSumsJob {
     for (int i = 0; i < half; i += 64) tma_load_2d_pair(at + kGemmTileBytes + i / 64 * kHeadBlock, b, bar, t.col0 + rank * half + i, b_k);
   }
   __device__ __forceinline__ uint32_t idesc(const HeadItem& t) const {
-    return umma_idesc_f16(std::is_same<T, __half>::value ? UMMA_F16 : UMMA_BF16, 256, p.bn, t.kind, 1);
+    return umma_idesc_f16(std::is_same<T, __half>::value ? UMMA_F16 : UMMA_BF16, 256, p.bn, t.kind != 0, 1);
   }
   __device__ __forceinline__ uint64_t a_desc(const HeadItem& t, uint32_t at) const { return umma_smem_desc_sw128(at, 1024, t.kind == 0 ? 16 : kHeadBlock); }
   __device__ __forceinline__ uint64_t b_desc(const HeadItem&, uint32_t at) const { return umma_smem_desc_sw128(at, 1024, kHeadBlock); }
@@ -910,7 +920,7 @@ struct HeadSumsJob {
     template <typename HandBack>
     __device__ __forceinline__ void take(const HeadItem& t, uint32_t acc, HandBack&& hand_back) {
       const HeadSumsParams& p = job.p;
-      const int width = t.kind == 0 ? 32 : 64, pieces = p.bn / width;  // 128 bytes of a row: fp32 sums of dx, 16 bits of dw
+      const int width = t.kind != 1 ? 32 : 64, pieces = p.bn / width;  // 128 bytes of a row: fp32 sums, 16 bits of dw
 #pragma unroll 1
       for (int c = part; c < pieces; c += 2) {
         const int col = t.col0 + c * width;
@@ -919,7 +929,7 @@ struct HeadSumsJob {
         __syncwarp();
         if (here) {
           const uint32_t at_row = stage + buf * kHeadChunkBytes + lane * 128;
-          if (t.kind == 0) {
+          if (t.kind != 1) {
             uint32_t v[32];
             tmem_ld_x32(acc + c * 32, v);
 #pragma unroll
@@ -953,7 +963,7 @@ struct HeadSumsJob {
           if (here) {
             uint8_t* const from = stage_ptr + buf * kHeadChunkBytes;
             const int row = t.row0 + row_in;
-            if (t.kind == 1) tma_store_2d(job.dw, from, col, p.v0 + row);
+            if (t.kind != 0) tma_store_2d(job.dw, from, col, t.slot * p.dw_slot_rows + p.v0 + row);
             else if (p.first) tma_store_2d(job.dx, from, col, static_cast<int>(t.slot * p.slot_rows) + row);
             else head_tma_add_2d(job.dx, from, col, static_cast<int>(t.slot * p.slot_rows) + row);
           }
@@ -1385,14 +1395,18 @@ __global__ void __launch_bounds__(kDbThreads) head_db_kernel(const HeadDbParams 
   static_cast<T*>(p.db)[p.v0 + col] = static_cast<T>(sum * head_scale(p.scale));
 }
 
-// dx: the parts' sums added in their order, scaled, rounded; zeros for rows that do not count. Eight values a thread.
+// dx, and dw where it was summed in parts: the parts' sums added in their order, scaled, rounded; zeros for rows that do not count. Eight values a thread.
 struct HeadDxParams {
-  const float* sums;  // [splits][slot_rows, dim]
+  const float* sums;     // [splits][slot_rows, dim]
   int splits;
   int64_t slot_rows;
-  int rows, dim;
+  int rows, dim;         // rows 0: no dx
   const int* place;
-  void* dx;           // [rows, dim]
+  void* dx;              // [rows, dim]
+  const float* dw_sums;  // [dw_splits][dw_slot_rows, dim]
+  int dw_splits, dw_slot_rows, vocab, twice;  // vocab 0: dw is there already
+  const int* count;
+  void* dw;              // [vocab, dim]
   HeadScale scale;
 };
 constexpr int kDxThreads = 256;
@@ -1402,15 +1416,20 @@ __global__ void __launch_bounds__(kDxThreads) head_dx_kernel(const HeadDxParams 
   grid_dependency_wait();
   grid_launch_dependents();
   const int words = p.dim >> 3;
-  const int64_t all = static_cast<int64_t>(p.rows) * words;
+  const int64_t all = static_cast<int64_t>(p.rows + p.vocab) * words;
   const float scale = head_scale(p.scale);
+  const int count = __ldg(p.count), dw_parts = head_dw_parts(count, p.twice, p.dw_splits);
   for (int64_t i = static_cast<int64_t>(blockIdx.x) * kDxThreads + threadIdx.x; i < all; i += static_cast<int64_t>(gridDim.x) * kDxThreads) {
     const int row = static_cast<int>(i / words), word = static_cast<int>(i - static_cast<int64_t>(row) * words);
-    const int at = __ldg(p.place + row);
+    const bool is_dw = row >= p.rows;
+    const int at = !is_dw ? __ldg(p.place + row) : count > 0 ? row - p.rows : -1, parts = is_dw ? dw_parts : p.splits;
+    const int64_t slot_rows = is_dw ? p.dw_slot_rows : p.slot_rows;
+    const float* const sums = is_dw ? p.dw_sums : p.sums;
     float4 a = make_float4(0.f, 0.f, 0.f, 0.f), b = a;
     if (at >= 0) {
-      for (int s = 0; s < p.splits; ++s) {
-        const float4* const from = reinterpret_cast<const float4*>(p.sums + (s * p.slot_rows + at) * p.dim) + 2 * word;
+#pragma unroll 4
+      for (int s = 0; s < parts; ++s) {
+        const float4* const from = reinterpret_cast<const float4*>(sums + (s * slot_rows + at) * p.dim) + 2 * word;
         const float4 u = __ldg(from), v = __ldg(from + 1);
         a.x += u.x; a.y += u.y; a.z += u.z; a.w += u.w;
         b.x += v.x; b.y += v.y; b.z += v.z; b.w += v.w;
@@ -1420,7 +1439,8 @@ __global__ void __launch_bounds__(kDxThreads) head_dx_kernel(const HeadDxParams 
     if (at >= 0)
       out = make_uint4(gemm_pack2<T>(a.x * scale, a.y * scale), gemm_pack2<T>(a.z * scale, a.w * scale), gemm_pack2<T>(b.x * scale, b.y * scale),
                        gemm_pack2<T>(b.z * scale, b.w * scale));
-    static_cast<uint4*>(p.dx)[i] = out;
+    if (is_dw) static_cast<uint4*>(p.dw)[i - static_cast<int64_t>(p.rows) * words] = out;
+    else static_cast<uint4*>(p.dx)[i] = out;
   }
 }
 

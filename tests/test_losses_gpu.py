@@ -166,6 +166,26 @@ def test_a_bias(shape: tuple[int, int, int], top: int, dtype: str) -> None:
         assert torch.equal(call(*leaves), loss)
 
 
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("masked", [0.0, 0.5, 0.99, 1.0])
+@pytest.mark.parametrize("shape", [(2500, 40, 72), (8191, 10, 32), (4097, 300, 264), (9000, 100, 1032), (700, 2, 8)])
+def test_small_vocabularies(shape: tuple[int, int, int], masked: float, dtype: str) -> None:  # dw in parts, of which there are fewer where few rows count
+    rows, vocab, dim = shape
+    x, w, y = layer(rows, vocab, dim, DTYPES[dtype])
+    y[torch.rand(rows, generator=torch.Generator(device="cuda").manual_seed(9), device="cuda") < masked] = -100
+    x, w = x.requires_grad_(True), w.requires_grad_(True)
+    for reduction, g in (("mean", torch.tensor(2.5, device="cuda")), ("none", normal(rows, seed=5))):
+        loss = ff.linear_cross_entropy(x, w, y, reduction=reduction)
+        dx, dw = torch.autograd.grad(loss, (x, w), g, retain_graph=True)
+        check(oracle.cross_entropy(x.detach(), w.detach(), y, -100, reduction, g), x, w, 1.0, loss, {"dx": dx, "dw": dw}, g, reduction)
+        again = torch.autograd.grad(loss, (x, w), g)
+        assert torch.equal(again[0], dx)
+        assert torch.equal(again[1], dw)
+        alone = ff.linear_cross_entropy(x.detach(), w, y, reduction=reduction)
+        (dw,) = torch.autograd.grad(alone, w, g)
+        check(oracle.cross_entropy(x.detach(), w.detach(), y, -100, reduction, g), x, w, 1.0, alone, {"dw": dw}, g, reduction)
+
+
 def test_one_entry_is_cross_entropy() -> None:
     x, w, y = layer(200, 900, 128, torch.bfloat16)
     a = ff.linear_distillation(x, w, y[:, None], normal(200, 1, seed=3), reduction="none")
