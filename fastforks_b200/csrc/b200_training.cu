@@ -34,8 +34,11 @@ template <typename T, int VEC, int N, int THREADS, int ROWS = 1>
 NormForm forward_form(int from = 0, int below = 1 << 30) { return {reinterpret_cast<const void*>(norm_rows_kernel<T, VEC, N, THREADS, ROWS>), THREADS, N, VEC, ROWS, from, below}; }
 template <typename T>
 const NormForm* forward_forms(bool wide_rows, int* count) {
-  static const NormForm values[] = {forward_form<T, 1, 1, 32>(), forward_form<T, 1, 4, 32>(), forward_form<T, 1, 8, 32>(), forward_form<T, 1, 4, 256>(), forward_form<T, 1, 8, 256>(),
-                                    forward_form<T, 1, 16, 256>(), forward_form<T, 1, 16, 1024>(), forward_form<T, 1, 32, 1024>()};
+  // Value by value, where rows are no whole 16-byte words. us of bf16 (threads x values): 9600 x 333 256 x 4 17.4, 128 x 4 13.2; 9600 x 1001 256 x 4 23.3, two
+  // 19.7; 1200 x 1901 256 x 8 9.8, two 6.8 (fp32 9.0, 9.8); 1200 x 3743 256 x 16 24.4, 512 x 8 17.2; 2400 x 5001 1024 x 16 72, 256 x 32 52, 512 x 16 39.5.
+  static const NormForm values[] = {forward_form<T, 1, 1, 32>(), forward_form<T, 1, 4, 32>(), forward_form<T, 1, 8, 32>(), forward_form<T, 1, 4, 128>(),
+                                    forward_form<T, 1, 4, 256>(0, 8), forward_form<T, 1, 4, 256, 2>(8), forward_form<T, 1, 8, 256>(0, 4), forward_form<T, 1, 8, 256, sizeof(T) == 2 ? 2 : 1>(4),
+                                    forward_form<T, 1, 8, 512>(), forward_form<T, 1, 16, 512>(), forward_form<T, 1, 16, 1024>(), forward_form<T, 1, 32, 1024>()};
   if (!wide_rows) {
     *count = static_cast<int>(std::size(values));
     return values;
@@ -59,8 +62,10 @@ template <typename T, int VEC, int N, int THREADS>
 NormForm grad_form() { return {reinterpret_cast<const void*>(norm_rows_grad_kernel<T, VEC, N, THREADS>), THREADS, N, VEC}; }
 template <typename T>
 const NormForm* grad_forms(bool wide_rows, int* count) {
-  static const NormForm values[] = {grad_form<T, 1, 1, 32>(), grad_form<T, 1, 4, 32>(), grad_form<T, 1, 8, 32>(), grad_form<T, 1, 8, 128>(), grad_form<T, 1, 16, 128>(),
-                                    grad_form<T, 1, 16, 256>(), grad_form<T, 1, 16, 512>(), grad_form<T, 1, 16, 1024>(), grad_form<T, 1, 32, 1024>()};
+  // us, 128 threads a row up to 1024 values and 16 of each up to 2048 -> these: 30000 x 333 in bf16 73 -> 40, 8192 x 1001 34 -> 29, 5000 x 1900 50 -> 40. 8 values of
+  // 512 threads up to 4096: 9000 x 3743 in fp32 97 -> 120, so not.
+  static const NormForm values[] = {grad_form<T, 1, 1, 32>(), grad_form<T, 1, 4, 32>(), grad_form<T, 1, 8, 32>(), grad_form<T, 1, 4, 128>(), grad_form<T, 1, 4, 256>(),
+                                    grad_form<T, 1, 8, 256>(), grad_form<T, 1, 16, 256>(), grad_form<T, 1, 16, 512>(), grad_form<T, 1, 16, 1024>(), grad_form<T, 1, 32, 1024>()};
   if (!wide_rows) {
     *count = static_cast<int>(std::size(values));
     return values;
@@ -179,7 +184,7 @@ int check_weight(const char* name, const void* p, const B200LayerNormArgs* a, bo
 // CTAs of the gradients' kernel: as many as run at once, so that each writes one part of dw and db and joining them costs little.
 int grad_ctas(const B200LayerNormArgs& a, const NormForm& f, int sms) {
   const int rows_each = f.threads == 32 ? kLnGradWarps : 1, threads = f.threads == 32 ? 32 * kLnGradWarps : f.threads;
-  const int per_sm = std::max(1, 512 / threads);
+  const int per_sm = std::max(1, (f.vectors * f.vec <= 8 ? 1024 : 512) / threads);
   return static_cast<int>(std::min<int64_t>((a.rows + rows_each - 1) / rows_each, static_cast<int64_t>(sms) * per_sm));
 }
 

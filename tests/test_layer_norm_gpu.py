@@ -88,7 +88,7 @@ def test_forward_and_gradients(shape: tuple[int, int], dtype: str) -> None:
         assert torch.equal(same, y)
 
 
-@pytest.mark.parametrize(("rows", "dim"), [(9601, 504), (2401, 776), (4801, 1024), (2401, 2040), (1201, 2056), (1201, 4096), (4801, 2600), (4801, 4096)])
+@pytest.mark.parametrize(("rows", "dim"), [(9601, 504), (2401, 776), (4801, 1024), (2401, 2040), (1201, 2056), (1201, 4096), (4801, 2600), (4801, 4096), (1185, 1001), (593, 1901), (601, 2047), (300, 4095), (300, 5001), (20, 8191)])
 def test_many_rows(rows: int, dim: int) -> None:  # odd: the last has no other to go with, where rows go two at a time
     x, w, b = normal(rows, dim, dtype=torch.bfloat16, seed=dim), normal(dim, dtype=torch.bfloat16, seed=1), normal(dim, dtype=torch.bfloat16, seed=2)
     y = torch.full((rows + 3, dim), 7.0, dtype=torch.bfloat16, device="cuda")
