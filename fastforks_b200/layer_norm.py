@@ -28,6 +28,14 @@ def _row_stride(t: torch.Tensor) -> int:
     return t.stride(0) if t.shape[0] > 1 else t.shape[1]
 
 
+def _shares(a: torch.Tensor, b: torch.Tensor) -> bool:
+    """Whether the memory that `a` and `b` span meets."""
+    if a.numel() == 0 or b.numel() == 0:
+        return False
+    (a0, a1), (b0, b1) = ((t.data_ptr(), t.data_ptr() + (1 + sum((n - 1) * s for n, s in zip(t.shape, t.stride(), strict=True))) * t.element_size()) for t in (a, b))
+    return a0 < b1 and b0 < a1
+
+
 def _args(x: torch.Tensor, weight: torch.Tensor | None, bias: torch.Tensor | None, eps: float) -> _lib.B200LayerNormArgs:
     a = _lib.B200LayerNormArgs()
     a.struct_size = ctypes.sizeof(a)
@@ -112,7 +120,7 @@ def layer_norm(
         weight: `[dim]` of x's type or float32, or None (ones).
         bias: `[dim]`, of the type of `weight`, or None (zeros).
         eps: Added to the variance.
-        out: Gets the result, contiguous; may be `x` itself (without gradients).
+        out: Gets the result, contiguous; may be `x` itself (without gradients), and shares no memory with the operands otherwise.
 
     Raises:
         ValueError: Operands outside the contract (checked before the launch).
@@ -139,6 +147,9 @@ def layer_norm(
     grad = torch.is_grad_enabled() and any(t.requires_grad for t in (x, *affine))
     if out is not None and (out.shape != x.shape or out.dtype != x.dtype or out.device != x.device or not out.is_contiguous() or grad or out.requires_grad):
         msg = f"{what}: out must be contiguous {tuple(x.shape)} {x.dtype} on {x.device} and nothing may require a gradient"
+        raise ValueError(msg)
+    if out is not None and ((_shares(out, x) and not (out.data_ptr() == x.data_ptr() and x.is_contiguous())) or any(_shares(out, t) for t in affine)):
+        msg = f"{what}: out shares memory with x, without being x, or with weight or bias"
         raise ValueError(msg)
     if x.numel() >= 2**31 * x.shape[-1]:
         msg = f"{what}: {x.numel() // x.shape[-1]} rows are too many"

@@ -223,3 +223,33 @@ def test_more_rows_than_fit_32_bits_of_offset() -> None:
     x = base.as_strided((rows, 64), (stride, 1))
     x.copy_(normal(rows, 64, dtype=torch.float16))
     assert torch.equal(ff.layer_norm(x), ff.layer_norm(x.contiguous()))
+
+
+def test_out_that_shares_memory_is_refused() -> None:
+    base = normal(20 * 64, dtype=torch.bfloat16)
+    x, w, b = base[: 10 * 64].view(10, 64), normal(64, dtype=torch.bfloat16, seed=1), normal(64, dtype=torch.bfloat16, seed=2)
+    want = ff.layer_norm(x, w, b)
+    before = base.clone()
+    for out in (base[64 : 11 * 64], base[1 : 10 * 64 + 1], base[9 * 64 + 63 : 19 * 64 + 63]):
+        with pytest.raises(ValueError, match="shares memory"):
+            ff.layer_norm(x, w, b, out=out.view(10, 64))
+    wide = base.view(10, 128)[:, :64]  # out would lie over its rows
+    with pytest.raises(ValueError, match="shares memory"):
+        ff.layer_norm(wide, w, b, out=x)
+    with pytest.raises(ValueError, match="shares memory"):
+        ff.layer_norm(x, base[19 * 64 :], b, out=base[10 * 64 :].view(10, 64))
+    assert torch.equal(base, before)
+    assert torch.equal(ff.layer_norm(x, w, b, out=base[10 * 64 :].view(10, 64)), want)  # side by side
+    assert torch.equal(ff.layer_norm(x, w, b, out=x), want)
+
+
+@pytest.mark.parametrize(("rows", "dim"), [(4001, 101), (1301, 1001), (2401, 1024), (700, 2600)])
+def test_a_chain_in_place_without_waiting(rows: int, dim: int) -> None:
+    x, w = normal(rows, dim, dtype=torch.bfloat16), 1 + 0.2 * normal(dim, dtype=torch.bfloat16, seed=1)
+    apart = x
+    for _ in range(30):
+        apart = ff.layer_norm(apart, w)
+        torch.cuda.synchronize()
+    for _ in range(30):
+        ff.layer_norm(x, w, out=x)
+    assert torch.equal(x, apart)
