@@ -283,7 +283,7 @@ struct HeadLossWork {
   FewPlan few;
   int bn, tiles_n, n_parts;
   int64_t parts_stride;
-  int64_t parts, picks, sums, bytes;
+  int64_t parts, picks, sums, cta_counts, bytes;
 };
 HeadLossWork head_loss_work(const B200HeadArgs& a, int sms) {
   const int pairs = std::max(1, sms / 2);
@@ -298,6 +298,7 @@ HeadLossWork head_loss_work(const B200HeadArgs& a, int sms) {
   w.parts = l.add(8LL * w.n_parts * w.parts_stride);
   w.picks = l.add(4LL * a.rows * std::max(a.top, 1));
   w.sums = l.add(4 * ((a.rows + 31) / 32));
+  w.cta_counts = l.add(a.rows > kCountedRows ? 4 * ((a.rows + 7) / 8) : 0);
   w.bytes = l.bytes;
   return w;
 }
@@ -487,8 +488,13 @@ int launch_loss(const B200HeadArgs& a, cudaStream_t stream) {
   r.status = dev->status;
   r.per_cta = std::min(kRowsMost, std::max(8, (a.rows + 2 * dev->sms - 1) / (2 * dev->sms)));
   {
+    const unsigned ctas = static_cast<unsigned>((a.rows + r.per_cta - 1) / r.per_cta);  // at most every 8 rows one
     void* args[] = {&r};
-    if (int rc = launch_kernel(reinterpret_cast<const void*>(head_rows_kernel), static_cast<unsigned>((a.rows + r.per_cta - 1) / r.per_cta), 1, kRowsThreads, 0, 1, stream, args, "head_rows kernel launch")) return rc;
+    if (a.rows > kCountedRows) {
+      r.cta_counts = at<int>(a.workspace, w.cta_counts);
+      if (int rc = launch_kernel(reinterpret_cast<const void*>(head_count_kernel), ctas, 1, kRowsThreads, 0, 1, stream, args, "head_count kernel launch")) return rc;
+    }
+    if (int rc = launch_kernel(reinterpret_cast<const void*>(head_rows_kernel), ctas, 1, kRowsThreads, 0, 1, stream, args, "head_rows kernel launch")) return rc;
   }
   HeadLogitsParams p = logits_params(a, s, dev->status);
   p.v0 = 0;
@@ -526,6 +532,8 @@ int launch_loss(const B200HeadArgs& a, cudaStream_t stream) {
   l.sums = at<float>(a.workspace, w.sums);
   l.finished = r.finished;
   void* args[] = {&l};
+  if (l.top == 1 && w.n_parts <= (a.rows >= kLossManyRows ? kLossManyParts : kLossFewParts))
+    return launch_kernel(reinterpret_cast<const void*>(head_loss_many_kernel), static_cast<unsigned>((a.rows + kLossManyThreads - 1) / kLossManyThreads), 1, kLossManyThreads, 0, 1, stream, args, "head_loss_many kernel launch");
   return launch_kernel(reinterpret_cast<const void*>(head_loss_kernel), static_cast<unsigned>((a.rows + 31) / 32), 1, kLossThreads, 0, 1, stream, args, "head_loss kernel launch");
 }
 

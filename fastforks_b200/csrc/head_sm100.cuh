@@ -10,11 +10,12 @@
 // row tiles are counted on the device.
 //
 //   head_entries_kernel  distillation: a row's p, its entropy, its entries in order of their tokens
+//   head_count_kernel    many rows: how many of each CTA's count
 //   head_rows_kernel     which rows count, where they go, their copy
 //   head_stats_kernel    logits of 256 x bn tiles in tensor memory; leaves a maximum and a sum of exponentials per row and half
 //                        of a tile's columns, and the logits of the row's entries
 //   head_few_kernel      the same of up to 64 rows
-//   head_loss_kernel     joins those to lse and loss
+//   head_loss_kernel     joins those to lse and loss (head_loss_many_kernel, where a row has little to join)
 //   head_coef_kernel     gradients that differ from row to row: one power of two for all
 //   head_grads_kernel    a piece of the vocabulary: the logits again, their gradient in 16 bits
 //   head_sums_kernel     dx += G w and dw = G^T x of that piece in one launch
@@ -1105,7 +1106,9 @@ __global__ void __launch_bounds__(kEntriesWarps * 32) head_entries_kernel(const 
 }
 
 // Which rows count, in the caller's order, and, where not all do, those rows of x together, with zeros behind the last up to the next
-// multiple of 64 (k of the products over rows). Every CTA counts the rows in front of its own: a few kilobytes out of L2.
+// multiple of 64 (k of the products over rows). Every CTA counts the rows in front of its own, a few kilobytes out of L2; where there are more
+// (kCountedRows), head_count_kernel has left each CTA's number (a loss
+// with the other kernels as they are now, without -> with it: 8192 x 10 x 64 11.6 -> 12.0 us, 24576 x 10 x 64 17.2 -> 14.1).
 struct HeadRowsParams {
   const void* targets;   // [rows] of target_bytes each, or null: `counts`
   const int8_t* counts;  // distillation: whether a row has an entry
@@ -1123,9 +1126,24 @@ struct HeadRowsParams {
   int* ids;              // [rows] targets as 32-bit entries (not for distillation)
   float* picks;          // [rows, top]: NaN for a target outside the vocabulary, which no tile writes
   float* loss;           // [rows] or null: 0 for rows that do not count
+  int* cta_counts;       // [CTAs] or null
   uint32_t* status;
 };
-constexpr int kRowsThreads = 256, kRowsMost = 1024, kRowsAtOnce = 8;
+constexpr int kRowsThreads = 256, kRowsMost = 1024, kRowsAtOnce = 8, kCountedRows = 8192;
+
+__device__ __forceinline__ int64_t head_target(const HeadRowsParams& p, int r) {
+  return p.target_bytes == 8 ? static_cast<const int64_t*>(p.targets)[r] : static_cast<int64_t>(static_cast<const int32_t*>(p.targets)[r]);
+}
+__device__ __forceinline__ bool head_counted(const HeadRowsParams& p, int r) { return p.targets == nullptr ? p.counts[r] != 0 : head_target(p, r) != p.ignore; }
+
+__global__ void __launch_bounds__(kRowsThreads) head_count_kernel(const HeadRowsParams p) {
+  grid_dependency_wait();
+  grid_launch_dependents();
+  const int r0 = blockIdx.x * p.per_cta, r1 = min(p.rows, r0 + p.per_cta);
+  int n = 0;
+  for (int base = r0; base < r1; base += kRowsThreads) n += __syncthreads_count(base + static_cast<int>(threadIdx.x) < r1 && head_counted(p, base + threadIdx.x));
+  if (threadIdx.x == 0) p.cta_counts[blockIdx.x] = n;
+}
 
 __global__ void __launch_bounds__(kRowsThreads) head_rows_kernel(const HeadRowsParams p) {
   __shared__ int from[kRowsMost], before_all, count_all, warp_sums[kRowsThreads / 32];
@@ -1134,15 +1152,21 @@ __global__ void __launch_bounds__(kRowsThreads) head_rows_kernel(const HeadRowsP
   grid_dependency_wait();
   grid_launch_dependents();
   __syncthreads();
-  const auto target = [&](int r) { return p.target_bytes == 8 ? static_cast<const int64_t*>(p.targets)[r] : static_cast<int64_t>(static_cast<const int32_t*>(p.targets)[r]); };
-  const auto counted = [&](int r) { return p.targets == nullptr ? p.counts[r] != 0 : target(r) != p.ignore; };
   const int r0 = blockIdx.x * p.per_cta, r1 = min(p.rows, r0 + p.per_cta);
   int before = 0, all = 0;
+  if (p.cta_counts != nullptr) {
+    for (int i = tid; i < static_cast<int>(gridDim.x); i += kRowsThreads) {
+      const int c = p.cta_counts[i];
+      all += c;
+      before += i < static_cast<int>(blockIdx.x) ? c : 0;
+    }
+  } else {
 #pragma unroll 8
-  for (int r = tid; r < p.rows; r += kRowsThreads) {
-    const int c = counted(r) ? 1 : 0;
-    all += c;
-    before += r < r0 ? c : 0;
+    for (int r = tid; r < p.rows; r += kRowsThreads) {
+      const int c = head_counted(p, r) ? 1 : 0;
+      all += c;
+      before += r < r0 ? c : 0;
+    }
   }
 #pragma unroll
   for (int d = 16; d > 0; d >>= 1) {
@@ -1158,7 +1182,7 @@ __global__ void __launch_bounds__(kRowsThreads) head_rows_kernel(const HeadRowsP
   const int count = count_all;
   for (int base = r0; base < r1; base += kRowsThreads) {
     const int r = base + tid;
-    const bool c = r < r1 && counted(r);
+    const bool c = r < r1 && head_counted(p, r);
     const unsigned mask = __ballot_sync(0xffffffffu, c);
     if (lane == 0) warp_sums[warp] = __popc(mask);
     __syncthreads();
@@ -1174,7 +1198,7 @@ __global__ void __launch_bounds__(kRowsThreads) head_rows_kernel(const HeadRowsP
       if (c) p.idx[to] = r;
       if (!c && p.loss != nullptr) p.loss[r] = 0.f;
       if (p.targets != nullptr) {
-        const int64_t y = target(r);
+        const int64_t y = head_target(p, r);
         const bool inside = y >= 0 && y < p.vocab;
         p.ids[r] = c && inside ? static_cast<int>(y) : kNoEntry;
         if (c && !inside) {
@@ -1210,8 +1234,9 @@ __global__ void __launch_bounds__(kRowsThreads) head_rows_kernel(const HeadRowsP
     for (int64_t i = static_cast<int64_t>(count) * words + tid; i < static_cast<int64_t>((count + 63) & ~63) * words; i += kRowsThreads) p.x_copy[i] = make_uint4(0, 0, 0, 0);
 }
 
-// lse and loss of 32 rows a CTA: a lane has a row and a warp every 32nd part; then a warp has a row and a lane every 32nd entry. The
-// last CTA adds up the CTAs' sums in their order.
+// head_loss_kernel: lse and loss of 32 rows a CTA: a lane has a row and a warp every 32nd part; then a warp has a row and a lane every 32nd entry.
+// head_loss_many_kernel: a thread has a row, where rows have one entry and few parts (a loss in us, without -> with it: 2 parts, 1024 x 10 x 64 11.5 -> 9.6,
+// 8192 x 10 x 64 16.9 -> 11.6; 16 to 64 parts, 4096 x 1000 x 256 17.0 -> 17.4, 8192 x 1000 x 256 24.7 -> 20.2). The last CTA adds up the CTAs' sums in their order.
 struct HeadLossParams {
   const int* count;
   const int* idx;
@@ -1229,33 +1254,108 @@ struct HeadLossParams {
   float* sums;           // [CTAs]
   unsigned* finished;
 };
-constexpr int kLossThreads = 1024, kLossAtOnce = 8;
+constexpr int kLossThreads = 1024, kLossAtOnce = 8, kLossManyThreads = 256, kLossManyParts = 64, kLossManyRows = 8192, kLossFewParts = 8;
+
+// Joins every so-manieth part of a row, from `i` on, to a maximum and a sum.
+__device__ __forceinline__ void head_join_parts(const HeadLossParams& p, int row, int i, int step, float* m_out, float* s_out) {
+  float m = -INFINITY, s = 0.f;
+  for (; i < p.n_parts; i += step * kLossAtOnce) {  // so many loads in flight, one maximum for them
+    float2 v[kLossAtOnce];
+#pragma unroll
+    for (int j = 0; j < kLossAtOnce; ++j) v[j] = i + step * j < p.n_parts ? __ldg(p.parts + (i + step * j) * p.parts_stride + row) : make_float2(-INFINITY, 0.f);
+    float m_new = m;
+#pragma unroll
+    for (int j = 0; j < kLossAtOnce; ++j) m_new = fmaxf(m_new, v[j].x);
+    const float from = m_new == -INFINITY ? 0.f : m_new;
+    s *= head_ex2(m - from);
+#pragma unroll
+    for (int j = 0; j < kLossAtOnce; ++j) s = fmaf(v[j].y, head_ex2(v[j].x - from), s);
+    m = m_new;
+  }
+  *m_out = m;
+  *s_out = s;
+}
+
+// What an entry adds to its row's loss. The maximum first, and the product unrounded, as it is behind the exponentials: where the entry is the maximum what
+// is left is the maximum's own rounding, which the sum holds too, and a small loss keeps its digits. An entry that does not count has no weight, and its logit
+// was never written.
+__device__ __forceinline__ float head_entry_loss(const HeadLossParams& p, int64_t at, float m, float log2_s) {
+  const float weight = p.p != nullptr ? __ldg(p.p + at) : 1.f;
+  return weight != 0.f ? weight * ((fmaf(-__ldg(p.picks + at), p.log2_scale, m) + log2_s) * 0.693147180559945f) : 0.f;
+}
+
+// The end of a row: its loss without the entropy -> as it is.
+__device__ __forceinline__ float head_finish_row(const HeadLossParams& p, int src, float loss, float lse2, bool write) {
+  if (p.entropy != nullptr) loss += __ldg(p.entropy + src);
+  loss *= p.tau * p.tau;
+  if (write) {
+    p.lse2[src] = isnan(loss) ? NAN : lse2;  // a row without a loss has no gradient either
+    if (p.loss != nullptr) p.loss[src] = loss;
+  }
+  return loss;
+}
+
+// The sum or the mean, of every CTA's sum, which thread 0 brings.
+template <int THREADS>
+__device__ __forceinline__ void head_total(const HeadLossParams& p, float sum, int count) {
+  __shared__ double cta_sums[THREADS / 32];
+  __shared__ bool last;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  if (threadIdx.x == 0) {
+    p.sums[blockIdx.x] = sum;
+    __threadfence();
+    last = atomicAdd(p.finished, 1u) == gridDim.x - 1;
+  }
+  __syncthreads();
+  if (!last) return;
+  __threadfence();
+  double all = 0.;
+  for (unsigned i = threadIdx.x; i < gridDim.x; i += THREADS) all += static_cast<double>(__ldcg(p.sums + i));
+#pragma unroll
+  for (int d = 16; d > 0; d >>= 1) all += __shfl_xor_sync(0xffffffffu, all, d);
+  if (lane == 0) cta_sums[warp] = all;
+  __syncthreads();
+  if (warp == 0) {
+    all = lane < THREADS / 32 ? cta_sums[lane] : 0.;
+#pragma unroll
+    for (int d = 16; d > 0; d >>= 1) all += __shfl_xor_sync(0xffffffffu, all, d);
+    if (lane == 0) *p.total = static_cast<float>(p.mean ? all / max(count, 1) : all);
+  }
+}
+
+__global__ void __launch_bounds__(kLossManyThreads) head_loss_many_kernel(const HeadLossParams p) {
+  __shared__ float warp_loss[kLossManyThreads / 32];
+  grid_dependency_wait();
+  grid_launch_dependents();
+  const int count = *p.count, row = blockIdx.x * kLossManyThreads + threadIdx.x;
+  float loss = 0.f;
+  if (row < count) {
+    const int src = __ldg(p.idx + row);
+    float m, s;
+    head_join_parts(p, row, 0, 1, &m, &s);
+    const float log2_s = log2f(s);
+    loss = head_finish_row(p, src, head_entry_loss(p, src, m, log2_s), m + log2_s, true);
+  }
+  if (p.total == nullptr) return;
+  const float sum = head_warp_sum(loss);
+  if ((threadIdx.x & 31) == 0) warp_loss[threadIdx.x >> 5] = sum;
+  __syncthreads();
+  float all = 0.f;
+  if (threadIdx.x == 0)
+#pragma unroll
+    for (int i = 0; i < kLossManyThreads / 32; ++i) all += warp_loss[i];
+  head_total<kLossManyThreads>(p, all, count);
+}
 
 __global__ void __launch_bounds__(kLossThreads) head_loss_kernel(const HeadLossParams p) {
   __shared__ float2 part[32][33];
   __shared__ float row_loss[32];
-  __shared__ double cta_sums[32];
-  __shared__ bool last;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   grid_dependency_wait();
   grid_launch_dependents();
   const int count = *p.count, row0 = blockIdx.x * 32;
   float m = -INFINITY, s = 0.f;
-  if (row0 + lane < count) {
-    for (int i = warp; i < p.n_parts; i += 32 * kLossAtOnce) {  // so many loads in flight, one maximum for them
-      float2 v[kLossAtOnce];
-#pragma unroll
-      for (int j = 0; j < kLossAtOnce; ++j) v[j] = i + 32 * j < p.n_parts ? __ldg(p.parts + (i + 32 * j) * p.parts_stride + row0 + lane) : make_float2(-INFINITY, 0.f);
-      float m_new = m;
-#pragma unroll
-      for (int j = 0; j < kLossAtOnce; ++j) m_new = fmaxf(m_new, v[j].x);
-      const float from = m_new == -INFINITY ? 0.f : m_new;
-      s *= head_ex2(m - from);
-#pragma unroll
-      for (int j = 0; j < kLossAtOnce; ++j) s = fmaf(v[j].y, head_ex2(v[j].x - from), s);
-      m = m_new;
-    }
-  }
+  if (row0 + lane < count) head_join_parts(p, row0 + lane, warp, 32, &m, &s);
   part[warp][lane] = make_float2(m, s);
   __syncthreads();
   const int row = row0 + warp;
@@ -1266,49 +1366,15 @@ __global__ void __launch_bounds__(kLossThreads) head_loss_kernel(const HeadLossP
 #pragma unroll
     for (int d = 16; d > 0; d >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, d));
     s = head_warp_sum(v.y * head_ex2(v.x - (m == -INFINITY ? 0.f : m)));
-    const float log2_s = log2f(s), lse2 = m + log2_s;
+    const float log2_s = log2f(s);
     const int src = __ldg(p.idx + row);
-    for (int k = lane; k < p.top; k += 32) {
-      const int64_t at = static_cast<int64_t>(src) * p.top + k;
-      const float weight = p.p != nullptr ? __ldg(p.p + at) : 1.f;
-      // An entry that does not count has no weight, and its logit was never written. The maximum first, and the product unrounded, as it is behind the
-      // exponentials: where the entry is the maximum what is left is the maximum's own rounding, which the sum holds too, and a small loss keeps its digits.
-      if (weight != 0.f) loss += weight * ((fmaf(-__ldg(p.picks + at), p.log2_scale, m) + log2_s) * 0.693147180559945f);
-    }
-    loss = head_warp_sum(loss);
-    if (p.entropy != nullptr) loss += __ldg(p.entropy + src);
-    loss *= p.tau * p.tau;
-    if (lane == 0) {
-      p.lse2[src] = isnan(loss) ? NAN : lse2;  // a row without a loss has no gradient either
-      if (p.loss != nullptr) p.loss[src] = loss;
-    }
+    for (int k = lane; k < p.top; k += 32) loss += head_entry_loss(p, static_cast<int64_t>(src) * p.top + k, m, log2_s);
+    loss = head_finish_row(p, src, head_warp_sum(loss), m + log2_s, lane == 0);
   }
   if (p.total == nullptr) return;
   if (lane == 0) row_loss[warp] = loss;
   __syncthreads();
-  if (warp == 0) {
-    const float sum = head_warp_sum(row_loss[lane]);
-    if (lane == 0) {
-      p.sums[blockIdx.x] = sum;
-      __threadfence();
-      last = atomicAdd(p.finished, 1u) == gridDim.x - 1;
-    }
-  }
-  __syncthreads();
-  if (!last) return;
-  __threadfence();
-  double all = 0.;
-  for (unsigned i = threadIdx.x; i < gridDim.x; i += kLossThreads) all += static_cast<double>(__ldcg(p.sums + i));
-#pragma unroll
-  for (int d = 16; d > 0; d >>= 1) all += __shfl_xor_sync(0xffffffffu, all, d);
-  if (lane == 0) cta_sums[warp] = all;
-  __syncthreads();
-  if (warp == 0) {
-    all = cta_sums[lane];
-#pragma unroll
-    for (int d = 16; d > 0; d >>= 1) all += __shfl_xor_sync(0xffffffffu, all, d);
-    if (lane == 0) *p.total = static_cast<float>(p.mean ? all / max(count, 1) : all);
-  }
+  head_total<kLossThreads>(p, warp == 0 ? head_warp_sum(row_loss[lane]) : 0.f, count);
 }
 
 // Gradients that differ from row to row, divided by the power of two above the largest: what goes into 16 bits is then at most 1.

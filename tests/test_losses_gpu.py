@@ -186,6 +186,26 @@ def test_small_vocabularies(shape: tuple[int, int, int], masked: float, dtype: s
         check(oracle.cross_entropy(x.detach(), w.detach(), y, -100, reduction, g), x, w, 1.0, alone, {"dw": dw}, g, reduction)
 
 
+@pytest.mark.parametrize("reduction", ["none", "mean"])
+@pytest.mark.parametrize("masked", [0.0, 0.3, 0.999, 1.0])
+@pytest.mark.parametrize("shape", [(16385, 19, 64), (40001, 700, 32), (20000, 10001, 16)])
+def test_many_rows(shape: tuple[int, int, int], masked: float, reduction: str) -> None:
+    rows, vocab, dim = shape
+    x, w, y = layer(rows, vocab, dim, torch.bfloat16)
+    y[torch.rand(rows, generator=torch.Generator(device="cuda").manual_seed(9), device="cuda") < masked] = -100
+    x, w = x.requires_grad_(True), w.requires_grad_(True)
+    g = normal(rows, seed=5) if reduction == "none" else torch.tensor(2.5, device="cuda")
+    loss = ff.linear_cross_entropy(x, w, y, reduction=reduction)
+    dx, dw = torch.autograd.grad(loss, (x, w), g)
+    check(oracle.cross_entropy(x.detach(), w.detach(), y, -100, reduction, g), x, w, 1.0, loss, {"dx": dx, "dw": dw}, g, reduction)
+    ids = torch.where(y < 0, -1, y)[:, None]
+    one = ff.linear_distillation(x, w, ids, torch.zeros(rows, 1, device="cuda"), reduction=reduction)
+    assert torch.equal(one, loss)
+    two, teacher = torch.cat((ids, -torch.ones_like(ids)), 1), torch.zeros(rows, 2, device="cuda")
+    other = ff.linear_distillation(x, w, two, teacher, reduction=reduction)
+    check(oracle.distillation(x.detach(), w.detach(), two, teacher, 1.0, reduction), x, w, 1.0, other, {}, None, reduction)
+
+
 def test_one_entry_is_cross_entropy() -> None:
     x, w, y = layer(200, 900, 128, torch.bfloat16)
     a = ff.linear_distillation(x, w, y[:, None], normal(200, 1, seed=3), reduction="none")
