@@ -421,9 +421,10 @@ at::Tensor rotary_scratch(const at::Tensor& like, const c10::cuda::CUDAStream& s
 using torch::autograd::AutogradContext;
 using torch::autograd::variable_list;
 
-// A gradient that comes in, as the kernels take it.
-at::Tensor incoming(const at::Tensor& g, const at::Tensor& like) {
-  if (!g.defined()) return at::zeros_like(like, at::MemoryFormat::Contiguous);
+// A gradient that comes in, as the kernels take it: what memory holds is its values (autograd passes on tensors that are yet to be negated).
+at::Tensor incoming(const at::Tensor& given, const at::Tensor& like) {
+  if (!given.defined()) return at::zeros_like(like, at::MemoryFormat::Contiguous);
+  const at::Tensor g = given.resolve_neg();
   return g.stride(-1) == 1 || g.size(-1) == 1 ? g : g.contiguous();
 }
 // Gradients that must not be differentiated again, should somebody try (the kernels have no second derivative).
@@ -614,7 +615,7 @@ struct LayerNormFunction : torch::autograd::Function<LayerNormFunction> {
       const at::NoGradGuard guard;
       const at::Tensor &x = saved[0], &w = saved[1], &b = saved[2];
       const c10::cuda::CUDAGuard on(x.device());
-      const at::Tensor g = grads[0].defined() ? grads[0].contiguous() : at::zeros_like(x, at::MemoryFormat::Contiguous);
+      const at::Tensor g = incoming(grads[0], x).contiguous();
       B200LayerNormArgs a;
       set_norm(&a, x, w, b, ctx->saved_data["eps"].toDouble());
       a.stats = static_cast<float*>(saved[3].data_ptr());
@@ -732,8 +733,7 @@ struct HeadLossFunction : torch::autograd::Function<HeadLossFunction> {
       const int64_t reduction = ctx->saved_data["reduction"].toInt();
       B200HeadArgs a;
       set_head(&a, x, w, bias, ctx->saved_data["top"].toInt(), ctx->saved_data["tau"].toDouble(), reduction);
-      at::Tensor g = grads[0];
-      if (!g.defined()) g = at::zeros({reduction == 0 ? a.rows : 1}, x.options().dtype(at::kFloat).requires_grad(false));
+      at::Tensor g = grads[0].defined() ? grads[0].resolve_neg() : at::zeros({reduction == 0 ? a.rows : 1}, x.options().dtype(at::kFloat).requires_grad(false));
       if (g.dim() > 1) g = g.reshape({-1});
       a.grad = static_cast<const float*>(g.data_ptr());
       a.grad_stride = g.dim() == 1 ? g.stride(0) : 0;

@@ -77,7 +77,7 @@ class _LayerNorm(torch.autograd.Function):
     @torch.autograd.function.once_differentiable
     def backward(ctx, g):  # noqa: ANN001, ANN205
         x, weight, bias, stats = ctx.saved_tensors
-        rows, g = _rows(x), _rows(g)
+        rows, g = _rows(x), _rows(g.resolve_neg())  # (autograd passes on tensors that are yet to be negated)
         want_x, want_w, want_b, _ = ctx.needs_input_grad
         a = _args(rows, weight, bias, ctx.eps)
         dx = torch.empty(x.shape, dtype=x.dtype, device=x.device) if want_x else None

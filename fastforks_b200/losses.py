@@ -108,6 +108,7 @@ class _HeadLoss(torch.autograd.Function):
     @torch.autograd.function.once_differentiable
     def backward(ctx, g):  # noqa: ANN001, ANN205
         x, w, bias, state = ctx.saved_tensors
+        g = g.resolve_neg()  # (autograd passes on tensors that are yet to be negated)
         rows, weight, vector = _rows(x), _rows(w), _vector(bias)
         a = _args(rows, weight, vector, ctx.top, ctx.tau, ctx.reduction)
         dx = torch.empty(x.shape, dtype=x.dtype, device=x.device) if ctx.needs_input_grad[1] else None

@@ -192,6 +192,8 @@ def _launch(  # noqa: PLR0913
 
 
 def _unit(g: torch.Tensor) -> torch.Tensor:
+    """A gradient that comes in, as the kernels take it: what memory holds is its values (autograd passes on tensors that are yet to be negated)."""
+    g = g.resolve_neg()
     return g if g.stride(-1) == 1 or g.shape[-1] == 1 else g.contiguous()
 
 

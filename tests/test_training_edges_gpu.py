@@ -1,0 +1,82 @@
+"""Edges of `layer_norm`, `linear_cross_entropy` and `linear_distillation` on a B200, on the full way and on the way of repeated calls.
+Tolerances are those of tests/test_layer_norm_gpu.py and tests/test_losses_gpu.py."""
+
+from __future__ import annotations
+
+from typing import TYPE_CHECKING
+
+import pytest
+import torch
+
+import fastforks_b200 as ff
+from fastforks_b200 import _lib
+from test_losses_gpu import integers, layer, normal
+
+if TYPE_CHECKING:
+    from collections.abc import Callable
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.fixture(autouse=True)
+def _kernels_ran_to_the_end():  # noqa: ANN202
+    yield
+    assert ff.device_status() == 0
+
+
+@pytest.fixture(params=["full", "repeated"])
+def way(request: pytest.FixtureRequest, monkeypatch: pytest.MonkeyPatch) -> str:
+    """Both ways of a call: the Python side's, and the host extension's once it is loaded."""
+    if request.param == "full":
+        monkeypatch.setattr(_lib, "fast", None)
+        monkeypatch.setattr(_lib, "use_fast", lambda: None)
+    else:
+        ff.layer_norm(torch.zeros(1, 8, device="cuda"))
+        assert _lib.fast is not None
+    return request.param
+
+
+def negated(t: torch.Tensor) -> torch.Tensor:
+    """`t` as a tensor that holds -t and a bit that says so, as the imaginary part of a conjugate does."""
+    view = torch._neg_view(-t)  # noqa: SLF001
+    assert view.is_neg()
+    assert torch.equal(view, t)
+    return view
+
+
+def operators() -> dict[str, tuple[Callable[..., torch.Tensor], tuple[torch.Tensor, ...]]]:
+    """Name -> call, its differentiable operands."""
+    x, w, y = layer(40, 300, 64, torch.bfloat16)
+    ids, teacher = integers(0, 300, (40, 5), 3), normal(40, 5)
+    bias = normal(300, dtype=torch.bfloat16, seed=4)
+    heads, table = normal(2, 7, 3, 64, dtype=torch.float16, seed=5), ff.rotary_table(7, 64, device="cuda")
+    weight = 1 + 0.2 * normal(64, seed=6)
+    return {
+        "ce none": (lambda a, b, c: ff.linear_cross_entropy(a, b, y, bias=c, reduction="none"), (x, w, bias)),
+        "ce mean": (lambda a, b, c: ff.linear_cross_entropy(a, b, y, bias=c), (x, w, bias)),
+        "kd none": (lambda a, b: ff.linear_distillation(a, b, ids, teacher, reduction="none"), (x, w)),
+        "layer norm": (lambda a, b, c: ff.layer_norm(a, b, c), (x, w[0], w[1])),
+        "layer norm of odd rows": (lambda a: ff.layer_norm(a), (normal(9, 33),)),
+        "rotary": (lambda a: ff.rotary(a, table), (heads,)),
+        "norm and rotary": (lambda a, b: torch.cat(ff.qk_norm_rotary(a, a * 2, b, b, table), 2), (heads, weight)),
+    }
+
+
+OPERATORS = ("ce none", "ce mean", "kd none", "layer norm", "layer norm of odd rows", "rotary", "norm and rotary")
+
+
+@pytest.mark.usefixtures("way")
+@pytest.mark.parametrize("name", OPERATORS)
+def test_gradients_that_come_in_with_a_lazy_negation(name: str) -> None:
+    call, operands = operators()[name]
+    leaves = [t.detach().clone().requires_grad_(True) for t in operands]
+    result = call(*leaves)
+    g = normal(result.numel(), dtype=result.dtype, seed=9).view(result.shape)
+    want = torch.autograd.grad(result, leaves, g, retain_graph=True)
+    got = torch.autograd.grad(result, leaves, negated(g), retain_graph=True)
+    assert all(torch.equal(a, b) for a, b in zip(got, want, strict=True))
+    if result.dtype == torch.float32:  # as it comes about: the imaginary part of a conjugate, every second number in memory
+        strided = torch.complex(g, -g).conj().imag
+        assert strided.is_neg()
+        got = torch.autograd.grad(result, leaves, strided)
+        assert all(torch.equal(a, b) for a, b in zip(got, want, strict=True))
