@@ -11,7 +11,7 @@ import ctypes
 import torch
 
 from . import _lib
-from .rotary import refuse_tangent
+from .rotary import as_held, refuse_negation, refuse_tangent
 
 _DTYPES = {torch.float16: _lib.F16, torch.bfloat16: _lib.BF16, torch.float32: _lib.F32}
 MAX_DIM = 32768
@@ -77,7 +77,7 @@ class _LayerNorm(torch.autograd.Function):
     @torch.autograd.function.once_differentiable
     def backward(ctx, g):  # noqa: ANN001, ANN205
         x, weight, bias, stats = ctx.saved_tensors
-        rows, g = _rows(x), _rows(g.resolve_neg())  # (autograd passes on tensors that are yet to be negated)
+        rows, g = _rows(x), _rows(as_held(g))
         want_x, want_w, want_b, _ = ctx.needs_input_grad
         a = _args(rows, weight, bias, ctx.eps)
         dx = torch.empty(x.shape, dtype=x.dtype, device=x.device) if want_x else None
@@ -131,6 +131,7 @@ def layer_norm(
         if done is not None:
             return done
     what = "layer_norm"
+    x, weight, bias = (as_held(t) for t in (x, weight, bias))
     if x.dtype not in _DTYPES or not x.is_cuda or x.dim() < 1 or not 1 <= x.shape[-1] <= MAX_DIM:
         msg = f"{what}: x must be a float16 / bfloat16 / float32 CUDA tensor [..., 1 .. {MAX_DIM}], got {tuple(x.shape)} {x.dtype} on {x.device}"
         raise ValueError(msg)
@@ -148,6 +149,8 @@ def layer_norm(
     if out is not None and (out.shape != x.shape or out.dtype != x.dtype or out.device != x.device or not out.is_contiguous() or grad or out.requires_grad):
         msg = f"{what}: out must be contiguous {tuple(x.shape)} {x.dtype} on {x.device} and nothing may require a gradient"
         raise ValueError(msg)
+    if out is not None:
+        refuse_negation(what, "out", out)
     if out is not None and ((_shares(out, x) and not (out.data_ptr() == x.data_ptr() and x.is_contiguous())) or any(_shares(out, t) for t in affine)):
         msg = f"{what}: out shares memory with x, without being x, or with weight or bias"
         raise ValueError(msg)

@@ -13,7 +13,7 @@ import math
 import torch
 
 from . import _lib
-from .rotary import refuse_tangent
+from .rotary import as_held, refuse_tangent
 
 _DTYPES = {torch.float16: _lib.F16, torch.bfloat16: _lib.BF16, torch.float32: _lib.F32}
 _REDUCTIONS = {"none": 0, "sum": 1, "mean": 2}
@@ -108,7 +108,7 @@ class _HeadLoss(torch.autograd.Function):
     @torch.autograd.function.once_differentiable
     def backward(ctx, g):  # noqa: ANN001, ANN205
         x, w, bias, state = ctx.saved_tensors
-        g = g.resolve_neg()  # (autograd passes on tensors that are yet to be negated)
+        g = as_held(g)
         rows, weight, vector = _rows(x), _rows(w), _vector(bias)
         a = _args(rows, weight, vector, ctx.top, ctx.tau, ctx.reduction)
         dx = torch.empty(x.shape, dtype=x.dtype, device=x.device) if ctx.needs_input_grad[1] else None
@@ -128,6 +128,7 @@ class _HeadLoss(torch.autograd.Function):
 def _run(what: str, x: torch.Tensor, w: torch.Tensor, bias: torch.Tensor | None, targets: torch.Tensor, teacher: torch.Tensor | None, ignore: int, tau: float, reduction: str) -> torch.Tensor:  # noqa: PLR0913
     shape = x.shape[:-1] if reduction == "none" else ()
     grad = torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x, w, bias))
+    x, w, bias = (as_held(t) for t in (x, w, bias))
     if x.numel() == 0:
         if grad:
             msg = f"{what}: x {tuple(x.shape)} without a row has no gradient"
@@ -234,6 +235,6 @@ def linear_distillation(  # noqa: PLR0913
         msg = f"{what}: temperature {temperature} must be positive and finite"
         raise ValueError(msg)
     k = teacher_ids.shape[-1]
-    ids, logits = (t.reshape(-1, k) for t in (teacher_ids, teacher_logits))
+    ids, logits = (t.reshape(-1, k) for t in (teacher_ids, as_held(teacher_logits)))
     ids, logits = (t if t.stride(1) == 1 or k == 1 else t.contiguous() for t in (ids, logits))
     return _run(what, x, weight, bias, ids, logits, 0, float(temperature), reduction)

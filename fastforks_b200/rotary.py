@@ -111,6 +111,18 @@ def refuse_tangent(what: str, name: str, t: torch.Tensor) -> None:
         raise ValueError(msg)
 
 
+def as_held(t: torch.Tensor | None) -> torch.Tensor | None:
+    """`t` with its values in memory: torch may keep a sign to be turned later (the imaginary part of a conjugate), of which the kernels know nothing."""
+    return t if t is None else t.resolve_neg()
+
+
+def refuse_negation(what: str, name: str, t: torch.Tensor) -> None:
+    """What is written to has no sign to be turned later: see `as_held`."""
+    if t.is_neg():
+        msg = f"{what}: {name} is a view that negates what it holds (resolve_neg)"
+        raise ValueError(msg)
+
+
 def _check_heads(what: str, name: str, t: torch.Tensor, like: torch.Tensor | None = None) -> None:
     if t.dim() != 4 or t.dtype not in _DTYPES or not t.is_cuda:  # noqa: PLR2004
         msg = f"{what}: {name} must be a float16 / bfloat16 / float32 CUDA [batch, tokens, heads, dim] tensor, got {tuple(t.shape)} {t.dtype} on {t.device}"
@@ -143,7 +155,7 @@ def _check_table(what: str, table: torch.Tensor | None, positions: torch.Tensor 
         raise ValueError(msg)
     else:
         positions = positions if positions.dtype == torch.int32 else positions.clamp(-1, 2**31 - 1).int()  # what 32 bits do not hold is out of range, too
-    return table.contiguous(), positions
+    return as_held(table).contiguous(), positions
 
 
 def _strides(t: torch.Tensor) -> tuple[int, int, int]:
@@ -192,8 +204,8 @@ def _launch(  # noqa: PLR0913
 
 
 def _unit(g: torch.Tensor) -> torch.Tensor:
-    """A gradient that comes in, as the kernels take it: what memory holds is its values (autograd passes on tensors that are yet to be negated)."""
-    g = g.resolve_neg()
+    """A gradient that comes in, as the kernels take it."""
+    g = as_held(g)
     return g if g.stride(-1) == 1 or g.shape[-1] == 1 else g.contiguous()
 
 
@@ -245,6 +257,7 @@ def rotary(
         done = _lib.fast.rotary(x, table, positions, interleaved)
         if done is not None:
             return done
+    x = as_held(x)
     _check_heads("rotary", "x", x)
     if table is None:
         msg = "rotary: table is None"
@@ -253,6 +266,7 @@ def rotary(
     grad = x.requires_grad and torch.is_grad_enabled()
     if out is not None:
         _check_heads("rotary", "out", out, x)
+        refuse_negation("rotary", "out", out)
         if grad or out.requires_grad or out.shape != x.shape:
             msg = f"rotary: out must be {tuple(x.shape)} and neither it nor x may require a gradient"
             raise ValueError(msg)
@@ -323,6 +337,7 @@ def qk_norm_rotary(  # noqa: PLR0913
         if done is not None:
             return done
     what = "qk_norm_rotary"
+    q, k, q_weight, k_weight = (as_held(t) for t in (q, k, q_weight, k_weight))
     _check_heads(what, "q", q)
     _check_heads(what, "k", k, q)
     weights = [w for w in (q_weight, k_weight) if w is not None]
@@ -342,6 +357,7 @@ def qk_norm_rotary(  # noqa: PLR0913
     if out is not None:
         for name, t, x in (("out[0]", out[0], q), ("out[1]", out[1], k)):
             _check_heads(what, name, t, x)
+            refuse_negation(what, name, t)
             if grad or t.requires_grad or t.shape != x.shape:
                 msg = f"{what}: {name} must be {tuple(x.shape)} and nothing may require a gradient"
                 raise ValueError(msg)

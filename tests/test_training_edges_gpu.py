@@ -80,3 +80,38 @@ def test_gradients_that_come_in_with_a_lazy_negation(name: str) -> None:
         assert strided.is_neg()
         got = torch.autograd.grad(result, leaves, strided)
         assert all(torch.equal(a, b) for a, b in zip(got, want, strict=True))
+
+
+@pytest.mark.usefixtures("way")
+@pytest.mark.parametrize("name", OPERATORS)
+def test_operands_with_a_lazy_negation(name: str) -> None:
+    call, operands = operators()[name]
+    leaves = [t.detach().clone().requires_grad_(True) for t in operands]
+    want = call(*leaves)
+    g = normal(want.numel(), dtype=want.dtype, seed=9).view(want.shape)
+    grads = torch.autograd.grad(want, leaves, g)
+    for i in range(len(leaves)):
+        result = call(*(negated(t) if j == i else t for j, t in enumerate(leaves)))
+        assert torch.equal(result, want)
+        assert all(torch.equal(a, b) for a, b in zip(torch.autograd.grad(result, leaves, g), grads, strict=True))
+        with torch.no_grad():
+            assert torch.equal(call(*(negated(t) if j == i else t for j, t in enumerate(leaves))), want)
+
+
+@pytest.mark.usefixtures("way")
+def test_a_teacher_a_table_and_an_out_with_a_lazy_negation() -> None:
+    x, w, _ = layer(40, 300, 64, torch.float16)
+    ids, teacher = integers(0, 300, (40, 5), 3), normal(40, 5)
+    assert torch.equal(ff.linear_distillation(x, w, ids, negated(teacher)), ff.linear_distillation(x, w, ids, teacher))
+    heads, table = x.view(2, 10, 2, 64).clone(), ff.rotary_table(10, 64, device="cuda")
+    assert torch.equal(ff.rotary(heads, negated(table)), ff.rotary(heads, table))
+    before = x.clone()
+    for refused in (
+        lambda: ff.layer_norm(x, out=negated(x.clone())),
+        lambda: ff.layer_norm(x, out=torch._neg_view(x)),  # noqa: SLF001
+        lambda: ff.rotary(heads, table, out=negated(heads.clone())),
+        lambda: ff.qk_norm_rotary(heads, heads, None, None, table, out=(heads, negated(heads.clone()))),
+    ):
+        with pytest.raises(ValueError, match="negat"):
+            refused()
+    assert torch.equal(x, before)
