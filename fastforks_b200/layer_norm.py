@@ -11,7 +11,7 @@ import ctypes
 import torch
 
 from . import _lib
-from .rotary import as_held, refuse_negation, refuse_tangent
+from .rotary import as_held, refuse_negation, refuse_tangent, written
 
 _DTYPES = {torch.float16: _lib.F16, torch.bfloat16: _lib.BF16, torch.float32: _lib.F32}
 MAX_DIM = 32768
@@ -120,7 +120,8 @@ def layer_norm(
         weight: `[dim]` of x's type or float32, or None (ones).
         bias: `[dim]`, of the type of `weight`, or None (zeros).
         eps: Added to the variance.
-        out: Gets the result, contiguous; may be `x` itself (without gradients), and shares no memory with the operands otherwise.
+        out: Gets the result, contiguous; may be `x` itself (without gradients), and shares no memory with the operands otherwise. Autograd
+            sees that it was written to.
 
     Raises:
         ValueError: Operands outside the contract (checked before the launch).
@@ -167,4 +168,6 @@ def layer_norm(
     y = torch.empty(x.shape, dtype=x.dtype, device=x.device) if out is None else out
     rows = _rows(x)
     _forward(rows, weight, bias, float(eps), y.view(rows.shape), stats=False)
+    if out is not None:
+        written(out)
     return y

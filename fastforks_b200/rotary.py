@@ -123,6 +123,14 @@ def refuse_negation(what: str, name: str, t: torch.Tensor) -> None:
         raise ValueError(msg)
 
 
+def written(*tensors: torch.Tensor) -> None:
+    """Tells autograd that a kernel wrote to these, so that a gradient that needs what was there raises. (Tensors of inference mode are in no gradient and
+    have no version.)"""
+    for t in tensors:
+        if not t.is_inference():
+            torch.autograd.graph.increment_version(t)
+
+
 def _check_heads(what: str, name: str, t: torch.Tensor, like: torch.Tensor | None = None) -> None:
     if t.dim() != 4 or t.dtype not in _DTYPES or not t.is_cuda:  # noqa: PLR2004
         msg = f"{what}: {name} must be a float16 / bfloat16 / float32 CUDA [batch, tokens, heads, dim] tensor, got {tuple(t.shape)} {t.dtype} on {t.device}"

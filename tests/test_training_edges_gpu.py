@@ -115,3 +115,36 @@ def test_a_teacher_a_table_and_an_out_with_a_lazy_negation() -> None:
         with pytest.raises(ValueError, match="negat"):
             refused()
     assert torch.equal(x, before)
+
+
+@pytest.mark.usefixtures("way")
+@pytest.mark.parametrize("saved_by", ["cross entropy", "distillation", "layer norm"])
+def test_a_saved_tensor_that_a_norm_writes_to_is_noticed(saved_by: str) -> None:
+    x, w, y = layer(40, 300, 64, torch.float16)
+    weight = w.detach().requires_grad_(True) if saved_by != "layer norm" else torch.ones(64, device="cuda", dtype=torch.float16, requires_grad=True)
+    call = {
+        "cross entropy": lambda t: ff.linear_cross_entropy(t, weight, y),
+        "distillation": lambda t: ff.linear_distillation(t, weight, y[:, None], torch.zeros(40, 1, device="cuda")),
+        "layer norm": lambda t: ff.layer_norm(t, weight).sum(),
+    }[saved_by]
+    for out in (lambda t: t, lambda t: t[3:5]):  # itself, and a part of it
+        held = x.clone()
+        loss = call(held)
+        ff.layer_norm(out(held), out=out(held))
+        with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+            torch.autograd.grad(loss, weight)
+    held = x.clone()
+    loss = call(held)
+    ff.layer_norm(held, out=torch.empty_like(held))  # another tensor: nothing is noticed, as nothing happened
+    torch.autograd.grad(loss, weight)
+
+
+@pytest.mark.usefixtures("way")
+def test_tensors_of_inference_mode_are_written_to() -> None:
+    x = normal(5, 64)
+    with torch.inference_mode():
+        kept = torch.empty_like(x)
+        inside = ff.layer_norm(x, out=torch.empty_like(x))
+    assert ff.layer_norm(x, out=kept) is kept  # they have no version
+    assert torch.equal(kept, ff.layer_norm(x))
+    assert torch.equal(inside, kept)
