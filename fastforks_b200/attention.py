@@ -17,6 +17,7 @@ from typing import TYPE_CHECKING
 import torch
 
 from . import _lib
+from .rotary import written
 
 if TYPE_CHECKING:
     from collections.abc import Sequence
@@ -266,6 +267,7 @@ def attention(  # noqa: PLR0913
     lib = _lib.library()
     b, n, h = _sizes(q, layout)
     _, nk, _ = _sizes(k, layout)
+    given = out
     if out is None:
         o = torch.empty((b, n, h, HEAD_DIM), device=q.device, dtype=q.dtype)
         out = o.transpose(1, 2) if layout == "bhnd" else o
@@ -321,6 +323,8 @@ def attention(  # noqa: PLR0913
     _lib.use_fast()
     for t in keep:  # the launch is asynchronous: tie temporaries to the stream
         t.record_stream(torch.cuda.current_stream(q.device))
+    if given is not None:
+        written(given)
     return out
 
 

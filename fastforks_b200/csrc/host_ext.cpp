@@ -78,6 +78,11 @@ bool plain(const at::Tensor& t, c10::DeviceIndex device) {
          !(t.requires_grad() && at::GradMode::is_enabled()) && t.has_storage();
 }
 
+// A caller's tensor that a kernel wrote to: a gradient that needs what was there has to see that. (Tensors of inference mode have no version.)
+void written(const at::Tensor& t) {
+  if (!t.is_inference()) t.unsafeGetTensorImpl()->bump_version();
+}
+
 at::Tensor empty_like_type(at::IntArrayRef sizes, const at::Tensor& like) {
   return at::detail::empty_cuda(sizes, like.scalar_type(), like.device(), std::nullopt);
 }
@@ -216,6 +221,7 @@ PyObject* py_attention(PyObject*, PyObject* const* args, Py_ssize_t n) {
   a.o = out.data_ptr();
   set_strides(a.o_stride, vo);
   if (launched([&] { return b200_attn_fwd(&a, reinterpret_cast<void*>(stream)); }) != B200_ATTN_OK) Py_RETURN_NONE;
+  if (args[6] != Py_None) written(out);
   return THPVariable_Wrap(out);
 }
 
@@ -284,6 +290,7 @@ PyObject* py_gemm(PyObject*, PyObject* const* args, Py_ssize_t n) {
   a.y = out.data_ptr();
   const c10::cuda::CUDAStream stream = c10::cuda::getCurrentCUDAStream(device);
   if (launched([&] { return b200_gemm(&a, stream.stream()); }) != B200_ATTN_OK) Py_RETURN_NONE;
+  if (args[6] != Py_None) written(out);
   return THPVariable_Wrap(out);
 }
 
@@ -319,6 +326,7 @@ PyObject* py_rope(PyObject*, PyObject* const* args, Py_ssize_t n) {
   a.q_scale = static_cast<float>(scale);
   const c10::cuda::CUDAStream stream = c10::cuda::getCurrentCUDAStream(device);
   if (launched([&] { return b200_rope_qk(&a, stream.stream()); }) != B200_ATTN_OK) Py_RETURN_FALSE;
+  written(*x);
   Py_RETURN_TRUE;
 }
 
@@ -859,6 +867,7 @@ PyObject* py_kv4_append(PyObject*, PyObject* const* args, Py_ssize_t n) {
   }
   const c10::cuda::CUDAStream stream = c10::cuda::getCurrentCUDAStream(device);
   if (launched([&] { return b200_kv4_append(&a, stream.stream()); }) != B200_ATTN_OK) Py_RETURN_NONE;
+  written(*tensor_of(args[0]));
   if (args[7] == Py_None) Py_RETURN_TRUE;
   return THPVariable_Wrap(out);
 }

@@ -13,6 +13,7 @@ import ctypes
 import torch
 
 from . import _lib
+from .rotary import written
 
 ACT_NONE, ACT_RELU, ACT_GELU, ACT_GELU_TANH = 0, 1, 5, 6  # the reference's codes (dpt_fused/__init__.py)
 _DTYPES = {torch.float16: _lib.F16, torch.bfloat16: _lib.BF16}
@@ -99,4 +100,6 @@ def gemm(  # noqa: PLR0913 - the epilogue terms
         code = _lib.library().b200_gemm(ctypes.byref(a), torch._C._cuda_getCurrentRawStream(x.device.index))  # noqa: SLF001
     _lib.raise_for_code(code, "gemm")
     _lib.use_fast()
+    if out is not None:
+        written(out)
     return y

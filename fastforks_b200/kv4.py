@@ -16,7 +16,7 @@ import threading
 import torch
 
 from . import _lib
-from .rotary import refuse_tangent
+from .rotary import refuse_tangent, written
 
 BLOCK = 16  # tokens
 HEAD_DIMS = (64, 128)
@@ -203,6 +203,7 @@ def kv4_append_(  # noqa: PLR0913
         _set(a, "q", q)
         _set(a, "q_out", out)
     _call(what, "b200_kv4_append", a, k.device)
+    written(cache, *(() if q is None else (out,)))
     return out
 
 
@@ -274,6 +275,7 @@ def kv4_attention(  # noqa: PLR0913
     if q.shape[2] == 0 or q.shape[2] % cache.shape[1]:
         msg = f"{what}: {q.shape[2]} q heads are no multiple of {cache.shape[1]} kv heads"
         raise ValueError(msg)
+    given = out is not None
     if out is None:
         out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
     else:
@@ -289,6 +291,8 @@ def kv4_attention(  # noqa: PLR0913
     work, counters = reserve_kv4_workspace(q.device.index)
     a.workspace, a.workspace_bytes, a.counters, a.counter_words = work.data_ptr(), work.numel(), counters.data_ptr(), counters.numel()
     _call(what, "b200_kv4_attention", a, q.device)
+    if given:
+        written(out)
     if _lib.fast is not None and (q.device.index, stream := torch._C._cuda_getCurrentRawStream(q.device.index)) in _WORKSPACES:  # noqa: SLF001
         _lib.fast.register_kv4_workspace(q.device.index, stream, work.data_ptr(), work.numel(), counters.data_ptr(), counters.numel())
     return out

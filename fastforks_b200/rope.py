@@ -14,6 +14,7 @@ import math
 import torch
 
 from . import _lib
+from .rotary import written
 
 HEAD_DIM = 64
 
@@ -73,4 +74,5 @@ def rope_qk_(qkv: torch.Tensor, cs: torch.Tensor, *, q_scale: float = 1.0) -> to
         code = _lib.library().b200_rope_qk(ctypes.byref(a), torch._C._cuda_getCurrentRawStream(qkv.device.index))  # noqa: SLF001
     _lib.raise_for_code(code, "rope_qk_")
     _lib.use_fast()
+    written(qkv)
     return qkv

@@ -284,6 +284,8 @@ def rotary(
         return _Rotary.apply(x, table, positions, interleaved)
     y = torch.empty(x.shape, dtype=x.dtype, device=x.device) if out is None else out
     _launch("rotary", [{"x": x, "y": y}], table, positions, interleaved=interleaved)
+    if out is not None:
+        written(out)
     return y
 
 
@@ -376,4 +378,6 @@ def qk_norm_rotary(  # noqa: PLR0913
         return _QkNormRotary.apply(q, k, q_weight, k_weight, table, positions, float(eps), interleaved)
     yq, yk = out if out is not None else (torch.empty(t.shape, dtype=t.dtype, device=t.device) for t in (q, k))
     _launch(what, [{"x": q, "y": yq, "w": q_weight}, {"x": k, "y": yk, "w": k_weight}], table, positions, interleaved=interleaved, norm=True, eps=float(eps))
+    if out is not None:
+        written(*out)
     return yq, yk
