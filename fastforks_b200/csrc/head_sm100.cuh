@@ -1458,7 +1458,7 @@ __global__ void __launch_bounds__(kDbThreads) head_db_kernel(const HeadDbParams 
   if (threadIdx.x >= 64 || col >= p.cols) return;
   float sum = 0.f;
   for (int i = 0; i < kDbThreads / 8; ++i) sum += sums[i][threadIdx.x];
-  static_cast<T*>(p.db)[p.v0 + col] = static_cast<T>(sum * head_scale(p.scale));
+  static_cast<T*>(p.db)[p.v0 + col] = static_cast<T>(count > 0 ? sum * head_scale(p.scale) : 0.f);  // (nothing is added up: 0 under any gradient, as dx and dw)
 }
 
 // dx, and dw where it was summed in parts: the parts' sums added in their order, scaled, rounded; zeros for rows that do not count. Eight values a thread.

@@ -148,3 +148,16 @@ def test_tensors_of_inference_mode_are_written_to() -> None:
     assert ff.layer_norm(x, out=kept) is kept  # they have no version
     assert torch.equal(kept, ff.layer_norm(x))
     assert torch.equal(inside, kept)
+
+
+@pytest.mark.usefixtures("way")
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize(("rows", "vocab"), [(40, 300), (300, 1000), (3000, 10)])
+def test_no_row_counts_under_a_gradient_that_is_not_finite(rows: int, vocab: int, dtype: torch.dtype) -> None:
+    """A sum divided by the number of rows that count: with none of them its gradient is infinite, and nothing is added to nothing."""
+    x, w, y = layer(rows, vocab, 64, dtype)
+    leaves = [t.detach().requires_grad_(True) for t in (x, w, normal(vocab, dtype=dtype, seed=4))]
+    for g in (float("inf"), float("nan")):
+        loss = ff.linear_cross_entropy(leaves[0], leaves[1], torch.full_like(y, -100), bias=leaves[2], reduction="sum")
+        for grad in torch.autograd.grad(loss, leaves, torch.tensor(g, device="cuda")):
+            assert not grad.any()
