@@ -10,7 +10,8 @@ import torch
 
 import fastforks_b200 as ff
 from fastforks_b200 import _lib
-from test_losses_gpu import integers, layer, normal
+from oracle import training_oracle as oracle
+from test_losses_gpu import check, integers, layer, normal
 
 if TYPE_CHECKING:
     from collections.abc import Callable
@@ -161,3 +162,66 @@ def test_no_row_counts_under_a_gradient_that_is_not_finite(rows: int, vocab: int
         loss = ff.linear_cross_entropy(leaves[0], leaves[1], torch.full_like(y, -100), bias=leaves[2], reduction="sum")
         for grad in torch.autograd.grad(loss, leaves, torch.tensor(g, device="cuda")):
             assert not grad.any()
+
+
+@pytest.mark.parametrize("size", [1e-40, 1e-30, 1e-3, 1e25, 1e37])
+def test_row_gradients_of_any_size_in_bfloat16(size: float) -> None:
+    """bfloat16 has fp32's range: nothing is flushed or infinite. Below 2^-126 gradients themselves have fewer digits than fp32's 24 (1e-40: some 16), and the
+    results are subnormal numbers, steps of 2^-133 apart: half of one is in the bounds."""
+    x, w, y = layer(100, 400, 64, torch.bfloat16)
+    x, w, b = x.requires_grad_(True), w.requires_grad_(True), normal(400, dtype=torch.bfloat16, seed=3).requires_grad_(True)
+    g = normal(100, seed=5).clamp(-4, 4) * size
+    g[::7] = 0
+    loss = ff.linear_cross_entropy(x, w, y, bias=b, reduction="none")
+    dx, dw, db = torch.autograd.grad(loss, (x, w, b), g)
+    r = oracle.cross_entropy(x.detach(), w.detach(), y, -100, "none", g, b.detach())
+    assert not dx[::7].any()
+    check(r, x, w, 1.0, loss, {"dx": dx, "dw": dw, "db": db}, g, "none", b)
+
+
+def test_row_gradients_past_the_range_of_float16() -> None:
+    """Infinities of the right sign, rows without a gradient 0, nothing NaN. (65520 lies half a step past the largest number; a sixteenth to either side
+    is left to the roundings before it.)"""
+    x, w, y = layer(100, 400, 64, torch.float16)
+    x, w = x.requires_grad_(True), w.requires_grad_(True)
+    g = normal(100, seed=5) * 1e25
+    g[::7] = 0
+    dx, dw = torch.autograd.grad(ff.linear_cross_entropy(x, w, y, reduction="none"), (x, w), g)
+    r = oracle.cross_entropy(x.detach(), w.detach(), y, -100, "none", g)
+    for got, ref in ((dx, r.dx), (dw, r.dw)):
+        assert not got.isnan().any()
+        sure = ref.abs() > 65520 * 17 / 16
+        # of what is computed from numbers of size 1e25 the last 2^-11 (and 2^-24 of a sum's size) is not known: all that matters is that it is far above 65520
+        sure &= ref.abs() > ref.abs().amax() * 2.0**-8
+        assert torch.equal(got[sure].double(), ref[sure].sign() * float("inf"))
+    assert not dx[::7].any()
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("kind", ["cross entropy", "distillation"])
+@pytest.mark.parametrize(("rows", "vocab", "dim"), [(300, 30000, 264), (2049, 8191, 136), (100, 500, 64)])
+def test_row_gradients_that_lie_decades_apart(rows: int, vocab: int, dim: int, kind: str, dtype: torch.dtype) -> None:
+    """A power of two is taken out of all rows together, so a row's gradients of logits have what fp16's subnormal numbers leave of them: the bounds' 2^-39 of
+    the largest row's. The first two sizes are past 128 rows and 2^31 products, where what is rounded off is not multiplied."""
+    x, w, y = layer(rows, vocab, dim, dtype)
+    y[::11] = -100
+    x, w, b = x.requires_grad_(True), w.requires_grad_(True), normal(vocab, dtype=dtype, seed=3).requires_grad_(True)
+    g = torch.exp(-14 * torch.rand(rows, generator=torch.Generator(device="cuda").manual_seed(6), device="cuda")) * normal(rows, seed=5).sign()  # 1 to 1e-6
+    if kind == "cross entropy":
+        loss = ff.linear_cross_entropy(x, w, y, bias=b, reduction="none")
+        r = oracle.cross_entropy(x.detach(), w.detach(), y, -100, "none", g, b.detach())
+        tau = 1.0
+    else:
+        ids, teacher, tau = integers(0, vocab, (rows, 9), 7), normal(rows, 9, seed=8), 2.0
+        ids[::11] = -1
+        loss = ff.linear_distillation(x, w, ids, teacher, bias=b, temperature=tau, reduction="none")
+        r = oracle.distillation(x.detach(), w.detach(), ids, teacher, tau, "none", g, b.detach())
+    dx, dw, db = torch.autograd.grad(loss, (x, w, b), g)
+    check(r, x, w, tau, loss, {"dx": dx, "dw": dw, "db": db}, g, "none", b)
+    # and each row by itself: of its own size, but for what is flushed
+    near = (dx.detach().double() - r.dx).norm(dim=1)
+    flushed = float(g.abs().max()) * tau * 2.0**-39 if dtype == torch.float16 else 0.0
+    counted = r.counts
+    tiny = torch.finfo(dtype).smallest_normal * torch.finfo(dtype).eps / 2 * dim**0.5
+    size = 2 * torch.finfo(dtype).eps / 2 * (r.dl.abs() @ w.detach().double().abs()).norm(dim=1)
+    assert bool((near[counted] <= (size + flushed * float(w.detach().double().abs().sum(0).norm()) + tiny)[counted]).all())
