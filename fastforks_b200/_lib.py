@@ -446,6 +446,8 @@ class B200HeadArgs(ctypes.Structure):
         ("dw", ctypes.c_void_p),
         ("bias", ctypes.c_void_p),
         ("dbias", ctypes.c_void_p),
+        ("whole", ctypes.c_int32),
+        ("reserved", ctypes.c_int32),
     )
 
 

@@ -308,7 +308,8 @@ HeadLossWork head_loss_work(const B200HeadArgs& a, int sms) {
 // 2047 x 50001 x 1024 609, 596, 596; 4096 x 64000 x 2048 (three quarters of the rows) 2378, 2335, 2299; 4096 x 128000 x 4096 12240, 12110, 12030.
 constexpr int64_t kPieceBytes = 256 << 20;
 // Where what the rounding of logits' gradients took is kept and multiplied too: few rows, whose products wait for memory, and products that are small beside
-// the host's side of a call (2^31 multiply-adds more each for dx and dw, some 5 us; a call's forward and backward pass through autograd take 75).
+// the host's side of a call (2^31 multiply-adds more each for dx and dw, some 5 us; a call's forward and backward pass through autograd take 75). Elsewhere the
+// caller says so (`whole`): 12 T D V operations in place of 8.
 constexpr int64_t kRestRows = 128, kRestProducts = int64_t(1) << 31;
 struct HeadGradWork {
   int64_t slot_rows;  // rows of G and of a part of dx
@@ -321,7 +322,7 @@ struct HeadGradWork {
 HeadGradWork head_grad_work(const B200HeadArgs& a, bool want_dx, bool want_dw, int pairs) {
   HeadGradWork w{};
   w.slot_rows = up(a.rows, 256);
-  w.g_rows = a.rows <= kRestRows || static_cast<double>(a.rows) * a.dim * a.vocab <= static_cast<double>(kRestProducts) ? 2 * w.slot_rows : w.slot_rows;
+  w.g_rows = a.whole != 0 || a.rows <= kRestRows || static_cast<double>(a.rows) * a.dim * a.vocab <= static_cast<double>(kRestProducts) ? 2 * w.slot_rows : w.slot_rows;
   const int64_t most = std::max<int64_t>(2048, kPieceBytes / (2 * w.g_rows) / 256 * 256);
   const int64_t pieces = (a.vocab + most - 1) / most;
   w.cols = static_cast<int>(up((a.vocab + pieces - 1) / pieces, 256));

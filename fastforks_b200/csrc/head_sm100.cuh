@@ -304,7 +304,8 @@ __device__ __forceinline__ void head_add_bias(float (&v)[32], const void* bias, 
 // G = 2^s coef_t (softmax(z_t) - p) is held in 16 bits, the operands' type: off by half a step at most, 2^-8 of a value (fp16 2^-11). s = 15 for
 // fp16, whose smallest normal number is 2^-14: a softmax of 2^-29 keeps all its bits; bfloat16 has fp32's range, s = 0. Over many rows that adds up to 1.1 to 1.45 times the error that
 // the results' own rounding has; of a few rows each hangs on one or two roundings, and 1.7 times came out. Few rows and small products (head_grad_work in
-// b200_training.cu) therefore keep what the rounding took, in as many rows more, and both go through the products: the error is that of the results' rounding.
+// b200_training.cu), and all others where the caller asks for it, therefore keep what the rounding took, in as many rows more, and both go through the
+// products: the error is that of the results' rounding.
 template <typename T, bool GRADS>
 struct HeadLogitsJob {
   const HeadLogitsParams& p;

@@ -721,7 +721,7 @@ at::Tensor head_loss(const at::Tensor& x, const at::Tensor& w, const at::Tensor&
 
 struct HeadLossFunction : torch::autograd::Function<HeadLossFunction> {
   // (x stands in for no bias, and `targets` for no teacher: apply() takes no undefined tensor.)
-  static at::Tensor forward(AutogradContext* ctx, const at::Tensor& x, const at::Tensor& w, const at::Tensor& vector, const at::Tensor& targets, const at::Tensor& logits, bool biased, bool distill, int64_t ignore, double tau, int64_t reduction) {
+  static at::Tensor forward(AutogradContext* ctx, const at::Tensor& x, const at::Tensor& w, const at::Tensor& vector, const at::Tensor& targets, const at::Tensor& logits, bool biased, bool distill, int64_t ignore, double tau, int64_t reduction, bool whole) {
     const at::Tensor teacher = distill ? logits : at::Tensor(), bias = biased ? vector : at::Tensor();
     at::Tensor state;
     at::Tensor loss = head_loss(x, w, bias, targets, teacher, ignore, tau, reduction, &state);
@@ -729,11 +729,12 @@ struct HeadLossFunction : torch::autograd::Function<HeadLossFunction> {
     ctx->saved_data["top"] = teacher.defined() ? targets.size(-1) : int64_t(0);
     ctx->saved_data["tau"] = tau;
     ctx->saved_data["reduction"] = reduction;
+    ctx->saved_data["whole"] = whole;
     return loss;
   }
   static variable_list backward(AutogradContext* ctx, const variable_list& grads) {
     const variable_list saved = ctx->get_saved_variables();
-    variable_list result(10);
+    variable_list result(11);
     {
       const at::NoGradGuard guard;
       const at::Tensor &x = saved[0], &w = saved[1], &bias = saved[2], &state = saved[3];
@@ -741,6 +742,7 @@ struct HeadLossFunction : torch::autograd::Function<HeadLossFunction> {
       const int64_t reduction = ctx->saved_data["reduction"].toInt();
       B200HeadArgs a;
       set_head(&a, x, w, bias, ctx->saved_data["top"].toInt(), ctx->saved_data["tau"].toDouble(), reduction);
+      a.whole = ctx->saved_data["whole"].toBool() ? 1 : 0;
       at::Tensor g = grads[0].defined() ? grads[0].resolve_neg() : at::zeros({reduction == 0 ? a.rows : 1}, x.options().dtype(at::kFloat).requires_grad(false));
       if (g.dim() > 1) g = g.reshape({-1});
       a.grad = static_cast<const float*>(g.data_ptr());
@@ -774,9 +776,9 @@ bool operand_of(const at::Tensor* t, c10::DeviceIndex device) {
          reinterpret_cast<uintptr_t>(t->data_ptr()) % 16 == 0;
 }
 
-// head_loss(x, weight, bias | None, targets, teacher | None, ignore, tau, reduction: 0 none, 1 sum, 2 mean)
+// head_loss(x, weight, bias | None, targets, teacher | None, ignore, tau, reduction: 0 none, 1 sum, 2 mean, whole gradients)
 PyObject* py_head_loss(PyObject*, PyObject* const* args, Py_ssize_t n) {
-  if (n != 8 || !PyLong_Check(args[5])) Py_RETURN_NONE;
+  if (n != 9 || !PyLong_Check(args[5]) || !PyBool_Check(args[8])) Py_RETURN_NONE;
   const c10::DeviceIndex device = c10::cuda::current_device();
   const at::Tensor *x = tensor_of(args[0]), *w = tensor_of(args[1]), *y = tensor_of(args[3]);
   if (!operand_of(x, device) || !operand_of(w, device) || w->dim() != 2 || w->scalar_type() != x->scalar_type() || w->size(1) != x->size(-1)) Py_RETURN_NONE;
@@ -803,7 +805,7 @@ PyObject* py_head_loss(PyObject*, PyObject* const* args, Py_ssize_t n) {
   }
   const bool biased = bias.defined(), distill = teacher.defined();
   if (wants_grad(*x) || wants_grad(*w) || (biased && wants_grad(bias)))
-    return THPVariable_Wrap(HeadLossFunction::apply(*x, *w, biased ? bias : *x, *y, distill ? teacher : *y, biased, distill, ignore, tau, reduction));
+    return THPVariable_Wrap(HeadLossFunction::apply(*x, *w, biased ? bias : *x, *y, distill ? teacher : *y, biased, distill, ignore, tau, reduction, args[8] == Py_True));
   at::Tensor state;
   return THPVariable_Wrap(head_loss(*x, *w, bias, *y, teacher, ignore, tau, reduction, &state));
 }

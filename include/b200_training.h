@@ -64,7 +64,8 @@ int b200_layer_norm_workspace(const B200LayerNormArgs* args, int64_t* bytes);
  * A token past the vocabulary makes NaN of its row (loss and gradients) and sets B200_STATUS_TARGET. Rows that do not count have loss 0 and no
  * gradient, and what x holds there is not looked at. The sum and the mean are over the rows that count, 0 where none does.
  * b200_head_grad gives dx = dl w, dw = dl^T x and dbias = sum over rows of dl, with dl = grad_t * tau * (softmax(z_t) - p at its tokens) held in `dtype` on its way into
- * the products. It reads the `state` of the forward call, which may be shared by several calls and stays as it is.
+ * the products (b200_head_grad, `whole` not 0: what that rounding takes goes through the products as well, half as many operations more; up to 128 rows or
+ * 2^31 products it does in any case). It reads the `state` of the forward call, which may be shared by several calls and stays as it is.
  * Products accumulate in fp32; sums are taken in a fixed order.
  */
 #define B200_HEAD_NONE 0 /* loss per row */
@@ -101,6 +102,8 @@ typedef struct B200HeadArgs {
   void* dw;             /* [vocab, dim] contiguous, or NULL: not asked for */
   const void* bias;     /* [vocab] of `dtype`, 16-byte aligned, or NULL */
   void* dbias;          /* [vocab] of `dtype`, 16-byte aligned, or NULL: not asked for */
+  int32_t whole;        /* gradient, and its workspace: see above */
+  int32_t reserved;
 } B200HeadArgs;
 
 int b200_head_loss(const B200HeadArgs* args, void* stream);
