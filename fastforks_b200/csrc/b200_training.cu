@@ -303,7 +303,8 @@ HeadLossWork head_loss_work(const B200HeadArgs& a, int sms) {
   return w;
 }
 
-// Gradients of logits in 16 bits of as many columns at a time as kPieceBytes holds, or 2048. Each piece costs the fp32 sums of dx once more
+// Gradients of logits in 16 bits of as many columns at a time as kPieceBytes holds, or 2048 where that is more (above 65536 rows: 1048576 x 4000 takes 4.3 GB); up to
+// 2048 columns, padded to 256, are one piece. Each piece costs the fp32 sums of dx once more
 // through L2 and HBM, under the products, and the rounds of two launches that are not full. us of a loss with its gradients at 128, 256 and 512 MB:
 // 2047 x 50001 x 1024 609, 596, 596; 4096 x 64000 x 2048 (three quarters of the rows) 2378, 2335, 2299; 4096 x 128000 x 4096 12240, 12110, 12030.
 constexpr int64_t kPieceBytes = 256 << 20;

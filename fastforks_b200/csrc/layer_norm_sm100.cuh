@@ -3,7 +3,8 @@
 //   mu = mean(x), r = 1 / sqrt(mean((x - mu)^2) + eps), h = (x - mu) r, y = h w + b
 //   t = dy w:  dx = r (t - mean(t) - h mean(t h)),  dw = sum_rows dy h,  db = sum_rows dy
 //
-// Both are bound by HBM: a row is read once, into registers, and everything that is computed of it comes from there. A row is shared by
+// Both have their floor in HBM's bytes: a row is read once, into registers, and everything that is computed of it comes from there. What binds them above it
+// is the chain of a row (load, two sums over its threads, store): in 16 bits neither memory nor issue slots are at their end. A row is shared by
 // as many threads as leave each some sixteen to thirty-two values; sums and the weights' gradients are fp32. norm_rows_kernel is the forward pass;
 // norm_ring_grad_kernel the gradients of rows on 16-byte boundaries of up to 8192 16-bit or 4096 fp32 values, norm_rows_grad_kernel of all others.
 #pragma once
@@ -408,8 +409,8 @@ __global__ void __launch_bounds__(THREADS == 32 ? 32 * kLnGradWarps : THREADS) n
 // no value is tested for being one; weights stay in registers as fp32 pairs (with a test and a conversion at each use a value took 29
 // instructions, and 8192 rows of 4096 54 us). us with the join, of bf16: a row a CTA with the next one in registers (norm_rows_grad_kernel) -> here, and
 // the time of the bytes: 8192 x 4096 75.0 -> 40.9 (30.8), 21920 x 1024 48.4 -> 30.8 (20.6), 30000 x 512 64.4 -> 20.5 (14.1), 300 x 4096 18.3 -> 7.8; fp32
-// 8192 x 4096 74.3 -> 67.7 (61.6), 5480 x 384 14.5 -> 8.9 (3.9). Bound by HBM at its mix of reads and writes and, at sixteen warps an SM, by the chain of
-// copy, sums and barrier of each row. The same for the forward pass was slower than rows in registers but for the largest calls (several
+// 8192 x 4096 74.3 -> 67.7 (61.6), 5480 x 384 14.5 -> 8.9 (3.9). Bound in fp32 by HBM and in 16 bits, at sixteen warps an SM, by the chain of copy, sums and
+// barrier of each row (8192 x 4096: DRAM 53 %, issue slots 41 %). The same for the forward pass was slower than rows in registers but for the largest calls (several
 // inputs in turn: 1200 x 4096 10.1 against 7.6, 5000 x 4096 19.7 and 19.6, 10000 x 4096 30.7 and 32.8): two barriers a row, and nothing that has to stay. (Groups added one after the other into one place took 5 us more at 16 groups.)
 constexpr int kLnMostWarps = 16, kLnMostSlots = 16, kLnRingBytes = 208 * 1024;
 constexpr uint32_t kStatusNormWait = 1u << 24;

@@ -124,7 +124,7 @@ def layer_norm(
             sees that it was written to.
 
     Raises:
-        ValueError: Operands outside the contract (checked before the launch).
+        ValueError: Operands outside the contract (checked before the launch), or no row at all where a gradient is wanted.
         KernelUnavailableError: The CUDA library is not built or does not load.
     """
     if out is None and _lib.fast is not None:

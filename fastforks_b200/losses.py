@@ -2,7 +2,8 @@
 teacher's largest logits.
 
 Host side of `b200_head_loss` and `b200_head_grad` (include/b200_training.h). The logits are computed tile by tile where their statistics are
-taken, and once more, in pieces of the vocabulary, where their gradients are; nothing of the size of rows times vocabulary is kept.
+taken, and once more, in pieces of the vocabulary, where their gradients are; nothing of the size of rows times vocabulary is kept from the loss to
+its gradients, and of a vocabulary of more than 2048 tokens there is never all of it at a time where rows are many.
 """
 
 from __future__ import annotations
@@ -162,14 +163,14 @@ def linear_cross_entropy(  # noqa: PLR0913
         weight: `[vocabulary, dim]` of x's type.
         targets: int64 or int32 `[...]`, the shape of x without its last dimension. One outside the vocabulary (and not `ignore_index`)
             makes NaN of its row, and `device_status()` reports it.
-        bias: `[vocabulary]` of x's type, or None.
+        bias: `[vocabulary]` of x's type, or None. Its gradient is summed over the rows 64 columns at a time: over few tokens that is most of the time.
         ignore_index: Target of rows that do not count: their loss is 0, they have no gradient, and what x holds there is not looked at.
         reduction: `"mean"` or `"sum"` over the rows that count (0 where none does), or `"none"`: the loss of each row.
         whole_gradients: Multiply what the rounding of the logits' gradients takes, too: the error of the results is then that of their own rounding (else 1.1 to
-            1.5 times as much), at half as many operations more and twice the scratch. Up to 128 rows or 2^31 products that is so in any case.
+            1.5 times as much), at half as many operations more and up to twice the scratch. Up to 128 rows or 2^31 products that is so in any case.
 
     Raises:
-        ValueError: Operands outside the contract (checked before the launch).
+        ValueError: Operands outside the contract (checked before the launch), or no row at all where a gradient is wanted.
         KernelUnavailableError: The CUDA library is not built or does not load.
     """
     if _lib.fast is not None:
@@ -218,7 +219,7 @@ def linear_distillation(  # noqa: PLR0913
         whole_gradients: As for `linear_cross_entropy`.
 
     Raises:
-        ValueError: Operands outside the contract (checked before the launch).
+        ValueError: Operands outside the contract (checked before the launch), or no row at all where a gradient is wanted.
         KernelUnavailableError: The CUDA library is not built or does not load.
     """
     if _lib.fast is not None and teacher_logits is not None:
