@@ -17,7 +17,7 @@ from typing import TYPE_CHECKING
 import torch
 
 from . import _lib
-from .rotary import written
+from .rotary import as_held, refuse_negation, written
 
 if TYPE_CHECKING:
     from collections.abc import Sequence
@@ -257,7 +257,10 @@ def attention(  # noqa: PLR0913
         done = host.attention(q, k, v, scale, layout == "bnhd", _SCHEDULES[schedule], out, bias, rel_h, rel_w, False)  # noqa: FBT003
         if done is not None:
             return done
+    q, k, v, bias = (as_held(t) for t in (q, k, v, bias))
     check_operands(q, k, v, layout, out)
+    if out is not None:
+        refuse_negation("attention", "out", out)
     if schedule not in _SCHEDULES:
         msg = f"attention: schedule {schedule!r}: expected one of {tuple(_SCHEDULES)}"
         raise ValueError(msg)
@@ -296,7 +299,7 @@ def attention(  # noqa: PLR0913
         a.bias, a.bias_dtype = bv.data_ptr(), _BIAS_DTYPES[bv.dtype]
         a.bias_stride[:] = bv.stride()[:3]
     if rel is not None:
-        rel_h, rel_w = rel
+        rel_h, rel_w = (as_held(t) for t in rel)
         if rel_h.dim() != 4 or rel_w.dim() != 4 or rel_h.dtype != rel_w.dtype:  # noqa: PLR2004
             msg = "attention: rel_h and rel_w must be 4-D tensors of one dtype"
             raise ValueError(msg)

@@ -212,7 +212,7 @@ PyObject* py_attention(PyObject*, PyObject* const* args, Py_ssize_t n) {
     }
   } else {
     const at::Tensor* given = tensor_of(args[6]);
-    if (given == nullptr || given->scalar_type() != q->scalar_type() || !given->is_cuda() || given->device().index() != device || given->sizes() != q->sizes())
+    if (given == nullptr || given->scalar_type() != q->scalar_type() || !given->is_cuda() || given->is_neg() || given->device().index() != device || given->sizes() != q->sizes())
       Py_RETURN_NONE;
     out = *given;
   }

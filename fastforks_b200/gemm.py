@@ -13,7 +13,7 @@ import ctypes
 import torch
 
 from . import _lib
-from .rotary import written
+from .rotary import as_held, refuse_negation, written
 
 ACT_NONE, ACT_RELU, ACT_GELU, ACT_GELU_TANH = 0, 1, 5, 6  # the reference's codes (dpt_fused/__init__.py)
 _DTYPES = {torch.float16: _lib.F16, torch.bfloat16: _lib.BF16}
@@ -64,6 +64,7 @@ def gemm(  # noqa: PLR0913 - the epilogue terms
         done = _lib.fast.gemm(x, w, bias, act, scale, res, out)
         if done is not None:
             return done
+    x, w, bias, scale, res = (as_held(t) for t in (x, w, bias, scale, res))
     if x.dtype not in _DTYPES or not x.is_cuda:
         msg = f"gemm: x must be a float16 / bfloat16 CUDA tensor, got {x.dtype} on {x.device}"
         raise ValueError(msg)
@@ -84,6 +85,7 @@ def gemm(  # noqa: PLR0913 - the epilogue terms
     if y.dtype != x.dtype or y.device != x.device:
         msg = f"gemm: out must be {x.dtype} on {x.device}"
         raise ValueError(msg)
+    refuse_negation("gemm", "out", y)
     a.y, a.ldy = y.data_ptr(), _rows(y, m, n, "out")
     for name, t, dtype in (("bias", bias, x.dtype), ("scale", scale, torch.float32)):
         if t is not None and (t.shape != (n,) or t.dtype != dtype or t.device != x.device or not t.is_contiguous()):

@@ -16,7 +16,7 @@ import threading
 import torch
 
 from . import _lib
-from .rotary import refuse_tangent, written
+from .rotary import as_held, refuse_negation, refuse_tangent, written
 
 BLOCK = 16  # tokens
 HEAD_DIMS = (64, 128)
@@ -173,6 +173,7 @@ def kv4_append_(  # noqa: PLR0913
         if done is not None:
             return done if q is not None else None
     what = "kv4_append_"
+    k, v, q, table = (as_held(t) for t in (k, v, q, table))
     dim = _check_cache(what, cache, page_table, lengths, _batch(what, "k", k))
     _check_heads(what, "k", k, cache, dim, heads=cache.shape[1])
     _check_heads(what, "v", v, cache, dim, like=k, heads=cache.shape[1])
@@ -180,6 +181,7 @@ def kv4_append_(  # noqa: PLR0913
         _check_heads(what, "q", q, cache, dim, like=k)
         if out is not None:
             _check_heads(what, "out", out, cache, dim, like=q, heads=q.shape[2])
+            refuse_negation(what, "out", out)
     elif out is not None:
         msg = f"{what}: out without q"
         raise ValueError(msg)
@@ -270,6 +272,7 @@ def kv4_attention(  # noqa: PLR0913
         if done is not None:
             return done
     what = "kv4_attention"
+    q = as_held(q)
     dim = _check_cache(what, cache, page_table, lengths, _batch(what, "q", q))
     _check_heads(what, "q", q, cache, dim)
     if q.shape[2] == 0 or q.shape[2] % cache.shape[1]:
@@ -280,6 +283,7 @@ def kv4_attention(  # noqa: PLR0913
         out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
     else:
         _check_heads(what, "out", out, cache, dim, like=q, heads=q.shape[2])
+        refuse_negation(what, "out", out)
     if q.numel() == 0:
         return out
     a = _lib.B200Kv4AttnArgs()

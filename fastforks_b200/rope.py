@@ -14,7 +14,7 @@ import math
 import torch
 
 from . import _lib
-from .rotary import written
+from .rotary import as_held, refuse_negation, written
 
 HEAD_DIM = 64
 
@@ -60,7 +60,8 @@ def rope_qk_(qkv: torch.Tensor, cs: torch.Tensor, *, q_scale: float = 1.0) -> to
     if qkv.requires_grad and torch.is_grad_enabled():
         msg = "rope_qk_: the kernels have no backward; qkv requires grad"
         raise ValueError(msg)
-    cs = cs.contiguous()
+    refuse_negation("rope_qk_", "qkv", qkv)
+    cs = as_held(cs).contiguous()
     q, k = qkv[:, :, 0], qkv[:, :, 1]
     a = _lib.B200RopeArgs()
     a.struct_size = ctypes.sizeof(_lib.B200RopeArgs)

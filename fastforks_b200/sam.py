@@ -23,6 +23,7 @@ import torch.nn.functional as F  # noqa: N812
 
 from . import _lib, encoder
 from .attention import attention
+from .rotary import as_held
 
 
 @dataclass(frozen=True)
@@ -121,6 +122,7 @@ def sam_rel_terms(q: torch.Tensor, rel_pos_h: torch.Tensor, rel_pos_w: torch.Ten
         done = _lib.fast.sam_rel_terms(q, rel_pos_h, rel_pos_w, side)
         if done is not None:
             return done
+    q, rel_pos_h, rel_pos_w = (as_held(t) for t in (q, rel_pos_h, rel_pos_w))
     if q.dim() != 4 or q.shape[-1] != 64 or q.stride(-1) != 1 or not q.is_cuda or q.dtype not in (torch.float16, torch.bfloat16):  # noqa: PLR2004
         msg = f"sam_rel_terms: q must be a float16 / bfloat16 CUDA [B, N, heads, 64] view with unit last stride, got {tuple(q.shape)} {q.dtype} {q.device}"
         raise ValueError(msg)
